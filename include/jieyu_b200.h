@@ -242,6 +242,109 @@ JYC_API int jyc_argmax(const float* logits, int n, int* out_index, void* stream)
 JYC_API int jyc_sample(float* logits, int vocab_size, float temperature, float repetition_penalty,
                        const int* out_ids, int prompt_len, int len, unsigned int* rng, int* next, void* stream);
 
+/* ---- paged K/V cache and batched sampling (DEVICE pointers, asynchronous) -
+ * No counterpart in the reference, which keeps one contiguous cache per
+ * sequence (libs/date_libs/date.h:89-147) and picks one token at a time. The
+ * arithmetic is that of the operators above: kv_pack_q8's rounding, rope_pos's
+ * rotation and slot order, attention_q8's scores. For several sequences that
+ * grow and end at their own times.
+ *
+ * A cache of pages: K and V rows of head_dim int8 with one fp32 scale each, in
+ * num_pages pages of page_size positions. Row (page, slot, kv head) starts at
+ * page * page_stride + slot * pos_stride + head * head_stride (int8 elements,
+ * the same for k and v), its scale at the s*_stride ones (floats). So
+ * [page][slot][kv head][dim] and [page][kv head][slot][dim] are both a choice
+ * of strides. k, v and the int8 strides are multiples of 4 bytes (of 16 bytes,
+ * with head_dim % 16 == 0, for the widest copies). The struct itself is read by
+ * the host during the call. */
+typedef struct jyc_kv_pages {
+    int8_t* k;
+    float*  ks;
+    int8_t* v;
+    float*  vs;
+    int num_pages;
+    int page_size;
+    long long page_stride, pos_stride, head_stride;
+    long long spage_stride, spos_stride, shead_stride;
+} jyc_kv_pages;
+
+/* Position p of sequence s is slot p % page_size of page
+ * page_table[s * table_stride + p / page_size] (int32, num_seqs rows of
+ * table_stride entries, so a sequence holds at most table_stride * page_size
+ * positions). Entries behind a sequence's last position are not read.
+ * Positions, lengths and page ids lie on the device, where the kernels check
+ * them: what is out of range is never read or written and sets the paged error
+ * word (jyc_paged_error). */
+
+/* Writes `rows` rows of K and V [row][num_kv_heads * head_dim] (both of row
+ * stride ld floats) into their pages: row i at position row_pos[i] of sequence
+ * row_seq[i] (row_seq NULL: sequence i, rows <= num_seqs). A row whose position
+ * is negative is skipped. cos/sin tables [rope_len][head_dim / 2]: K is rotated
+ * by its row's position first, as jyc_rope_pos does; NULL: K arrives rotated.
+ * Bytes and scales equal jyc_kv_pack_q8's. Two rows of one call must not name
+ * the same position of the same page (that slot would hold a mixture). head_dim
+ * % 4 == 0, <= 256. */
+JYC_API int jyc_kv_append_paged_q8(const float* K, const float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                   const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                   int num_seqs, const float* cos_table, const float* sin_table, int rope_len,
+                                   const jyc_kv_pages* pages, void* stream);
+
+/* The reverse: K and V rows [row][num_kv_heads * head_dim] of row stride ld
+ * from the pages, q * scale in fp32 (K as it is stored, that is rotated). Rows
+ * with a negative position are left as they were. */
+JYC_API int jyc_kv_read_paged_q8(float* K, float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                 const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                 int num_seqs, const jyc_kv_pages* pages, void* stream);
+
+/* Attention of one new token per sequence over its pages: query row s
+ * [num_heads * head_dim] at Q + s * ldq (the position seq_lens[s] - 1, whose K
+ * and V are in the cache already), keys 0 .. seq_lens[s] - 1, out row s at
+ * out + s * ldo. The query is quantised per head and scored as in
+ * jyc_attention_q8 (int32 dots, dot * ((ks * qs) * 1/sqrt(head_dim)), fp32
+ * softmax, V scaled by vs). cos/sin tables: the query is rotated by its
+ * position first; NULL: it arrives rotated. A sequence of length <= 0 gets a
+ * row of zeros, as does one whose query position lies behind the tables; a
+ * length above table_stride * page_size is cut to that; keys on a page that is
+ * out of range weigh nothing (the last three set the error word). num_heads a
+ * multiple of num_kv_heads, head_dim % 4 == 0, <= 256.
+ * The lengths stay on the device, so a captured call replays for new ones.
+ * workspace: at least jyc_attention_paged_q8_workspace bytes, 16-byte aligned,
+ * its contents without meaning before and after the call; calls that may
+ * overlap in time (other streams, other graphs) need one each. NULL: scratch is
+ * taken in stream order, as jyc_attention_q8 does. */
+JYC_API int jyc_attention_paged_q8(const float* Q, int ldq, float* out, int ldo, int num_heads, int num_kv_heads,
+                                   int head_dim, const int* seq_lens, const int* page_table, int table_stride,
+                                   int num_seqs, const float* cos_table, const float* sin_table, int rope_len,
+                                   const jyc_kv_pages* pages, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace of the call above on the current device (0: bad shape). */
+JYC_API size_t jyc_attention_paged_q8_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim);
+
+/* Bits set by the paged operators on the current device since the last reset: 1 a
+ * sequence, position or length out of range, 2 a page id out of range, 4 a
+ * position behind the RoPE tables. Synchronises with the device. */
+JYC_API int jyc_paged_error(int reset);
+
+/* The next token of every row of logits [rows][vocab_size] (row stride ld,
+ * read only). Per row r (device arrays of `rows` entries; a NULL array means
+ * its default for every row):
+ *   temperature (1)  T <= 0 or NaN: the first index of the maximum, as
+ *                    jyc_argmax; else weights w = exp((l - max) / T) (a weight
+ *                    below 2^-40 counts as zero);
+ *   top_k (off)      the k largest logits, ties to the lower index; k <= 0: off;
+ *   top_p (off)      of those, the shortest run from the largest whose weights
+ *                    reach top_p of theirs, at least one token; >= 1 or NaN: off;
+ *   min_p (off)      of those, weights >= min(min_p, 1) (the largest is 1).
+ * The pick is the first kept index, in index order, whose running sum of
+ * weights exceeds u[r] times their sum (u in [0, 1); the last kept one if none
+ * does). probs[r] (probs may be NULL) is its weight over that sum, 1 for a
+ * greedy row. NaN logits are never picked; a row whose logits are all NaN or
+ * -inf gives id -1 and probability 0. Equal +inf logits share the draw. Sums
+ * are held in 64-bit fixed point, so a row's pick does not depend on the other
+ * rows or on the order of execution. vocab_size <= 2^20. */
+JYC_API int jyc_sample_batch(const float* logits, int ld, int rows, int vocab_size, const float* temperature,
+                             const int* top_k, const float* top_p, const float* min_p, const float* u, int* out_ids,
+                             float* out_probs, void* stream);
+
 /* ---- operator entry points with the reference's calling convention ------
  * HOST pointers in the reference's own layouts, caller-owned, synchronous:
  * each call copies its operands to the device, runs the device entry point

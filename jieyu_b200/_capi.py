@@ -69,6 +69,17 @@ class ModelDesc(C.Structure):
     ]
 
 
+class KVPages(C.Structure):
+    """Layout of jyc_kv_pages: an int8 K/V cache in pages, by strides."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("ks", C.c_void_p), ("v", C.c_void_p), ("vs", C.c_void_p),
+        ("num_pages", C.c_int), ("page_size", C.c_int),
+        ("page_stride", C.c_longlong), ("pos_stride", C.c_longlong), ("head_stride", C.c_longlong),
+        ("spage_stride", C.c_longlong), ("spos_stride", C.c_longlong), ("shead_stride", C.c_longlong),
+    ]
+
+
 TOKEN_CB = C.CFUNCTYPE(C.c_int, C.c_int, C.c_void_p)
 
 # (name, restype, argtypes) of every exported entry point.
@@ -107,6 +118,14 @@ SIGNATURES = [
     ("jyc_host_ffn", _I, [_P, _P, _P, _P, _P, _I, _I, _I]),
     ("jyc_argmax", _I, [_P, _I, _P, _P]),
     ("jyc_sample", _I, [_P, _I, C.c_float, C.c_float, _P, _I, _I, _P, _P, _P]),
+    ("jyc_kv_append_paged_q8", _I,
+     [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _I, C.POINTER(KVPages), _P]),
+    ("jyc_kv_read_paged_q8", _I, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, C.POINTER(KVPages), _P]),
+    ("jyc_attention_paged_q8", _I,
+     [_P, _I, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _I, C.POINTER(KVPages), _P, _SZ, _P]),
+    ("jyc_attention_paged_q8_workspace", _SZ, [_I, _I, _I, _I]),
+    ("jyc_paged_error", _I, [_I]),
+    ("jyc_sample_batch", _I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
     ("jyc_model_create", _P, [C.POINTER(ModelDesc)]),
     ("jyc_model_free", None, [_P]),
     ("jyc_model_weight_bytes_per_token", C.c_double, [_P]),

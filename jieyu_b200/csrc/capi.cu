@@ -7,6 +7,7 @@
 
 #include "kernels.cuh"
 #include "mega.cuh"
+#include "paged.cuh"
 #include "tcgemm.cuh"
 #include "skinny.cuh"
 
@@ -376,6 +377,141 @@ JYC_API int jyc_sample(float* logits, int vocab_size, float temperature, float r
         return arg_error("sample: penalty needs out_ids[prompt_len..len)");
     return launch_sample(logits, vocab_size, temperature, repetition_penalty, out_ids, prompt_len, len, rng, next,
                          S(stream));
+}
+
+// ---------------------------------------------------------------------------
+// Paged K/V cache and batched sampling.
+}  // extern "C"
+
+namespace {
+
+// The arguments that the paged operators share; `what` names the caller.
+int check_paged(const char* what, int num_kv_heads, int head_dim, const int* page_table, int table_stride,
+                int num_seqs, const jyc_kv_pages* p) {
+    const std::string w = std::string(what) + ": ";
+    if (num_kv_heads <= 0) return arg_error(w + "num_kv_heads must be positive");
+    if (head_dim <= 0 || head_dim % 4 || head_dim > 256)
+        return arg_error(w + "head_dim must be a multiple of 4, <= 256");
+    if (num_seqs < 0 || table_stride < 0) return arg_error(w + "negative page table shape");
+    if (!page_table || !p || !p->k || !p->ks || !p->v || !p->vs) return arg_error(w + "null pointer");
+    if (p->num_pages <= 0 || p->page_size <= 0) return arg_error(w + "num_pages and page_size must be positive");
+    if ((long long)table_stride * p->page_size > 0x7fffffffLL)
+        return arg_error(w + "table_stride * page_size must fit an int");
+    if (p->page_stride < 0 || p->pos_stride < 0 || p->head_stride < 0 || p->spage_stride < 0 || p->spos_stride < 0 ||
+        p->shead_stride < 0)
+        return arg_error(w + "negative page stride");
+    if ((((uintptr_t)p->k | (uintptr_t)p->v) & 3) || ((p->page_stride | p->pos_stride | p->head_stride) & 3))
+        return arg_error(w + "k, v and their strides must be multiples of 4 bytes");
+    if ((((uintptr_t)p->ks | (uintptr_t)p->vs | (uintptr_t)page_table) & 3))
+        return arg_error(w + "misaligned scales or page table");
+    return JYC_OK;
+}
+
+int check_rope(const char* what, const float* cos_table, const float* sin_table, int rope_len) {
+    if (!cos_table != !sin_table) return arg_error(std::string(what) + ": cos and sin tables come together");
+    if (cos_table && rope_len <= 0) return arg_error(std::string(what) + ": rope_len must be positive");
+    return JYC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+JYC_API int jyc_kv_append_paged_q8(const float* K, const float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                   const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                   int num_seqs, const float* cos_table, const float* sin_table, int rope_len,
+                                   const jyc_kv_pages* pages, void* stream) {
+    clear_error();
+    TRY(check_paged("kv_append_paged_q8", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    TRY(check_rope("kv_append_paged_q8", cos_table, sin_table, rope_len));
+    if (rows < 0) return arg_error("kv_append_paged_q8: negative rows");
+    if (ld < (long long)num_kv_heads * head_dim) return arg_error("kv_append_paged_q8: ld below num_kv_heads * head_dim");
+    if (!row_seq && rows > num_seqs) return arg_error("kv_append_paged_q8: more rows than sequences without row_seq");
+    if (rows == 0) return JYC_OK;
+    if (!K || !V || !row_pos) return arg_error("kv_append_paged_q8: null pointer");
+    const PagedKV kv{*pages, page_table, table_stride, num_seqs};
+    return launch_paged_append(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv,
+                               PagedRope{cos_table, sin_table, rope_len}, S(stream));
+}
+
+JYC_API int jyc_kv_read_paged_q8(float* K, float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                 const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                 int num_seqs, const jyc_kv_pages* pages, void* stream) {
+    clear_error();
+    TRY(check_paged("kv_read_paged_q8", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    if (rows < 0) return arg_error("kv_read_paged_q8: negative rows");
+    if (ld < (long long)num_kv_heads * head_dim) return arg_error("kv_read_paged_q8: ld below num_kv_heads * head_dim");
+    if (!row_seq && rows > num_seqs) return arg_error("kv_read_paged_q8: more rows than sequences without row_seq");
+    if (rows == 0) return JYC_OK;
+    if (!K || !V || !row_pos) return arg_error("kv_read_paged_q8: null pointer");
+    const PagedKV kv{*pages, page_table, table_stride, num_seqs};
+    return launch_paged_read(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv, S(stream));
+}
+
+JYC_API size_t jyc_attention_paged_q8_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim) {
+    clear_error();
+    if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+        head_dim % 4 || head_dim > 256) {
+        arg_error("attention_paged_q8_workspace: bad shape");
+        return 0;
+    }
+    return paged_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim);
+}
+
+JYC_API int jyc_attention_paged_q8(const float* Q, int ldq, float* out, int ldo, int num_heads, int num_kv_heads,
+                                   int head_dim, const int* seq_lens, const int* page_table, int table_stride,
+                                   int num_seqs, const float* cos_table, const float* sin_table, int rope_len,
+                                   const jyc_kv_pages* pages, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    TRY(check_paged("attention_paged_q8", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    TRY(check_rope("attention_paged_q8", cos_table, sin_table, rope_len));
+    if (num_heads <= 0 || num_heads % num_kv_heads)
+        return arg_error("attention_paged_q8: num_heads must be a multiple of num_kv_heads");
+    if (ldq < (long long)num_heads * head_dim || ldo < (long long)num_heads * head_dim)
+        return arg_error("attention_paged_q8: ldq and ldo must hold num_heads * head_dim");
+    if (num_seqs == 0) return JYC_OK;
+    if (!Q || !out || !seq_lens) return arg_error("attention_paged_q8: null pointer");
+    const size_t need = paged_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim);
+    if (need == 0) return JYC_ERR_CUDA;
+    if (workspace && workspace_bytes < need) return arg_error("attention_paged_q8: workspace too small");
+    if ((uintptr_t)workspace & 15) return arg_error("attention_paged_q8: workspace must be 16-byte aligned");
+    PagedAttn a{};
+    a.Q = Q; a.ldq = ldq; a.out = out; a.ldo = ldo;
+    a.H = num_heads; a.KV = num_kv_heads; a.hd = head_dim; a.lens = seq_lens;
+    a.kv = PagedKV{*pages, page_table, table_stride, num_seqs};
+    a.rope = PagedRope{cos_table, sin_table, rope_len};
+    a.scale = 1.0f / sqrtf((float)head_dim);
+    Scratch sc(S(stream));
+    unsigned char* own = nullptr;
+    if (!workspace) TRY(sc.get(&own, need));
+    return launch_paged_attention(a, workspace ? workspace : own, S(stream));
+}
+
+JYC_API int jyc_paged_error(int reset) {
+    clear_error();
+    int* p = paged_error_word();
+    if (!p) {
+        set_error("paged_error: no device");
+        return JYC_ERR_CUDA;
+    }
+    int v = 0;
+    JYC_CUDA(cudaDeviceSynchronize());
+    JYC_CUDA(cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost));
+    if (reset && v) JYC_CUDA(cudaMemset(p, 0, sizeof(int)));
+    return v;
+}
+
+JYC_API int jyc_sample_batch(const float* logits, int ld, int rows, int vocab_size, const float* temperature,
+                             const int* top_k, const float* top_p, const float* min_p, const float* u, int* out_ids,
+                             float* out_probs, void* stream) {
+    clear_error();
+    if (rows < 0 || vocab_size <= 0) return arg_error("sample_batch: need rows >= 0 and vocab_size > 0");
+    if (vocab_size > kPickMaxVocab) return arg_error("sample_batch: vocab_size above 2^20");
+    if (ld < vocab_size) return arg_error("sample_batch: ld below vocab_size");
+    if (rows == 0) return JYC_OK;
+    if (!logits || !u || !out_ids) return arg_error("sample_batch: null pointer");
+    const PickArgs a{logits, ld, rows, vocab_size, temperature, top_k, top_p, min_p, u, out_ids, out_probs};
+    return launch_pick(a, S(stream));
 }
 
 }  // extern "C"

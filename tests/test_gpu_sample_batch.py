@@ -1,0 +1,237 @@
+"""jyc_sample_batch against the 64-bit definition of _paged.picks: the same token in every row,
+except where a sum lies within the fixed-point rounding of a border (then either neighbour)."""
+import numpy as np
+import pytest
+
+import _paged as P
+from _util import dev, host
+from jieyu_b200 import _capi
+
+pytestmark = pytest.mark.gpu
+
+
+def _call(torch, logits, V, T, k, p, mp, u, ids, probs, ld=None, stream=None):
+    return _capi.load().jyc_sample_batch(
+        logits.data_ptr(), logits.stride(0) if ld is None else ld, len(u), V, P.ptr(T), P.ptr(k), P.ptr(p), P.ptr(mp),
+        P.ptr(u), P.ptr(ids), P.ptr(probs), torch.cuda.current_stream().cuda_stream if stream is None else stream)
+
+
+def _run(torch, l, T=None, k=None, p=None, mp=None, u=None, pad=0, off=0):
+    """l [rows][V] float32; returns ids and probabilities, and checks both against the definition."""
+    rows, V = l.shape
+    buf = np.full(rows * (V + pad) + off, 1e30, np.float32)  # what lies behind a row must not be read as logits
+    buf[off:].reshape(rows, V + pad)[:, :V] = l
+    d = dev(torch, buf)
+    before = d.clone()
+    asd = lambda x, t: None if x is None else dev(torch, np.asarray(x, t))  # noqa: E731
+    Td, kd, pd, md, ud = asd(T, np.float32), asd(k, np.int32), asd(p, np.float32), asd(mp, np.float32), asd(u, np.float32)
+    ids = torch.full((rows + 1,), -9, dtype=torch.int32, device="cuda")
+    probs = torch.full((rows + 1,), -9.0, device="cuda")
+    view = d[off:].as_strided((rows, V), (V + pad, 1))
+    _capi.check(_call(torch, view, V, Td, kd, pd, md, ud, ids, probs, ld=V + pad))
+    gi, gp = host(ids), host(probs)
+    assert gi[rows] == -9 and gp[rows] == -9.0
+    assert np.array_equal(host(d).view(np.uint32), host(before).view(np.uint32))
+    at = lambda x, r, t: None if x is None else t(x[r])  # noqa: E731
+    for r in range(rows):
+        want = P.picks(l[r], 1.0 if T is None else np.float32(T[r]), at(k, r, int), at(p, r, float), at(mp, r, float),
+                       u[r])
+        assert int(gi[r]) in want, (r, int(gi[r]), want)
+        # the quotient of two sums that each carry the fixed-point rounding, rounded to fp32 (and
+        # 2^-40 for a border token moved in or out of the sum when several picks are allowed)
+        tol = want[int(gi[r])] * (P.U24 + V * 2.0 ** -42 + 2.0 ** -43) + 2.0 ** -42
+        if len(want) == 1:
+            assert abs(gp[r] - want[int(gi[r])]) <= tol, (r, gp[r], want)
+    again = torch.empty_like(ids)
+    _capi.check(_call(torch, view, V, Td, kd, pd, md, ud, again, None, ld=V + pad))
+    assert np.array_equal(host(again)[:rows], gi[:rows])
+    return gi[:rows], gp[:rows]
+
+
+def _logits(rng, rows, V, kind):
+    l = (2.5 * rng.normal(size=(rows, V))).astype(np.float32)
+    for r in range(rows):
+        n = min(V, 24)
+        l[r, rng.choice(V, n, replace=False)] = (8 + 6 * rng.random(n)).astype(np.float32)
+    if kind == "bf16":  # many equal logits
+        l = (l.view(np.uint32) & 0xFFFF0000).view(np.float32)
+    elif kind == "equal":
+        l[:] = 3.25
+    elif kind == "two":
+        l = np.where(rng.random((rows, V)) < 0.3, np.float32(2.0), np.float32(1.0)).astype(np.float32)
+    elif kind == "masked":
+        l[rng.random((rows, V)) < 0.9] = -np.inf
+        l[rng.random((rows, V)) < 0.02] = np.nan
+        l[:, V // 2] = 1.0
+    elif kind == "lowest":  # a mask of the type's lowest value
+        l[rng.random((rows, V)) < 0.9] = np.finfo(np.float32).min
+        l[:, V // 2] = 1.0
+    elif kind == "huge":
+        l = (l * 1e37).astype(np.float32)
+    elif kind == "tiny":
+        l = (l * 1e-39).astype(np.float32)
+    elif kind == "falling":
+        l = -np.sort(-l, axis=1)
+    elif kind == "flat":
+        l = (l * 0.01).astype(np.float32)
+    elif kind == "peak":
+        l[:, V // 3] = 60.0
+    return l
+
+
+SETTINGS = [  # temperature, top-k, top-p, min-p
+    (None, None, None, None), (0.7, 50, None, None), (1.0, None, 0.9, None), (1.3, None, None, 0.05),
+    (0.8, 40, 0.95, 0.02), (1.0, 1, 0.5, None), (2.0, 3000, 0.999, None), (0.05, 10, 0.3, 0.5),
+    (1.0, 0, 1.0, 0.0), (5.0, None, 0.5, None), (1.0, None, 0.0, None), (1.0, 2, 1.5, -1.0),
+]
+
+
+@pytest.mark.parametrize("V", [1, 2, 17, 1000, 1023, 4097, 32000])
+@pytest.mark.parametrize("kind", ["plain", "bf16", "equal", "two", "masked", "lowest", "huge", "tiny", "falling",
+                                  "flat", "peak"])
+def test_picks(cuda, V, kind):
+    rng = np.random.default_rng(V * 13 + len(kind))
+    l = _logits(rng, len(SETTINGS), V, kind)
+    u = rng.random(len(SETTINGS)).astype(np.float32)
+    for i in range(3):
+        off = {0: 1.0, 1: 0, 2: 1.0, 3: 0.0}
+        col = lambda c: [s[c] if s[c] is not None else off[c] for s in SETTINGS]  # noqa: E731
+        _run(cuda, l, col(0), col(1), col(2), col(3), u, pad=(0, 3, 4)[i], off=(0, 1, 0)[i])
+        u = rng.random(len(SETTINGS)).astype(np.float32)
+
+
+@pytest.mark.parametrize("T,k,p,mp", SETTINGS)
+def test_arrays_may_be_absent(cuda, T, k, p, mp):
+    rng = np.random.default_rng(77)
+    rows = 5
+    l = _logits(rng, rows, 5003, "plain")
+    full = lambda x: None if x is None else [x] * rows  # noqa: E731
+    _run(cuda, l, full(T), full(k), full(p), full(mp), rng.random(rows).astype(np.float32))
+
+
+@pytest.mark.parametrize("rows,V", [(1, 151936), (3, 128256), (40, 50257), (300, 2048), (700, 3), (1, 1 << 20)])
+def test_large(cuda, rows, V):
+    rng = np.random.default_rng(V)
+    l = _logits(rng, rows, V, "plain")
+    i = np.arange(rows) if rows > 1 else np.array([4])
+    _run(cuda, l, np.where(i % 5 == 0, 0.0, 0.5 + rng.random(rows)), np.where(i % 3 == 1, 50, 0),
+         np.where(i % 2 == 0, 0.9, 1.0), np.where(i % 7 == 2, 0.05, 0.0), rng.random(rows).astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", ["flat", "equal", "bf16", "two"])
+def test_large_and_flat(cuda, kind):
+    """Borders that fall among tens of thousands of (nearly) equal logits."""
+    rng = np.random.default_rng(5)
+    rows, V = 6, 128256
+    l = _logits(rng, rows, V, kind)
+    _run(cuda, l, [1.0] * rows, [0, 60000, 0, 100000, 1, 0], [0.5, 1.0, 0.9, 0.7, 0.5, 1.0], [0, 0, 0, 0, 0, 0.9],
+         rng.random(rows).astype(np.float32))
+
+
+def test_draws_at_the_ends(cuda):
+    """u of 0, just below 1, and out of range or NaN: always a kept token."""
+    l = np.full((6, 50), -np.inf, np.float32)
+    l[:, [7, 20, 33]] = [0.0, 1.0, 0.5]
+    u = np.array([0.0, 1 - 2.0 ** -24, 1.0, 2.0, -0.5, np.nan], np.float32)
+    torch = cuda
+    d, ud = dev(torch, l), dev(torch, u)
+    ids = torch.empty(6, dtype=torch.int32, device="cuda")
+    _capi.check(_call(torch, d, 50, None, None, None, None, ud, ids, None))
+    assert host(ids).tolist() == [7, 33, 33, 33, 7, 33]
+
+
+def test_greedy_rows_equal_argmax(cuda):
+    torch = cuda
+    rng = np.random.default_rng(2)
+    V = 5000
+    l = np.round(3 * rng.normal(size=(4, V))).astype(np.float32)  # ties everywhere
+    l[1, 17] = np.nan
+    l[2, :] = -0.0
+    l[2, 5] = 0.0
+    d = dev(torch, l)
+    ids = torch.empty(4, dtype=torch.int32, device="cuda")
+    probs = torch.empty(4, device="cuda")
+    T = dev(torch, np.array([0.0, -1.0, np.nan, 0.0], np.float32))
+    u = dev(torch, np.zeros(4, np.float32))
+    _capi.check(_call(torch, d, V, T, None, None, None, u, ids, probs))
+    got = host(ids)
+    for r in (0, 1, 3):
+        one = torch.empty(1, dtype=torch.int32, device="cuda")
+        _capi.check(_capi.load().jyc_argmax(d[r].data_ptr(), V, one.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        assert got[r] == int(one)
+    assert got[2] == 0  # the two zeros are equal
+    assert np.all(host(probs) == 1.0)
+
+
+def test_rows_that_hold_nothing_and_infinities(cuda):
+    torch = cuda
+    V = 300
+    l = np.zeros((6, V), np.float32)
+    l[0] = -np.inf
+    l[1] = np.nan
+    l[2, ::2], l[2, 1::2] = np.nan, -np.inf
+    l[3, [10, 200]] = np.inf
+    l[4] = -np.inf
+    l[4, 99] = -3e38
+    l[5, 250] = np.inf
+    for T in (0.0, 1.0, np.inf):
+        T6 = np.full(6, T, np.float32)
+        d = dev(torch, l)
+        ids = torch.empty(6, dtype=torch.int32, device="cuda")
+        probs = torch.empty(6, device="cuda")
+        u = dev(torch, np.full(6, 0.75, np.float32))
+        _capi.check(_call(torch, d, V, dev(torch, T6), None, None, None, u, ids, probs))
+        got, p = host(ids), host(probs)
+        assert got[:3].tolist() == [-1, -1, -1] and np.all(p[:3] == 0.0)
+        assert got[3] == (10 if T == 0 else 200) and p[3] == (1.0 if T == 0 else 0.5)
+        assert got[4] == 99 and p[4] == 1.0
+        assert got[5] == 250 and p[5] == 1.0
+
+
+def test_captured_and_on_two_streams(cuda):
+    torch = cuda
+    rng = np.random.default_rng(6)
+    rows, V = 9, 20000
+    l = [_logits(rng, rows, V, "plain") for _ in range(3)]
+    k = dev(torch, np.full(rows, 30, np.int32))
+    d = dev(torch, l[0])
+    u = rng.random(rows).astype(np.float32)
+    ud = dev(torch, u)
+    ids = torch.empty(rows, dtype=torch.int32, device="cuda")
+    _capi.check(_call(torch, d, V, None, k, None, None, ud, ids, None))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        _capi.check(_call(torch, d, V, None, k, None, None, ud, ids, None))
+    for x in l:
+        d.copy_(torch.from_numpy(x))
+        g.replay()
+        got = host(ids)
+        assert all(int(got[r]) in P.picks(x[r], 1.0, 30, None, None, u[r]) for r in range(rows))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ds = [dev(torch, x) for x in l[:2]]
+    outs = [torch.empty(rows, dtype=torch.int32, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            _capi.check(_call(torch, ds[i], V, None, k, None, None, ud, outs[i], None, stream=streams[i].cuda_stream))
+    torch.cuda.synchronize()
+    for i in range(2):
+        got = host(outs[i])
+        assert all(int(got[r]) in P.picks(l[i][r], 1.0, 30, None, None, u[r]) for r in range(rows))
+
+
+def test_distribution(cuda):
+    """Equally spaced u sweep the inverse CDF: each token is picked as often as its weight says, to one."""
+    torch = cuda
+    rng = np.random.default_rng(4)
+    V, n = 40, 4096
+    row = rng.normal(size=V).astype(np.float32)
+    l = np.repeat(row[None], n, 0)
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    ids, probs = _run(torch, l, [1.1] * n, [20] * n, [0.9] * n, [0.0] * n, u)
+    keep = np.unique(ids)
+    w = P.weights(row, np.float64(np.float32(1.1)))[1][keep]
+    count = np.array([(ids == i).sum() for i in keep])
+    assert np.all(np.abs(count - n * w / w.sum()) <= 1.0 + 1e-6)
+    assert np.all(np.diff(ids) >= 0)
