@@ -455,7 +455,7 @@ JYC_API size_t jyc_attention_paged_q8_workspace(int num_seqs, int num_heads, int
         arg_error("attention_paged_q8_workspace: bad shape");
         return 0;
     }
-    return paged_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim);
+    return paged_attention_workspace(num_heads, num_kv_heads, head_dim);
 }
 
 JYC_API int jyc_attention_paged_q8(const float* Q, int ldq, float* out, int ldo, int num_heads, int num_kv_heads,
@@ -471,7 +471,7 @@ JYC_API int jyc_attention_paged_q8(const float* Q, int ldq, float* out, int ldo,
         return arg_error("attention_paged_q8: ldq and ldo must hold num_heads * head_dim");
     if (num_seqs == 0) return JYC_OK;
     if (!Q || !out || !seq_lens) return arg_error("attention_paged_q8: null pointer");
-    const size_t need = paged_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim);
+    const size_t need = paged_attention_workspace(num_heads, num_kv_heads, head_dim);
     if (need == 0) return JYC_ERR_CUDA;
     if (workspace && workspace_bytes < need) return arg_error("attention_paged_q8: workspace too small");
     if ((uintptr_t)workspace & 15) return arg_error("attention_paged_q8: workspace must be 16-byte aligned");

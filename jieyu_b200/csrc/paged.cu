@@ -3,8 +3,10 @@
 // back as fp32, and attended over by one new token per sequence (the score,
 // softmax and P.V of attention_q8.h:38-184).
 #include "paged.cuh"
+#include "ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace jyc {
 
@@ -132,92 +134,689 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
     for (int e = lane; e < hd; e += 32) dst[e] = __fmul_rn((float)src[e], sc);
 }
 
-// CTA = (query head, sequence), 8 warps; warp w takes positions w, w + 8, ...
-// with its own online softmax: one position at a time, a lane holds up to 8
-// dims. The warps' (m, l, o) are joined at the end.
-constexpr int kSimpleWarps = 8;
+// ---------------------------------------------------------------------------
+// Attention of one new token per sequence.
+//
+// out = sum_j p_j vs_j v_j / sum_j p_j, p_j = exp(dot_j (ks_j qs) / sqrt(hd)),
+// one pass over the keys with a running reference. In base 2, with vs_j =
+// 2^e_j f_j (1 <= f_j < 2): ref = max_j (s_j + e_j) - 13, b_j = 2^(s_j - ref);
+// the weights w_j = b_j vs_j are below 2^14 and the largest is at least 2^13,
+// so as a pair of fp16 (hi + lo, 22 bits) they neither overflow nor lose a
+// small vs that carries all the weight; the denominator adds the b_j.
+//
+// A step reads sum(len) * KV * (2 hd + 8) bytes and is bound by them, so: work
+// is a line of units (a unit: TK keys of one kv head of one sequence, 16-byte
+// cp.async rows), cut into equal runs for all resident warps whatever the
+// lengths; a warp keeps its next units in flight in its own ring in shared
+// memory across the borders of sequences and has no barrier in its loop. The
+// (up to 8 or 16) query heads of a kv head are the rows of one m16 tile:
+// q.k with mma.m16n8k32 s8 (exact dots), P.V with mma.m16n8k16 f16 (V is exact
+// in fp16). Up to 8 heads, the hi halves are rows 0-7 and the lo halves rows
+// 8-15 of the same product. Each unit's product starts from zero and is added
+// in fp32 with round to nearest (the tensor cores' own sums may truncate).
+//
+// A run that covers an item (a kv head of a sequence) whole writes its rows of
+// out; the others leave (o, ref, l) in the workspace and a second kernel,
+// launched early, joins them. The warps of a CTA inside one item are joined in
+// shared memory first.
 
-__global__ void __launch_bounds__(kSimpleWarps * 32) paged_attention_kernel(PagedAttn a) {
-    __shared__ float s_m[kSimpleWarps], s_l[kSimpleWarps], s_o[kSimpleWarps][256];
-    const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = h / (a.H / a.KV), hd = a.hd, half = hd >> 1, nq = hd >> 2;
+constexpr int kPaWarps = 4;
+constexpr float kPaShift = 13.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void pa_copy(uint32_t dst, const void* src) {
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// bytes 0, 2 (ODD: 1, 3) of x = q ^ 0x80 as the halves q: 0x6400 | u is 1024 + u
+template <bool ODD>
+__device__ __forceinline__ uint32_t pa_half2(uint32_t x) {
+    const uint32_t m = __byte_perm(x, 0x64646464u, ODD ? 0x4341 : 0x4240);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pa_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Sizes of one instantiation: HDP is the head size rounded up (the columns
+// behind it hold whatever the ring held, finite as integers; they meet zero
+// query columns and unread output columns), ROWS the query heads of a unit.
+template <int HDP, int ROWS>
+struct PaCfg {
+    static constexpr int TK = HDP <= 128 ? 32 : 16;   // keys of a unit
+    static constexpr int ST = HDP <= 64 ? 3 : HDP <= 128 ? 2 : 3;
+    static constexpr int PITCH = HDP + 16;            // odd in 16-byte chunks: ldmatrix rows in distinct banks
+    static constexpr int VOFF = TK * PITCH, SOFF = 2 * TK * PITCH;
+    static constexpr int STAGE = SOFF + 8 * TK + 16;  // K, V, ks, vs, valid mask
+    static constexpr int CTAS = HDP <= 128 ? 3 : 2;   // resident per SM
+    static constexpr int PART = ROWS * (HDP + 2);     // floats of a partial: o, then (ref, l) per row
+    static constexpr int RING = ST * STAGE > PART * 4 ? ST * STAGE : (PART * 4 + 15) / 16 * 16;
+    static constexpr int SMEM = kPaWarps * RING;
+};
+
+// What the kernels share about the line of units.
+struct PaPlan {
+    int units_row;  // kv heads * query blocks
+    int qblocks;    // blocks of ROWS query heads per kv head
+    int tk;
+    int ctas;       // of the main kernel
+    bool wide_copy; // 16-byte copies
+};
+// Item that a warp's run starts and another one ends.
+struct PaTail {
+    long long u0, u1;  // units of the item; u1 == 0: none
+    int b, r;
+};
+struct PaWork {
+    long long* total;  // units of the call
+    PaTail* tail;      // [warps]
+    float* part;       // [warps][2][PART]: an item's later part (0), its first (1)
+};
+
+__device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
     int len = a.lens[b];
-    const long long cap = (long long)a.kv.table_stride * a.kv.p.page_size;
+    if (len <= 0) return 0;
+    const int cap = a.kv.table_stride * a.kv.p.page_size;
     if (len > cap) {
         paged_flag(kPagedErrPos);
-        len = (int)cap;
+        len = cap;
     }
-    float* out = a.out + (size_t)b * a.ldo + (size_t)h * hd;
-    if (len > 0 && a.rope.cos_t && len > a.rope.len) {
+    if (a.rope.cos_t && len > a.rope.len) {
         paged_flag(kPagedErrRope);
         len = 0;
     }
-    if (len <= 0) {
-        for (int e = threadIdx.x; e < hd; e += blockDim.x) out[e] = 0.0f;
-        return;
+    return len;
+}
+// Warps that get units, and where the run of warp w starts.
+__device__ __forceinline__ long long pa_workers(long long U, int ctas) {
+    return min((long long)ctas * kPaWarps, U);
+}
+__device__ __forceinline__ long long pa_start(long long U, long long workers, long long w) {
+    return w >= workers ? U : U * w / workers;
+}
+
+struct PaCursor {
+    int b, r, t, nt, len;  // sequence, row of units, unit and units in it, length
+};
+__device__ __forceinline__ void pa_seek(const PagedAttn& a, int tk, PaCursor& c) {
+    c.len = 0;
+    while (c.b < a.kv.num_seqs && (c.len = pa_len(a, c.b)) == 0) c.b++;
+    c.nt = (c.len + tk - 1) / tk;
+}
+__device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, PaCursor& c) {
+    if (++c.t < c.nt) return;
+    c.t = 0;
+    if (++c.r < pl.units_row) return;
+    c.r = 0;
+    c.b++;
+    pa_seek(a, pl.tk, c);
+}
+
+template <int HDP, int ROWS>
+__global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
+    paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work) {
+    using G = PaCfg<HDP, ROWS>;
+    constexpr int TK = G::TK, ST = G::ST, PITCH = G::PITCH;
+    constexpr int NK = HDP / 32, NJ = TK / 8, NC = HDP / 32, E = ROWS / 8;  // E: rows a lane holds
+    extern __shared__ __align__(128) unsigned char pa_sm[];
+    __shared__ long long s_scan[kPaWarps * 32 + 1];
+    __shared__ PaCursor s_cur[kPaWarps];
+    __shared__ long long s_first[kPaWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int wid = blockIdx.x * kPaWarps + warp;
+    const int B = a.kv.num_seqs, group = a.H / a.KV, hd = a.hd;
+    griddep_launch();
+
+    // where the units of each sequence lie in the line
+    const int per = (B + kPaWarps * 32 - 1) / (kPaWarps * 32);
+    const int bs = min(B, tid * per), be = min(B, bs + per);
+    long long mine = 0;
+    for (int b = bs; b < be; b++) mine += (pa_len(a, b) + TK - 1) / TK;
+    mine *= pl.units_row;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
     }
-    float4 x[2];
-    int slot4[2];
-    float amax = 0.0f;
-    for (int t = 0; t < 2; t++) {
-        const int qd = lane + 32 * t;
-        slot4[t] = qd;
-        x[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (qd >= nq) continue;
-        x[t] = load4(a.Q + (size_t)b * a.ldq + (size_t)h * hd + 4 * qd, false);
-        if (a.rope.cos_t) {
-            x[t] = rotate4(x[t], a.rope.cos_t + (size_t)(len - 1) * half, a.rope.sin_t + (size_t)(len - 1) * half, qd);
-            slot4[t] = rope_slot(2 * qd, half) >> 1;
-        }
-        amax = fmaxf(amax, amax4(x[t]));
-    }
-    amax = warp_max(amax);
-    const float inv = q8_inv(amax), qs = q8_scale(amax);
-    const uint32_t q[2] = {pack4(x[0], inv), pack4(x[1], inv)};
-    float m = -INFINITY, l = 0.0f, o[2][4] = {};
-    for (int j = warp; j < len; j += kSimpleWarps) {
-        const int page = paged_page(a.kv, b, j);
-        if (page < 0) continue;
-        const int slot = j % a.kv.p.page_size;
-        const uint32_t* kr = reinterpret_cast<const uint32_t*>(a.kv.p.k + paged_off(a.kv, page, slot, kvh));
-        const uint32_t* vr = reinterpret_cast<const uint32_t*>(a.kv.p.v + paged_off(a.kv, page, slot, kvh));
-        int dot = 0;
-        for (int t = 0; t < 2; t++)
-            if (lane + 32 * t < nq) dot = __dp4a((int)q[t], (int)kr[slot4[t]], dot);
-        for (int i = 16; i > 0; i >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, i);
-        const size_t so = paged_soff(a.kv, page, slot, kvh);
-        const float sc = __fmul_rn((float)dot, __fmul_rn(__fmul_rn(a.kv.p.ks[so], qs), a.scale));
-        const float mn = fmaxf(m, sc);
-        const float al = m == -INFINITY ? 0.0f : expf(m - mn), e = expf(sc - mn), w = e * a.kv.p.vs[so];
-        m = mn;
-        l = l * al + e;
-        for (int t = 0; t < 2; t++) {
-            float f[4] = {};
-            if (lane + 32 * t < nq) u8x4_to_f32(vr[lane + 32 * t] ^ 0x80808080u, f);
-            for (int i = 0; i < 4; i++) o[t][i] = __fmaf_rn(w, f[i], o[t][i] * al);
-        }
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-    for (int t = 0; t < 2; t++)
-        if (lane + 32 * t < nq)
-            for (int i = 0; i < 4; i++) s_o[warp][4 * (lane + 32 * t) + i] = o[t][i];
+    if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < kSimpleWarps; w++) M = fmaxf(M, s_m[w]);
-    for (int e = threadIdx.x; e < hd; e += blockDim.x) {
-        float O = 0.0f;
-        L = 0.0f;
-        for (int w = 0; w < kSimpleWarps; w++) {
-            if (s_m[w] == -INFINITY) continue;
-            const float wgt = expf(s_m[w] - M);
-            L = __fmaf_rn(wgt, s_l[w], L);
-            O = __fmaf_rn(wgt, s_o[w][e], O);
-        }
-        out[e] = M == -INFINITY ? 0.0f : O / L;
+    long long U = 0, ex = incl - mine;
+    for (int w = 0; w < kPaWarps; w++) {
+        if (w < warp) ex += s_scan[w];
+        U += s_scan[w];
     }
+    const long long workers = pa_workers(U, gridDim.x);
+    if (blockIdx.x == 0 && tid == 0) *work.total = U;
+    for (int w = 0; w < kPaWarps; w++) {
+        const long long u = pa_start(U, workers, (long long)blockIdx.x * kPaWarps + w);
+        if (u < ex || u >= ex + mine) continue;
+        long long at = ex;
+        for (int b = bs; b < be; b++) {
+            const int len = pa_len(a, b), nt = (len + TK - 1) / TK;
+            const long long n = (long long)nt * pl.units_row;
+            if (u < at + n) {
+                const int k = (int)(u - at);
+                s_cur[w] = PaCursor{b, k / nt, k % nt, nt, len};
+                s_first[w] = u - k % nt;  // first unit of the item that the run starts in
+                break;
+            }
+            at += n;
+        }
+    }
+    // sequences without a key: rows of zeros
+    for (int b = blockIdx.x; b < B; b += gridDim.x)
+        if (pa_len(a, b) == 0)
+            for (int e = tid; e < a.H * hd; e += kPaWarps * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
+    __syncthreads();
+
+    const long long u0 = pa_start(U, workers, wid), u1 = pa_start(U, workers, wid + 1);
+    const long long c0 = pa_start(U, workers, (long long)blockIdx.x * kPaWarps);
+    const long long c1 = pa_start(U, workers, (long long)(blockIdx.x + 1) * kPaWarps);
+    const int count = (int)(u1 - u0);
+    unsigned char* ring = pa_sm + warp * G::RING;
+    const uint32_t ring_a = smem_u32(ring);
+    PaCursor cur = PaCursor{0, 0, 0, 0, 0};
+    long long item0 = 0;
+    if (count > 0) {
+        cur = s_cur[warp];
+        item0 = s_first[warp];
+    }
+    // every warp of the CTA inside one item: joined below
+    bool joint = false, whole = false;  // whole: and they are all of it
+    if (c1 > c0) {
+        const long long first = s_first[0], end = first + s_cur[0].nt;
+        joint = c1 <= end;
+        whole = c0 == first && c1 == end;
+    }
+    if (lane == 0) work.tail[wid].u1 = 0;
+
+    // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
+    PaCursor nx = cur;
+    int issued = 0;  // units whose pages are looked up
+    int pg = -1, slot = 0, h = 0;
+    bool ok = false;
+    auto lookup = [&] {
+        ok = false;
+        if (issued < count) {
+            const int pos = nx.t * TK + lane;
+            h = nx.r / pl.qblocks;
+            if (lane < TK && pos < nx.len) {
+                const int idx = pos / a.kv.p.page_size;
+                slot = pos - idx * a.kv.p.page_size;
+                pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
+                ok = true;
+            }
+            pa_next(a, pl, nx);
+        }
+        issued++;
+    };
+    auto issue = [&](int st) {  // copies of the unit that was looked up last
+        if (ok && (pg < 0 || pg >= a.kv.p.num_pages)) {
+            paged_flag(kPagedErrPage);
+            ok = false;
+        }
+        const uint32_t base = ring_a + st * G::STAGE;
+        const unsigned mask = __ballot_sync(0xffffffffu, ok);
+        long long off = 0;
+        if (ok) {
+            off = (long long)paged_off(a.kv, pg, slot, h);
+            const size_t so = paged_soff(a.kv, pg, slot, h);
+            pa_copy<4>(base + G::SOFF + 4 * lane, a.kv.p.ks + so);
+            pa_copy<4>(base + G::SOFF + 4 * TK + 4 * lane, a.kv.p.vs + so);
+        }
+        if (lane == 0) *reinterpret_cast<unsigned*>(ring + st * G::STAGE + G::SOFF + 8 * TK) = mask;
+        if (mask != 0u) {
+            if (pl.wide_copy) {
+                constexpr int LPR = HDP <= 64 ? 4 : HDP <= 128 ? 8 : 16, RPI = 32 / LPR;  // lanes per row, rows per step
+                const int c = lane & (LPR - 1);
+#pragma unroll
+                for (int i = 0; i < TK / RPI; i++) {
+                    const int row = i * RPI + lane / LPR;
+                    const long long o = __shfl_sync(0xffffffffu, off, row);
+                    if (((mask >> row) & 1) && c * 16 < hd) {
+                        pa_copy<16>(base + row * PITCH + c * 16, a.kv.p.k + o + c * 16);
+                        pa_copy<16>(base + G::VOFF + row * PITCH + c * 16, a.kv.p.v + o + c * 16);
+                    }
+                }
+            } else {
+                for (int row = 0; row < TK; row++) {
+                    const long long o = __shfl_sync(0xffffffffu, off, row);
+                    if (!((mask >> row) & 1)) continue;
+                    for (int c = lane; c * 4 < hd; c += 32) {
+                        pa_copy<4>(base + row * PITCH + c * 4, a.kv.p.k + o + c * 4);
+                        pa_copy<4>(base + G::VOFF + row * PITCH + c * 4, a.kv.p.v + o + c * 4);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    lookup();
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) {
+        issue(i);
+        lookup();
+    }
+
+    uint32_t qa[NK][4];
+    float qsl[E], ref[E], l[E], o[HDP / 16][E][4];
+    bool fresh = true;
+    int st = 0;
+    const float up = __fmul_rn(a.scale, 1.44269504088896341f);
+
+    for (int n = 0; n < count; n++) {
+        if (fresh) {
+            // the item's query heads: rotated, quantised per head, straight into the A fragments; lane (g, t)
+            // holds bytes 4t..4t+3 of every 16 of rows g and g + 8
+            fresh = false;
+            const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
+            const int half = hd >> 1;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int row = qb * ROWS + 8 * e + g;
+                const bool live = row < group;
+                const float* q = a.Q + (size_t)cur.b * a.ldq + (size_t)(kvh * group + (live ? row : 0)) * hd;
+                const size_t tp = (size_t)(cur.len - 1) * half;
+                float4 x[2 * NK];
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 2 * NK; i++) {
+                    int src = 4 * i + t;  // quad stored in slot 4 i + t
+                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (!live || 4 * src >= hd) continue;
+                    if (a.rope.cos_t) {
+                        src = rope_slot(2 * src, half) >> 1;  // its own inverse
+                        x[i] = rotate4(load4(q + 4 * src, false), a.rope.cos_t + tp, a.rope.sin_t + tp, src);
+                    } else {
+                        x[i] = load4(q + 4 * src, false);
+                    }
+                    amax = fmaxf(amax, amax4(x[i]));
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const float inv = q8_inv(amax);
+                qsl[e] = __fmul_rn(q8_scale(amax), up);
+#pragma unroll
+                for (int i = 0; i < 2 * NK; i++) qa[i >> 1][e + 2 * (i & 1)] = pack4(x[i], inv);
+                ref[e] = -INFINITY;
+                l[e] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < HDP / 16; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
+            }
+            if (E == 1)
+#pragma unroll
+                for (int i = 0; i < NK; i++) qa[i][1] = qa[i][3] = 0u;
+        }
+        // the next unit's copies go to the stage that the last iteration read
+        __syncwarp();
+        issue(st == 0 ? ST - 1 : st - 1);
+        lookup();
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        __syncwarp();
+        const unsigned char* sb = ring + st * G::STAGE;
+        const uint32_t base = ring_a + st * G::STAGE;
+        const unsigned mask = *reinterpret_cast<const unsigned*>(sb + G::SOFF + 8 * TK);
+        const float* sks = reinterpret_cast<const float*>(sb + G::SOFF);
+        const float* svs = sks + TK;
+
+        // scores of keys 8 j + 2 t, + 1 for rows g (and g + 8), in base 2
+        float s[NJ][E][2];
+        float top[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) top[e] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            int c[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < NK; k += 2) {
+                uint32_t b[4];
+                pa_ldsm(base + (8 * j + (lane & 7)) * PITCH + (2 * k + (lane >> 3)) * 16, b);
+                pa_mma_s8(qa[k], b[0], b[1], c);
+                if (k + 1 < NK) pa_mma_s8(qa[k + 1], b[2], b[3], c);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int key = 8 * j + 2 * t + i;
+                const float kf = sks[key];
+                const int ex = min(max((int)((__float_as_uint(svs[key]) >> 23) & 255u), 63), 253) - 127;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float v = (mask >> key) & 1 ? __fmul_rn((float)c[2 * e + i], __fmul_rn(kf, qsl[e])) : -INFINITY;
+                    s[j][e][i] = v;
+                    top[e] = fmaxf(top[e], v + (float)ex);
+                }
+            }
+        }
+        float al[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+            const float nr = fmaxf(ref[e], top[e] - kPaShift);
+            al[e] = ref[e] == -INFINITY ? 0.0f : ex2(ref[e] - nr);
+            ref[e] = nr;
+            l[e] *= al[e];
+        }
+        // weights as A fragments: keys 16 k + 2 t, + 1 in a0 (a1), 8 later in a2 (a3)
+        uint32_t hi[TK / 16][4], lo[E == 1 ? 1 : TK / 16][4];
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const float v0 = svs[8 * j + 2 * t], v1 = svs[8 * j + 2 * t + 1];
+            const bool m0 = (mask >> (8 * j + 2 * t)) & 1, m1 = (mask >> (8 * j + 2 * t + 1)) & 1;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float b0 = m0 ? ex2(s[j][e][0] - ref[e]) : 0.0f, b1 = m1 ? ex2(s[j][e][1] - ref[e]) : 0.0f;
+                l[e] += b0 + b1;
+                const float w0 = m0 ? b0 * v0 : 0.0f, w1 = m1 ? b1 * v1 : 0.0f;
+                const uint32_t ph = pa_pack(w0, w1);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
+                const uint32_t pl2 = pa_pack(w0 - hf.x, w1 - hf.y);
+                const int f = 2 * (j & 1);
+                if (E == 1) {
+                    hi[j >> 1][f] = ph;
+                    hi[j >> 1][f + 1] = pl2;
+                } else {
+                    hi[j >> 1][f + e] = ph;
+                    lo[E == 1 ? 0 : j >> 1][f + e] = pl2;
+                }
+            }
+        }
+        // P.V: 32 dims at a time; a transposed load gives each lane two neighbouring dims of two keys, so the
+        // even dims make one n8 tile and the odd ones another: lane t ends with dims 4 t .. 4 t + 3 of every 16
+#pragma unroll
+        for (int d = 0; d < NC; d++) {
+            float c[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < TK / 16; k++) {
+                uint32_t v[4];
+                pa_ldsm_t(base + G::VOFF + (16 * k + (lane & 15)) * PITCH + (2 * d + (lane >> 4)) * 16, v);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t e0 = pa_half2<false>(v[2 * i]), e1 = pa_half2<false>(v[2 * i + 1]);
+                    const uint32_t o0 = pa_half2<true>(v[2 * i]), o1 = pa_half2<true>(v[2 * i + 1]);
+                    pa_mma_f16(hi[k], e0, e1, c[2 * i]);
+                    pa_mma_f16(hi[k], o0, o1, c[2 * i + 1]);
+                    if (E == 2) {
+                        pa_mma_f16(lo[E == 1 ? 0 : k], e0, e1, c[2 * i]);
+                        pa_mma_f16(lo[E == 1 ? 0 : k], o0, o1, c[2 * i + 1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float* od = o[2 * d + (i >> 1)][0];
+                if (E == 1) {
+                    od[i & 1] = __fmaf_rn(od[i & 1], al[0], c[i][0] + c[i][2]);
+                    od[2 + (i & 1)] = __fmaf_rn(od[2 + (i & 1)], al[0], c[i][1] + c[i][3]);
+                } else {
+                    float* oe = o[2 * d + (i >> 1)][E - 1];
+                    od[i & 1] = __fmaf_rn(od[i & 1], al[0], c[i][0]);
+                    od[2 + (i & 1)] = __fmaf_rn(od[2 + (i & 1)], al[0], c[i][1]);
+                    oe[i & 1] = __fmaf_rn(oe[i & 1], al[E - 1], c[i][2]);
+                    oe[2 + (i & 1)] = __fmaf_rn(oe[2 + (i & 1)], al[E - 1], c[i][3]);
+                }
+            }
+        }
+        st = st == ST - 1 ? 0 : st + 1;
+
+        const bool item_end = cur.t == cur.nt - 1;
+        if (!item_end && n + 1 < count) {
+            cur.t++;
+            continue;
+        }
+        // the end of an item or of the run
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+        const bool from_start = item0 >= u0;
+        if (from_start && item_end) {
+            const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int row = qb * ROWS + 8 * e + g;
+                if (row >= group) continue;
+                float* out = a.out + (size_t)cur.b * a.ldo + (size_t)(kvh * group + row) * hd;
+                const float inv = l[e] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[e]);
+#pragma unroll
+                for (int d = 0; d < HDP / 16; d++)
+                    if (16 * d + 4 * t < hd)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) out[16 * d + 4 * t + i] = o[d][e][i] * inv;
+            }
+        } else {
+            if (from_start && lane == 0 && !whole) work.tail[wid] = PaTail{item0, item0 + cur.nt, cur.b, cur.r};
+            if (joint) break;  // o, ref and l stay in registers
+            float* part = work.part + ((size_t)wid * 2 + (from_start ? 1 : 0)) * G::PART;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int row = 8 * e + g;
+#pragma unroll
+                for (int d = 0; d < HDP / 16; d++)
+                    *reinterpret_cast<float4*>(part + row * HDP + 16 * d + 4 * t) =
+                        make_float4(o[d][e][0], o[d][e][1], o[d][e][2], o[d][e][3]);
+                if (t == 0) *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(ref[e], l[e]);
+            }
+        }
+        if (n + 1 < count) {
+            item0 += cur.nt;
+            pa_next(a, pl, cur);
+            fresh = true;
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!joint || (whole && pa_start(U, workers, (long long)blockIdx.x * kPaWarps + 1) == c1)) return;
+
+    // join the CTA's warps (their rings are free now)
+    float* buf = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int row = 8 * e + g;
+        if (count > 0)
+#pragma unroll
+            for (int d = 0; d < HDP / 16; d++)
+                *reinterpret_cast<float4*>(buf + row * HDP + 16 * d + 4 * t) =
+                    make_float4(o[d][e][0], o[d][e][1], o[d][e][2], o[d][e][3]);
+        if (t == 0)
+            *reinterpret_cast<float2*>(buf + ROWS * HDP + 2 * row) =
+                count > 0 ? make_float2(ref[e], l[e]) : make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+    const PaCursor c = s_cur[0];
+    const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
+    float* part = work.part + ((size_t)blockIdx.x * kPaWarps * 2 + (c0 == s_first[0] ? 1 : 0)) * G::PART;
+    for (int i = tid; i < ROWS * HDP / 4; i += kPaWarps * 32) {
+        const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kPaWarps; w++)
+            M = fmaxf(M, reinterpret_cast<const float*>(pa_sm + w * G::RING)[ROWS * HDP + 2 * row]);
+        for (int w = 0; w < kPaWarps; w++) {
+            const float* wb = reinterpret_cast<const float*>(pa_sm + w * G::RING);
+            const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
+            if (wr == -INFINITY && wl == 0.0f) continue;
+            const float f = wr == -INFINITY ? 0.0f : ex2(wr - M);
+            const float4 x = *reinterpret_cast<const float4*>(wb + row * HDP + d);
+            L = __fmaf_rn(f, wl, L);
+            O = make_float4(__fmaf_rn(f, x.x, O.x), __fmaf_rn(f, x.y, O.y), __fmaf_rn(f, x.z, O.z), __fmaf_rn(f, x.w, O.w));
+        }
+        if (whole) {
+            if (qb * ROWS + row < group && d < hd) {
+                float* out = a.out + (size_t)c.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd + d;
+                const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+                out[0] = O.x * inv;
+                out[1] = O.y * inv;
+                out[2] = O.z * inv;
+                out[3] = O.w * inv;
+            }
+        } else {
+            *reinterpret_cast<float4*>(part + row * HDP + d) = O;
+            if (d == 0) *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(M, L);
+        }
+    }
+}
+
+// CTA = the warps of one CTA of the kernel above: the items that start in their
+// runs and end in another one. Warp = query row; the parts of an item are, in
+// order, those of single warps at its ends and one of every CTA inside it.
+constexpr int kPaJoinWarps = 8;
+template <int HDP, int ROWS>
+__global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
+    using G = PaCfg<HDP, ROWS>;
+    constexpr int ND = (HDP + 127) / 128;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.H / a.KV, hd = a.hd;
+    griddep_wait();
+    const long long U = *work.total, workers = pa_workers(U, pl.ctas);
+    for (int wi = 0; wi < kPaWarps; wi++) {
+        const long long wf = (long long)blockIdx.x * kPaWarps + wi;
+        const PaTail tail = work.tail[wf];
+        if (tail.u1 == 0) continue;
+        long long wl = (tail.u1 - 1) * workers / U;
+        while (pa_start(U, workers, wl + 1) <= tail.u1 - 1) wl++;
+        while (pa_start(U, workers, wl) > tail.u1 - 1) wl--;
+        const long long cf = wf / kPaWarps, cl = wl / kPaWarps;
+        auto inside = [&](long long c) {
+            return pa_start(U, workers, c * kPaWarps) >= tail.u0 && pa_start(U, workers, (c + 1) * kPaWarps) <= tail.u1;
+        };
+        const bool ff = inside(cf), fl = inside(cl);
+        const int na = ff ? 1 : (int)(min(wl, cf * kPaWarps + kPaWarps - 1) - wf) + 1;
+        const int nm = (int)max(0LL, cl - cf - 1), nb = cl == cf ? 0 : fl ? 1 : (int)(wl - cl * kPaWarps) + 1;
+        const int np = na + nm + nb;
+        auto piece = [&](int i) -> const float* {
+            const long long w = i < na ? wf + i : i < na + nm ? (cf + 1 + i - na) * kPaWarps : cl * kPaWarps + (i - na - nm);
+            return work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
+        };
+        const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
+        for (int row = warp; row < ROWS && qb * ROWS + row < group; row += kPaJoinWarps) {
+            float M = -INFINITY, L = 0.0f;
+            for (int i = lane; i < np; i += 32) M = fmaxf(M, piece(i)[ROWS * HDP + 2 * row]);
+            M = warp_max(M);
+            float4 O[ND];
+#pragma unroll
+            for (int d = 0; d < ND; d++) O[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int i = 0; i < np; i++) {
+                const float* p = piece(i);
+                const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * row);
+                const float f = rl.x == -INFINITY ? 0.0f : ex2(rl.x - M);
+                L = __fmaf_rn(f, rl.y, L);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    if (128 * d + 4 * lane >= HDP) continue;
+                    const float4 x = *reinterpret_cast<const float4*>(p + row * HDP + 128 * d + 4 * lane);
+                    O[d] = make_float4(__fmaf_rn(f, x.x, O[d].x), __fmaf_rn(f, x.y, O[d].y), __fmaf_rn(f, x.z, O[d].z),
+                                       __fmaf_rn(f, x.w, O[d].w));
+                }
+            }
+            const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+            float* out = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const int e = 128 * d + 4 * lane;
+                if (e >= hd) continue;
+                out[e] = O[d].x * inv;
+                out[e + 1] = O[d].y * inv;
+                out[e + 2] = O[d].z * inv;
+                out[e + 3] = O[d].w * inv;
+            }
+        }
+    }
+}
+
+// SMs of the current device (0: no device).
+int sm_count() {
+    static std::atomic<int> sms[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+template <int HDP, int ROWS>
+size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
+    const size_t warps = (size_t)ctas * kPaWarps, at = align16(warps * sizeof(PaTail));
+    if (w) *w = PaWork{reinterpret_cast<long long*>(base), reinterpret_cast<PaTail*>(base + 16),
+                       reinterpret_cast<float*>(base + 16 + at)};
+    return 16 + at + warps * 2 * PaCfg<HDP, ROWS>::PART * sizeof(float);
+}
+
+template <int HDP, int ROWS>
+int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
+    using G = PaCfg<HDP, ROWS>;
+    // the attribute belongs to the device
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    JYC_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      G::SMEM));
+        if (dev < 64) ready[dev].store(true, std::memory_order_release);
+    }
+    const long long cap = (long long)a.kv.table_stride * a.kv.p.page_size, tiles = (cap + G::TK - 1) / G::TK;
+    const long long most = (long long)a.kv.num_seqs * pl.units_row;  // items; times tiles: units
+    const long long want = tiles >= (1LL << 31) / std::max(1LL, most) ? 1LL << 31 : most * tiles;
+    pl.tk = G::TK;
+    pl.ctas = (int)std::max(1LL, std::min((long long)sms * G::CTAS, (want + kPaWarps - 1) / kPaWarps));
+    PaWork w;
+    pa_work_bytes<HDP, ROWS>(sms * G::CTAS, static_cast<unsigned char*>(work), &w);
+    paged_attention_kernel<HDP, ROWS><<<pl.ctas, kPaWarps * 32, G::SMEM, s>>>(a, pl, w);
+    JYC_LAUNCHED();
+    if (tiles <= 1) return JYC_OK;  // an item is one unit: none is split
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pl.ctas);
+    cfg.blockDim = dim3(kPaJoinWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, ROWS>, a, pl, w));
+    JYC_LAUNCHED();
+    return JYC_OK;
 }
 
 bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
@@ -243,12 +842,40 @@ int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, cons
     return JYC_OK;
 }
 
-size_t paged_attention_workspace(int, int, int, int) { return 16; }
+// The instantiation of a shape: head size rounded up, and 16 query heads per
+// unit above 8 (up to 8, hi and lo weights share one product).
+#define PA_CASES(F, ...)                                                      \
+    do {                                                                      \
+        const bool many = H / KV > 8;                                         \
+        if (hd <= 64) return many ? F<64, 16>(__VA_ARGS__) : F<64, 8>(__VA_ARGS__);     \
+        if (hd <= 128) return many ? F<128, 16>(__VA_ARGS__) : F<128, 8>(__VA_ARGS__);  \
+        if (hd <= 192) return many ? F<192, 16>(__VA_ARGS__) : F<192, 8>(__VA_ARGS__);  \
+        return many ? F<256, 16>(__VA_ARGS__) : F<256, 8>(__VA_ARGS__);       \
+    } while (0)
 
-int launch_paged_attention(const PagedAttn& a, void*, cudaStream_t s) {
-    paged_attention_kernel<<<dim3(a.H, a.kv.num_seqs), kSimpleWarps * 32, 0, s>>>(a);
-    JYC_LAUNCHED();
-    return JYC_OK;
+template <int HDP, int ROWS>
+static size_t pa_workspace(int sms) {
+    return pa_work_bytes<HDP, ROWS>(sms * PaCfg<HDP, ROWS>::CTAS, nullptr, nullptr);
+}
+
+size_t paged_attention_workspace(int H, int KV, int hd) {
+    const int sms = sm_count();
+    if (sms == 0) {
+        cuda_fail(cudaErrorNoDevice, "paged attention: device query");
+        return 0;
+    }
+    PA_CASES(pa_workspace, sms);
+}
+
+int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
+    const int H = a.H, KV = a.KV, hd = a.hd, sms = sm_count();
+    PaPlan pl{};
+    pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
+    pl.units_row = KV * pl.qblocks;
+    const jyc_kv_pages& p = a.kv.p;
+    pl.wide_copy = hd % 16 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
+                   ((p.page_stride | p.pos_stride | p.head_stride) & 15) == 0;
+    PA_CASES(pa_launch, a, pl, sms, work, s);
 }
 
 }  // namespace jyc

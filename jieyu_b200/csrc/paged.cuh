@@ -44,7 +44,7 @@ struct PagedAttn {
     PagedRope rope;
     float scale;  // 1/sqrtf(hd)
 };
-size_t paged_attention_workspace(int seqs, int H, int KV, int hd);
+size_t paged_attention_workspace(int H, int KV, int hd);
 int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s);
 
 struct PickArgs {
