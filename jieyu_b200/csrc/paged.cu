@@ -162,6 +162,7 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
 
 constexpr int kPaWarps = 4;
 constexpr float kPaShift = 13.0f;
+constexpr float kPaLow = -1.7e38f;  // reference before any key: below every score, and its differences stay finite
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -173,6 +174,19 @@ __device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], uint32_t b0, u
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the same from a constant: c = v + a b
+__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int v, int (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(v));
+}
+__device__ __forceinline__ void pa_mma_f16_0(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float (&c)[4]) {
     asm volatile(
@@ -218,13 +232,19 @@ template <int HDP, int ROWS>
 struct PaCfg {
     static constexpr int TK = HDP <= 128 ? 32 : 16;   // keys of a unit
     static constexpr int ST = HDP <= 64 ? 3 : HDP <= 128 ? 2 : 3;
-    static constexpr int PITCH = HDP + 16;            // odd in 16-byte chunks: ldmatrix rows in distinct banks
-    static constexpr int VOFF = TK * PITCH, SOFF = 2 * TK * PITCH;
-    static constexpr int STAGE = SOFF + 8 * TK + 16;  // K, V, ks, vs, valid mask
+    static constexpr int VOFF = TK * HDP, SOFF = 2 * TK * HDP, MOFF = SOFF + 8 * TK;
+    static constexpr int STAGE = MOFF + 16;           // K, V, ks, vs, valid mask
     static constexpr int CTAS = HDP <= 128 ? 3 : 2;   // resident per SM
     static constexpr int PART = ROWS * (HDP + 2);     // floats of a partial: o, then (ref, l) per row
-    static constexpr int RING = ST * STAGE > PART * 4 ? ST * STAGE : (PART * 4 + 15) / 16 * 16;
+    static constexpr int FOFF = ST * STAGE;           // the current unit's keys, a float4 each
+    static constexpr int RING = FOFF + 16 * TK;
     static constexpr int SMEM = kPaWarps * RING;
+    static_assert(PART * 4 <= RING, "a partial fits the ring");
+    // byte of 16-byte chunk c of row r: chunks are swapped inside groups of 8 (of 4 where a row is no
+    // multiple of 128 bytes) so that the 8 rows of an ldmatrix tile lie in distinct banks
+    static __device__ __forceinline__ int at(int r, int c) {
+        return r * HDP + 16 * (HDP % 128 == 0 ? c ^ (r & 7) : c ^ ((r >> 1) & 3));
+    }
 };
 
 // What the kernels share about the line of units.
@@ -234,6 +254,8 @@ struct PaPlan {
     int tk;
     int ctas;       // of the main kernel
     bool wide_copy; // 16-byte copies
+    uint32_t div_m; // pos / page_size = pos * div_m >> div_s, for pos < 2^31
+    int div_s;
 };
 // Item that a warp's run starts and another one ends.
 struct PaTail {
@@ -289,10 +311,10 @@ template <int HDP, int ROWS>
 __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work) {
     using G = PaCfg<HDP, ROWS>;
-    constexpr int TK = G::TK, ST = G::ST, PITCH = G::PITCH;
+    constexpr int TK = G::TK, ST = G::ST;
     constexpr int NK = HDP / 32, NJ = TK / 8, NC = HDP / 32, E = ROWS / 8;  // E: rows a lane holds
     extern __shared__ __align__(128) unsigned char pa_sm[];
-    __shared__ long long s_scan[kPaWarps * 32 + 1];
+    __shared__ long long s_scan[kPaWarps];
     __shared__ PaCursor s_cur[kPaWarps];
     __shared__ long long s_first[kPaWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -373,9 +395,9 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         ok = false;
         if (issued < count) {
             const int pos = nx.t * TK + lane;
-            h = nx.r / pl.qblocks;
+            h = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
             if (lane < TK && pos < nx.len) {
-                const int idx = pos / a.kv.p.page_size;
+                const int idx = (int)(((unsigned long long)pos * pl.div_m) >> pl.div_s);
                 slot = pos - idx * a.kv.p.page_size;
                 pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
                 ok = true;
@@ -384,8 +406,12 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         }
         issued++;
     };
+    constexpr int LPR = HDP <= 64 ? 4 : HDP <= 128 ? 8 : 16, RPI = 32 / LPR;  // lanes per row, rows per step
+    const int cc = (lane & (LPR - 1)) * 16, cr = lane / LPR;
+    const int8_t* const kcol = a.kv.p.k + cc;
+    const int8_t* const vcol = a.kv.p.v + cc;
     auto issue = [&](int st) {  // copies of the unit that was looked up last
-        if (ok && (pg < 0 || pg >= a.kv.p.num_pages)) {
+        if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
             paged_flag(kPagedErrPage);
             ok = false;
         }
@@ -398,28 +424,27 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
             pa_copy<4>(base + G::SOFF + 4 * lane, a.kv.p.ks + so);
             pa_copy<4>(base + G::SOFF + 4 * TK + 4 * lane, a.kv.p.vs + so);
         }
-        if (lane == 0) *reinterpret_cast<unsigned*>(ring + st * G::STAGE + G::SOFF + 8 * TK) = mask;
-        if (mask != 0u) {
-            if (pl.wide_copy) {
-                constexpr int LPR = HDP <= 64 ? 4 : HDP <= 128 ? 8 : 16, RPI = 32 / LPR;  // lanes per row, rows per step
-                const int c = lane & (LPR - 1);
+        if (lane == 0) *reinterpret_cast<unsigned*>(ring + st * G::STAGE + G::MOFF) = mask;
+        if (pl.wide_copy) {
+            const bool all = mask == (TK == 32 ? ~0u : (1u << (TK & 31)) - 1u);
 #pragma unroll
-                for (int i = 0; i < TK / RPI; i++) {
-                    const int row = i * RPI + lane / LPR;
-                    const long long o = __shfl_sync(0xffffffffu, off, row);
-                    if (((mask >> row) & 1) && c * 16 < hd) {
-                        pa_copy<16>(base + row * PITCH + c * 16, a.kv.p.k + o + c * 16);
-                        pa_copy<16>(base + G::VOFF + row * PITCH + c * 16, a.kv.p.v + o + c * 16);
-                    }
+            for (int i = 0; i < TK / RPI; i++) {
+                const int row = i * RPI + cr;
+                const long long o = __shfl_sync(0xffffffffu, off, row);
+                if (cc < hd && (all || ((mask >> row) & 1))) {
+                    const uint32_t dst = base + G::at(row, cc / 16);
+                    pa_copy<16>(dst, kcol + o);
+                    pa_copy<16>(dst + G::VOFF, vcol + o);
                 }
-            } else {
-                for (int row = 0; row < TK; row++) {
-                    const long long o = __shfl_sync(0xffffffffu, off, row);
-                    if (!((mask >> row) & 1)) continue;
-                    for (int c = lane; c * 4 < hd; c += 32) {
-                        pa_copy<4>(base + row * PITCH + c * 4, a.kv.p.k + o + c * 4);
-                        pa_copy<4>(base + G::VOFF + row * PITCH + c * 4, a.kv.p.v + o + c * 4);
-                    }
+            }
+        } else {
+            for (int row = 0; row < TK; row++) {
+                const long long o = __shfl_sync(0xffffffffu, off, row);
+                if (!((mask >> row) & 1)) continue;
+                for (int c = lane; c * 4 < hd; c += 32) {
+                    const uint32_t dst = base + G::at(row, c / 4) + (c & 3) * 4;
+                    pa_copy<4>(dst, a.kv.p.k + o + c * 4);
+                    pa_copy<4>(dst + G::VOFF, a.kv.p.v + o + c * 4);
                 }
             }
         }
@@ -472,7 +497,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
                 qsl[e] = __fmul_rn(q8_scale(amax), up);
 #pragma unroll
                 for (int i = 0; i < 2 * NK; i++) qa[i >> 1][e + 2 * (i & 1)] = pack4(x[i], inv);
-                ref[e] = -INFINITY;
+                ref[e] = kPaLow;
                 l[e] = 0.0f;
 #pragma unroll
                 for (int d = 0; d < HDP / 16; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
@@ -489,35 +514,46 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         __syncwarp();
         const unsigned char* sb = ring + st * G::STAGE;
         const uint32_t base = ring_a + st * G::STAGE;
-        const unsigned mask = *reinterpret_cast<const unsigned*>(sb + G::SOFF + 8 * TK);
-        const float* sks = reinterpret_cast<const float*>(sb + G::SOFF);
-        const float* svs = sks + TK;
+        // lane j: key j's {ks, 0 or -inf, e, vs}; a key that does not count has a score of -inf and vs = 0.
+        // e is kept within 2^-64..2^126: the quantiser's scales are 0 or above 2^-34
+        float4* keys = reinterpret_cast<float4*>(ring + G::FOFF);
+        if (lane < TK) {
+            const bool in = (*reinterpret_cast<const unsigned*>(sb + G::MOFF) >> lane) & 1;
+            const float* sc = reinterpret_cast<const float*>(sb + G::SOFF);
+            const float v = in ? sc[TK + lane] : 0.0f;
+            const int ex = min(max((int)((__float_as_uint(v) >> 23) & 255u), 63), 253) - 127;
+            keys[lane] = in ? make_float4(sc[lane], 0.0f, (float)ex, v) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        }
+        __syncwarp();
 
-        // scores of keys 8 j + 2 t, + 1 for rows g (and g + 8), in base 2
-        float s[NJ][E][2];
+        // scores of keys 8 j + 2 t, + 1 for rows g (and g + 8), in base 2; the dots start at the bits of
+        // 1.5 * 2^23 (|dot| <= 256 * 127^2 < 2^22), so an exact subtraction makes them floats
+        float s[NJ][E][2], vs[NJ][2];
         float top[E];
 #pragma unroll
         for (int e = 0; e < E; e++) top[e] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            int c[4] = {0, 0, 0, 0};
+            int c[4];
 #pragma unroll
             for (int k = 0; k < NK; k += 2) {
                 uint32_t b[4];
-                pa_ldsm(base + (8 * j + (lane & 7)) * PITCH + (2 * k + (lane >> 3)) * 16, b);
-                pa_mma_s8(qa[k], b[0], b[1], c);
-                if (k + 1 < NK) pa_mma_s8(qa[k + 1], b[2], b[3], c);
+                pa_ldsm(base + G::at(8 * j + (lane & 7), 2 * k + (lane >> 3)), b);
+                if (k == 0)
+                    pa_mma_s8(qa[k], b[0], b[1], 0x4B400000, c);
+                else
+                    pa_mma_s8(qa[k], b[0], b[1], c);
+                pa_mma_s8(qa[k + 1], b[2], b[3], c);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int key = 8 * j + 2 * t + i;
-                const float kf = sks[key];
-                const int ex = min(max((int)((__float_as_uint(svs[key]) >> 23) & 255u), 63), 253) - 127;
+                const float4 key = keys[8 * j + 2 * t + i];
+                vs[j][i] = key.w;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float v = (mask >> key) & 1 ? __fmul_rn((float)c[2 * e + i], __fmul_rn(kf, qsl[e])) : -INFINITY;
-                    s[j][e][i] = v;
-                    top[e] = fmaxf(top[e], v + (float)ex);
+                    const float dot = __fsub_rn(__int_as_float(c[2 * e + i]), 12582912.0f);
+                    s[j][e][i] = __fmaf_rn(dot, __fmul_rn(key.x, qsl[e]), key.y);
+                    top[e] = fmaxf(top[e], s[j][e][i] + key.z);
                 }
             }
         }
@@ -527,7 +563,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
             const float nr = fmaxf(ref[e], top[e] - kPaShift);
-            al[e] = ref[e] == -INFINITY ? 0.0f : ex2(ref[e] - nr);
+            al[e] = ex2(ref[e] - nr);
             ref[e] = nr;
             l[e] *= al[e];
         }
@@ -535,13 +571,11 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         uint32_t hi[TK / 16][4], lo[E == 1 ? 1 : TK / 16][4];
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const float v0 = svs[8 * j + 2 * t], v1 = svs[8 * j + 2 * t + 1];
-            const bool m0 = (mask >> (8 * j + 2 * t)) & 1, m1 = (mask >> (8 * j + 2 * t + 1)) & 1;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const float b0 = m0 ? ex2(s[j][e][0] - ref[e]) : 0.0f, b1 = m1 ? ex2(s[j][e][1] - ref[e]) : 0.0f;
+                const float b0 = ex2(s[j][e][0] - ref[e]), b1 = ex2(s[j][e][1] - ref[e]);
                 l[e] += b0 + b1;
-                const float w0 = m0 ? b0 * v0 : 0.0f, w1 = m1 ? b1 * v1 : 0.0f;
+                const float w0 = b0 * vs[j][0], w1 = b1 * vs[j][1];
                 const uint32_t ph = pa_pack(w0, w1);
                 const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
                 const uint32_t pl2 = pa_pack(w0 - hf.x, w1 - hf.y);
@@ -561,19 +595,22 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         for (int d = 0; d < NC; d++) {
             float c[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
-#pragma unroll
             for (int k = 0; k < TK / 16; k++) {
                 uint32_t v[4];
-                pa_ldsm_t(base + G::VOFF + (16 * k + (lane & 15)) * PITCH + (2 * d + (lane >> 4)) * 16, v);
+                pa_ldsm_t(base + G::VOFF + G::at(16 * k + (lane & 15), 2 * d + (lane >> 4)), v);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const uint32_t e0 = pa_half2<false>(v[2 * i]), e1 = pa_half2<false>(v[2 * i + 1]);
                     const uint32_t o0 = pa_half2<true>(v[2 * i]), o1 = pa_half2<true>(v[2 * i + 1]);
-                    pa_mma_f16(hi[k], e0, e1, c[2 * i]);
-                    pa_mma_f16(hi[k], o0, o1, c[2 * i + 1]);
+                    if (k == 0) {
+                        pa_mma_f16_0(hi[k], e0, e1, c[2 * i]);
+                        pa_mma_f16_0(hi[k], o0, o1, c[2 * i + 1]);
+                    } else {
+                        pa_mma_f16(hi[k], e0, e1, c[2 * i]);
+                        pa_mma_f16(hi[k], o0, o1, c[2 * i + 1]);
+                    }
                     if (E == 2) {
                         pa_mma_f16(lo[E == 1 ? 0 : k], e0, e1, c[2 * i]);
                         pa_mma_f16(lo[E == 1 ? 0 : k], o0, o1, c[2 * i + 1]);
@@ -658,7 +695,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
                     make_float4(o[d][e][0], o[d][e][1], o[d][e][2], o[d][e][3]);
         if (t == 0)
             *reinterpret_cast<float2*>(buf + ROWS * HDP + 2 * row) =
-                count > 0 ? make_float2(ref[e], l[e]) : make_float2(-INFINITY, 0.0f);
+                count > 0 ? make_float2(ref[e], l[e]) : make_float2(kPaLow, 0.0f);
     }
     __syncthreads();
     const PaCursor c = s_cur[0];
@@ -666,15 +703,15 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
     float* part = work.part + ((size_t)blockIdx.x * kPaWarps * 2 + (c0 == s_first[0] ? 1 : 0)) * G::PART;
     for (int i = tid; i < ROWS * HDP / 4; i += kPaWarps * 32) {
         const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
-        float M = -INFINITY, L = 0.0f;
+        float M = kPaLow, L = 0.0f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = 0; w < kPaWarps; w++)
             M = fmaxf(M, reinterpret_cast<const float*>(pa_sm + w * G::RING)[ROWS * HDP + 2 * row]);
         for (int w = 0; w < kPaWarps; w++) {
             const float* wb = reinterpret_cast<const float*>(pa_sm + w * G::RING);
             const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
-            if (wr == -INFINITY && wl == 0.0f) continue;
-            const float f = wr == -INFINITY ? 0.0f : ex2(wr - M);
+            if (wl == 0.0f) continue;  // no key (a warp without units left no o)
+            const float f = ex2(wr - M);
             const float4 x = *reinterpret_cast<const float4*>(wb + row * HDP + d);
             L = __fmaf_rn(f, wl, L);
             O = make_float4(__fmaf_rn(f, x.x, O.x), __fmaf_rn(f, x.y, O.y), __fmaf_rn(f, x.z, O.z), __fmaf_rn(f, x.w, O.w));
@@ -727,7 +764,7 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn
         };
         const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
         for (int row = warp; row < ROWS && qb * ROWS + row < group; row += kPaJoinWarps) {
-            float M = -INFINITY, L = 0.0f;
+            float M = kPaLow, L = 0.0f;
             for (int i = lane; i < np; i += 32) M = fmaxf(M, piece(i)[ROWS * HDP + 2 * row]);
             M = warp_max(M);
             float4 O[ND];
@@ -737,7 +774,7 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn
             for (int i = 0; i < np; i++) {
                 const float* p = piece(i);
                 const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * row);
-                const float f = rl.x == -INFINITY ? 0.0f : ex2(rl.x - M);
+                const float f = ex2(rl.x - M);
                 L = __fmaf_rn(f, rl.y, L);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
@@ -872,6 +909,12 @@ int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
     PaPlan pl{};
     pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
     pl.units_row = KV * pl.qblocks;
+    // n / d for n < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) < d <= 2^s, so the
+    // error of n m / 2^(31+s) is below 2^-31 n < 1 / d at every n; m < 2^32
+    int sh = 0;
+    while ((1LL << sh) < a.kv.p.page_size) sh++;
+    pl.div_s = 31 + sh;
+    pl.div_m = (uint32_t)(((1ULL << pl.div_s) + a.kv.p.page_size - 1) / a.kv.p.page_size);
     const jyc_kv_pages& p = a.kv.p;
     pl.wide_copy = hd % 16 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
                    ((p.page_stride | p.pos_stride | p.head_stride) & 15) == 0;
