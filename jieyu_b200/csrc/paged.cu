@@ -148,19 +148,19 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
 // is a line of units (a unit: TK keys of one kv head of one sequence, 16-byte
 // cp.async rows), cut into equal runs for all resident warps whatever the
 // lengths; a warp keeps its next units in flight in its own ring in shared
-// memory across the borders of sequences and has no barrier in its loop. The
-// (up to 8 or 16) query heads of a kv head are the rows of one m16 tile:
-// q.k with mma.m16n8k32 s8 (exact dots), P.V with mma.m16n8k16 f16 (V is exact
-// in fp16). Up to 8 heads, the hi halves are rows 0-7 and the lo halves rows
-// 8-15 of the same product. Each unit's product starts from zero and is added
-// in fp32 with round to nearest (the tensor cores' own sums may truncate).
+// memory across the borders of sequences and has no barrier in its loop.
+// Keys are the rows of both products and the (up to 8 or 16) query heads of a
+// kv head the columns, so nothing of a tile is padding at 8 heads: S^T = K Q^T
+// with mma.m16n8k32 s8 (exact dots), O^T = V^T P^T with mma.m16n8k16 f16 (V is
+// exact in fp16), the weights transposed between them by movmatrix. Each
+// unit's product starts from zero and is added in fp32 with round to nearest
+// (the tensor cores' own sums may truncate).
 //
 // A run that covers an item (a kv head of a sequence) whole writes its rows of
 // out; the others leave (o, ref, l) in the workspace and a second kernel,
 // launched early, joins them. The warps of a CTA inside one item are joined in
 // shared memory first.
 
-constexpr int kPaWarps = 4;
 constexpr float kPaShift = 13.0f;
 constexpr float kPaLow = -1.7e38f;  // reference before any key: below every score, and its differences stay finite
 
@@ -169,30 +169,32 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int (&c)[4]) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// the same from a constant: c = v + a b
-__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int v, int (&c)[4]) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+// c = v + a b for a constant v, and c += a b
+__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int v, int (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(v));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(v));
 }
-__device__ __forceinline__ void pa_mma_f16_0(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float (&c)[4]) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[2], float v, float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(v));
 }
-__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float (&c)[4]) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[2], float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// 8 x 8 halves, lane (g, t) holding (g, 2 t) and (g, 2 t + 1), transposed
+__device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -227,18 +229,20 @@ __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
 
 // Sizes of one instantiation: HDP is the head size rounded up (the columns
 // behind it hold whatever the ring held, finite as integers; they meet zero
-// query columns and unread output columns), ROWS the query heads of a unit.
-template <int HDP, int ROWS>
+// query columns and unread output columns), E the blocks of 8 query heads of a
+// unit.
+template <int HDP, int E>
 struct PaCfg {
-    static constexpr int TK = HDP <= 128 ? 32 : 16;   // keys of a unit
-    static constexpr int ST = HDP <= 64 ? 3 : HDP <= 128 ? 2 : 3;
+    static constexpr int TK = HDP <= 128 ? 32 : 16;      // keys of a unit
+    static constexpr int WARPS = HDP <= 128 ? 12 : 8;    // one CTA per SM
+    static constexpr int ST = HDP <= 64 ? 4 : HDP <= 128 ? 2 : 3;
+    static constexpr int ROWS = 8 * E;
     static constexpr int VOFF = TK * HDP, SOFF = 2 * TK * HDP, MOFF = SOFF + 8 * TK;
-    static constexpr int STAGE = MOFF + 16;           // K, V, ks, vs, valid mask
-    static constexpr int CTAS = HDP <= 128 ? 3 : 2;   // resident per SM
-    static constexpr int PART = ROWS * (HDP + 2);     // floats of a partial: o, then (ref, l) per row
-    static constexpr int FOFF = ST * STAGE;           // the current unit's keys, a float4 each
+    static constexpr int STAGE = MOFF + 16;              // K, V, ks, vs, valid mask
+    static constexpr int PART = ROWS * (HDP + 2);        // floats of a partial: o, then (ref, l) per row
+    static constexpr int FOFF = ST * STAGE;              // the current unit's keys, a float4 each
     static constexpr int RING = FOFF + 16 * TK;
-    static constexpr int SMEM = kPaWarps * RING;
+    static constexpr int SMEM = WARPS * RING;
     static_assert(PART * 4 <= RING, "a partial fits the ring");
     // byte of 16-byte chunk c of row r: chunks are swapped inside groups of 8 (of 4 where a row is no
     // multiple of 128 bytes) so that the 8 rows of an ldmatrix tile lie in distinct banks
@@ -251,21 +255,33 @@ struct PaCfg {
 struct PaPlan {
     int units_row;  // kv heads * query blocks
     int qblocks;    // blocks of ROWS query heads per kv head
-    int tk;
-    int ctas;       // of the main kernel
+    int tk, warps;  // keys of a unit, warps of a CTA
     bool wide_copy; // 16-byte copies
     uint32_t div_m; // pos / page_size = pos * div_m >> div_s, for pos < 2^31
     int div_s;
 };
-// Item that a warp's run starts and another one ends.
+// The line cut into runs: worker w starts at w * base + min(w, rest).
+struct PaLine {
+    long long base, rest, workers;
+    int per_cta;  // workers of a CTA
+    __device__ __forceinline__ long long start(long long w) const {
+        w = min(w, workers);
+        return w * base + min(w, rest);
+    }
+    __device__ __forceinline__ long long worker(long long u) const {  // whose run holds unit u
+        const long long big = rest * (base + 1);
+        return u < big ? u / (base + 1) : rest + (u - big) / base;
+    }
+};
+// Item that a worker's run starts and another one ends.
 struct PaTail {
     long long u0, u1;  // units of the item; u1 == 0: none
     int b, r;
 };
 struct PaWork {
-    long long* total;  // units of the call
-    PaTail* tail;      // [warps]
-    float* part;       // [warps][2][PART]: an item's later part (0), its first (1)
+    PaLine* line;
+    PaTail* tail;      // [workers]
+    float* part;       // [workers][2][PART]: an item's later part (0), its first (1)
 };
 
 __device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
@@ -282,12 +298,17 @@ __device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
     }
     return len;
 }
-// Warps that get units, and where the run of warp w starts.
-__device__ __forceinline__ long long pa_workers(long long U, int ctas) {
-    return min((long long)ctas * kPaWarps, U);
-}
-__device__ __forceinline__ long long pa_start(long long U, long long workers, long long w) {
-    return w >= workers ? U : U * w / workers;
+// Runs of U units: as many workers as there are warps, or units; a few per CTA
+// at least, whose parts are joined in shared memory.
+constexpr int kPaFewWarps = 4;
+__device__ __forceinline__ PaLine pa_line(long long U, int ctas, int warps) {
+    PaLine l;
+    const long long each = (U + ctas - 1) / ctas;
+    l.per_cta = (int)min((long long)warps, max((long long)kPaFewWarps, each));
+    l.workers = min((long long)ctas * l.per_cta, U);
+    l.base = l.workers ? U / l.workers : 0;
+    l.rest = l.workers ? U % l.workers : 0;
+    return l;
 }
 
 struct PaCursor {
@@ -307,23 +328,22 @@ __device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, Pa
     pa_seek(a, pl.tk, c);
 }
 
-template <int HDP, int ROWS>
-__global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
+template <int HDP, int E>
+__global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, ROWS>;
-    constexpr int TK = G::TK, ST = G::ST;
-    constexpr int NK = HDP / 32, NJ = TK / 8, NC = HDP / 32, E = ROWS / 8;  // E: rows a lane holds
+    using G = PaCfg<HDP, E>;
+    constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS;
+    constexpr int NK = HDP / 32, NM = TK / 16, ND = HDP / 16;
     extern __shared__ __align__(128) unsigned char pa_sm[];
-    __shared__ long long s_scan[kPaWarps];
-    __shared__ PaCursor s_cur[kPaWarps];
-    __shared__ long long s_first[kPaWarps];
+    __shared__ long long s_scan[WARPS];
+    __shared__ PaCursor s_cur[WARPS];
+    __shared__ long long s_first[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int wid = blockIdx.x * kPaWarps + warp;
     const int B = a.kv.num_seqs, group = a.H / a.KV, hd = a.hd;
     griddep_launch();
 
     // where the units of each sequence lie in the line
-    const int per = (B + kPaWarps * 32 - 1) / (kPaWarps * 32);
+    const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
     const int bs = min(B, tid * per), be = min(B, bs + per);
     long long mine = 0;
     for (int b = bs; b < be; b++) mine += (pa_len(a, b) + TK - 1) / TK;
@@ -337,14 +357,15 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
     long long U = 0, ex = incl - mine;
-    for (int w = 0; w < kPaWarps; w++) {
+    for (int w = 0; w < WARPS; w++) {
         if (w < warp) ex += s_scan[w];
         U += s_scan[w];
     }
-    const long long workers = pa_workers(U, gridDim.x);
-    if (blockIdx.x == 0 && tid == 0) *work.total = U;
-    for (int w = 0; w < kPaWarps; w++) {
-        const long long u = pa_start(U, workers, (long long)blockIdx.x * kPaWarps + w);
+    const PaLine line = pa_line(U, gridDim.x, WARPS);
+    if (blockIdx.x == 0 && tid == 0) *work.line = line;
+    const long long w0 = (long long)blockIdx.x * line.per_cta;
+    for (int w = 0; w < line.per_cta; w++) {
+        const long long u = line.start(w0 + w);
         if (u < ex || u >= ex + mine) continue;
         long long at = ex;
         for (int b = bs; b < be; b++) {
@@ -362,13 +383,13 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
     // sequences without a key: rows of zeros
     for (int b = blockIdx.x; b < B; b += gridDim.x)
         if (pa_len(a, b) == 0)
-            for (int e = tid; e < a.H * hd; e += kPaWarps * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
+            for (int e = tid; e < a.H * hd; e += WARPS * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
     __syncthreads();
 
-    const long long u0 = pa_start(U, workers, wid), u1 = pa_start(U, workers, wid + 1);
-    const long long c0 = pa_start(U, workers, (long long)blockIdx.x * kPaWarps);
-    const long long c1 = pa_start(U, workers, (long long)(blockIdx.x + 1) * kPaWarps);
-    const int count = (int)(u1 - u0);
+    const bool worker = warp < line.per_cta;
+    const long long u0 = line.start(w0 + warp), u1 = line.start(w0 + warp + 1);
+    const long long c0 = line.start(w0), c1 = line.start(w0 + line.per_cta);
+    const int count = worker ? (int)(u1 - u0) : 0;
     unsigned char* ring = pa_sm + warp * G::RING;
     const uint32_t ring_a = smem_u32(ring);
     PaCursor cur = PaCursor{0, 0, 0, 0, 0};
@@ -377,25 +398,30 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         cur = s_cur[warp];
         item0 = s_first[warp];
     }
-    // every warp of the CTA inside one item: joined below
+    // every worker of the CTA inside one item: joined below
     bool joint = false, whole = false;  // whole: and they are all of it
     if (c1 > c0) {
         const long long first = s_first[0], end = first + s_cur[0].nt;
         joint = c1 <= end;
         whole = c0 == first && c1 == end;
     }
-    if (lane == 0) work.tail[wid].u1 = 0;
+    if (worker && lane == 0) work.tail[w0 + warp].u1 = 0;
 
     // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
     PaCursor nx = cur;
     int issued = 0;  // units whose pages are looked up
-    int pg = -1, slot = 0, h = 0;
+    int pg = -1, slot = 0, h = -1;
+    long long hoff = 0, hsoff = 0;  // of kv head h
     bool ok = false;
     auto lookup = [&] {
         ok = false;
         if (issued < count) {
-            const int pos = nx.t * TK + lane;
-            h = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
+            const int pos = nx.t * TK + lane, hn = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
+            if (hn != h) {
+                h = hn;
+                hoff = (long long)h * a.kv.p.head_stride;
+                hsoff = (long long)h * a.kv.p.shead_stride;
+            }
             if (lane < TK && pos < nx.len) {
                 const int idx = (int)(((unsigned long long)pos * pl.div_m) >> pl.div_s);
                 slot = pos - idx * a.kv.p.page_size;
@@ -419,8 +445,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
         long long off = 0;
         if (ok) {
-            off = (long long)paged_off(a.kv, pg, slot, h);
-            const size_t so = paged_soff(a.kv, pg, slot, h);
+            off = (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff;
+            const long long so = (long long)pg * a.kv.p.spage_stride + (long long)slot * a.kv.p.spos_stride + hsoff;
             pa_copy<4>(base + G::SOFF + 4 * lane, a.kv.p.ks + so);
             pa_copy<4>(base + G::SOFF + 4 * TK + 4 * lane, a.kv.p.vs + so);
         }
@@ -457,16 +483,18 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         lookup();
     }
 
-    uint32_t qa[NK][4];
-    float qsl[E], ref[E], l[E], o[HDP / 16][E][4];
+    // lane (g, t): query head g (and g + 8) as B fragments, bytes 4 t .. 4 t + 3 of every 16; of the results the
+    // heads 2 t, 2 t + 1 (and 8 more), for which it keeps the reference, its share of the sum, and the dims 2 g,
+    // 2 g + 1 of every 16
+    uint32_t qf[NK][E][2];
+    float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4];
     bool fresh = true;
     int st = 0;
     const float up = __fmul_rn(a.scale, 1.44269504088896341f);
 
     for (int n = 0; n < count; n++) {
         if (fresh) {
-            // the item's query heads: rotated, quantised per head, straight into the A fragments; lane (g, t)
-            // holds bytes 4t..4t+3 of every 16 of rows g and g + 8
+            // the item's query heads: rotated and quantised per head
             fresh = false;
             const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
             const int half = hd >> 1;
@@ -493,18 +521,18 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
                 }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const float inv = q8_inv(amax);
-                qsl[e] = __fmul_rn(q8_scale(amax), up);
+                const float inv = q8_inv(amax), sc = __fmul_rn(q8_scale(amax), up);
 #pragma unroll
-                for (int i = 0; i < 2 * NK; i++) qa[i >> 1][e + 2 * (i & 1)] = pack4(x[i], inv);
-                ref[e] = kPaLow;
-                l[e] = 0.0f;
+                for (int i = 0; i < 2 * NK; i++) qf[i >> 1][e][i & 1] = pack4(x[i], inv);
 #pragma unroll
-                for (int d = 0; d < HDP / 16; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
+                for (int i = 0; i < 2; i++) {
+                    qsl[e][i] = __shfl_sync(0xffffffffu, sc, 4 * (2 * t + i));
+                    ref[e][i] = kPaLow;
+                    l[e][i] = 0.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
             }
-            if (E == 1)
-#pragma unroll
-                for (int i = 0; i < NK; i++) qa[i][1] = qa[i][3] = 0u;
         }
         // the next unit's copies go to the stage that the last iteration read
         __syncwarp();
@@ -526,111 +554,105 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         }
         __syncwarp();
 
-        // scores of keys 8 j + 2 t, + 1 for rows g (and g + 8), in base 2; the dots start at the bits of
+        // scores of keys 16 m + g, + 8 and heads 2 t, + 1, in base 2; the dots start at the bits of
         // 1.5 * 2^23 (|dot| <= 256 * 127^2 < 2^22), so an exact subtraction makes them floats
-        float s[NJ][E][2], vs[NJ][2];
-        float top[E];
+        float s[NM][E][4], vs[NM][2];
+        float top[E][2];
 #pragma unroll
-        for (int e = 0; e < E; e++) top[e] = -INFINITY;
+        for (int e = 0; e < E; e++) top[e][0] = top[e][1] = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            int c[4];
+        for (int m = 0; m < NM; m++) {
+            int c[E][4];
 #pragma unroll
-            for (int k = 0; k < NK; k += 2) {
-                uint32_t b[4];
-                pa_ldsm(base + G::at(8 * j + (lane & 7), 2 * k + (lane >> 3)), b);
-                if (k == 0)
-                    pa_mma_s8(qa[k], b[0], b[1], 0x4B400000, c);
-                else
-                    pa_mma_s8(qa[k], b[0], b[1], c);
-                pa_mma_s8(qa[k + 1], b[2], b[3], c);
+            for (int k = 0; k < NK; k++) {
+                uint32_t kf[4];
+                pa_ldsm(base + G::at(16 * m + (lane & 15), 2 * k + (lane >> 4)), kf);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if (k == 0)
+                        pa_mma_s8(kf, qf[k][e], 0x4B400000, c[e]);
+                    else
+                        pa_mma_s8(kf, qf[k][e], c[e]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float4 key = keys[8 * j + 2 * t + i];
-                vs[j][i] = key.w;
+                const float4 key = keys[16 * m + 8 * i + g];
+                vs[m][i] = key.w;
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const float dot = __fsub_rn(__int_as_float(c[2 * e + i]), 12582912.0f);
-                    s[j][e][i] = __fmaf_rn(dot, __fmul_rn(key.x, qsl[e]), key.y);
-                    top[e] = fmaxf(top[e], s[j][e][i] + key.z);
-                }
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float dot = __fsub_rn(__int_as_float(c[e][2 * i + j]), 12582912.0f);
+                        const float v = __fmaf_rn(dot, __fmul_rn(key.x, qsl[e][j]), key.y);
+                        s[m][e][2 * i + j] = v;
+                        top[e][j] = fmaxf(top[e][j], v + key.z);
+                    }
             }
         }
-        float al[E];
+        float al[E][2];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-            const float nr = fmaxf(ref[e], top[e] - kPaShift);
-            al[e] = ex2(ref[e] - nr);
-            ref[e] = nr;
-            l[e] *= al[e];
-        }
-        // weights as A fragments: keys 16 k + 2 t, + 1 in a0 (a1), 8 later in a2 (a3)
-        uint32_t hi[TK / 16][4], lo[E == 1 ? 1 : TK / 16][4];
+        for (int e = 0; e < E; e++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float b0 = ex2(s[j][e][0] - ref[e]), b1 = ex2(s[j][e][1] - ref[e]);
-                l[e] += b0 + b1;
-                const float w0 = b0 * vs[j][0], w1 = b1 * vs[j][1];
-                const uint32_t ph = pa_pack(w0, w1);
-                const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
-                const uint32_t pl2 = pa_pack(w0 - hf.x, w1 - hf.y);
-                const int f = 2 * (j & 1);
-                if (E == 1) {
-                    hi[j >> 1][f] = ph;
-                    hi[j >> 1][f + 1] = pl2;
-                } else {
-                    hi[j >> 1][f + e] = ph;
-                    lo[E == 1 ? 0 : j >> 1][f + e] = pl2;
-                }
+            for (int j = 0; j < 2; j++) {
+                float x = top[e][j];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(ref[e][j], x - kPaShift);
+                al[e][j] = ex2(ref[e][j] - x);
+                ref[e][j] = x;
+                l[e][j] *= al[e][j];
             }
-        }
-        // P.V: 32 dims at a time; a transposed load gives each lane two neighbouring dims of two keys, so the
-        // even dims make one n8 tile and the odd ones another: lane t ends with dims 4 t .. 4 t + 3 of every 16
+        // weights, transposed into B fragments: head g, keys 16 m + 2 t, + 1 and 8 later
+        uint32_t hi[NM][E][2], lo[NM][E][2];
 #pragma unroll
-        for (int d = 0; d < NC; d++) {
-            float c[4][4];
+        for (int m = 0; m < NM; m++)
 #pragma unroll
-            for (int k = 0; k < TK / 16; k++) {
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float b0 = ex2(s[m][e][2 * i] - ref[e][0]), b1 = ex2(s[m][e][2 * i + 1] - ref[e][1]);
+                    l[e][0] += b0;
+                    l[e][1] += b1;
+                    const float w0 = b0 * vs[m][i], w1 = b1 * vs[m][i];
+                    const uint32_t ph = pa_pack(w0, w1);
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
+                    hi[m][e][i] = pa_transpose(ph);
+                    lo[m][e][i] = pa_transpose(pa_pack(w0 - hf.x, w1 - hf.y));
+                }
+        // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
+        // rows g of the tile, the odd ones rows g + 8
+#pragma unroll
+        for (int d = 0; d < ND; d += 2) {
+            float c[2][E][4];
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
                 uint32_t v[4];
-                pa_ldsm_t(base + G::VOFF + G::at(16 * k + (lane & 15), 2 * d + (lane >> 4)), v);
+                pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const uint32_t e0 = pa_half2<false>(v[2 * i]), e1 = pa_half2<false>(v[2 * i + 1]);
-                    const uint32_t o0 = pa_half2<true>(v[2 * i]), o1 = pa_half2<true>(v[2 * i + 1]);
-                    if (k == 0) {
-                        pa_mma_f16_0(hi[k], e0, e1, c[2 * i]);
-                        pa_mma_f16_0(hi[k], o0, o1, c[2 * i + 1]);
-                    } else {
-                        pa_mma_f16(hi[k], e0, e1, c[2 * i]);
-                        pa_mma_f16(hi[k], o0, o1, c[2 * i + 1]);
-                    }
-                    if (E == 2) {
-                        pa_mma_f16(lo[E == 1 ? 0 : k], e0, e1, c[2 * i]);
-                        pa_mma_f16(lo[E == 1 ? 0 : k], o0, o1, c[2 * i + 1]);
+                    const uint32_t vf[4] = {pa_half2<false>(v[2 * i]), pa_half2<true>(v[2 * i]),
+                                            pa_half2<false>(v[2 * i + 1]), pa_half2<true>(v[2 * i + 1])};
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        if (m == 0)
+                            pa_mma_f16(vf, hi[m][e], 0.0f, c[i][e]);
+                        else
+                            pa_mma_f16(vf, hi[m][e], c[i][e]);
+                        pa_mma_f16(vf, lo[m][e], c[i][e]);
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float* od = o[2 * d + (i >> 1)][0];
-                if (E == 1) {
-                    od[i & 1] = __fmaf_rn(od[i & 1], al[0], c[i][0] + c[i][2]);
-                    od[2 + (i & 1)] = __fmaf_rn(od[2 + (i & 1)], al[0], c[i][1] + c[i][3]);
-                } else {
-                    float* oe = o[2 * d + (i >> 1)][E - 1];
-                    od[i & 1] = __fmaf_rn(od[i & 1], al[0], c[i][0]);
-                    od[2 + (i & 1)] = __fmaf_rn(od[2 + (i & 1)], al[0], c[i][1]);
-                    oe[i & 1] = __fmaf_rn(oe[i & 1], al[E - 1], c[i][2]);
-                    oe[2 + (i & 1)] = __fmaf_rn(oe[2 + (i & 1)], al[E - 1], c[i][3]);
-                }
-            }
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
         }
         st = st == ST - 1 ? 0 : st + 1;
 
@@ -641,38 +663,46 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         }
         // the end of an item or of the run
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        }
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
         const bool from_start = item0 >= u0;
         if (from_start && item_end) {
             const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int row = qb * ROWS + 8 * e + g;
-                if (row >= group) continue;
-                float* out = a.out + (size_t)cur.b * a.ldo + (size_t)(kvh * group + row) * hd;
-                const float inv = l[e] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[e]);
+            for (int e = 0; e < E; e++)
 #pragma unroll
-                for (int d = 0; d < HDP / 16; d++)
-                    if (16 * d + 4 * t < hd)
+                for (int j = 0; j < 2; j++) {
+                    const int row = qb * ROWS + 8 * e + 2 * t + j;
+                    if (row >= group) continue;
+                    float* out = a.out + (size_t)cur.b * a.ldo + (size_t)(kvh * group + row) * hd;
+                    const float inv = l[e][j] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[e][j]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) out[16 * d + 4 * t + i] = o[d][e][i] * inv;
-            }
+                    for (int d = 0; d < ND; d++)
+                        if (16 * d + 2 * g < hd) {
+                            out[16 * d + 2 * g] = o[d][e][j] * inv;
+                            out[16 * d + 2 * g + 1] = o[d][e][2 + j] * inv;
+                        }
+                }
         } else {
-            if (from_start && lane == 0 && !whole) work.tail[wid] = PaTail{item0, item0 + cur.nt, cur.b, cur.r};
+            if (from_start && lane == 0 && !whole)
+                work.tail[w0 + warp] = PaTail{item0, item0 + cur.nt, cur.b, cur.r};
             if (joint) break;  // o, ref and l stay in registers
-            float* part = work.part + ((size_t)wid * 2 + (from_start ? 1 : 0)) * G::PART;
+            float* part = work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int row = 8 * e + g;
+            for (int e = 0; e < E; e++)
 #pragma unroll
-                for (int d = 0; d < HDP / 16; d++)
-                    *reinterpret_cast<float4*>(part + row * HDP + 16 * d + 4 * t) =
-                        make_float4(o[d][e][0], o[d][e][1], o[d][e][2], o[d][e][3]);
-                if (t == 0) *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(ref[e], l[e]);
-            }
+                for (int j = 0; j < 2; j++) {
+                    const int row = 8 * e + 2 * t + j;
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+                        *reinterpret_cast<float2*>(part + row * HDP + 16 * d + 2 * g) =
+                            make_float2(o[d][e][j], o[d][e][2 + j]);
+                    if (g == 0)
+                        *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(ref[e][j], l[e][j]);
+                }
         }
         if (n + 1 < count) {
             item0 += cur.nt;
@@ -681,33 +711,36 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (!joint || (whole && pa_start(U, workers, (long long)blockIdx.x * kPaWarps + 1) == c1)) return;
+    if (!joint || (whole && line.start(w0 + 1) == c1)) return;
 
-    // join the CTA's warps (their rings are free now)
+    // join the CTA's workers (their rings are free now)
     float* buf = reinterpret_cast<float*>(ring);
+    if (worker)
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int row = 8 * e + g;
-        if (count > 0)
+        for (int e = 0; e < E; e++)
 #pragma unroll
-            for (int d = 0; d < HDP / 16; d++)
-                *reinterpret_cast<float4*>(buf + row * HDP + 16 * d + 4 * t) =
-                    make_float4(o[d][e][0], o[d][e][1], o[d][e][2], o[d][e][3]);
-        if (t == 0)
-            *reinterpret_cast<float2*>(buf + ROWS * HDP + 2 * row) =
-                count > 0 ? make_float2(ref[e], l[e]) : make_float2(kPaLow, 0.0f);
-    }
+            for (int j = 0; j < 2; j++) {
+                const int row = 8 * e + 2 * t + j;
+                if (count > 0)
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+                        *reinterpret_cast<float2*>(buf + row * HDP + 16 * d + 2 * g) =
+                            make_float2(o[d][e][j], o[d][e][2 + j]);
+                if (g == 0)
+                    *reinterpret_cast<float2*>(buf + ROWS * HDP + 2 * row) =
+                        count > 0 ? make_float2(ref[e][j], l[e][j]) : make_float2(kPaLow, 0.0f);
+            }
     __syncthreads();
     const PaCursor c = s_cur[0];
     const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
-    float* part = work.part + ((size_t)blockIdx.x * kPaWarps * 2 + (c0 == s_first[0] ? 1 : 0)) * G::PART;
-    for (int i = tid; i < ROWS * HDP / 4; i += kPaWarps * 32) {
+    float* part = work.part + ((size_t)w0 * 2 + (c0 == s_first[0] ? 1 : 0)) * G::PART;
+    for (int i = tid; i < ROWS * HDP / 4; i += WARPS * 32) {
         const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
         float M = kPaLow, L = 0.0f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < kPaWarps; w++)
+        for (int w = 0; w < line.per_cta; w++)
             M = fmaxf(M, reinterpret_cast<const float*>(pa_sm + w * G::RING)[ROWS * HDP + 2 * row]);
-        for (int w = 0; w < kPaWarps; w++) {
+        for (int w = 0; w < line.per_cta; w++) {
             const float* wb = reinterpret_cast<const float*>(pa_sm + w * G::RING);
             const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
             if (wl == 0.0f) continue;  // no key (a warp without units left no o)
@@ -732,69 +765,63 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<HDP, ROWS>::CTAS)
     }
 }
 
-// CTA = the warps of one CTA of the kernel above: the items that start in their
-// runs and end in another one. Warp = query row; the parts of an item are, in
-// order, those of single warps at its ends and one of every CTA inside it.
-constexpr int kPaJoinWarps = 8;
-template <int HDP, int ROWS>
-__global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, ROWS>;
-    constexpr int ND = (HDP + 127) / 128;
+// The items that start in one worker's run and end in another's: four warps
+// per worker, a warp for every fourth query row. The parts of an item are, in
+// order, those of single workers at its ends and one of every CTA inside it.
+constexpr int kPaJoinWorkers = 4;
+template <int HDP, int E>
+__global__ void __launch_bounds__(kPaJoinWorkers * 128) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
+    using G = PaCfg<HDP, E>;
+    constexpr int ROWS = G::ROWS, NV = (HDP + 127) / 128;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.H / a.KV, hd = a.hd;
+    const long long wf = (long long)blockIdx.x * kPaJoinWorkers + (warp >> 2);
     griddep_wait();
-    const long long U = *work.total, workers = pa_workers(U, pl.ctas);
-    for (int wi = 0; wi < kPaWarps; wi++) {
-        const long long wf = (long long)blockIdx.x * kPaWarps + wi;
-        const PaTail tail = work.tail[wf];
-        if (tail.u1 == 0) continue;
-        long long wl = (tail.u1 - 1) * workers / U;
-        while (pa_start(U, workers, wl + 1) <= tail.u1 - 1) wl++;
-        while (pa_start(U, workers, wl) > tail.u1 - 1) wl--;
-        const long long cf = wf / kPaWarps, cl = wl / kPaWarps;
-        auto inside = [&](long long c) {
-            return pa_start(U, workers, c * kPaWarps) >= tail.u0 && pa_start(U, workers, (c + 1) * kPaWarps) <= tail.u1;
-        };
-        const bool ff = inside(cf), fl = inside(cl);
-        const int na = ff ? 1 : (int)(min(wl, cf * kPaWarps + kPaWarps - 1) - wf) + 1;
-        const int nm = (int)max(0LL, cl - cf - 1), nb = cl == cf ? 0 : fl ? 1 : (int)(wl - cl * kPaWarps) + 1;
-        const int np = na + nm + nb;
-        auto piece = [&](int i) -> const float* {
-            const long long w = i < na ? wf + i : i < na + nm ? (cf + 1 + i - na) * kPaWarps : cl * kPaWarps + (i - na - nm);
-            return work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
-        };
-        const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
-        for (int row = warp; row < ROWS && qb * ROWS + row < group; row += kPaJoinWarps) {
-            float M = kPaLow, L = 0.0f;
-            for (int i = lane; i < np; i += 32) M = fmaxf(M, piece(i)[ROWS * HDP + 2 * row]);
-            M = warp_max(M);
-            float4 O[ND];
+    const PaLine line = *work.line;
+    if (wf >= line.workers) return;
+    const PaTail tail = work.tail[wf];
+    if (tail.u1 == 0) return;
+    const long long wl = line.worker(tail.u1 - 1);
+    const int per = line.per_cta, cf = (int)(wf / per), cl = (int)(wl / per);
+    auto inside = [&](long long c) { return line.start(c * per) >= tail.u0 && line.start((c + 1) * per) <= tail.u1; };
+    const int na = inside(cf) ? 1 : (int)(min(wl, (long long)cf * per + per - 1) - wf) + 1;
+    const int nm = max(0, cl - cf - 1), nb = cl == cf ? 0 : inside(cl) ? 1 : (int)(wl - (long long)cl * per) + 1;
+    const int np = na + nm + nb;
+    auto piece = [&](int i) -> const float* {
+        const long long w = i < na ? wf + i : i < na + nm ? (long long)(cf + 1 + i - na) * per : (long long)cl * per + (i - na - nm);
+        return work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
+    };
+    const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
+    for (int row = warp & 3; row < ROWS && qb * ROWS + row < group; row += 4) {
+        float M = kPaLow, L = 0.0f;
+        for (int i = lane; i < np; i += 32) M = fmaxf(M, piece(i)[ROWS * HDP + 2 * row]);
+        M = warp_max(M);
+        float4 O[NV];
 #pragma unroll
-            for (int d = 0; d < ND; d++) O[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int d = 0; d < NV; d++) O[d] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-            for (int i = 0; i < np; i++) {
-                const float* p = piece(i);
-                const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * row);
-                const float f = ex2(rl.x - M);
-                L = __fmaf_rn(f, rl.y, L);
+        for (int i = 0; i < np; i++) {
+            const float* p = piece(i);
+            const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * row);
+            const float f = ex2(rl.x - M);
+            L = __fmaf_rn(f, rl.y, L);
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    if (128 * d + 4 * lane >= HDP) continue;
-                    const float4 x = *reinterpret_cast<const float4*>(p + row * HDP + 128 * d + 4 * lane);
-                    O[d] = make_float4(__fmaf_rn(f, x.x, O[d].x), __fmaf_rn(f, x.y, O[d].y), __fmaf_rn(f, x.z, O[d].z),
-                                       __fmaf_rn(f, x.w, O[d].w));
-                }
+            for (int d = 0; d < NV; d++) {
+                if (128 * d + 4 * lane >= HDP) continue;
+                const float4 x = *reinterpret_cast<const float4*>(p + row * HDP + 128 * d + 4 * lane);
+                O[d] = make_float4(__fmaf_rn(f, x.x, O[d].x), __fmaf_rn(f, x.y, O[d].y), __fmaf_rn(f, x.z, O[d].z),
+                                   __fmaf_rn(f, x.w, O[d].w));
             }
-            const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-            float* out = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd;
+        }
+        const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+        float* out = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd;
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                const int e = 128 * d + 4 * lane;
-                if (e >= hd) continue;
-                out[e] = O[d].x * inv;
-                out[e + 1] = O[d].y * inv;
-                out[e + 2] = O[d].z * inv;
-                out[e + 3] = O[d].w * inv;
-            }
+        for (int d = 0; d < NV; d++) {
+            const int e = 128 * d + 4 * lane;
+            if (e >= hd) continue;
+            out[e] = O[d].x * inv;
+            out[e + 1] = O[d].y * inv;
+            out[e + 2] = O[d].z * inv;
+            out[e + 3] = O[d].w * inv;
         }
     }
 }
@@ -812,46 +839,49 @@ int sm_count() {
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
-template <int HDP, int ROWS>
+template <int HDP, int E>
 size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
-    const size_t warps = (size_t)ctas * kPaWarps, at = align16(warps * sizeof(PaTail));
-    if (w) *w = PaWork{reinterpret_cast<long long*>(base), reinterpret_cast<PaTail*>(base + 16),
-                       reinterpret_cast<float*>(base + 16 + at)};
-    return 16 + at + warps * 2 * PaCfg<HDP, ROWS>::PART * sizeof(float);
+    const size_t workers = (size_t)ctas * PaCfg<HDP, E>::WARPS;
+    const size_t head = align16(sizeof(PaLine)), at = align16(workers * sizeof(PaTail));
+    if (w) *w = PaWork{reinterpret_cast<PaLine*>(base), reinterpret_cast<PaTail*>(base + head),
+                       reinterpret_cast<float*>(base + head + at)};
+    return head + at + workers * 2 * PaCfg<HDP, E>::PART * sizeof(float);
 }
 
-template <int HDP, int ROWS>
+template <int HDP, int E>
 int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
-    using G = PaCfg<HDP, ROWS>;
+    using G = PaCfg<HDP, E>;
     // the attribute belongs to the device
     static std::atomic<bool> ready[64];
     int dev = 0;
     JYC_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       G::SMEM));
         if (dev < 64) ready[dev].store(true, std::memory_order_release);
     }
     const long long cap = (long long)a.kv.table_stride * a.kv.p.page_size, tiles = (cap + G::TK - 1) / G::TK;
-    const long long most = (long long)a.kv.num_seqs * pl.units_row;  // items; times tiles: units
-    const long long want = tiles >= (1LL << 31) / std::max(1LL, most) ? 1LL << 31 : most * tiles;
+    const long long items = (long long)a.kv.num_seqs * pl.units_row;
+    // no more CTAs than the longest possible lengths have units for
+    const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles;
+    const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
     pl.tk = G::TK;
-    pl.ctas = (int)std::max(1LL, std::min((long long)sms * G::CTAS, (want + kPaWarps - 1) / kPaWarps));
+    pl.warps = G::WARPS;
     PaWork w;
-    pa_work_bytes<HDP, ROWS>(sms * G::CTAS, static_cast<unsigned char*>(work), &w);
-    paged_attention_kernel<HDP, ROWS><<<pl.ctas, kPaWarps * 32, G::SMEM, s>>>(a, pl, w);
+    pa_work_bytes<HDP, E>(sms, static_cast<unsigned char*>(work), &w);
+    paged_attention_kernel<HDP, E><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w);
     JYC_LAUNCHED();
     if (tiles <= 1) return JYC_OK;  // an item is one unit: none is split
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pl.ctas);
-    cfg.blockDim = dim3(kPaJoinWarps * 32);
+    cfg.gridDim = dim3((ctas * G::WARPS + kPaJoinWorkers - 1) / kPaJoinWorkers);
+    cfg.blockDim = dim3(kPaJoinWorkers * 128);
     cfg.stream = s;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, ROWS>, a, pl, w));
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, E>, a, pl, w));
     JYC_LAUNCHED();
     return JYC_OK;
 }
@@ -879,20 +909,20 @@ int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, cons
     return JYC_OK;
 }
 
-// The instantiation of a shape: head size rounded up, and 16 query heads per
-// unit above 8 (up to 8, hi and lo weights share one product).
-#define PA_CASES(F, ...)                                                      \
-    do {                                                                      \
-        const bool many = H / KV > 8;                                         \
-        if (hd <= 64) return many ? F<64, 16>(__VA_ARGS__) : F<64, 8>(__VA_ARGS__);     \
-        if (hd <= 128) return many ? F<128, 16>(__VA_ARGS__) : F<128, 8>(__VA_ARGS__);  \
-        if (hd <= 192) return many ? F<192, 16>(__VA_ARGS__) : F<192, 8>(__VA_ARGS__);  \
-        return many ? F<256, 16>(__VA_ARGS__) : F<256, 8>(__VA_ARGS__);       \
+// The instantiation of a shape: head size rounded up, and two blocks of 8 query
+// heads per unit above 8.
+#define PA_CASES(F, ...)                                                          \
+    do {                                                                          \
+        const bool many = H / KV > 8;                                             \
+        if (hd <= 64) return many ? F<64, 2>(__VA_ARGS__) : F<64, 1>(__VA_ARGS__);    \
+        if (hd <= 128) return many ? F<128, 2>(__VA_ARGS__) : F<128, 1>(__VA_ARGS__); \
+        if (hd <= 192) return many ? F<192, 2>(__VA_ARGS__) : F<192, 1>(__VA_ARGS__); \
+        return many ? F<256, 2>(__VA_ARGS__) : F<256, 1>(__VA_ARGS__);            \
     } while (0)
 
-template <int HDP, int ROWS>
+template <int HDP, int E>
 static size_t pa_workspace(int sms) {
-    return pa_work_bytes<HDP, ROWS>(sms * PaCfg<HDP, ROWS>::CTAS, nullptr, nullptr);
+    return pa_work_bytes<HDP, E>(sms, nullptr, nullptr);
 }
 
 size_t paged_attention_workspace(int H, int KV, int hd) {
