@@ -321,7 +321,8 @@ JYC_API size_t jyc_attention_paged_q8_workspace(int num_seqs, int num_heads, int
 
 /* Bits set by the paged operators on the current device since the last reset: 1 a
  * sequence, position or length out of range, 2 a page id out of range, 4 a
- * position behind the RoPE tables. Synchronises with the device. */
+ * position behind the RoPE tables, 8 a bounded wait gave up (an internal fault:
+ * that call's result is not valid). Synchronises with the device. */
 JYC_API int jyc_paged_error(int reset);
 
 /* The next token of every row of logits [rows][vocab_size] (row stride ld,

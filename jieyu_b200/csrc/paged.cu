@@ -5,6 +5,8 @@
 #include "paged.cuh"
 #include "ptx.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -145,10 +147,11 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
 // small vs that carries all the weight; the denominator adds the b_j.
 //
 // A step reads sum(len) * KV * (2 hd + 8) bytes and is bound by them, so: work
-// is a line of units (a unit: TK keys of one kv head of one sequence, 16-byte
-// cp.async rows), cut into equal runs for all resident warps whatever the
-// lengths; a warp keeps its next units in flight in its own ring in shared
-// memory across the borders of sequences and has no barrier in its loop.
+// is a line of units (a unit: TK keys of one kv head of one sequence), cut into equal runs for all resident warps whatever the lengths; a
+// warp keeps its next units in flight in its own ring in shared memory across
+// the borders of sequences and has no barrier in its loop. Heads of 64 or 128
+// on pages that divide a unit or that units divide come by one tensor copy per
+// page, K and V each; other shapes by 16- or 4-byte cp.async.
 // Keys are the rows of both products and the (up to 8 or 16) query heads of a
 // kv head the columns, so nothing of a tile is padding at 8 heads: S^T = K Q^T
 // with mma.m16n8k32 s8 (exact dots), O^T = V^T P^T with mma.m16n8k16 f16 (V is
@@ -231,18 +234,21 @@ __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
 // behind it hold whatever the ring held, finite as integers; they meet zero
 // query columns and unread output columns), E the blocks of 8 query heads of a
 // unit.
-template <int HDP, int E>
+template <int HDP, int E, bool TMA>
 struct PaCfg {
     static constexpr int TK = HDP <= 128 ? 32 : 16;      // keys of a unit
     static constexpr int WARPS = HDP <= 128 ? 12 : 8;    // one CTA per SM
     static constexpr int ST = HDP <= 64 ? 4 : HDP <= 128 ? 2 : 3;
     static constexpr int ROWS = 8 * E;
     static constexpr int VOFF = TK * HDP, SOFF = 2 * TK * HDP, MOFF = SOFF + 8 * TK;
-    static constexpr int STAGE = MOFF + 16;              // K, V, ks, vs, valid mask
+    // K and V; then ks, vs and the valid mask, which the tensor copies' variant keeps in registers. A tensor
+    // copy's swizzle goes by the address: stages on 1024 bytes
+    static constexpr int STAGE = TMA ? SOFF : MOFF + 16;
     static constexpr int PART = ROWS * (HDP + 2);        // floats of a partial: o, then (ref, l) per row
     static constexpr int FOFF = ST * STAGE;              // the current unit's keys, a float4 each
-    static constexpr int RING = FOFF + 16 * TK;
-    static constexpr int SMEM = WARPS * RING;
+    static constexpr int RING = TMA ? (FOFF + 16 * TK + 1023) / 1024 * 1024 : FOFF + 16 * TK;
+    static constexpr int SLACK = TMA ? 1024 : 0;         // to align the first stage
+    static constexpr int SMEM = WARPS * RING + SLACK;
     static_assert(PART * 4 <= RING, "a partial fits the ring");
     // byte of 16-byte chunk c of row r: chunks are swapped inside groups of 8 (of 4 where a row is no
     // multiple of 128 bytes) so that the 8 rows of an ldmatrix tile lie in distinct banks
@@ -252,11 +258,15 @@ struct PaCfg {
 };
 
 // What the kernels share about the line of units.
+struct PaMaps {
+    CUtensorMap k, v;
+};
 struct PaPlan {
     int units_row;  // kv heads * query blocks
     int qblocks;    // blocks of ROWS query heads per kv head
     int tk, warps;  // keys of a unit, warps of a CTA
     bool wide_copy; // 16-byte copies
+    int box;        // keys of a tensor copy
     uint32_t div_m; // pos / page_size = pos * div_m >> div_s, for pos < 2^31
     int div_s;
 };
@@ -328,19 +338,46 @@ __device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, Pa
     pa_seek(a, pl.tk, c);
 }
 
-template <int HDP, int E>
-__global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
-    paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, E>;
+// A wait that did not end at once: gives up after 2^31 SM cycles (about a
+// second) and sets the error word; the unit then counts for nothing.
+__device__ __noinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > (1LL << 31)) {
+            paged_flag(kPagedErrWait);
+            return false;
+        }
+    return true;
+}
+// box of a map's tensor [page][slot][kv head][dim] -> shared memory (this CTA's)
+__device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* map, int h, int slot, int page,
+                                               uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(h), "r"(slot), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+template <int HDP, int E, bool TMA>
+__global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
+    paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work, const __grid_constant__ PaMaps maps) {
+    using G = PaCfg<HDP, E, TMA>;
     constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS;
     constexpr int NK = HDP / 32, NM = TK / 16, ND = HDP / 16;
-    extern __shared__ __align__(128) unsigned char pa_sm[];
+    extern __shared__ __align__(128) unsigned char pa_raw[];
+    unsigned char* const pa_sm = TMA ? pa_raw + (-smem_u32(pa_raw) & 1023u) : pa_raw;
+    __shared__ __align__(8) uint64_t s_bar[WARPS][ST];
     __shared__ long long s_scan[WARPS];
     __shared__ PaCursor s_cur[WARPS];
     __shared__ long long s_first[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int B = a.kv.num_seqs, group = a.H / a.KV, hd = a.hd;
+    const int B = a.kv.num_seqs, group = a.H / a.KV, hd = TMA ? HDP : a.hd;
     griddep_launch();
+    if (TMA && lane == 0) {
+        for (int i = 0; i < ST; i++) mbar_init(&s_bar[warp][i], 1);
+        mbar_fence_init();
+    }
 
     // where the units of each sequence lie in the line
     const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
@@ -432,6 +469,8 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
         }
         issued++;
     };
+    float ksq[ST - 1], vsq[ST - 1];
+    bool inq[ST - 1];
     constexpr int LPR = HDP <= 64 ? 4 : HDP <= 128 ? 8 : 16, RPI = 32 / LPR;  // lanes per row, rows per step
     const int cc = (lane & (LPR - 1)) * 16, cr = lane / LPR;
     const int8_t* const kcol = a.kv.p.k + cc;
@@ -440,6 +479,32 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
         if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
             paged_flag(kPagedErrPage);
             ok = false;
+        }
+        if constexpr (TMA) {
+            // the scales of the units in flight wait in registers (lane j: key j)
+#pragma unroll
+            for (int i = 0; i + 1 < ST - 1; i++) {
+                ksq[i] = ksq[i + 1];
+                vsq[i] = vsq[i + 1];
+                inq[i] = inq[i + 1];
+            }
+            ksq[ST - 2] = vsq[ST - 2] = 0.0f;
+            inq[ST - 2] = ok;
+            const bool lead = ok && (lane & (pl.box - 1)) == 0;
+            const unsigned leads = __ballot_sync(0xffffffffu, lead);
+            if (lane == 0) mbar_expect_tx(&s_bar[warp][st], __popc(leads) * pl.box * (2 * HDP));
+            __syncwarp();
+            if (lead) {
+                const uint32_t dst = ring_a + st * G::STAGE + lane * HDP;
+                pa_tensor_copy(dst, &maps.k, h, slot, pg, &s_bar[warp][st]);
+                pa_tensor_copy(dst + G::VOFF, &maps.v, h, slot, pg, &s_bar[warp][st]);
+            }
+            if (ok) {
+                const long long so = (long long)pg * a.kv.p.spage_stride + (long long)slot * a.kv.p.spos_stride + hsoff;
+                ksq[ST - 2] = __ldg(a.kv.p.ks + so);
+                vsq[ST - 2] = __ldg(a.kv.p.vs + so);
+            }
+            return;
         }
         const uint32_t base = ring_a + st * G::STAGE;
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
@@ -490,6 +555,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4];
     bool fresh = true;
     int st = 0;
+    uint32_t phase = 0u;
     const float up = __fmul_rn(a.scale, 1.44269504088896341f);
 
     for (int n = 0; n < count; n++) {
@@ -536,21 +602,35 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
         }
         // the next unit's copies go to the stage that the last iteration read
         __syncwarp();
+        bool in = false;
+        float kscale = 0.0f, vscale = 0.0f;
+        if constexpr (TMA) {
+            in = inq[0];
+            kscale = ksq[0];
+            vscale = vsq[0];
+        }
         issue(st == 0 ? ST - 1 : st - 1);
         lookup();
-        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        __syncwarp();
+        if constexpr (TMA) {
+            if (!mbar_try_wait(&s_bar[warp][st], phase) && !pa_wait(&s_bar[warp][st], phase)) in = false;
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+            __syncwarp();
+        }
         const unsigned char* sb = ring + st * G::STAGE;
         const uint32_t base = ring_a + st * G::STAGE;
         // lane j: key j's {ks, 0 or -inf, e, vs}; a key that does not count has a score of -inf and vs = 0.
         // e is kept within 2^-64..2^126: the quantiser's scales are 0 or above 2^-34
         float4* keys = reinterpret_cast<float4*>(ring + G::FOFF);
         if (lane < TK) {
-            const bool in = (*reinterpret_cast<const unsigned*>(sb + G::MOFF) >> lane) & 1;
-            const float* sc = reinterpret_cast<const float*>(sb + G::SOFF);
-            const float v = in ? sc[TK + lane] : 0.0f;
-            const int ex = min(max((int)((__float_as_uint(v) >> 23) & 255u), 63), 253) - 127;
-            keys[lane] = in ? make_float4(sc[lane], 0.0f, (float)ex, v) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            if constexpr (!TMA) {
+                in = (*reinterpret_cast<const unsigned*>(sb + G::MOFF) >> lane) & 1;
+                const float* sc = reinterpret_cast<const float*>(sb + G::SOFF);
+                kscale = sc[lane];
+                vscale = in ? sc[TK + lane] : 0.0f;
+            }
+            const int ex = min(max((int)((__float_as_uint(vscale) >> 23) & 255u), 63), 253) - 127;
+            keys[lane] = in ? make_float4(kscale, 0.0f, (float)ex, vscale) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         }
         __syncwarp();
 
@@ -654,7 +734,10 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
                     for (int j = 0; j < 4; j++)
                         o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
         }
-        st = st == ST - 1 ? 0 : st + 1;
+        if (++st == ST) {
+            st = 0;
+            phase ^= 1u;
+        }
 
         const bool item_end = cur.t == cur.nt - 1;
         if (!item_end && n + 1 < count) {
@@ -710,7 +793,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
             fresh = true;
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!joint || (whole && line.start(w0 + 1) == c1)) return;
 
     // join the CTA's workers (their rings are free now)
@@ -765,16 +848,20 @@ __global__ void __launch_bounds__(PaCfg<HDP, E>::WARPS * 32, 1)
     }
 }
 
-// The items that start in one worker's run and end in another's: four warps
-// per worker, a warp for every fourth query row. The parts of an item are, in
-// order, those of single workers at its ends and one of every CTA inside it.
-constexpr int kPaJoinWorkers = 4;
-template <int HDP, int E>
-__global__ void __launch_bounds__(kPaJoinWorkers * 128) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, E>;
-    constexpr int ROWS = G::ROWS, NV = (HDP + 127) / 128;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.H / a.KV, hd = a.hd;
-    const long long wf = (long long)blockIdx.x * kPaJoinWorkers + (warp >> 2);
+// The items that start in one worker's run and end in another's: a CTA per
+// worker. The parts of an item are, in order, those of single workers at its
+// ends and one of every CTA inside it; warp w adds parts w, w + 8, ... for RB
+// query rows at a time (every load of a part in flight at once), then the
+// warps' sums are joined in shared memory.
+constexpr int kPaJoinWarps = 8;
+template <int HDP, int E, bool TMA>
+__global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
+    using G = PaCfg<HDP, E, TMA>;
+    constexpr int ROWS = G::ROWS, NV = (HDP + 127) / 128, RB = HDP <= 128 ? 8 : 4;
+    __shared__ __align__(16) float s_o[kPaJoinWarps][RB][HDP];
+    __shared__ float2 s_rl[kPaJoinWarps][RB];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
+    const long long wf = blockIdx.x;
     griddep_wait();
     const PaLine line = *work.line;
     if (wf >= line.workers) return;
@@ -786,42 +873,63 @@ __global__ void __launch_bounds__(kPaJoinWorkers * 128) paged_join_kernel(PagedA
     const int na = inside(cf) ? 1 : (int)(min(wl, (long long)cf * per + per - 1) - wf) + 1;
     const int nm = max(0, cl - cf - 1), nb = cl == cf ? 0 : inside(cl) ? 1 : (int)(wl - (long long)cl * per) + 1;
     const int np = na + nm + nb;
-    auto piece = [&](int i) -> const float* {
-        const long long w = i < na ? wf + i : i < na + nm ? (long long)(cf + 1 + i - na) * per : (long long)cl * per + (i - na - nm);
-        return work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
-    };
     const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
-    for (int row = warp & 3; row < ROWS && qb * ROWS + row < group; row += 4) {
-        float M = kPaLow, L = 0.0f;
-        for (int i = lane; i < np; i += 32) M = fmaxf(M, piece(i)[ROWS * HDP + 2 * row]);
-        M = warp_max(M);
-        float4 O[NV];
+    for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += RB) {
+        const int rows = min(RB, group - qb * ROWS - r0);
+        float4 o[RB][NV];
+        float ref = kPaLow, l = 0.0f;  // of row lane % RB
 #pragma unroll
-        for (int d = 0; d < NV; d++) O[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int i = 0; i < np; i++) {
-            const float* p = piece(i);
-            const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * row);
-            const float f = ex2(rl.x - M);
-            L = __fmaf_rn(f, rl.y, L);
+        for (int r = 0; r < RB; r++)
 #pragma unroll
-            for (int d = 0; d < NV; d++) {
-                if (128 * d + 4 * lane >= HDP) continue;
-                const float4 x = *reinterpret_cast<const float4*>(p + row * HDP + 128 * d + 4 * lane);
-                O[d] = make_float4(__fmaf_rn(f, x.x, O[d].x), __fmaf_rn(f, x.y, O[d].y), __fmaf_rn(f, x.z, O[d].z),
-                                   __fmaf_rn(f, x.w, O[d].w));
+            for (int d = 0; d < NV; d++) o[r][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = warp; i < np; i += kPaJoinWarps) {
+            const int w = i < na ? (int)wf + i : i < na + nm ? (cf + 1 + i - na) * per : cl * per + (i - na - nm);
+            const float* p = work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
+            const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * (r0 + (lane & (RB - 1))));
+            float4 x[RB][NV];
+#pragma unroll
+            for (int r = 0; r < RB; r++)
+#pragma unroll
+                for (int d = 0; d < NV; d++)
+                    x[r][d] = r < rows && 128 * d + 4 * lane < HDP
+                                  ? *reinterpret_cast<const float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float nr = fmaxf(ref, rl.x), fa = ex2(ref - nr), fb = ex2(rl.x - nr);
+            l = __fmaf_rn(l, fa, rl.y * fb);
+            ref = nr;
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                const float ga = __shfl_sync(0xffffffffu, fa, r), gb = __shfl_sync(0xffffffffu, fb, r);
+#pragma unroll
+                for (int d = 0; d < NV; d++) {
+                    o[r][d].x = __fmaf_rn(o[r][d].x, ga, x[r][d].x * gb);
+                    o[r][d].y = __fmaf_rn(o[r][d].y, ga, x[r][d].y * gb);
+                    o[r][d].z = __fmaf_rn(o[r][d].z, ga, x[r][d].z * gb);
+                    o[r][d].w = __fmaf_rn(o[r][d].w, ga, x[r][d].w * gb);
+                }
             }
         }
-        const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-        float* out = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd;
+        __syncthreads();  // the last row block's sums are read
 #pragma unroll
-        for (int d = 0; d < NV; d++) {
-            const int e = 128 * d + 4 * lane;
-            if (e >= hd) continue;
-            out[e] = O[d].x * inv;
-            out[e + 1] = O[d].y * inv;
-            out[e + 2] = O[d].z * inv;
-            out[e + 3] = O[d].w * inv;
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int d = 0; d < NV; d++)
+                if (128 * d + 4 * lane < HDP) *reinterpret_cast<float4*>(&s_o[warp][r][128 * d + 4 * lane]) = o[r][d];
+        if (lane < RB) s_rl[warp][lane] = make_float2(ref, l);
+        __syncthreads();
+        const int used = min(np, kPaJoinWarps);
+        for (int i = tid; i < rows * HDP; i += kPaJoinWarps * 32) {
+            const int r = i / HDP, d = i % HDP;
+            float M = kPaLow, L = 0.0f, O = 0.0f;
+            for (int w = 0; w < used; w++) M = fmaxf(M, s_rl[w][r].x);
+            for (int w = 0; w < used; w++) {
+                const float f = ex2(s_rl[w][r].x - M);
+                L = __fmaf_rn(f, s_rl[w][r].y, L);
+                O = __fmaf_rn(f, s_o[w][r][d], O);
+            }
+            if (d < hd)
+                a.out[(size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + r0 + r) * hd + d] =
+                    L == 0.0f ? 0.0f : __fdiv_rn(O, L);
         }
     }
 }
@@ -839,24 +947,60 @@ int sm_count() {
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
-template <int HDP, int E>
+template <int HDP, int E, bool TMA>
 size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
-    const size_t workers = (size_t)ctas * PaCfg<HDP, E>::WARPS;
+    const size_t workers = (size_t)ctas * PaCfg<HDP, E, TMA>::WARPS;
     const size_t head = align16(sizeof(PaLine)), at = align16(workers * sizeof(PaTail));
     if (w) *w = PaWork{reinterpret_cast<PaLine*>(base), reinterpret_cast<PaTail*>(base + head),
                        reinterpret_cast<float*>(base + head + at)};
-    return head + at + workers * 2 * PaCfg<HDP, E>::PART * sizeof(float);
+    return head + at + workers * 2 * PaCfg<HDP, E, TMA>::PART * sizeof(float);
 }
 
-template <int HDP, int E>
+// Map of a cache array as [page][slot][kv head][dim], boxes of `box` slots of one head.
+int pa_map(CUtensorMap* m, int8_t* base, const PagedAttn& a, int box) {
+    static std::atomic<void*> entry;
+    void* fn = entry.load(std::memory_order_acquire);
+    if (!fn) {
+        cudaDriverEntryPointQueryResult found;
+        JYC_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !fn) return cuda_fail(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+        entry.store(fn, std::memory_order_release);
+    }
+    const jyc_kv_pages& p = a.kv.p;
+    const cuuint64_t dims[4] = {(cuuint64_t)a.hd, (cuuint64_t)a.KV, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
+    // the stride of a dimension of one entry is not used, but has to be one
+    const cuuint64_t strides[3] = {(cuuint64_t)(a.KV > 1 ? p.head_stride : a.hd),
+                                   (cuuint64_t)(p.page_size > 1 ? p.pos_stride : a.hd),
+                                   (cuuint64_t)(p.num_pages > 1 ? p.page_stride : a.hd)};
+    const cuuint32_t boxes[4] = {(cuuint32_t)a.hd, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn)(
+        m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        a.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return JYC_OK;
+}
+
+// Tensor copies need rows of 64 or 128 bytes, strides below 2^40 that are multiples of 16 bytes, pages that
+// a unit of 32 keys fills or that fill a unit, and boxes that start on 128 bytes of shared memory.
+bool pa_tensor_copies(const PagedAttn& a, bool aligned) {
+    const jyc_kv_pages& p = a.kv.p;
+    const long long far = std::max(p.page_stride, std::max(p.pos_stride, p.head_stride));
+    const bool nonzero = (p.head_stride > 0 || a.KV == 1) && (p.pos_stride > 0 || p.page_size == 1) &&
+                         (p.page_stride > 0 || p.num_pages == 1);
+    return aligned && nonzero && far < (1LL << 40) && (a.hd == 64 || a.hd == 128) &&
+           (p.page_size % 32 == 0 || (32 % p.page_size == 0 && p.page_size * a.hd % 128 == 0));
+}
+
+template <int HDP, int E, bool TMA>
 int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
-    using G = PaCfg<HDP, E>;
+    using G = PaCfg<HDP, E, TMA>;
     // the attribute belongs to the device
     static std::atomic<bool> ready[64];
     int dev = 0;
     JYC_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, E, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       G::SMEM));
         if (dev < 64) ready[dev].store(true, std::memory_order_release);
     }
@@ -867,21 +1011,28 @@ int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s
     const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
     pl.tk = G::TK;
     pl.warps = G::WARPS;
+    PaMaps maps{};
+    if (TMA) {
+        pl.box = std::min(a.kv.p.page_size, G::TK);
+        int r = pa_map(&maps.k, a.kv.p.k, a, pl.box);
+        if (r == JYC_OK) r = pa_map(&maps.v, a.kv.p.v, a, pl.box);
+        if (r != JYC_OK) return r;
+    }
     PaWork w;
-    pa_work_bytes<HDP, E>(sms, static_cast<unsigned char*>(work), &w);
-    paged_attention_kernel<HDP, E><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w);
+    pa_work_bytes<HDP, E, TMA>(sms, static_cast<unsigned char*>(work), &w);
+    paged_attention_kernel<HDP, E, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, maps);
     JYC_LAUNCHED();
     if (tiles <= 1) return JYC_OK;  // an item is one unit: none is split
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((ctas * G::WARPS + kPaJoinWorkers - 1) / kPaJoinWorkers);
-    cfg.blockDim = dim3(kPaJoinWorkers * 128);
+    cfg.gridDim = dim3(ctas * G::WARPS);
+    cfg.blockDim = dim3(kPaJoinWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, E>, a, pl, w));
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, E, TMA>, a, pl, w));
     JYC_LAUNCHED();
     return JYC_OK;
 }
@@ -909,20 +1060,20 @@ int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, cons
     return JYC_OK;
 }
 
-// The instantiation of a shape: head size rounded up, and two blocks of 8 query
-// heads per unit above 8.
-#define PA_CASES(F, ...)                                                          \
-    do {                                                                          \
-        const bool many = H / KV > 8;                                             \
-        if (hd <= 64) return many ? F<64, 2>(__VA_ARGS__) : F<64, 1>(__VA_ARGS__);    \
-        if (hd <= 128) return many ? F<128, 2>(__VA_ARGS__) : F<128, 1>(__VA_ARGS__); \
-        if (hd <= 192) return many ? F<192, 2>(__VA_ARGS__) : F<192, 1>(__VA_ARGS__); \
-        return many ? F<256, 2>(__VA_ARGS__) : F<256, 1>(__VA_ARGS__);            \
+// The instantiation of a shape: head size rounded up, two blocks of 8 query
+// heads per unit above 8, and how the rows are copied.
+#define PA_CASES(F, TMA, ...)                                                                   \
+    do {                                                                                        \
+        const bool many = H / KV > 8;                                                           \
+        if (hd <= 64) return many ? F<64, 2, TMA>(__VA_ARGS__) : F<64, 1, TMA>(__VA_ARGS__);    \
+        if (hd <= 128) return many ? F<128, 2, TMA>(__VA_ARGS__) : F<128, 1, TMA>(__VA_ARGS__); \
+        if (hd <= 192) return many ? F<192, 2, false>(__VA_ARGS__) : F<192, 1, false>(__VA_ARGS__); \
+        return many ? F<256, 2, false>(__VA_ARGS__) : F<256, 1, false>(__VA_ARGS__);            \
     } while (0)
 
-template <int HDP, int E>
+template <int HDP, int E, bool TMA>
 static size_t pa_workspace(int sms) {
-    return pa_work_bytes<HDP, E>(sms, nullptr, nullptr);
+    return pa_work_bytes<HDP, E, TMA>(sms, nullptr, nullptr);
 }
 
 size_t paged_attention_workspace(int H, int KV, int hd) {
@@ -931,7 +1082,7 @@ size_t paged_attention_workspace(int H, int KV, int hd) {
         cuda_fail(cudaErrorNoDevice, "paged attention: device query");
         return 0;
     }
-    PA_CASES(pa_workspace, sms);
+    PA_CASES(pa_workspace, false, sms);
 }
 
 int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
@@ -948,7 +1099,8 @@ int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
     const jyc_kv_pages& p = a.kv.p;
     pl.wide_copy = hd % 16 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
                    ((p.page_stride | p.pos_stride | p.head_stride) & 15) == 0;
-    PA_CASES(pa_launch, a, pl, sms, work, s);
+    if (pa_tensor_copies(a, pl.wide_copy)) PA_CASES(pa_launch, true, a, pl, sms, work, s);
+    PA_CASES(pa_launch, false, a, pl, sms, work, s);
 }
 
 }  // namespace jyc

@@ -25,6 +25,7 @@ struct PagedRope {
 constexpr int kPagedErrPos = 1;   // sequence or position out of range
 constexpr int kPagedErrPage = 2;  // page id out of range
 constexpr int kPagedErrRope = 4;  // position behind the RoPE tables
+constexpr int kPagedErrWait = 8;  // a copy's bounded wait gave up
 
 int* paged_error_word();
 

@@ -208,6 +208,13 @@ ATTEND = [  # H, KV, hd, page, heads_first, rope, gap, lengths
     (8, 2, 132, 16, False, False, 0, [70]),
     (2, 2, 252, 16, False, True, 4, [70, 300]),
     (6, 2, 64, 16, False, False, 4, [70, 300]),                # 16-byte heads at 4-byte strides
+    (8, 2, 64, 1, False, True, 0, [5, 100]),                   # pages of 1, 2, 4, 8 and 96 positions
+    (8, 2, 64, 2, True, True, 0, [5, 100]),
+    (12, 1, 128, 1, True, True, 0, [33, 95]),
+    (4, 2, 128, 4, False, False, 16, [33, 95]),
+    (16, 2, 128, 8, True, True, 0, [260, 31]),
+    (20, 2, 64, 96, False, True, 0, [96, 97, 500]),
+    (8, 1, 128, 2048, False, True, 0, [2049, 100]),
 ]
 
 
