@@ -56,15 +56,19 @@ __device__ __forceinline__ float4 load4(const float* p, bool vec) {
     return make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
 }
 
-// Quad qd (elements 4 qd .. 4 qd + 3: pairs 2 qd, 2 qd + 1) rotated by the
-// table rows c, s (rope_pos's rounding: one product rounded, one fused sum).
-__device__ __forceinline__ float4 rotate4(float4 x, const float* c, const float* s, int qd) {
-    const float c0 = __ldg(c + 2 * qd), c1 = __ldg(c + 2 * qd + 1), s0 = __ldg(s + 2 * qd), s1 = __ldg(s + 2 * qd + 1);
+__device__ __forceinline__ float2 load2(const float* p, bool vec) {
+    if (vec) return __ldg(reinterpret_cast<const float2*>(p));
+    return make_float2(__ldg(p), __ldg(p + 1));
+}
+
+// Two pairs rotated by their table entries (rope_pos's rounding: one product
+// rounded, one fused sum).
+__device__ __forceinline__ float4 rotate4(float4 x, float2 c, float2 s) {
     float4 r;
-    r.x = __fmaf_rn(x.x, c0, -__fmul_rn(x.y, s0));
-    r.y = __fmaf_rn(x.x, s0, __fmul_rn(x.y, c0));
-    r.z = __fmaf_rn(x.z, c1, -__fmul_rn(x.w, s1));
-    r.w = __fmaf_rn(x.z, s1, __fmul_rn(x.w, c1));
+    r.x = __fmaf_rn(x.x, c.x, -__fmul_rn(x.y, s.x));
+    r.y = __fmaf_rn(x.x, s.x, __fmul_rn(x.y, c.x));
+    r.z = __fmaf_rn(x.z, c.y, -__fmul_rn(x.w, s.y));
+    r.w = __fmaf_rn(x.z, s.y, __fmul_rn(x.w, c.y));
     return r;
 }
 __device__ __forceinline__ float amax4(float4 x) {
@@ -102,7 +106,9 @@ __global__ void paged_append_kernel(const float* K, const float* V, int ld, int 
         const int qd = lane + 32 * t;
         if (qd >= nq) continue;
         x[t] = load4(src + 4 * qd, vec);
-        if (rot) x[t] = rotate4(x[t], rope.cos_t + (size_t)pos * half, rope.sin_t + (size_t)pos * half, qd);
+        if (rot)
+            x[t] = rotate4(x[t], load2(rope.cos_t + (size_t)pos * half + 2 * qd, vec),
+                           load2(rope.sin_t + (size_t)pos * half + 2 * qd, vec));
         amax = fmaxf(amax, amax4(x[t]));
     }
     amax = warp_max(amax);
@@ -141,10 +147,11 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
 //
 // out = sum_j p_j vs_j v_j / sum_j p_j, p_j = exp(dot_j (ks_j qs) / sqrt(hd)),
 // one pass over the keys with a running reference. In base 2, with vs_j =
-// 2^e_j f_j (1 <= f_j < 2): ref = max_j (s_j + e_j) - 13, b_j = 2^(s_j - ref);
-// the weights w_j = b_j vs_j are below 2^14 and the largest is at least 2^13,
-// so as a pair of fp16 (hi + lo, 22 bits) they neither overflow nor lose a
-// small vs that carries all the weight; the denominator adds the b_j.
+// 2^e_j f_j (1 <= f_j < 2): b_j = 2^(s_j - ref), w_j = b_j vs_j < 2^(1 + s_j +
+// e_j - ref). The reference follows the maximum of s_j + e_j, not of s_j, so
+// that the weights neither overflow a format of limited range (integers, or
+// pairs of fp16 with 22 bits) nor lose a small vs that carries all the weight;
+// the denominator adds the b_j.
 //
 // A step reads sum(len) * KV * (2 hd + 8) bytes and is bound by them, so: work
 // is a line of units (a unit: TK keys of one kv head of one sequence), cut into equal runs for all resident warps whatever the lengths; a
@@ -152,19 +159,30 @@ __global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, 
 // the borders of sequences and has no barrier in its loop. Heads of 64 or 128
 // on pages that divide a unit or that units divide come by one tensor copy per
 // page, K and V each; other shapes by 16- or 4-byte cp.async.
-// Keys are the rows of both products and the (up to 8 or 16) query heads of a
-// kv head the columns, so nothing of a tile is padding at 8 heads: S^T = K Q^T
-// with mma.m16n8k32 s8 (exact dots), O^T = V^T P^T with mma.m16n8k16 f16 (V is
-// exact in fp16), the weights transposed between them by movmatrix. Each
-// unit's product starts from zero and is added in fp32 with round to nearest
-// (the tensor cores' own sums may truncate).
+// Keys are the rows of both products and the query heads of a kv head the
+// columns: S^T = K Q^T with mma.m16n8k32 s8 (exact dots), then O^T = V^T P^T,
+// the weights transposed between them by movmatrix.
+//
+// Up to 8 heads of up to 128 dims: the weights are rounded to 31-bit integers
+// (reference 27 below the maximum, raised when a weight would pass 2^30 times
+// the reference), whose four bytes are columns of an integer product with V's
+// own bytes: mma.m16n8k32 s8 x u8, exact, summed in 32-bit integers over up to
+// 2000 units; a rounding is 2^-28 of the largest weight at most. V needs no
+// conversion (a byte permute), and no accumulator is touched between units.
+// Beyond that the integers would not fit the registers: hi and lo halves of
+// the weights and mma.m16n8k16 f16 (V is exact in fp16); each unit's product
+// starts from zero and is added in fp32 with round to nearest (the tensor
+// cores' own sums may truncate).
 //
 // A run that covers an item (a kv head of a sequence) whole writes its rows of
-// out; the others leave (o, ref, l) in the workspace and a second kernel,
-// launched early, joins them. The warps of a CTA inside one item are joined in
-// shared memory first.
+// out; the others leave parts (o, ref, l), which are joined inside the CTA where
+// the item ends in it (through shared memory when the CTA has one item only,
+// through the workspace otherwise), and by a second kernel where it does not:
+// one part per CTA that the item touches.
 
-constexpr float kPaShift = 13.0f;
+constexpr float kPaShift = 13.0f;              // halves: the largest weight is in 2^13 .. 2^14
+constexpr float kPaSet = 27.0f, kPaMost = 30.0f;  // digits: 2^27 .. 2^28 when the reference is set, below 2^31 ever
+constexpr int kPaFlush = 2000;                 // units whose digit sums fit 32 bits: 32 * 255 * 128 each
 constexpr float kPaLow = -1.7e38f;  // reference before any key: below every score, and its differences stay finite
 
 __device__ __forceinline__ float ex2(float x) {
@@ -180,6 +198,12 @@ __device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t
 }
 __device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// c += a b, a signed, b unsigned bytes
+__device__ __forceinline__ void pa_mma_s8u8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -211,12 +235,20 @@ __device__ __forceinline__ void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
                  : "r"(addr)
                  : "memory");
 }
+// The cache is read once a step: its lines leave L2 first, so that code, queries and parts stay there
+// (measured: without the hint a kernel's end runs at DRAM latency, instruction by instruction).
+// Scales of neighbouring heads may share a sector, which other SMs want too: no hint.
+__device__ __forceinline__ void pa_copy_scale(uint32_t dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void pa_copy(uint32_t dst, const void* src) {
+__device__ __forceinline__ void pa_copy(uint32_t dst, const void* src, uint64_t policy) {
     if (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
+                     : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+        asm volatile("cp.async.ca.shared.global.L2::cache_hint [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "l"(policy)
+                     : "memory");
 }
 // bytes 0, 2 (ODD: 1, 3) of x = q ^ 0x80 as the halves q: 0x6400 | u is 1024 + u
 template <bool ODD>
@@ -232,20 +264,25 @@ __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
 
 // Sizes of one instantiation: HDP is the head size rounded up (the columns
 // behind it hold whatever the ring held, finite as integers; they meet zero
-// query columns and unread output columns), E the blocks of 8 query heads of a
-// unit.
-template <int HDP, int E, bool TMA>
+// query columns and unread output columns), HEADS the query heads of a unit.
+template <int HDP, int HEADS, bool TMA>
 struct PaCfg {
-    static constexpr int TK = HDP <= 128 ? 32 : 16;      // keys of a unit
-    static constexpr int WARPS = HDP <= 128 ? 12 : 8;    // one CTA per SM
-    static constexpr int ST = HDP <= 64 ? 4 : HDP <= 128 ? 2 : 3;
-    static constexpr int ROWS = 8 * E;
+    static constexpr bool DIG = HEADS <= 8 && HDP <= 128;  // weights as digits, else as halves
+    static constexpr int TK = HDP <= 128 ? 32 : 16;        // keys of a unit
+    // one CTA per SM. Few warps with many units in flight each and room for every accumulator in registers beat more
+    // warps with fewer: 131072 keys of 8 x 128, 4 heads each, take 78 us with 12 warps of 2 stages, 62 with 8 of 3
+    static constexpr int WARPS = HDP <= 64 || (HDP <= 128 && HEADS == 16) ? 12 : 8;
+    static constexpr int ST = HDP <= 64 ? 4 : HDP <= 128 && HEADS == 16 ? 2 : 3;
+    static constexpr int NT = HEADS <= 4 ? 2 : 4;          // n8 tiles of digits: 4 digits of each head
+    static constexpr int E = HEADS <= 8 ? 1 : 2;           // n8 tiles of heads
+    static constexpr int ROWS = HEADS;
     static constexpr int VOFF = TK * HDP, SOFF = 2 * TK * HDP, MOFF = SOFF + 8 * TK;
-    // K and V; then ks, vs and the valid mask, which the tensor copies' variant keeps in registers. A tensor
-    // copy's swizzle goes by the address: stages on 1024 bytes
+    // K and V; then ks, vs and the valid mask. A tensor copy's swizzle goes by the address: stages on 1024 bytes,
+    // the scales behind all of them
     static constexpr int STAGE = TMA ? SOFF : MOFF + 16;
     static constexpr int PART = ROWS * (HDP + 2);        // floats of a partial: o, then (ref, l) per row
-    static constexpr int FOFF = ST * STAGE;              // the current unit's keys, a float4 each
+    static constexpr int KOFF = ST * STAGE;              // tensor copies: ks and vs of the stages
+    static constexpr int FOFF = KOFF + (TMA ? ST * 8 * TK : 0);  // the current unit's keys, a float4 each
     static constexpr int RING = TMA ? (FOFF + 16 * TK + 1023) / 1024 * 1024 : FOFF + 16 * TK;
     static constexpr int SLACK = TMA ? 1024 : 0;         // to align the first stage
     static constexpr int SMEM = WARPS * RING + SLACK;
@@ -266,6 +303,7 @@ struct PaPlan {
     int qblocks;    // blocks of ROWS query heads per kv head
     int tk, warps;  // keys of a unit, warps of a CTA
     bool wide_copy; // 16-byte copies
+    bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
     int box;        // keys of a tensor copy
     uint32_t div_m; // pos / page_size = pos * div_m >> div_s, for pos < 2^31
     int div_s;
@@ -278,19 +316,21 @@ struct PaLine {
         w = min(w, workers);
         return w * base + min(w, rest);
     }
-    __device__ __forceinline__ long long worker(long long u) const {  // whose run holds unit u
+    __device__ __forceinline__ int worker(long long u) const {  // whose run holds unit u
         const long long big = rest * (base + 1);
-        return u < big ? u / (base + 1) : rest + (u - big) / base;
+        if (u >> 32) return (int)(u < big ? u / (base + 1) : rest + (u - big) / base);
+        return (int)(u < big ? (unsigned)u / (unsigned)(base + 1) : (unsigned)rest + (unsigned)(u - big) / (unsigned)base);
     }
 };
-// Item that a worker's run starts and another one ends.
+// Item that starts in a CTA and ends in a later one.
 struct PaTail {
-    long long u0, u1;  // units of the item; u1 == 0: none
+    int ctas;  // CTAs after the first that hold parts of it; 0: no such item
+    int slot;  // its first part
     int b, r;
+    int per_cta;
 };
 struct PaWork {
-    PaLine* line;
-    PaTail* tail;      // [workers]
+    PaTail* tail;      // [CTAs]
     float* part;       // [workers][2][PART]: an item's later part (0), its first (1)
 };
 
@@ -313,11 +353,17 @@ __device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
 constexpr int kPaFewWarps = 4;
 __device__ __forceinline__ PaLine pa_line(long long U, int ctas, int warps) {
     PaLine l;
-    const long long each = (U + ctas - 1) / ctas;
+    const long long each = U >> 31 ? warps : ((unsigned)U + ctas - 1) / (unsigned)ctas;
     l.per_cta = (int)min((long long)warps, max((long long)kPaFewWarps, each));
     l.workers = min((long long)ctas * l.per_cta, U);
-    l.base = l.workers ? U / l.workers : 0;
-    l.rest = l.workers ? U % l.workers : 0;
+    l.base = l.rest = 0;
+    if (U >> 32) {
+        l.base = U / l.workers;
+        l.rest = U % l.workers;
+    } else if (l.workers) {
+        l.base = (unsigned)U / (unsigned)l.workers;
+        l.rest = (unsigned)U % (unsigned)l.workers;
+    }
     return l;
 }
 
@@ -329,8 +375,8 @@ __device__ __forceinline__ void pa_seek(const PagedAttn& a, int tk, PaCursor& c)
     while (c.b < a.kv.num_seqs && (c.len = pa_len(a, c.b)) == 0) c.b++;
     c.nt = (c.len + tk - 1) / tk;
 }
-__device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, PaCursor& c) {
-    if (++c.t < c.nt) return;
+__device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, PaCursor& c, int step) {
+    if ((c.t += step) < c.nt) return;
     c.t = 0;
     if (++c.r < pl.units_row) return;
     c.r = 0;
@@ -351,31 +397,112 @@ __device__ __noinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
 }
 // box of a map's tensor [page][slot][kv head][dim] -> shared memory (this CTA's)
 __device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* map, int h, int slot, int page,
-                                               uint64_t* bar) {
+                                               uint64_t* bar, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(map), "r"(0), "r"(h), "r"(slot), "r"(page), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+        "l"(map), "r"(0), "r"(h), "r"(slot), "r"(page), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
 
-template <int HDP, int E, bool TMA>
-__global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
+// One warp's sum of parts for RB query rows: every load of a part is in flight
+// at once. Lane i holds dims 4 i .. 4 i + 3 of every 128, and (ref, l) of row i % RB.
+template <int HDP, int HEADS, bool TMA>
+struct PaSum {
+    using G = PaCfg<HDP, HEADS, TMA>;
+    static constexpr int RB = HDP <= 128 && HEADS >= 8 ? 8 : 4, NV = (HDP + 127) / 128;
+    float4 o[RB][NV];
+    float ref, l;
+    // parts i = first, first + step, ... < np at work slots slot(i), rows r0 .. r0 + rows - 1
+    template <class F>
+    __device__ __forceinline__ void add(const float* part, int r0, int rows, int np, int first, int step, F slot) {
+        const int lane = threadIdx.x & 31;
+        ref = kPaLow;
+        l = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int d = 0; d < NV; d++) o[r][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i = first; i < np; i += step) {
+            const float* p = part + (size_t)slot(i) * G::PART;
+            const float2 rl = *reinterpret_cast<const float2*>(p + G::ROWS * HDP + 2 * (r0 + (lane & (RB - 1))));
+            float4 x[RB][NV];
+#pragma unroll
+            for (int r = 0; r < RB; r++)
+#pragma unroll
+                for (int d = 0; d < NV; d++)
+                    x[r][d] = r < rows && 128 * d + 4 * lane < HDP
+                                  ? *reinterpret_cast<const float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float nr = fmaxf(ref, rl.x), fa = ex2(ref - nr), fb = ex2(rl.x - nr);
+            l = __fmaf_rn(l, fa, rl.y * fb);
+            ref = nr;
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                const float ga = __shfl_sync(0xffffffffu, fa, r), gb = __shfl_sync(0xffffffffu, fb, r);
+#pragma unroll
+                for (int d = 0; d < NV; d++) {
+                    o[r][d].x = __fmaf_rn(o[r][d].x, ga, x[r][d].x * gb);
+                    o[r][d].y = __fmaf_rn(o[r][d].y, ga, x[r][d].y * gb);
+                    o[r][d].z = __fmaf_rn(o[r][d].z, ga, x[r][d].z * gb);
+                    o[r][d].w = __fmaf_rn(o[r][d].w, ga, x[r][d].w * gb);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* p, int r0, int rows) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int d = 0; d < NV; d++)
+                if (r < rows && 128 * d + 4 * lane < HDP)
+                    *reinterpret_cast<float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane) = o[r][d];
+        if (lane < rows) *reinterpret_cast<float2*>(p + G::ROWS * HDP + 2 * (r0 + lane)) = make_float2(ref, l);
+    }
+    __device__ __forceinline__ void finish(float* out, int rows, int hd) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            const float lr = __shfl_sync(0xffffffffu, l, r), inv = lr == 0.0f ? 0.0f : __fdiv_rn(1.0f, lr);
+#pragma unroll
+            for (int d = 0; d < NV; d++) {
+                const int e = 128 * d + 4 * lane;
+                if (r >= rows || e >= hd) continue;
+                float* to = out + (size_t)r * hd + e;
+                to[0] = o[r][d].x * inv;
+                to[1] = o[r][d].y * inv;
+                to[2] = o[r][d].z * inv;
+                to[3] = o[r][d].w * inv;
+            }
+        }
+    }
+};
+
+template <int HDP, int HEADS, bool TMA>
+__global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work, const __grid_constant__ PaMaps maps) {
-    using G = PaCfg<HDP, E, TMA>;
-    constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS;
+    using G = PaCfg<HDP, HEADS, TMA>;
+    constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS, E = G::E, NT = G::NT;
+    constexpr bool DIG = G::DIG;
     constexpr int NK = HDP / 32, NM = TK / 16, ND = HDP / 16;
     extern __shared__ __align__(128) unsigned char pa_raw[];
     unsigned char* const pa_sm = TMA ? pa_raw + (-smem_u32(pa_raw) & 1023u) : pa_raw;
-    __shared__ __align__(8) uint64_t s_bar[WARPS][ST];
-    __shared__ long long s_scan[WARPS];
+    __shared__ __align__(8) uint64_t s_bar[WARPS][ST][2];  // K, V
+    __shared__ long long s_scan[WARPS], s_ex[WARPS * 32];
+    const uint64_t policy = policy_evict_first();
     __shared__ PaCursor s_cur[WARPS];
     __shared__ long long s_first[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int B = a.kv.num_seqs, group = a.H / a.KV, hd = TMA ? HDP : a.hd;
     griddep_launch();
     if (TMA && lane == 0) {
-        for (int i = 0; i < ST; i++) mbar_init(&s_bar[warp][i], 1);
+        if (warp == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+        }
+        for (int i = 0; i < 2 * ST; i++) mbar_init(&s_bar[warp][0][i], 1);
         mbar_fence_init();
     }
 
@@ -399,22 +526,29 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
         U += s_scan[w];
     }
     const PaLine line = pa_line(U, gridDim.x, WARPS);
-    if (blockIdx.x == 0 && tid == 0) *work.line = line;
     const long long w0 = (long long)blockIdx.x * line.per_cta;
-    for (int w = 0; w < line.per_cta; w++) {
-        const long long u = line.start(w0 + w);
-        if (u < ex || u >= ex + mine) continue;
-        long long at = ex;
-        for (int b = bs; b < be; b++) {
-            const int len = pa_len(a, b), nt = (len + TK - 1) / TK;
-            const long long n = (long long)nt * pl.units_row;
-            if (u < at + n) {
-                const int k = (int)(u - at);
-                s_cur[w] = PaCursor{b, k / nt, k % nt, nt, len};
-                s_first[w] = u - k % nt;  // first unit of the item that the run starts in
-                break;
+    s_ex[tid] = ex;
+    __syncthreads();
+    {
+        // warp: where its run starts (the last thread's segment that starts at or before it)
+        const long long u = line.start(w0 + warp);
+        if (warp < line.per_cta && u < U) {
+            int lo = 0;
+#pragma unroll
+            for (int i = 1 << (31 - __builtin_clz(WARPS * 32)); i > 0; i >>= 1)
+                if (lo + i < WARPS * 32 && s_ex[lo + i] <= u) lo += i;
+            long long at = s_ex[lo];
+            for (int b = min(B, lo * per); b < B; b++) {
+                const int len = pa_len(a, b), nt = (len + TK - 1) / TK;
+                const long long n = (long long)nt * pl.units_row;
+                if (u < at + n) {
+                    const int k = (int)(u - at), r = k / nt;
+                    s_cur[warp] = PaCursor{b, r, k - r * nt, nt, len};
+                    s_first[warp] = u - (k - r * nt);  // first unit of the item that the run starts in
+                    break;
+                }
+                at += n;
             }
-            at += n;
         }
     }
     // sequences without a key: rows of zeros
@@ -424,25 +558,32 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
     __syncthreads();
 
     const bool worker = warp < line.per_cta;
-    const long long u0 = line.start(w0 + warp), u1 = line.start(w0 + warp + 1);
-    const long long c0 = line.start(w0), c1 = line.start(w0 + line.per_cta);
-    const int count = worker ? (int)(u1 - u0) : 0;
-    unsigned char* ring = pa_sm + warp * G::RING;
-    const uint32_t ring_a = smem_u32(ring);
-    PaCursor cur = PaCursor{0, 0, 0, 0, 0};
-    long long item0 = 0;
-    if (count > 0) {
-        cur = s_cur[warp];
-        item0 = s_first[warp];
-    }
-    // every worker of the CTA inside one item: joined below
-    bool joint = false, whole = false;  // whole: and they are all of it
+    const long long u0 = line.start(w0 + warp), c0 = line.start(w0), c1 = line.start(w0 + line.per_cta);
+    // every run of the CTA inside one item: its warps take units in turn (neighbours in memory at the same time)
+    // and are joined below. whole: and they are all of it
+    bool joint = false, whole = false;
     if (c1 > c0) {
         const long long first = s_first[0], end = first + s_cur[0].nt;
         joint = c1 <= end;
         whole = c0 == first && c1 == end;
     }
-    if (worker && lane == 0) work.tail[w0 + warp].u1 = 0;
+    int count = worker ? (int)(line.start(w0 + warp + 1) - u0) : 0;
+    const int step = joint ? line.per_cta : 1;
+    unsigned char* ring = pa_sm + warp * G::RING;
+    const uint32_t ring_a = smem_u32(ring);
+    PaCursor cur = PaCursor{0, 0, 0, 0, 0};
+    long long item0 = 0;
+    if (joint) {
+        cur = s_cur[0];
+        cur.t += warp;
+        const int units = (int)(c1 - c0);
+        count = worker && warp < units ? (units - warp + step - 1) / step : 0;
+    } else if (count > 0) {
+        cur = s_cur[warp];
+        item0 = s_first[warp];
+    }
+    const bool alone = whole && c1 - c0 == 1;
+    if (tid == 0) work.tail[blockIdx.x].ctas = 0;
 
     // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
     PaCursor nx = cur;
@@ -465,46 +606,47 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                 pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
                 ok = true;
             }
-            pa_next(a, pl, nx);
+            pa_next(a, pl, nx, step);
         }
         issued++;
     };
-    float ksq[ST - 1], vsq[ST - 1];
-    bool inq[ST - 1];
+    bool lead = false;
+    unsigned bytes = 0u, counts = 0u;  // counts: whether this lane's key counts, of the unit issued last in bit 0
     constexpr int LPR = HDP <= 64 ? 4 : HDP <= 128 ? 8 : 16, RPI = 32 / LPR;  // lanes per row, rows per step
     const int cc = (lane & (LPR - 1)) * 16, cr = lane / LPR;
     const int8_t* const kcol = a.kv.p.k + cc;
     const int8_t* const vcol = a.kv.p.v + cc;
-    auto issue = [&](int st) {  // copies of the unit that was looked up last
+    // tensor copies of the unit that was looked up last: K and its keys' scales (lane j copies and reads key j's),
+    // then V
+    auto issue_k = [&](int st) {
         if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
             paged_flag(kPagedErrPage);
             ok = false;
         }
-        if constexpr (TMA) {
-            // the scales of the units in flight wait in registers (lane j: key j)
-#pragma unroll
-            for (int i = 0; i + 1 < ST - 1; i++) {
-                ksq[i] = ksq[i + 1];
-                vsq[i] = vsq[i + 1];
-                inq[i] = inq[i + 1];
-            }
-            ksq[ST - 2] = vsq[ST - 2] = 0.0f;
-            inq[ST - 2] = ok;
-            const bool lead = ok && (lane & (pl.box - 1)) == 0;
-            const unsigned leads = __ballot_sync(0xffffffffu, lead);
-            if (lane == 0) mbar_expect_tx(&s_bar[warp][st], __popc(leads) * pl.box * (2 * HDP));
-            __syncwarp();
-            if (lead) {
-                const uint32_t dst = ring_a + st * G::STAGE + lane * HDP;
-                pa_tensor_copy(dst, &maps.k, h, slot, pg, &s_bar[warp][st]);
-                pa_tensor_copy(dst + G::VOFF, &maps.v, h, slot, pg, &s_bar[warp][st]);
-            }
-            if (ok) {
-                const long long so = (long long)pg * a.kv.p.spage_stride + (long long)slot * a.kv.p.spos_stride + hsoff;
-                ksq[ST - 2] = __ldg(a.kv.p.ks + so);
-                vsq[ST - 2] = __ldg(a.kv.p.vs + so);
-            }
-            return;
+        counts = counts << 1 | (ok ? 1u : 0u);
+        lead = ok && (lane & (pl.box - 1)) == 0;
+        bytes = __popc(__ballot_sync(0xffffffffu, lead)) * pl.box * HDP;
+        uint64_t* bar = &s_bar[warp][st][0];
+        if (lane == 0) mbar_expect_tx(bar, bytes);
+        __syncwarp();
+        if (lead) pa_tensor_copy(ring_a + st * G::STAGE + lane * HDP, &maps.k, h, slot, pg, bar, policy);
+        if (ok) {
+            const long long so = (long long)pg * a.kv.p.spage_stride + (long long)slot * a.kv.p.spos_stride + hsoff;
+            pa_copy_scale(ring_a + G::KOFF + st * 8 * TK + 4 * lane, a.kv.p.ks + so);
+            pa_copy_scale(ring_a + G::KOFF + st * 8 * TK + 4 * TK + 4 * lane, a.kv.p.vs + so);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto issue_v = [&](int st) {
+        uint64_t* bar = &s_bar[warp][st][1];
+        if (lane == 0) mbar_expect_tx(bar, bytes);
+        __syncwarp();
+        if (lead) pa_tensor_copy(ring_a + st * G::STAGE + G::VOFF + lane * HDP, &maps.v, h, slot, pg, bar, policy);
+    };
+    auto issue = [&](int st) {  // K, V and scales by cp.async
+        if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
+            paged_flag(kPagedErrPage);
+            ok = false;
         }
         const uint32_t base = ring_a + st * G::STAGE;
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
@@ -512,8 +654,8 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
         if (ok) {
             off = (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff;
             const long long so = (long long)pg * a.kv.p.spage_stride + (long long)slot * a.kv.p.spos_stride + hsoff;
-            pa_copy<4>(base + G::SOFF + 4 * lane, a.kv.p.ks + so);
-            pa_copy<4>(base + G::SOFF + 4 * TK + 4 * lane, a.kv.p.vs + so);
+            pa_copy_scale(base + G::SOFF + 4 * lane, a.kv.p.ks + so);
+            pa_copy_scale(base + G::SOFF + 4 * TK + 4 * lane, a.kv.p.vs + so);
         }
         if (lane == 0) *reinterpret_cast<unsigned*>(ring + st * G::STAGE + G::MOFF) = mask;
         if (pl.wide_copy) {
@@ -524,8 +666,8 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                 const long long o = __shfl_sync(0xffffffffu, off, row);
                 if (cc < hd && (all || ((mask >> row) & 1))) {
                     const uint32_t dst = base + G::at(row, cc / 16);
-                    pa_copy<16>(dst, kcol + o);
-                    pa_copy<16>(dst + G::VOFF, vcol + o);
+                    pa_copy<16>(dst, kcol + o, policy);
+                    pa_copy<16>(dst + G::VOFF, vcol + o, policy);
                 }
             }
         } else {
@@ -534,26 +676,56 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                 if (!((mask >> row) & 1)) continue;
                 for (int c = lane; c * 4 < hd; c += 32) {
                     const uint32_t dst = base + G::at(row, c / 4) + (c & 3) * 4;
-                    pa_copy<4>(dst, a.kv.p.k + o + c * 4);
-                    pa_copy<4>(dst + G::VOFF, a.kv.p.v + o + c * 4);
+                    pa_copy<4>(dst, a.kv.p.k + o + c * 4, policy);
+                    pa_copy<4>(dst + G::VOFF, a.kv.p.v + o + c * 4, policy);
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    lookup();
-#pragma unroll
-    for (int i = 0; i < ST - 1; i++) {
-        issue(i);
+    auto begin = [&] {  // copies of the first units
         lookup();
-    }
+#pragma unroll 1
+        for (int i = 0; i < (TMA ? ST : ST - 1); i++) {
+            if constexpr (TMA) {
+                issue_k(i);
+                issue_v(i);
+            } else {
+                issue(i);
+            }
+            lookup();
+        }
+    };
 
     // lane (g, t): query head g (and g + 8) as B fragments, bytes 4 t .. 4 t + 3 of every 16; of the results the
     // heads 2 t, 2 t + 1 (and 8 more), for which it keeps the reference, its share of the sum, and the dims 2 g,
     // 2 g + 1 of every 16
     uint32_t qf[NK][E][2];
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4];
-    bool fresh = true;
+    int acc[DIG ? ND : 1][NT][4];
+    int summed = 0;  // units in acc
+    // digits of this lane's columns: bytes 0 and 2, or 1 and 3, of heads 2 t, 2 t + 1 (up to 4 heads: of heads
+    // 2 (t % 2), + 1); all four of them (up to 8)
+    const uint32_t pick = HEADS <= 4 && t >= 2 ? 0x7351 : 0x6240;
+    const float weigh = HEADS <= 4 && t >= 2 ? 256.0f : 1.0f;
+    auto settle = [&] {  // o += what acc holds
+#pragma unroll
+        for (int d = 0; d < (DIG ? ND : 0); d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (HEADS <= 4) {
+                    o[d][0][j] += weigh * __fmaf_rn((float)acc[d][1][j], 65536.0f, (float)acc[d][0][j]);
+                } else {
+                    const float lo = __fmaf_rn((float)acc[d][1][j], 256.0f, (float)acc[d][0][j]);
+                    const float hi = __fmaf_rn((float)acc[d][NT - 1][j], 256.0f, (float)acc[d][NT - 2][j]);
+                    o[d][0][j] += __fmaf_rn(hi, 65536.0f, lo);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; i++) acc[d][i][j] = 0;
+            }
+        summed = 0;
+    };
+    bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
     int st = 0;
     uint32_t phase = 0u;
     const float up = __fmul_rn(a.scale, 1.44269504088896341f);
@@ -566,23 +738,31 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
             const int half = hd >> 1;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const int row = qb * ROWS + 8 * e + g;
+                const int row = qb * ROWS + 8 * e + (HEADS <= 4 ? g & 3 : g);
                 const bool live = row < group;
                 const float* q = a.Q + (size_t)cur.b * a.ldq + (size_t)(kvh * group + (live ? row : 0)) * hd;
                 const size_t tp = (size_t)(cur.len - 1) * half;
+                const bool rot = a.rope.cos_t != nullptr;
                 float4 x[2 * NK];
+                float2 c[2 * NK], sn[2 * NK];
                 float amax = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2 * NK; i++) {
                     int src = 4 * i + t;  // quad stored in slot 4 i + t
                     x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (!live || 4 * src >= hd) continue;
-                    if (a.rope.cos_t) {
+                    if (rot) {
                         src = rope_slot(2 * src, half) >> 1;  // its own inverse
-                        x[i] = rotate4(load4(q + 4 * src, false), a.rope.cos_t + tp, a.rope.sin_t + tp, src);
-                    } else {
-                        x[i] = load4(q + 4 * src, false);
+                        c[i] = load2(a.rope.cos_t + tp + 2 * src, pl.wide_q);
+                        sn[i] = load2(a.rope.sin_t + tp + 2 * src, pl.wide_q);
                     }
+                    x[i] = load4(q + 4 * src, pl.wide_q);
+                }
+                // the queries are on their way before the first copies fill the memory system's queues
+                if (e == 0 && n == 0) begin();
+#pragma unroll
+                for (int i = 0; i < 2 * NK; i++) {
+                    if (rot && live && 4 * (4 * i + t) < hd) x[i] = rotate4(x[i], c[i], sn[i]);
                     amax = fmaxf(amax, amax4(x[i]));
                 }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -599,21 +779,26 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
             }
+#pragma unroll
+            for (int d = 0; d < (DIG ? ND : 0); d++)
+#pragma unroll
+                for (int i = 0; i < NT; i++) acc[d][i][0] = acc[d][i][1] = acc[d][i][2] = acc[d][i][3] = 0;
+            summed = 0;
         }
-        // the next unit's copies go to the stage that the last iteration read
-        __syncwarp();
         bool in = false;
-        float kscale = 0.0f, vscale = 0.0f;
+        float kscale, vscale;
         if constexpr (TMA) {
-            in = inq[0];
-            kscale = ksq[0];
-            vscale = vsq[0];
-        }
-        issue(st == 0 ? ST - 1 : st - 1);
-        lookup();
-        if constexpr (TMA) {
-            if (!mbar_try_wait(&s_bar[warp][st], phase) && !pa_wait(&s_bar[warp][st], phase)) in = false;
+            in = (counts >> (ST - 1)) & 1u;
+            asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+            const float* sc = reinterpret_cast<const float*>(ring + G::KOFF + st * 8 * TK);
+            kscale = sc[lane];
+            vscale = in ? sc[TK + lane] : 0.0f;
+            if (!mbar_try_wait(&s_bar[warp][st][0], phase) && !pa_wait(&s_bar[warp][st][0], phase)) in = false;
         } else {
+            // the next unit's copies go to the stage that the last iteration read
+            __syncwarp();
+            issue(st == 0 ? ST - 1 : st - 1);
+            lookup();
             asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
             __syncwarp();
         }
@@ -630,7 +815,9 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                 vscale = in ? sc[TK + lane] : 0.0f;
             }
             const int ex = min(max((int)((__float_as_uint(vscale) >> 23) & 255u), 63), 253) - 127;
-            keys[lane] = in ? make_float4(kscale, 0.0f, (float)ex, vscale) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            // 0, or NaN where vs is not a number or infinite: so is the row then, whatever becomes of its weights
+            const float bias = __fsub_rn(vscale, vscale);
+            keys[lane] = in ? make_float4(kscale, bias, (float)ex, vscale) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         }
         __syncwarp();
 
@@ -670,69 +857,153 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                     }
             }
         }
-        float al[E][2];
+        if constexpr (TMA) {  // K is read: the unit ST ahead may take its place
+            __syncwarp();
+            issue_k(st);
+        }
+        if constexpr (DIG) {
+            // a weight too large for the reference, or sums near the end of 32 bits: both are rare
+            const bool high = top[0][0] > ref[0][0] + kPaMost || top[0][1] > ref[0][1] + kPaMost;
+            if (__any_sync(0xffffffffu, high) || summed == kPaFlush) {
+                settle();
 #pragma unroll
-        for (int e = 0; e < E; e++)
+                for (int j = 0; j < 2; j++) {
+                    float x = top[0][j];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = x > ref[0][j] + kPaMost ? x - kPaSet : ref[0][j];
+                    const float al = ex2(ref[0][j] - x);
+                    ref[0][j] = x;
+                    l[0][j] *= al;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float x = top[e][j];
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                x = fmaxf(ref[e][j], x - kPaShift);
-                al[e][j] = ex2(ref[e][j] - x);
-                ref[e][j] = x;
-                l[e][j] *= al[e][j];
-            }
-        // weights, transposed into B fragments: head g, keys 16 m + 2 t, + 1 and 8 later
-        uint32_t hi[NM][E][2], lo[NM][E][2];
-#pragma unroll
-        for (int m = 0; m < NM; m++)
-#pragma unroll
-            for (int e = 0; e < E; e++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float b0 = ex2(s[m][e][2 * i] - ref[e][0]), b1 = ex2(s[m][e][2 * i + 1] - ref[e][1]);
-                    l[e][0] += b0;
-                    l[e][1] += b1;
-                    const float w0 = b0 * vs[m][i], w1 = b1 * vs[m][i];
-                    const uint32_t ph = pa_pack(w0, w1);
-                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
-                    hi[m][e][i] = pa_transpose(ph);
-                    lo[m][e][i] = pa_transpose(pa_pack(w0 - hf.x, w1 - hf.y));
-                }
-        // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
-        // rows g of the tile, the odd ones rows g + 8
-#pragma unroll
-        for (int d = 0; d < ND; d += 2) {
-            float c[2][E][4];
-#pragma unroll
-            for (int m = 0; m < NM; m++) {
-                uint32_t v[4];
-                pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v);
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t vf[4] = {pa_half2<false>(v[2 * i]), pa_half2<true>(v[2 * i]),
-                                            pa_half2<false>(v[2 * i + 1]), pa_half2<true>(v[2 * i + 1])};
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        if (m == 0)
-                            pa_mma_f16(vf, hi[m][e], 0.0f, c[i][e]);
-                        else
-                            pa_mma_f16(vf, hi[m][e], c[i][e]);
-                        pa_mma_f16(vf, lo[m][e], c[i][e]);
+                    for (int d = 0; d < ND; d++) {
+                        o[d][0][j] *= al;
+                        o[d][0][2 + j] *= al;
                     }
                 }
             }
+            summed++;
+            // weights as integers; their bytes, transposed, are B fragments: column g (a digit of a head), keys
+            // 16 m + 2 t, + 8, + 1, + 9
+            uint32_t pf[NT][2];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int m = 0; m < NM; m++) {
+                uint32_t w[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float bj = ex2(s[m][0][2 * i + j] - ref[0][j]);
+                        l[0][j] += bj;
+                        w[i][j] = __float2uint_rn(bj * vs[m][i]);
+                    }
+                if (HEADS <= 4) {
+                    const uint32_t x0 = __byte_perm(w[0][0], w[1][0], pick), x1 = __byte_perm(w[0][1], w[1][1], pick);
+                    pf[0][m] = pa_transpose(__byte_perm(x0, x1, 0x5410));
+                    pf[1][m] = pa_transpose(__byte_perm(x0, x1, 0x7632));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {  // bytes 2 i, 2 i + 1
+                        const uint32_t sel = i == 0 ? 0x5140 : 0x7362;
+                        const uint32_t x0 = __byte_perm(w[0][0], w[1][0], sel), x1 = __byte_perm(w[0][1], w[1][1], sel);
+                        pf[2 * i][m] = pa_transpose(__byte_perm(x0, x1, 0x5410));
+                        pf[2 * i + 1][m] = pa_transpose(__byte_perm(x0, x1, 0x7632));
+                    }
+                }
+            }
+            if constexpr (TMA)
+                if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
+            // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
+            // rows g of the tile, the odd ones rows g + 8
+#pragma unroll
+            for (int d = 0; d < ND; d += 2) {
+                uint32_t v[NM][4];
+#pragma unroll
+                for (int m = 0; m < NM; m++)
+                    pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v[m]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t vf[4] = {__byte_perm(v[0][2 * i], v[0][2 * i + 1], 0x6240),
+                                            __byte_perm(v[0][2 * i], v[0][2 * i + 1], 0x7351),
+                                            __byte_perm(v[NM - 1][2 * i], v[NM - 1][2 * i + 1], 0x6240),
+                                            __byte_perm(v[NM - 1][2 * i], v[NM - 1][2 * i + 1], 0x7351)};
+#pragma unroll
+                    for (int n8 = 0; n8 < NT; n8++) pa_mma_s8u8(vf, pf[n8], acc[d + i][n8]);
+                }
+            }
+        } else {
+            float al[E][2];
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float x = top[e][j];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(ref[e][j], x - kPaShift);
+                    al[e][j] = ex2(ref[e][j] - x);
+                    ref[e][j] = x;
+                    l[e][j] *= al[e][j];
+                }
+            // weights, transposed into B fragments: head g, keys 16 m + 2 t, + 1 and 8 later
+            uint32_t hi[NM][E][2], lo[NM][E][2];
+#pragma unroll
+            for (int m = 0; m < NM; m++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
+                    for (int i = 0; i < 2; i++) {
+                        const float b0 = ex2(s[m][e][2 * i] - ref[e][0]), b1 = ex2(s[m][e][2 * i + 1] - ref[e][1]);
+                        l[e][0] += b0;
+                        l[e][1] += b1;
+                        const float w0 = b0 * vs[m][i], w1 = b1 * vs[m][i];
+                        const uint32_t ph = pa_pack(w0, w1);
+                        const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
+                        hi[m][e][i] = pa_transpose(ph);
+                        lo[m][e][i] = pa_transpose(pa_pack(w0 - hf.x, w1 - hf.y));
+                    }
+            if constexpr (TMA)
+                if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
+            // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
+            // rows g of the tile, the odd ones rows g + 8
+#pragma unroll
+            for (int d = 0; d < ND; d += 2) {
+                float c[2][E][4];
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    uint32_t v[4];
+                    pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const uint32_t vf[4] = {pa_half2<false>(v[2 * i]), pa_half2<true>(v[2 * i]),
+                                                pa_half2<false>(v[2 * i + 1]), pa_half2<true>(v[2 * i + 1])};
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            if (m == 0)
+                                pa_mma_f16(vf, hi[m][e], 0.0f, c[i][e]);
+                            else
+                                pa_mma_f16(vf, hi[m][e], c[i][e]);
+                            pa_mma_f16(vf, lo[m][e], c[i][e]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
+            }
+        }
+        if constexpr (TMA) {
+            __syncwarp();
+            issue_v(st);
+            lookup();
         }
         if (++st == ST) {
             st = 0;
@@ -740,11 +1011,19 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
         }
 
         const bool item_end = cur.t == cur.nt - 1;
-        if (!item_end && n + 1 < count) {
-            cur.t++;
+        if (n + 1 < count && (joint || !item_end)) {
+            cur.t += step;
             continue;
         }
         // the end of an item or of the run
+        if constexpr (DIG) {
+            settle();
+            if (HEADS <= 4)  // lanes t and t + 2 hold two digits each of the same heads
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[d][0][j] += __shfl_xor_sync(0xffffffffu, o[d][0][j], 2);
+        }
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
@@ -752,7 +1031,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
         const bool from_start = item0 >= u0;
-        if (from_start && item_end) {
+        if (joint ? alone : from_start && item_end) {
             const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
 #pragma unroll
             for (int e = 0; e < E; e++)
@@ -770,15 +1049,15 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
                         }
                 }
         } else {
-            if (from_start && lane == 0 && !whole)
-                work.tail[w0 + warp] = PaTail{item0, item0 + cur.nt, cur.b, cur.r};
             if (joint) break;  // o, ref and l stay in registers
+            tail = from_start;
             float* part = work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART;
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const int row = 8 * e + 2 * t + j;
+                    if (row >= ROWS) continue;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
                         *reinterpret_cast<float2*>(part + row * HDP + 16 * d + 2 * g) =
@@ -789,12 +1068,46 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
         }
         if (n + 1 < count) {
             item0 += cur.nt;
-            pa_next(a, pl, cur);
+            pa_next(a, pl, cur, 1);
             fresh = true;
         }
     }
-    if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (!joint || (whole && line.start(w0 + 1) == c1)) return;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // CTAs behind this one that hold parts of an item that ends at unit `end`
+    auto later = [&](long long end) { return (int)(line.worker(end - 1) / line.per_cta) - (int)blockIdx.x; };
+    if (!joint) {
+        // the items that this CTA's runs share: the warp where one starts joins its parts (warp 0 those of the
+        // item that came into the CTA), in place
+        __syncthreads();
+        if (c1 == c0) return;
+        const long long first = s_first[0], end0 = first + s_cur[0].nt;
+        for (int pass = warp == 0 ? 0 : 1; pass < 2; pass++) {
+            const bool head = pass == 0;
+            if (head ? first >= c0 : !tail) continue;
+            const long long end = head ? end0 : item0 + cur.nt;
+            const int own = (int)(w0 + warp) * 2 + (head ? 0 : 1);
+            int np = 1;
+            while (warp + np < line.per_cta && line.start(w0 + warp + np) < end) np++;
+            const PaCursor it = head ? s_cur[0] : cur;
+            const bool ends = !head && end <= c1;
+            if (!head && !ends && lane == 0)
+                work.tail[blockIdx.x] = PaTail{later(end), own, it.b, it.r, line.per_cta};
+            if (np == 1) continue;
+            const int qb = it.r % pl.qblocks, kvh = it.r / pl.qblocks;
+            auto slot_of = [&](int i) { return i == 0 ? own : (int)(w0 + warp + i) * 2; };
+            for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += PaSum<HDP, HEADS, TMA>::RB) {
+                PaSum<HDP, HEADS, TMA> sum;
+                const int rows = min(PaSum<HDP, HEADS, TMA>::RB, group - qb * ROWS - r0);
+                sum.add(work.part, r0, rows, np, 0, 1, slot_of);
+                if (ends)
+                    sum.finish(a.out + (size_t)it.b * a.ldo + (size_t)(kvh * group + qb * ROWS + r0) * hd, rows, hd);
+                else
+                    sum.store(work.part + (size_t)own * G::PART, r0, rows);
+            }
+        }
+        return;
+    }
+    if (alone) return;  // written
 
     // join the CTA's workers (their rings are free now)
     float* buf = reinterpret_cast<float*>(ring);
@@ -804,6 +1117,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = 8 * e + 2 * t + j;
+                if (row >= ROWS) continue;
                 if (count > 0)
 #pragma unroll
                     for (int d = 0; d < ND; d++)
@@ -816,13 +1130,18 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
     __syncthreads();
     const PaCursor c = s_cur[0];
     const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
-    float* part = work.part + ((size_t)w0 * 2 + (c0 == s_first[0] ? 1 : 0)) * G::PART;
+    const int own = (int)w0 * 2 + (c0 == s_first[0] ? 1 : 0);
+    float* part = work.part + (size_t)own * G::PART;
+    if (tid == 0 && !whole && c0 == s_first[0])
+        work.tail[blockIdx.x] = PaTail{later(s_first[0] + c.nt), own, c.b, c.r, line.per_cta};
     for (int i = tid; i < ROWS * HDP / 4; i += WARPS * 32) {
         const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
         float M = kPaLow, L = 0.0f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
         for (int w = 0; w < line.per_cta; w++)
             M = fmaxf(M, reinterpret_cast<const float*>(pa_sm + w * G::RING)[ROWS * HDP + 2 * row]);
+#pragma unroll 1
         for (int w = 0; w < line.per_cta; w++) {
             const float* wb = reinterpret_cast<const float*>(pa_sm + w * G::RING);
             const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
@@ -848,74 +1167,34 @@ __global__ void __launch_bounds__(PaCfg<HDP, E, TMA>::WARPS * 32, 1)
     }
 }
 
-// The items that start in one worker's run and end in another's: a CTA per
-// worker. The parts of an item are, in order, those of single workers at its
-// ends and one of every CTA inside it; warp w adds parts w, w + 8, ... for RB
-// query rows at a time (every load of a part in flight at once), then the
-// warps' sums are joined in shared memory.
+// The items that start in one CTA of the kernel above and end in a later one:
+// a CTA each. Warp w adds parts w, w + 8, ..., then the warps' sums are joined
+// in shared memory.
 constexpr int kPaJoinWarps = 8;
-template <int HDP, int E, bool TMA>
+template <int HDP, int HEADS, bool TMA>
 __global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, E, TMA>;
-    constexpr int ROWS = G::ROWS, NV = (HDP + 127) / 128, RB = HDP <= 128 ? 8 : 4;
+    using G = PaCfg<HDP, HEADS, TMA>;
+    using Sum = PaSum<HDP, HEADS, TMA>;
+    constexpr int ROWS = G::ROWS, NV = Sum::NV, RB = Sum::RB;
     __shared__ __align__(16) float s_o[kPaJoinWarps][RB][HDP];
     __shared__ float2 s_rl[kPaJoinWarps][RB];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
-    const long long wf = blockIdx.x;
     griddep_wait();
-    const PaLine line = *work.line;
-    if (wf >= line.workers) return;
-    const PaTail tail = work.tail[wf];
-    if (tail.u1 == 0) return;
-    const long long wl = line.worker(tail.u1 - 1);
-    const int per = line.per_cta, cf = (int)(wf / per), cl = (int)(wl / per);
-    auto inside = [&](long long c) { return line.start(c * per) >= tail.u0 && line.start((c + 1) * per) <= tail.u1; };
-    const int na = inside(cf) ? 1 : (int)(min(wl, (long long)cf * per + per - 1) - wf) + 1;
-    const int nm = max(0, cl - cf - 1), nb = cl == cf ? 0 : inside(cl) ? 1 : (int)(wl - (long long)cl * per) + 1;
-    const int np = na + nm + nb;
-    const int qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
+    const PaTail tail = work.tail[blockIdx.x];
+    if (tail.ctas == 0) return;
+    const int np = tail.ctas + 1, qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
+    auto slot_of = [&](int i) { return i == 0 ? tail.slot : ((int)blockIdx.x + i) * tail.per_cta * 2; };
     for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += RB) {
         const int rows = min(RB, group - qb * ROWS - r0);
-        float4 o[RB][NV];
-        float ref = kPaLow, l = 0.0f;  // of row lane % RB
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int d = 0; d < NV; d++) o[r][d] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = warp; i < np; i += kPaJoinWarps) {
-            const int w = i < na ? (int)wf + i : i < na + nm ? (cf + 1 + i - na) * per : cl * per + (i - na - nm);
-            const float* p = work.part + ((size_t)w * 2 + (i == 0 ? 1 : 0)) * G::PART;
-            const float2 rl = *reinterpret_cast<const float2*>(p + ROWS * HDP + 2 * (r0 + (lane & (RB - 1))));
-            float4 x[RB][NV];
-#pragma unroll
-            for (int r = 0; r < RB; r++)
-#pragma unroll
-                for (int d = 0; d < NV; d++)
-                    x[r][d] = r < rows && 128 * d + 4 * lane < HDP
-                                  ? *reinterpret_cast<const float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float nr = fmaxf(ref, rl.x), fa = ex2(ref - nr), fb = ex2(rl.x - nr);
-            l = __fmaf_rn(l, fa, rl.y * fb);
-            ref = nr;
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const float ga = __shfl_sync(0xffffffffu, fa, r), gb = __shfl_sync(0xffffffffu, fb, r);
-#pragma unroll
-                for (int d = 0; d < NV; d++) {
-                    o[r][d].x = __fmaf_rn(o[r][d].x, ga, x[r][d].x * gb);
-                    o[r][d].y = __fmaf_rn(o[r][d].y, ga, x[r][d].y * gb);
-                    o[r][d].z = __fmaf_rn(o[r][d].z, ga, x[r][d].z * gb);
-                    o[r][d].w = __fmaf_rn(o[r][d].w, ga, x[r][d].w * gb);
-                }
-            }
-        }
-        __syncthreads();  // the last row block's sums are read
+        Sum sum;
+        sum.add(work.part, r0, rows, np, warp, kPaJoinWarps, slot_of);
+        if (r0) __syncthreads();  // the last row block's sums are read
 #pragma unroll
         for (int r = 0; r < RB; r++)
 #pragma unroll
             for (int d = 0; d < NV; d++)
-                if (128 * d + 4 * lane < HDP) *reinterpret_cast<float4*>(&s_o[warp][r][128 * d + 4 * lane]) = o[r][d];
-        if (lane < RB) s_rl[warp][lane] = make_float2(ref, l);
+                if (128 * d + 4 * lane < HDP) *reinterpret_cast<float4*>(&s_o[warp][r][128 * d + 4 * lane]) = sum.o[r][d];
+        if (lane < RB) s_rl[warp][lane] = make_float2(sum.ref, sum.l);
         __syncthreads();
         const int used = min(np, kPaJoinWarps);
         for (int i = tid; i < rows * HDP; i += kPaJoinWarps * 32) {
@@ -947,13 +1226,12 @@ int sm_count() {
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
-template <int HDP, int E, bool TMA>
+template <int HDP, int HEADS, bool TMA>
 size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
-    const size_t workers = (size_t)ctas * PaCfg<HDP, E, TMA>::WARPS;
-    const size_t head = align16(sizeof(PaLine)), at = align16(workers * sizeof(PaTail));
-    if (w) *w = PaWork{reinterpret_cast<PaLine*>(base), reinterpret_cast<PaTail*>(base + head),
-                       reinterpret_cast<float*>(base + head + at)};
-    return head + at + workers * 2 * PaCfg<HDP, E, TMA>::PART * sizeof(float);
+    const size_t workers = (size_t)ctas * PaCfg<HDP, HEADS, TMA>::WARPS;
+    const size_t at = align16(ctas * sizeof(PaTail));
+    if (w) *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + at)};
+    return at + workers * 2 * PaCfg<HDP, HEADS, TMA>::PART * sizeof(float);
 }
 
 // Map of a cache array as [page][slot][kv head][dim], boxes of `box` slots of one head.
@@ -975,7 +1253,7 @@ int pa_map(CUtensorMap* m, int8_t* base, const PagedAttn& a, int box) {
     const cuuint32_t boxes[4] = {(cuuint32_t)a.hd, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
     const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn)(
         m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        a.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+        a.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_64B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
     return JYC_OK;
@@ -992,15 +1270,15 @@ bool pa_tensor_copies(const PagedAttn& a, bool aligned) {
            (p.page_size % 32 == 0 || (32 % p.page_size == 0 && p.page_size * a.hd % 128 == 0));
 }
 
-template <int HDP, int E, bool TMA>
+template <int HDP, int HEADS, bool TMA>
 int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
-    using G = PaCfg<HDP, E, TMA>;
+    using G = PaCfg<HDP, HEADS, TMA>;
     // the attribute belongs to the device
     static std::atomic<bool> ready[64];
     int dev = 0;
     JYC_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, E, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, HEADS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       G::SMEM));
         if (dev < 64) ready[dev].store(true, std::memory_order_release);
     }
@@ -1019,12 +1297,12 @@ int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s
         if (r != JYC_OK) return r;
     }
     PaWork w;
-    pa_work_bytes<HDP, E, TMA>(sms, static_cast<unsigned char*>(work), &w);
-    paged_attention_kernel<HDP, E, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, maps);
+    pa_work_bytes<HDP, HEADS, TMA>(sms, static_cast<unsigned char*>(work), &w);
+    paged_attention_kernel<HDP, HEADS, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, maps);
     JYC_LAUNCHED();
     if (tiles <= 1) return JYC_OK;  // an item is one unit: none is split
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas * G::WARPS);
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kPaJoinWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute at{};
@@ -1032,12 +1310,13 @@ int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, E, TMA>, a, pl, w));
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, HEADS, TMA>, a, pl, w));
     JYC_LAUNCHED();
     return JYC_OK;
 }
 
 bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
+bool aligned8(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t)q) & 7) == 0; }
 
 }  // namespace
 
@@ -1046,7 +1325,8 @@ int launch_paged_append(const float* K, const float* V, int ld, int rows, int KV
     const long long units = (long long)rows * KV * 2;
     if (units == 0) return JYC_OK;
     paged_append_kernel<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(K, V, ld, rows, KV, hd, row_seq, row_pos, kv, rope,
-                                                                    aligned16(K, ld) && aligned16(V, ld));
+                                                                    aligned16(K, ld) && aligned16(V, ld) &&
+                                                                        aligned8(rope.cos_t, rope.sin_t));
     JYC_LAUNCHED();
     return JYC_OK;
 }
@@ -1060,20 +1340,26 @@ int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, cons
     return JYC_OK;
 }
 
-// The instantiation of a shape: head size rounded up, two blocks of 8 query
-// heads per unit above 8, and how the rows are copied.
-#define PA_CASES(F, TMA, ...)                                                                   \
-    do {                                                                                        \
-        const bool many = H / KV > 8;                                                           \
-        if (hd <= 64) return many ? F<64, 2, TMA>(__VA_ARGS__) : F<64, 1, TMA>(__VA_ARGS__);    \
-        if (hd <= 128) return many ? F<128, 2, TMA>(__VA_ARGS__) : F<128, 1, TMA>(__VA_ARGS__); \
-        if (hd <= 192) return many ? F<192, 2, false>(__VA_ARGS__) : F<192, 1, false>(__VA_ARGS__); \
-        return many ? F<256, 2, false>(__VA_ARGS__) : F<256, 1, false>(__VA_ARGS__);            \
+// The instantiation of a shape: head size and query heads per unit rounded up,
+// and how the rows are copied.
+#define PA_CASES(F, TMA, ...)                                                                     \
+    do {                                                                                          \
+        const int G = H / KV;                                                                     \
+        if (hd <= 64) {                                                                           \
+            if (G <= 4) return F<64, 4, TMA>(__VA_ARGS__);                                        \
+            return G <= 8 ? F<64, 8, TMA>(__VA_ARGS__) : F<64, 16, TMA>(__VA_ARGS__);             \
+        }                                                                                         \
+        if (hd <= 128) {                                                                          \
+            if (G <= 4) return F<128, 4, TMA>(__VA_ARGS__);                                       \
+            return G <= 8 ? F<128, 8, TMA>(__VA_ARGS__) : F<128, 16, TMA>(__VA_ARGS__);           \
+        }                                                                                         \
+        if (hd <= 192) return G <= 8 ? F<192, 8, false>(__VA_ARGS__) : F<192, 16, false>(__VA_ARGS__); \
+        return G <= 8 ? F<256, 8, false>(__VA_ARGS__) : F<256, 16, false>(__VA_ARGS__);           \
     } while (0)
 
-template <int HDP, int E, bool TMA>
+template <int HDP, int HEADS, bool TMA>
 static size_t pa_workspace(int sms) {
-    return pa_work_bytes<HDP, E, TMA>(sms, nullptr, nullptr);
+    return pa_work_bytes<HDP, HEADS, TMA>(sms, nullptr, nullptr);
 }
 
 size_t paged_attention_workspace(int H, int KV, int hd) {
@@ -1090,6 +1376,7 @@ int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
     PaPlan pl{};
     pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
     pl.units_row = KV * pl.qblocks;
+    pl.wide_q = aligned16(a.Q, a.ldq) && aligned8(a.rope.cos_t, a.rope.sin_t);
     // n / d for n < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) < d <= 2^s, so the
     // error of n m / 2^(31+s) is below 2^-31 n < 1 / d at every n; m < 2^32
     int sh = 0;
