@@ -510,7 +510,12 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
     const int bs = min(B, tid * per), be = min(B, bs + per);
     long long mine = 0;
-    for (int b = bs; b < be; b++) mine += (pa_len(a, b) + TK - 1) / TK;
+    bool none = false;  // one of this CTA's share of sequences has no key
+    for (int b = bs; b < be; b++) {
+        const int len = pa_len(a, b);
+        mine += (len + TK - 1) / TK;
+        none |= len == 0 && b % gridDim.x == blockIdx.x;
+    }
     mine *= pl.units_row;
     long long incl = mine;
 #pragma unroll
@@ -519,7 +524,10 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
         if (lane >= o) incl += x;
     }
     if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
+    if (__syncthreads_or(none))  // rows of zeros
+        for (int b = blockIdx.x; b < B; b += gridDim.x)
+            if (pa_len(a, b) == 0)
+                for (int e = tid; e < a.H * hd; e += WARPS * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
     long long U = 0, ex = incl - mine;
     for (int w = 0; w < WARPS; w++) {
         if (w < warp) ex += s_scan[w];
@@ -551,10 +559,6 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             }
         }
     }
-    // sequences without a key: rows of zeros
-    for (int b = blockIdx.x; b < B; b += gridDim.x)
-        if (pa_len(a, b) == 0)
-            for (int e = tid; e < a.H * hd; e += WARPS * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
     __syncthreads();
 
     const bool worker = warp < line.per_cta;
@@ -684,7 +688,6 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto begin = [&] {  // copies of the first units
-        lookup();
 #pragma unroll 1
         for (int i = 0; i < (TMA ? ST : ST - 1); i++) {
             if constexpr (TMA) {
@@ -734,6 +737,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
         if (fresh) {
             // the item's query heads: rotated and quantised per head
             fresh = false;
+            if (n == 0) lookup();
             const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
             const int half = hd >> 1;
 #pragma unroll
