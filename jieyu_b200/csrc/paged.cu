@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 namespace jyc {
 
@@ -20,6 +21,38 @@ int* paged_error_word() {
     int* p = nullptr;
     if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_paged_err) != cudaSuccess) return nullptr;
     return p;
+}
+
+int sm_count() {
+    static std::atomic<int> sms[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+int max_dynamic_smem(const void* kernel, int bytes) {
+    // the attribute belongs to the kernel and the device: remembered for the first 64 devices, set again otherwise
+    struct Entry {
+        const void* kernel;
+        uint64_t devices;
+    };
+    static Entry done[32];
+    static std::mutex mu;
+    int dev = 0;
+    JYC_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    Entry* e = done;
+    while (e < done + 32 && e->kernel && e->kernel != kernel) e++;
+    if (e < done + 32 && e->kernel && dev < 64 && (e->devices >> dev & 1)) return JYC_OK;
+    JYC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (e < done + 32 && dev < 64) {
+        e->kernel = kernel;
+        e->devices |= 1ull << dev;
+    }
+    return JYC_OK;
 }
 
 namespace {
@@ -1217,17 +1250,6 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn
     }
 }
 
-// SMs of the current device (0: no device).
-int sm_count() {
-    static std::atomic<int> sms[64];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
-
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 template <int HDP, int HEADS, bool TMA>
@@ -1277,15 +1299,8 @@ bool pa_tensor_copies(const PagedAttn& a, bool aligned) {
 template <int HDP, int HEADS, bool TMA>
 int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
     using G = PaCfg<HDP, HEADS, TMA>;
-    // the attribute belongs to the device
-    static std::atomic<bool> ready[64];
-    int dev = 0;
-    JYC_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        JYC_CUDA(cudaFuncSetAttribute(paged_attention_kernel<HDP, HEADS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      G::SMEM));
-        if (dev < 64) ready[dev].store(true, std::memory_order_release);
-    }
+    if (int e = max_dynamic_smem(reinterpret_cast<const void*>(paged_attention_kernel<HDP, HEADS, TMA>), G::SMEM))
+        return e;
     const long long cap = (long long)a.kv.table_stride * a.kv.p.page_size, tiles = (cap + G::TK - 1) / G::TK;
     const long long items = (long long)a.kv.num_seqs * pl.units_row;
     // no more CTAs than the longest possible lengths have units for

@@ -28,6 +28,10 @@ constexpr int kPagedErrRope = 4;  // position behind the RoPE tables
 constexpr int kPagedErrWait = 8;  // a copy's bounded wait gave up
 
 int* paged_error_word();
+// SMs of the current device (0: no device).
+int sm_count();
+// The kernel's limit of dynamic shared memory on the current device, set once for each.
+int max_dynamic_smem(const void* kernel, int bytes);
 
 int launch_paged_append(const float* K, const float* V, int ld, int rows, int KV, int hd, const int* row_seq,
                         const int* row_pos, const PagedKV& kv, const PagedRope& rope, cudaStream_t s);
