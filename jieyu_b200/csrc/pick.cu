@@ -9,16 +9,20 @@
 // are the same in any order.
 //
 // A row belongs to a cluster of 1 to 8 CTAs that exchange through distributed
-// shared memory, so one launch serves one row or hundreds:
-//   greedy   the maximum, one pass.
-//   top-k up to 1024   every lane keeps four maxima of its part; the k-th
-//            largest of a CTA's maxima bounds the k-th largest logit from
-//            below, and the few tokens above the bound are sorted by one CTA,
-//            which ends the row alone.
-//   otherwise  a histogram of counts over (max - l) / T, whose bins bound the
-//            mass above them; the tokens of the bins where the border may lie
-//            are sorted (or split again while they are too many), then the
-//            kept weights are summed in index order.
+// shared memory, so one launch serves one row or hundreds. Nothing is sorted.
+//   1  the maximum (a greedy row ends here); every lane keeps four maxima.
+//   2  a bin of (max - l) / T such that the tokens up to it are few and hold the
+//      kept set: with top-k by the k-th of those maxima (as many logits are as
+//      large), with min-p by min_p itself, with top-p a guess that is checked.
+//      One pass puts those tokens, in index order, into pools (one per warp).
+//   3  pools of 4096 tokens in all or fewer: one CTA takes them and ends the row,
+//      finding each border by bisection over keys.
+//      More: a histogram over the bins bounds the running count or mass, the
+//      tokens of the one or two bins where the border may lie are ranked (or
+//      split again while they are too many), and the kept weights are summed
+//      in index order, warp by warp, then token by token where the draw falls.
+//   Rows without a filter, and rows whose pools overflow or miss the border, go
+//   through 3 over all their logits instead of the pools.
 // Floor: one read of the logits. Later passes find them in L2.
 #include <cooperative_groups.h>
 
@@ -35,8 +39,10 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
-constexpr int kPickList = 4096;      // tokens that one CTA sorts
-constexpr int kPickTopK = 1024;      // largest k of the short way
+constexpr int kPickList = 4096;      // tokens that one CTA ends a row with
+constexpr int kPickTopK = 1024;      // largest k bounded by maxima
+constexpr int kPickPool = 512;       // tokens of a warp's pool
+constexpr int kPickRank = 512;       // tokens of a border that are ranked
 constexpr int kPickBins = 1024;
 constexpr int kPickMaxCluster = 8;
 constexpr float kPickSpan = 40.0f;   // powers of two that the bins cover
@@ -53,14 +59,15 @@ __device__ __forceinline__ float pick_value(u64 comp) {
 
 struct PickShared {
     u64 list[kPickList];
-    u64 w[kPickTopK];
+    u64 pool[kPickWarps][kPickPool];
+    u64 w[kPickRank];
     uint32_t hist[kPickBins], tot[kPickBins];
     double pow2[64];                   // 2^(j / 64)
     u64 x[2][kPickMaxCluster];         // exchanges between CTAs, two turns
     u64 sums[kPickMaxCluster][kPickWarps];
     u64 red[kPickWarps];
     u64 tau;
-    uint32_t count;
+    uint32_t count, inside[kPickWarps];
     int b1, b2;
 };
 
@@ -73,6 +80,7 @@ struct PickRow {
     double c;               // log2(e) / T
     float bin_scale;
     int C, rank, turn;
+    int pooled;             // tokens in the warp's pool; -1: the passes go over all logits
     PickShared* s;
 
     // four logits at i, i + 1, ... < w1 (NaN behind the end)
@@ -90,7 +98,7 @@ struct PickRow {
     }
     // 2^t by 2^(j / 64) and the exponential series: |s| <= ln 2 / 128, remainder s^5 / 120 < 4e-14
     __device__ __forceinline__ u64 weight(float x) const {
-        if (x == mx) return (u64)kOne;
+        if (x == mx) return (u64)kOne;  // infinite ones too
         const double t = ((double)x - (double)mx) * c;
         if (!(t >= -40.0)) return 0ull;  // NaN and -inf too
         const double m = __fma_rn(t, 64.0, 0x1.8p52);
@@ -108,6 +116,25 @@ struct PickRow {
         if (x == mx) return 0;
         const float b = __fmul_rn(__fsub_rn(mx, x), bin_scale);
         return b < (float)(kPickBins - 1) ? (int)b : kPickBins - 1;
+    }
+    // f(logit, index, whether there is one) for the warp's tokens, in index order, by whole warps
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        const int lane = threadIdx.x & 31;
+        if (pooled >= 0) {
+            const u64* p = s->pool[threadIdx.x >> 5];
+            for (int i = lane; i - lane < pooled; i += 32) {
+                const u64 comp = i < pooled ? p[i] : 0ull;
+                f(pick_value(comp), pick_index(comp), i < pooled);
+            }
+            return;
+        }
+        for (int i = w0; i < w1; i += 128) {
+            float x[4];
+            load(i + 4 * lane, x);
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(x[j], i + 4 * lane + j, x[j] > -INFINITY);
+        }
     }
     __device__ void sync() const {
         if (C > 1)
@@ -170,24 +197,6 @@ __device__ __forceinline__ T pick_scan(T v, T* red) {
     return before + v;
 }
 
-// bitonic sort, descending; n a power of two
-__device__ void pick_sort(u64* a, int n) {
-    __syncthreads();
-    for (int k = 2; k <= n; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < n / 2; i += kPickThreads) {
-                const int lo = (i & ~(j - 1)) * 2 + (i & (j - 1)), hi = lo + j;
-                const u64 x = a[lo], y = a[hi];
-                if ((x < y) == ((lo & k) == 0)) {
-                    a[lo] = y;
-                    a[hi] = x;
-                }
-            }
-            __syncthreads();
-        }
-}
-__device__ __forceinline__ int pick_pow2(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
-
 // Appends comp to the CTA's list where `take` holds (whole warps call it); s->count counts on past the end.
 __device__ __forceinline__ void pick_append(PickShared* s, bool take, u64 comp) {
     const unsigned m = __ballot_sync(0xffffffffu, take);
@@ -196,26 +205,24 @@ __device__ __forceinline__ void pick_append(PickShared* s, bool take, u64 comp) 
     uint32_t at = 0u;
     if (lane == 0) at = atomicAdd(&s->count, (uint32_t)__popc(m));
     at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
-    if (take && at < kPickList) s->list[at] = comp;
+    if (take && at < kPickRank) s->list[at] = comp;
 }
 
-// The CTAs' lists joined in the first one's, when they fit. Returns their total (-1: too many), the same in
-// every CTA; the list is complete in CTA 0 after the next sync.
-__device__ int pick_collect(PickRow& r) {
-    __syncthreads();
-    const uint32_t mine = r.s->count;
+// The CTAs' lists (of `mine` tokens each) joined in the first one's, in the CTAs' order, when they are at most
+// `most`. Returns their total (-1: too many), the same in every CTA; the list is complete after the call.
+__device__ int pick_collect(PickRow& r, uint32_t mine, int most) {
     const u64* x = r.exchange(mine);
     u64 total = 0ull, before = 0ull;
     for (int i = 0; i < r.C; i++) {
         if (i < r.rank) before += x[i];
         total += x[i];
     }
-    if (total > (u64)kPickList) return -1;
-    if (r.rank > 0) {
+    if (total <= (u64)most && r.rank > 0) {
         u64* to = cg::this_cluster().map_shared_rank(r.s, 0)->list;
         for (uint32_t i = threadIdx.x; i < mine; i += kPickThreads) to[before + i] = r.s->list[i];
     }
-    return (int)total;
+    r.sync();
+    return total <= (u64)most ? (int)total : -1;
 }
 
 // Sums of the CTA's histograms in s->tot of every CTA.
@@ -237,8 +244,9 @@ __device__ void pick_total(PickRow& r) {
 }
 
 // Where the prefix of {comp >= tau0} ends whose metric (number of tokens, or mass) first reaches `target`:
-// the comp of its last token. The histogram of the logits' bins is in s->hist (this CTA's share).
-__device__ u64 pick_border(PickRow& r, bool by_mass, double target, u64 tau0) {
+// the comp of its last token. s->hist holds this CTA's histogram of the bins: tokens, or for a mass their
+// weights over the bin's largest, in units of 1 / unit.
+__device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit, u64 tau0) {
     PickShared* s = r.s;
     const int tid = threadIdx.x;
     int lo_bin = 0, hi_bin = kPickBins - 1, level = 0, shift = 0;
@@ -253,11 +261,12 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, u64 tau0) {
             const int b = 2 * tid + i;
             const double n = (double)s->tot[b];
             lo[i] = hi[i] = n;
-            if (by_mass) {
+            if (by_mass && n > 0.0) {
                 if (level == 0) {
-                    const double step = kPickSpan / kPickBins;
-                    hi[i] = n * exp2(-step * b) * kOne * (1.0 + 1e-4);
-                    lo[i] = b == kPickBins - 1 ? 0.0 : n * exp2(-step * (b + 1)) * kOne * (1.0 - 1e-4);
+                    // a token's share is rounded by half a unit and lies above 0.97; 1e-5: the fp32 bins and shares
+                    const double top = n / unit * exp2(-(double)kPickSpan / kPickBins * b) * kOne, e = 0.52 / unit + 1e-5;
+                    hi[i] = top * (1.0 + e);
+                    lo[i] = top * (1.0 - e);
                 } else {
                     const u64 top = chi - ((u64)b << shift), span = ((u64)1 << shift) - 1ull;
                     hi[i] = n * (double)r.weight(pick_value(top));
@@ -268,18 +277,17 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, u64 tau0) {
         double* red = reinterpret_cast<double*>(s->red);
         const double cl1 = pick_scan(lo[0] + lo[1], red) + above, cl0 = cl1 - lo[1];
         const double ch1 = pick_scan(hi[0] + hi[1], red) + above, ch0 = ch1 - hi[1];
-        if (tid == 0) s->b1 = s->b2 = kPickBins - 1;
+        if (tid == 0) {
+            s->b1 = s->b2 = kPickBins - 1;
+            s->count = 0u;
+        }
         __syncthreads();
         // sums of doubles may be off by a few parts in 2^53 per bin
         const double early = target * (1.0 - 1e-12), late = by_mass ? target * (1.0 + 1e-12) : target;
         if (ch1 >= early) atomicMin(&s->b1, ch0 >= early ? 2 * tid : 2 * tid + 1);
         if (cl1 >= late) atomicMin(&s->b2, cl0 >= late ? 2 * tid : 2 * tid + 1);
-        if (tid == 0) s->count = 0u;
         __syncthreads();
         const int b1 = s->b1, b2 = max(s->b2, s->b1);
-        u64 n = 0ull;
-        for (int b = b1 + tid; b <= b2; b += kPickThreads) n += s->tot[b];
-        n = pick_reduce(n, s->red, pick_add);
         const u64 chi1 = level == 0 ? ~0ull : chi - ((u64)b1 << shift);
         const u64 end = (u64)(b2 + 1) << shift;
         const u64 clo1 = level == 0 ? 0ull : chi - clo < end ? clo : chi - end + 1ull;
@@ -287,62 +295,42 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, u64 tau0) {
             lo_bin = b1;
             hi_bin = b2;
         }
-        const bool fits = n <= (u64)kPickList;
-        // what lies above the members, exactly; the members themselves, or their range
+        // what lies above the members, exactly; the members themselves, and their range
         u64 up = 0ull, first = ~0ull, last = 0ull;
-        for (int i = r.w0; i < r.w1; i += 128) {
-            float x[4];
-            r.load(i + 4 * (tid & 31), x);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const u64 comp = pick_comp(x[j], i + 4 * (tid & 31) + j);
-                bool in = x[j] > -INFINITY && comp >= tau0, over = false;
+        r.each([&](float x, int idx, bool is) {
+            const u64 comp = pick_comp(x, idx);
+            bool in = is && comp >= tau0;
+            if (in) {
+                const int b = r.bin(x);
+                const bool over = b < lo_bin || (b <= hi_bin && comp > chi1);
+                in = !over && b <= hi_bin && comp >= clo1;
+                if (over) up += by_mass ? r.weight(x) : 1ull;
                 if (in) {
-                    const int b = r.bin(x[j]);
-                    over = b < lo_bin || (b <= hi_bin && comp > chi1);
-                    in = !over && b <= hi_bin && comp >= clo1;
-                    if (over) up += by_mass ? r.weight(x[j]) : 1ull;
-                    if (in) {
-                        first = pick_min(first, comp);
-                        last = pick_max(last, comp);
-                    }
+                    first = pick_min(first, comp);
+                    last = pick_max(last, comp);
                 }
-                if (fits) pick_append(s, in, comp);
             }
-        }
-        above = (double)pick_sum(r, up);
-        if (fits) {
-            const int total = pick_collect(r);
-            r.sync();
+            pick_append(s, in, comp);
+        });
+        up = pick_sum(r, up);
+        above = (double)up;
+        const int total = pick_collect(r, s->count, kPickRank);
+        if (total >= 0) {
             if (r.rank == 0) {
-                const int size = pick_pow2(max(total, 1));
-                for (int i = total + tid; i < size; i += kPickThreads) s->list[i] = 0ull;
-                pick_sort(s->list, size);
-                // the first one at which the running metric reaches the target
-                const int per = (size + kPickThreads - 1) / kPickThreads, i0 = min(total, tid * per);
-                const int i1 = min(total, i0 + per);
-                u64 sum = 0ull;
-                for (int i = i0; i < i1; i++) sum += by_mass ? r.weight(pick_value(s->list[i])) : 1ull;
-                const u64 incl = pick_scan(sum, s->red);
-                u64 run = (u64)above + incl - sum;
-                if (tid == 0) s->b1 = max(total - 1, 0);
+                // the token up to which the running metric reaches the target, and before which it does not
+                const u64 mine = tid < total ? s->list[tid] : 0ull;
+                const u64 own = tid < total ? (by_mass ? r.weight(pick_value(mine)) : 1ull) : 0ull;
+                if (tid < kPickRank) s->w[tid] = own;
+                u64 lowest = pick_reduce(tid < total ? mine : ~0ull, s->red, pick_min);
+                u64 run = up;
+                for (int j = 0; j < total; j++)
+                    if (s->list[j] > mine) run += s->w[j];
+                if (tid == 0) s->tau = total ? lowest : tau0;
                 __syncthreads();
-                if (i1 > i0 && (double)run < target && (double)(run + sum) >= target) {
-                    int i = i0;
-                    for (; i < i1 - 1; i++) {
-                        run += by_mass ? r.weight(pick_value(s->list[i])) : 1ull;
-                        if ((double)run >= target) break;
-                    }
-                    atomicMin(&s->b1, i);
-                } else if (i1 > i0 && (double)run >= target) {
-                    atomicMin(&s->b1, i0);  // reached before: the first token, at least
-                }
+                const bool reached = tid < total && (double)(run + own) >= target;
+                if (reached && ((double)run < target || run == up)) s->tau = mine;
                 __syncthreads();
-                if (tid == 0) {
-                    const u64 tau = s->list[s->b1];
-                    for (int c = 0; c < r.C; c++)
-                        (r.C > 1 ? cg::this_cluster().map_shared_rank(s, c) : s)->tau = tau;
-                }
+                if (tid > 0 && tid < r.C) cg::this_cluster().map_shared_rank(s, tid)->tau = s->tau;
             }
             r.sync();
             return s->tau;
@@ -361,17 +349,12 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, u64 tau0) {
         while (((chi - clo) >> shift) >= (u64)kPickBins) shift++;
         for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
         __syncthreads();
-        for (int i = r.w0; i < r.w1; i += 128) {
-            float x[4];
-            r.load(i + 4 * (tid & 31), x);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const u64 comp = pick_comp(x[j], i + 4 * (tid & 31) + j);
-                if (!(x[j] > -INFINITY) || comp < tau0 || comp < clo || comp > chi) continue;
-                const int b = r.bin(x[j]);
-                if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->hist[(chi - comp) >> shift], 1u);
-            }
-        }
+        r.each([&](float x, int idx, bool is) {
+            const u64 comp = pick_comp(x, idx);
+            if (!is || comp < tau0 || comp < clo || comp > chi) return;
+            const int b = r.bin(x);
+            if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->hist[(chi - comp) >> shift], 1u);
+        });
     }
 }
 
@@ -380,58 +363,101 @@ __device__ __forceinline__ void pick_write(const PickArgs& a, int row, int id, f
     if (a.probs) a.probs[row] = p;
 }
 
-// CTA 0 of the row: `n` tokens in s->list, the top-k among them: filters, draw.
-__device__ void pick_short(const PickArgs& a, PickRow& r, int row, int n, int K, float P, double mp) {
+// CTA 0 of the row ends it: `n` tokens in s->list, in index order, that hold the kept set; `rest` is the mass of
+// the others. False if the top-p border lies among those.
+__device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K, float P, double mp, u64 rest) {
     PickShared* s = r.s;
     const int tid = threadIdx.x;
-    const int size = pick_pow2(n);
-    for (int i = n + tid; i < size; i += kPickThreads) s->list[i] = 0ull;
-    pick_sort(s->list, size);
-    n = min(n, K);
-    // two tokens per thread
-    u64 w[2], c[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        c[i] = 2 * tid + i < n ? s->list[2 * tid + i] : 0ull;
-        w[i] = 2 * tid + i < n ? r.weight(pick_value(c[i])) : 0ull;
+    u64 low = ~0ull;
+    for (int i = tid; i < n; i += kPickThreads) low = pick_min(low, s->list[i] >> 32);
+    const uint32_t least = (uint32_t)pick_reduce(low, s->red, pick_min);
+    const uint32_t most = f32_order_key(r.mx);
+    auto count = [&](uint32_t key) {  // tokens of keys at least `key`
+        int c = 0;
+        if (n <= kPickThreads) return __syncthreads_count(tid < n && (uint32_t)(s->list[tid] >> 32) >= key);
+        for (int i = tid; i < n; i += kPickThreads) c += (uint32_t)(s->list[i] >> 32) >= key;
+        return (int)pick_reduce((u64)c, s->red, pick_add);
+    };
+    auto mass = [&](uint32_t key) {
+        u64 m = 0ull;
+        for (int i = tid; i < n; i += kPickThreads)
+            if ((uint32_t)(s->list[i] >> 32) >= key) m += r.weight(pick_value(s->list[i]));
+        return pick_reduce(m, s->red, pick_add);
+    };
+    // kept: keys above tau, and the first `ties` (by index) equal to it
+    uint32_t tau = least;
+    u64 ties = ~0ull;
+    if (K < n) {
+        uint32_t lo = least, hi = most;  // the largest key that K tokens reach
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo + 1u) / 2u;
+            if (count(mid) >= K)
+                lo = mid;
+            else
+                hi = mid - 1u;
+        }
+        tau = lo;
+        ties = (u64)(K - (tau < most ? count(tau + 1u) : 0));
     }
-    u64 incl = pick_scan(w[0] + w[1], s->red);
-    const u64 M = pick_reduce(incl, s->red, pick_max);
-    const double need = P < 1.0f ? (double)P * (double)M : (double)~0ull;
-    const u64 before[2] = {incl - w[0] - w[1], incl - w[1]};
-    u64 kept = 0ull;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int at = 2 * tid + i;
-        const bool keep = w[i] > 0ull && (at == 0 || (double)before[i] < need) && (double)w[i] >= mp * kOne;
-        if (at < kPickTopK) s->w[at] = keep ? w[i] : 0ull;
-        kept += keep;
+    if (P < 1.0f) {
+        const u64 wt = r.weight(pick_value((u64)tau << 32)), over = tau < most ? mass(tau + 1u) : 0ull;
+        const u64 M = (ties == ~0ull ? mass(tau) : over + ties * wt) + rest;
+        const double need = (double)P * (double)M;
+        // the largest key above tau down to which the mass reaches `need`; else tau
+        if (tau < most && (double)over >= need) {
+            uint32_t lo = tau + 1u, hi = most;
+            while (lo < hi) {
+                const uint32_t mid = lo + (hi - lo + 1u) / 2u;
+                if ((double)mass(mid) >= need)
+                    lo = mid;
+                else
+                    hi = mid - 1u;
+            }
+            tau = lo;
+            ties = ~0ull;
+        } else if ((double)(M - rest) < need) {
+            return false;
+        }
+        const u64 w = r.weight(pick_value((u64)tau << 32)), above = tau < most ? mass(tau + 1u) : 0ull;
+        u64 m = w ? (u64)fmax(0.0, (need - (double)above) / (double)w) : 1ull;
+        m = m > 1ull ? m - 1ull : 1ull;
+        while (m < ties && m < (u64)n && (double)(above + m * w) < need) m++;
+        ties = pick_min(ties, m);
     }
-    const int m = (int)pick_reduce(kept, s->red, pick_add);  // they are the first m
-    // in index order
-    const int msize = pick_pow2(m);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int at = 2 * tid + i;
-        if (at < msize) s->list[at] = at < m ? (c[i] << 32 | (u64)at) : 0ull;
-    }
-    pick_sort(s->list, msize);
-    u64 ord[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        ord[i] = 2 * tid + i < m ? s->list[2 * tid + i] : 0ull;
-        w[i] = 2 * tid + i < m ? s->w[(uint32_t)ord[i]] : 0ull;
-    }
-    incl = pick_scan(w[0] + w[1], s->red);
-    const u64 S = pick_reduce(incl, s->red, pick_max);
+    // sums of the kept weights in index order; a thread's tokens lie side by side
+    const int per = (n + kPickThreads - 1) / kPickThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    u64 equal = 0ull;
+    for (int i = i0; i < i1; i++) equal += (uint32_t)(s->list[i] >> 32) == tau;
+    const u64 seen0 = pick_scan(equal, s->red) - equal;
+    auto kept = [&](int i, u64& seen) -> u64 {
+        const uint32_t k = (uint32_t)(s->list[i] >> 32);
+        if (k < tau || (k == tau && seen++ >= ties)) return 0ull;
+        const u64 w = r.weight(pick_value(s->list[i]));
+        return (double)w >= mp * kOne ? w : 0ull;
+    };
+    u64 sum = 0ull, seen = seen0;
+    for (int i = i0; i < i1; i++) sum += kept(i, seen);
+    u64 run = pick_scan(sum, s->red);
+    const u64 S = pick_reduce(run, s->red, pick_max);
+    run -= sum;
+    // the first token whose running sum passes the target; the last kept one if none does
     const double target = (double)a.u[row] * (double)S;
-    u64 run = incl - w[0] - w[1];
-    const bool inside = !((double)run > target) && ((double)incl > target || incl == S);
-    if (w[0] > 0ull && (inside || (run == 0ull && (double)run > target))) {
-        int i = 0;
-        if (w[1] > 0ull && !((double)(run + w[0]) > target)) i = 1;
-        pick_write(a, row, pick_index(ord[i] >> 32), (float)((double)w[i] / (double)S));
+    const bool inside = !((double)run > target) && ((double)(run + sum) > target || run + sum == S);
+    if (sum > 0ull && (inside || (run == 0ull && (double)run > target))) {
+        u64 got = 0ull;
+        int id = -1;
+        seen = seen0;
+        for (int i = i0; i < i1; i++) {
+            const u64 w = kept(i, seen);
+            if (w == 0ull) continue;
+            run += w;
+            got = w;
+            id = pick_index(s->list[i]);
+            if ((double)run > target) break;
+        }
+        pick_write(a, row, id, (float)((double)got / (double)S));
     }
+    return true;
 }
 
 __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C, int chunk) {
@@ -487,51 +513,137 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     r.c = 1.44269504088896340736 / (double)Tf;
     r.bin_scale = (float)(r.c * (kPickBins / (double)kPickSpan));
 
-    if (K > 0 && K <= kPickTopK && K < V) {
-        // the k-th largest of this CTA's maxima: at least k logits are as large
+    r.pooled = -1;
+    const bool by_k = K > 0 && K < V, by_p = P < 1.0f;
+    // the last bin whose tokens go to the pools (-1: no pools)
+    int most = -1;
+    const bool bound_k = by_k && K <= kPickTopK;
+    if (bound_k || (by_p && !by_k)) {
+        // enough of the CTA's maxima: K of them (at least K logits are as large), or all but a few, down to 2^-24
+        for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++) s->list[4 * tid + j] = (u64)f32_order_key(m4[j] + 0.0f) << 32;
-        pick_sort(s->list, 4 * kPickThreads);
-        u64 bound = s->list[K - 1];
-        const u64* b = r.exchange(bound);
-        for (int i = 0; i < C; i++) bound = pick_max(bound, b[i]);
+        for (int j = 0; j < 4; j++)
+            if (m4[j] > -INFINITY) atomicAdd(&s->hist[r.bin(m4[j])], 1u);
+        if (tid == 0) s->b1 = kPickBins - 1;
+        __syncthreads();
+        const uint32_t n0 = s->hist[2 * tid], n1 = s->hist[2 * tid + 1];
+        const u64 c = pick_scan((u64)n0 + n1, s->red), enough = bound_k ? K : 4 * kPickThreads * 15 / 16;
+        if (c >= enough) atomicMin(&s->b1, c - n1 >= enough ? 2 * tid : 2 * tid + 1);
+        __syncthreads();
+        u64 b = s->b1;
+        if (bound_k) {
+            const u64* e = r.exchange(b);
+            for (int i = 0; i < C; i++) b = pick_min(b, e[i]);
+        } else {
+            b = pick_min(b, kPickBins * 24 / 40);
+            const u64* e = r.exchange(b);  // the same for all
+            for (int i = 0; i < C; i++) b = pick_max(b, e[i]);
+        }
+        most = (int)b;
+    } else if (!by_k && mp > 0x1p-38) {
+        most = min(kPickBins - 1, (int)(-log2(mp) * (kPickBins / (double)kPickSpan) * (1.0 + 1e-5)) + 1);
+    }
+    u64 rest = 0ull;
+    if (most >= 0) {
+        // tokens of bins up to `most` into the warp's pool, in index order; the others' mass for top-p
+        int n = 0;
+        const bool sums = by_p && !by_k;
         for (int i = r.w0; i < r.w1; i += 128) {
             float q[4];
             r.load(i + 4 * lane, q);
+            unsigned mine = 0u;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const u64 comp = pick_comp(q[j], i + 4 * lane + j);
-                pick_append(s, q[j] > -INFINITY && comp >= bound, comp);
+                if (!(q[j] > -INFINITY)) continue;
+                if (r.bin(q[j]) <= most)
+                    mine |= 1u << j;
+                else if (sums)
+                    rest += r.weight(q[j]);
             }
+            if (!__any_sync(0xffffffffu, mine != 0u)) continue;
+            const int own = __popc(mine);
+            int at = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += y;
+            }
+            const int all = __shfl_sync(0xffffffffu, at, 31);
+            at += n - own;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (mine >> j & 1u) {
+                    if (at < kPickPool) s->pool[warp][at] = pick_comp(q[j], i + 4 * lane + j);
+                    at++;
+                }
+            n += all;
         }
-        const int n = pick_collect(r);
-        r.sync();
-        if (n >= 0) {
-            if (r.rank == 0) pick_short(a, r, row, n, K, P, mp);
-            return;
+        // all of them to CTA 0, when they are few
+        if (lane == 0) s->inside[warp] = (uint32_t)n;
+        __syncthreads();
+        uint32_t before = 0u, total = 0u, largest = 0u;
+        for (int i = 0; i < kPickWarps; i++) {
+            const uint32_t c = s->inside[i];
+            if (i < warp) before += c;
+            total += c;
+            largest = max(largest, c);
+        }
+        const bool fits = largest <= kPickPool && total <= kPickList;
+        if (fits)
+            for (int i = lane; i < n; i += 32) s->list[before + i] = s->pool[warp][i];
+        __syncthreads();
+        if (sums) rest = pick_sum(r, rest);
+        const int found = pick_collect(r, fits ? total : kPickList + 1u, kPickList);
+        if (found >= 0) {
+            if (tid == 0) s->tau = 1ull;
+            bool done = true;
+            if (r.rank == 0) done = pick_short(a, r, row, found, by_k ? K : found, P, mp, rest);
+            if (!sums) return;
+            const u64* e = r.exchange(done ? 1ull : 0ull);
+            if (e[0]) return;
+        } else {
+            // pools that are too many for one CTA serve the passes below
+            const u64* e = r.exchange(largest);
+            u64 l = 0ull;
+            for (int i = 0; i < C; i++) l = pick_max(l, e[i]);
+            if (l <= (u64)kPickPool) r.pooled = n;
         }
     }
 
+    if (r.pooled < 0) rest = 0ull;
+    const double unit = (double)(1u << (V <= 1 << 17 ? 14 : 11));  // V of them fit 32 bits
     u64 tau = 0ull;
-    const bool by_k = K > 0 && K < V, by_p = P < 1.0f;
     for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); pass++) {
-        // histogram of the logits' bins among {comp >= tau}, and their mass for top-p
+        // histogram of the bins among {comp >= tau}: tokens, or for top-p their weights over the bin's largest, and
+        // the mass
         for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
         __syncthreads();
         u64 mass = 0ull;
-        for (int i = r.w0; i < r.w1; i += 128) {
-            float q[4];
-            r.load(i + 4 * lane, q);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (!(q[j] > -INFINITY) || pick_comp(q[j], i + 4 * lane + j) < tau) continue;
-                atomicAdd(&s->hist[r.bin(q[j])], 1u);
-                if (pass == 1) mass += r.weight(q[j]);
+        const float up = kPickSpan / kPickBins;
+        r.each([&](float x, int idx, bool is) {
+            if (!is || pick_comp(x, idx) < tau) return;
+            const int b = r.bin(x);
+            uint32_t n = 1u;
+            if (pass == 1) {
+                const u64 w = r.weight(x);
+                mass += w;
+                n = __float2uint_rn((float)w * (exp2f(up * (float)b) * (float)(unit / kOne)));
+            }
+            if (n) atomicAdd(&s->hist[b], n);
+        });
+        double target = (double)K;
+        if (pass == 1) {
+            const u64 M = pick_sum(r, mass);
+            target = (double)P * (double)(M + rest);
+            if (r.pooled >= 0 && (double)M < target) {  // the border is not in the pools: over all logits
+                r.pooled = -1;
+                rest = 0ull;
+                pass--;
+                continue;
             }
         }
-        double target = (double)K;
-        if (pass == 1) target = (double)P * (double)pick_sum(r, mass);
-        tau = pick_border(r, pass == 1, target, tau);
+        tau = pick_border(r, pass == 1, target, unit, tau);
     }
 
     // sums of the kept weights by warp, in index order
@@ -541,12 +653,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         return (double)w >= mp * kOne ? w : 0ull;
     };
     u64 sum = 0ull;
-    for (int i = r.w0; i < r.w1; i += 128) {
-        float q[4];
-        r.load(i + 4 * lane, q);
-#pragma unroll
-        for (int j = 0; j < 4; j++) sum += kept(q[j], i + 4 * lane + j);
-    }
+    r.each([&](float x, int idx, bool is) { sum += is ? kept(x, idx) : 0ull; });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane < C) (C > 1 ? cg::this_cluster().map_shared_rank(s, lane) : s)->sums[r.rank][warp] = sum;
@@ -563,12 +670,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     if (sum == 0ull || !(inside || (before == 0ull && (double)before > target))) return;
     int id = -1;
     u64 got = 0ull;
-    for (int i = r.w0; i < r.w1; i += 128) {
-        float q[4];
-        r.load(i + 4 * lane, q);
+    const int step = r.pooled >= 0 ? 32 : 128, end = r.pooled >= 0 ? r.pooled : r.w1;
+    for (int i = r.pooled >= 0 ? 0 : r.w0; i < end; i += step) {
+        float q[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        int first = i + 4 * lane;
+        if (r.pooled < 0) {
+            r.load(first, q);
+        } else if (i + lane < end) {
+            q[0] = pick_value(s->pool[warp][i + lane]);
+            first = pick_index(s->pool[warp][i + lane]);
+        }
         u64 w[4], own = 0ull;
 #pragma unroll
-        for (int j = 0; j < 4; j++) own += w[j] = kept(q[j], i + 4 * lane + j);
+        for (int j = 0; j < 4; j++) own += w[j] = kept(q[j], first + j);
         u64 incl = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -584,7 +698,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         for (int j = 0; j < 4; j++) {
             if (w[j] == 0ull || passed) continue;
             run += w[j];
-            mine = i + 4 * lane + j;
+            mine = first + j;
             mw = w[j];
             passed = (double)run > target;
         }
