@@ -41,7 +41,8 @@ typedef unsigned long long u64;
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 constexpr int kPickList = 4096;      // tokens that one CTA ends a row with
 constexpr int kPickTopK = 1024;      // largest k bounded by maxima
-constexpr int kPickPool = 512;       // tokens of a warp's pool
+constexpr int kPickPool = 2048;      // tokens of a warp's pool
+constexpr int kPickPairs = 256;      // tokens whose top-p is decided by comparing all pairs
 constexpr int kPickRank = 512;       // tokens of a border that are ranked
 constexpr int kPickBins = 1024;
 constexpr int kPickMaxCluster = 8;
@@ -59,7 +60,10 @@ __device__ __forceinline__ float pick_value(u64 comp) {
 
 struct PickShared {
     u64 list[kPickList];
-    u64 pool[kPickWarps][kPickPool];
+    union {
+        uint16_t pool[kPickWarps][kPickPool];  // positions in the warp's part (at most 2^16 logits)
+        u64 top[kPickTopK];                    // the top-k, when one CTA ends the row
+    };
     u64 w[kPickRank];
     uint32_t hist[kPickBins], tot[kPickBins];
     double pow2[64];                   // 2^(j / 64)
@@ -77,7 +81,7 @@ struct PickRow {
     int V, v0, v1, w0, w1;  // the CTA's part, the warp's part
     bool vec;
     float mx;
-    double c;               // log2(e) / T
+    double c, mxc;          // log2(e) / T, and mx times that
     float bin_scale;
     int C, rank, turn;
     int pooled;             // tokens in the warp's pool; -1: the passes go over all logits
@@ -96,20 +100,22 @@ struct PickRow {
             for (int j = 0; j < 4; j++) x[j] = i + j < w1 ? __ldg(l + i + j) : __int_as_float(0x7FC00000);
         }
     }
-    // 2^t by 2^(j / 64) and the exponential series: |s| <= ln 2 / 128, remainder s^5 / 120 < 4e-14
-    __device__ __forceinline__ u64 weight(float x) const {
-        if (x == mx) return (u64)kOne;  // infinite ones too
-        const double t = ((double)x - (double)mx) * c;
-        if (!(t >= -40.0)) return 0ull;  // NaN and -inf too
+    // The weight of x in units of 2^-42, a whole number. 2^t by 2^(j / 64) and the series of 2^f: |f| <= 1 / 128,
+    // remainder (f ln 2)^5 / 120 < 4e-14
+    __device__ __forceinline__ double weight_d(float x) const {
+        const double t = __fma_rn((double)x, c, -mxc);
         const double m = __fma_rn(t, 64.0, 0x1.8p52);
         const int n = __double2loint(m);
-        const double s1 = __fma_rn(m - 0x1.8p52, -1.0 / 64.0, t) * 0.693147180559945309417;
-        double p = __fma_rn(s1, 1.0 / 24.0, 1.0 / 6.0);
-        p = __fma_rn(p, s1, 0.5);
-        p = __fma_rn(p, s1, 1.0);
-        p = __fma_rn(p, s1, 1.0) * s->pow2[n & 63];
-        const double q = __hiloint2double(__double2hiint(p) + (((n >> 6) + 42) << 20), __double2loint(p));
-        return (u64)__double_as_longlong(q + 0x1p52) & 0xFFFFFFFFFFFFFull;
+        const double f = __fma_rn(m - 0x1.8p52, -1.0 / 64.0, t);
+        double p = __fma_rn(f, 0.00961812910762847716, 0.0555041086648215800);
+        p = __fma_rn(p, f, 0.240226506959100712);
+        p = __fma_rn(p, f, 0.693147180559945309);
+        p = __fma_rn(p, f, 1.0) * s->pow2[n & 63];
+        const double q = __hiloint2double(__double2hiint(p) + ((n & ~63) << 14) + (42 << 20), __double2loint(p));
+        return t >= -40.0 ? (q + 0x1p52) - 0x1p52 : 0.0;  // 0 for NaN and -inf too
+    }
+    __device__ __forceinline__ u64 weight(float x) const {
+        return x == mx ? (u64)kOne : (u64)weight_d(x);  // the maximum may be infinite
     }
     // bin of a logit above -inf: larger logits never lie in a later bin
     __device__ __forceinline__ int bin(float x) const {
@@ -122,10 +128,10 @@ struct PickRow {
     __device__ __forceinline__ void each(F f) const {
         const int lane = threadIdx.x & 31;
         if (pooled >= 0) {
-            const u64* p = s->pool[threadIdx.x >> 5];
+            const uint16_t* p = s->pool[threadIdx.x >> 5];
             for (int i = lane; i - lane < pooled; i += 32) {
-                const u64 comp = i < pooled ? p[i] : 0ull;
-                f(pick_value(comp), pick_index(comp), i < pooled);
+                const int idx = w0 + (i < pooled ? p[i] : 0);
+                f(i < pooled ? __ldg(l + idx) : -INFINITY, idx, i < pooled);
             }
             return;
         }
@@ -298,13 +304,14 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         // what lies above the members, exactly; the members themselves, and their range
         u64 up = 0ull, first = ~0ull, last = 0ull;
         r.each([&](float x, int idx, bool is) {
+            const int b = is ? r.bin(x) : kPickBins;
+            bool in = b <= hi_bin;
+            if (!__any_sync(0xffffffffu, in)) return;
             const u64 comp = pick_comp(x, idx);
-            bool in = is && comp >= tau0;
             if (in) {
-                const int b = r.bin(x);
-                const bool over = b < lo_bin || (b <= hi_bin && comp > chi1);
-                in = !over && b <= hi_bin && comp >= clo1;
-                if (over) up += by_mass ? r.weight(x) : 1ull;
+                const bool over = b < lo_bin || comp > chi1;
+                in = !over && comp >= clo1 && comp >= tau0;
+                if (over && comp >= tau0) up += by_mass ? r.weight(x) : 1ull;
                 if (in) {
                     first = pick_min(first, comp);
                     last = pick_max(last, comp);
@@ -368,8 +375,9 @@ __device__ __forceinline__ void pick_write(const PickArgs& a, int row, int id, f
 __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K, float P, double mp, u64 rest) {
     PickShared* s = r.s;
     const int tid = threadIdx.x;
+    const u64* list = s->list;
     u64 low = ~0ull;
-    for (int i = tid; i < n; i += kPickThreads) low = pick_min(low, s->list[i] >> 32);
+    for (int i = tid; i < n; i += kPickThreads) low = pick_min(low, list[i] >> 32);
     const uint32_t least = (uint32_t)pick_reduce(low, s->red, pick_min);
     const uint32_t most = f32_order_key(r.mx);
     auto count = [&](uint32_t key) {  // tokens of keys at least `key`
@@ -381,7 +389,7 @@ __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K,
     auto mass = [&](uint32_t key) {
         u64 m = 0ull;
         for (int i = tid; i < n; i += kPickThreads)
-            if ((uint32_t)(s->list[i] >> 32) >= key) m += r.weight(pick_value(s->list[i]));
+            if ((uint32_t)(list[i] >> 32) >= key) m += r.weight(pick_value(list[i]));
         return pick_reduce(m, s->red, pick_add);
     };
     // kept: keys above tau, and the first `ties` (by index) equal to it
@@ -399,7 +407,40 @@ __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K,
         tau = lo;
         ties = (u64)(K - (tau < most ? count(tau + 1u) : 0));
     }
-    if (P < 1.0f) {
+    if (K < n && K <= kPickTopK) {  // on with the top-k alone, in index order
+        const int per = (n + kPickThreads - 1) / kPickThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+        u64 both = 0ull;  // keys above tau, keys equal to it
+        for (int i = i0; i < i1; i++) {
+            const uint32_t k = (uint32_t)(list[i] >> 32);
+            both += ((u64)(k > tau) << 32) + (k == tau);
+        }
+        const u64 before = pick_scan(both, s->red) - both;
+        uint32_t above = (uint32_t)(before >> 32), equal = (uint32_t)before;
+        for (int i = i0; i < i1; i++) {
+            const uint32_t k = (uint32_t)(list[i] >> 32);
+            if (k > tau || (k == tau && equal < ties)) s->top[above + min((u64)equal, ties)] = list[i];
+            above += k > tau;
+            equal += k == tau;
+        }
+        __syncthreads();
+        list = s->top;
+        n = K;
+        ties = ~0ull;
+    }
+    u64 bar = 0ull;  // comps from here on, as far as decided below
+    if (P < 1.0f && n <= kPickPairs) {
+        // the mass in front of each token, over all pairs
+        const u64 mine = tid < n ? list[tid] : 0ull, own = tid < n ? r.weight(pick_value(mine)) : 0ull;
+        if (tid < n) s->w[tid] = own;
+        const u64 M = pick_reduce(own, s->red, pick_add);
+        const double need = (double)P * (double)(M + rest);
+        if ((double)M < need) return false;
+        u64 front = 0ull;
+        if (tid < n)
+            for (int j = 0; j < n; j++) front += list[j] > mine ? s->w[j] : 0ull;
+        bar = pick_reduce(tid < n && (front == 0ull || (double)front < need) ? mine : ~0ull, s->red, pick_min);
+        tau = 0u;
+    } else if (P < 1.0f) {
         const u64 wt = r.weight(pick_value((u64)tau << 32)), over = tau < most ? mass(tau + 1u) : 0ull;
         const u64 M = (ties == ~0ull ? mass(tau) : over + ties * wt) + rest;
         const double need = (double)P * (double)M;
@@ -426,13 +467,17 @@ __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K,
     }
     // sums of the kept weights in index order; a thread's tokens lie side by side
     const int per = (n + kPickThreads - 1) / kPickThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    u64 equal = 0ull;
-    for (int i = i0; i < i1; i++) equal += (uint32_t)(s->list[i] >> 32) == tau;
-    const u64 seen0 = pick_scan(equal, s->red) - equal;
+    u64 seen0 = 0ull;
+    if (ties != ~0ull) {
+        u64 equal = 0ull;
+        for (int i = i0; i < i1; i++) equal += (uint32_t)(list[i] >> 32) == tau;
+        seen0 = pick_scan(equal, s->red) - equal;
+    }
     auto kept = [&](int i, u64& seen) -> u64 {
-        const uint32_t k = (uint32_t)(s->list[i] >> 32);
-        if (k < tau || (k == tau && seen++ >= ties)) return 0ull;
-        const u64 w = r.weight(pick_value(s->list[i]));
+        const u64 c = list[i];
+        const uint32_t k = (uint32_t)(c >> 32);
+        if (k < tau || c < bar || (k == tau && seen++ >= ties)) return 0ull;
+        const u64 w = r.weight(pick_value(c));
         return (double)w >= mp * kOne ? w : 0ull;
     };
     u64 sum = 0ull, seen = seen0;
@@ -452,7 +497,7 @@ __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K,
             if (w == 0ull) continue;
             run += w;
             got = w;
-            id = pick_index(s->list[i]);
+            id = pick_index(list[i]);
             if ((double)run > target) break;
         }
         pick_write(a, row, id, (float)((double)got / (double)S));
@@ -511,6 +556,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     }
     r.mx = pick_value(top);
     r.c = 1.44269504088896340736 / (double)Tf;
+    r.mxc = (double)r.mx * r.c;
     r.bin_scale = (float)(r.c * (kPickBins / (double)kPickSpan));
 
     r.pooled = -1;
@@ -518,8 +564,18 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     // the last bin whose tokens go to the pools (-1: no pools)
     int most = -1;
     const bool bound_k = by_k && K <= kPickTopK;
-    if (bound_k || (by_p && !by_k)) {
-        // enough of the CTA's maxima: K of them (at least K logits are as large), or all but a few, down to 2^-24
+    if (by_p && !by_k) {
+        // all tokens below 2^-e weigh less than 2^-e V, which is less than (1 - P) of all when 2^e = V / ((1 - P) M')
+        // for a part M' of the mass; here that of the maxima, rounded down
+        float part = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (m4[j] > -INFINITY) part += exp2f(-__fmul_rn(__fsub_rn(r.mx, m4[j]), (float)r.c));
+        const double M = fmax(1.0, 0.99 / kOne * (double)pick_sum(r, (u64)(part * (float)kOne)));
+        const double e = log2((double)V / ((1.0 - (double)P) * M));
+        most = max(0, min(kPickBins - 1, (int)(e * (kPickBins / (double)kPickSpan)) + 1));
+    } else if (bound_k) {
+        // K of the CTA's maxima: at least K logits are as large
         for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
         __syncthreads();
 #pragma unroll
@@ -528,18 +584,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         if (tid == 0) s->b1 = kPickBins - 1;
         __syncthreads();
         const uint32_t n0 = s->hist[2 * tid], n1 = s->hist[2 * tid + 1];
-        const u64 c = pick_scan((u64)n0 + n1, s->red), enough = bound_k ? K : 4 * kPickThreads * 15 / 16;
+        const u64 c = pick_scan((u64)n0 + n1, s->red), enough = K;
         if (c >= enough) atomicMin(&s->b1, c - n1 >= enough ? 2 * tid : 2 * tid + 1);
         __syncthreads();
         u64 b = s->b1;
-        if (bound_k) {
-            const u64* e = r.exchange(b);
-            for (int i = 0; i < C; i++) b = pick_min(b, e[i]);
-        } else {
-            b = pick_min(b, kPickBins * 24 / 40);
-            const u64* e = r.exchange(b);  // the same for all
-            for (int i = 0; i < C; i++) b = pick_max(b, e[i]);
-        }
+        const u64* e = r.exchange(b);
+        for (int i = 0; i < C; i++) b = pick_min(b, e[i]);
         most = (int)b;
     } else if (!by_k && mp > 0x1p-38) {
         most = min(kPickBins - 1, (int)(-log2(mp) * (kPickBins / (double)kPickSpan) * (1.0 + 1e-5)) + 1);
@@ -549,36 +599,43 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         // tokens of bins up to `most` into the warp's pool, in index order; the others' mass for top-p
         int n = 0;
         const bool sums = by_p && !by_k;
+        const float limit = most < kPickBins - 1 ? (float)(most + 1) : INFINITY;  // bin <= most: below it
+        double others = 0.0;
         for (int i = r.w0; i < r.w1; i += 128) {
             float q[4];
             r.load(i + 4 * lane, q);
-            unsigned mine = 0u;
+            bool in[4];
+            unsigned own = 0u;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (!(q[j] > -INFINITY)) continue;
-                if (r.bin(q[j]) <= most)
-                    mine |= 1u << j;
-                else if (sums)
-                    rest += r.weight(q[j]);
+                in[j] = q[j] > -INFINITY && !(__fmul_rn(__fsub_rn(r.mx, q[j]), r.bin_scale) >= limit);
+                own += in[j];
             }
-            if (!__any_sync(0xffffffffu, mine != 0u)) continue;
-            const int own = __popc(mine);
-            int at = own;
+            if (sums) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const double w = r.weight_d(q[j]);
+                    others += in[j] ? 0.0 : w;
+                }
+            }
+            if (!__any_sync(0xffffffffu, own != 0u)) continue;
+            unsigned at = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, at, o);
+                const unsigned y = __shfl_up_sync(0xffffffffu, at, o);
                 if (lane >= o) at += y;
             }
             const int all = __shfl_sync(0xffffffffu, at, 31);
             at += n - own;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (mine >> j & 1u) {
-                    if (at < kPickPool) s->pool[warp][at] = pick_comp(q[j], i + 4 * lane + j);
+                if (in[j]) {
+                    if (at < kPickPool) s->pool[warp][at] = (uint16_t)(i + 4 * lane + j - r.w0);
                     at++;
                 }
             n += all;
         }
+        rest = (u64)others;
         // all of them to CTA 0, when they are few
         if (lane == 0) s->inside[warp] = (uint32_t)n;
         __syncthreads();
@@ -591,7 +648,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         }
         const bool fits = largest <= kPickPool && total <= kPickList;
         if (fits)
-            for (int i = lane; i < n; i += 32) s->list[before + i] = s->pool[warp][i];
+            for (int i = lane; i < n; i += 32) {
+                const int idx = r.w0 + s->pool[warp][i];
+                s->list[before + i] = pick_comp(__ldg(r.l + idx), idx);
+            }
         __syncthreads();
         if (sums) rest = pick_sum(r, rest);
         const int found = pick_collect(r, fits ? total : kPickList + 1u, kPickList);
@@ -622,7 +682,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         u64 mass = 0ull;
         const float up = kPickSpan / kPickBins;
         r.each([&](float x, int idx, bool is) {
-            if (!is || pick_comp(x, idx) < tau) return;
+            if (!is || (tau != 0ull && pick_comp(x, idx) < tau)) return;
             const int b = r.bin(x);
             uint32_t n = 1u;
             if (pass == 1) {
@@ -648,7 +708,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
 
     // sums of the kept weights by warp, in index order
     auto kept = [&](float q, int i) -> u64 {
-        if (!(q > -INFINITY) || pick_comp(q, i) < tau) return 0ull;
+        if (!(q > -INFINITY) || (tau != 0ull && pick_comp(q, i) < tau)) return 0ull;
         const u64 w = r.weight(q);
         return (double)w >= mp * kOne ? w : 0ull;
     };
@@ -677,8 +737,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         if (r.pooled < 0) {
             r.load(first, q);
         } else if (i + lane < end) {
-            q[0] = pick_value(s->pool[warp][i + lane]);
-            first = pick_index(s->pool[warp][i + lane]);
+            first = r.w0 + s->pool[warp][i + lane];
+            q[0] = __ldg(r.l + first);
         }
         u64 w[4], own = 0ull;
 #pragma unroll
