@@ -41,10 +41,10 @@ typedef unsigned long long u64;
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 constexpr int kPickList = 4096;      // tokens that one CTA ends a row with
 constexpr int kPickTopK = 1024;      // largest k bounded by maxima
-constexpr int kPickPool = 2048;      // tokens of a warp's pool
+constexpr int kPickPool = 1920;      // tokens of a warp's pool: two CTAs share an SM's memory
 constexpr int kPickPairs = 256;      // tokens whose top-p is decided by comparing all pairs
 constexpr int kPickRank = 512;       // tokens of a border that are ranked
-constexpr int kPickBins = 1024;
+constexpr int kPickBins = 2048, kPickPer = kPickBins / kPickThreads;
 constexpr int kPickMaxCluster = 8;
 constexpr float kPickSpan = 40.0f;   // powers of two that the bins cover
 constexpr double kOne = 0x1p42;      // a weight of 1
@@ -59,13 +59,19 @@ __device__ __forceinline__ float pick_value(u64 comp) {
 }
 
 struct PickShared {
-    u64 list[kPickList];
+    union {
+        u64 list[kPickList];
+        struct {
+            u64 first[kPickList / 2];  // a border's tokens, while the totals are in use
+            uint32_t tot[kPickBins];
+        };
+    };
     union {
         uint16_t pool[kPickWarps][kPickPool];  // positions in the warp's part (at most 2^16 logits)
         u64 top[kPickTopK];                    // the top-k, when one CTA ends the row
     };
-    u64 w[kPickRank];
-    uint32_t hist[kPickBins], tot[kPickBins];
+    ulonglong2 pair[kPickRank];        // comp, metric
+    uint32_t hist[kPickBins];
     double pow2[64];                   // 2^(j / 64)
     u64 x[2][kPickMaxCluster];         // exchanges between CTAs, two turns
     u64 sums[kPickMaxCluster][kPickWarps];
@@ -123,15 +129,21 @@ struct PickRow {
         const float b = __fmul_rn(__fsub_rn(mx, x), bin_scale);
         return b < (float)(kPickBins - 1) ? (int)b : kPickBins - 1;
     }
-    // f(logit, index, whether there is one) for the warp's tokens, in index order, by whole warps
+    // f(logit, index, whether there is one) for the warp's tokens, by whole warps
     template <class F>
     __device__ __forceinline__ void each(F f) const {
         const int lane = threadIdx.x & 31;
         if (pooled >= 0) {
             const uint16_t* p = s->pool[threadIdx.x >> 5];
-            for (int i = lane; i - lane < pooled; i += 32) {
-                const int idx = w0 + (i < pooled ? p[i] : 0);
-                f(i < pooled ? __ldg(l + idx) : -INFINITY, idx, i < pooled);
+            for (int i = lane; i - lane < pooled; i += 128) {  // four loads on their way at a time
+                int idx[4];
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) idx[j] = w0 + (i + 32 * j < pooled ? p[i + 32 * j] : 0);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] = i + 32 * j < pooled ? __ldg(l + idx[j]) : -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; j++) f(x[j], idx[j], i + 32 * j < pooled);
             }
             return;
         }
@@ -260,16 +272,16 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
     double above = 0.0;  // metric of what lies above the members
     while (true) {
         pick_total(r);
-        // bounds of the metric up to each bin; two bins per thread
-        double lo[2], hi[2];
+        // bounds of the metric up to each bin; a thread's bins lie side by side
+        double lo[kPickPer], hi[kPickPer], lo_all = 0.0, hi_all = 0.0;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int b = 2 * tid + i;
+        for (int i = 0; i < kPickPer; i++) {
+            const int b = kPickPer * tid + i;
             const double n = (double)s->tot[b];
             lo[i] = hi[i] = n;
             if (by_mass && n > 0.0) {
                 if (level == 0) {
-                    // a token's share is rounded by half a unit and lies above 0.97; 1e-5: the fp32 bins and shares
+                    // a token's share is rounded by half a unit and lies above 0.98; 1e-5: the fp32 bins and shares
                     const double top = n / unit * exp2(-(double)kPickSpan / kPickBins * b) * kOne, e = 0.52 / unit + 1e-5;
                     hi[i] = top * (1.0 + e);
                     lo[i] = top * (1.0 - e);
@@ -279,10 +291,11 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
                     lo[i] = n * (double)r.weight(pick_value(top > span ? top - span : 0ull));
                 }
             }
+            lo_all += lo[i];
+            hi_all += hi[i];
         }
         double* red = reinterpret_cast<double*>(s->red);
-        const double cl1 = pick_scan(lo[0] + lo[1], red) + above, cl0 = cl1 - lo[1];
-        const double ch1 = pick_scan(hi[0] + hi[1], red) + above, ch0 = ch1 - hi[1];
+        double cl = pick_scan(lo_all, red) + above - lo_all, ch = pick_scan(hi_all, red) + above - hi_all;
         if (tid == 0) {
             s->b1 = s->b2 = kPickBins - 1;
             s->count = 0u;
@@ -290,8 +303,23 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         __syncthreads();
         // sums of doubles may be off by a few parts in 2^53 per bin
         const double early = target * (1.0 - 1e-12), late = by_mass ? target * (1.0 + 1e-12) : target;
-        if (ch1 >= early) atomicMin(&s->b1, ch0 >= early ? 2 * tid : 2 * tid + 1);
-        if (cl1 >= late) atomicMin(&s->b2, cl0 >= late ? 2 * tid : 2 * tid + 1);
+        // the first bins that reach the target; threads well behind them stay out
+        bool no1 = ch > early * (1.0 + 1e-9), no2 = cl > late * (1.0 + 1e-9);
+#pragma unroll
+        for (int i = 0; i < kPickPer; i++) {
+            ch += hi[i];
+            cl += lo[i];
+            if (!no1 && ch >= early) {
+                atomicMin(&s->b1, kPickPer * tid + i);
+                no1 = true;
+            }
+            if (!no2 && cl >= late) {
+                atomicMin(&s->b2, kPickPer * tid + i);
+                no2 = true;
+            }
+        }
+        if (above >= early && tid == 0) atomicMin(&s->b1, 0);
+        if (above >= late && tid == 0) atomicMin(&s->b2, 0);
         __syncthreads();
         const int b1 = s->b1, b2 = max(s->b2, s->b1);
         const u64 chi1 = level == 0 ? ~0ull : chi - ((u64)b1 << shift);
@@ -327,11 +355,14 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
                 // the token up to which the running metric reaches the target, and before which it does not
                 const u64 mine = tid < total ? s->list[tid] : 0ull;
                 const u64 own = tid < total ? (by_mass ? r.weight(pick_value(mine)) : 1ull) : 0ull;
-                if (tid < kPickRank) s->w[tid] = own;
+                s->pair[tid] = make_ulonglong2(mine, own);
                 u64 lowest = pick_reduce(tid < total ? mine : ~0ull, s->red, pick_min);
                 u64 run = up;
-                for (int j = 0; j < total; j++)
-                    if (s->list[j] > mine) run += s->w[j];
+#pragma unroll 8
+                for (int j = 0; j < total; j++) {
+                    const ulonglong2 q = s->pair[j];
+                    run += q.x > mine ? q.y : 0ull;
+                }
                 if (tid == 0) s->tau = total ? lowest : tau0;
                 __syncthreads();
                 const bool reached = tid < total && (double)(run + own) >= target;
@@ -431,13 +462,17 @@ __device__ bool pick_short(const PickArgs& a, PickRow& r, int row, int n, int K,
     if (P < 1.0f && n <= kPickPairs) {
         // the mass in front of each token, over all pairs
         const u64 mine = tid < n ? list[tid] : 0ull, own = tid < n ? r.weight(pick_value(mine)) : 0ull;
-        if (tid < n) s->w[tid] = own;
+        s->pair[tid] = make_ulonglong2(mine, own);
         const u64 M = pick_reduce(own, s->red, pick_add);
         const double need = (double)P * (double)(M + rest);
         if ((double)M < need) return false;
         u64 front = 0ull;
         if (tid < n)
-            for (int j = 0; j < n; j++) front += list[j] > mine ? s->w[j] : 0ull;
+#pragma unroll 8
+            for (int j = 0; j < n; j++) {
+                const ulonglong2 q = s->pair[j];
+                front += q.x > mine ? q.y : 0ull;
+            }
         bar = pick_reduce(tid < n && (front == 0ull || (double)front < need) ? mine : ~0ull, s->red, pick_min);
         tau = 0u;
     } else if (P < 1.0f) {
@@ -583,9 +618,15 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
             if (m4[j] > -INFINITY) atomicAdd(&s->hist[r.bin(m4[j])], 1u);
         if (tid == 0) s->b1 = kPickBins - 1;
         __syncthreads();
-        const uint32_t n0 = s->hist[2 * tid], n1 = s->hist[2 * tid + 1];
-        const u64 c = pick_scan((u64)n0 + n1, s->red), enough = K;
-        if (c >= enough) atomicMin(&s->b1, c - n1 >= enough ? 2 * tid : 2 * tid + 1);
+        u64 in_bin[kPickPer], here = 0ull;
+#pragma unroll
+        for (int i = 0; i < kPickPer; i++) here += in_bin[i] = s->hist[kPickPer * tid + i];
+        u64 c = pick_scan(here, s->red) - here;
+#pragma unroll
+        for (int i = 0; i < kPickPer; i++) {
+            if (c < (u64)K && c + in_bin[i] >= (u64)K) s->b1 = kPickPer * tid + i;  // one bin of all
+            c += in_bin[i];
+        }
         __syncthreads();
         u64 b = s->b1;
         const u64* e = r.exchange(b);
