@@ -120,38 +120,52 @@ struct PickRow {
         const double q = __hiloint2double(__double2hiint(p) + ((n & ~63) << 14) + (42 << 20), __double2loint(p));
         return t >= -40.0 ? (q + 0x1p52) - 0x1p52 : 0.0;  // 0 for NaN and -inf too
     }
-    __device__ __forceinline__ u64 weight(float x) const {
-        return x == mx ? (u64)kOne : (u64)weight_d(x);  // the maximum may be infinite
+    __device__ __forceinline__ double mass(float x) const {
+        const double w = weight_d(x);
+        return x == mx ? kOne : w;  // the maximum may be infinite
     }
+    __device__ __forceinline__ u64 weight(float x) const { return (u64)mass(x); }
     // bin of a logit above -inf: larger logits never lie in a later bin
     __device__ __forceinline__ int bin(float x) const {
         if (x == mx) return 0;
         const float b = __fmul_rn(__fsub_rn(mx, x), bin_scale);
         return b < (float)(kPickBins - 1) ? (int)b : kPickBins - 1;
     }
-    // f(logit, index, whether there is one) for the warp's tokens, by whole warps
+    // adds the weight's share of its bin's largest, in units of 1 / unit, to the bin (fp32: off by less than 1e-5
+    // and half a unit)
+    __device__ __forceinline__ void share(float x, float unit) const {
+        const float b = x == mx ? 0.0f : fminf(__fmul_rn(__fsub_rn(mx, x), bin_scale), (float)kPickBins);
+        const int n = min((int)b, kPickBins - 1);
+        atomicAdd(&s->hist[n], __float2uint_rn(unit * exp2f((kPickSpan / kPickBins) * ((float)n - b))));
+    }
+    // f(four logits, their indices, whether there are any) for the warp's tokens, by whole warps: four at a time,
+    // so that loads and double-precision chains overlap
     template <class F>
     __device__ __forceinline__ void each(F f) const {
         const int lane = threadIdx.x & 31;
-        if (pooled >= 0) {
-            const uint16_t* p = s->pool[threadIdx.x >> 5];
-            for (int i = lane; i - lane < pooled; i += 128) {  // four loads on their way at a time
-                int idx[4];
-                float x[4];
+        const bool pools = pooled >= 0;
+        const uint16_t* p = s->pool[threadIdx.x >> 5];
+        float x[4];
+        int idx[4];
+        bool is[4];
+        for (int i = pools ? 0 : w0; i < (pools ? pooled : w1); i += 128) {
+            if (pools) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) idx[j] = w0 + (i + 32 * j < pooled ? p[i + 32 * j] : 0);
+                for (int j = 0; j < 4; j++) {
+                    is[j] = i + 32 * j + lane < pooled;
+                    idx[j] = w0 + (is[j] ? p[i + 32 * j + lane] : 0);
+                }
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] = i + 32 * j < pooled ? __ldg(l + idx[j]) : -INFINITY;
+                for (int j = 0; j < 4; j++) x[j] = is[j] ? __ldg(l + idx[j]) : -INFINITY;
+            } else {
+                load(i + 4 * lane, x);
 #pragma unroll
-                for (int j = 0; j < 4; j++) f(x[j], idx[j], i + 32 * j < pooled);
+                for (int j = 0; j < 4; j++) {
+                    idx[j] = i + 4 * lane + j;
+                    is[j] = x[j] > -INFINITY;
+                }
             }
-            return;
-        }
-        for (int i = w0; i < w1; i += 128) {
-            float x[4];
-            load(i + 4 * lane, x);
-#pragma unroll
-            for (int j = 0; j < 4; j++) f(x[j], i + 4 * lane + j, x[j] > -INFINITY);
+            f(x, idx, is);
         }
     }
     __device__ void sync() const {
@@ -264,7 +278,8 @@ __device__ void pick_total(PickRow& r) {
 // Where the prefix of {comp >= tau0} ends whose metric (number of tokens, or mass) first reaches `target`:
 // the comp of its last token. s->hist holds this CTA's histogram of the bins: tokens, or for a mass their
 // weights over the bin's largest, in units of 1 / unit.
-__device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit, u64 tau0) {
+// *kept: the metric that this warp's tokens have in the prefix.
+__device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit, u64 tau0, u64* kept) {
     PickShared* s = r.s;
     const int tid = threadIdx.x;
     int lo_bin = 0, hi_bin = kPickBins - 1, level = 0, shift = 0;
@@ -330,24 +345,50 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
             hi_bin = b2;
         }
         // what lies above the members, exactly; the members themselves, and their range
-        u64 up = 0ull, first = ~0ull, last = 0ull;
-        r.each([&](float x, int idx, bool is) {
-            const int b = is ? r.bin(x) : kPickBins;
-            bool in = b <= hi_bin;
-            if (!__any_sync(0xffffffffu, in)) return;
-            const u64 comp = pick_comp(x, idx);
-            if (in) {
-                const bool over = b < lo_bin || comp > chi1;
-                in = !over && comp >= clo1 && comp >= tau0;
-                if (over && comp >= tau0) up += by_mass ? r.weight(x) : 1ull;
-                if (in) {
-                    first = pick_min(first, comp);
-                    last = pick_max(last, comp);
+        u64 first = ~0ull, last = 0ull;
+        double over_sum = 0.0;  // whole numbers below 2^53
+        r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
+            bool over[4], in[4], some = false, members = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int b = is[j] ? r.bin(x[j]) : kPickBins;
+                over[j] = b < lo_bin;
+                in[j] = b >= lo_bin && b <= hi_bin;
+                some |= over[j];
+                members |= in[j];
+            }
+            if (tau0 != 0ull && __any_sync(0xffffffffu, some)) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) over[j] = over[j] && pick_comp(x[j], idx[j]) >= tau0;
+            }
+            if (__any_sync(0xffffffffu, members)) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const u64 comp = pick_comp(x[j], idx[j]);
+                    if (in[j]) {
+                        over[j] = comp > chi1 && comp >= tau0;
+                        in[j] = comp <= chi1 && comp >= clo1 && comp >= tau0;
+                        some |= over[j];
+                    }
+                    if (in[j]) {
+                        first = pick_min(first, comp);
+                        last = pick_max(last, comp);
+                    }
+                    pick_append(s, in[j], comp);
                 }
             }
-            pick_append(s, in, comp);
+            if (!__any_sync(0xffffffffu, some)) return;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double w = by_mass ? r.mass(x[j]) : 1.0;
+                over_sum += over[j] ? w : 0.0;
+            }
         });
-        up = pick_sum(r, up);
+        u64 up = (u64)over_sum;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) up += __shfl_xor_sync(0xffffffffu, up, o);
+        const u64 warp_up = up;
+        up = pick_sum(r, (tid & 31) == 0 ? up : 0ull);
         above = (double)up;
         const int total = pick_collect(r, s->count, kPickRank);
         if (total >= 0) {
@@ -371,7 +412,18 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
                 if (tid > 0 && tid < r.C) cg::this_cluster().map_shared_rank(s, tid)->tau = s->tau;
             }
             r.sync();
-            return s->tau;
+            const u64 tau = s->tau;
+            const ulonglong2* pair = (r.C > 1 ? cg::this_cluster().map_shared_rank(s, 0) : s)->pair;
+            u64 mine = 0ull;
+            for (int i = tid & 31; i < total; i += 32) {
+                const ulonglong2 q = pair[i];
+                const int idx = pick_index(q.x);
+                if (q.x >= tau && idx >= r.w0 && idx < r.w1) mine += q.y;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+            *kept = warp_up + mine;
+            return tau;
         }
         // too many: split the members' range of comps
         first = pick_reduce(first, s->red, pick_min);
@@ -387,11 +439,14 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         while (((chi - clo) >> shift) >= (u64)kPickBins) shift++;
         for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
         __syncthreads();
-        r.each([&](float x, int idx, bool is) {
-            const u64 comp = pick_comp(x, idx);
-            if (!is || comp < tau0 || comp < clo || comp > chi) return;
-            const int b = r.bin(x);
-            if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->hist[(chi - comp) >> shift], 1u);
+        r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const u64 comp = pick_comp(x[j], idx[j]);
+                if (!is[j] || comp < tau0 || comp < clo || comp > chi) continue;
+                const int b = r.bin(x[j]);
+                if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->hist[(chi - comp) >> shift], 1u);
+            }
         });
     }
 }
@@ -635,13 +690,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     } else if (!by_k && mp > 0x1p-38) {
         most = min(kPickBins - 1, (int)(-log2(mp) * (kPickBins / (double)kPickSpan) * (1.0 + 1e-5)) + 1);
     }
-    u64 rest = 0ull;
+    const double unit = (double)(1u << (V <= 1 << 17 ? 14 : 11));  // V of them fit 32 bits
+    u64 rest = 0ull, M = 0ull;
+    bool have = false;
     if (most >= 0) {
         // tokens of bins up to `most` into the warp's pool, in index order; the others' mass for top-p
         int n = 0;
         const bool sums = by_p && !by_k;
         const float limit = most < kPickBins - 1 ? (float)(most + 1) : INFINITY;  // bin <= most: below it
-        double others = 0.0;
+        double others = 0.0, all_mass = 0.0;
+        if (sums) {
+            for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
+            __syncthreads();
+        }
         for (int i = r.w0; i < r.w1; i += 128) {
             float q[4];
             r.load(i + 4 * lane, q);
@@ -655,8 +716,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
             if (sums) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const double w = r.weight_d(q[j]);
+                    const double w = r.mass(q[j]);
+                    all_mass += w;
                     others += in[j] ? 0.0 : w;
+                    if (in[j]) r.share(q[j], (float)unit);
                 }
             }
             if (!__any_sync(0xffffffffu, own != 0u)) continue;
@@ -677,6 +740,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
             n += all;
         }
         rest = (u64)others;
+        M = (u64)all_mass;
         // all of them to CTA 0, when they are few
         if (lane == 0) s->inside[warp] = (uint32_t)n;
         __syncthreads();
@@ -694,7 +758,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
                 s->list[before + i] = pick_comp(__ldg(r.l + idx), idx);
             }
         __syncthreads();
-        if (sums) rest = pick_sum(r, rest);
+        if (sums) {
+            rest = pick_sum(r, rest);
+            M = pick_sum(r, M);
+            // the border is among the histogram's tokens: it serves the passes below
+            have = (double)P * (double)M <= (double)(M - rest);
+        }
         const int found = pick_collect(r, fits ? total : kPickList + 1u, kPickList);
         if (found >= 0) {
             if (tid == 0) s->tau = 1ull;
@@ -712,39 +781,30 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         }
     }
 
-    if (r.pooled < 0) rest = 0ull;
-    const double unit = (double)(1u << (V <= 1 << 17 ? 14 : 11));  // V of them fit 32 bits
-    u64 tau = 0ull;
+    u64 tau = 0ull, sum = 0ull;
     for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); pass++) {
-        // histogram of the bins among {comp >= tau}: tokens, or for top-p their weights over the bin's largest, and
-        // the mass
-        for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
-        __syncthreads();
-        u64 mass = 0ull;
-        const float up = kPickSpan / kPickBins;
-        r.each([&](float x, int idx, bool is) {
-            if (!is || (tau != 0ull && pick_comp(x, idx) < tau)) return;
-            const int b = r.bin(x);
-            uint32_t n = 1u;
-            if (pass == 1) {
-                const u64 w = r.weight(x);
-                mass += w;
-                n = __float2uint_rn((float)w * (exp2f(up * (float)b) * (float)(unit / kOne)));
-            }
-            if (n) atomicAdd(&s->hist[b], n);
-        });
-        double target = (double)K;
-        if (pass == 1) {
-            const u64 M = pick_sum(r, mass);
-            target = (double)P * (double)(M + rest);
-            if (r.pooled >= 0 && (double)M < target) {  // the border is not in the pools: over all logits
-                r.pooled = -1;
-                rest = 0ull;
-                pass--;
-                continue;
-            }
+        if (!have) {
+            // histogram of the bins among {comp >= tau}: tokens, or for top-p their weights, and the mass
+            if (pass == 1 && !by_k) r.pooled = -1;  // the pools miss the border
+            for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
+            __syncthreads();
+            double all = 0.0;
+            r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = is[j] && (tau == 0ull || pick_comp(x[j], idx[j]) >= tau);
+                    if (pass == 1) {
+                        const double w = r.mass(x[j]);
+                        all += in ? w : 0.0;
+                        if (in) r.share(x[j], (float)unit);
+                    } else if (in) {
+                        atomicAdd(&s->hist[r.bin(x[j])], 1u);
+                    }
+                }
+            });
+            if (pass == 1) M = pick_sum(r, (u64)all);
         }
-        tau = pick_border(r, pass == 1, target, unit, tau);
+        tau = pick_border(r, pass == 1, pass == 1 ? (double)P * (double)M : (double)K, unit, tau, &sum);
     }
 
     // sums of the kept weights by warp, in index order
@@ -753,10 +813,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         const u64 w = r.weight(q);
         return (double)w >= mp * kOne ? w : 0ull;
     };
-    u64 sum = 0ull;
-    r.each([&](float x, int idx, bool is) { sum += is ? kept(x, idx) : 0ull; });
+    if (!by_p || mp > 0.0) {  // else the border's search has summed them
+        double all = 0.0;     // whole numbers up to 2^53: a lane has 2^11 of them at most
+        r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            for (int j = 0; j < 4; j++) {
+                const double w = r.mass(x[j]);
+                all += is[j] && w >= mp * kOne && (tau == 0ull || pick_comp(x[j], idx[j]) >= tau) ? w : 0.0;
+            }
+        });
+        sum = (u64)all;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
     if (lane < C) (C > 1 ? cg::this_cluster().map_shared_rank(s, lane) : s)->sums[r.rank][warp] = sum;
     r.sync();
     u64 before = 0ull, S = 0ull;
