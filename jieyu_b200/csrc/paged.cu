@@ -112,67 +112,134 @@ __device__ __forceinline__ uint32_t pack4(float4 x, float inv) {
            ((uint32_t)(q8_round(x.z, inv) & 255) << 16) | ((uint32_t)(q8_round(x.w, inv) & 255) << 24);
 }
 
-// One warp per (row, kv head, K or V); a lane holds up to two quads.
-__global__ void paged_append_kernel(const float* K, const float* V, int ld, int rows, int KV, int hd,
-                                    const int* row_seq, const int* row_pos, PagedKV kv, PagedRope rope, bool vec) {
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (unit >= (long long)rows * KV * 2) return;
-    const int i = (int)(unit / (KV * 2)), r = (int)(unit % (KV * 2));
-    const int h = r >> 1;
-    const bool is_k = (r & 1) == 0;
-    const int pos = row_pos[i];
-    if (pos < 0) return;
-    const int page = paged_page(kv, row_seq ? row_seq[i] : i, pos);
-    if (page < 0) return;
-    const bool rot = rope.cos_t != nullptr && is_k;
-    if (rope.cos_t != nullptr && pos >= rope.len) {
-        paged_flag(kPagedErrRope);
-        return;
-    }
-    const int half = hd >> 1, nq = hd >> 2;
-    const float* src = (is_k ? K : V) + (size_t)i * ld + (size_t)h * hd;
-    float4 x[2];
-    float amax = 0.0f;
+// ---------------------------------------------------------------------------
+// Append and read back: bound by their bytes (append reads 8 hd and writes 2 hd
+// + 8 per row and kv head, read the reverse). A unit is one head of K or of V of
+// one row; LANES lanes hold a unit, QUADS groups of four dims each, so a warp
+// has 32 / LANES units side by side (neighbouring heads: whole sectors) and
+// kRowUnits of them in flight, whose loads are all issued before the first is
+// used; only where a unit goes waits for its row's position and page.
+constexpr int kRowUnits = 4, kRowThreads = 256;
+
+struct RowUnit {
+    int row, head;
+    bool is_k, live;
+    int seq, pos;
+};
+template <int LANES>
+__device__ __forceinline__ RowUnit row_unit(long long u, int rows, int KV, const int* row_seq, const int* row_pos) {
+    RowUnit x;
+    x.live = u < (long long)rows * KV * 2;
+    x.row = x.live ? (int)(u / (KV * 2)) : 0;
+    const int r = x.live ? (int)(u - (long long)x.row * KV * 2) : 0;
+    x.is_k = r < KV;
+    x.head = x.is_k ? r : r - KV;
+    x.pos = x.live ? __ldg(row_pos + x.row) : -1;
+    x.seq = row_seq && x.live ? __ldg(row_seq + x.row) : x.row;
+    x.live = x.live && x.pos >= 0;
+    return x;
+}
+
+template <int LANES, int QUADS>
+__global__ void __launch_bounds__(kRowThreads) paged_append_kernel(const float* K, const float* V, int ld, int rows,
+                                                                   int KV, int hd, const int* row_seq,
+                                                                   const int* row_pos, PagedKV kv, PagedRope rope,
+                                                                   bool vec) {
+    constexpr int SIDE = 32 / LANES;
+    const int lane = threadIdx.x & 31, sub = lane & (LANES - 1), half = hd >> 1, nq = hd >> 2;
+    const long long w = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+    RowUnit x[kRowUnits];
+    float4 v[kRowUnits][QUADS];
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int qd = lane + 32 * t;
-        if (qd >= nq) continue;
-        x[t] = load4(src + 4 * qd, vec);
-        if (rot)
-            x[t] = rotate4(x[t], load2(rope.cos_t + (size_t)pos * half + 2 * qd, vec),
-                           load2(rope.sin_t + (size_t)pos * half + 2 * qd, vec));
-        amax = fmaxf(amax, amax4(x[t]));
-    }
-    amax = warp_max(amax);
-    const float inv = q8_inv(amax);
-    const int slot = pos % kv.p.page_size;
-    uint32_t* dst = reinterpret_cast<uint32_t*>((is_k ? kv.p.k : kv.p.v) + paged_off(kv, page, slot, h));
-    if (lane == 0) (is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, h)] = q8_scale(amax);
+    for (int i = 0; i < kRowUnits; i++) {
+        x[i] = row_unit<LANES>((w * kRowUnits + i) * SIDE + lane / LANES, rows, KV, row_seq, row_pos);
+        const float* src = (x[i].is_k ? K : V) + (size_t)x[i].row * ld + (size_t)x[i].head * hd;
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int qd = lane + 32 * t;
-        if (qd < nq) dst[rot ? rope_slot(2 * qd, half) >> 1 : qd] = pack4(x[t], inv);
+        for (int t = 0; t < QUADS; t++) {
+            const int qd = sub + LANES * t;
+            v[i][t] = qd < nq ? load4(src + 4 * qd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowUnits; i++) {
+        int page = -1;
+        if (x[i].live) page = paged_page(kv, x[i].seq, x[i].pos);
+        if (page >= 0 && rope.cos_t != nullptr && x[i].pos >= rope.len) {
+            paged_flag(kPagedErrRope);
+            page = -1;
+        }
+        const bool rot = rope.cos_t != nullptr && x[i].is_k && page >= 0;
+        float amax = 0.0f;
+#pragma unroll
+        for (int t = 0; t < QUADS; t++) {
+            const int qd = sub + LANES * t;
+            if (rot && qd < nq) {
+                const size_t at = (size_t)x[i].pos * half + 2 * qd;
+                v[i][t] = rotate4(v[i][t], load2(rope.cos_t + at, vec), load2(rope.sin_t + at, vec));
+            }
+            amax = fmaxf(amax, amax4(v[i][t]));
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (page < 0) continue;
+        const int slot = x[i].pos % kv.p.page_size;
+        const float inv = q8_inv(amax);
+        uint32_t* dst = reinterpret_cast<uint32_t*>((x[i].is_k ? kv.p.k : kv.p.v) + paged_off(kv, page, slot, x[i].head));
+        if (sub == 0) (x[i].is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, x[i].head)] = q8_scale(amax);
+#pragma unroll
+        for (int t = 0; t < QUADS; t++) {
+            const int qd = sub + LANES * t;
+            if (qd < nq) dst[rot ? rope_slot(2 * qd, half) >> 1 : qd] = pack4(v[i][t], inv);
+        }
     }
 }
 
-__global__ void paged_read_kernel(float* K, float* V, int ld, int rows, int KV, int hd, const int* row_seq,
-                                  const int* row_pos, PagedKV kv) {
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (unit >= (long long)rows * KV * 2) return;
-    const int i = (int)(unit / (KV * 2)), r = (int)(unit % (KV * 2));
-    const int h = r >> 1;
-    const bool is_k = (r & 1) == 0;
-    const int pos = row_pos[i];
-    if (pos < 0) return;
-    const int page = paged_page(kv, row_seq ? row_seq[i] : i, pos);
-    if (page < 0) return;
-    const int slot = pos % kv.p.page_size;
-    const int8_t* src = (is_k ? kv.p.k : kv.p.v) + paged_off(kv, page, slot, h);
-    const float sc = (is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, h)];
-    float* dst = (is_k ? K : V) + (size_t)i * ld + (size_t)h * hd;
-    for (int e = lane; e < hd; e += 32) dst[e] = __fmul_rn((float)src[e], sc);
+template <int LANES, int QUADS>
+__global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float* V, int ld, int rows, int KV, int hd,
+                                                                 const int* row_seq, const int* row_pos, PagedKV kv,
+                                                                 bool vec) {
+    constexpr int SIDE = 32 / LANES;
+    const int lane = threadIdx.x & 31, sub = lane & (LANES - 1), nq = hd >> 2;
+    const long long w = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+    RowUnit x[kRowUnits];
+    uint32_t v[kRowUnits][QUADS];
+    float sc[kRowUnits];
+#pragma unroll
+    for (int i = 0; i < kRowUnits; i++)
+        x[i] = row_unit<LANES>((w * kRowUnits + i) * SIDE + lane / LANES, rows, KV, row_seq, row_pos);
+#pragma unroll
+    for (int i = 0; i < kRowUnits; i++) {
+        const int page = x[i].live ? paged_page(kv, x[i].seq, x[i].pos) : -1;
+        x[i].live = page >= 0;
+        const int slot = x[i].pos % kv.p.page_size;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>((x[i].is_k ? kv.p.k : kv.p.v) +
+                                                                (x[i].live ? paged_off(kv, page, slot, x[i].head) : 0));
+        sc[i] = x[i].live ? (x[i].is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, x[i].head)] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < QUADS; t++) {
+            const int qd = sub + LANES * t;
+            v[i][t] = x[i].live && qd < nq ? src[qd] : 0u;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowUnits; i++) {
+        if (!x[i].live) continue;
+        float* dst = (x[i].is_k ? K : V) + (size_t)x[i].row * ld + (size_t)x[i].head * hd;
+#pragma unroll
+        for (int t = 0; t < QUADS; t++) {
+            const int qd = sub + LANES * t;
+            if (qd >= nq) continue;
+            float f[4];
+            u8x4_to_f32(v[i][t] ^ 0x80808080u, f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] = __fmul_rn(f[j], sc[i]);
+            if (vec)
+                *reinterpret_cast<float4*>(dst + 4 * qd) = make_float4(f[0], f[1], f[2], f[3]);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++) dst[4 * qd + j] = f[j];
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1339,22 +1406,30 @@ bool aligned8(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t
 
 }  // namespace
 
+// Lanes of a unit and quads of a lane by head size.
+#define ROW_CASES(KERNEL, ...)                                                                     \
+    do {                                                                                           \
+        const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : 32, per = kRowUnits * (32 / lanes);       \
+        const long long units = (long long)rows * KV * 2, warps = (units + per - 1) / per;         \
+        const unsigned grid = (unsigned)((warps + kRowThreads / 32 - 1) / (kRowThreads / 32));     \
+        if (hd <= 32) KERNEL<8, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                      \
+        else if (hd <= 64) KERNEL<16, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                \
+        else if (hd <= 128) KERNEL<32, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);               \
+        else KERNEL<32, 2><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                              \
+    } while (0)
+
 int launch_paged_append(const float* K, const float* V, int ld, int rows, int KV, int hd, const int* row_seq,
                         const int* row_pos, const PagedKV& kv, const PagedRope& rope, cudaStream_t s) {
-    const long long units = (long long)rows * KV * 2;
-    if (units == 0) return JYC_OK;
-    paged_append_kernel<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(K, V, ld, rows, KV, hd, row_seq, row_pos, kv, rope,
-                                                                    aligned16(K, ld) && aligned16(V, ld) &&
-                                                                        aligned8(rope.cos_t, rope.sin_t));
+    const bool vec = aligned16(K, ld) && aligned16(V, ld) && aligned8(rope.cos_t, rope.sin_t);
+    ROW_CASES(paged_append_kernel, K, V, ld, rows, KV, hd, row_seq, row_pos, kv, rope, vec);
     JYC_LAUNCHED();
     return JYC_OK;
 }
 
 int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, const int* row_seq, const int* row_pos,
                       const PagedKV& kv, cudaStream_t s) {
-    const long long units = (long long)rows * KV * 2;
-    if (units == 0) return JYC_OK;
-    paged_read_kernel<<<(unsigned)((units + 7) / 8), 256, 0, s>>>(K, V, ld, rows, KV, hd, row_seq, row_pos, kv);
+    const bool vec = aligned16(K, ld) && aligned16(V, ld);
+    ROW_CASES(paged_read_kernel, K, V, ld, rows, KV, hd, row_seq, row_pos, kv, vec);
     JYC_LAUNCHED();
     return JYC_OK;
 }

@@ -58,6 +58,12 @@ __device__ __forceinline__ float pick_value(u64 comp) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
+__device__ __forceinline__ float pick_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 struct PickShared {
     union {
         u64 list[kPickList];
@@ -87,12 +93,16 @@ struct PickRow {
     int V, v0, v1, w0, w1;  // the CTA's part, the warp's part
     bool vec;
     float mx;
-    double c, mxc;          // log2(e) / T, and mx times that
+    double c;               // log2(e) / T
+    bool endless;           // the maximum is infinite
     float bin_scale;
     int C, rank, turn;
     int pooled;             // tokens in the warp's pool; -1: the passes go over all logits
     PickShared* s;
 
+    // a logit as the passes take it: under an infinite maximum, 0 where it is infinite too, else -inf
+    __device__ __forceinline__ float seen(float x) const { return !endless ? x : x == INFINITY ? 0.0f : -INFINITY; }
+    __device__ __forceinline__ float at(int i) const { return seen(__ldg(l + i)); }
     // four logits at i, i + 1, ... < w1 (NaN behind the end)
     __device__ __forceinline__ void load(int i, float (&x)[4]) const {
         if (vec && i + 3 < w1) {
@@ -105,11 +115,14 @@ struct PickRow {
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = i + j < w1 ? __ldg(l + i + j) : __int_as_float(0x7FC00000);
         }
+        if (endless)
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = seen(x[j]);
     }
     // The weight of x in units of 2^-42, a whole number. 2^t by 2^(j / 64) and the series of 2^f: |f| <= 1 / 128,
     // remainder (f ln 2)^5 / 120 < 4e-14
-    __device__ __forceinline__ double weight_d(float x) const {
-        const double t = __fma_rn((double)x, c, -mxc);
+    __device__ __forceinline__ double mass(float x) const {
+        const double t = ((double)x - (double)mx) * c;
         const double m = __fma_rn(t, 64.0, 0x1.8p52);
         const int n = __double2loint(m);
         const double f = __fma_rn(m - 0x1.8p52, -1.0 / 64.0, t);
@@ -120,23 +133,22 @@ struct PickRow {
         const double q = __hiloint2double(__double2hiint(p) + ((n & ~63) << 14) + (42 << 20), __double2loint(p));
         return t >= -40.0 ? (q + 0x1p52) - 0x1p52 : 0.0;  // 0 for NaN and -inf too
     }
-    __device__ __forceinline__ double mass(float x) const {
-        const double w = weight_d(x);
-        return x == mx ? kOne : w;  // the maximum may be infinite
-    }
     __device__ __forceinline__ u64 weight(float x) const { return (u64)mass(x); }
-    // bin of a logit above -inf: larger logits never lie in a later bin
-    __device__ __forceinline__ int bin(float x) const {
-        if (x == mx) return 0;
-        const float b = __fmul_rn(__fsub_rn(mx, x), bin_scale);
-        return b < (float)(kPickBins - 1) ? (int)b : kPickBins - 1;
+    // Bins of powers of 2^(40 / 2048), the nearest one: larger logits never lie in a later bin. The place of a
+    // logit above -inf among them (0 for the maximum), and its bin.
+    __device__ __forceinline__ float place(float x) const {
+        return fminf(__fmul_rn(__fsub_rn(mx, x), bin_scale), (float)(kPickBins - 1));
     }
-    // adds the weight's share of its bin's largest, in units of 1 / unit, to the bin (fp32: off by less than 1e-5
-    // and half a unit)
-    __device__ __forceinline__ void share(float x, float unit) const {
-        const float b = x == mx ? 0.0f : fminf(__fmul_rn(__fsub_rn(mx, x), bin_scale), (float)kPickBins);
-        const int n = min((int)b, kPickBins - 1);
-        atomicAdd(&s->hist[n], __float2uint_rn(unit * exp2f((kPickSpan / kPickBins) * ((float)n - b))));
+    static __device__ __forceinline__ int bin_at(float place) {
+        return __float_as_int(__fadd_rn(place, 12582912.0f)) - 0x4B400000;  // 1.5 * 2^23: to the nearest
+    }
+    __device__ __forceinline__ int bin(float x) const { return bin_at(place(x)); }
+    // adds the weight's share of 2^-(bin's middle) to the bin, in units of 1 / unit (fp32: off by less than 1e-5 and
+    // half a unit)
+    __device__ __forceinline__ void share(float place, float unit) const {
+        const float near = __fadd_rn(place, 12582912.0f), off = __fsub_rn(__fsub_rn(near, 12582912.0f), place);
+        const float n = __fmul_rn(unit, pick_ex2((kPickSpan / kPickBins) * off));
+        atomicAdd(&s->hist[__float_as_int(near) - 0x4B400000], __float2uint_rn(n));
     }
     // f(four logits, their indices, whether there are any) for the warp's tokens, by whole warps: four at a time,
     // so that loads and double-precision chains overlap
@@ -145,26 +157,32 @@ struct PickRow {
         const int lane = threadIdx.x & 31;
         const bool pools = pooled >= 0;
         const uint16_t* p = s->pool[threadIdx.x >> 5];
-        float x[4];
-        int idx[4];
-        bool is[4];
-        for (int i = pools ? 0 : w0; i < (pools ? pooled : w1); i += 128) {
+        const int end = pools ? pooled : w1;
+        float x[4], nx[4];
+        int idx[4], nidx[4];
+        auto fetch = [&](int i) {  // one step ahead of its use
             if (pools) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    is[j] = i + 32 * j + lane < pooled;
-                    idx[j] = w0 + (is[j] ? p[i + 32 * j + lane] : 0);
-                }
+                for (int j = 0; j < 4; j++) nidx[j] = i + 32 * j + lane < pooled ? w0 + p[i + 32 * j + lane] : -1;
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] = is[j] ? __ldg(l + idx[j]) : -INFINITY;
+                for (int j = 0; j < 4; j++) nx[j] = nidx[j] >= 0 ? at(nidx[j]) : -INFINITY;
             } else {
-                load(i + 4 * lane, x);
+                load(i + 4 * lane, nx);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    idx[j] = i + 4 * lane + j;
-                    is[j] = x[j] > -INFINITY;
-                }
+                for (int j = 0; j < 4; j++) nidx[j] = i + 4 * lane + j;
             }
+        };
+        int i = pools ? 0 : w0;
+        if (i < end) fetch(i);
+        for (; i < end; i += 128) {
+            bool is[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[j] = nx[j];
+                idx[j] = nidx[j];
+                is[j] = x[j] > -INFINITY;
+            }
+            if (i + 128 < end) fetch(i + 128);
             f(x, idx, is);
         }
     }
@@ -296,7 +314,7 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
             lo[i] = hi[i] = n;
             if (by_mass && n > 0.0) {
                 if (level == 0) {
-                    // a token's share is rounded by half a unit and lies above 0.98; 1e-5: the fp32 bins and shares
+                    // a token's share is rounded by half a unit and lies above 0.99; 1e-5: the fp32 places and shares
                     const double top = n / unit * exp2(-(double)kPickSpan / kPickBins * b) * kOne, e = 0.52 / unit + 1e-5;
                     hi[i] = top * (1.0 + e);
                     lo[i] = top * (1.0 - e);
@@ -393,32 +411,46 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         const int total = pick_collect(r, s->count, kPickRank);
         if (total >= 0) {
             if (r.rank == 0) {
-                // the token up to which the running metric reaches the target, and before which it does not
+                // the token up to which the running metric reaches the target: first its key, by bisection, then its
+                // place among equal ones
                 const u64 mine = tid < total ? s->list[tid] : 0ull;
+                const uint32_t key = (uint32_t)(mine >> 32);
                 const u64 own = tid < total ? (by_mass ? r.weight(pick_value(mine)) : 1ull) : 0ull;
-                s->pair[tid] = make_ulonglong2(mine, own);
-                u64 lowest = pick_reduce(tid < total ? mine : ~0ull, s->red, pick_min);
-                u64 run = up;
-#pragma unroll 8
-                for (int j = 0; j < total; j++) {
-                    const ulonglong2 q = s->pair[j];
-                    run += q.x > mine ? q.y : 0ull;
+                uint32_t lo_key = (uint32_t)pick_reduce(tid < total ? (u64)key : ~0ull, s->red, pick_min);
+                uint32_t hi_key = (uint32_t)pick_reduce((u64)key, s->red, pick_max);
+                const uint32_t top_key = hi_key;
+                auto reach = [&](uint32_t k) { return up + pick_reduce(key >= k ? own : 0ull, s->red, pick_add); };
+                while (lo_key < hi_key) {
+                    const uint32_t mid = lo_key + (hi_key - lo_key + 1u) / 2u;
+                    if ((double)reach(mid) >= target)
+                        lo_key = mid;
+                    else
+                        hi_key = mid - 1u;
                 }
-                if (tid == 0) s->tau = total ? lowest : tau0;
+                const u64 over = lo_key < top_key ? reach(lo_key + 1u) : up;
+                const bool equal = tid < total && key == lo_key;
+                const int equals = __syncthreads_count(equal);
+                if (tid == 0) s->tau = tau0;  // no token at all
+                s->pair[tid] = make_ulonglong2(equal ? mine : 0ull, 0ull);
                 __syncthreads();
-                const bool reached = tid < total && (double)(run + own) >= target;
-                if (reached && ((double)run < target || run == up)) s->tau = mine;
+                if (equal) {
+                    u64 at = 0ull;  // equal ones of lower index
+                    if (equals > 1)
+                        for (int j = 0; j < total; j++) at += s->pair[j].x > mine;
+                    // the first whose sum reaches the target; the last if none does
+                    const bool before = at > 0ull && (double)(over + at * own) >= target;
+                    if (!before && ((double)(over + (at + 1ull) * own) >= target || (int)at == equals - 1)) s->tau = mine;
+                }
                 __syncthreads();
                 if (tid > 0 && tid < r.C) cg::this_cluster().map_shared_rank(s, tid)->tau = s->tau;
             }
             r.sync();
             const u64 tau = s->tau;
-            const ulonglong2* pair = (r.C > 1 ? cg::this_cluster().map_shared_rank(s, 0) : s)->pair;
-            u64 mine = 0ull;
-            for (int i = tid & 31; i < total; i += 32) {
-                const ulonglong2 q = pair[i];
-                const int idx = pick_index(q.x);
-                if (q.x >= tau && idx >= r.w0 && idx < r.w1) mine += q.y;
+            u64 mine = 0ull;  // this CTA's members lie first in its list
+            for (int i = tid & 31; i < (int)s->count; i += 32) {
+                const u64 comp = s->list[i];
+                const int idx = pick_index(comp);
+                if (comp >= tau && idx >= r.w0 && idx < r.w1) mine += by_mass ? r.weight(pick_value(comp)) : 1ull;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -605,6 +637,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     r.C = C;
     r.rank = blockIdx.x - row * C;
     r.turn = 0;
+    r.endless = false;
     r.l = a.logits + (size_t)row * a.ld;
     r.V = V;
     r.vec = ((uintptr_t)r.l & 15) == 0;
@@ -645,9 +678,14 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         return;
     }
     r.mx = pick_value(top);
+    r.endless = isinf(r.mx);
+    if (r.endless) {
+        r.mx = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) m4[j] = r.seen(m4[j]);
+    }
     r.c = 1.44269504088896340736 / (double)Tf;
-    r.mxc = (double)r.mx * r.c;
-    r.bin_scale = (float)(r.c * (kPickBins / (double)kPickSpan));
+    r.bin_scale = fminf((float)(r.c * (kPickBins / (double)kPickSpan)), 1e30f);
 
     r.pooled = -1;
     const bool by_k = K > 0 && K < V, by_p = P < 1.0f;
@@ -697,30 +735,36 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         // tokens of bins up to `most` into the warp's pool, in index order; the others' mass for top-p
         int n = 0;
         const bool sums = by_p && !by_k;
-        const float limit = most < kPickBins - 1 ? (float)(most + 1) : INFINITY;  // bin <= most: below it
-        double others = 0.0, all_mass = 0.0;
+        const float limit = most < kPickBins - 1 ? (float)most + 0.5f : INFINITY;  // bin <= most: up to it
+        double others = 0.0, all = 0.0;
         if (sums) {
             for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
             __syncthreads();
         }
+        float ahead[4];
+        if (r.w0 < r.w1) r.load(r.w0 + 4 * lane, ahead);
         for (int i = r.w0; i < r.w1; i += 128) {
-            float q[4];
-            r.load(i + 4 * lane, q);
+            const float q[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
+            if (i + 128 < r.w1) r.load(i + 128 + 4 * lane, ahead);
+            float place[4];
             bool in[4];
             unsigned own = 0u;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                in[j] = q[j] > -INFINITY && !(__fmul_rn(__fsub_rn(r.mx, q[j]), r.bin_scale) >= limit);
+                place[j] = r.place(q[j]);
+                in[j] = q[j] > -INFINITY && !(place[j] > limit);
                 own += in[j];
             }
             if (sums) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const double w = r.mass(q[j]);
-                    all_mass += w;
+                    all += w;
                     others += in[j] ? 0.0 : w;
-                    if (in[j]) r.share(q[j], (float)unit);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (in[j]) r.share(place[j], (float)unit);
             }
             if (!__any_sync(0xffffffffu, own != 0u)) continue;
             unsigned at = own;
@@ -729,7 +773,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
                 const unsigned y = __shfl_up_sync(0xffffffffu, at, o);
                 if (lane >= o) at += y;
             }
-            const int all = __shfl_sync(0xffffffffu, at, 31);
+            const int total = __shfl_sync(0xffffffffu, at, 31);
             at += n - own;
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -737,10 +781,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
                     if (at < kPickPool) s->pool[warp][at] = (uint16_t)(i + 4 * lane + j - r.w0);
                     at++;
                 }
-            n += all;
+            n += total;
         }
         rest = (u64)others;
-        M = (u64)all_mass;
+        M = (u64)all;
         // all of them to CTA 0, when they are few
         if (lane == 0) s->inside[warp] = (uint32_t)n;
         __syncthreads();
@@ -755,7 +799,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         if (fits)
             for (int i = lane; i < n; i += 32) {
                 const int idx = r.w0 + s->pool[warp][i];
-                s->list[before + i] = pick_comp(__ldg(r.l + idx), idx);
+                s->list[before + i] = pick_comp(r.at(idx), idx);
             }
         __syncthreads();
         if (sums) {
@@ -796,7 +840,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
                     if (pass == 1) {
                         const double w = r.mass(x[j]);
                         all += in ? w : 0.0;
-                        if (in) r.share(x[j], (float)unit);
+                        if (in) r.share(r.place(x[j]), (float)unit);
                     } else if (in) {
                         atomicAdd(&s->hist[r.bin(x[j])], 1u);
                     }
@@ -848,7 +892,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
             r.load(first, q);
         } else if (i + lane < end) {
             first = r.w0 + s->pool[warp][i + lane];
-            q[0] = __ldg(r.l + first);
+            q[0] = r.at(first);
         }
         u64 w[4], own = 0ull;
 #pragma unroll
@@ -893,7 +937,7 @@ int launch_pick(const PickArgs& a, cudaStream_t s) {
     const int sms = sm_count();
     if (sms == 0) return cuda_fail(cudaErrorNoDevice, "sample_batch: device query");
     int C = 1;
-    while (C < kPickMaxCluster && (long long)a.rows * 2 * C <= 2 * sms && a.V / (2 * C) >= 4096) C *= 2;
+    while (C < kPickMaxCluster && (long long)a.rows * 2 * C <= 8 * sms && a.V / (2 * C) >= 4096) C *= 2;
     const int chunk = ((a.V + C - 1) / C + 3) / 4 * 4;
     if (int e = max_dynamic_smem(reinterpret_cast<const void*>(pick_kernel), (int)sizeof(PickShared))) return e;
     cudaLaunchConfig_t cfg{};
