@@ -388,22 +388,19 @@ namespace {
 // The arguments that the paged operators share; `what` names the caller.
 int check_paged(const char* what, int num_kv_heads, int head_dim, const int* page_table, int table_stride,
                 int num_seqs, const jyc_kv_pages* p) {
-    const std::string w = std::string(what) + ": ";
-    if (num_kv_heads <= 0) return arg_error(w + "num_kv_heads must be positive");
-    if (head_dim <= 0 || head_dim % 4 || head_dim > 256)
-        return arg_error(w + "head_dim must be a multiple of 4, <= 256");
-    if (num_seqs < 0 || table_stride < 0) return arg_error(w + "negative page table shape");
-    if (!page_table || !p || !p->k || !p->ks || !p->v || !p->vs) return arg_error(w + "null pointer");
-    if (p->num_pages <= 0 || p->page_size <= 0) return arg_error(w + "num_pages and page_size must be positive");
-    if ((long long)table_stride * p->page_size > 0x7fffffffLL)
-        return arg_error(w + "table_stride * page_size must fit an int");
+    auto bad = [&](const char* msg) { return arg_error(std::string(what) + ": " + msg); };
+    if (num_kv_heads <= 0) return bad("num_kv_heads must be positive");
+    if (head_dim <= 0 || head_dim % 4 || head_dim > 256) return bad("head_dim must be a multiple of 4, <= 256");
+    if (num_seqs < 0 || table_stride < 0) return bad("negative page table shape");
+    if (!page_table || !p || !p->k || !p->ks || !p->v || !p->vs) return bad("null pointer");
+    if (p->num_pages <= 0 || p->page_size <= 0) return bad("num_pages and page_size must be positive");
+    if ((long long)table_stride * p->page_size > 0x7fffffffLL) return bad("table_stride * page_size must fit an int");
     if (p->page_stride < 0 || p->pos_stride < 0 || p->head_stride < 0 || p->spage_stride < 0 || p->spos_stride < 0 ||
         p->shead_stride < 0)
-        return arg_error(w + "negative page stride");
+        return bad("negative page stride");
     if ((((uintptr_t)p->k | (uintptr_t)p->v) & 3) || ((p->page_stride | p->pos_stride | p->head_stride) & 3))
-        return arg_error(w + "k, v and their strides must be multiples of 4 bytes");
-    if ((((uintptr_t)p->ks | (uintptr_t)p->vs | (uintptr_t)page_table) & 3))
-        return arg_error(w + "misaligned scales or page table");
+        return bad("k, v and their strides must be multiples of 4 bytes");
+    if (((uintptr_t)p->ks | (uintptr_t)p->vs | (uintptr_t)page_table) & 3) return bad("misaligned scales or page table");
     return JYC_OK;
 }
 
@@ -429,7 +426,7 @@ JYC_API int jyc_kv_append_paged_q8(const float* K, const float* V, int ld, int r
     if (!row_seq && rows > num_seqs) return arg_error("kv_append_paged_q8: more rows than sequences without row_seq");
     if (rows == 0) return JYC_OK;
     if (!K || !V || !row_pos) return arg_error("kv_append_paged_q8: null pointer");
-    const PagedKV kv{*pages, page_table, table_stride, num_seqs};
+    const PagedKV kv{*pages, page_table, table_stride, num_seqs, fast_div(pages->page_size)};
     return launch_paged_append(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv,
                                PagedRope{cos_table, sin_table, rope_len}, S(stream));
 }
@@ -444,7 +441,7 @@ JYC_API int jyc_kv_read_paged_q8(float* K, float* V, int ld, int rows, int num_k
     if (!row_seq && rows > num_seqs) return arg_error("kv_read_paged_q8: more rows than sequences without row_seq");
     if (rows == 0) return JYC_OK;
     if (!K || !V || !row_pos) return arg_error("kv_read_paged_q8: null pointer");
-    const PagedKV kv{*pages, page_table, table_stride, num_seqs};
+    const PagedKV kv{*pages, page_table, table_stride, num_seqs, fast_div(pages->page_size)};
     return launch_paged_read(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv, S(stream));
 }
 
@@ -478,7 +475,7 @@ JYC_API int jyc_attention_paged_q8(const float* Q, int ldq, float* out, int ldo,
     PagedAttn a{};
     a.Q = Q; a.ldq = ldq; a.out = out; a.ldo = ldo;
     a.H = num_heads; a.KV = num_kv_heads; a.hd = head_dim; a.lens = seq_lens;
-    a.kv = PagedKV{*pages, page_table, table_stride, num_seqs};
+    a.kv = PagedKV{*pages, page_table, table_stride, num_seqs, fast_div(pages->page_size)};
     a.rope = PagedRope{cos_table, sin_table, rope_len};
     a.scale = 1.0f / sqrtf((float)head_dim);
     Scratch sc(S(stream));

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <mutex>
 
 namespace jyc {
@@ -61,19 +62,23 @@ __device__ __forceinline__ void paged_flag(int bit) {
     if ((*(volatile int*)&g_paged_err & bit) == 0) atomicOr(&g_paged_err, bit);
 }
 
-// Page id of position `pos` of sequence `seq`, -1 (and the error word) when
-// the sequence, the position or the id is out of range.
-__device__ __forceinline__ int paged_page(const PagedKV& kv, int seq, int pos) {
-    if (seq < 0 || seq >= kv.num_seqs || pos / kv.p.page_size >= kv.table_stride) {
+// Table entry of position `pos` of sequence `seq`, -1 (and the error word)
+// when the sequence or the position is out of range; *slot: its place there.
+__device__ __forceinline__ int paged_entry(const PagedKV& kv, int seq, int pos, int* slot) {
+    const int idx = kv.by_page(pos);
+    *slot = pos - idx * kv.p.page_size;
+    if (seq < 0 || seq >= kv.num_seqs || idx >= kv.table_stride) {
         paged_flag(kPagedErrPos);
         return -1;
     }
-    const int page = kv.table[(size_t)seq * kv.table_stride + pos / kv.p.page_size];
-    if (page < 0 || page >= kv.p.num_pages) {
-        paged_flag(kPagedErrPage);
-        return -1;
-    }
-    return page;
+    const int page = __ldg(kv.table + (size_t)seq * kv.table_stride + idx);
+    return page == -1 ? INT_MIN : page;  // -1: already flagged
+}
+// Whether an entry is a page; flags one that is not.
+__device__ __forceinline__ bool paged_valid(const PagedKV& kv, int page) {
+    if (page >= 0 && page < kv.p.num_pages) return true;
+    if (page != -1) paged_flag(kPagedErrPage);
+    return false;
 }
 __device__ __forceinline__ size_t paged_off(const PagedKV& kv, int page, int slot, int h) {
     return (size_t)((long long)page * kv.p.page_stride + (long long)slot * kv.p.pos_stride +
@@ -107,36 +112,54 @@ __device__ __forceinline__ float4 rotate4(float4 x, float2 c, float2 s) {
 __device__ __forceinline__ float amax4(float4 x) {
     return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 }
+// q8_round of four values without its clamp: |x| <= amax and inv <= 127 / amax
+// (1 + 2^-24), so the product stays below 127.5 (and a NaN, or an infinity
+// times inv = 0, converts to 0 as there).
 __device__ __forceinline__ uint32_t pack4(float4 x, float inv) {
-    return (uint32_t)(q8_round(x.x, inv) & 255) | ((uint32_t)(q8_round(x.y, inv) & 255) << 8) |
-           ((uint32_t)(q8_round(x.z, inv) & 255) << 16) | ((uint32_t)(q8_round(x.w, inv) & 255) << 24);
+    const int a = __float2int_rn(__fmul_rn(x.x, inv)), b = __float2int_rn(__fmul_rn(x.y, inv));
+    const int c = __float2int_rn(__fmul_rn(x.z, inv)), d = __float2int_rn(__fmul_rn(x.w, inv));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // ---------------------------------------------------------------------------
 // Append and read back: bound by their bytes (append reads 8 hd and writes 2 hd
-// + 8 per row and kv head, read the reverse). A unit is one head of K or of V of
-// one row; LANES lanes hold a unit, QUADS groups of four dims each, so a warp
-// has 32 / LANES units side by side (neighbouring heads: whole sectors) and
-// kRowUnits of them in flight, whose loads are all issued before the first is
-// used; only where a unit goes waits for its row's position and page.
+// + 8 per row and kv head, read the reverse), once the bookkeeping of a row is
+// shared: a warp takes kRowUnits * (32 / LANES) heads of K or of V of one row.
+// LANES lanes hold a head, QUADS groups of four dims each; neighbouring heads
+// lie side by side in a warp (whole sectors), and the loads of all units are
+// issued before the first is used; only where a unit goes waits for the row's
+// position and page. (A warp of heads of several rows, each with its own
+// position, page and 64-bit offsets, executes 265 instructions per head of 128
+// and is bound by them: 82 us for 16384 rows of 8 heads.)
 constexpr int kRowUnits = 4, kRowThreads = 256;
 
-struct RowUnit {
-    int row, head;
-    bool is_k, live;
-    int seq, pos;
+struct RowWarp {
+    int row, head;  // first head of this lane
+    bool is_k;
+    int page, slot; // page: as paged_entry returns it, -1: nothing to do
+    int pos;
 };
 template <int LANES>
-__device__ __forceinline__ RowUnit row_unit(long long u, int rows, int KV, const int* row_seq, const int* row_pos) {
-    RowUnit x;
-    x.live = u < (long long)rows * KV * 2;
-    x.row = x.live ? (int)(u / (KV * 2)) : 0;
-    const int r = x.live ? (int)(u - (long long)x.row * KV * 2) : 0;
-    x.is_k = r < KV;
-    x.head = x.is_k ? r : r - KV;
-    x.pos = x.live ? __ldg(row_pos + x.row) : -1;
-    x.seq = row_seq && x.live ? __ldg(row_seq + x.row) : x.row;
-    x.live = x.live && x.pos >= 0;
+__device__ __forceinline__ RowWarp row_warp(int rows, int chunks, const FastDiv& by_row, const int* row_seq,
+                                            const int* row_pos, const PagedKV& kv, int rope_len) {
+    const int w = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    RowWarp x;
+    x.row = by_row(w);
+    const int r = w - x.row * 2 * chunks;
+    x.is_k = r < chunks;
+    x.head = (x.is_k ? r : r - chunks) * kRowUnits * (32 / LANES) + lane / LANES;
+    x.page = -1;
+    x.pos = -1;
+    x.slot = 0;
+    if (x.row >= rows) return x;
+    x.pos = __ldg(row_pos + x.row);
+    const int seq = row_seq ? __ldg(row_seq + x.row) : x.row;
+    if (x.pos < 0) return x;
+    if (rope_len >= 0 && x.pos >= rope_len) {
+        paged_flag(kPagedErrRope);
+        return x;
+    }
+    x.page = paged_entry(kv, seq, x.pos, &x.slot);
     return x;
 }
 
@@ -144,52 +167,53 @@ template <int LANES, int QUADS>
 __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(const float* K, const float* V, int ld, int rows,
                                                                    int KV, int hd, const int* row_seq,
                                                                    const int* row_pos, PagedKV kv, PagedRope rope,
-                                                                   bool vec) {
+                                                                   int chunks, FastDiv by_row, bool vec) {
     constexpr int SIDE = 32 / LANES;
-    const int lane = threadIdx.x & 31, sub = lane & (LANES - 1), half = hd >> 1, nq = hd >> 2;
-    const long long w = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-    RowUnit x[kRowUnits];
+    const int sub = threadIdx.x & (LANES - 1), half = hd >> 1, nq = hd >> 2;
+    const bool tables = rope.cos_t != nullptr;
+    const RowWarp x = row_warp<LANES>(rows, chunks, by_row, row_seq, row_pos, kv, tables ? rope.len : -1);
+    if (x.page == -1) return;
     float4 v[kRowUnits][QUADS];
+    float2 c[QUADS], sn[QUADS];
+    const float* src = (x.is_k ? K : V) + (size_t)x.row * ld + (size_t)x.head * hd;
 #pragma unroll
-    for (int i = 0; i < kRowUnits; i++) {
-        x[i] = row_unit<LANES>((w * kRowUnits + i) * SIDE + lane / LANES, rows, KV, row_seq, row_pos);
-        const float* src = (x[i].is_k ? K : V) + (size_t)x[i].row * ld + (size_t)x[i].head * hd;
+    for (int i = 0; i < kRowUnits; i++)
 #pragma unroll
         for (int t = 0; t < QUADS; t++) {
             const int qd = sub + LANES * t;
-            v[i][t] = qd < nq ? load4(src + 4 * qd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[i][t] = qd < nq && x.head + i * SIDE < KV ? load4(src + i * SIDE * hd + 4 * qd, vec)
+                                                        : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+    const bool rot = tables && x.is_k;
+#pragma unroll
+    for (int t = 0; t < QUADS; t++) {
+        const int qd = sub + LANES * t;
+        const bool use = rot && qd < nq;
+        c[t] = use ? load2(rope.cos_t + (size_t)x.pos * half + 2 * qd, vec) : make_float2(1.0f, 1.0f);
+        sn[t] = use ? load2(rope.sin_t + (size_t)x.pos * half + 2 * qd, vec) : make_float2(0.0f, 0.0f);
     }
+    if (!paged_valid(kv, x.page)) return;
+    int8_t* dst = (x.is_k ? kv.p.k : kv.p.v) + paged_off(kv, x.page, x.slot, x.head);
+    float* sc = (x.is_k ? kv.p.ks : kv.p.vs) + paged_soff(kv, x.page, x.slot, x.head);
 #pragma unroll
     for (int i = 0; i < kRowUnits; i++) {
-        int page = -1;
-        if (x[i].live) page = paged_page(kv, x[i].seq, x[i].pos);
-        if (page >= 0 && rope.cos_t != nullptr && x[i].pos >= rope.len) {
-            paged_flag(kPagedErrRope);
-            page = -1;
-        }
-        const bool rot = rope.cos_t != nullptr && x[i].is_k && page >= 0;
         float amax = 0.0f;
 #pragma unroll
         for (int t = 0; t < QUADS; t++) {
-            const int qd = sub + LANES * t;
-            if (rot && qd < nq) {
-                const size_t at = (size_t)x[i].pos * half + 2 * qd;
-                v[i][t] = rotate4(v[i][t], load2(rope.cos_t + at, vec), load2(rope.sin_t + at, vec));
-            }
+            if (rot) v[i][t] = rotate4(v[i][t], c[t], sn[t]);
             amax = fmaxf(amax, amax4(v[i][t]));
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (page < 0) continue;
-        const int slot = x[i].pos % kv.p.page_size;
+        if (x.head + i * SIDE >= KV) continue;
         const float inv = q8_inv(amax);
-        uint32_t* dst = reinterpret_cast<uint32_t*>((x[i].is_k ? kv.p.k : kv.p.v) + paged_off(kv, page, slot, x[i].head));
-        if (sub == 0) (x[i].is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, x[i].head)] = q8_scale(amax);
+        if (sub == 0) sc[i * SIDE * kv.p.shead_stride] = q8_scale(amax);
 #pragma unroll
         for (int t = 0; t < QUADS; t++) {
             const int qd = sub + LANES * t;
-            if (qd < nq) dst[rot ? rope_slot(2 * qd, half) >> 1 : qd] = pack4(v[i][t], inv);
+            if (qd < nq)
+                *reinterpret_cast<uint32_t*>(dst + i * SIDE * kv.p.head_stride +
+                                             4 * (rot ? rope_slot(2 * qd, half) >> 1 : qd)) = pack4(v[i][t], inv);
         }
     }
 }
@@ -197,34 +221,31 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(const float* 
 template <int LANES, int QUADS>
 __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float* V, int ld, int rows, int KV, int hd,
                                                                  const int* row_seq, const int* row_pos, PagedKV kv,
-                                                                 bool vec) {
+                                                                 int chunks, FastDiv by_row, bool vec) {
     constexpr int SIDE = 32 / LANES;
-    const int lane = threadIdx.x & 31, sub = lane & (LANES - 1), nq = hd >> 2;
-    const long long w = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-    RowUnit x[kRowUnits];
+    const int sub = threadIdx.x & (LANES - 1), nq = hd >> 2;
+    const RowWarp x = row_warp<LANES>(rows, chunks, by_row, row_seq, row_pos, kv, -1);
+    if (x.page == -1 || !paged_valid(kv, x.page)) return;
+    const int8_t* src = (x.is_k ? kv.p.k : kv.p.v) + paged_off(kv, x.page, x.slot, x.head);
+    const float* scp = (x.is_k ? kv.p.ks : kv.p.vs) + paged_soff(kv, x.page, x.slot, x.head);
     uint32_t v[kRowUnits][QUADS];
     float sc[kRowUnits];
 #pragma unroll
-    for (int i = 0; i < kRowUnits; i++)
-        x[i] = row_unit<LANES>((w * kRowUnits + i) * SIDE + lane / LANES, rows, KV, row_seq, row_pos);
-#pragma unroll
     for (int i = 0; i < kRowUnits; i++) {
-        const int page = x[i].live ? paged_page(kv, x[i].seq, x[i].pos) : -1;
-        x[i].live = page >= 0;
-        const int slot = x[i].pos % kv.p.page_size;
-        const uint32_t* src = reinterpret_cast<const uint32_t*>((x[i].is_k ? kv.p.k : kv.p.v) +
-                                                                (x[i].live ? paged_off(kv, page, slot, x[i].head) : 0));
-        sc[i] = x[i].live ? (x[i].is_k ? kv.p.ks : kv.p.vs)[paged_soff(kv, page, slot, x[i].head)] : 0.0f;
+        const bool live = x.head + i * SIDE < KV;
+        sc[i] = live ? __ldg(scp + i * SIDE * kv.p.shead_stride) : 0.0f;
 #pragma unroll
         for (int t = 0; t < QUADS; t++) {
             const int qd = sub + LANES * t;
-            v[i][t] = x[i].live && qd < nq ? src[qd] : 0u;
+            v[i][t] = live && qd < nq
+                          ? __ldg(reinterpret_cast<const uint32_t*>(src + i * SIDE * kv.p.head_stride) + qd)
+                          : 0u;
         }
     }
+    float* dst = (x.is_k ? K : V) + (size_t)x.row * ld + (size_t)x.head * hd;
 #pragma unroll
     for (int i = 0; i < kRowUnits; i++) {
-        if (!x[i].live) continue;
-        float* dst = (x[i].is_k ? K : V) + (size_t)x[i].row * ld + (size_t)x[i].head * hd;
+        if (x.head + i * SIDE >= KV) continue;
 #pragma unroll
         for (int t = 0; t < QUADS; t++) {
             const int qd = sub + LANES * t;
@@ -233,11 +254,12 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float
             u8x4_to_f32(v[i][t] ^ 0x80808080u, f);
 #pragma unroll
             for (int j = 0; j < 4; j++) f[j] = __fmul_rn(f[j], sc[i]);
+            float* to = dst + i * SIDE * hd + 4 * qd;
             if (vec)
-                *reinterpret_cast<float4*>(dst + 4 * qd) = make_float4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
             else
 #pragma unroll
-                for (int j = 0; j < 4; j++) dst[4 * qd + j] = f[j];
+                for (int j = 0; j < 4; j++) to[j] = f[j];
         }
     }
 }
@@ -405,8 +427,6 @@ struct PaPlan {
     bool wide_copy; // 16-byte copies
     bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
     int box;        // keys of a tensor copy
-    uint32_t div_m; // pos / page_size = pos * div_m >> div_s, for pos < 2^31
-    int div_s;
 };
 // The line cut into runs: worker w starts at w * base + min(w, rest).
 struct PaLine {
@@ -705,7 +725,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 hsoff = (long long)h * a.kv.p.shead_stride;
             }
             if (lane < TK && pos < nx.len) {
-                const int idx = (int)(((unsigned long long)pos * pl.div_m) >> pl.div_s);
+                const int idx = a.kv.by_page(pos);
                 slot = pos - idx * a.kv.p.page_size;
                 pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
                 ok = true;
@@ -1317,6 +1337,15 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn
     }
 }
 
+// The cache of rows r0, r0 + 1, ... when a row is its own sequence.
+PagedKV shifted(PagedKV kv, const int* row_seq, int r0) {
+    if (!row_seq) {
+        kv.table += (size_t)r0 * kv.table_stride;
+        kv.num_seqs -= r0;
+    }
+    return kv;
+}
+
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 template <int HDP, int HEADS, bool TMA>
@@ -1406,32 +1435,47 @@ bool aligned8(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t
 
 }  // namespace
 
-// Lanes of a unit and quads of a lane by head size.
-#define ROW_CASES(KERNEL, ...)                                                                     \
-    do {                                                                                           \
-        const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : 32, per = kRowUnits * (32 / lanes);       \
-        const long long units = (long long)rows * KV * 2, warps = (units + per - 1) / per;         \
-        const unsigned grid = (unsigned)((warps + kRowThreads / 32 - 1) / (kRowThreads / 32));     \
-        if (hd <= 32) KERNEL<8, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                      \
-        else if (hd <= 64) KERNEL<16, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                \
-        else if (hd <= 128) KERNEL<32, 1><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);               \
-        else KERNEL<32, 2><<<grid, kRowThreads, 0, s>>>(__VA_ARGS__);                              \
-    } while (0)
+// Lanes of a head and quads of a lane by head size; rows in launches of fewer
+// than 2^30 warps. f(first row, rows, CTAs, warps that share K or V of a row).
+template <class F>
+static int row_launches(int rows, int KV, int hd, F f) {
+    const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : 32, per = kRowUnits * (32 / lanes), chunks = (KV + per - 1) / per;
+    const int most = std::max(1, (1 << 30) / (2 * chunks)), warps = kRowThreads / 32;
+    for (int r0 = 0; r0 < rows; r0 += most) {
+        const int n = std::min(most, rows - r0);
+        f(r0, n, (unsigned)(((long long)n * 2 * chunks + warps - 1) / warps), chunks);
+        JYC_LAUNCHED();
+        if (rows - r0 <= most) break;
+    }
+    return JYC_OK;
+}
 
 int launch_paged_append(const float* K, const float* V, int ld, int rows, int KV, int hd, const int* row_seq,
                         const int* row_pos, const PagedKV& kv, const PagedRope& rope, cudaStream_t s) {
     const bool vec = aligned16(K, ld) && aligned16(V, ld) && aligned8(rope.cos_t, rope.sin_t);
-    ROW_CASES(paged_append_kernel, K, V, ld, rows, KV, hd, row_seq, row_pos, kv, rope, vec);
-    JYC_LAUNCHED();
-    return JYC_OK;
+    const auto kernel = hd <= 32    ? paged_append_kernel<8, 1>
+                        : hd <= 64  ? paged_append_kernel<16, 1>
+                        : hd <= 128 ? paged_append_kernel<32, 1>
+                                    : paged_append_kernel<32, 2>;
+    return row_launches(rows, KV, hd, [&](int r0, int n, unsigned grid, int chunks) {
+        kernel<<<grid, kRowThreads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
+                                            row_seq ? row_seq + r0 : nullptr, row_pos + r0, shifted(kv, row_seq, r0),
+                                            rope, chunks, fast_div(2 * chunks), vec);
+    });
 }
 
 int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, const int* row_seq, const int* row_pos,
                       const PagedKV& kv, cudaStream_t s) {
     const bool vec = aligned16(K, ld) && aligned16(V, ld);
-    ROW_CASES(paged_read_kernel, K, V, ld, rows, KV, hd, row_seq, row_pos, kv, vec);
-    JYC_LAUNCHED();
-    return JYC_OK;
+    const auto kernel = hd <= 32    ? paged_read_kernel<8, 1>
+                        : hd <= 64  ? paged_read_kernel<16, 1>
+                        : hd <= 128 ? paged_read_kernel<32, 1>
+                                    : paged_read_kernel<32, 2>;
+    return row_launches(rows, KV, hd, [&](int r0, int n, unsigned grid, int chunks) {
+        kernel<<<grid, kRowThreads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
+                                            row_seq ? row_seq + r0 : nullptr, row_pos + r0, shifted(kv, row_seq, r0),
+                                            chunks, fast_div(2 * chunks), vec);
+    });
 }
 
 // The instantiation of a shape: head size and query heads per unit rounded up,
@@ -1471,12 +1515,6 @@ int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
     pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
     pl.units_row = KV * pl.qblocks;
     pl.wide_q = aligned16(a.Q, a.ldq) && aligned8(a.rope.cos_t, a.rope.sin_t);
-    // n / d for n < 2^31: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), m d - 2^(31+s) < d <= 2^s, so the
-    // error of n m / 2^(31+s) is below 2^-31 n < 1 / d at every n; m < 2^32
-    int sh = 0;
-    while ((1LL << sh) < a.kv.p.page_size) sh++;
-    pl.div_s = 31 + sh;
-    pl.div_m = (uint32_t)(((1ULL << pl.div_s) + a.kv.p.page_size - 1) / a.kv.p.page_size);
     const jyc_kv_pages& p = a.kv.p;
     pl.wide_copy = hd % 16 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
                    ((p.page_stride | p.pos_stride | p.head_stride) & 15) == 0;

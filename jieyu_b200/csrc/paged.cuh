@@ -6,6 +6,19 @@
 
 namespace jyc {
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d) < 2^32, m d -
+// 2^(31+s) < d <= 2^s, so n m / 2^(31+s) is above n / d by less than n 2^-31 / d < 1 / d.
+struct FastDiv {
+    uint32_t m;
+    int s;
+    __device__ __forceinline__ int operator()(int n) const { return (int)(((unsigned long long)(uint32_t)n * m) >> s); }
+};
+inline FastDiv fast_div(int d) {
+    int s = 0;
+    while ((1LL << s) < d) s++;
+    return FastDiv{(uint32_t)(((1ULL << (31 + s)) + (unsigned)d - 1) / (unsigned)d), 31 + s};
+}
+
 // Where a position of a sequence lives: page id = table[seq * table_stride +
 // pos / page_size], then the strides of jyc_kv_pages.
 struct PagedKV {
@@ -13,6 +26,7 @@ struct PagedKV {
     const int* table;
     int table_stride;  // table entries per sequence
     int num_seqs;
+    FastDiv by_page;   // position / page_size
 };
 
 struct PagedRope {
