@@ -271,7 +271,8 @@ typedef struct jyc_kv_pages {
 /* Position p of sequence s is slot p % page_size of page
  * page_table[s * table_stride + p / page_size] (int32, num_seqs rows of
  * table_stride entries, so a sequence holds at most table_stride * page_size
- * positions). Entries behind a sequence's last position are not read.
+ * positions; their product is below 2^31 - 255). Entries behind a sequence's
+ * last position are not read.
  * Positions, lengths and page ids lie on the device, where the kernels check
  * them: what is out of range is never read or written and sets the paged error
  * word (jyc_paged_error). */
@@ -301,7 +302,8 @@ JYC_API int jyc_kv_read_paged_q8(float* K, float* V, int ld, int rows, int num_k
  * and V are in the cache already), keys 0 .. seq_lens[s] - 1, out row s at
  * out + s * ldo. The query is quantised per head and scored as in
  * jyc_attention_q8 (int32 dots, dot * ((ks * qs) * 1/sqrt(head_dim)), fp32
- * softmax, V scaled by vs). cos/sin tables: the query is rotated by its
+ * softmax, V scaled by vs; scales are not negative, and one that is not finite
+ * makes the rows that attend to it NaN). cos/sin tables: the query is rotated by its
  * position first; NULL: it arrives rotated. A sequence of length <= 0 gets a
  * row of zeros, as does one whose query position lies behind the tables; a
  * length above table_stride * page_size is cut to that; keys on a page that is

@@ -394,7 +394,8 @@ int check_paged(const char* what, int num_kv_heads, int head_dim, const int* pag
     if (num_seqs < 0 || table_stride < 0) return bad("negative page table shape");
     if (!page_table || !p || !p->k || !p->ks || !p->v || !p->vs) return bad("null pointer");
     if (p->num_pages <= 0 || p->page_size <= 0) return bad("num_pages and page_size must be positive");
-    if ((long long)table_stride * p->page_size > 0x7fffffffLL) return bad("table_stride * page_size must fit an int");
+    if ((long long)table_stride * p->page_size > 0x7fffff00LL)
+        return bad("table_stride * page_size must be below 2^31 - 255");
     if (p->page_stride < 0 || p->pos_stride < 0 || p->head_stride < 0 || p->spage_stride < 0 || p->spos_stride < 0 ||
         p->shead_stride < 0)
         return bad("negative page stride");

@@ -11,19 +11,25 @@
 // A row belongs to a cluster of 1 to 8 CTAs that exchange through distributed
 // shared memory, so one launch serves one row or hundreds. Nothing is sorted.
 //   1  the maximum (a greedy row ends here); every lane keeps four maxima.
-//   2  a bin of (max - l) / T such that the tokens up to it are few and hold the
-//      kept set: with top-k by the k-th of those maxima (as many logits are as
-//      large), with min-p by min_p itself, with top-p a guess that is checked.
-//      One pass puts those tokens, in index order, into pools (one per warp).
+//   2  a bin of (max - l) / T such that the tokens up to it hold the kept set and
+//      are as few as can be told: with top-k from the k-th of those maxima (as
+//      many logits are as large), with min-p from min_p itself, with top-p from a
+//      bound on the mass of all smaller ones. One pass puts those tokens, in index
+//      order, into pools (one per warp), sums all weights and adds the pools' to a
+//      histogram of the bins (fp32 shares in fixed point: bounds of 4e-5).
 //   3  pools of 4096 tokens in all or fewer: one CTA takes them and ends the row,
 //      finding each border by bisection over keys.
-//      More: a histogram over the bins bounds the running count or mass, the
-//      tokens of the one or two bins where the border may lie are ranked (or
-//      split again while they are too many), and the kept weights are summed
-//      in index order, warp by warp, then token by token where the draw falls.
-//   Rows without a filter, and rows whose pools overflow or miss the border, go
+//      More: the histogram bounds the running count or mass, so the border lies in
+//      one or two bins; their tokens go to one CTA (or are split again while they
+//      are more than 512), which finds the last kept one by bisection. The kept
+//      weights are summed by warp, in index order; the warp that the draw falls in
+//      walks its tokens.
+//   Rows without a filter, with k above 2048, and rows whose pools overflow go
 //   through 3 over all their logits instead of the pools.
-// Floor: one read of the logits. Later passes find them in L2.
+// Floor: one read of the logits; later passes find them in L2. What is left of
+// the time is the chain of passes and exchanges of a row (about 20 us for one row
+// with top-k, 55 with top-p alone), and with many rows the instructions of the
+// exact weights (22 per logit and pass, 11 of them in double precision).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -40,10 +46,10 @@ typedef unsigned long long u64;
 
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 constexpr int kPickList = 4096;      // tokens that one CTA ends a row with
-constexpr int kPickTopK = 1024;      // largest k bounded by maxima
+constexpr int kPickTopK = 2048;      // largest k bounded by maxima: as many as a CTA keeps
 constexpr int kPickPool = 1920;      // tokens of a warp's pool: two CTAs share an SM's memory
 constexpr int kPickPairs = 256;      // tokens whose top-p is decided by comparing all pairs
-constexpr int kPickRank = 512;       // tokens of a border that are ranked
+constexpr int kPickRank = 512;       // tokens among which one CTA looks for a border
 constexpr int kPickBins = 2048, kPickPer = kPickBins / kPickThreads;
 constexpr int kPickMaxCluster = 8;
 constexpr float kPickSpan = 40.0f;   // powers of two that the bins cover
@@ -295,7 +301,7 @@ __device__ void pick_total(PickRow& r) {
 
 // Where the prefix of {comp >= tau0} ends whose metric (number of tokens, or mass) first reaches `target`:
 // the comp of its last token. s->hist holds this CTA's histogram of the bins: tokens, or for a mass their
-// weights over the bin's largest, in units of 1 / unit.
+// weights over that of the bin's middle, in units of 1 / unit.
 // *kept: the metric that this warp's tokens have in the prefix.
 __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit, u64 tau0, u64* kept) {
     PickShared* s = r.s;
@@ -698,7 +704,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         float part = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (m4[j] > -INFINITY) part += exp2f(-__fmul_rn(__fsub_rn(r.mx, m4[j]), (float)r.c));
+            if (m4[j] > -INFINITY) {
+                const float d = __fsub_rn(r.mx, m4[j]);
+                part += d == 0.0f ? 1.0f : exp2f(-__fmul_rn(d, (float)r.c));
+            }
         const double M = fmax(1.0, 0.99 / kOne * (double)pick_sum(r, (u64)(part * (float)kOne)));
         const double e = log2((double)V / ((1.0 - (double)P) * M));
         most = max(0, min(kPickBins - 1, (int)(e * (kPickBins / (double)kPickSpan)) + 1));
@@ -810,7 +819,6 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         }
         const int found = pick_collect(r, fits ? total : kPickList + 1u, kPickList);
         if (found >= 0) {
-            if (tid == 0) s->tau = 1ull;
             bool done = true;
             if (r.rank == 0) done = pick_short(a, r, row, found, by_k ? K : found, P, mp, rest);
             if (!sums) return;
@@ -930,8 +938,11 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
 
 }  // namespace
 
-// CTAs of a row: as many as fill the machine once at two CTAs per SM, while a
-// CTA keeps 4096 logits or more.
+// CTAs of a row: up to 8 CTAs per SM in all, while a CTA keeps 4096 logits or
+// more. Rows differ in their work, so many small CTAs even it out (256 mixed
+// rows of 128256: 347 us with one CTA each, 265 with four; 64 rows of top-p
+// alone: 148 with four, 158 with eight); below 4096 logits the exchanges cost
+// more than the passes (62 rows of 14783, k = 1150: 58 us, 80 at 2048).
 int launch_pick(const PickArgs& a, cudaStream_t s) {
     if (a.rows == 0) return JYC_OK;
     const int sms = sm_count();

@@ -272,6 +272,43 @@ def test_attention_many_and_long(cuda, B, longest):
     _check(torch, pool, q, lens, H, host(out), rows=rows)
 
 
+def test_attention_sums_of_very_long_runs(cuda):
+    """Runs of more than 2000 units of 32 keys with the largest digits there are: equal scores, every
+    V byte 127. 1300 sequences of 131072 positions share one set of pages."""
+    torch = cuda
+    H, KV, hd, page, n, B = 2, 1, 64, 64, 131072, 1300
+    pool = P.Pool(torch, n // page, page, KV, hd, np.tile(np.arange(n // page), (B, 1)))
+    pool.v8.fill_(127)
+    pool.ks.fill_(0.01)
+    pool.vs.fill_(0.015)  # just below 2^-6: its weights have the largest fractions
+    pool.k8.fill_(3)
+    q = torch.randn(B, H * hd, device="cuda")
+    out = torch.empty(B, H * hd, device="cuda")
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    _capi.check(P.attend(torch, pool, q, out, H, lens, work=P.workspace(torch, B, H, KV, hd)))
+    want = 127 * float(np.float32(0.015))
+    # equal weights: the quotient of two sums, each of n / 32 rounded partial sums at most
+    assert np.abs(host(out) - want).max() <= want * P.U24 * (2 * n / 32 + 64)
+
+
+def test_attention_scales_that_are_not_finite(cuda):
+    """A NaN or infinite scale of a key in range makes its heads' rows NaN, and no other row."""
+    torch = cuda
+    H, KV, hd, page = 8, 2, 64, 16
+    rng = np.random.default_rng(3)
+    for name, value in (("ks", np.nan), ("vs", np.nan), ("vs", np.inf)):
+        pool = P.Pool(torch, 6, page, KV, hd, np.arange(6).reshape(2, 3))
+        for b in range(2):
+            pool.put_random(rng, b, 48)
+        getattr(pool, "ks" if name == "ks" else "vs")[1, 5, 0] = value  # sequence 0, position 21, kv head 0
+        q = rng.normal(size=(2, H * hd)).astype(np.float32)
+        out = torch.empty(2, H * hd, device="cuda")
+        lens = dev(torch, np.array([40, 48], np.int32))
+        _capi.check(P.attend(torch, pool, dev(torch, q), out, H, lens, work=P.workspace(torch, 2, H, KV, hd)))
+        got = host(out).reshape(2, H, hd)
+        assert np.isnan(got[0, :4]).all() and np.isfinite(got[0, 4:]).all() and np.isfinite(got[1]).all()
+
+
 def test_attention_wide_range_of_scales(cuda):
     """V scales over 12 decades: the key with all the weight has the smallest one."""
     torch = cuda

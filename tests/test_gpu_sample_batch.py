@@ -118,6 +118,20 @@ def test_large(cuda, rows, V):
          np.where(i % 2 == 0, 0.9, 1.0), np.where(i % 7 == 2, 0.05, 0.0), rng.random(rows).astype(np.float32))
 
 
+def test_large_k_and_hot_rows(cuda):
+    """k around the largest that a CTA's maxima bound (2048) and beyond it, temperatures that leave one
+    token or all of them, and top-p next to 1."""
+    rng = np.random.default_rng(11)
+    V = 50000
+    k = [1023, 1024, 1025, 2047, 2048, 2049, 4000, 49999, 0, 0, 0, 0, 0, 3000, 2048, 700]
+    n = len(k)
+    l = _logits(rng, n, V, "plain")
+    T = [1.0, 0.7, 1.3, 1.0, 2.0, 1.0, 1.0, 1.0, 1e-38, 1e-30, 1e4, 30.0, 1.3, 1.0, 5.0, 1e30]
+    p = [1.0, 0.9, 1.0, 0.99, 1.0, 0.5, 0.95, 0.9, 0.9, 1.0, 0.7, 0.99, 1 - 2.0 ** -24, 1 - 2.0 ** -23, 0.9, 0.3]
+    for mp in (0.0, 1e-4):
+        _run(cuda, l, T, k, p, [mp] * n, rng.random(n).astype(np.float32))
+
+
 @pytest.mark.parametrize("kind", ["flat", "equal", "bf16", "two"])
 def test_large_and_flat(cuda, kind):
     """Borders that fall among tens of thousands of (nearly) equal logits."""
