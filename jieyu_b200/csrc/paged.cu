@@ -271,40 +271,43 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float
 // one pass over the keys with a running reference. In base 2, with vs_j =
 // 2^e_j f_j (1 <= f_j < 2): b_j = 2^(s_j - ref), w_j = b_j vs_j < 2^(1 + s_j +
 // e_j - ref). The reference follows the maximum of s_j + e_j, not of s_j, so
-// that the weights neither overflow a format of limited range (integers, or
-// pairs of fp16 with 22 bits) nor lose a small vs that carries all the weight;
-// the denominator adds the b_j.
+// that the weights neither overflow pairs of fp16 (22 bits) nor lose a small vs
+// that carries all the weight; the denominator adds the b_j.
 //
 // A step reads sum(len) * KV * (2 hd + 8) bytes and is bound by them, so: work
-// is a line of units (a unit: TK keys of one kv head of one sequence), cut into equal runs for all resident warps whatever the lengths; a
-// warp keeps its next units in flight in its own ring in shared memory across
-// the borders of sequences and has no barrier in its loop. Heads of 64 or 128
-// on pages that divide a unit or that units divide come by one tensor copy per
-// page, K and V each; other shapes by 16- or 4-byte cp.async.
+// is a line of units (a unit: TK keys of one kv head of one sequence), cut into
+// equal runs for all resident warps whatever the lengths; a warp keeps its next
+// units in flight in its own ring in shared memory across the borders of
+// sequences and has no barrier in its loop. Heads of 64 or 128 on pages that
+// divide a unit or that units divide come by one tensor copy per page, K and V
+// each; other shapes by 16- or 4-byte cp.async.
 // Keys are the rows of both products and the query heads of a kv head the
 // columns: S^T = K Q^T with mma.m16n8k32 s8 (exact dots), then O^T = V^T P^T,
 // the weights transposed between them by movmatrix.
 //
-// Up to 8 heads of up to 128 dims: the weights are rounded to 31-bit integers
-// (reference 27 below the maximum, raised when a weight would pass 2^30 times
-// the reference), whose four bytes are columns of an integer product with V's
-// own bytes: mma.m16n8k32 s8 x u8, exact, summed in 32-bit integers over up to
-// 2000 units; a rounding is 2^-28 of the largest weight at most. V needs no
-// conversion (a byte permute), and no accumulator is touched between units.
-// Beyond that the integers would not fit the registers: hi and lo halves of
-// the weights and mma.m16n8k16 f16 (V is exact in fp16); each unit's product
-// starts from zero and is added in fp32 with round to nearest (the tensor
-// cores' own sums may truncate).
+// The weights go in as fp16 halves hi + lo (22 bits; the largest is held
+// within 2^13 .. 2^14, so a lost bit is at most 2^-25, 2^-38 of it) against
+// V's bytes as fp16 (exact): mma.m16n8k16, each unit's product from zero and
+// added in fp32 with round to nearest (the tensor cores' own sums may
+// truncate). 4 heads fill 8 columns with their hi and lo halves: half the
+// products (heads of 96: 50 us against 54 with a column a head). Integer
+// weights (4 byte columns a head, V unconverted) were as fast at 4 heads and
+// slower at 8: 131072 keys of 8 x 128 89 us against 68.
 //
 // A run that covers an item (a kv head of a sequence) whole writes its rows of
 // out; the others leave parts (o, ref, l), which are joined inside the CTA where
 // the item ends in it (through shared memory when the CTA has one item only,
 // through the workspace otherwise), and by a second kernel where it does not:
 // one part per CTA that the item touches.
+//
+// Measured: 131072 keys of 8 x 128 67 us (floor 43; 7 TB/s while every warp
+// streams), 64 sequences of 2048 to 2176 keys of 8 x 64 43 us (floor 23), 45 of
+// 1 to 8192 keys of 8 x 128 83 us (floor 60). What is over the floor is the
+// ends: finding each warp's run in lens, Q and the page table before the first
+// key (8 us), the spread of the warps' ends and the joins (8), the second
+// kernel (4).
 
-constexpr float kPaShift = 13.0f;              // halves: the largest weight is in 2^13 .. 2^14
-constexpr float kPaSet = 27.0f, kPaMost = 30.0f;  // digits: 2^27 .. 2^28 when the reference is set, below 2^31 ever
-constexpr int kPaFlush = 2000;                 // units whose digit sums fit 32 bits: 32 * 255 * 128 each
+constexpr float kPaShift = 13.0f;    // the largest weight is in 2^13 .. 2^14
 constexpr float kPaLow = -1.7e38f;  // reference before any key: below every score, and its differences stay finite
 
 __device__ __forceinline__ float ex2(float x) {
@@ -320,12 +323,6 @@ __device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t
 }
 __device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-// c += a b, a signed, b unsigned bytes
-__device__ __forceinline__ void pa_mma_s8u8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -389,13 +386,12 @@ __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
 // query columns and unread output columns), HEADS the query heads of a unit.
 template <int HDP, int HEADS, bool TMA>
 struct PaCfg {
-    static constexpr bool DIG = HEADS <= 8 && HDP <= 128;  // weights as digits, else as halves
     static constexpr int TK = HDP <= 128 ? 32 : 16;        // keys of a unit
-    // one CTA per SM. Few warps with many units in flight each and room for every accumulator in registers beat more
-    // warps with fewer: 131072 keys of 8 x 128, 4 heads each, take 78 us with 12 warps of 2 stages, 62 with 8 of 3
-    static constexpr int WARPS = HDP <= 64 || (HDP <= 128 && HEADS == 16) ? 12 : 8;
-    static constexpr int ST = HDP <= 64 ? 4 : HDP <= 128 && HEADS == 16 ? 2 : 3;
-    static constexpr int NT = HEADS <= 4 ? 2 : 4;          // n8 tiles of digits: 4 digits of each head
+    // one CTA per SM. Above 64 dims few warps with more units in flight each and room for every accumulator in
+    // registers beat more warps with fewer: 131072 keys of 8 x 128, 4 heads each, take 78 us with 12 warps of 2
+    // stages, 66 with 8 of 3; 64 sequences of 2112 keys of 8 x 64 take 43 with 12 warps, 47 with 8
+    static constexpr int WARPS = HDP <= 64 ? 12 : 8;
+    static constexpr int ST = 3;
     static constexpr int E = HEADS <= 8 ? 1 : 2;           // n8 tiles of heads
     static constexpr int ROWS = HEADS;
     static constexpr int VOFF = TK * HDP, SOFF = 2 * TK * HDP, MOFF = SOFF + 8 * TK;
@@ -604,8 +600,7 @@ template <int HDP, int HEADS, bool TMA>
 __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work, const __grid_constant__ PaMaps maps) {
     using G = PaCfg<HDP, HEADS, TMA>;
-    constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS, E = G::E, NT = G::NT;
-    constexpr bool DIG = G::DIG;
+    constexpr int TK = G::TK, ST = G::ST, WARPS = G::WARPS, ROWS = G::ROWS, E = G::E;
     constexpr int NK = HDP / 32, NM = TK / 16, ND = HDP / 16;
     extern __shared__ __align__(128) unsigned char pa_raw[];
     unsigned char* const pa_sm = TMA ? pa_raw + (-smem_u32(pa_raw) & 1023u) : pa_raw;
@@ -825,29 +820,6 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     // 2 g + 1 of every 16
     uint32_t qf[NK][E][2];
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4];
-    int acc[DIG ? ND : 1][NT][4];
-    int summed = 0;  // units in acc
-    // digits of this lane's columns: bytes 0 and 2, or 1 and 3, of heads 2 t, 2 t + 1 (up to 4 heads: of heads
-    // 2 (t % 2), + 1); all four of them (up to 8)
-    const uint32_t pick = HEADS <= 4 && t >= 2 ? 0x7351 : 0x6240;
-    const float weigh = HEADS <= 4 && t >= 2 ? 256.0f : 1.0f;
-    auto settle = [&] {  // o += what acc holds
-#pragma unroll
-        for (int d = 0; d < (DIG ? ND : 0); d++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (HEADS <= 4) {
-                    o[d][0][j] += weigh * __fmaf_rn((float)acc[d][1][j], 65536.0f, (float)acc[d][0][j]);
-                } else {
-                    const float lo = __fmaf_rn((float)acc[d][1][j], 256.0f, (float)acc[d][0][j]);
-                    const float hi = __fmaf_rn((float)acc[d][NT - 1][j], 256.0f, (float)acc[d][NT - 2][j]);
-                    o[d][0][j] += __fmaf_rn(hi, 65536.0f, lo);
-                }
-#pragma unroll
-                for (int i = 0; i < NT; i++) acc[d][i][j] = 0;
-            }
-        summed = 0;
-    };
     bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
     int st = 0;
     uint32_t phase = 0u;
@@ -903,11 +875,6 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
             }
-#pragma unroll
-            for (int d = 0; d < (DIG ? ND : 0); d++)
-#pragma unroll
-                for (int i = 0; i < NT; i++) acc[d][i][0] = acc[d][i][1] = acc[d][i][2] = acc[d][i][3] = 0;
-            summed = 0;
         }
         bool in = false;
         float kscale, vscale;
@@ -985,144 +952,73 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             __syncwarp();
             issue_k(st);
         }
-        if constexpr (DIG) {
-            // a weight too large for the reference, or sums near the end of 32 bits: both are rare
-            const bool high = top[0][0] > ref[0][0] + kPaMost || top[0][1] > ref[0][1] + kPaMost;
-            if (__any_sync(0xffffffffu, high) || summed == kPaFlush) {
-                settle();
+        float al[E][2];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float x = top[0][j];
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = x > ref[0][j] + kPaMost ? x - kPaSet : ref[0][j];
-                    const float al = ex2(ref[0][j] - x);
-                    ref[0][j] = x;
-                    l[0][j] *= al;
+        for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        o[d][0][j] *= al;
-                        o[d][0][2 + j] *= al;
-                    }
-                }
+            for (int j = 0; j < 2; j++) {
+                float x = top[e][j];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(ref[e][j], x - kPaShift);
+                al[e][j] = ex2(ref[e][j] - x);
+                ref[e][j] = x;
+                l[e][j] *= al[e][j];
             }
-            summed++;
-            // weights as integers; their bytes, transposed, are B fragments: column g (a digit of a head), keys
-            // 16 m + 2 t, + 8, + 1, + 9
-            uint32_t pf[NT][2];
+        // weights, transposed into B fragments: column g, keys 16 m + 2 t, + 1 and 8 later. A column is a head;
+        // of 4 heads or fewer, columns 0-3 are the hi halves and 4-7 the lo halves of the same heads
+        uint32_t hi[NM][E][2], lo[NM][E][2];
 #pragma unroll
-            for (int m = 0; m < NM; m++) {
-                uint32_t w[2][2];
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const float bj = ex2(s[m][0][2 * i + j] - ref[0][j]);
-                        l[0][j] += bj;
-                        w[i][j] = __float2uint_rn(bj * vs[m][i]);
-                    }
-                if (HEADS <= 4) {
-                    const uint32_t x0 = __byte_perm(w[0][0], w[1][0], pick), x1 = __byte_perm(w[0][1], w[1][1], pick);
-                    pf[0][m] = pa_transpose(__byte_perm(x0, x1, 0x5410));
-                    pf[1][m] = pa_transpose(__byte_perm(x0, x1, 0x7632));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {  // bytes 2 i, 2 i + 1
-                        const uint32_t sel = i == 0 ? 0x5140 : 0x7362;
-                        const uint32_t x0 = __byte_perm(w[0][0], w[1][0], sel), x1 = __byte_perm(w[0][1], w[1][1], sel);
-                        pf[2 * i][m] = pa_transpose(__byte_perm(x0, x1, 0x5410));
-                        pf[2 * i + 1][m] = pa_transpose(__byte_perm(x0, x1, 0x7632));
-                    }
-                }
-            }
-            if constexpr (TMA)
-                if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
-            // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
-            // rows g of the tile, the odd ones rows g + 8
-#pragma unroll
-            for (int d = 0; d < ND; d += 2) {
-                uint32_t v[NM][4];
-#pragma unroll
-                for (int m = 0; m < NM; m++)
-                    pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v[m]);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t vf[4] = {__byte_perm(v[0][2 * i], v[0][2 * i + 1], 0x6240),
-                                            __byte_perm(v[0][2 * i], v[0][2 * i + 1], 0x7351),
-                                            __byte_perm(v[NM - 1][2 * i], v[NM - 1][2 * i + 1], 0x6240),
-                                            __byte_perm(v[NM - 1][2 * i], v[NM - 1][2 * i + 1], 0x7351)};
-#pragma unroll
-                    for (int n8 = 0; n8 < NT; n8++) pa_mma_s8u8(vf, pf[n8], acc[d + i][n8]);
-                }
-            }
-        } else {
-            float al[E][2];
+        for (int m = 0; m < NM; m++)
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float x = top[e][j];
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(ref[e][j], x - kPaShift);
-                    al[e][j] = ex2(ref[e][j] - x);
-                    ref[e][j] = x;
-                    l[e][j] *= al[e][j];
+                for (int i = 0; i < 2; i++) {
+                    const float b0 = ex2(s[m][e][2 * i] - ref[e][0]), b1 = ex2(s[m][e][2 * i + 1] - ref[e][1]);
+                    l[e][0] += b0;
+                    l[e][1] += b1;
+                    const float w0 = b0 * vs[m][i], w1 = b1 * vs[m][i];
+                    const uint32_t ph = pa_pack(w0, w1);
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
+                    const uint32_t pl2 = pa_pack(w0 - hf.x, w1 - hf.y);
+                    hi[m][e][i] = pa_transpose(HEADS <= 4 && t >= 2 ? pl2 : ph);
+                    if (HEADS > 4) lo[m][e][i] = pa_transpose(pl2);
                 }
-            // weights, transposed into B fragments: head g, keys 16 m + 2 t, + 1 and 8 later
-            uint32_t hi[NM][E][2], lo[NM][E][2];
+        if constexpr (TMA)
+            if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
+        // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
+        // rows g of the tile, the odd ones rows g + 8
 #pragma unroll
-            for (int m = 0; m < NM; m++)
+        for (int d = 0; d < ND; d += 2) {
+            float c[2][E][4];
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                uint32_t v[4];
+                pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t vf[4] = {pa_half2<false>(v[2 * i]), pa_half2<true>(v[2 * i]),
+                                            pa_half2<false>(v[2 * i + 1]), pa_half2<true>(v[2 * i + 1])};
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        if (m == 0)
+                            pa_mma_f16(vf, hi[m][e], 0.0f, c[i][e]);
+                        else
+                            pa_mma_f16(vf, hi[m][e], c[i][e]);
+                        if (HEADS > 4) pa_mma_f16(vf, lo[m][e], c[i][e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float b0 = ex2(s[m][e][2 * i] - ref[e][0]), b1 = ex2(s[m][e][2 * i + 1] - ref[e][1]);
-                        l[e][0] += b0;
-                        l[e][1] += b1;
-                        const float w0 = b0 * vs[m][i], w1 = b1 * vs[m][i];
-                        const uint32_t ph = pa_pack(w0, w1);
-                        const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&ph));
-                        hi[m][e][i] = pa_transpose(ph);
-                        lo[m][e][i] = pa_transpose(pa_pack(w0 - hf.x, w1 - hf.y));
-                    }
-            if constexpr (TMA)
-                if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
-            // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
-            // rows g of the tile, the odd ones rows g + 8
-#pragma unroll
-            for (int d = 0; d < ND; d += 2) {
-                float c[2][E][4];
-#pragma unroll
-                for (int m = 0; m < NM; m++) {
-                    uint32_t v[4];
-                    pa_ldsm_t(base + G::VOFF + G::at(16 * m + (lane & 15), d + (lane >> 4)), v);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] ^= 0x80808080u;
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const uint32_t vf[4] = {pa_half2<false>(v[2 * i]), pa_half2<true>(v[2 * i]),
-                                                pa_half2<false>(v[2 * i + 1]), pa_half2<true>(v[2 * i + 1])};
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            if (m == 0)
-                                pa_mma_f16(vf, hi[m][e], 0.0f, c[i][e]);
-                            else
-                                pa_mma_f16(vf, hi[m][e], c[i][e]);
-                            pa_mma_f16(vf, lo[m][e], c[i][e]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
-            }
+                    for (int j = 0; j < 4; j++)
+                        o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
         }
         if constexpr (TMA) {
             __syncwarp();
@@ -1140,14 +1036,11 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             continue;
         }
         // the end of an item or of the run
-        if constexpr (DIG) {
-            settle();
-            if (HEADS <= 4)  // lanes t and t + 2 hold two digits each of the same heads
+        if (HEADS <= 4)  // lanes t and t + 2 hold the sums of hi and lo halves of the same heads
 #pragma unroll
-                for (int d = 0; d < ND; d++)
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) o[d][0][j] += __shfl_xor_sync(0xffffffffu, o[d][0][j], 2);
-        }
+                for (int j = 0; j < 4; j++) o[d][0][j] += __shfl_xor_sync(0xffffffffu, o[d][0][j], 2);
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
