@@ -419,7 +419,7 @@ struct PaMaps {
 struct PaPlan {
     int units_row;  // kv heads * query blocks
     int qblocks;    // blocks of ROWS query heads per kv head
-    int tk, warps;  // keys of a unit, warps of a CTA
+    int tk;         // keys of a unit
     bool wide_copy; // 16-byte copies
     bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
     int box;        // keys of a tensor copy
@@ -1296,7 +1296,6 @@ int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s
     const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles;
     const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
     pl.tk = G::TK;
-    pl.warps = G::WARPS;
     PaMaps maps{};
     if (TMA) {
         pl.box = std::min(a.kv.p.page_size, G::TK);
@@ -1384,7 +1383,11 @@ int launch_paged_read(float* K, float* V, int ld, int rows, int KV, int hd, cons
             if (G <= 4) return F<128, 4, TMA>(__VA_ARGS__);                                       \
             return G <= 8 ? F<128, 8, TMA>(__VA_ARGS__) : F<128, 16, TMA>(__VA_ARGS__);           \
         }                                                                                         \
-        if (hd <= 192) return G <= 8 ? F<192, 8, false>(__VA_ARGS__) : F<192, 16, false>(__VA_ARGS__); \
+        if (hd <= 192) {                                                                          \
+            if (G <= 4) return F<192, 4, false>(__VA_ARGS__);                                     \
+            return G <= 8 ? F<192, 8, false>(__VA_ARGS__) : F<192, 16, false>(__VA_ARGS__);       \
+        }                                                                                         \
+        if (G <= 4) return F<256, 4, false>(__VA_ARGS__);                                         \
         return G <= 8 ? F<256, 8, false>(__VA_ARGS__) : F<256, 16, false>(__VA_ARGS__);           \
     } while (0)
 

@@ -214,7 +214,9 @@ ATTEND = [  # H, KV, hd, page, heads_first, rope, gap, lengths
     (4, 2, 128, 4, False, False, 16, [33, 95]),
     (16, 2, 128, 8, True, True, 0, [260, 31]),
     (20, 2, 64, 96, False, True, 0, [96, 97, 500]),
-    (8, 1, 128, 2048, False, True, 0, [2049, 100]),
+    (8, 1, 128, 2048, False, True, 0, [2049, 100]),    (14, 2, 192, 16, True, True, 0, [300, 33]),                # large heads, 5 to 8 of them and more
+    (16, 2, 256, 32, False, True, 0, [300, 17]),
+    (22, 2, 256, 16, True, False, 0, [130, 1000]),
 ]
 
 
