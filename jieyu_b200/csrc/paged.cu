@@ -906,8 +906,8 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 vscale = in ? sc[TK + lane] : 0.0f;
             }
             const int ex = min(max((int)((__float_as_uint(vscale) >> 23) & 255u), 63), 253) - 127;
-            // 0, or NaN where vs is not a number or infinite: so is the row then, whatever becomes of its weights
-            const float bias = __fsub_rn(vscale, vscale);
+            // 0, or NaN where ks or vs is not a number or infinite: so is the row then, whatever its weight
+            const float bias = __fsub_rn(kscale, kscale) + __fsub_rn(vscale, vscale);
             keys[lane] = in ? make_float4(kscale, bias, (float)ex, vscale) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         }
         __syncwarp();

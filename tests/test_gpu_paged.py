@@ -311,6 +311,23 @@ def test_attention_scales_that_are_not_finite(cuda):
         assert np.isnan(got[0, :4]).all() and np.isfinite(got[0, 4:]).all() and np.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("H,hd,side", [(4, 64, -1), (8, 128, 1), (16, 96, -1)])
+def test_attention_infinite_key_scale(cuda, H, hd, side):
+    """An infinite scale of K is not a weight of zero, whatever the sign of the key's dots."""
+    torch = cuda
+    page = 16
+    rng = np.random.default_rng(5)
+    pool = P.Pool(torch, 3, page, 1, hd, np.arange(3)[None])
+    pool.put_random(rng, 0, 48)
+    pool.k8[1, 5, 0, :] = side * 100
+    pool.ks[1, 5, 0] = np.inf
+    q = np.abs(rng.normal(size=(1, H * hd))).astype(np.float32)  # the dots with that key: all of its sign
+    out = torch.empty(1, H * hd, device="cuda")
+    lens = dev(torch, np.array([40], np.int32))
+    _capi.check(P.attend(torch, pool, dev(torch, q), out, H, lens, work=P.workspace(torch, 1, H, 1, hd)))
+    assert np.isnan(host(out)).all()
+
+
 def test_attention_wide_range_of_scales(cuda):
     """V scales over 12 decades: the key with all the weight has the smallest one."""
     torch = cuda
