@@ -665,9 +665,10 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 const int len = pa_len(a, b), nt = (len + TK - 1) / TK;
                 const long long n = (long long)nt * pl.units_row;
                 if (u < at + n) {
-                    const int k = (int)(u - at), r = k / nt;
-                    s_cur[warp] = PaCursor{b, r, k - r * nt, nt, len};
-                    s_first[warp] = u - (k - r * nt);  // first unit of the item that the run starts in
+                    const long long k = u - at;
+                    const int r = k >> 31 ? (int)(k / nt) : (int)k / nt, t0 = (int)(k - (long long)r * nt);
+                    s_cur[warp] = PaCursor{b, r, t0, nt, len};
+                    s_first[warp] = u - t0;  // first unit of the item that the run starts in
                     break;
                 }
                 at += n;
