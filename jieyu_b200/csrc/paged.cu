@@ -130,8 +130,12 @@ __device__ __forceinline__ uint32_t pack4(float4 x, float inv) {
 // issued before the first is used; only where a unit goes waits for the row's
 // position and page. (A warp of heads of several rows, each with its own
 // position, page and 64-bit offsets, executes 265 instructions per head of 128
-// and is bound by them: 82 us for 16384 rows of 8 heads.)
-constexpr int kRowUnits = 4, kRowThreads = 256;
+// and is bound by them.) Half as many units in flight per warp cost a fifth
+// (read of 32768 rows of 8 x 128 88 us against 74), twice as many gain nothing;
+// CTAs of 4 warps fill the SMs more evenly than 8 (append 97 -> 91 us).
+// Measured at 8 x 128: 32768 rows read in 72 us (4.7 TB/s; floor 52), 16384 rows
+// appended and read back in 91 us (floor 52).
+constexpr int kRowUnits = 4, kRowThreads = 128;
 
 struct RowWarp {
     int row, head;  // first head of this lane
