@@ -21,14 +21,14 @@
 //      finding each border by bisection over keys.
 //      More: the histogram bounds the running count or mass, so the border lies in
 //      one or two bins; their tokens go to one CTA (or are split again while they
-//      are more than 512), which finds the last kept one by bisection. The kept
-//      weights are summed by warp, in index order; the warp that the draw falls in
-//      walks its tokens.
+//      are more than 512), which finds the last kept one by sums over digits of
+//      the keys. The kept weights are summed by warp, in index order; the warp
+//      that the draw falls in walks its tokens.
 //   Rows without a filter, with k above 2048, and rows whose pools overflow go
 //   through 3 over all their logits instead of the pools.
 // Floor: one read of the logits; later passes find them in L2. What is left of
 // the time is the chain of passes and exchanges of a row (about 20 us for one row
-// with top-k, 55 with top-p alone), and with many rows the instructions of the
+// with top-k, 49 with top-p alone), and with many rows the instructions of the
 // exact weights (22 per logit and pass, 11 of them in double precision).
 #include <cooperative_groups.h>
 
@@ -50,6 +50,8 @@ constexpr int kPickTopK = 2048;      // largest k bounded by maxima: as many as 
 constexpr int kPickPool = 1920;      // tokens of a warp's pool: two CTAs share an SM's memory
 constexpr int kPickPairs = 256;      // tokens whose top-p is decided by comparing all pairs
 constexpr int kPickRank = 512;       // tokens among which one CTA looks for a border
+constexpr int kPickGather = 128;     // tokens that a warp gathers before it weighs them
+constexpr int kPickDigit = 9;        // bits of a key's digit in that search: a bin a thread
 constexpr int kPickBins = 2048, kPickPer = kPickBins / kPickThreads;
 constexpr int kPickMaxCluster = 8;
 constexpr float kPickSpan = 40.0f;   // powers of two that the bins cover
@@ -86,9 +88,10 @@ struct PickShared {
     uint32_t hist[kPickBins];
     double pow2[64];                   // 2^(j / 64)
     u64 x[2][kPickMaxCluster];         // exchanges between CTAs, two turns
+    u64 x4[kPickMaxCluster][4];
     u64 sums[kPickMaxCluster][kPickWarps];
-    u64 red[kPickWarps];
-    u64 tau;
+    u64 red[kPickWarps], red2[kPickWarps];
+    u64 tau, border;
     uint32_t count, inside[kPickWarps];
     int b1, b2;
 };
@@ -198,15 +201,11 @@ struct PickRow {
         else
             __syncthreads();
     }
-    // v of every CTA, in s->x[turn][rank of it] after the call; v from thread 0
+    __device__ PickShared* of(int r) const { return C > 1 ? cg::this_cluster().map_shared_rank(s, r) : s; }
+    // v of every CTA (the same in its threads), in s->x[turn][rank of it] after the call
     __device__ const u64* exchange(u64 v) {
         turn ^= 1;
-        if (C > 1) {
-            if (threadIdx.x == 0)
-                for (int r = 0; r < C; r++) cg::this_cluster().map_shared_rank(s, r)->x[turn][rank] = v;
-        } else if (threadIdx.x == 0) {
-            s->x[turn][0] = v;
-        }
+        if ((int)threadIdx.x < C) of(threadIdx.x)->x[turn][rank] = v;
         sync();
         return s->x[turn];
     }
@@ -264,15 +263,15 @@ __device__ __forceinline__ void pick_append(PickShared* s, bool take, u64 comp) 
     if (take && at < kPickRank) s->list[at] = comp;
 }
 
-// The CTAs' lists (of `mine` tokens each) joined in the first one's, in the CTAs' order, when they are at most
-// `most`. Returns their total (-1: too many), the same in every CTA; the list is complete after the call.
-__device__ int pick_collect(PickRow& r, uint32_t mine, int most) {
-    const u64* x = r.exchange(mine);
+// The CTAs' lists (CTA i's of x[step * i] tokens) joined in the first one's, in the CTAs' order, when they are at
+// most `most`. Returns their total (-1: too many), the same in every CTA; the list is complete after the call.
+__device__ int pick_collect(PickRow& r, const u64* x, int step, int most) {
     u64 total = 0ull, before = 0ull;
     for (int i = 0; i < r.C; i++) {
-        if (i < r.rank) before += x[i];
-        total += x[i];
+        if (i < r.rank) before += x[step * i];
+        total += x[step * i];
     }
+    const uint32_t mine = (uint32_t)x[step * r.rank];
     if (total <= (u64)most && r.rank > 0) {
         u64* to = cg::this_cluster().map_shared_rank(r.s, 0)->list;
         for (uint32_t i = threadIdx.x; i < mine; i += kPickThreads) to[before + i] = r.s->list[i];
@@ -309,6 +308,7 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
     int lo_bin = 0, hi_bin = kPickBins - 1, level = 0, shift = 0;
     u64 chi = ~0ull, clo = 0ull;
     double above = 0.0;  // metric of what lies above the members
+    const double per_unit = kOne / unit, e = 0.52 / unit + 1.1e-5;
     while (true) {
         pick_total(r);
         // bounds of the metric up to each bin; a thread's bins lie side by side
@@ -320,8 +320,9 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
             lo[i] = hi[i] = n;
             if (by_mass && n > 0.0) {
                 if (level == 0) {
-                    // a token's share is rounded by half a unit and lies above 0.99; 1e-5: the fp32 places and shares
-                    const double top = n / unit * exp2(-(double)kPickSpan / kPickBins * b) * kOne, e = 0.52 / unit + 1e-5;
+                    // a token's share is rounded by half a unit and lies above 0.99; 1e-5: the fp32 places and shares;
+                    // 1e-6: the power here
+                    const double top = n * per_unit * (double)pick_ex2(-kPickSpan / kPickBins * (float)b);
                     hi[i] = top * (1.0 + e);
                     lo[i] = top * (1.0 - e);
                 } else {
@@ -370,7 +371,20 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         }
         // what lies above the members, exactly; the members themselves, and their range
         u64 first = ~0ull, last = 0ull;
-        double over_sum = 0.0;  // whole numbers below 2^53
+        u64 up = 0ull;
+        // weights are dear: the warp gathers the tokens that lie above, and weighs them four a lane
+        float* gather = reinterpret_cast<float*>(s->pair) + (tid >> 5) * kPickGather;
+        int held = 0;
+        const int lane = tid & 31;
+        auto weigh = [&] {
+            __syncwarp();
+            double w = 0.0;
+#pragma unroll
+            for (int j = 0; j < kPickGather / 32; j++) w += lane + 32 * j < held ? r.mass(gather[lane + 32 * j]) : 0.0;
+            up += (u64)w;
+            __syncwarp();
+            held = 0;
+        };
         r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
             bool over[4], in[4], some = false, members = false;
 #pragma unroll
@@ -404,17 +418,23 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
             if (!__any_sync(0xffffffffu, some)) return;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const double w = by_mass ? r.mass(x[j]) : 1.0;
-                over_sum += over[j] ? w : 0.0;
+                if (!by_mass) {
+                    up += over[j];
+                    continue;
+                }
+                const unsigned m = __ballot_sync(0xffffffffu, over[j]);
+                if (held + __popc(m) > kPickGather) weigh();
+                if (over[j]) gather[held + __popc(m & ((1u << lane) - 1u))] = x[j];
+                held += __popc(m);
             }
         });
-        u64 up = (u64)over_sum;
+        if (held) weigh();
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) up += __shfl_xor_sync(0xffffffffu, up, o);
         const u64 warp_up = up;
         up = pick_sum(r, (tid & 31) == 0 ? up : 0ull);
         above = (double)up;
-        const int total = pick_collect(r, s->count, kPickRank);
+        const int total = pick_collect(r, r.exchange(s->count), 1, kPickRank);
         if (total >= 0) {
             if (r.rank == 0) {
                 // the token up to which the running metric reaches the target: first its key, by bisection, then its
@@ -422,16 +442,40 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
                 const u64 mine = tid < total ? s->list[tid] : 0ull;
                 const uint32_t key = (uint32_t)(mine >> 32);
                 const u64 own = tid < total ? (by_mass ? r.weight(pick_value(mine)) : 1ull) : 0ull;
-                uint32_t lo_key = (uint32_t)pick_reduce(tid < total ? (u64)key : ~0ull, s->red, pick_min);
-                uint32_t hi_key = (uint32_t)pick_reduce((u64)key, s->red, pick_max);
-                const uint32_t top_key = hi_key;
+                const uint32_t low_key = (uint32_t)pick_reduce(tid < total ? (u64)key : ~0ull, s->red, pick_min);
+                const uint32_t top_key = (uint32_t)pick_reduce((u64)key, s->red, pick_max);
                 auto reach = [&](uint32_t k) { return up + pick_reduce(key >= k ? own : 0ull, s->red, pick_add); };
-                while (lo_key < hi_key) {
-                    const uint32_t mid = lo_key + (hi_key - lo_key + 1u) / 2u;
-                    if ((double)reach(mid) >= target)
-                        lo_key = mid;
-                    else
-                        hi_key = mid - 1u;
+                uint32_t lo_key = low_key;
+                if ((double)up >= target) {
+                    lo_key = top_key;
+                } else if ((double)reach(low_key) >= target) {
+                    // digit by digit: sums of the weights (below 2^43) by digit in two words of 22 and 21 bits
+                    uint32_t* words = reinterpret_cast<uint32_t*>(s->pair);
+                    u64 over = up;
+                    const uint32_t off = key - low_key;
+                    uint32_t prefix = 0u;
+                    for (int bit = 32 - __clz((int)(top_key - low_key)); bit > 0;) {
+                        const int next = max(0, bit - kPickDigit);
+                        words[tid] = words[kPickThreads + tid] = 0u;
+                        __syncthreads();
+                        if (own && (bit == 32 || off >> bit == prefix)) {
+                            const uint32_t d = (off >> next) & ((1u << (bit - next)) - 1u);
+                            atomicAdd(&words[d], (uint32_t)own & 0x3FFFFFu);
+                            atomicAdd(&words[kPickThreads + d], (uint32_t)(own >> 22));
+                        }
+                        __syncthreads();
+                        const int d = kPickThreads - 1 - tid;  // larger keys first
+                        const u64 n = words[d] + ((u64)words[kPickThreads + d] << 22), upto = over + pick_scan(n, s->red);
+                        if ((double)upto >= target && (double)(upto - n) < target) {
+                            s->b1 = d;
+                            s->border = upto - n;
+                        }
+                        __syncthreads();
+                        over = s->border;
+                        prefix = prefix << (bit - next) | (uint32_t)s->b1;
+                        bit = next;
+                    }
+                    lo_key = low_key + prefix;
                 }
                 const u64 over = lo_key < top_key ? reach(lo_key + 1u) : up;
                 const bool equal = tid < total && key == lo_key;
@@ -811,13 +855,38 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
                 s->list[before + i] = pick_comp(r.at(idx), idx);
             }
         __syncthreads();
+        // the CTAs' sums, numbers of tokens and largest pools, in one exchange
         if (sums) {
-            rest = pick_sum(r, rest);
-            M = pick_sum(r, M);
-            // the border is among the histogram's tokens: it serves the passes below
-            have = (double)P * (double)M <= (double)(M - rest);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                rest += __shfl_xor_sync(0xffffffffu, rest, o);
+                M += __shfl_xor_sync(0xffffffffu, M, o);
+            }
+            if (lane == 0) {
+                s->red[warp] = rest;
+                s->red2[warp] = M;
+            }
+            __syncthreads();
+            rest = M = 0ull;
+            for (int w = 0; w < kPickWarps; w++) {
+                rest += s->red[w];
+                M += s->red2[w];
+            }
         }
-        const int found = pick_collect(r, fits ? total : kPickList + 1u, kPickList);
+        if (tid < 4 * C)
+            r.of(tid >> 2)->x4[r.rank][tid & 3] = (tid & 2) == 0 ? ((tid & 1) == 0 ? rest : M)
+                                                  : (tid & 1) == 0 ? (u64)(fits ? total : kPickList + 1u) : (u64)largest;
+        r.sync();
+        rest = M = 0ull;
+        u64 widest = 0ull;
+        for (int i = 0; i < C; i++) {
+            rest += s->x4[i][0];
+            M += s->x4[i][1];
+            widest = pick_max(widest, s->x4[i][3]);
+        }
+        // the border is among the histogram's tokens: it serves the passes below
+        have = sums && (double)P * (double)M <= (double)(M - rest);
+        const int found = pick_collect(r, &s->x4[0][2], 4, kPickList);
         if (found >= 0) {
             bool done = true;
             if (r.rank == 0) done = pick_short(a, r, row, found, by_k ? K : found, P, mp, rest);
@@ -826,10 +895,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
             if (e[0]) return;
         } else {
             // pools that are too many for one CTA serve the passes below
-            const u64* e = r.exchange(largest);
-            u64 l = 0ull;
-            for (int i = 0; i < C; i++) l = pick_max(l, e[i]);
-            if (l <= (u64)kPickPool) r.pooled = n;
+            if (widest <= (u64)kPickPool) r.pooled = n;
         }
     }
 
@@ -892,19 +958,27 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     if (sum == 0ull || !(inside || (before == 0ull && (double)before > target))) return;
     int id = -1;
     u64 got = 0ull;
-    const int step = r.pooled >= 0 ? 32 : 128, end = r.pooled >= 0 ? r.pooled : r.w1;
-    for (int i = r.pooled >= 0 ? 0 : r.w0; i < end; i += step) {
-        float q[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        int first = i + 4 * lane;
-        if (r.pooled < 0) {
-            r.load(first, q);
-        } else if (i + lane < end) {
-            first = r.w0 + s->pool[warp][i + lane];
-            q[0] = r.at(first);
+    const bool pools = r.pooled >= 0;
+    const int end = pools ? r.pooled : r.w1;
+    for (int i = pools ? 0 : r.w0; i < end; i += 128) {
+        float q[4];
+        int idx[4];
+        if (pools) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int k = i + 4 * lane + j;
+                idx[j] = k < end ? r.w0 + s->pool[warp][k] : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) q[j] = idx[j] >= 0 ? r.at(idx[j]) : -INFINITY;
+        } else {
+            r.load(i + 4 * lane, q);
+#pragma unroll
+            for (int j = 0; j < 4; j++) idx[j] = i + 4 * lane + j;
         }
         u64 w[4], own = 0ull;
 #pragma unroll
-        for (int j = 0; j < 4; j++) own += w[j] = kept(q[j], first + j);
+        for (int j = 0; j < 4; j++) own += w[j] = kept(q[j], idx[j]);
         u64 incl = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -920,7 +994,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         for (int j = 0; j < 4; j++) {
             if (w[j] == 0ull || passed) continue;
             run += w[j];
-            mine = first + j;
+            mine = idx[j];
             mw = w[j];
             passed = (double)run > target;
         }
@@ -938,17 +1012,18 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
 
 }  // namespace
 
-// CTAs of a row: up to 8 CTAs per SM in all, while a CTA keeps 4096 logits or
-// more. Rows differ in their work, so many small CTAs even it out (256 mixed
-// rows of 128256: 347 us with one CTA each, 265 with four; 64 rows of top-p
-// alone: 148 with four, 158 with eight); below 4096 logits the exchanges cost
-// more than the passes (62 rows of 14783, k = 1150: 58 us, 80 at 2048).
+// CTAs of a row: up to 4 CTAs per SM in all, while a CTA keeps 4096 logits or
+// more. Two are resident; rows differ in their work, so a second wave evens it
+// out (256 mixed rows of 128256: 367 us with one CTA each, 257 with two, 259
+// with four; 140 rows of top-p alone: 214, 192 and 283); below 4096 logits the
+// exchanges cost more than the passes (62 rows of 14783, k = 1150: 58 us, 80 at
+// 2048).
 int launch_pick(const PickArgs& a, cudaStream_t s) {
     if (a.rows == 0) return JYC_OK;
     const int sms = sm_count();
     if (sms == 0) return cuda_fail(cudaErrorNoDevice, "sample_batch: device query");
     int C = 1;
-    while (C < kPickMaxCluster && (long long)a.rows * 2 * C <= 8 * sms && a.V / (2 * C) >= 4096) C *= 2;
+    while (C < kPickMaxCluster && (long long)a.rows * 2 * C <= 4 * sms && a.V / (2 * C) >= 4096) C *= 2;
     const int chunk = ((a.V + C - 1) / C + 3) / 4 * 4;
     if (int e = max_dynamic_smem(reinterpret_cast<const void*>(pick_kernel), (int)sizeof(PickShared))) return e;
     cudaLaunchConfig_t cfg{};
