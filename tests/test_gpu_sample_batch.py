@@ -142,6 +142,24 @@ def test_large_and_flat(cuda, kind):
          rng.random(rows).astype(np.float32))
 
 
+def test_border_among_logits_of_both_signs(cuda):
+    """The border's tokens lie in one narrow bin, on both sides of zero and over ten decades."""
+    rng = np.random.default_rng(19)
+    high, low = 2100, 400
+    k = [0, 0, 0, 2150, 2300, 2301, 2499, 2300]
+    n = len(k)
+    l = np.empty((n, high + low), np.float32)
+    for r in range(n):
+        x = np.concatenate([5e9 * (1 - 1e-3 * rng.random(high)),
+                            rng.choice([-1, 1], low) * 10.0 ** rng.uniform(-5, 5, low)])
+        l[r] = rng.permutation(x)
+    w = np.exp((l[0].astype(np.float64) - l[0].max()) / 1e9)
+    tail = w[l[0] < 1e9].sum() / w.sum()
+    p = [1 - 0.5 * tail, 1 - 0.9 * tail, 1 - 0.01 * tail, 1.0, 1.0, 1.0, 1.0, 1 - 0.3 * tail]
+    for u in (rng.random(n), 1 - 0.5 * tail * rng.random(n)):
+        _run(cuda, l, [1e9] * n, k, p, None, np.minimum(u, 1 - 2.0 ** -24).astype(np.float32))
+
+
 def test_draws_at_the_ends(cuda):
     """u of 0, just below 1, and out of range or NaN: always a kept token."""
     l = np.full((6, 50), -np.inf, np.float32)
