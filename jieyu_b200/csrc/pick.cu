@@ -28,8 +28,10 @@
 //   through 3 over all their logits instead of the pools.
 // Floor: one read of the logits; later passes find them in L2. What is left of
 // the time is the chain of passes and exchanges of a row (about 20 us for one row
-// with top-k, 49 with top-p alone), and with many rows the instructions of the
-// exact weights (22 per logit and pass, 11 of them in double precision).
+// with top-k, 49 with top-p alone); with many rows too: warps wait at barriers
+// more than for memory, and 41 % of the issue slots are busy, with the exact
+// weights above all (22 instructions per logit and pass, 11 of them in double
+// precision).
 #include <cooperative_groups.h>
 
 #include <algorithm>
