@@ -723,10 +723,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     }
     u64 top = best > -INFINITY ? pick_comp(best, at) : 0ull;
     top = pick_reduce(top, s->red, pick_max);
-    const u64* x = r.exchange(top);
-    for (int i = 0; i < C; i++) top = pick_max(top, x[i]);
+    if (C > 1) {
+        // Another CTA's shared memory exists once that CTA has started: here each leaves its maximum in its own, and
+        // takes the others' behind the barrier.
+        if (tid == 0) s->x[r.turn][r.rank] = top;
+        r.sync();
+        top = lane < C ? r.of(lane)->x[r.turn][lane] : 0ull;
+#pragma unroll
+        for (int o = kPickMaxCluster / 2; o > 0; o >>= 1) top = pick_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = __shfl_sync(0xffffffffu, top, 0);
+    }
     if (top == 0ull || !(Tf > 0.0f)) {
         if (r.rank == 0 && tid == 0) pick_write(a, row, top ? pick_index(top) : -1, top ? 1.0f : 0.0f);
+        r.sync();  // until the others have read
         return;
     }
     r.mx = pick_value(top);

@@ -267,3 +267,28 @@ def test_distribution(cuda):
     count = np.array([(ids == i).sum() for i in keep])
     assert np.all(np.abs(count - n * w / w.sum()) <= 1.0 + 1e-6)
     assert np.all(np.diff(ids) >= 0)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 65536), (60, 65536), (150, 32768), (37, 131072)])
+def test_clusters_that_start_late(cuda, rows, V):
+    """Rows of 2 to 8 CTAs while another stream's kernels hold most of the SMs, so that the CTAs of a row
+    find their places at different times: every call gives the picks of the definition."""
+    torch = cuda
+    rng = np.random.default_rng(rows + V)
+    l = _logits(rng, rows, V, "plain")
+    u = rng.random(rows).astype(np.float32)
+    d, ud = dev(torch, l), dev(torch, u)
+    k = dev(torch, np.full(rows, 40, np.int32))
+    want = [P.picks(l[r], 1.0, 40, None, None, u[r]) for r in range(rows)]
+    ids = torch.full((32, rows), -9, dtype=torch.int32, device="cuda")
+    busy, here = torch.cuda.Stream(), torch.cuda.Stream()
+    a = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(32):
+        with torch.cuda.stream(busy):
+            a.mul_(1.0).add_(0.0)
+        _capi.check(_call(torch, d, V, None, k, None, None, ud, ids[i], None, stream=here.cuda_stream))
+    torch.cuda.synchronize()
+    got = host(ids)
+    for r in range(rows):
+        assert set(got[:, r].tolist()) <= set(want[r]), r
