@@ -339,7 +339,7 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         double* red = reinterpret_cast<double*>(s->red);
         double cl = pick_scan(lo_all, red) + above - lo_all, ch = pick_scan(hi_all, red) + above - hi_all;
         if (tid == 0) {
-            s->b1 = s->b2 = kPickBins - 1;
+            s->b1 = s->b2 = kPickBins;
             s->count = 0u;
         }
         __syncthreads();
@@ -363,10 +363,15 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         if (above >= early && tid == 0) atomicMin(&s->b1, 0);
         if (above >= late && tid == 0) atomicMin(&s->b2, 0);
         __syncthreads();
-        const int b1 = s->b1, b2 = max(s->b2, s->b1);
+        if (!by_mass && s->b1 == kPickBins) {  // fewer tokens than that: all of them
+            *kept = 0ull;                      // (only the kept mass is asked for)
+            return tau0;
+        }
+        // the last bin that holds comps of [clo, chi]; the border's bins lie up to it, so nothing below wraps
+        const int last_bin = level == 0 ? kPickBins - 1 : (int)((chi - clo) >> shift);
+        const int b1 = min(s->b1, last_bin), b2 = min(max(s->b2, s->b1), last_bin);
         const u64 chi1 = level == 0 ? ~0ull : chi - ((u64)b1 << shift);
-        const u64 end = (u64)(b2 + 1) << shift;
-        const u64 clo1 = level == 0 ? 0ull : chi - clo < end ? clo : chi - end + 1ull;
+        const u64 clo1 = level == 0 ? 0ull : b2 == last_bin ? clo : chi - ((u64)(b2 + 1) << shift) + 1ull;
         if (level == 0) {
             lo_bin = b1;
             hi_bin = b2;

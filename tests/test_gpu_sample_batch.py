@@ -292,3 +292,24 @@ def test_clusters_that_start_late(cuda, rows, V):
     got = host(ids)
     for r in range(rows):
         assert set(got[:, r].tolist()) <= set(want[r]), r
+
+
+@pytest.mark.parametrize("V", [4000, 10001, 70000])
+def test_k_above_the_number_of_tokens(cuda, V):
+    """A large k over a row with fewer logits than that (the others -inf or NaN), more than a thousand of
+    which lie far below the maximum, down to the type's lowest value: all of them are kept."""
+    rng = np.random.default_rng(V)
+    k = [0.6, 0.5, 0.45, 0.9, 0.41, 0.399]  # of V; 0.4 of V are logits
+    rows, n = len(k), 2 * V // 5
+    l = np.full((rows, V), -np.inf, np.float32)
+    for r in range(rows):
+        at = rng.permutation(V)
+        x = np.concatenate([[0.0], np.full(3 * n // 4, -40.0), -(10.0 ** rng.uniform(np.log10(40), 38, n))])[:n]
+        x[n // 2] = np.finfo(np.float32).min
+        if r % 2:
+            x[1: n // 4] = -rng.random(n // 4 - 1)  # some with weight
+        l[r, at[:n]] = x
+        l[r, at[n: n + V // 5]] = np.nan
+    k = [int(f * V) for f in k]
+    for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
+        _run(cuda, l, [1.0] * rows, k, None, [0.0, 0.0, 0.5, 0.5, 0.0, 0.0], u.astype(np.float32))
