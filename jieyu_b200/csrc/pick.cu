@@ -55,6 +55,7 @@ constexpr int kPickRank = 512;       // tokens among which one CTA looks for a b
 constexpr int kPickGather = 128;     // tokens that a warp gathers before it weighs them
 constexpr int kPickDigit = 9;        // bits of a key's digit in that search: a bin a thread
 constexpr int kPickBins = 2048, kPickPer = kPickBins / kPickThreads;
+constexpr int kPickWide = kPickBins / 2;  // bins of 64-bit sums, in the same memory
 constexpr int kPickMaxCluster = 8;
 constexpr float kPickSpan = 40.0f;   // powers of two that the bins cover
 constexpr double kOne = 0x1p42;      // a weight of 1
@@ -79,7 +80,10 @@ struct PickShared {
         u64 list[kPickList];
         struct {
             u64 first[kPickList / 2];  // a border's tokens, while the totals are in use
-            uint32_t tot[kPickBins];
+            union {
+                uint32_t tot[kPickBins];
+                u64 wide_tot[kPickWide];
+            };
         };
     };
     union {
@@ -87,7 +91,10 @@ struct PickShared {
         u64 top[kPickTopK];                    // the top-k, when one CTA ends the row
     };
     ulonglong2 pair[kPickRank];        // comp, metric
-    uint32_t hist[kPickBins];
+    union {
+        uint32_t hist[kPickBins];
+        u64 wide[kPickWide];
+    };
     double pow2[64];                   // 2^(j / 64)
     u64 x[2][kPickMaxCluster];         // exchanges between CTAs, two turns
     u64 x4[kPickMaxCluster][4];
@@ -282,103 +289,133 @@ __device__ int pick_collect(PickRow& r, const u64* x, int step, int most) {
     return total <= (u64)most ? (int)total : -1;
 }
 
-// Sums of the CTA's histograms in s->tot of every CTA.
-__device__ void pick_total(PickRow& r) {
+// Sums of the CTA's histograms (s->hist, s->wide) in s->tot (s->wide_tot) of every CTA.
+template <class T>
+__device__ void pick_total(PickRow& r, T* hist, T* tot) {
+    constexpr int bins = sizeof(T) == 4 ? kPickBins : kPickWide;
     r.sync();
     if (r.C == 1) {
-        for (int b = threadIdx.x; b < kPickBins; b += kPickThreads) r.s->tot[b] = r.s->hist[b];
+        for (int b = threadIdx.x; b < bins; b += kPickThreads) tot[b] = hist[b];
         __syncthreads();
         return;
     }
-    const int per = kPickBins / r.C;
+    const int per = bins / r.C;
     for (int i = threadIdx.x; i < per; i += kPickThreads) {
         const int b = r.rank * per + i;
-        uint32_t n = 0u;
-        for (int c = 0; c < r.C; c++) n += cg::this_cluster().map_shared_rank(r.s, c)->hist[b];
-        for (int c = 0; c < r.C; c++) cg::this_cluster().map_shared_rank(r.s, c)->tot[b] = n;
+        T n = 0;
+        for (int c = 0; c < r.C; c++) n += cg::this_cluster().map_shared_rank(hist, c)[b];
+        for (int c = 0; c < r.C; c++) cg::this_cluster().map_shared_rank(tot, c)[b] = n;
     }
     r.sync();
 }
 
+// One step of the search below: the members (comps of [*clo, *chi] from tau0 on, of the bins lo_bin .. hi_bin) are split
+// into bins of exact sums, and the range shrinks to the bin in which the metric reaches `target` (the last one if none
+// does); `up`: the metric above the range. Few rows need it: a call, so that it takes no registers from the others (64 rows
+// of top-p 132 us, 139 with the step in line; 256 mixed rows 250 and 261).
+__device__ __noinline__ void pick_split(PickRow r, bool by_mass, double target, u64 tau0, int lo_bin, int hi_bin, u64 up,
+                                        u64* clo_p, u64* chi_p) {
+    constexpr int PER = kPickWide / kPickThreads;
+    PickShared* s = r.s;
+    const int tid = threadIdx.x;
+    const u64 clo = *clo_p, chi = *chi_p;
+    int shift = 0;
+    while (((chi - clo) >> shift) >= (u64)kPickWide) shift++;
+    for (int b = tid; b < kPickWide; b += kPickThreads) s->wide[b] = 0ull;
+    if (tid == 0) s->b1 = (double)up >= target ? 0 : kPickWide;
+    __syncthreads();
+    r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const u64 comp = pick_comp(x[j], idx[j]);
+            if (!is[j] || comp < tau0 || comp < clo || comp > chi) continue;
+            const int b = r.bin(x[j]);
+            if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->wide[(chi - comp) >> shift], by_mass ? r.weight(x[j]) : 1ull);
+        }
+    });
+    pick_total(r, s->wide, s->wide_tot);
+    u64 in_bin[PER], all = 0ull;  // a thread's bins lie side by side
+#pragma unroll
+    for (int i = 0; i < PER; i++) all += in_bin[i] = s->wide_tot[PER * tid + i];
+    u64 c = up + pick_scan(all, s->red) - all;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {  // one bin of all, or none
+        if ((double)c < target && (double)(c + in_bin[i]) >= target) s->b1 = PER * tid + i;
+        c += in_bin[i];
+    }
+    __syncthreads();
+    const int last = (int)((chi - clo) >> shift), b = min(s->b1, last);
+    const u64 top = chi - ((u64)b << shift);
+    *chi_p = top;
+    if (b < last) *clo_p = top - ((1ull << shift) - 1ull);
+}
+
 // Where the prefix of {comp >= tau0} ends whose metric (number of tokens, or mass) first reaches `target`:
 // the comp of its last token. s->hist holds this CTA's histogram of the bins: tokens, or for a mass their
-// weights over that of the bin's middle, in units of 1 / unit.
+// weights over that of the bin's middle, in units of 1 / unit. Those bound the metric: the border lies in one bin or
+// in a few, whose tokens are the members. While they are too many, their range of comps is split into bins of
+// exact sums: the border lies in one of them. A range starts and ends with a member and holds 512 comps or more, so
+// each time at least two bins are occupied, and what is left is smaller by a factor of 512: seven times at most, the
+// comps having 64 bits.
 // *kept: the metric that this warp's tokens have in the prefix.
 __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit, u64 tau0, u64* kept) {
     PickShared* s = r.s;
     const int tid = threadIdx.x;
-    int lo_bin = 0, hi_bin = kPickBins - 1, level = 0, shift = 0;
-    u64 chi = ~0ull, clo = 0ull;
-    double above = 0.0;  // metric of what lies above the members
+    u64 chi = ~0ull, clo = 0ull;  // the members' range
+    u64 up = 0ull;                // metric of what lies above them
+    if (tid == 0) s->b1 = s->b2 = kPickBins;
+    pick_total(r, s->hist, s->tot);
+    // bounds of the metric up to each bin; a thread's bins lie side by side
     const double per_unit = kOne / unit, e = 0.52 / unit + 1.1e-5;
+    double lo[kPickPer], hi[kPickPer], lo_all = 0.0, hi_all = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPickPer; i++) {
+        const int b = kPickPer * tid + i;
+        const double n = (double)s->tot[b];
+        lo[i] = hi[i] = n;
+        if (by_mass && n > 0.0) {
+            // a token's share is rounded by half a unit and lies above 0.99; 1e-5: the fp32 places and shares;
+            // 1e-6: the power here
+            const double top = n * per_unit * (double)pick_ex2(-kPickSpan / kPickBins * (float)b);
+            hi[i] = top * (1.0 + e);
+            lo[i] = top * (1.0 - e);
+        }
+        lo_all += lo[i];
+        hi_all += hi[i];
+    }
+    double* red = reinterpret_cast<double*>(s->red);
+    double cl = pick_scan(lo_all, red) - lo_all, ch = pick_scan(hi_all, red) - hi_all;
+    // sums of doubles may be off by a few parts in 2^53 per bin
+    const double early = target * (1.0 - 1e-12), late = by_mass ? target * (1.0 + 1e-12) : target;
+    // the first bins that reach the target; threads well behind them stay out
+    bool no1 = ch > early * (1.0 + 1e-9), no2 = cl > late * (1.0 + 1e-9);
+#pragma unroll
+    for (int i = 0; i < kPickPer; i++) {
+        ch += hi[i];
+        cl += lo[i];
+        if (!no1 && ch >= early) {
+            atomicMin(&s->b1, kPickPer * tid + i);
+            no1 = true;
+        }
+        if (!no2 && cl >= late) {
+            atomicMin(&s->b2, kPickPer * tid + i);
+            no2 = true;
+        }
+    }
+    if (tid == 0 && !(early > 0.0)) atomicMin(&s->b1, 0);
+    if (tid == 0 && !(late > 0.0)) atomicMin(&s->b2, 0);
+    __syncthreads();
+    if (!by_mass && s->b1 == kPickBins) {  // fewer tokens than that: all of them
+        *kept = 0ull;                      // (only the kept mass is asked for)
+        return tau0;
+    }
+    const int lo_bin = min(s->b1, kPickBins - 1), hi_bin = min(max(s->b2, s->b1), kPickBins - 1);
     while (true) {
-        pick_total(r);
-        // bounds of the metric up to each bin; a thread's bins lie side by side
-        double lo[kPickPer], hi[kPickPer], lo_all = 0.0, hi_all = 0.0;
-#pragma unroll
-        for (int i = 0; i < kPickPer; i++) {
-            const int b = kPickPer * tid + i;
-            const double n = (double)s->tot[b];
-            lo[i] = hi[i] = n;
-            if (by_mass && n > 0.0) {
-                if (level == 0) {
-                    // a token's share is rounded by half a unit and lies above 0.99; 1e-5: the fp32 places and shares;
-                    // 1e-6: the power here
-                    const double top = n * per_unit * (double)pick_ex2(-kPickSpan / kPickBins * (float)b);
-                    hi[i] = top * (1.0 + e);
-                    lo[i] = top * (1.0 - e);
-                } else {
-                    const u64 top = chi - ((u64)b << shift), span = ((u64)1 << shift) - 1ull;
-                    hi[i] = n * (double)r.weight(pick_value(top));
-                    lo[i] = n * (double)r.weight(pick_value(top > span ? top - span : 0ull));
-                }
-            }
-            lo_all += lo[i];
-            hi_all += hi[i];
-        }
-        double* red = reinterpret_cast<double*>(s->red);
-        double cl = pick_scan(lo_all, red) + above - lo_all, ch = pick_scan(hi_all, red) + above - hi_all;
-        if (tid == 0) {
-            s->b1 = s->b2 = kPickBins;
-            s->count = 0u;
-        }
+        if (tid == 0) s->count = 0u;
         __syncthreads();
-        // sums of doubles may be off by a few parts in 2^53 per bin
-        const double early = target * (1.0 - 1e-12), late = by_mass ? target * (1.0 + 1e-12) : target;
-        // the first bins that reach the target; threads well behind them stay out
-        bool no1 = ch > early * (1.0 + 1e-9), no2 = cl > late * (1.0 + 1e-9);
-#pragma unroll
-        for (int i = 0; i < kPickPer; i++) {
-            ch += hi[i];
-            cl += lo[i];
-            if (!no1 && ch >= early) {
-                atomicMin(&s->b1, kPickPer * tid + i);
-                no1 = true;
-            }
-            if (!no2 && cl >= late) {
-                atomicMin(&s->b2, kPickPer * tid + i);
-                no2 = true;
-            }
-        }
-        if (above >= early && tid == 0) atomicMin(&s->b1, 0);
-        if (above >= late && tid == 0) atomicMin(&s->b2, 0);
-        __syncthreads();
-        if (!by_mass && s->b1 == kPickBins) {  // fewer tokens than that: all of them
-            *kept = 0ull;                      // (only the kept mass is asked for)
-            return tau0;
-        }
-        // the last bin that holds comps of [clo, chi]; the border's bins lie up to it, so nothing below wraps
-        const int last_bin = level == 0 ? kPickBins - 1 : (int)((chi - clo) >> shift);
-        const int b1 = min(s->b1, last_bin), b2 = min(max(s->b2, s->b1), last_bin);
-        const u64 chi1 = level == 0 ? ~0ull : chi - ((u64)b1 << shift);
-        const u64 clo1 = level == 0 ? 0ull : b2 == last_bin ? clo : chi - ((u64)(b2 + 1) << shift) + 1ull;
-        if (level == 0) {
-            lo_bin = b1;
-            hi_bin = b2;
-        }
         // what lies above the members, exactly; the members themselves, and their range
         u64 first = ~0ull, last = 0ull;
-        u64 up = 0ull;
+        up = 0ull;
         // weights are dear: the warp gathers the tokens that lie above, and weighs them four a lane
         float* gather = reinterpret_cast<float*>(s->pair) + (tid >> 5) * kPickGather;
         int held = 0;
@@ -411,8 +448,8 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
                 for (int j = 0; j < 4; j++) {
                     const u64 comp = pick_comp(x[j], idx[j]);
                     if (in[j]) {
-                        over[j] = comp > chi1 && comp >= tau0;
-                        in[j] = comp <= chi1 && comp >= clo1 && comp >= tau0;
+                        over[j] = comp > chi && comp >= tau0;
+                        in[j] = comp <= chi && comp >= clo && comp >= tau0;
                         some |= over[j];
                     }
                     if (in[j]) {
@@ -440,7 +477,6 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         for (int o = 16; o > 0; o >>= 1) up += __shfl_xor_sync(0xffffffffu, up, o);
         const u64 warp_up = up;
         up = pick_sum(r, (tid & 31) == 0 ? up : 0ull);
-        above = (double)up;
         const int total = pick_collect(r, r.exchange(s->count), 1, kPickRank);
         if (total >= 0) {
             if (r.rank == 0) {
@@ -523,20 +559,7 @@ __device__ u64 pick_border(PickRow& r, bool by_mass, double target, double unit,
         for (int i = 0; i < r.C; i++) last = pick_max(last, x1[i]);
         clo = first;
         chi = last;
-        level++;
-        shift = 0;
-        while (((chi - clo) >> shift) >= (u64)kPickBins) shift++;
-        for (int b = tid; b < kPickBins; b += kPickThreads) s->hist[b] = 0u;
-        __syncthreads();
-        r.each([&](const float (&x)[4], const int (&idx)[4], const bool (&is)[4]) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const u64 comp = pick_comp(x[j], idx[j]);
-                if (!is[j] || comp < tau0 || comp < clo || comp > chi) continue;
-                const int b = r.bin(x[j]);
-                if (b >= lo_bin && b <= hi_bin) atomicAdd(&s->hist[(chi - comp) >> shift], 1u);
-            }
-        });
+        pick_split(r, by_mass, target, tau0, lo_bin, hi_bin, up, &clo, &chi);
     }
 }
 

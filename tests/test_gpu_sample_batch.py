@@ -313,3 +313,39 @@ def test_k_above_the_number_of_tokens(cuda, V):
     k = [int(f * V) for f in k]
     for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
         _run(cuda, l, [1.0] * rows, k, None, [0.0, 0.0, 0.5, 0.5, 0.0, 0.0], u.astype(np.float32))
+
+
+def _group_borders(rng, x, T, rows):
+    """top-p values whose border falls around the end of a group of equal logits of x."""
+    values, count = np.unique(x, return_counts=True)
+    w = P.weights(values, np.float64(np.float32(T)))[1]
+    upto = np.cumsum((count * w)[::-1])
+    at = rng.integers(0, len(values), rows)
+    off = np.array([0.5, 0.02, 0.98, -0.5, 1.5, 0.3])[np.arange(rows) % 6]  # of the group's last token
+    return np.clip((upto[at] - off * w[::-1][at]) / upto[-1], 1e-6, 1 - 2.0 ** -24)
+
+
+@pytest.mark.parametrize("V", [5000, 20000, 131072])
+@pytest.mark.parametrize("kind", ["two", "near", "steps", "bf16", "equal"])
+def test_borders_at_the_end_of_equal_logits(cuda, V, kind):
+    """Thousands of equal logits beside others that weigh almost the same, the border of top-p in the last
+    token of a group or beside it; with a large top-k too."""
+    rng = np.random.default_rng(V + len(kind))
+    rows = 12
+    l = np.empty((rows, V), np.float32)
+    T = [1.0, 0.7, 1.0, 3.0] * 3
+    for r in range(rows):
+        if kind == "two":
+            l[r] = np.where(rng.permutation(V) < V // 2, 1.0, 0.99)
+        elif kind == "near":
+            l[r] = np.where(rng.permutation(V) < V - 1 - r, 4.0, 3.984375)
+        elif kind == "steps":
+            l[r] = rng.choice([4.0, 3.984375, 3.96875, 2.0], V)
+        elif kind == "bf16":
+            l[r] = ((4 + 0.02 * rng.normal(size=V)).astype(np.float32).view(np.uint32) & 0xFFFF0000).view(np.float32)
+        else:
+            l[r] = 3.25
+    p = [_group_borders(rng, l[r], T[r], rows)[r] for r in range(rows)]
+    k = np.where(np.arange(rows) % 4 == 3, V - 7, 0)
+    for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
+        _run(cuda, l, T, k, p, None, u.astype(np.float32))
