@@ -113,6 +113,7 @@ struct PickRow {
     float mx;
     double c;               // log2(e) / T
     bool endless;           // the maximum is infinite
+    float lift, mx_lift;    // places are differences of logits times lift, a power of two: fp32 holds them
     float bin_scale;
     int C, rank, turn;
     int pooled;             // tokens in the warp's pool; -1: the passes go over all logits
@@ -155,7 +156,7 @@ struct PickRow {
     // Bins of powers of 2^(40 / 2048), the nearest one: larger logits never lie in a later bin. The place of a
     // logit above -inf among them (0 for the maximum), and its bin.
     __device__ __forceinline__ float place(float x) const {
-        return fminf(__fmul_rn(__fsub_rn(mx, x), bin_scale), (float)(kPickBins - 1));
+        return fminf(__fmul_rn(__fmaf_rn(-x, lift, mx_lift), bin_scale), (float)(kPickBins - 1));
     }
     static __device__ __forceinline__ int bin_at(float place) {
         return __float_as_int(__fadd_rn(place, 12582912.0f)) - 0x4B400000;  // 1.5 * 2^23: to the nearest
@@ -774,7 +775,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         for (int j = 0; j < 4; j++) m4[j] = r.seen(m4[j]);
     }
     r.c = 1.44269504088896340736 / (double)Tf;
-    r.bin_scale = fminf((float)(r.c * (kPickBins / (double)kPickSpan)), 1e30f);
+    // a difference passes fp32's range only under a maximum above 2^103: there of halves
+    r.lift = r.mx >= 0x1p100f ? 0.5f : 1.0f;
+    r.mx_lift = r.mx * r.lift;
+    r.bin_scale = fminf((float)(r.c * (kPickBins / (double)kPickSpan) / r.lift), 1e30f);
 
     r.pooled = -1;
     const bool by_k = K > 0 && K < V, by_p = P < 1.0f;
@@ -787,10 +791,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         float part = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (m4[j] > -INFINITY) {
-                const float d = __fsub_rn(r.mx, m4[j]);
-                part += d == 0.0f ? 1.0f : exp2f(-__fmul_rn(d, (float)r.c));
-            }
+            if (m4[j] > -INFINITY) part += exp2f(-kPickSpan / kPickBins * r.place(m4[j]));
         const double M = fmax(1.0, 0.99 / kOne * (double)pick_sum(r, (u64)(part * (float)kOne)));
         const double e = log2((double)V / ((1.0 - (double)P) * M));
         most = max(0, min(kPickBins - 1, (int)(e * (kPickBins / (double)kPickSpan)) + 1));

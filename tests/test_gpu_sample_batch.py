@@ -349,3 +349,51 @@ def test_borders_at_the_end_of_equal_logits(cuda, V, kind):
     k = np.where(np.arange(rows) % 4 == 3, V - 7, 0)
     for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
         _run(cuda, l, T, k, p, None, u.astype(np.float32))
+
+
+def _allowed(l, T, k, p, mp, u):
+    """Every (id, probability) that the definition allows: where the border of top-p lies within the rounding
+    of the sums (with equal weights it may lie on one exactly), one token more or fewer is kept, and the same
+    id comes with either probability. A prefix by top-p is a prefix by count."""
+    l64, w = P.weights(l, np.float64(np.float32(T)))
+    order = np.argsort(-l64, kind="stable")[: k if 0 < k < len(l) else len(l)]
+    ns = {len(order)}
+    if p < 1:
+        sums, slack = np.cumsum(w[order]), len(l) * 2.0 ** -43 + 2.0 ** -44 * w.sum()
+        need = np.float64(np.float32(p)) * sums[-1]
+        ns = {1 + int(np.searchsorted(sums, x)) for x in (need, need - slack, need + slack)}
+    return {x for n in ns for x in P.picks(l, T, max(1, n), None, mp, u).items()}
+
+
+def _run_at_borders(torch, l, T, k, p, mp, u):
+    rows, V = l.shape
+    d, ud = dev(torch, l), dev(torch, u)
+    args = [dev(torch, np.asarray(x, t)) for x, t in ((T, np.float32), (k, np.int32), (p, np.float32), (mp, np.float32))]
+    ids = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+    probs = torch.full((rows,), -9.0, device="cuda")
+    _capi.check(_call(torch, d, V, *args, ud, ids, probs))
+    gi, gp = host(ids), host(probs)
+    for r in range(rows):
+        want = _allowed(l[r], T[r], k[r], p[r], mp[r], u[r])
+        assert any(i == gi[r] and abs(gp[r] - q) <= q * (P.U24 + V * 2.0 ** -42 + 2.0 ** -43) + 2.0 ** -42
+                   for i, q in want), (r, gi[r], gp[r], want)
+
+
+@pytest.mark.parametrize("V", [2, 300, 6000, 40000])
+@pytest.mark.parametrize("T", [1e38, 3e37, 3e38, np.inf])
+def test_logits_over_the_whole_range(cuda, V, T):
+    """Logits of both signs next to the type's limits, whose differences fp32 does not hold, at temperatures
+    that leave them weight: top-p, min-p, top-k and all of them."""
+    rng = np.random.default_rng(V)
+    settings = [(0, 1.0, 0.0), (0, 1.0, 1e-3), (0, 1.0, 0.05), (0, 0.999, 0.0), (0, 0.9, 0.0), (0, 0.5, 0.01),
+                (V // 2, 1.0, 0.0), (V // 2, 0.7, 0.0), (3, 0.9, 0.0), (0, 1 - 2.0 ** -20, 0.0)]
+    rows = len(settings)
+    l = (3.4e38 * rng.uniform(-1, 1, (rows, V))).astype(np.float32)
+    l[:, 0], l[:, -1] = 3e38, -3e38
+    l[1::3, V // 3] = np.finfo(np.float32).min
+    l[2::3, V // 2] = np.finfo(np.float32).max
+    if V > 2:
+        l[:, 1], l[:, 2] = np.nan, -np.inf
+    k, p, mp = zip(*settings)
+    for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24), np.zeros(rows)):
+        _run_at_borders(cuda, l, [T] * rows, k, p, mp, u.astype(np.float32))
