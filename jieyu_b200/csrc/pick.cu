@@ -775,10 +775,13 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
         for (int j = 0; j < 4; j++) m4[j] = r.seen(m4[j]);
     }
     r.c = 1.44269504088896340736 / (double)Tf;
-    // a difference passes fp32's range only under a maximum above 2^103: there of halves
-    r.lift = r.mx >= 0x1p100f ? 0.5f : 1.0f;
+    // Bins of a difference of 1. fp32 holds it for T above 7e-29; below, 2^-64 of it, the logits times 2^64. Where the
+    // maximum is too large for that, every other logit is 2^-84 away or more: 1e30 puts it behind all bins too. A
+    // difference passes fp32's range only under a maximum above 2^103: there of halves.
+    const double per_one = r.c * (kPickBins / (double)kPickSpan);
+    r.lift = r.mx >= 0x1p100f ? 0.5f : per_one > 1e30 && fabsf(r.mx) < 0x1p-60f ? 0x1p64f : 1.0f;
     r.mx_lift = r.mx * r.lift;
-    r.bin_scale = fminf((float)(r.c * (kPickBins / (double)kPickSpan) / r.lift), 1e30f);
+    r.bin_scale = (float)fmin(per_one / r.lift, 1e30);
 
     r.pooled = -1;
     const bool by_k = K > 0 && K < V, by_p = P < 1.0f;

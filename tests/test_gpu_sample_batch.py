@@ -397,3 +397,23 @@ def test_logits_over_the_whole_range(cuda, V, T):
     k, p, mp = zip(*settings)
     for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24), np.zeros(rows)):
         _run_at_borders(cuda, l, [T] * rows, k, p, mp, u.astype(np.float32))
+
+
+@pytest.mark.parametrize("T", [1e-30, 7e-29, 3e-38, 1.5e-44])
+def test_tiny_temperatures(cuda, T):
+    """Thousands of tokens with weight at temperatures near the least that fp32 holds: logits of T's own
+    size, around zero or all of one sign, and beside them ordinary ones."""
+    rng = np.random.default_rng(3)
+    V = 20000
+    settings = [(0, 0.5, 0.0), (0, 0.9, 0.0), (0, 0.999, 0.0), (0, 1.0, 0.01), (5000, 0.7, 0.0), (40, 0.9, 0.0),
+                (0, 1 - 2.0 ** -20, 0.0), (0, 1.0, 0.0), (0, 0.8, 0.05)]
+    rows = len(settings)
+    T = float(np.float32(T))
+    l = np.empty((rows, V), np.float32)
+    for r in range(rows):
+        l[r] = (T * (rng.choice([-40.0, 0.0, 25.0]) + 20 * rng.random(V))).astype(np.float32)
+        l[r, rng.integers(0, V, 50)] = -1.0
+        l[r, rng.integers(0, V, 50)] = -np.inf
+    k, p, mp = zip(*settings)
+    for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
+        _run_at_borders(cuda, l, [T] * rows, k, p, mp, u.astype(np.float32))
