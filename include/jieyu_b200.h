@@ -336,7 +336,7 @@ JYC_API int jyc_paged_error(int reset);
  *   top_k (off)      the k largest logits, ties to the lower index; k <= 0: off;
  *   top_p (off)      of those, the shortest run from the largest whose weights
  *                    reach top_p of theirs, at least one token; >= 1 or NaN: off;
- *   min_p (off)      of those, weights >= min(min_p, 1) (the largest is 1).
+ *   min_p (off)      of those, weights >= min(min_p, 1) (the largest is 1); <= 0 or NaN: off.
  * The pick is the first kept index, in index order, whose running sum of
  * weights exceeds u[r] times their sum (u in [0, 1); the last kept one if none
  * does). probs[r] (probs may be NULL) is its weight over that sum, 1 for a

@@ -730,7 +730,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
     const float Tf = a.temperature ? a.temperature[row] : 1.0f;
     const int K = a.top_k ? a.top_k[row] : 0;
     const float P = a.top_p ? a.top_p[row] : 1.0f;
-    const double mp = a.min_p ? fmin((double)a.min_p[row], 1.0) : 0.0;
+    const float mf = a.min_p ? a.min_p[row] : 0.0f;
+    const double mp = mf > 0.0f ? fmin((double)mf, 1.0) : 0.0;  // NaN: off
     if (tid < 64) s->pow2[tid] = exp2((double)tid / 64.0);
     if (tid == 0) s->count = 0u;
 

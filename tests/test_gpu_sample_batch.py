@@ -417,3 +417,24 @@ def test_tiny_temperatures(cuda, T):
     k, p, mp = zip(*settings)
     for u in (rng.random(rows), np.full(rows, 1 - 2.0 ** -24)):
         _run_at_borders(cuda, l, [T] * rows, k, p, mp, u.astype(np.float32))
+
+
+def test_nan_filters_are_off(cuda):
+    """NaN in top-p or min-p means the filter's default, as for a row without it."""
+    torch = cuda
+    rng = np.random.default_rng(8)
+    rows, V = 40, 900
+    l = _logits(rng, 1, V, "plain").repeat(rows, 0)
+    u = ((np.arange(rows) + 0.5) / rows).astype(np.float32)
+    d, ud = dev(torch, l), dev(torch, u)
+    nan, k = dev(torch, np.full(rows, np.nan, np.float32)), dev(torch, np.full(rows, 200, np.int32))
+    got = []
+    for p, mp in ((None, None), (nan, None), (None, nan), (nan, nan)):
+        for top_k in (None, k):
+            ids = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+            probs = torch.zeros(rows, device="cuda")
+            _capi.check(_call(torch, d, V, None, top_k, p, mp, ud, ids, probs))
+            got.append((host(ids), host(probs)))
+    for i in range(2, len(got)):
+        assert np.array_equal(got[i][0], got[i % 2][0]) and np.array_equal(got[i][1], got[i % 2][1]), i
+    assert len(set(got[0][0].tolist())) > 1
