@@ -495,7 +495,7 @@ JYC_API int jyc_paged_error(int reset) {
     int v = 0;
     JYC_CUDA(cudaDeviceSynchronize());
     JYC_CUDA(cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost));
-    if (reset && v) JYC_CUDA(cudaMemset(p, 0, sizeof(int)));
+    if (reset && v) TRY(paged_error_clear(v));
     return v;
 }
 

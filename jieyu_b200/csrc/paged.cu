@@ -24,6 +24,16 @@ int* paged_error_word() {
     return p;
 }
 
+static __global__ void paged_error_clear_kernel(int bits) { atomicAnd(&g_paged_err, ~bits); }
+
+int paged_error_clear(int bits) {
+    // not a memset: a call on a stream that the default one does not order could set its bit before that
+    paged_error_clear_kernel<<<1, 1>>>(bits);
+    JYC_LAUNCHED();
+    JYC_CUDA(cudaStreamSynchronize(nullptr));
+    return JYC_OK;
+}
+
 int sm_count() {
     static std::atomic<int> sms[64];
     int dev = 0, n = 0;

@@ -42,6 +42,8 @@ constexpr int kPagedErrRope = 4;  // position behind the RoPE tables
 constexpr int kPagedErrWait = 8;  // a copy's bounded wait gave up
 
 int* paged_error_word();
+// Clears these bits, and no other that a call sets meanwhile; they are clear on return.
+int paged_error_clear(int bits);
 // SMs of the current device (0: no device).
 int sm_count();
 // The kernel's limit of dynamic shared memory on the current device, set once for each.

@@ -610,3 +610,48 @@ def test_decode_steps_of_ragged_sequences(cuda):
             assert np.abs(host(out)[b] - o).max() <= tol
             ok = P.picks(host(logits)[b], float(T[b]), int(top_k[b]), float(top_p[b]), None, float(u[b]))
             assert int(token[b]) in ok, (step, b)
+
+
+def test_error_word_reset_loses_nothing(cuda):
+    """A flag raised by a call that is issued right after a reset, on a stream that the default one does not
+    order, is still there to be read, while another thread keeps the default stream busy."""
+    import threading
+    torch = cuda
+    lib = _capi.load()
+    pool = P.Pool(torch, 2, 8, 1, 64, [[0, 99]])
+    x = torch.zeros(1, 64, device="cuda")
+    seq = torch.zeros(1, dtype=torch.int32, device="cuda")
+    far, bad = (torch.tensor([p], dtype=torch.int32, device="cuda") for p in (16, 8))
+    stream = torch.cuda.Stream()
+
+    def append(pos, s):
+        _capi.check(lib.jyc_kv_append_paged_q8(
+            P.ptr(x), P.ptr(x), 64, 1, 1, 64, P.ptr(seq), P.ptr(pos), P.ptr(pool.table), 2, 1, None, None, 0,
+            C.byref(pool.desc), s))
+
+    big = torch.zeros(1 << 26, device="cuda")
+    ends = threading.Event()
+
+    def work():
+        done = [torch.cuda.Event() for _ in range(8)]  # eight passes ahead
+        for i in range(1 << 20):
+            done[i % 8].synchronize()
+            if ends.is_set():
+                break
+            big.add_(1.0)
+            done[i % 8].record()
+
+    torch.cuda.synchronize()
+    other = threading.Thread(target=work)
+    other.start()
+    try:
+        for i in range(300):
+            append(far, stream.cuda_stream)             # out of range: bit 1
+            assert lib.jyc_paged_error(1) == 1, i
+            append(bad, stream.cuda_stream)             # a bad page: bit 2
+            stream.synchronize()
+            assert lib.jyc_paged_error(1) == 2, i
+            assert lib.jyc_paged_error(0) == 0, i
+    finally:
+        ends.set()
+        other.join()
