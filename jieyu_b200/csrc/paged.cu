@@ -515,8 +515,8 @@ __device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, Pa
 }
 
 // A wait that did not end at once: gives up after 2^31 SM cycles (about a
-// second) and sets the error word; the unit then counts for nothing.
-__device__ __noinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
+// second) and sets the error word; the warp's run then ends with that unit.
+__device__ __noinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity) {
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity))
         if (clock64() - t0 > (1LL << 31)) {
@@ -524,6 +524,9 @@ __device__ __noinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
             return false;
         }
     return true;
+}
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
+    return mbar_try_wait(bar, parity) || pa_wait_slow(bar, parity);
 }
 // box of a map's tensor [page][slot][kv head][dim] -> shared memory (this CTA's)
 __device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* map, int h, int slot, int page,
@@ -836,6 +839,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     uint32_t qf[NK][E][2];
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4];
     bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
+    bool gave_up = false;
     int st = 0;
     uint32_t phase = 0u;
     const float up = __fmul_rn(a.scale, 1.44269504088896341f);
@@ -899,7 +903,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             const float* sc = reinterpret_cast<const float*>(ring + G::KOFF + st * 8 * TK);
             kscale = sc[lane];
             vscale = in ? sc[TK + lane] : 0.0f;
-            if (!mbar_try_wait(&s_bar[warp][st][0], phase) && !pa_wait(&s_bar[warp][st][0], phase)) in = false;
+            if (!pa_wait(&s_bar[warp][st][0], phase)) gave_up = true;
         } else {
             // the next unit's copies go to the stage that the last iteration read
             __syncwarp();
@@ -964,8 +968,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             }
         }
         if constexpr (TMA) {  // K is read: the unit ST ahead may take its place
-            __syncwarp();
-            issue_k(st);
+            if (!__any_sync(0xffffffffu, gave_up)) issue_k(st);
         }
         float al[E][2];
 #pragma unroll
@@ -1001,7 +1004,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                     if (HEADS > 4) lo[m][e][i] = pa_transpose(pl2);
                 }
         if constexpr (TMA)
-            if (!mbar_try_wait(&s_bar[warp][st][1], phase)) pa_wait(&s_bar[warp][st][1], phase);
+            if (!pa_wait(&s_bar[warp][st][1], phase)) gave_up = true;
         // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
         // rows g of the tile, the odd ones rows g + 8
 #pragma unroll
@@ -1036,9 +1039,13 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                         o[d + i][e][j] = __fmaf_rn(o[d + i][e][j], al[e][j & 1], c[i][e][j]);
         }
         if constexpr (TMA) {
-            __syncwarp();
-            issue_v(st);
-            lookup();
+            if (__any_sync(0xffffffffu, gave_up)) {
+                count = n + 1;  // the run ends here
+                gave_up = true;
+            } else {
+                issue_v(st);
+                lookup();
+            }
         }
         if (++st == ST) {
             st = 0;
@@ -1105,6 +1112,15 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (TMA && gave_up)  // the copies that are still on their way write to this CTA's memory
+        for (int i = 0; i < ST; i++) {
+            pa_wait(&s_bar[warp][st][0], phase);
+            pa_wait(&s_bar[warp][st][1], phase);
+            if (++st == ST) {
+                st = 0;
+                phase ^= 1u;
+            }
+        }
     // CTAs behind this one that hold parts of an item that ends at unit `end`
     auto later = [&](long long end) { return (int)(line.worker(end - 1) / line.per_cta) - (int)blockIdx.x; };
     if (!joint) {
