@@ -111,6 +111,12 @@ class ClockSampler:
                 "reasons": sorted(reasons)}
 
 
+def times_cpu_baseline(args):
+    """Whether a line carries the reference's own CPU decode: not where it was not built."""
+    from oracle.bind import reference_available
+    return not args.no_cpu_baseline and reference_available()
+
+
 def reference_decode_sample(hw, threads, new_tokens=16, prompt_len=16, reps=2):
     """The reference's own generate() (oracle/_ref: the jieyu headers compiled
     unmodified) on this host: decode tok/s over a bounded sample."""
@@ -358,7 +364,7 @@ def run_c1(args):
     e2e_value = sum_over_ranks(e2e_steps * DECODE) / e2e_s
 
     cpu = None
-    if rank == 0 and world == 1 and not args.no_cpu_baseline:
+    if rank == 0 and world == 1 and times_cpu_baseline(args):
         threads = os.cpu_count() or 1
         dec, _, cores = reference_decode_sample(hw, threads)
         cpu = {"value": dec, "unit": UNIT, "cores": cores, "kind": "reference",
@@ -604,7 +610,7 @@ def run_headline(args):
         m.close()
 
     cpu = None
-    if rank == 0 and world == 1 and not args.no_cpu_baseline:
+    if rank == 0 and world == 1 and times_cpu_baseline(args):
         rd = RefContextDecode(hw.desc, cfg.layers, cfg.kv_heads, cfg.head_dim, cfg.max_seq, CTX,
                               os.cpu_count() or 1)
         rd.run(1)
