@@ -303,7 +303,8 @@ JYC_API int jyc_kv_read_paged_q8(float* K, float* V, int ld, int rows, int num_k
  * out + s * ldo. The query is quantised per head and scored as in
  * jyc_attention_q8 (int32 dots, dot * ((ks * qs) * 1/sqrt(head_dim)), fp32
  * softmax, V scaled by vs; scales are not negative, and one that is not finite
- * makes the rows that attend to it NaN). cos/sin tables: the query is rotated by its
+ * makes the rows that attend to it NaN; a row whose scores pass 1e38 in magnitude
+ * has no meaning). cos/sin tables: the query is rotated by its
  * position first; NULL: it arrives rotated. A sequence of length <= 0 gets a
  * row of zeros, as does one whose query position lies behind the tables; a
  * length above table_stride * page_size is cut to that; keys on a page that is

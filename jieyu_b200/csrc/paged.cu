@@ -132,19 +132,21 @@ __device__ __forceinline__ uint32_t pack4(float4 x, float inv) {
 }
 
 // ---------------------------------------------------------------------------
-// Append and read back: bound by their bytes (append reads 8 hd and writes 2 hd
-// + 8 per row and kv head, read the reverse), once the bookkeeping of a row is
-// shared: a warp takes kRowUnits * (32 / LANES) heads of K or of V of one row.
-// LANES lanes hold a head, QUADS groups of four dims each; neighbouring heads
-// lie side by side in a warp (whole sectors), and the loads of all units are
-// issued before the first is used; only where a unit goes waits for the row's
-// position and page. (A warp of heads of several rows, each with its own
+// Append and read back: append reads 8 hd and writes 2 hd + 8 bytes per row and
+// kv head, read the reverse. The bookkeeping of a row is shared: a warp takes
+// kRowUnits * (32 / LANES) heads of K or of V of one row. LANES lanes hold a
+// head, QUADS groups of four dims each; neighbouring heads lie side by side in a
+// warp (whole sectors), and the loads of all units are issued before the first
+// is used. They wait for the row's position (a skipped row loads nothing), in
+// append not for its page, which only the stores need. (A warp of heads of several rows, each with its own
 // position, page and 64-bit offsets, executes 265 instructions per head of 128
 // and is bound by them.) Half as many units in flight per warp cost a fifth
 // (read of 32768 rows of 8 x 128 88 us against 74), twice as many gain nothing;
 // CTAs of 4 warps fill the SMs more evenly than 8 (append 97 -> 91 us).
-// Measured at 8 x 128: 32768 rows read in 72 us (4.7 TB/s; floor 52), 16384 rows
-// appended and read back in 91 us (floor 52).
+// Measured at 8 x 128: 16384 rows appended in 55.5 us (floor 26), bound by
+// instructions: 168 per head and warp, issue slots 76 % busy with half of the warps
+// resident (56 registers). 32768 rows read in 72 us (4.7 TB/s; floor 52): the warps
+// wait for position, page and row in a chain (issue slots 55 % busy).
 constexpr int kRowUnits = 4, kRowThreads = 128;
 
 struct RowWarp {
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float
 //
 // Measured: 131072 keys of 8 x 128 67 us (floor 43; 7 TB/s while every warp
 // streams), 64 sequences of 2048 to 2176 keys of 8 x 64 43 us (floor 23), 45 of
-// 1 to 8192 keys of 8 x 128 83 us (floor 60). What is over the floor is the
+// 1 to 8192 keys of 8 x 128 79 to 85 us by their lengths (floor 60). What is over the floor is the
 // ends: finding each warp's run in lens, Q and the page table before the first
 // key (8 us), the spread of the warps' ends and the joins (8), the second
 // kernel (4).
@@ -1309,8 +1311,8 @@ int pa_map(CUtensorMap* m, int8_t* base, const PagedAttn& a, int box) {
 
 // Tensor copies need rows of 64 or 128 bytes, strides below 2^40 that are multiples of 16 bytes, pages that
 // a unit of 32 keys fills or that fill a unit, and boxes that start on 128 bytes of shared memory. Against 16-byte
-// cp.async: 64 sequences of 2112 keys of 8 x 64 44 us to 61, 45 of 1 to 8192 keys of 8 x 128 87 to 91, one of 131072
-// the same.
+// cp.async: 64 sequences of 2112 keys of 8 x 64 44 us to 61, 45 of 1 to 8192 keys of 8 x 128 85 to 88, but one of
+// 131072 keys 67 to 62.
 bool pa_tensor_copies(const PagedAttn& a, bool aligned) {
     const jyc_kv_pages& p = a.kv.p;
     const long long far = std::max(p.page_stride, std::max(p.pos_stride, p.head_stride));
@@ -1447,7 +1449,7 @@ int launch_paged_attention(const PagedAttn& a, void* work, cudaStream_t s) {
     pl.units_row = KV * pl.qblocks;
     pl.wide_q = aligned16(a.Q, a.ldq) && aligned8(a.rope.cos_t, a.rope.sin_t);
     const jyc_kv_pages& p = a.kv.p;
-    // 16-byte copies, else 4-byte ones (131072 keys of 8 x 128: 66 us to 145)
+    // 16-byte copies, else 4-byte ones (131072 keys of 8 x 128: 62 us to 142; 64 sequences of 2112 of 8 x 64: 61 to 119)
     pl.wide_copy = hd % 16 == 0 && (((uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0 &&
                    ((p.page_stride | p.pos_stride | p.head_stride) & 15) == 0;
     if (pa_tensor_copies(a, pl.wide_copy)) PA_CASES(pa_launch, true, a, pl, sms, work, s);

@@ -20,18 +20,18 @@
 //   3  pools of 4096 tokens in all or fewer: one CTA takes them and ends the row,
 //      finding each border by bisection over keys.
 //      More: the histogram bounds the running count or mass, so the border lies in
-//      one or two bins; their tokens go to one CTA (or are split again while they
-//      are more than 512), which finds the last kept one by sums over digits of
+//      one or two bins; their tokens go to one CTA (or are split by exact sums while
+//      they are more than 512), which finds the last kept one by sums over digits of
 //      the keys. The kept weights are summed by warp, in index order; the warp
 //      that the draw falls in walks its tokens.
 //   Rows without a filter, with k above 2048, and rows whose pools overflow go
 //   through 3 over all their logits instead of the pools.
 // Floor: one read of the logits; later passes find them in L2. What is left of
-// the time is the chain of passes and exchanges of a row (about 20 us for one row
-// with top-k, 49 with top-p alone); with many rows too: warps wait at barriers
-// more than for memory, and 41 % of the issue slots are busy, with the exact
-// weights above all (22 instructions per logit and pass, 11 of them in double
-// precision).
+// the time is the chain of passes and exchanges of a row (21 us for one row with
+// top-k, 49 with top-p alone); with many rows too: warps wait at barriers more than
+// for memory (64 rows of top-p: 5.8 stalls an issue against 1.7), and 42 % of the
+// issue slots are busy. They execute 203 instructions per 32 logits over all
+// passes; the exact weights of one pass are 22 of them, 11 in double precision.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1058,10 +1058,11 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(PickArgs a, int C
 
 // CTAs of a row: up to 4 CTAs per SM in all, while a CTA keeps 4096 logits or
 // more. Two are resident; rows differ in their work, so a second wave evens it
-// out (256 mixed rows of 128256: 367 us with one CTA each, 257 with two, 259
-// with four; 140 rows of top-p alone: 214, 192 and 283); below 4096 logits the
-// exchanges cost more than the passes (62 rows of 14783, k = 1150: 58 us, 80 at
-// 2048).
+// out (256 mixed rows of 128256: 357 us with one CTA each, 250 with two, 241
+// with four; 140 rows of top-p alone with two, four and eight: 207, 183 and 271).
+// 64 rows would rather have one wave (top-p alone with two, four and eight each: 195,
+// 128 and 134 us; mixed: 126, 83 and 116). Below 4096 logits the exchanges cost more
+// than the passes (62 rows of 14783, k = 1150: 35 us, 40 at 2048).
 int launch_pick(const PickArgs& a, cudaStream_t s) {
     if (a.rows == 0) return JYC_OK;
     const int sms = sm_count();
