@@ -278,9 +278,9 @@ def _four(x):
     hd, groups = x.shape[-1], _groups(x.shape[-1])
     pad = 32 * groups - hd
     spread = lambda fill: torch.nn.functional.pad(x, (0, pad), value=fill).unflatten(-1, (groups, 32))  # noqa: E731
-    low, high = spread(math.inf).amin(-1), spread(-math.inf).amax(-1)
-    step = ((high - low) / torch.full_like(low, 15.0)).clamp(max=65504.0).half().float()
-    low = low.clamp(-65504.0, 65504.0).half().float()
+    low, high = (a.clamp(-65504.0, 65504.0) for a in (spread(math.inf).amin(-1), spread(-math.inf).amax(-1)))
+    step = ((high - low) / torch.full_like(low, 15.0)).half().float()
+    low = low.half().float()
     inverse = torch.where(step > 0, 1.0 / step, 0.0)
     q = ((spread(0.0) - low[..., None]) * inverse[..., None]).round().clamp(0, 15)
     if pad:
@@ -545,7 +545,7 @@ def _f32(x):
 
 
 def _f16(x):
-    return np.clip(x, -65504.0, 65504.0).astype(np.float32).astype(np.float16).astype(np.float64)
+    return np.asarray(x, np.float64).astype(np.float32).astype(np.float16).astype(np.float64)
 
 
 def _np(x):
@@ -579,7 +579,7 @@ def _through_four_bits(x):
     out = np.empty_like(x)
     for d in range(0, x.shape[-1], 32):
         g = x[..., d: d + 32]
-        low, high = g.min(-1, keepdims=True), g.max(-1, keepdims=True)
+        low, high = (np.clip(a, -65504.0, 65504.0) for a in (g.min(-1, keepdims=True), g.max(-1, keepdims=True)))
         step, base = _f16(_f32(_f32(high - low) / 15.0)), _f16(low)
         inverse = np.where(step > 0, _f32(1.0 / np.where(step > 0, step, 1.0)), 0.0)
         q = np.clip(np.rint(_f32(_f32(g - base) * inverse)), 0, 15)
