@@ -109,6 +109,34 @@ JYC_API long long jyc_kernel_launches(void);
 JYC_API int jyc_rope_table(int max_seq, int head_dim, float theta,
                            float* cos_out, float* sin_out);
 
+/* Scaling of the RoPE frequencies for contexts longer than a model's first one
+ * (no counterpart in the reference). f_j = theta^(-2j / rot_dim) becomes, with
+ * L = original_len and n_j = L f_j / (2 pi) the turns that pair j makes in it:
+ *   JYC_ROPE_NONE    f_j
+ *   JYC_ROPE_LINEAR  f_j / factor
+ *   JYC_ROPE_NTK     (theta * factor^(rot_dim / (rot_dim - 2)))^(-2j / rot_dim)
+ *   JYC_ROPE_BANDS   n_j <= low: f_j / factor; n_j >= high: f_j; between them
+ *                    f_j ((1 - t) / factor + t), t = (n_j - low) / (high - low)
+ *   JYC_ROPE_RAMP    the same with t linear in j: j_low is the pair that makes
+ *                    `high` turns, rounded down, j_high the one that makes
+ *                    `low`, rounded up, both within 0 .. rot_dim - 1,
+ *                    t = 1 - (j - j_low) / (j_high - j_low) held within 0 .. 1;
+ *                    cos and sin are multiplied by attention (0: 0.1 ln(factor) + 1).
+ * factor >= 1; low < high and original_len > 0 where they are used. */
+enum { JYC_ROPE_NONE = 0, JYC_ROPE_LINEAR = 1, JYC_ROPE_NTK = 2, JYC_ROPE_BANDS = 3, JYC_ROPE_RAMP = 4 };
+typedef struct jyc_rope_scaling {
+    int kind;
+    float factor;
+    int original_len;
+    float low, high;
+    float attention;
+} jyc_rope_scaling;
+/* Tables [max_seq][rot_dim / 2] with scaled frequencies: angles in double, cos
+ * and sin rounded once (jyc_rope_table's are the reference's, all in float).
+ * scaling NULL: none. rot_dim even. HOST pointers. */
+JYC_API int jyc_rope_table_scaled(int max_seq, int rot_dim, float theta, const jyc_rope_scaling* scaling,
+                                  float* cos_out, float* sin_out);
+
 /* Seeded synthetic data (no reference counterpart: the reference has no
  * quantiser, GGUF blocks are copied raw, libs/gguf_libs/gguf_convert.h:201-229).
  * Values are an exact integer function of (seed, stream, index):
@@ -348,6 +376,136 @@ JYC_API int jyc_paged_error(int reset);
 JYC_API int jyc_sample_batch(const float* logits, int ld, int rows, int vocab_size, const float* temperature,
                              const int* top_k, const float* top_p, const float* min_p, const float* u, int* out_ids,
                              float* out_probs, void* stream);
+
+/* ---- rotary rows and 8-bit products (DEVICE pointers, asynchronous; no counterpart in the
+ * reference, whose rope_pos rotates whole heads of consecutive positions and whose products take
+ * fp32 activations) */
+
+/* Rotary positions of the operators below: the first rot_dim dims of a head
+ * (even, <= head_dim) turn by their row's position, the others stay. Pair j is
+ * dims (2j, 2j + 1) or (j, j + rot_dim / 2), and keeps its place (jyc_rope_pos's
+ * pairs take the reference's slot order; a product of a query and a key that
+ * were turned the same way is the same). Tables [len][rot_dim / 2] on the device, as
+ * jyc_rope_table and jyc_rope_table_scaled make them; rounding as jyc_rope_pos:
+ * one product rounded, one fused sum. The struct is read by the host during the
+ * call. */
+enum { JYC_ROPE_PAIRS = 0, JYC_ROPE_HALVES = 1 };
+typedef struct jyc_rope {
+    const float* cos_table;
+    const float* sin_table;
+    int len;
+    int rot_dim;
+    int layout;
+} jyc_rope;
+
+/* Y = X turned by its rows' positions: rows of num_heads * head_dim floats at X
+ * + i * ldx, Y + i * ldy, row i at position row_pos[i] (device). Y may be X with
+ * ldy == ldx; other overlaps are not allowed. Query and key heads that lie side
+ * by side in a row go in one call. A row with a negative position is left as
+ * it was, as is one whose position lies behind the tables (which sets bit 4 of
+ * the paged error word, jyc_paged_error). */
+JYC_API int jyc_rope_rows(const float* X, int ldx, float* Y, int ldy, int rows, int num_heads, int head_dim,
+                          const int* row_pos, const jyc_rope* rope, void* stream);
+
+/* Rows of x [rows][k] (row stride ldx floats) in 8 bits with one scale each:
+ * kv_pack_q8's rule over a whole row (jyc_kv_pack_q8), q at row stride ldq bytes. A NaN
+ * counts as 0; a row with an infinity gets an infinite scale and zeros. k > 0. */
+JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_t* q, int ldq, float* scale,
+                                 void* stream);
+
+/* C[m][n] = (sum_k A[i][k] W[j][k]) * (a_scale[i] * w_scale[j]) + bias[j]: the
+ * whole-number sum is exact (32 bits), then rounded to fp32, multiplied and
+ * added, one rounding each. A [m] rows of stride lda bytes and their scales
+ * (jyc_quantize_rows_i8's), W [n] rows of stride ldw (one per output channel)
+ * and theirs, C rows of stride ldc floats; bias may be NULL. A and W are
+ * 16-byte aligned, lda and ldw multiples of 16; what lies between k and a
+ * row's stride does not count. k <= 131071 (127^2 k, and 128^2 k, stay below
+ * 2^31). Nothing is allocated. */
+JYC_API int jyc_matmul_i8(const int8_t* A, int lda, const float* a_scale, const int8_t* W, int ldw,
+                          const float* w_scale, const float* bias, float* C, int ldc, int m, int n, int k,
+                          void* stream);
+
+/* ---- paged K/V cache in 4 bits (DEVICE pointers, asynchronous) ----------- *
+ * The cache above at 5 bits a value, for contexts that do not fit in 8: rows in
+ * groups of 32 dims (the last may be shorter), each with two fp16 numbers: low,
+ * its smallest value, and step, a fifteenth of its range (values held within
+ * +-65504, infinities too; both rounded to nearest); value i is low + step * q_i,
+ * q_i = rint((x_i - low) * (1 / step)) within 0 .. 15 (fp32; 0 where step is 0).
+ * A NaN is stored as q = 0, and not counted in low and step.
+ * With G = ceil(head_dim / 32), a row of one kv head is 16 G bytes: byte b of
+ * group g holds dims 32 g + b (low bits) and 32 g + 16 + b (high bits), dims
+ * behind head_dim as 0; its parameters are G pairs (step, low). Row (page, slot, kv head)
+ * starts at page * page_stride + slot * pos_stride + head * head_stride (bytes;
+ * k, v and the strides are multiples of 16), its parameters at the p*_stride
+ * ones (in pairs, of 4 bytes), its accumulated weight at the m*_stride ones
+ * (floats). Rows of different (page, slot, head) do not overlap. mass may be
+ * NULL where no operator needs it. Pages, page tables, lengths and the error
+ * word are as for jyc_kv_pages. */
+typedef struct jyc_kv_pages_q4 {
+    uint8_t*  k;
+    uint16_t* kp;
+    uint8_t*  v;
+    uint16_t* vp;
+    float*    mass;
+    int num_pages;
+    int page_size;
+    long long page_stride, pos_stride, head_stride;
+    long long ppage_stride, ppos_stride, phead_stride;
+    long long mpage_stride, mpos_stride, mhead_stride;
+} jyc_kv_pages_q4;
+
+/* jyc_kv_append_paged_q8 for these pages. rope NULL: K arrives turned; else
+ * row i turns by rope_pos[i] (rope_pos NULL: row_pos[i]; they differ once rows
+ * were evicted; a negative one, like one behind the tables, skips the row and
+ * sets bit 4). The rows' mass, where there is one, starts at 0. */
+JYC_API int jyc_kv_append_paged_q4(const float* K, const float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                   const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                   int num_seqs, const jyc_rope* rope, const int* rope_pos,
+                                   const jyc_kv_pages_q4* pages, void* stream);
+
+/* jyc_kv_read_paged_q8 for these pages: low + step * q, rounded once. */
+JYC_API int jyc_kv_read_paged_q4(float* K, float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                 const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                 int num_seqs, const jyc_kv_pages_q4* pages, void* stream);
+
+/* jyc_attention_paged_q8 for these pages: the query is quantised to 8 bits per
+ * head, the score of a key is qs * sum_g (step_g * dot_g + low_g * qsum_g) / sqrt(head_dim)
+ * with whole-number dots and query sums of each group, out = sum p v / sum p.
+ * rope: the query turns by rope_pos[s] (NULL: seq_lens[s] - 1); a position
+ * outside of the tables gives a row of zeros and sets bit 4. With mass, each
+ * key's weight p / sum p, summed over the query heads of its kv head, is added
+ * to its place (one addition per key and call; keys that several sequences of a
+ * call share get theirs in no fixed order). A low or step that is not finite
+ * makes the rows that attend to it NaN, and their weights.
+ * workspace: at least jyc_attention_paged_q4_workspace bytes, 16-byte aligned;
+ * as for jyc_attention_paged_q8, NULL takes scratch in stream order. */
+JYC_API int jyc_attention_paged_q4(const float* Q, int ldq, float* out, int ldo, int num_heads, int num_kv_heads,
+                                   int head_dim, const int* seq_lens, const int* page_table, int table_stride,
+                                   int num_seqs, const jyc_rope* rope, const int* rope_pos,
+                                   const jyc_kv_pages_q4* pages, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+/* Bytes of workspace of the call above on the current device (0: bad shape).
+ * capacity: table_stride * page_size for calls with mass, 0 for those without. */
+JYC_API size_t jyc_attention_paged_q4_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                                int capacity);
+
+/* Leaves behind the rows of least accumulated weight: of a sequence longer than
+ * budget each kv head keeps its last `recent` rows and, of the others, the
+ * budget - recent of largest mass (ties to the lower position; NaN is below
+ * every number), a sequence within the budget all of its rows. Kept rows go,
+ * in their order and with their parameters and mass, to positions 0, 1, ... of
+ * the pages of new_table [num_seqs][new_stride] (new_stride * page_size >=
+ * budget); new_lens[s] = min(seq_lens[s], budget) (not below 0). kept
+ * [num_seqs][num_kv_heads][budget] gets their old positions, -1 behind the
+ * last. The pages of new_table are other ones than those of page_table (a
+ * sequence that keeps all of its rows may name its old pages, which then stay
+ * as they are); afterwards the old pages are free. new_lens is another array
+ * than seq_lens. pages->mass must be there. 0 <= recent <= budget, budget > 0.
+ * A row whose old or new page is out of range is not copied (error word). */
+JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, int num_kv_heads, int head_dim,
+                                  const int* page_table, int table_stride, int num_seqs, const int* new_table,
+                                  int new_stride, int* new_lens, int* kept, const jyc_kv_pages_q4* pages,
+                                  void* stream);
 
 /* ---- operator entry points with the reference's calling convention ------
  * HOST pointers in the reference's own layouts, caller-owned, synchronous:

@@ -80,6 +80,36 @@ class KVPages(C.Structure):
     ]
 
 
+JYC_ROPE_NONE, JYC_ROPE_LINEAR, JYC_ROPE_NTK, JYC_ROPE_BANDS, JYC_ROPE_RAMP = 0, 1, 2, 3, 4  # jyc_rope_scaling.kind
+JYC_ROPE_PAIRS, JYC_ROPE_HALVES = 0, 1  # jyc_rope.layout
+
+
+class RopeScaling(C.Structure):
+    """Layout of jyc_rope_scaling."""
+
+    _fields_ = [("kind", C.c_int), ("factor", C.c_float), ("original_len", C.c_int), ("low", C.c_float),
+                ("high", C.c_float), ("attention", C.c_float)]
+
+
+class Rope(C.Structure):
+    """Layout of jyc_rope: device tables, the dims they turn and how pairs lie."""
+
+    _fields_ = [("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("len", C.c_int), ("rot_dim", C.c_int),
+                ("layout", C.c_int)]
+
+
+class KVPagesQ4(C.Structure):
+    """Layout of jyc_kv_pages_q4: a 4-bit K/V cache in pages, by strides."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("kp", C.c_void_p), ("v", C.c_void_p), ("vp", C.c_void_p), ("mass", C.c_void_p),
+        ("num_pages", C.c_int), ("page_size", C.c_int),
+        ("page_stride", C.c_longlong), ("pos_stride", C.c_longlong), ("head_stride", C.c_longlong),
+        ("ppage_stride", C.c_longlong), ("ppos_stride", C.c_longlong), ("phead_stride", C.c_longlong),
+        ("mpage_stride", C.c_longlong), ("mpos_stride", C.c_longlong), ("mhead_stride", C.c_longlong),
+    ]
+
+
 TOKEN_CB = C.CFUNCTYPE(C.c_int, C.c_int, C.c_void_p)
 
 # (name, restype, argtypes) of every exported entry point.
@@ -89,6 +119,7 @@ SIGNATURES = [
     ("jyc_last_error", C.c_char_p, []),
     ("jyc_kernel_launches", C.c_longlong, []),
     ("jyc_rope_table", _I, [_I, _I, _F, _P, _P]),
+    ("jyc_rope_table_scaled", _I, [_I, _I, _F, C.POINTER(RopeScaling), _P, _P]),
     ("jyc_synth_f32", _I, [_U64, _U64, _F, _P, _SZ]),
     ("jyc_synth_q8_0", _I, [_U64, _U64, _F, _P, _SZ, _SZ]),
     ("jyc_synth_ids", _I, [_U64, _U64, _I, _P, _SZ]),
@@ -126,6 +157,17 @@ SIGNATURES = [
     ("jyc_attention_paged_q8_workspace", _SZ, [_I, _I, _I, _I]),
     ("jyc_paged_error", _I, [_I]),
     ("jyc_sample_batch", _I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    ("jyc_rope_rows", _I, [_P, _I, _P, _I, _I, _I, _I, _P, C.POINTER(Rope), _P]),
+    ("jyc_quantize_rows_i8", _I, [_P, _I, _I, _I, _P, _I, _P, _P]),
+    ("jyc_matmul_i8", _I, [_P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P]),
+    ("jyc_kv_append_paged_q4", _I,
+     [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, C.POINTER(Rope), _P, C.POINTER(KVPagesQ4), _P]),
+    ("jyc_kv_read_paged_q4", _I, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, C.POINTER(KVPagesQ4), _P]),
+    ("jyc_attention_paged_q4", _I,
+     [_P, _I, _P, _I, _I, _I, _I, _P, _P, _I, _I, C.POINTER(Rope), _P, C.POINTER(KVPagesQ4), _P, _SZ, _P]),
+    ("jyc_attention_paged_q4_workspace", _SZ, [_I, _I, _I, _I, _I]),
+    ("jyc_kv_evict_paged_q4", _I,
+     [_P, _I, _I, _I, _I, _P, _I, _I, _P, _I, _P, _P, C.POINTER(KVPagesQ4), _P]),
     ("jyc_model_create", _P, [C.POINTER(ModelDesc)]),
     ("jyc_model_free", None, [_P]),
     ("jyc_model_weight_bytes_per_token", C.c_double, [_P]),

@@ -5,9 +5,12 @@
 #include <mutex>
 #include <vector>
 
+#include "i8.cuh"
 #include "kernels.cuh"
 #include "mega.cuh"
 #include "paged.cuh"
+#include "paged4.cuh"
+#include "rope.cuh"
 #include "tcgemm.cuh"
 #include "skinny.cuh"
 
@@ -510,6 +513,201 @@ JYC_API int jyc_sample_batch(const float* logits, int ld, int rows, int vocab_si
     if (!logits || !u || !out_ids) return arg_error("sample_batch: null pointer");
     const PickArgs a{logits, ld, rows, vocab_size, temperature, top_k, top_p, min_p, u, out_ids, out_probs};
     return launch_pick(a, S(stream));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Rotary rows, 8-bit products and the 4-bit paged cache.
+namespace {
+
+int check_rope_view(const char* what, const jyc_rope* r, int head_dim, RopeView* v) {
+    auto bad = [&](const char* msg) { return arg_error(std::string(what) + ": " + msg); };
+    *v = RopeView{nullptr, nullptr, 0, 0, false};
+    if (!r) return JYC_OK;
+    if (!r->cos_table || !r->sin_table) return bad("cos and sin tables come together");
+    if (((uintptr_t)r->cos_table | (uintptr_t)r->sin_table) & 3) return bad("misaligned tables");
+    if (r->len <= 0) return bad("the tables' len must be positive");
+    if (r->rot_dim <= 0 || r->rot_dim % 2 || r->rot_dim > head_dim) return bad("rot_dim must be even, <= head_dim");
+    if (r->layout != JYC_ROPE_PAIRS && r->layout != JYC_ROPE_HALVES) return bad("unknown rope layout");
+    *v = RopeView{r->cos_table, r->sin_table, r->len, r->rot_dim / 2, r->layout == JYC_ROPE_HALVES};
+    return JYC_OK;
+}
+
+// The arguments that the operators of the 4-bit pages share.
+int check_paged4(const char* what, int num_kv_heads, int head_dim, const int* page_table, int table_stride,
+                 int num_seqs, const jyc_kv_pages_q4* p) {
+    auto bad = [&](const char* msg) { return arg_error(std::string(what) + ": " + msg); };
+    if (num_kv_heads <= 0) return bad("num_kv_heads must be positive");
+    if (head_dim <= 0 || head_dim % 4 || head_dim > 256) return bad("head_dim must be a multiple of 4, <= 256");
+    if (num_seqs < 0 || table_stride < 0) return bad("negative page table shape");
+    if (!page_table || !p || !p->k || !p->kp || !p->v || !p->vp) return bad("null pointer");
+    if (p->num_pages <= 0 || p->page_size <= 0) return bad("num_pages and page_size must be positive");
+    if ((long long)table_stride * p->page_size > 0x7fffff00LL)
+        return bad("table_stride * page_size must be below 2^31 - 255");
+    if (p->page_stride < 0 || p->pos_stride < 0 || p->head_stride < 0 || p->ppage_stride < 0 || p->ppos_stride < 0 ||
+        p->phead_stride < 0 || p->mpage_stride < 0 || p->mpos_stride < 0 || p->mhead_stride < 0)
+        return bad("negative page stride");
+    if ((((uintptr_t)p->k | (uintptr_t)p->v) & 15) || ((p->page_stride | p->pos_stride | p->head_stride) & 15))
+        return bad("k, v and their strides must be multiples of 16 bytes");
+    if (((uintptr_t)p->kp | (uintptr_t)p->vp | (uintptr_t)p->mass | (uintptr_t)page_table) & 3)
+        return bad("misaligned parameters, mass or page table");
+    return JYC_OK;
+}
+
+// Of one launch's grid: heads of sequences, rows of kept positions.
+constexpr long long kMaxItems = 0x7fffffffLL;
+
+int paged4_view(const jyc_kv_pages_q4* pages, const int* page_table, int table_stride, int num_seqs, PagedKV4* kv) {
+    int* err = paged_error_word();
+    if (!err) return cuda_fail(cudaErrorNoDevice, "paged error word");
+    *kv = PagedKV4{*pages, page_table, table_stride, num_seqs, fast_div(pages->page_size), err};
+    return JYC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+JYC_API int jyc_rope_rows(const float* X, int ldx, float* Y, int ldy, int rows, int num_heads, int head_dim,
+                          const int* row_pos, const jyc_rope* rope, void* stream) {
+    clear_error();
+    if (rows < 0 || num_heads <= 0 || head_dim <= 0) return arg_error("rope_rows: bad shape");
+    if (!rope) return arg_error("rope_rows: null rope");
+    RopeView r;
+    TRY(check_rope_view("rope_rows", rope, head_dim, &r));
+    if ((long long)num_heads * head_dim > ldx || (long long)num_heads * head_dim > ldy)
+        return arg_error("rope_rows: ldx and ldy must hold num_heads * head_dim");
+    if (rows == 0) return JYC_OK;
+    if (!X || !Y || !row_pos) return arg_error("rope_rows: null pointer");
+    if (X == Y && ldx != ldy) return arg_error("rope_rows: in place needs ldx == ldy");
+    return launch_rope_rows(X, ldx, Y, ldy, rows, num_heads, head_dim, row_pos, r, S(stream));
+}
+
+JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_t* q, int ldq, float* scale,
+                                 void* stream) {
+    clear_error();
+    if (rows < 0 || k <= 0) return arg_error("quantize_rows_i8: need rows >= 0 and k > 0");
+    if (ldx < k || ldq < k) return arg_error("quantize_rows_i8: ldx and ldq must hold k");
+    if (rows == 0) return JYC_OK;
+    if (!x || !q || !scale) return arg_error("quantize_rows_i8: null pointer");
+    return launch_quantize_rows(x, ldx, rows, k, q, ldq, scale, S(stream));
+}
+
+JYC_API int jyc_matmul_i8(const int8_t* A, int lda, const float* a_scale, const int8_t* W, int ldw,
+                          const float* w_scale, const float* bias, float* C, int ldc, int m, int n, int k,
+                          void* stream) {
+    clear_error();
+    if (m < 0 || n <= 0 || k <= 0) return arg_error("matmul_i8: need m >= 0 and n, k > 0");
+    if (k > 131071) return arg_error("matmul_i8: k above 131071 can pass 32-bit sums");
+    if (lda < k || ldw < k || ldc < n) return arg_error("matmul_i8: lda and ldw must hold k, ldc must hold n");
+    if ((lda | ldw) & 15) return arg_error("matmul_i8: lda and ldw must be multiples of 16");
+    if (m == 0) return JYC_OK;
+    if (!A || !a_scale || !W || !w_scale || !C) return arg_error("matmul_i8: null pointer");
+    if (((uintptr_t)A | (uintptr_t)W) & 15) return arg_error("matmul_i8: A and W must be 16-byte aligned");
+    return launch_i8_gemm(I8Gemm{A, lda, a_scale, W, ldw, w_scale, bias, C, ldc, m, n, k}, S(stream));
+}
+
+JYC_API int jyc_kv_append_paged_q4(const float* K, const float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                   const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                   int num_seqs, const jyc_rope* rope, const int* rope_pos,
+                                   const jyc_kv_pages_q4* pages, void* stream) {
+    clear_error();
+    TRY(check_paged4("kv_append_paged_q4", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    RopeView r;
+    TRY(check_rope_view("kv_append_paged_q4", rope, head_dim, &r));
+    if (rows < 0) return arg_error("kv_append_paged_q4: negative rows");
+    if (ld < (long long)num_kv_heads * head_dim) return arg_error("kv_append_paged_q4: ld below num_kv_heads * head_dim");
+    if (!row_seq && rows > num_seqs) return arg_error("kv_append_paged_q4: more rows than sequences without row_seq");
+    if (rows == 0) return JYC_OK;
+    if (!K || !V || !row_pos) return arg_error("kv_append_paged_q4: null pointer");
+    PagedKV4 kv;
+    TRY(paged4_view(pages, page_table, table_stride, num_seqs, &kv));
+    return launch_paged4_append(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, rope_pos, kv, r, S(stream));
+}
+
+JYC_API int jyc_kv_read_paged_q4(float* K, float* V, int ld, int rows, int num_kv_heads, int head_dim,
+                                 const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
+                                 int num_seqs, const jyc_kv_pages_q4* pages, void* stream) {
+    clear_error();
+    TRY(check_paged4("kv_read_paged_q4", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    if (rows < 0) return arg_error("kv_read_paged_q4: negative rows");
+    if (ld < (long long)num_kv_heads * head_dim) return arg_error("kv_read_paged_q4: ld below num_kv_heads * head_dim");
+    if (!row_seq && rows > num_seqs) return arg_error("kv_read_paged_q4: more rows than sequences without row_seq");
+    if (rows == 0) return JYC_OK;
+    if (!K || !V || !row_pos) return arg_error("kv_read_paged_q4: null pointer");
+    PagedKV4 kv;
+    TRY(paged4_view(pages, page_table, table_stride, num_seqs, &kv));
+    return launch_paged4_read(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv, S(stream));
+}
+
+JYC_API size_t jyc_attention_paged_q4_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                                int capacity) {
+    clear_error();
+    if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+        head_dim % 4 || head_dim > 256 || capacity < 0 || capacity > 0x7fffff00 ||
+        (long long)num_seqs * num_heads > kMaxItems) {
+        arg_error("attention_paged_q4_workspace: bad shape");
+        return 0;
+    }
+    const size_t n = paged4_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim, capacity);
+    if (n == 0) cuda_fail(cudaErrorNoDevice, "attention_paged_q4_workspace: device query");
+    return n;
+}
+
+JYC_API int jyc_attention_paged_q4(const float* Q, int ldq, float* out, int ldo, int num_heads, int num_kv_heads,
+                                   int head_dim, const int* seq_lens, const int* page_table, int table_stride,
+                                   int num_seqs, const jyc_rope* rope, const int* rope_pos,
+                                   const jyc_kv_pages_q4* pages, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    clear_error();
+    TRY(check_paged4("attention_paged_q4", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    RopeView r;
+    TRY(check_rope_view("attention_paged_q4", rope, head_dim, &r));
+    if (num_heads <= 0 || num_heads % num_kv_heads)
+        return arg_error("attention_paged_q4: num_heads must be a multiple of num_kv_heads");
+    if (ldq < (long long)num_heads * head_dim || ldo < (long long)num_heads * head_dim)
+        return arg_error("attention_paged_q4: ldq and ldo must hold num_heads * head_dim");
+    if ((long long)num_seqs * num_heads > kMaxItems) return arg_error("attention_paged_q4: num_seqs * num_heads above 2^31 - 1");
+    if (num_seqs == 0) return JYC_OK;
+    if (!Q || !out || !seq_lens) return arg_error("attention_paged_q4: null pointer");
+    const int capacity = pages->mass ? table_stride * pages->page_size : 0;
+    const size_t need = paged4_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim, capacity);
+    if (need == 0) return cuda_fail(cudaErrorNoDevice, "attention_paged_q4: device query");
+    if (workspace && workspace_bytes < need) return arg_error("attention_paged_q4: workspace too small");
+    if ((uintptr_t)workspace & 15) return arg_error("attention_paged_q4: workspace must be 16-byte aligned");
+    PagedAttn4 a{};
+    a.Q = Q; a.ldq = ldq; a.out = out; a.ldo = ldo;
+    a.H = num_heads; a.KV = num_kv_heads; a.hd = head_dim; a.lens = seq_lens; a.rope_pos = r.cos_t ? rope_pos : nullptr;
+    TRY(paged4_view(pages, page_table, table_stride, num_seqs, &a.kv));
+    a.rope = r;
+    a.scale = 1.0f / sqrtf((float)head_dim);
+    Scratch sc(S(stream));
+    unsigned char* own = nullptr;
+    if (!workspace) TRY(sc.get(&own, need));
+    return launch_paged4_attention(a, workspace ? workspace : own, S(stream));
+}
+
+JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, int num_kv_heads, int head_dim,
+                                  const int* page_table, int table_stride, int num_seqs, const int* new_table,
+                                  int new_stride, int* new_lens, int* kept, const jyc_kv_pages_q4* pages,
+                                  void* stream) {
+    clear_error();
+    TRY(check_paged4("kv_evict_paged_q4", num_kv_heads, head_dim, page_table, table_stride, num_seqs, pages));
+    if (budget <= 0 || recent < 0 || recent > budget) return arg_error("kv_evict_paged_q4: need 0 <= recent <= budget, budget > 0");
+    if (!pages->mass) return arg_error("kv_evict_paged_q4: the pages have no mass");
+    if (new_stride < 0 || (long long)new_stride * pages->page_size < budget || (long long)new_stride * pages->page_size > 0x7fffff00LL)
+        return arg_error("kv_evict_paged_q4: new_stride * page_size must hold the budget, below 2^31 - 255");
+    if ((long long)num_seqs * num_kv_heads > kMaxItems / budget)
+        return arg_error("kv_evict_paged_q4: num_seqs * num_kv_heads * budget above 2^31 - 1");
+    if (num_seqs == 0) return JYC_OK;
+    if (!seq_lens || !new_table || !new_lens || !kept) return arg_error("kv_evict_paged_q4: null pointer");
+    if (seq_lens == new_lens) return arg_error("kv_evict_paged_q4: new_lens must be another array than seq_lens");
+    PagedEvict4 e{};
+    e.lens = seq_lens; e.budget = budget; e.recent = recent; e.KV = num_kv_heads; e.hd = head_dim;
+    TRY(paged4_view(pages, page_table, table_stride, num_seqs, &e.kv));
+    e.new_table = new_table; e.new_stride = new_stride; e.new_lens = new_lens; e.kept = kept;
+    return launch_paged4_evict(e, S(stream));
 }
 
 }  // extern "C"

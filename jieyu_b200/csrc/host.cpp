@@ -160,6 +160,48 @@ JYC_API int jyc_rope_table(int max_seq, int head_dim, float theta, float* cos_ou
     return JYC_OK;
 }
 
+JYC_API int jyc_rope_table_scaled(int max_seq, int rot_dim, float theta, const jyc_rope_scaling* scaling,
+                                  float* cos_out, float* sin_out) {
+    if (max_seq <= 0 || rot_dim <= 0 || (rot_dim & 1) || !(theta > 0.0f) || !cos_out || !sin_out)
+        return arg_error("jyc_rope_table_scaled: bad arguments");
+    const int half = rot_dim / 2;
+    const double pi = 3.14159265358979323846, r = rot_dim;
+    const jyc_rope_scaling s = scaling ? *scaling : jyc_rope_scaling{JYC_ROPE_NONE, 1.0f, 0, 0.0f, 0.0f, 0.0f};
+    const double factor = s.factor, L = s.original_len;
+    if (s.kind < JYC_ROPE_NONE || s.kind > JYC_ROPE_RAMP) return arg_error("jyc_rope_table_scaled: unknown scaling");
+    if (s.kind != JYC_ROPE_NONE && !(factor >= 1.0 && factor < 1e30))
+        return arg_error("jyc_rope_table_scaled: factor must be at least 1");
+    if (s.kind == JYC_ROPE_NTK && rot_dim == 2) return arg_error("jyc_rope_table_scaled: NTK scaling needs rot_dim > 2");
+    if (s.kind >= JYC_ROPE_BANDS && !(s.original_len > 0 && s.low > 0.0f && s.low < s.high && s.high < 1e30f))
+        return arg_error("jyc_rope_table_scaled: need original_len > 0 and 0 < low < high");
+    if (s.kind == JYC_ROPE_RAMP && !(theta > 1.0f && s.attention >= 0.0f && s.attention < 1e30f))
+        return arg_error("jyc_rope_table_scaled: need theta > 1 and attention >= 0");
+    double gain = 1.0, base = theta;
+    if (s.kind == JYC_ROPE_NTK) base = theta * std::pow(factor, r / (r - 2.0));
+    double from = 0.0, to = 1.0;  // pairs between which the ramp falls
+    if (s.kind == JYC_ROPE_RAMP) {
+        const auto pair = [&](double turns) { return r * std::log(L / (2.0 * pi * turns)) / (2.0 * std::log((double)theta)); };
+        const auto held = [&](double j) { return j < 0.0 ? 0.0 : j > r - 1.0 ? r - 1.0 : j; };
+        from = held(std::floor(pair(s.high)));
+        to = held(std::ceil(pair(s.low)));
+        if (to <= from) to = from + 0.001;
+        gain = s.attention > 0.0f ? (double)s.attention : 0.1 * std::log(factor) + 1.0;
+    }
+    for (int j = 0; j < half; j++) {
+        double f = std::pow(base, -2.0 * j / r), t = 1.0;
+        if (s.kind == JYC_ROPE_LINEAR) t = 0.0;
+        if (s.kind == JYC_ROPE_BANDS) t = (L * f / (2.0 * pi) - s.low) / ((double)s.high - s.low);
+        if (s.kind == JYC_ROPE_RAMP) t = 1.0 - (j - from) / (to - from);
+        t = t < 0.0 ? 0.0 : t > 1.0 ? 1.0 : t;
+        if (s.kind != JYC_ROPE_NONE && s.kind != JYC_ROPE_NTK) f = (1.0 - t) * f / factor + t * f;
+        for (int i = 0; i < max_seq; i++) {
+            cos_out[(size_t)i * half + j] = (float)(gain * std::cos(i * f));
+            sin_out[(size_t)i * half + j] = (float)(gain * std::sin(i * f));
+        }
+    }
+    return JYC_OK;
+}
+
 JYC_API int jyc_synth_f32(uint64_t seed, uint64_t stream, float std_dev, float* out, size_t n) {
     if (!out && n) return arg_error("jyc_synth_f32: null output");
     const uint64_t base = stream_base(seed, stream);
