@@ -3,6 +3,7 @@
 // back as fp32, and attended over by one new token per sequence (the score,
 // softmax and P.V of attention_q8.h:38-184).
 #include "paged.cuh"
+#include "paged_line.cuh"
 #include "ptx.cuh"
 
 #include <cuda.h>
@@ -323,68 +324,6 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(float* K, float
 // key (8 us), the spread of the warps' ends and the joins (8), the second
 // kernel (4).
 
-constexpr float kPaShift = 13.0f;    // the largest weight is in 2^13 .. 2^14
-constexpr float kPaLow = -1.7e38f;  // reference before any key: below every score, and its differences stay finite
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// c = v + a b for a constant v, and c += a b
-__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int v, int (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(v));
-}
-__device__ __forceinline__ void pa_mma_s8(const uint32_t (&a)[4], const uint32_t (&b)[2], int (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[2], float v, float (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(v));
-}
-__device__ __forceinline__ void pa_mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[2], float (&c)[4]) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-// 8 x 8 halves, lane (g, t) holding (g, 2 t) and (g, 2 t + 1), transposed
-__device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-// The cache is read once a step: its lines leave L2 first, so that code, queries and parts stay there
-// (measured: without the hint a kernel's end runs at DRAM latency, instruction by instruction).
-// Scales of neighbouring heads may share a sector, which other SMs want too: no hint.
-__device__ __forceinline__ void pa_copy_scale(uint32_t dst, const float* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void pa_copy(uint32_t dst, const void* src, uint64_t policy) {
-    if (N == 16)
-        asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
-                     : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global.L2::cache_hint [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "l"(policy)
-                     : "memory");
-}
 // bytes 0, 2 (ODD: 1, 3) of x = q ^ 0x80 as the halves q: 0x6400 | u is 1024 + u
 template <bool ODD>
 __device__ __forceinline__ uint32_t pa_half2(uint32_t x) {
@@ -392,16 +331,30 @@ __device__ __forceinline__ uint32_t pa_half2(uint32_t x) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t pa_pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
+    int len = a.lens[b];
+    if (len <= 0) return 0;
+    const int cap = a.kv.table_stride * a.kv.p.page_size;
+    if (len > cap) {
+        paged_flag(kPagedErrPos);
+        len = cap;
+    }
+    if (a.rope.cos_t && len > a.rope.len) {
+        paged_flag(kPagedErrRope);
+        len = 0;
+    }
+    return len;
 }
 
 // Sizes of one instantiation: HDP is the head size rounded up (the columns
 // behind it hold whatever the ring held, finite as integers; they meet zero
 // query columns and unread output columns), HEADS the query heads of a unit.
-template <int HDP, int HEADS, bool TMA>
+template <int HDP_, int HEADS, bool TMA>
 struct PaCfg {
+    using Args = PagedAttn;
+    static __device__ __forceinline__ int len(const PagedAttn& a, int b) { return pa_len(a, b); }
+    static constexpr bool STAT = false;
+    static constexpr int HDP = HDP_;
     static constexpr int TK = HDP <= 128 ? 32 : 16;        // keys of a unit
     // one CTA per SM. Above 64 dims few warps with more units in flight each and room for every accumulator in
     // registers beat more warps with fewer: 131072 keys of 8 x 128, 4 heads each, take 78 us with 12 warps of 2
@@ -432,90 +385,6 @@ struct PaCfg {
 struct PaMaps {
     CUtensorMap k, v;
 };
-struct PaPlan {
-    int units_row;  // kv heads * query blocks
-    int qblocks;    // blocks of ROWS query heads per kv head
-    int tk;         // keys of a unit
-    bool wide_copy; // 16-byte copies
-    bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
-    int box;        // keys of a tensor copy
-};
-// The line cut into runs: worker w starts at w * base + min(w, rest).
-struct PaLine {
-    long long base, rest, workers;
-    int per_cta;  // workers of a CTA
-    __device__ __forceinline__ long long start(long long w) const {
-        w = min(w, workers);
-        return w * base + min(w, rest);
-    }
-    __device__ __forceinline__ int worker(long long u) const {  // whose run holds unit u
-        const long long big = rest * (base + 1);
-        if (u >> 32) return (int)(u < big ? u / (base + 1) : rest + (u - big) / base);
-        return (int)(u < big ? (unsigned)u / (unsigned)(base + 1) : (unsigned)rest + (unsigned)(u - big) / (unsigned)base);
-    }
-};
-// Item that starts in a CTA and ends in a later one.
-struct PaTail {
-    int ctas;  // CTAs after the first that hold parts of it; 0: no such item
-    int slot;  // its first part
-    int b, r;
-    int per_cta;
-};
-struct PaWork {
-    PaTail* tail;      // [CTAs]
-    float* part;       // [workers][2][PART]: an item's later part (0), its first (1)
-};
-
-__device__ __forceinline__ int pa_len(const PagedAttn& a, int b) {
-    int len = a.lens[b];
-    if (len <= 0) return 0;
-    const int cap = a.kv.table_stride * a.kv.p.page_size;
-    if (len > cap) {
-        paged_flag(kPagedErrPos);
-        len = cap;
-    }
-    if (a.rope.cos_t && len > a.rope.len) {
-        paged_flag(kPagedErrRope);
-        len = 0;
-    }
-    return len;
-}
-// Runs of U units: as many workers as there are warps, or units; a few per CTA
-// at least, whose parts are joined in shared memory.
-constexpr int kPaFewWarps = 4;
-__device__ __forceinline__ PaLine pa_line(long long U, int ctas, int warps) {
-    PaLine l;
-    const long long each = U >> 31 ? warps : ((unsigned)U + ctas - 1) / (unsigned)ctas;
-    l.per_cta = (int)min((long long)warps, max((long long)kPaFewWarps, each));
-    l.workers = min((long long)ctas * l.per_cta, U);
-    l.base = l.rest = 0;
-    if (U >> 32) {
-        l.base = U / l.workers;
-        l.rest = U % l.workers;
-    } else if (l.workers) {
-        l.base = (unsigned)U / (unsigned)l.workers;
-        l.rest = (unsigned)U % (unsigned)l.workers;
-    }
-    return l;
-}
-
-struct PaCursor {
-    int b, r, t, nt, len;  // sequence, row of units, unit and units in it, length
-};
-__device__ __forceinline__ void pa_seek(const PagedAttn& a, int tk, PaCursor& c) {
-    c.len = 0;
-    while (c.b < a.kv.num_seqs && (c.len = pa_len(a, c.b)) == 0) c.b++;
-    c.nt = (c.len + tk - 1) / tk;
-}
-__device__ __forceinline__ void pa_next(const PagedAttn& a, const PaPlan& pl, PaCursor& c, int step) {
-    if ((c.t += step) < c.nt) return;
-    c.t = 0;
-    if (++c.r < pl.units_row) return;
-    c.r = 0;
-    c.b++;
-    pa_seek(a, pl.tk, c);
-}
-
 // A wait that did not end at once: gives up after 2^31 SM cycles (about a
 // second) and sets the error word; the warp's run then ends with that unit.
 __device__ __noinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity) {
@@ -540,81 +409,6 @@ __device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* 
         : "memory");
 }
 
-// One warp's sum of parts for RB query rows: every load of a part is in flight
-// at once. Lane i holds dims 4 i .. 4 i + 3 of every 128, and (ref, l) of row i % RB.
-template <int HDP, int HEADS, bool TMA>
-struct PaSum {
-    using G = PaCfg<HDP, HEADS, TMA>;
-    static constexpr int RB = HDP <= 128 && HEADS >= 8 ? 8 : 4, NV = (HDP + 127) / 128;
-    float4 o[RB][NV];
-    float ref, l;
-    // parts i = first, first + step, ... < np at work slots slot(i), rows r0 .. r0 + rows - 1
-    template <class F>
-    __device__ __forceinline__ void add(const float* part, int r0, int rows, int np, int first, int step, F slot) {
-        const int lane = threadIdx.x & 31;
-        ref = kPaLow;
-        l = 0.0f;
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int d = 0; d < NV; d++) o[r][d] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int i = first; i < np; i += step) {
-            const float* p = part + (size_t)slot(i) * G::PART;
-            const float2 rl = *reinterpret_cast<const float2*>(p + G::ROWS * HDP + 2 * (r0 + (lane & (RB - 1))));
-            float4 x[RB][NV];
-#pragma unroll
-            for (int r = 0; r < RB; r++)
-#pragma unroll
-                for (int d = 0; d < NV; d++)
-                    x[r][d] = r < rows && 128 * d + 4 * lane < HDP
-                                  ? *reinterpret_cast<const float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float nr = fmaxf(ref, rl.x), fa = ex2(ref - nr), fb = ex2(rl.x - nr);
-            l = __fmaf_rn(l, fa, rl.y * fb);
-            ref = nr;
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const float ga = __shfl_sync(0xffffffffu, fa, r), gb = __shfl_sync(0xffffffffu, fb, r);
-#pragma unroll
-                for (int d = 0; d < NV; d++) {
-                    o[r][d].x = __fmaf_rn(o[r][d].x, ga, x[r][d].x * gb);
-                    o[r][d].y = __fmaf_rn(o[r][d].y, ga, x[r][d].y * gb);
-                    o[r][d].z = __fmaf_rn(o[r][d].z, ga, x[r][d].z * gb);
-                    o[r][d].w = __fmaf_rn(o[r][d].w, ga, x[r][d].w * gb);
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void store(float* p, int r0, int rows) const {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int d = 0; d < NV; d++)
-                if (r < rows && 128 * d + 4 * lane < HDP)
-                    *reinterpret_cast<float4*>(p + (r0 + r) * HDP + 128 * d + 4 * lane) = o[r][d];
-        if (lane < rows) *reinterpret_cast<float2*>(p + G::ROWS * HDP + 2 * (r0 + lane)) = make_float2(ref, l);
-    }
-    __device__ __forceinline__ void finish(float* out, int rows, int hd) const {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const float lr = __shfl_sync(0xffffffffu, l, r), inv = lr == 0.0f ? 0.0f : __fdiv_rn(1.0f, lr);
-#pragma unroll
-            for (int d = 0; d < NV; d++) {
-                const int e = 128 * d + 4 * lane;
-                if (r >= rows || e >= hd) continue;
-                float* to = out + (size_t)r * hd + e;
-                to[0] = o[r][d].x * inv;
-                to[1] = o[r][d].y * inv;
-                to[2] = o[r][d].z * inv;
-                to[3] = o[r][d].w * inv;
-            }
-        }
-    }
-};
-
 template <int HDP, int HEADS, bool TMA>
 __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work, const __grid_constant__ PaMaps maps) {
@@ -624,12 +418,10 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     extern __shared__ __align__(128) unsigned char pa_raw[];
     unsigned char* const pa_sm = TMA ? pa_raw + (-smem_u32(pa_raw) & 1023u) : pa_raw;
     __shared__ __align__(8) uint64_t s_bar[WARPS][ST][2];  // K, V
-    __shared__ long long s_scan[WARPS], s_ex[WARPS * 32];
+    __shared__ PaShared<G> sh;
     const uint64_t policy = policy_evict_first();
-    __shared__ PaCursor s_cur[WARPS];
-    __shared__ long long s_first[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int B = a.kv.num_seqs, group = a.H / a.KV, hd = TMA ? HDP : a.hd;
+    const int group = a.H / a.KV, hd = TMA ? HDP : a.hd;
     griddep_launch();
     if (TMA && lane == 0) {
         if (warp == 0) {
@@ -640,88 +432,15 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
         mbar_fence_init();
     }
 
-    // where the units of each sequence lie in the line
-    const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
-    const int bs = min(B, tid * per), be = min(B, bs + per);
-    long long mine = 0;
-    bool none = false;  // one of this CTA's share of sequences has no key
-    for (int b = bs; b < be; b++) {
-        const int len = pa_len(a, b);
-        mine += (len + TK - 1) / TK;
-        none |= len == 0 && b % gridDim.x == blockIdx.x;
-    }
-    mine *= pl.units_row;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    if (__syncthreads_or(none))  // rows of zeros
-        for (int b = blockIdx.x; b < B; b += gridDim.x)
-            if (pa_len(a, b) == 0)
-                for (int e = tid; e < a.H * hd; e += WARPS * 32) a.out[(size_t)b * a.ldo + e] = 0.0f;
-    long long U = 0, ex = incl - mine;
-    for (int w = 0; w < WARPS; w++) {
-        if (w < warp) ex += s_scan[w];
-        U += s_scan[w];
-    }
-    const PaLine line = pa_line(U, gridDim.x, WARPS);
-    const long long w0 = (long long)blockIdx.x * line.per_cta;
-    s_ex[tid] = ex;
-    __syncthreads();
-    {
-        // warp: where its run starts (the last thread's segment that starts at or before it)
-        const long long u = line.start(w0 + warp);
-        if (warp < line.per_cta && u < U) {
-            int lo = 0;
-#pragma unroll
-            for (int i = 1 << (31 - __builtin_clz(WARPS * 32)); i > 0; i >>= 1)
-                if (lo + i < WARPS * 32 && s_ex[lo + i] <= u) lo += i;
-            long long at = s_ex[lo];
-            for (int b = min(B, lo * per); b < B; b++) {
-                const int len = pa_len(a, b), nt = (len + TK - 1) / TK;
-                const long long n = (long long)nt * pl.units_row;
-                if (u < at + n) {
-                    const long long k = u - at;
-                    const int r = k >> 31 ? (int)(k / nt) : (int)k / nt, t0 = (int)(k - (long long)r * nt);
-                    s_cur[warp] = PaCursor{b, r, t0, nt, len};
-                    s_first[warp] = u - t0;  // first unit of the item that the run starts in
-                    break;
-                }
-                at += n;
-            }
-        }
-    }
-    __syncthreads();
-
-    const bool worker = warp < line.per_cta;
-    const long long u0 = line.start(w0 + warp), c0 = line.start(w0), c1 = line.start(w0 + line.per_cta);
-    // every run of the CTA inside one item: its warps take units in turn (neighbours in memory at the same time)
-    // and are joined below. whole: and they are all of it
-    bool joint = false, whole = false;
-    if (c1 > c0) {
-        const long long first = s_first[0], end = first + s_cur[0].nt;
-        joint = c1 <= end;
-        whole = c0 == first && c1 == end;
-    }
-    int count = worker ? (int)(line.start(w0 + warp + 1) - u0) : 0;
-    const int step = joint ? line.per_cta : 1;
+    const PaRun run = pa_start<G>(a, pl, sh, hd);
+    const long long w0 = run.w0, u0 = run.u0;
+    const bool joint = run.joint, alone = run.alone;
+    const int step = run.step;
+    int count = run.count;
+    PaCursor cur = run.cur;
+    long long item0 = run.item0;
     unsigned char* ring = pa_sm + warp * G::RING;
     const uint32_t ring_a = smem_u32(ring);
-    PaCursor cur = PaCursor{0, 0, 0, 0, 0};
-    long long item0 = 0;
-    if (joint) {
-        cur = s_cur[0];
-        cur.t += warp;
-        const int units = (int)(c1 - c0);
-        count = worker && warp < units ? (units - warp + step - 1) / step : 0;
-    } else if (count > 0) {
-        cur = s_cur[warp];
-        item0 = s_first[warp];
-    }
-    const bool alone = whole && c1 - c0 == 1;
     if (tid == 0) work.tail[blockIdx.x].ctas = 0;
 
     // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
@@ -745,7 +464,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
                 ok = true;
             }
-            pa_next(a, pl, nx, step);
+            pa_next<G>(a, pl, nx, step);
         }
         issued++;
     };
@@ -1073,43 +792,15 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
         const bool from_start = item0 >= u0;
         if (joint ? alone : from_start && item_end) {
-            const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int row = qb * ROWS + 8 * e + 2 * t + j;
-                    if (row >= group) continue;
-                    float* out = a.out + (size_t)cur.b * a.ldo + (size_t)(kvh * group + row) * hd;
-                    const float inv = l[e][j] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[e][j]);
-#pragma unroll
-                    for (int d = 0; d < ND; d++)
-                        if (16 * d + 2 * g < hd) {
-                            out[16 * d + 2 * g] = o[d][e][j] * inv;
-                            out[16 * d + 2 * g + 1] = o[d][e][2 + j] * inv;
-                        }
-                }
+            pa_finish<G>(a, pl, work, cur, hd, o, ref, l);
         } else {
             if (joint) break;  // o, ref and l stay in registers
             tail = from_start;
-            float* part = work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int row = 8 * e + 2 * t + j;
-                    if (row >= ROWS) continue;
-#pragma unroll
-                    for (int d = 0; d < ND; d++)
-                        *reinterpret_cast<float2*>(part + row * HDP + 16 * d + 2 * g) =
-                            make_float2(o[d][e][j], o[d][e][2 + j]);
-                    if (g == 0)
-                        *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(ref[e][j], l[e][j]);
-                }
+            pa_store<G>(work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART, true, o, ref, l);
         }
         if (n + 1 < count) {
             item0 += cur.nt;
-            pa_next(a, pl, cur, 1);
+            pa_next<G>(a, pl, cur, 1);
             fresh = true;
         }
     }
@@ -1123,144 +814,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                 phase ^= 1u;
             }
         }
-    // CTAs behind this one that hold parts of an item that ends at unit `end`
-    auto later = [&](long long end) { return (int)(line.worker(end - 1) / line.per_cta) - (int)blockIdx.x; };
-    if (!joint) {
-        // the items that this CTA's runs share: the warp where one starts joins its parts (warp 0 those of the
-        // item that came into the CTA), in place
-        __syncthreads();
-        if (c1 == c0) return;
-        const long long first = s_first[0], end0 = first + s_cur[0].nt;
-        for (int pass = warp == 0 ? 0 : 1; pass < 2; pass++) {
-            const bool head = pass == 0;
-            if (head ? first >= c0 : !tail) continue;
-            const long long end = head ? end0 : item0 + cur.nt;
-            const int own = (int)(w0 + warp) * 2 + (head ? 0 : 1);
-            int np = 1;
-            while (warp + np < line.per_cta && line.start(w0 + warp + np) < end) np++;
-            const PaCursor it = head ? s_cur[0] : cur;
-            const bool ends = !head && end <= c1;
-            if (!head && !ends && lane == 0)
-                work.tail[blockIdx.x] = PaTail{later(end), own, it.b, it.r, line.per_cta};
-            if (np == 1) continue;
-            const int qb = it.r % pl.qblocks, kvh = it.r / pl.qblocks;
-            auto slot_of = [&](int i) { return i == 0 ? own : (int)(w0 + warp + i) * 2; };
-            for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += PaSum<HDP, HEADS, TMA>::RB) {
-                PaSum<HDP, HEADS, TMA> sum;
-                const int rows = min(PaSum<HDP, HEADS, TMA>::RB, group - qb * ROWS - r0);
-                sum.add(work.part, r0, rows, np, 0, 1, slot_of);
-                if (ends)
-                    sum.finish(a.out + (size_t)it.b * a.ldo + (size_t)(kvh * group + qb * ROWS + r0) * hd, rows, hd);
-                else
-                    sum.store(work.part + (size_t)own * G::PART, r0, rows);
-            }
-        }
-        return;
-    }
-    if (alone) return;  // written
-
-    // join the CTA's workers (their rings are free now)
-    float* buf = reinterpret_cast<float*>(ring);
-    if (worker)
-#pragma unroll
-        for (int e = 0; e < E; e++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int row = 8 * e + 2 * t + j;
-                if (row >= ROWS) continue;
-                if (count > 0)
-#pragma unroll
-                    for (int d = 0; d < ND; d++)
-                        *reinterpret_cast<float2*>(buf + row * HDP + 16 * d + 2 * g) =
-                            make_float2(o[d][e][j], o[d][e][2 + j]);
-                if (g == 0)
-                    *reinterpret_cast<float2*>(buf + ROWS * HDP + 2 * row) =
-                        count > 0 ? make_float2(ref[e][j], l[e][j]) : make_float2(kPaLow, 0.0f);
-            }
-    __syncthreads();
-    const PaCursor c = s_cur[0];
-    const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
-    const int own = (int)w0 * 2 + (c0 == s_first[0] ? 1 : 0);
-    float* part = work.part + (size_t)own * G::PART;
-    if (tid == 0 && !whole && c0 == s_first[0])
-        work.tail[blockIdx.x] = PaTail{later(s_first[0] + c.nt), own, c.b, c.r, line.per_cta};
-    for (int i = tid; i < ROWS * HDP / 4; i += WARPS * 32) {
-        const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
-        float M = kPaLow, L = 0.0f;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int w = 0; w < line.per_cta; w++)
-            M = fmaxf(M, reinterpret_cast<const float*>(pa_sm + w * G::RING)[ROWS * HDP + 2 * row]);
-#pragma unroll 1
-        for (int w = 0; w < line.per_cta; w++) {
-            const float* wb = reinterpret_cast<const float*>(pa_sm + w * G::RING);
-            const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
-            if (wl == 0.0f) continue;  // no key (a warp without units left no o)
-            const float f = ex2(wr - M);
-            const float4 x = *reinterpret_cast<const float4*>(wb + row * HDP + d);
-            L = __fmaf_rn(f, wl, L);
-            O = make_float4(__fmaf_rn(f, x.x, O.x), __fmaf_rn(f, x.y, O.y), __fmaf_rn(f, x.z, O.z), __fmaf_rn(f, x.w, O.w));
-        }
-        if (whole) {
-            if (qb * ROWS + row < group && d < hd) {
-                float* out = a.out + (size_t)c.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd + d;
-                const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-                out[0] = O.x * inv;
-                out[1] = O.y * inv;
-                out[2] = O.z * inv;
-                out[3] = O.w * inv;
-            }
-        } else {
-            *reinterpret_cast<float4*>(part + row * HDP + d) = O;
-            if (d == 0) *reinterpret_cast<float2*>(part + ROWS * HDP + 2 * row) = make_float2(M, L);
-        }
-    }
-}
-
-// The items that start in one CTA of the kernel above and end in a later one:
-// a CTA each. Warp w adds parts w, w + 8, ..., then the warps' sums are joined
-// in shared memory.
-constexpr int kPaJoinWarps = 8;
-template <int HDP, int HEADS, bool TMA>
-__global__ void __launch_bounds__(kPaJoinWarps * 32) paged_join_kernel(PagedAttn a, PaPlan pl, PaWork work) {
-    using G = PaCfg<HDP, HEADS, TMA>;
-    using Sum = PaSum<HDP, HEADS, TMA>;
-    constexpr int ROWS = G::ROWS, NV = Sum::NV, RB = Sum::RB;
-    __shared__ __align__(16) float s_o[kPaJoinWarps][RB][HDP];
-    __shared__ float2 s_rl[kPaJoinWarps][RB];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
-    griddep_wait();
-    const PaTail tail = work.tail[blockIdx.x];
-    if (tail.ctas == 0) return;
-    const int np = tail.ctas + 1, qb = tail.r % pl.qblocks, kvh = tail.r / pl.qblocks;
-    auto slot_of = [&](int i) { return i == 0 ? tail.slot : ((int)blockIdx.x + i) * tail.per_cta * 2; };
-    for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += RB) {
-        const int rows = min(RB, group - qb * ROWS - r0);
-        Sum sum;
-        sum.add(work.part, r0, rows, np, warp, kPaJoinWarps, slot_of);
-        if (r0) __syncthreads();  // the last row block's sums are read
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int d = 0; d < NV; d++)
-                if (128 * d + 4 * lane < HDP) *reinterpret_cast<float4*>(&s_o[warp][r][128 * d + 4 * lane]) = sum.o[r][d];
-        if (lane < RB) s_rl[warp][lane] = make_float2(sum.ref, sum.l);
-        __syncthreads();
-        const int used = min(np, kPaJoinWarps);
-        for (int i = tid; i < rows * HDP; i += kPaJoinWarps * 32) {
-            const int r = i / HDP, d = i % HDP;
-            float M = kPaLow, L = 0.0f, O = 0.0f;
-            for (int w = 0; w < used; w++) M = fmaxf(M, s_rl[w][r].x);
-            for (int w = 0; w < used; w++) {
-                const float f = ex2(s_rl[w][r].x - M);
-                L = __fmaf_rn(f, s_rl[w][r].y, L);
-                O = __fmaf_rn(f, s_o[w][r][d], O);
-            }
-            if (d < hd)
-                a.out[(size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + r0 + r) * hd + d] =
-                    L == 0.0f ? 0.0f : __fdiv_rn(O, L);
-        }
-    }
+    pa_end<G>(a, pl, work, sh, run, count, cur, item0, tail, pa_sm, hd, o, ref, l);
 }
 
 // The cache of rows r0, r0 + 1, ... when a row is its own sequence.
@@ -1278,7 +832,7 @@ template <int HDP, int HEADS, bool TMA>
 size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
     const size_t workers = (size_t)ctas * PaCfg<HDP, HEADS, TMA>::WARPS;
     const size_t at = align16(ctas * sizeof(PaTail));
-    if (w) *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + at)};
+    if (w) *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + at), nullptr};
     return at + workers * 2 * PaCfg<HDP, HEADS, TMA>::PART * sizeof(float);
 }
 
@@ -1354,12 +908,11 @@ int pa_launch(const PagedAttn& a, PaPlan pl, int sms, void* work, cudaStream_t s
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<HDP, HEADS, TMA>, a, pl, w));
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<G>, a, pl, w));
     JYC_LAUNCHED();
     return JYC_OK;
 }
 
-bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
 bool aligned8(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t)q) & 7) == 0; }
 
 }  // namespace
