@@ -3,6 +3,7 @@
 // (the scores and softmax of attention_q8, libs/model_libs/attention/attention_q8.h:38-184), which leaves
 // each key's weight on it, and the rows of least weight are left behind.
 #include "paged4.cuh"
+#include "paged_line.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -231,123 +232,608 @@ __device__ __forceinline__ int p4_len(const PagedAttn4& a, int b) {
     return len;
 }
 
-constexpr int kP4MaxGroups = 8;
-// A warp per key, a lane per dim of each group; a CTA per sequence and query head.
-__device__ __forceinline__ float p4_simple_score(const PagedAttn4& a, const float* qv, int page, int slot, int kvh,
-                                                 int lane) {
-    const int groups = (a.hd + 31) / 32;
-    const uint8_t* row = a.kv.p.k + p4_off(a.kv.p, page, slot, kvh);
-    const uint32_t* par = reinterpret_cast<const uint32_t*>(a.kv.p.kp) + p4_poff(a.kv.p, page, slot, kvh);
-    float s = 0.0f;
-    for (int g = 0; g < groups; g++) {
-        const int q = row[16 * g + (lane & 15)] >> (lane & 16 ? 4 : 0) & 15;
-        s += qv[32 * g + lane] * __fmaf_rn(p4_step(par[g]), (float)q, p4_low(par[g]));
-        // 0, or NaN where a parameter of K or V is not finite
-        const uint32_t pv = reinterpret_cast<const uint32_t*>(a.kv.p.vp)[p4_poff(a.kv.p, page, slot, kvh) + g];
-        const float all = p4_step(par[g]) * 0.0f + p4_low(par[g]) * 0.0f + p4_step(pv) * 0.0f + p4_low(pv) * 0.0f;
-        s += all;
-    }
-    return warp_sum(s);
+// Sizes of one instantiation: GP groups (the head size rounded up), HEADS query heads of a unit.
+template <int GP, int HEADS>
+struct P4Cfg {
+    using Args = PagedAttn4;
+    static __device__ __forceinline__ int len(const PagedAttn4& a, int b) { return p4_len(a, b); }
+    static constexpr bool STAT = true;
+    static constexpr int HDP = 32 * GP, TK = 32;
+    static constexpr int WARPS = GP <= 2 ? 16 : GP <= 4 ? 12 : 8;
+    static constexpr int ST = GP <= 6 ? 3 : 2;
+    static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
+    static constexpr int ROWS = HEADS;
+    static constexpr int PITCH = 16 * GP + 16;  // an odd number of 16-byte chunks: 8 rows of an ldmatrix tile in distinct banks
+    static constexpr int VOFF = TK * PITCH, KPOFF = 2 * TK * PITCH, VPOFF = KPOFF + 4 * GP * TK;
+    static constexpr int STAGE = VPOFF + 4 * GP * TK;
+    static constexpr int PART = ROWS * (HDP + 2);  // floats of a partial: o, then (ref, l) per row
+    static constexpr int RING = ST * STAGE, SMEM = WARPS * RING;
+    static_assert(PART * 4 <= RING, "a partial fits the ring");
+};
+// Where the scores (base 2) of unit `t` of row of units `r` of a sequence lie, for the kernel that gathers the weights:
+// [key][ROWS].
+struct P4Scores {
+    float* s;  // nullptr: no weights are gathered
+    long long tiles;
+};
+__device__ __forceinline__ size_t p4_score_at(const P4Scores& sc, const PaPlan& pl, int b, int r, int t, int rows) {
+    return ((size_t)((long long)b * pl.units_row + r) * sc.tiles + t) * 32 * rows;
 }
-__device__ __forceinline__ float p4_simple_query(const PagedAttn4& a, int b, int h, int len, float* s_q) {
-    const int lane = threadIdx.x & 31;
-    __shared__ float s_scale;
-    if (threadIdx.x < 32) {
-        float x[kP4MaxGroups], amax = 0.0f;
-        const float* q = a.Q + (size_t)b * a.ldq + (size_t)h * a.hd;
-        const int pos = a.rope_pos ? a.rope_pos[b] : len - 1;
-        for (int g = 0; g < kP4MaxGroups; g++) {
-            const int d = 32 * g + lane;
-            x[g] = 0.0f;
-            if (d >= a.hd) continue;
-            if (a.rope.cos_t) {
-                const float4 y = turned4(q, d & ~3, a.rope, pos, false);
-                x[g] = (d & 3) == 0 ? y.x : (d & 3) == 1 ? y.y : (d & 3) == 2 ? y.z : y.w;
-            } else {
-                x[g] = q[d];
-            }
-            amax = fmaxf(amax, fabsf(x[g]));
+__device__ __forceinline__ __half2 p4_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t p4_u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+template <int N>
+__device__ __forceinline__ void p4_words(const uint32_t* p, uint32_t (&w)[N]) {  // N even
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * i);
+            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
         }
-        amax = warp_max(amax);
-        for (int g = 0; g < kP4MaxGroups; g++) s_q[32 * g + lane] = (float)q8_round(x[g], q8_inv(amax));
-        if (lane == 0) s_scale = __fmul_rn(q8_scale(amax), a.scale);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p + 2 * i);
+            w[2 * i] = x.x; w[2 * i + 1] = x.y;
+        }
     }
-    __syncthreads();
-    return s_scale;
 }
-__global__ void __launch_bounds__(128) paged4_attention_simple(PagedAttn4 a, float2* stat) {
-    __shared__ float s_q[32 * kP4MaxGroups], s_o[4][32 * kP4MaxGroups], s_m[4], s_l[4];
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, kvh = h / (a.H / a.KV);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = (a.hd + 31) / 32;
-    const int len = p4_len(a, b);
-    float* out = a.out + (size_t)b * a.ldo + (size_t)h * a.hd;
-    if (len == 0) {
-        for (int d = threadIdx.x; d < a.hd; d += 128) out[d] = 0.0f;
-        return;
+__device__ __forceinline__ void p4_copy(uint32_t dst, const void* src, int bytes) {
+    if (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else if (bytes == 8)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int GP, int HEADS>
+__global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
+    paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, int param_copy) {
+    using G = P4Cfg<GP, HEADS>;
+    constexpr int TK = G::TK, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PITCH = G::PITCH;
+    extern __shared__ __align__(128) unsigned char p4_sm[];
+    __shared__ PaShared<G> sh;
+    const uint64_t policy = policy_evict_first();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int group = a.H / a.KV, hd = a.hd, groups = (hd + 31) >> 5;
+    griddep_launch();
+    const PaRun run = pa_start<G>(a, pl, sh, hd);
+    const long long w0 = run.w0, u0 = run.u0;
+    const bool joint = run.joint;
+    const int step = run.step, count = run.count;
+    PaCursor cur = run.cur;
+    long long item0 = run.item0;
+    unsigned char* const ring = p4_sm + warp * G::RING;
+    const uint32_t ring_a = smem_u32(ring);
+    if (tid == 0) work.tail[blockIdx.x].ctas = 0;
+    if (groups < GP)  // K's parameters behind the head's last group: no copy writes them
+        for (int st = 0; st < ST; st++)
+            for (int i = groups; i < GP; i++)
+                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::KPOFF)[GP * lane + i] = 0u;
+
+    // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
+    PaCursor nx = cur;
+    int issued = 0;  // units whose pages are looked up
+    int pg = -1, slot = 0, h = -1;
+    long long hoff = 0, hpoff = 0;  // of kv head h
+    bool ok = false;
+    unsigned counts = 0u;  // whether this lane's key counts, of the unit issued last in bit 0
+    auto lookup = [&] {
+        ok = false;
+        if (issued < count) {
+            const int pos = nx.t * TK + lane, hn = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
+            if (hn != h) {
+                h = hn;
+                hoff = (long long)h * a.kv.p.head_stride;
+                hpoff = (long long)h * a.kv.p.phead_stride;
+            }
+            if (pos < nx.len) {
+                const int idx = a.kv.by_page(pos);
+                slot = pos - idx * a.kv.p.page_size;
+                pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
+                ok = true;
+            }
+            pa_next<G>(a, pl, nx, step);
+        }
+        issued++;
+    };
+    constexpr int LPR = GP <= 2 ? 2 : GP <= 4 ? 4 : 8, RPI = 32 / LPR;  // lanes per row, rows per step
+    const int cc = lane & (LPR - 1), cr = lane / LPR;
+    const uint8_t* const kcol = a.kv.p.k + 16 * cc;
+    const uint8_t* const vcol = a.kv.p.v + 16 * cc;
+    auto issue = [&](int st) {
+        if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
+            p4_flag(a.kv, kPagedErrPage);
+            ok = false;
+        }
+        counts = counts << 1 | (ok ? 1u : 0u);
+        const uint32_t base = ring_a + st * G::STAGE;
+        const unsigned mask = __ballot_sync(0xffffffffu, ok);
+        long long off = 0;
+        if (ok) {
+            off = (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff;
+            const long long po = (long long)pg * a.kv.p.ppage_stride + (long long)slot * a.kv.p.ppos_stride + hpoff;
+            const uint32_t* const kp = reinterpret_cast<const uint32_t*>(a.kv.p.kp) + po;
+            const uint32_t* const vp = reinterpret_cast<const uint32_t*>(a.kv.p.vp) + po;
+            const uint32_t dst = base + G::KPOFF + 4 * GP * lane;
+            for (int i = 0; i < 4 * groups; i += param_copy) {
+                p4_copy(dst + i, reinterpret_cast<const unsigned char*>(kp) + i, param_copy);
+                p4_copy(dst + (G::VPOFF - G::KPOFF) + i, reinterpret_cast<const unsigned char*>(vp) + i, param_copy);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TK / RPI; i++) {
+            const int row = i * RPI + cr;
+            const long long o = __shfl_sync(0xffffffffu, off, row);
+            if (cc < groups && ((mask >> row) & 1)) {
+                const uint32_t dst = base + row * PITCH + 16 * cc;
+                pa_copy<16>(dst, kcol + o, policy);
+                pa_copy<16>(dst + G::VOFF, vcol + o, policy);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    // lane (g, t): query head g (and g + 8) as B fragments, bytes 4 t .. 4 t + 3 of every 16, its sums over groups as
+    // halves; of the results the heads 2 t, 2 t + 1 (and 8 more), for which it keeps the reference, its share of the
+    // sum, the dims 2 g, 2 g + 1 of every 16, and what group g's lowest values add
+    uint32_t qf[GP][E][2], qsum[E][2];
+    float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4], olow[E][2];
+    bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
+    int st = 0;
+    const float up = __fmul_rn(a.scale, 1.44269504088896341f);
+
+    for (int n = 0; n < count; n++) {
+        if (fresh) {
+            // the item's query heads: turned and quantised per head
+            fresh = false;
+            if (n == 0) {
+                lookup();
+#pragma unroll 1
+                for (int i = 0; i < ST - 1; i++) {
+                    issue(i);
+                    lookup();
+                }
+            }
+            const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
+            const int pos = a.rope.cos_t ? (a.rope_pos ? __ldg(a.rope_pos + cur.b) : cur.len - 1) : 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int row = qb * ROWS + 8 * e + (HEADS <= 4 ? g & 3 : g);
+                const bool live = row < group;
+                const float* q = a.Q + (size_t)cur.b * a.ldq + (size_t)(kvh * group + (live ? row : 0)) * hd;
+                float4 x[2 * GP];
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 2 * GP; i++) {
+                    const int d = 16 * i + 4 * t;
+                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (live && d < hd) x[i] = a.rope.cos_t ? turned4(q, d, a.rope, pos, pl.wide_rope) : p4_load4(q + d, pl.wide_q);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * GP; i++)
+                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const float inv = q8_inv(amax), sc = __fmul_rn(q8_scale(amax), up);
+                qsum[e][0] = qsum[e][1] = 0u;
+#pragma unroll
+                for (int i = 0; i < 2 * GP; i++) {
+                    const uint32_t b = (uint32_t)(q8_round(x[i].x, inv) & 255) | (uint32_t)(q8_round(x[i].y, inv) & 255) << 8 |
+                                       (uint32_t)(q8_round(x[i].z, inv) & 255) << 16 | (uint32_t)q8_round(x[i].w, inv) << 24;
+                    qf[i >> 1][e][i & 1] = b;
+                }
+#pragma unroll
+                for (int i = 0; i < GP; i++) {
+                    int sum = __dp4a((int)qf[i][e][1], 0x01010101, __dp4a((int)qf[i][e][0], 0x01010101, 0));
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    // |sum| <= 4064: a multiple of 4 and what is left of it are halves
+                    if (i >> 1 == t) {
+                        const uint32_t hi = __half_as_ushort(__int2half_rn(sum & ~3)), lo = __half_as_ushort(__int2half_rn(sum & 3));
+                        qsum[e][0] |= hi << 16 * (i & 1);
+                        qsum[e][1] |= lo << 16 * (i & 1);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    qsl[e][i] = __shfl_sync(0xffffffffu, sc, 4 * (2 * t + i));
+                    ref[e][i] = kPaLow;
+                    l[e][i] = 0.0f;
+                    olow[e][i] = 0.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
+            }
+        }
+        // the next unit's copies go to the stage that the last iteration read
+        __syncwarp();
+        issue(st == 0 ? ST - 1 : st - 1);
+        lookup();
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        __syncwarp();
+        unsigned char* const sb = ring + st * G::STAGE;
+        const uint32_t base = ring_a + st * G::STAGE;
+
+        // lane j, key j: whether it counts and its parameters are finite; V's steps as halves of 2^(e - 15), e their
+        // largest exponent in the group, and lowest values, both laid out in place by group as the products read them
+        const bool in = (counts >> (ST - 1)) & 1u;
+        bool clean;
+        float bias, fg[GP];
+        {
+            uint32_t kw[GP], vw[GP];
+            p4_words(reinterpret_cast<const uint32_t*>(sb + G::KPOFF) + GP * lane, kw);
+            p4_words(reinterpret_cast<const uint32_t*>(sb + G::VPOFF) + GP * lane, vw);
+            __half2 z = __float2half2_rn(0.0f);
+#pragma unroll
+            for (int i = 0; i < GP; i++) {
+                if (!in || i >= groups) vw[i] = 0u;
+                z = __hfma2(p4_h2(kw[i]), __float2half2_rn(0.0f), z);
+                z = __hfma2(p4_h2(vw[i]), __float2half2_rn(0.0f), z);
+            }
+            bias = __low2float(z) + __high2float(z);  // 0 or NaN
+            clean = __all_sync(0xffffffffu, in && bias == 0.0f);
+            if (!in) bias = -INFINITY;
+            __syncwarp();  // all have read their parameters
+            __half* const to = reinterpret_cast<__half*>(sb + G::VPOFF) + 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
+#pragma unroll
+            for (int i = 0; i < GP; i++) {
+                const uint32_t top = min(__reduce_max_sync(0xffffffffu, vw[i] & 0x7fffu) >> 10, 30u);
+                const uint32_t up15 = top == 30u ? 0x0200u : (30u - top) << 10;  // 2^(15 - top)
+                to[32 * i] = __hmul(__ushort_as_half((unsigned short)vw[i]), __ushort_as_half((unsigned short)up15));
+                to[32 * (GP + i)] = __ushort_as_half((unsigned short)(vw[i] >> 16));
+                fg[i] = __uint_as_float((top + 9u + 127u) << 23);  // 2^(top - 15), and 2^24 for V's numbers as subnormal halves
+            }
+        }
+        __syncwarp();
+
+        // scores of keys 8 i + g and heads 2 t, + 1, in base 2: the lowest values' share as a product of halves, then the
+        // groups' whole-number dots, which start at the bits of 1.5 * 2^23 (|dot| < 2^16), so an exact subtraction makes
+        // them floats
+        float s[4][E][2];
+        {
+            const uint32_t* const kp = reinterpret_cast<const uint32_t*>(sb + G::KPOFF);
+            uint32_t low[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint2 w = make_uint2(0u, 0u);
+                if (2 * t < GP) w = *reinterpret_cast<const uint2*>(kp + GP * (8 * i + g) + 2 * t);
+                low[i] = __byte_perm(w.x, w.y, 0x7632);
+            }
+            float acc[2][E][4];
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const uint32_t lf[4] = {low[2 * m], low[2 * m + 1], low[2 * m], low[2 * m + 1]};
+#pragma unroll
+                for (int e = 0; e < E; e++) pa_mma_f16(lf, qsum[e], 0.0f, acc[m][e]);
+            }
+#pragma unroll
+            for (int i0 = 0; i0 < GP; i0 += 2) {
+                uint32_t w[4][2];
+#pragma unroll
+                for (int i = 0; i < 4; i++) p4_words(kp + GP * (8 * i + g) + i0, w[i]);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    uint32_t r[4];
+                    pa_ldsm(base + lane * PITCH + 16 * (i0 + k), r);
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        const uint32_t kf[4] = {r[2 * m] & 0x0F0F0F0Fu, r[2 * m + 1] & 0x0F0F0F0Fu,
+                                                r[2 * m] >> 4 & 0x0F0F0F0Fu, r[2 * m + 1] >> 4 & 0x0F0F0F0Fu};
+                        const float s0 = p4_step(w[2 * m][k]), s1 = p4_step(w[2 * m + 1][k]);
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            int c[4];
+                            pa_mma_s8(kf, qf[i0 + k][e], 0x4B400000, c);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                acc[m][e][j] = __fmaf_rn(j < 2 ? s0 : s1, __fsub_rn(__int_as_float(c[j]), 12582912.0f), acc[m][e][j]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) s[i][e][j] = __fmul_rn(acc[i >> 1][e][2 * (i & 1) + j], qsl[e][j]);
+        }
+        if (!clean) {  // keys that do not count: -inf, whatever the ring held; NaN where a parameter is not finite
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = __shfl_sync(0xffffffffu, bias, 8 * i + g);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) s[i][e][j] = x == -INFINITY ? -INFINITY : s[i][e][j] + x;
+            }
+        }
+        if (scores.s && (HEADS > 4 || t < 2)) {
+            float* const to = scores.s + p4_score_at(scores, pl, cur.b, cur.r, cur.t, ROWS) + 2 * t;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    *reinterpret_cast<float2*>(to + ROWS * (8 * i + g) + 8 * e) = make_float2(s[i][e][0], s[i][e][1]);
+        }
+        float al[E][2];
+        bool same = true;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = fmaxf(fmaxf(s[0][e][j], s[1][e][j]), fmaxf(s[2][e][j], s[3][e][j]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(ref[e][j], x - kPaShift);
+                al[e][j] = ex2(ref[e][j] - x);
+                same &= ref[e][j] == x;
+                ref[e][j] = x;
+            }
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    l[e][j] *= al[e][j];
+                    olow[e][j] *= al[e][j];
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        o[d][e][j] *= al[e][j];
+                        o[d][e][2 + j] *= al[e][j];
+                    }
+                }
+        }
+        // weights as halves hi + lo, transposed: column g, keys 8 i + 2 t, + 1
+        uint32_t hi[4][E], lo[4][E];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float b0 = ex2(s[i][e][0] - ref[e][0]), b1 = ex2(s[i][e][1] - ref[e][1]);
+                l[e][0] += b0;
+                l[e][1] += b1;
+                const uint32_t ph = pa_pack(b0, b1);
+                const float2 hf = __half22float2(p4_h2(ph));
+                hi[i][e] = pa_transpose(ph);
+                lo[i][e] = pa_transpose(pa_pack(b0 - hf.x, b1 - hf.y));
+            }
+        // the lowest values' share: rows are groups
+        {
+            uint4 lw = make_uint4(0u, 0u, 0u, 0u);
+            if (g < GP) lw = *reinterpret_cast<const uint4*>(sb + G::VPOFF + 64 * (GP + g) + 16 * t);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                float c[4];
+                const uint32_t a0[4] = {lw.x, 0u, lw.y, 0u}, a1[4] = {lw.z, 0u, lw.w, 0u};
+                if (HEADS <= 4) {
+                    const uint32_t b0[2] = {g < 4 ? hi[0][e] : lo[0][e], g < 4 ? hi[1][e] : lo[1][e]};
+                    const uint32_t b1[2] = {g < 4 ? hi[2][e] : lo[2][e], g < 4 ? hi[3][e] : lo[3][e]};
+                    pa_mma_f16(a0, b0, 0.0f, c);
+                    pa_mma_f16(a1, b1, c);
+                } else {
+                    const uint32_t b0[2] = {hi[0][e], hi[1][e]}, b1[2] = {hi[2][e], hi[3][e]};
+                    const uint32_t b2[2] = {lo[0][e], lo[1][e]}, b3[2] = {lo[2][e], lo[3][e]};
+                    pa_mma_f16(a0, b2, 0.0f, c);
+                    pa_mma_f16(a1, b3, c);
+                    pa_mma_f16(a0, b0, c);
+                    pa_mma_f16(a1, b1, c);
+                }
+                olow[e][0] += c[0];
+                olow[e][1] += c[1];
+            }
+        }
+        // P.V, a group at a time: V's numbers as subnormal halves (q * 2^-24, the high ones 16 times that), rows g dims 2 g,
+        // rows g + 8 dims 2 g + 1 of 16; a weight times a step as halves: hi rounded, lo what that left and lo's share.
+        // 4 heads fill 8 columns with their hi and lo halves
+        uint32_t zl[4];
+        if (HEADS <= 4)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                zl[i] = g < 4 ? 0u : hi[i][0] ^ 0x80008000u;
+                lo[i][0] = g < 4 ? 0u : lo[i][0];
+            }
+#pragma unroll
+        for (int i0 = 0; i0 < GP; i0++) {
+            uint32_t r[4];
+            pa_ldsm_t(base + G::VOFF + lane * PITCH + 16 * i0, r);
+            const uint4 sv = *reinterpret_cast<const uint4*>(sb + G::VPOFF + 64 * i0 + 16 * t);
+            const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
+            float c[2][E][4];
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                uint32_t bh[E][2], bl[E][2];
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const __half2 w = p4_h2(sw[2 * m + i]), ph = p4_h2(hi[2 * m + i][e]), pw = p4_h2(lo[2 * m + i][e]);
+                        if (HEADS <= 4) {
+                            bh[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hmul2_rn(p4_h2(zl[2 * m + i]), w))));
+                        } else {
+                            const __half2 x = __hmul2_rn(ph, w);
+                            bh[e][i] = p4_u(x);
+                            bl[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hneg2(x))));
+                        }
+                    }
+                const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t mk = k ? 0x00F000F0u : 0x000F000Fu;
+                    const uint32_t vf[4] = {x0 & mk, y0 & mk, x1 & mk, y1 & mk};
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        if (m == 0)
+                            pa_mma_f16(vf, bh[e], 0.0f, c[k][e]);
+                        else
+                            pa_mma_f16(vf, bh[e], c[k][e]);
+                        if (HEADS > 4) pa_mma_f16(vf, bl[e], c[k][e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[2 * i0 + k][e][j] = __fmaf_rn(c[k][e][j], k ? fg[i0] * 0.0625f : fg[i0], o[2 * i0 + k][e][j]);
+        }
+        if (++st == ST) st = 0;
+
+        const bool item_end = cur.t == cur.nt - 1;
+        if (n + 1 < count && (joint || !item_end)) {
+            cur.t += step;
+            continue;
+        }
+        // the end of an item or of the run
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float x = __shfl_sync(0xffffffffu, olow[e][j], 4 * (d >> 1) + t);
+                    o[d][e][j] += x;
+                    o[d][e][2 + j] += x;
+                }
+        if (HEADS <= 4)  // lanes t and t + 2 hold the sums of hi and lo halves of the same heads
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[d][0][j] += __shfl_xor_sync(0xffffffffu, o[d][0][j], 2);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
+        const bool from_start = item0 >= u0;
+        if (joint ? run.alone : from_start && item_end) {
+            pa_finish<G>(a, pl, work, cur, hd, o, ref, l);
+        } else {
+            if (joint) break;  // o, ref and l stay in registers
+            tail = from_start;
+            pa_store<G>(work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART, true, o, ref, l);
+        }
+        if (n + 1 < count) {
+            item0 += cur.nt;
+            pa_next<G>(a, pl, cur, 1);
+            fresh = true;
+        }
     }
-    const float scale = p4_simple_query(a, b, h, len, s_q);
-    float m = -INFINITY, l = 0.0f, o[kP4MaxGroups] = {};
-    for (int j = warp; j < len; j += 4) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    pa_end<G>(a, pl, work, sh, run, count, cur, item0, tail, p4_sm, hd, o, ref, l);
+}
+
+// The weights of the scores that the kernel above left, added to their keys' mass: a thread per key.
+constexpr int kP4MassThreads = 256;
+template <int ROWS>
+__global__ void __launch_bounds__(kP4MassThreads) paged4_mass_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores) {
+    griddep_wait();
+    const int b = blockIdx.x / a.KV, kvh = blockIdx.x - b * a.KV, group = a.H / a.KV;
+    const int len = p4_len(a, b);
+    const float2* const stat = work.stat + (size_t)b * a.H + (size_t)kvh * group;
+    for (long long j = (long long)blockIdx.y * kP4MassThreads + threadIdx.x; j < len; j += (long long)gridDim.y * kP4MassThreads) {
         int slot;
-        const int page = p4_entry(a.kv, b, j, &slot);
-        if (!p4_valid(a.kv, page)) continue;
-        const float s = __fmul_rn(p4_simple_score(a, s_q, page, slot, kvh, lane), scale);
-        const float nm = m == m && s == s ? fmaxf(m, s) : NAN, f = m == -INFINITY ? 0.0f : __expf(m - nm), p = expf(s - nm);
-        l = l * f + p;
-        const uint8_t* row = a.kv.p.v + p4_off(a.kv.p, page, slot, kvh);
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(a.kv.p.vp) + p4_poff(a.kv.p, page, slot, kvh);
-        for (int g = 0; g < groups; g++) {
-            const int q = row[16 * g + (lane & 15)] >> (lane & 16 ? 4 : 0) & 15;
-            o[g] = o[g] * f + p * __fmaf_rn(p4_step(par[g]), (float)q, p4_low(par[g]));
-        }
-        m = nm;
-    }
-    for (int g = 0; g < kP4MaxGroups; g++) s_o[warp][32 * g + lane] = o[g];
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-    __syncthreads();
-    float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), L = 0.0f;
-    for (int w = 0; w < 4; w++)
-        if (s_m[w] != s_m[w]) M = NAN;
-    for (int w = 0; w < 4; w++)
-        if (!(s_m[w] == -INFINITY)) L += s_l[w] * expf(s_m[w] - M);
-    for (int d = threadIdx.x; d < a.hd; d += 128) {
-        float v = 0.0f;
-        for (int w = 0; w < 4; w++)
-            if (!(s_m[w] == -INFINITY)) v += s_o[w][d] * expf(s_m[w] - M);
-        out[d] = L == 0.0f ? 0.0f : v / L;
-    }
-    if (stat && threadIdx.x == 0) stat[blockIdx.x] = make_float2(M, L);
-}
-__global__ void __launch_bounds__(128) paged4_mass_simple(PagedAttn4 a, const float2* stat, float* sums) {
-    __shared__ float s_q[32 * kP4MaxGroups];
-    const int b = blockIdx.x / a.KV, kvh = blockIdx.x % a.KV, group = a.H / a.KV;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int len = p4_len(a, b);
-    if (len == 0) return;
-    for (int i = 0; i < group; i++) {
-        const int h = kvh * group + i;
-        __syncthreads();
-        const float scale = p4_simple_query(a, b, h, len, s_q);
-        const float2 ml = stat[b * a.H + h];
-        for (int j = warp; j < len; j += 4) {
-            int slot;
-            const int page = p4_entry(a.kv, b, j, &slot);
-            if (!p4_valid(a.kv, page)) continue;
-            const float s = __fmul_rn(p4_simple_score(a, s_q, page, slot, kvh, lane), scale);
-            if (lane == 0) {
-                float* sum = sums + (size_t)blockIdx.x * a.kv.table_stride * a.kv.p.page_size + j;
-                const float w = (i == 0 ? 0.0f : *sum) + expf(s - ml.x) / ml.y;
-                if (i < group - 1)
-                    *sum = w;
-                else
-                    atomicAdd(a.kv.p.mass + p4_moff(a.kv.p, page, slot, kvh), w);
+        const int page = p4_entry(a.kv, b, (int)j, &slot);
+        float sum = 0.0f;
+        for (int qb = 0; qb < pl.qblocks; qb++) {
+            const float* s = scores.s + p4_score_at(scores, pl, b, kvh * pl.qblocks + qb, (int)(j >> 5), ROWS) + (j & 31) * ROWS;
+            float4 x[ROWS / 4];
+#pragma unroll
+            for (int i = 0; i < ROWS / 4; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(s) + i);
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) {
+                if (qb * ROWS + i >= group) break;
+                const float2 ri = __ldcg(stat + qb * ROWS + i);
+                const float4 v = x[i >> 2];
+                const float y = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+                sum += ex2(y - ri.x) * ri.y;
             }
         }
+        if (p4_valid(a.kv, page)) atomicAdd(a.kv.p.mass + p4_moff(a.kv.p, page, slot, kvh), sum);
     }
 }
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+// The workspace of one call: tails, parts, and where weights are gathered stat and scores.
+template <int GP, int HEADS>
+size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* base, PaWork* w, P4Scores* sc) {
+    using G = P4Cfg<GP, HEADS>;
+    const int qblocks = (H / KV + HEADS - 1) / HEADS;
+    const size_t parts = align16(ctas * sizeof(PaTail));
+    const size_t stat = align16(parts + (size_t)ctas * G::WARPS * 2 * G::PART * sizeof(float));
+    if (capacity == 0) {
+        if (w) *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts), nullptr};
+        if (sc) *sc = P4Scores{nullptr, 0};
+        return stat;
+    }
+    const size_t score = align16(stat + (size_t)seqs * H * sizeof(float2));
+    const long long tiles = ((long long)capacity + 31) / 32;
+    if (w)
+        *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts), reinterpret_cast<float2*>(base + stat)};
+    if (sc) *sc = P4Scores{reinterpret_cast<float*>(base + score), tiles};
+    return score + (size_t)seqs * KV * qblocks * tiles * 32 * HEADS * sizeof(float);
+}
+
+// A launch behind the last one, which it waits for by itself.
+template <class... Params, class... Args>
+int p4_follow(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    JYC_LAUNCHED();
+    return JYC_OK;
+}
+
+template <int GP, int HEADS>
+int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
+    using G = P4Cfg<GP, HEADS>;
+    if (int e = max_dynamic_smem(reinterpret_cast<const void*>(paged4_attention_kernel<GP, HEADS>), G::SMEM)) return e;
+    const int capacity = a.kv.table_stride * a.kv.p.page_size, groups = (a.hd + 31) / 32;
+    const long long tiles = ((long long)capacity + G::TK - 1) / G::TK;
+    const long long items = (long long)a.kv.num_seqs * pl.units_row;
+    // no more CTAs than the longest possible lengths have units for
+    const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles;
+    const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
+    pl.tk = G::TK;
+    PaWork w;
+    P4Scores sc;
+    p4_work<GP, HEADS>(sms, a.kv.num_seqs, a.H, a.KV, a.kv.p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc);
+    // a key's parameters by the widest copies that all of them allow
+    const jyc_kv_pages_q4& p = a.kv.p;
+    const uintptr_t at = (uintptr_t)p.kp | (uintptr_t)p.vp | (uintptr_t)(4 * (p.ppage_stride | p.ppos_stride | p.phead_stride));
+    const int copy = groups % 4 == 0 && at % 16 == 0 ? 16 : groups % 2 == 0 && at % 8 == 0 ? 8 : 4;
+    paged4_attention_kernel<GP, HEADS><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, sc, copy);
+    JYC_LAUNCHED();
+    if (tiles > 1)  // else an item is one unit: none is split
+        if (int e = p4_follow(paged_join_kernel<G>, dim3(ctas), kPaJoinWarps * 32, s, a, pl, w)) return e;
+    if (!sc.s || capacity == 0) return JYC_OK;
+    const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
+    const unsigned chunks = (unsigned)std::min({most, (8LL * sms + heads - 1) / heads, 65535LL});
+    return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, s, a, pl, w, sc);
+}
+
+// The instantiation of a shape: groups and query heads per unit rounded up.
+#define P4_CASES(F, ...)                                                                     \
+    do {                                                                                     \
+        const int R = H / KV;                                                                \
+        if (hd <= 64) return R <= 4 ? F<2, 4>(__VA_ARGS__) : R <= 8 ? F<2, 8>(__VA_ARGS__) : F<2, 16>(__VA_ARGS__);  \
+        if (hd <= 128) return R <= 4 ? F<4, 4>(__VA_ARGS__) : R <= 8 ? F<4, 8>(__VA_ARGS__) : F<4, 16>(__VA_ARGS__); \
+        if (hd <= 192) return R <= 4 ? F<6, 4>(__VA_ARGS__) : R <= 8 ? F<6, 8>(__VA_ARGS__) : F<6, 16>(__VA_ARGS__); \
+        return R <= 4 ? F<8, 4>(__VA_ARGS__) : R <= 8 ? F<8, 8>(__VA_ARGS__) : F<8, 16>(__VA_ARGS__);                \
+    } while (0)
 
 // ---------------------------------------------------------------------------
 // Eviction: a CTA finds which rows a kv head of a sequence keeps, then warps
@@ -459,8 +945,6 @@ __global__ void __launch_bounds__(256) paged4_move_kernel(PagedEvict4 e) {
     if (lane == 0) p.mass[p4_moff(p, dp, ds, h)] = p.mass[p4_moff(p, sp, ss, h)];
 }
 
-bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
-
 // The cache of rows r0, r0 + 1, ... when a row is its own sequence.
 PagedKV4 shifted(PagedKV4 kv, const int* row_seq, int r0) {
     if (!row_seq) {
@@ -516,20 +1000,25 @@ int launch_paged4_read(float* K, float* V, int ld, int rows, int KV, int hd, con
     });
 }
 
-size_t paged4_attention_workspace(int seqs, int H, int KV, int, int capacity) {
-    return sm_count() ? 16 + sizeof(float2) * seqs * H + sizeof(float) * (size_t)seqs * KV * capacity : 0;
+template <int GP, int HEADS>
+static size_t p4_workspace(int sms, int seqs, int H, int KV, int capacity) {
+    return p4_work<GP, HEADS>(sms, seqs, H, KV, capacity, nullptr, nullptr, nullptr);
+}
+
+size_t paged4_attention_workspace(int seqs, int H, int KV, int hd, int capacity) {
+    const int sms = sm_count();
+    if (sms == 0) return 0;
+    P4_CASES(p4_workspace, sms, seqs, H, KV, capacity);
 }
 
 int launch_paged4_attention(const PagedAttn4& a, void* work, cudaStream_t s) {
-    float2* stat = a.kv.p.mass ? static_cast<float2*>(work) : nullptr;
-    paged4_attention_simple<<<a.kv.num_seqs * a.H, 128, 0, s>>>(a, stat);
-    JYC_LAUNCHED();
-    if (stat) {
-        paged4_mass_simple<<<a.kv.num_seqs * a.KV, 128, 0, s>>>(
-            a, stat, reinterpret_cast<float*>(stat + (size_t)a.kv.num_seqs * a.H));
-        JYC_LAUNCHED();
-    }
-    return JYC_OK;
+    const int H = a.H, KV = a.KV, hd = a.hd, sms = sm_count();
+    PaPlan pl{};
+    pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
+    pl.units_row = KV * pl.qblocks;
+    pl.wide_q = aligned16(a.Q, a.ldq);
+    pl.wide_rope = pl.wide_q && rope_wide(a.rope);
+    P4_CASES(p4_launch, a, pl, sms, work, s);
 }
 
 int launch_paged4_evict(const PagedEvict4& e, cudaStream_t s) {

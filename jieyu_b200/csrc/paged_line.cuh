@@ -84,6 +84,7 @@ struct PaPlan {
     bool wide_copy; // 16-byte copies
     bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
     int box;        // keys of a tensor copy
+    bool wide_rope; // turned4's wide form
 };
 // The line cut into runs: worker w starts at w * base + min(w, rest).
 struct PaLine {
