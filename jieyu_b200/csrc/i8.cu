@@ -1,7 +1,19 @@
 // i8.cu — C = (A W^T) * (a_scale w_scale) + bias over 8-bit integers with 32-bit sums, and the rows of
 // fp32 activations in 8 bits that go into it (kv_pack_q8's rule over a whole row,
 // libs/model_libs/attention/attention_q8.h:24-35).
+//
+// The products run on tcgen05.mma kind::i8: M = 128 output channels, so that neighbouring lanes of the
+// accumulator are neighbouring columns of C (a warp stores 128 contiguous bytes of a row straight from tensor
+// memory, no pass through shared memory), N = a tile of tokens, K in chunks of 128 bytes brought by tensor copies
+// (TMA) in the 128-byte swizzle that the products read. Copies fill what lies outside of A, W and k with zeros, so edges
+// need no care but at the stores. Whole-number sums are exact, so K may be split in any way with the same result.
 #include "i8.cuh"
+#include "kernels.cuh"
+#include "mega.cuh"
+#include "paged.cuh"
+#include "ptx.cuh"
+#include "tc.cuh"
+#include "tmap.cuh"
 
 #include <algorithm>
 
@@ -29,28 +41,358 @@ __global__ void __launch_bounds__(kQrThreads) quantize_rows_kernel(const float* 
     for (int i = tid; i < k; i += kQrThreads) to[i] = (int8_t)q8_round(__ldg(row + i), inv);
 }
 
+// ---------------------------------------------------------------------------
+constexpr int kErrI8 = 10;     // device error word: a bounded wait gave up
+constexpr int kI8Rows = 128;   // output channels of a tile
+constexpr int kI8Chunk = 128;  // bytes of K of a stage
+constexpr int kI8Threads = 192;  // copies, products, four warps of results
+
+// D[tmem] (+)= A[smem] . B[smem]^T, signed bytes, 32-bit sums
+__device__ __forceinline__ void i8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32-bit sums, signed bytes, both K-major, M = 128
+__device__ __forceinline__ constexpr uint32_t i8_idesc(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kI8Rows >> 4) << 24);
+}
+// box of a map's tensor [row][k] -> shared memory (this CTA's)
+__device__ __forceinline__ void i8_copy(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+// 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void i8_tmem_ld16(uint32_t ta, int* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(ta)
+        : "memory");
+}
+__device__ __forceinline__ void i8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Sum, scales and bias: one rounding each.
-__device__ __forceinline__ float i8_out(int sum, float as, float ws, const float* bias, int j) {
+__device__ __forceinline__ float i8_out(int sum, float as, float ws, bool add, float bias) {
     const float v = __fmul_rn(__int2float_rn(sum), __fmul_rn(as, ws));
-    return bias ? __fadd_rn(v, __ldg(bias + j)) : v;
+    return add ? __fadd_rn(v, bias) : v;
 }
 
-// A warp computes one output channel for up to 8 rows: lanes along k.
-__global__ void __launch_bounds__(256) i8_simple_kernel(I8Gemm g) {
-    const int j = blockIdx.x * 8 + (threadIdx.x >> 5), i0 = blockIdx.y * 8, lane = threadIdx.x & 31;
-    if (j >= g.n) return;
-    int acc[8] = {};
-    for (int k = lane; k < g.k; k += 32) {
-        const int w = g.W[(size_t)j * g.ldw + k];
-        for (int r = 0; r < 8; r++)
-            if (i0 + r < g.m) acc[r] += w * g.A[(size_t)(i0 + r) * g.lda + k];
+struct I8Maps {
+    CUtensorMap w, a;
+};
+
+// Bounded waits of one CTA: after any of them gave up, every later one is skipped.
+struct I8Wait {
+    int* err;
+    volatile int* abort;
+    __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        if (mbar_wait_err(bar, parity, err, kErrI8)) return true;
+        *abort = 1;
+        return false;
     }
-    for (int r = 0; r < 8; r++) {
-        int v = acc[r];
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0 && i0 + r < g.m)
-            g.C[(size_t)(i0 + r) * g.ldc + j] = i8_out(v, __ldg(g.as + i0 + r), __ldg(g.ws + j), g.bias, j);
+};
+
+// Many tiles: one CTA per SM takes every gridDim.x-th tile of 128 channels x BN tokens, tokens first. Two accumulators: a
+// tile's results leave while the next one's products run.
+template <int BN>
+struct I8Big {
+    static constexpr int kStage = kI8Rows * kI8Chunk + BN * kI8Chunk, kStages = 4;
+    static constexpr int kSmem = 1024 + kStages * kStage;
+};
+template <int BN>
+__global__ void __launch_bounds__(kI8Threads, 1) i8_big_kernel(I8Gemm g, const __grid_constant__ I8Maps maps, int* err) {
+    using C = I8Big<BN>;
+    extern __shared__ unsigned char i8_raw[];
+    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], accf[2], acce[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    unsigned char* const sm = i8_raw + (-smem_u32(i8_raw) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tt = (g.m + BN - 1) / BN, tiles = (g.n + kI8Rows - 1) / kI8Rows * tt, nch = (g.k + kI8Chunk - 1) / kI8Chunk;
+    const I8Wait wait{err, &s_abort};
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&accf[b], 1);
+            mbar_init(&acce[b], 128);
+        }
+        s_abort = 0;
+        mbar_fence_init();
     }
+    if (warp == 0) {
+        __syncwarp();
+        tmem_alloc(&s_tmem, 2 * BN);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    griddep_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
+                for (int c = 0; c < nch; c++, it++) {
+                    const int s = it % C::kStages;
+                    if (it >= C::kStages && !(ok = wait(&empty[s], ((it / C::kStages) - 1) & 1))) break;
+                    mbar_expect_tx(&full[s], C::kStage);
+                    i8_copy(sm + s * C::kStage, &maps.w, c * kI8Chunk, tile / tt * kI8Rows, &full[s]);
+                    i8_copy(sm + s * C::kStage + kI8Rows * kI8Chunk, &maps.a, c * kI8Chunk, tile % tt * BN, &full[s]);
+                }
+            // no copy may still be landing when the CTA exits (matters only after an error)
+            for (int j = max(0, it - C::kStages); j < it; j++)
+                mbar_wait_err(&full[j % C::kStages], (j / C::kStages) & 1, err, kErrI8);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int it = 0, i = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, i++) {
+                const int b = i & 1;
+                if (i >= 2 && !(ok = wait(&acce[b], ((i >> 1) - 1) & 1))) break;
+                tc_fence_after();
+                for (int c = 0; c < nch; c++, it++) {
+                    const int s = it % C::kStages;
+                    if (!(ok = wait(&full[s], (it / C::kStages) & 1))) break;
+                    tc_fence_after();
+                    const uint32_t st = smem_u32(sm + s * C::kStage);
+                    const uint64_t w = sw128_desc(st), a = sw128_desc(st + kI8Rows * kI8Chunk);
+#pragma unroll
+                    for (int k = 0; k < kI8Chunk / 32; k++)  // 32 bytes of K, in 16-byte units
+                        i8_mma(tmem + (uint32_t)(BN * b), w + 2 * k, a + 2 * k, i8_idesc(BN), c != 0 || k != 0);
+                    tc_commit(&empty[s]);
+                }
+                if (ok) tc_commit(&accf[b]);
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        int i = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, i++) {
+            const int b = i & 1, j = tile / tt * kI8Rows + 32 * q + lane, t0 = tile % tt * BN;
+            const bool col = j < g.n;
+            const float ws = col ? __ldg(g.ws + j) : 0.0f, bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
+            if (!__all_sync(0xffffffffu, wait(&accf[b], (i >> 1) & 1))) break;
+            tc_fence_after();
+            const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(BN * b);
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                int v[16];
+                i8_tmem_ld16(ta + c, v);
+                const int t = t0 + c + (lane & 15);
+                const float as = t < g.m ? __ldg(g.as + t) : 0.0f;
+                float* to = g.C + (size_t)(t0 + c) * g.ldc + j;
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const float y = i8_out(v[u], __shfl_sync(0xffffffffu, as, u), ws, g.bias != nullptr, bias);
+                    if (col && t0 + c + u < g.m) to[(size_t)u * g.ldc] = y;
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(&acce[b]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
+    }
+}
+
+// Few tiles: a CTA computes one tile over one part of K; the parts of a tile are the CTAs of a cluster, which leave
+// their sums in shared memory and each add up a share of the tokens.
+template <int BN>
+struct I8Few {
+    static constexpr int kStage = kI8Rows * kI8Chunk + BN * kI8Chunk;
+    static constexpr int kStages = 100 * 1024 / kStage > 6 ? 6 : 100 * 1024 / kStage;  // two CTAs per SM
+    static constexpr int kCols = BN < 32 ? 32 : BN;
+    static constexpr int kSmem = 1024 + kStages * kStage;
+    static_assert(BN * kI8Rows * 4 <= kStages * kStage, "the sums fit the stages");
+};
+template <int BN>
+__global__ void __launch_bounds__(kI8Threads) i8_few_kernel(I8Gemm g, const __grid_constant__ I8Maps maps, int* err) {
+    using C = I8Few<BN>;
+    extern __shared__ unsigned char i8_raw[];
+    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], accf;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    unsigned char* const sm = i8_raw + (-smem_u32(i8_raw) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, parts = gridDim.z, z = blockIdx.z;
+    const int chunks = (g.k + kI8Chunk - 1) / kI8Chunk;
+    const int c0 = (int)((long long)chunks * z / parts), nch = (int)((long long)chunks * (z + 1) / parts) - c0;  // > 0
+    const I8Wait wait{err, &s_abort};
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&accf, 1);
+        s_abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == 0) {
+        __syncwarp();
+        tmem_alloc(&s_tmem, C::kCols);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    griddep_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (; it < nch; it++) {
+                const int s = it % C::kStages;
+                if (it >= C::kStages && !wait(&empty[s], ((it / C::kStages) - 1) & 1)) break;
+                mbar_expect_tx(&full[s], C::kStage);
+                i8_copy(sm + s * C::kStage, &maps.w, (c0 + it) * kI8Chunk, blockIdx.x * kI8Rows, &full[s]);
+                i8_copy(sm + s * C::kStage + kI8Rows * kI8Chunk, &maps.a, (c0 + it) * kI8Chunk, blockIdx.y * BN, &full[s]);
+            }
+            for (int j = max(0, it - C::kStages); j < it; j++)
+                mbar_wait_err(&full[j % C::kStages], (j / C::kStages) & 1, err, kErrI8);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int it = 0;
+            for (; it < nch; it++) {
+                const int s = it % C::kStages;
+                if (!wait(&full[s], (it / C::kStages) & 1)) break;
+                tc_fence_after();
+                const uint32_t st = smem_u32(sm + s * C::kStage);
+                const uint64_t w = sw128_desc(st), a = sw128_desc(st + kI8Rows * kI8Chunk);
+#pragma unroll
+                for (int k = 0; k < kI8Chunk / 32; k++) i8_mma(tmem, w + 2 * k, a + 2 * k, i8_idesc(BN), it != 0 || k != 0);
+                tc_commit(&empty[s]);
+            }
+            if (it == nch) tc_commit(&accf);
+        }
+    }
+    int* const sums = reinterpret_cast<int*>(sm);  // [token][channel]; every product that read the stages is done
+    const int q = warp & 3, j = blockIdx.x * kI8Rows + 32 * q + lane, t0 = blockIdx.y * BN;
+    const bool col = j < g.n;
+    float ws = 0.0f, bias = 0.0f;
+    if (warp >= 2) {
+        ws = col ? __ldg(g.ws + j) : 0.0f;
+        bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
+        const bool ok = __all_sync(0xffffffffu, wait(&accf, 0));
+        tc_fence_after();
+        const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16);
+        if (ok)
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                if (t0 + c >= g.m) break;
+                int v[16];
+                i8_tmem_ld16(ta + c, v);
+                if (parts > 1) {
+#pragma unroll
+                    for (int u = 0; u < 16; u++) sums[(c + u) * kI8Rows + 32 * q + lane] = v[u];
+                    continue;
+                }
+                const int t = t0 + c + (lane & 15);
+                const float as = t < g.m ? __ldg(g.as + t) : 0.0f;
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const float y = i8_out(v[u], __shfl_sync(0xffffffffu, as, u), ws, g.bias != nullptr, bias);
+                    if (col && t0 + c + u < g.m) g.C[(size_t)(t0 + c + u) * g.ldc + j] = y;
+                }
+            }
+    }
+    if (parts > 1) {
+        __syncwarp();
+        i8_cluster_sync();
+        if (warp >= 2) {
+            const int live = min(BN, g.m - t0), first = live * z / parts, last = live * (z + 1) / parts;
+            for (int t = first; t < last; t++) {
+                int sum = 0;
+                uint32_t at = smem_u32(sums + t * kI8Rows + 32 * q + lane);
+                for (int p = 0; p < parts; p++) {
+                    uint32_t far;
+                    int v;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(at), "r"(p));
+                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(far) : "memory");
+                    sum += v;
+                }
+                if (col) g.C[(size_t)(t0 + t) * g.ldc + j] = i8_out(sum, __ldg(g.as + t0 + t), ws, g.bias != nullptr, bias);
+            }
+        }
+        __syncwarp();
+        i8_cluster_sync();  // no CTA's memory goes while another one reads it
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, C::kCols);
+    }
+}
+
+// Map of an array [rows][k] of bytes, boxes of 128 bytes of `box` rows.
+int i8_map(CUtensorMap* m, const int8_t* base, int rows, int k, int ld, int box) {
+    void* fn = nullptr;
+    if (int e = tensor_map_encoder(&fn)) return e;
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t boxes[2] = {kI8Chunk, (cuuint32_t)box}, step[2] = {1, 1};
+    const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn)(
+        m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, boxes, step,
+        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return JYC_OK;
+}
+
+template <class Kernel>
+int i8_start(Kernel kernel, const I8Gemm& g, const I8Maps& maps, dim3 grid, int cluster, int smem, cudaStream_t s) {
+    if (int e = max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kI8Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 1;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = cluster;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, kernel, g, maps, device_error_word()));
+    JYC_LAUNCHED();
+    return JYC_OK;
+}
+
+template <int BN>
+int i8_few(const I8Gemm& g, I8Maps maps, int sms, cudaStream_t s) {
+    if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, BN)) return e;
+    const long long tiles = (long long)((g.n + kI8Rows - 1) / kI8Rows) * ((g.m + BN - 1) / BN);
+    const int chunks = (g.k + kI8Chunk - 1) / kI8Chunk;
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= 2 * sms && chunks >= 4 * parts) parts *= 2;
+    return i8_start(i8_few_kernel<BN>, g, maps, dim3((g.n + kI8Rows - 1) / kI8Rows, (g.m + BN - 1) / BN, parts), parts,
+                    I8Few<BN>::kSmem, s);
 }
 
 }  // namespace
@@ -61,19 +403,21 @@ int launch_quantize_rows(const float* x, int ldx, int rows, int k, int8_t* q, in
     return JYC_OK;
 }
 
-int launch_i8_gemm(const I8Gemm& a, cudaStream_t s) {
-    const int most = 8 * 65535;
-    for (int r0 = 0; r0 < a.m; r0 += most) {
-        I8Gemm g = a;
-        g.A += (size_t)r0 * a.lda;
-        g.as += r0;
-        g.C += (size_t)r0 * a.ldc;
-        g.m = std::min(most, a.m - r0);
-        i8_simple_kernel<<<dim3((g.n + 7) / 8, (g.m + 7) / 8), 256, 0, s>>>(g);
-        JYC_LAUNCHED();
-        if (a.m - r0 <= most) break;
+int launch_i8_gemm(const I8Gemm& g, cudaStream_t s) {
+    const int sms = sm_count();
+    if (sms == 0) return cuda_fail(cudaErrorNoDevice, "matmul_i8: device query");
+    I8Maps maps{};
+    if (int e = i8_map(&maps.w, g.W, g.n, g.k, g.ldw, kI8Rows)) return e;
+    constexpr int BN = 256;
+    const long long tiles = (long long)((g.n + kI8Rows - 1) / kI8Rows) * ((g.m + BN - 1) / BN);
+    if (g.m > 128 && tiles * 2 > sms) {
+        if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, BN)) return e;
+        return i8_start(i8_big_kernel<BN>, g, maps, dim3((unsigned)std::min<long long>(tiles, sms)), 1, I8Big<BN>::kSmem, s);
     }
-    return JYC_OK;
+    if (g.m <= 16) return i8_few<16>(g, maps, sms, s);
+    if (g.m <= 32) return i8_few<32>(g, maps, sms, s);
+    if (g.m <= 64) return i8_few<64>(g, maps, sms, s);
+    return i8_few<128>(g, maps, sms, s);
 }
 
 }  // namespace jyc

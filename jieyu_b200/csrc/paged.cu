@@ -5,8 +5,7 @@
 #include "paged.cuh"
 #include "paged_line.cuh"
 #include "ptx.cuh"
-
-#include <cuda.h>
+#include "tmap.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -838,14 +837,8 @@ size_t pa_work_bytes(int ctas, unsigned char* base, PaWork* w) {
 
 // Map of a cache array as [page][slot][kv head][dim], boxes of `box` slots of one head.
 int pa_map(CUtensorMap* m, int8_t* base, const PagedAttn& a, int box) {
-    static std::atomic<void*> entry;
-    void* fn = entry.load(std::memory_order_acquire);
-    if (!fn) {
-        cudaDriverEntryPointQueryResult found;
-        JYC_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
-        if (found != cudaDriverEntryPointSuccess || !fn) return cuda_fail(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
-        entry.store(fn, std::memory_order_release);
-    }
+    void* fn = nullptr;
+    if (int e = tensor_map_encoder(&fn)) return e;
     const jyc_kv_pages& p = a.kv.p;
     const cuuint64_t dims[4] = {(cuuint64_t)a.hd, (cuuint64_t)a.KV, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
     // the stride of a dimension of one entry is not used, but has to be one

@@ -47,7 +47,9 @@ def _inputs(rng, m, n, k):
 SHAPES = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (1, 300, 1000), (2, 7, 31), (3, 129, 4090), (5, 64, 127), (8, 256, 512),
           (9, 130, 333), (16, 1000, 640), (17, 40, 2048), (31, 257, 96), (33, 512, 129), (48, 384, 4090),
           (64, 128, 1024), (65, 255, 257), (100, 500, 300), (127, 129, 130), (128, 256, 128), (129, 1024, 4096),
-          (200, 127, 1000), (256, 256, 384), (257, 513, 700), (300, 2000, 64), (640, 384, 1111), (1000, 136, 272)]
+          (200, 127, 1000), (256, 256, 384), (257, 513, 700), (300, 2000, 64), (640, 384, 1111), (1000, 136, 272),
+          # many tiles: one or several for each SM, ragged in every direction
+          (520, 4160, 130), (1300, 4200, 200), (700, 13001, 64), (129, 19000, 417), (2049, 2500, 900)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
