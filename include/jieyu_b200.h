@@ -500,7 +500,8 @@ JYC_API size_t jyc_attention_paged_q4_workspace(int num_seqs, int num_heads, int
  * last. The pages of new_table are other ones than those of page_table (a
  * sequence that keeps all of its rows may name its old pages, which then stay
  * as they are); afterwards the old pages are free. new_lens is another array
- * than seq_lens. pages->mass must be there. 0 <= recent <= budget, budget > 0.
+ * than seq_lens. pages->mass must be there. 0 <= recent <= budget, budget > 0,
+ * num_seqs * num_kv_heads * budget <= 2^30.
  * A row whose old or new page is out of range is not copied (error word). */
 JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, int num_kv_heads, int head_dim,
                                   const int* page_table, int table_stride, int num_seqs, const int* new_table,

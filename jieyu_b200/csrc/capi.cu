@@ -555,7 +555,7 @@ int check_paged4(const char* what, int num_kv_heads, int head_dim, const int* pa
     return JYC_OK;
 }
 
-// Of one launch's grid: heads of sequences, rows of kept positions.
+// Of one launch's grid: heads of sequences.
 constexpr long long kMaxItems = 0x7fffffffLL;
 
 int paged4_view(const jyc_kv_pages_q4* pages, const int* page_table, int table_stride, int num_seqs, PagedKV4* kv) {
@@ -698,8 +698,8 @@ JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, i
     if (!pages->mass) return arg_error("kv_evict_paged_q4: the pages have no mass");
     if (new_stride < 0 || (long long)new_stride * pages->page_size < budget || (long long)new_stride * pages->page_size > 0x7fffff00LL)
         return arg_error("kv_evict_paged_q4: new_stride * page_size must hold the budget, below 2^31 - 255");
-    if ((long long)num_seqs * num_kv_heads > kMaxItems / budget)
-        return arg_error("kv_evict_paged_q4: num_seqs * num_kv_heads * budget above 2^31 - 1");
+    if ((long long)num_seqs * num_kv_heads > (1LL << 30) / budget)
+        return arg_error("kv_evict_paged_q4: num_seqs * num_kv_heads * budget above 2^30");
     if (num_seqs == 0) return JYC_OK;
     if (!seq_lens || !new_table || !new_lens || !kept) return arg_error("kv_evict_paged_q4: null pointer");
     if (seq_lens == new_lens) return arg_error("kv_evict_paged_q4: new_lens must be another array than seq_lens");

@@ -44,6 +44,8 @@ constexpr int kPagedErrWait = 8;  // a copy's bounded wait gave up
 int* paged_error_word();
 // Clears these bits, and no other that a call sets meanwhile; they are clear on return.
 int paged_error_clear(int bits);
+// Rows of ld floats at p lie on 16 bytes.
+inline bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
 // SMs of the current device (0: no device).
 int sm_count();
 // The kernel's limit of dynamic shared memory on the current device, set once for each.

@@ -836,113 +836,234 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     } while (0)
 
 // ---------------------------------------------------------------------------
-// Eviction: a CTA finds which rows a kv head of a sequence keeps, then warps
-// copy them.
-constexpr int kEvThreads = 1024;
+// Eviction: a cluster finds which rows a kv head of a sequence keeps, then groups
+// of lanes copy them.
+//
+// Select: the border among the masses' order keys (the `want`-th largest) digit by
+// digit, 11, 11 and 10 bits: each CTA counts the digits of its slice of the positions in
+// shared memory, all CTAs of the cluster add up all counts and find the same digit. Then
+// kept positions are counted slice by slice and warp by warp, and written in their order.
+// Keys of slices up to kEvSpan positions stay in shared memory (131072 positions of one
+// sequence: 8 CTAs a head), those of longer ones are read again for each digit. Masses
+// differ little in their first digit, so the counts have kEvCopies copies, a lane's own of 8.
+constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvSpan = 24576;
+constexpr int kEvBins = 2048, kEvCopies = 8, kEvMaxCluster = 8;
+constexpr int kEvSmem = ((kEvCopies + 3) * kEvBins + kEvSpan) * 4;
 
 // larger mass -> larger key; NaN below every number, -0 as 0
 __device__ __forceinline__ uint32_t ev_key(float m) { return f32_order_key(m + 0.0f); }
+__device__ __forceinline__ void ev_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ev_far(const int* p, int rank) {
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
 
-__global__ void __launch_bounds__(kEvThreads) paged4_select_kernel(PagedEvict4 e) {
-    __shared__ int s_hist[256], s_digit, s_above, s_scan[kEvThreads / 32][2];
-    const int b = blockIdx.x / e.KV, h = blockIdx.x % e.KV, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict4 e, int ctas) {
+    extern __shared__ int ev_sm[];
+    int* const copies = ev_sm;                        // [bin][copy]
+    int* const sums = ev_sm + kEvCopies * kEvBins;    // [digit][bin]: this CTA's counts
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(ev_sm + (kEvCopies + 3) * kEvBins);
+    __shared__ int s_warp[kEvWarps], s_digit, s_above, s_count[2], s_more[kEvWarps], s_equal[kEvWarps];
+    griddep_launch();
+    const int rank = blockIdx.x % ctas, item = blockIdx.x / ctas, b = item / e.KV, h = item - b * e.KV;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int len = max(e.lens[b], 0);
     const int cap = e.kv.table_stride * e.kv.p.page_size;
     if (len > cap) {
         p4_flag(e.kv, kPagedErrPos);
         len = cap;
     }
-    int* kept = e.kept + (size_t)blockIdx.x * e.budget;
-    const int n = min(len, e.budget);
-    if (h == 0 && tid == 0) e.new_lens[b] = n;
-    if (len <= e.budget) {
-        for (int i = tid; i < e.budget; i += kEvThreads) kept[i] = i < len ? i : -1;
+    int* kept = e.kept + (size_t)item * e.budget;
+    if (h == 0 && rank == 0 && tid == 0) e.new_lens[b] = min(len, e.budget);
+    if (len <= e.budget) {  // the whole cluster
+        for (int i = rank * kEvThreads + tid; i < e.budget; i += ctas * kEvThreads) kept[i] = i < len ? i : -1;
         return;
     }
     const int old = len - e.recent, want = e.budget - e.recent;  // want < old
-    auto key = [&](int i) {
+    for (int i = rank * kEvThreads + tid; i < e.recent; i += ctas * kEvThreads) kept[want + i] = old + i;
+    if (want == 0) return;  // the whole cluster
+    // this CTA's slice, and this warp's part of it: whole 32s of positions
+    const int slice = (old + ctas - 1) / ctas, from = min(old, rank * slice), size = min(old, from + slice) - from;
+    const int seg = (size + kEvThreads - 1) / kEvThreads * 32, w0 = min(size, warp * seg), w1 = min(size, w0 + seg);
+    const bool cached = size <= kEvSpan;
+    auto fetch = [&](int i) {
         int slot;
-        const int page = p4_entry(e.kv, b, i, &slot);
+        const int page = p4_entry(e.kv, b, from + i, &slot);
         return p4_valid(e.kv, page) ? ev_key(e.kv.p.mass[p4_moff(e.kv.p, page, slot, h)]) : 0u;
     };
-    uint32_t prefix = 0u;
-    int left = want;  // of those that share the prefix, how many are kept
-    if (want > 0)
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kEvThreads) s_hist[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < old; i += kEvThreads) {
-                const uint32_t k = key(i);
-                if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[k >> shift & 255], 1);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int above = 0, d = 255;
-                while (above + s_hist[d] < left) above += s_hist[d--];
-                s_digit = d;
+    if (cached) {
+#pragma unroll 4
+        for (int i = w0 + lane; i < w1; i += 32) keys[i] = fetch(i);
+    }
+    auto key = [&](int i) { return cached ? keys[i] : fetch(i); };
+    uint32_t border = 0u;
+    int left = want;  // of those that share the border's digits, how many are kept
+#pragma unroll 1
+    for (int d = 0; d < 3; d++) {
+        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d < 2 ? 2048 : 1024;
+        for (int i = tid; i < kEvCopies * kEvBins / 4; i += kEvThreads) reinterpret_cast<int4*>(copies)[i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+#pragma unroll 4
+        for (int i = w0 + lane; i < w1; i += 32) {
+            const uint32_t k = key(i);
+            if (d == 0 || (k ^ border) >> (d == 1 ? 21 : 10) == 0)
+                atomicAdd(&copies[(k >> shift & (bins - 1)) * kEvCopies + (lane & (kEvCopies - 1))], 1);
+        }
+        __syncthreads();
+        int mine[2];  // counts of bins 2 tid, 2 tid + 1
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int4* c = reinterpret_cast<const int4*>(copies + (2 * tid + k) * kEvCopies);
+            const int4 x = c[0], y = c[1];
+            mine[k] = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
+            sums[d * kEvBins + 2 * tid + k] = mine[k];
+        }
+        if (ctas > 1) {
+            __syncwarp();
+            ev_cluster_sync();
+            for (int r = 0; r < ctas; r++)
+                if (r != rank)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) mine[k] += ev_far(sums + d * kEvBins + 2 * tid + k, r);
+        }
+        // counts of all bins above this thread's: a suffix sum over the CTA
+        const int both = mine[0] + mine[1];
+        int incl = both;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_down_sync(0xffffffffu, incl, o);
+            if (lane + o < 32) incl += x;
+        }
+        if (lane == 0) s_warp[warp] = incl;
+        __syncthreads();
+        int above = incl - both;
+        for (int w = warp + 1; w < kEvWarps; w++) above += s_warp[w];
+#pragma unroll
+        for (int k = 1; k >= 0; k--) {
+            if (above < left && above + mine[k] >= left) {  // one thread of the CTA
+                s_digit = 2 * tid + k;
                 s_above = above;
             }
-            __syncthreads();
-            prefix |= (uint32_t)s_digit << shift;
-            left -= s_above;
-            __syncthreads();
+            above += mine[k];
         }
-    // positions in order: those above the border, and the first `left` that equal it
-    int base = 0, ties = 0;
-    for (int i0 = 0; i0 < len; i0 += kEvThreads) {
-        const int i = i0 + tid;
-        const uint32_t k = want > 0 && i < old ? key(i) : 0u;
-        const bool tie = want > 0 && i < old && k == prefix, sure = i < len && (i >= old || (want > 0 && k > prefix));
-        const unsigned ties_w = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) s_scan[warp][0] = __popc(ties_w);
         __syncthreads();
-        int before = ties + __popc(ties_w & ((1u << lane) - 1u));
-        for (int w = 0; w < kEvThreads / 32; w++) {
-            if (w < warp) before += s_scan[w][0];
-            ties += s_scan[w][0];
-        }
-        const bool keep = sure || (tie && before < left);
-        const unsigned keep_w = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) s_scan[warp][1] = __popc(keep_w);
-        __syncthreads();
-        int at = base + __popc(keep_w & ((1u << lane) - 1u));
-        for (int w = 0; w < kEvThreads / 32; w++) {
-            if (w < warp) at += s_scan[w][1];
-            base += s_scan[w][1];
-        }
-        if (keep) kept[at] = i;
-        __syncthreads();
+        border |= (uint32_t)s_digit << shift;
+        left -= s_above;
     }
+    // rows above the border and at it: of this warp, of the warps and CTAs before it
+    int more = 0, equal = 0;
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32) {
+        const uint32_t k = key(i);
+        more += k > border;
+        equal += k == border;
+    }
+    more = __reduce_add_sync(0xffffffffu, more);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) {
+        s_more[warp] = more;
+        s_equal[warp] = equal;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int a = __reduce_add_sync(0xffffffffu, s_more[lane]), c = __reduce_add_sync(0xffffffffu, s_equal[lane]);
+        if (lane == 0) {
+            s_count[0] = a;
+            s_count[1] = c;
+        }
+    }
+    int out = __reduce_add_sync(0xffffffffu, lane < warp ? s_more[lane] : 0);
+    int ties = __reduce_add_sync(0xffffffffu, lane < warp ? s_equal[lane] : 0);
+    if (ctas > 1) {
+        __syncwarp();
+        ev_cluster_sync();
+        for (int r = 0; r < rank; r++) {
+            out += ev_far(&s_count[0], r);
+            ties += ev_far(&s_count[1], r);
+        }
+    }
+    // of rows at the border the first `left` in order are kept
+    out += min(ties, left);
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < w1 ? key(i) : 0u;
+        const bool tie = i < w1 && k == border;
+        const unsigned t = __ballot_sync(0xffffffffu, tie), below = (1u << lane) - 1u;
+        const bool keep = tie ? ties + __popc(t & below) < left : i < w1 && k > border;
+        const unsigned m = __ballot_sync(0xffffffffu, keep);
+        if (keep) kept[out + __popc(m & below)] = from + i;
+        ties += __popc(t);
+        out += __popc(m);
+    }
+    __syncwarp();
+    if (ctas > 1) ev_cluster_sync();  // no CTA's memory goes while another one reads it
 }
 
-__global__ void __launch_bounds__(256) paged4_move_kernel(PagedEvict4 e) {
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (w >= (long long)e.kv.num_seqs * e.KV * e.budget) return;
-    const int item = (int)(w / e.budget), to = (int)(w - (long long)item * e.budget), b = item / e.KV, h = item % e.KV;
-    const int from = e.kept[w];
-    if (from < 0) return;
-    int ss, ds;
-    const int sp = p4_entry(e.kv, b, from, &ss);
-    PagedKV4 dst = e.kv;
-    dst.table = e.new_table;
-    dst.table_stride = e.new_stride;
-    const int dp = p4_entry(dst, b, to, &ds);
-    const bool ok = p4_valid(e.kv, sp) && p4_valid(e.kv, dp);
-    if (!ok) return;
+// A row is copied by as many lanes as it has 16-byte chunks (rounded up to a power of two), each with one chunk of K and
+// one of V, the parameters word by word among them; kMvRows rows of a thread in flight.
+constexpr int kMvThreads = 256, kMvRows = 4;
+template <int LANES>
+__global__ void __launch_bounds__(kMvThreads) paged4_move_kernel(PagedEvict4 e, FastDiv by_budget, FastDiv by_kv,
+                                                                 FastDiv by_new_page) {
+    constexpr int SIDE = kMvThreads / LANES;
+    griddep_wait();
+    const int sub = threadIdx.x & (LANES - 1), groups = (e.hd + 31) >> 5, total = e.kv.num_seqs * e.KV * e.budget;
     const jyc_kv_pages_q4& p = e.kv.p;
-    const size_t so = p4_off(p, sp, ss, h), to_ = p4_off(p, dp, ds, h);
-    const size_t sq = p4_poff(p, sp, ss, h), dq = p4_poff(p, dp, ds, h);
-    const int groups = (e.hd + 31) / 32;
-    if (lane < 4 * groups) {
-        reinterpret_cast<uint32_t*>(p.k + to_)[lane] = reinterpret_cast<const uint32_t*>(p.k + so)[lane];
-        reinterpret_cast<uint32_t*>(p.v + to_)[lane] = reinterpret_cast<const uint32_t*>(p.v + so)[lane];
+    const int w0 = blockIdx.x * (SIDE * kMvRows) + threadIdx.x / LANES;
+    int from[kMvRows], b[kMvRows], h[kMvRows], to[kMvRows];
+#pragma unroll
+    for (int i = 0; i < kMvRows; i++) {
+        const int w = w0 + i * SIDE;
+        from[i] = w < total ? __ldcg(e.kept + w) : -1;
+        const int item = by_budget(w);
+        to[i] = w - item * e.budget;
+        b[i] = by_kv(item);
+        h[i] = item - b[i] * e.KV;
     }
-    if (lane < groups) {
-        reinterpret_cast<uint32_t*>(p.kp)[dq + lane] = reinterpret_cast<const uint32_t*>(p.kp)[sq + lane];
-        reinterpret_cast<uint32_t*>(p.vp)[dq + lane] = reinterpret_cast<const uint32_t*>(p.vp)[sq + lane];
+    int sp[kMvRows], ss[kMvRows], dp[kMvRows], ds[kMvRows];
+#pragma unroll
+    for (int i = 0; i < kMvRows; i++) {
+        sp[i] = dp[i] = -1;
+        if (from[i] < 0) continue;
+        sp[i] = p4_entry(e.kv, b[i], from[i], &ss[i]);
+        const int idx = by_new_page(to[i]);
+        ds[i] = to[i] - idx * p.page_size;
+        dp[i] = __ldg(e.new_table + (size_t)b[i] * e.new_stride + idx);
     }
-    if (lane == 0) p.mass[p4_moff(p, dp, ds, h)] = p.mass[p4_moff(p, sp, ss, h)];
+    uint4 k[kMvRows], v[kMvRows];
+    uint32_t kp[kMvRows], vp[kMvRows];
+    float m[kMvRows];
+    bool ok[kMvRows];
+#pragma unroll
+    for (int i = 0; i < kMvRows; i++) {
+        ok[i] = from[i] >= 0 && p4_valid(e.kv, sp[i]);
+        if (from[i] >= 0 && (dp[i] < 0 || dp[i] >= p.num_pages)) {
+            p4_flag(e.kv, kPagedErrPage);
+            ok[i] = false;
+        }
+        if (!ok[i] || sub >= groups) continue;
+        const size_t so = p4_off(p, sp[i], ss[i], h[i]) + 16 * sub, sq = p4_poff(p, sp[i], ss[i], h[i]) + sub;
+        k[i] = *reinterpret_cast<const uint4*>(p.k + so);
+        v[i] = *reinterpret_cast<const uint4*>(p.v + so);
+        kp[i] = reinterpret_cast<const uint32_t*>(p.kp)[sq];
+        vp[i] = reinterpret_cast<const uint32_t*>(p.vp)[sq];
+        if (sub == 0) m[i] = p.mass[p4_moff(p, sp[i], ss[i], h[i])];
+    }
+#pragma unroll
+    for (int i = 0; i < kMvRows; i++) {
+        if (!ok[i] || sub >= groups) continue;
+        const size_t to_ = p4_off(p, dp[i], ds[i], h[i]) + 16 * sub, dq = p4_poff(p, dp[i], ds[i], h[i]) + sub;
+        *reinterpret_cast<uint4*>(p.k + to_) = k[i];
+        *reinterpret_cast<uint4*>(p.v + to_) = v[i];
+        reinterpret_cast<uint32_t*>(p.kp)[dq] = kp[i];
+        reinterpret_cast<uint32_t*>(p.vp)[dq] = vp[i];
+        if (sub == 0) p.mass[p4_moff(p, dp[i], ds[i], h[i])] = m[i];
+    }
 }
 
 // The cache of rows r0, r0 + 1, ... when a row is its own sequence.
@@ -1022,12 +1143,30 @@ int launch_paged4_attention(const PagedAttn4& a, void* work, cudaStream_t s) {
 }
 
 int launch_paged4_evict(const PagedEvict4& e, cudaStream_t s) {
-    paged4_select_kernel<<<e.kv.num_seqs * e.KV, kEvThreads, 0, s>>>(e);
+    if (int r = max_dynamic_smem(reinterpret_cast<const void*>(paged4_select_kernel), kEvSmem)) return r;
+    const int items = e.kv.num_seqs * e.KV, sms = sm_count();
+    const long long capacity = (long long)e.kv.table_stride * e.kv.p.page_size;
+    // CTAs of a head: while the SMs hold them all and each has a few thousand positions
+    int ctas = 1;
+    while (ctas < kEvMaxCluster && (long long)items * ctas * 2 <= sms && capacity >= 4096LL * ctas) ctas *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)items * ctas);
+    cfg.blockDim = dim3(kEvThreads);
+    cfg.dynamicSmemBytes = kEvSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    JYC_CUDA(cudaLaunchKernelEx(&cfg, paged4_select_kernel, e, ctas));
     JYC_LAUNCHED();
-    const long long warps = (long long)e.kv.num_seqs * e.KV * e.budget;
-    paged4_move_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(e);
-    JYC_LAUNCHED();
-    return JYC_OK;
+    const int groups = (e.hd + 31) / 32, lanes = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
+    const long long rows = (long long)items * e.budget, per = (long long)kMvThreads / lanes * kMvRows;
+    const auto kernel = lanes == 1 ? paged4_move_kernel<1> : lanes == 2 ? paged4_move_kernel<2> : lanes == 4 ? paged4_move_kernel<4> : paged4_move_kernel<8>;
+    return p4_follow(kernel, dim3((unsigned)((rows + per - 1) / per)), kMvThreads, s, e, fast_div(e.budget), fast_div(e.KV),
+                     e.kv.by_page);
 }
 
 }  // namespace jyc

@@ -521,8 +521,6 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32)
     }
 }
 
-inline bool aligned16(const void* p, int ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
-
 }  // namespace
 
 }  // namespace jyc
