@@ -384,30 +384,6 @@ struct PaCfg {
 struct PaMaps {
     CUtensorMap k, v;
 };
-// A wait that did not end at once: gives up after 2^31 SM cycles (about a
-// second) and sets the error word; the warp's run then ends with that unit.
-__device__ __noinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-        if (clock64() - t0 > (1LL << 31)) {
-            paged_flag(kPagedErrWait);
-            return false;
-        }
-    return true;
-}
-__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) {
-    return mbar_try_wait(bar, parity) || pa_wait_slow(bar, parity);
-}
-// box of a map's tensor [page][slot][kv head][dim] -> shared memory (this CTA's)
-__device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* map, int h, int slot, int page,
-                                               uint64_t* bar, uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-        "l"(map), "r"(0), "r"(h), "r"(slot), "r"(page), "r"(smem_u32(bar)), "l"(policy)
-        : "memory");
-}
-
 template <int HDP, int HEADS, bool TMA>
 __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     paged_attention_kernel(PagedAttn a, PaPlan pl, PaWork work, const __grid_constant__ PaMaps maps) {
@@ -623,7 +599,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
             const float* sc = reinterpret_cast<const float*>(ring + G::KOFF + st * 8 * TK);
             kscale = sc[lane];
             vscale = in ? sc[TK + lane] : 0.0f;
-            if (!pa_wait(&s_bar[warp][st][0], phase)) gave_up = true;
+            if (!pa_wait(&s_bar[warp][st][0], phase, &g_paged_err)) gave_up = true;
         } else {
             // the next unit's copies go to the stage that the last iteration read
             __syncwarp();
@@ -724,7 +700,7 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
                     if (HEADS > 4) lo[m][e][i] = pa_transpose(pl2);
                 }
         if constexpr (TMA)
-            if (!pa_wait(&s_bar[warp][st][1], phase)) gave_up = true;
+            if (!pa_wait(&s_bar[warp][st][1], phase, &g_paged_err)) gave_up = true;
         // P.V: a transposed load gives lane (g, t) dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: the even dims are
         // rows g of the tile, the odd ones rows g + 8
 #pragma unroll
@@ -806,8 +782,8 @@ __global__ void __launch_bounds__(PaCfg<HDP, HEADS, TMA>::WARPS * 32, 1)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (TMA && gave_up)  // the copies that are still on their way write to this CTA's memory
         for (int i = 0; i < ST; i++) {
-            pa_wait(&s_bar[warp][st][0], phase);
-            pa_wait(&s_bar[warp][st][1], phase);
+            pa_wait(&s_bar[warp][st][0], phase, &g_paged_err);
+            pa_wait(&s_bar[warp][st][1], phase, &g_paged_err);
             if (++st == ST) {
                 st = 0;
                 phase ^= 1u;

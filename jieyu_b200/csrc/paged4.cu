@@ -5,6 +5,7 @@
 #include "paged4.cuh"
 #include "paged_line.cuh"
 #include "ptx.cuh"
+#include "tmap.cuh"
 
 #include <algorithm>
 #include <climits>
@@ -232,8 +233,8 @@ __device__ __forceinline__ int p4_len(const PagedAttn4& a, int b) {
     return len;
 }
 
-// Sizes of one instantiation: GP groups (the head size rounded up), HEADS query heads of a unit.
-template <int GP, int HEADS>
+// Sizes of one instantiation: GP groups (the head size rounded up), HEADS query heads of a unit, rows by tensor copies.
+template <int GP, int HEADS, bool TMA>
 struct P4Cfg {
     using Args = PagedAttn4;
     static __device__ __forceinline__ int len(const PagedAttn4& a, int b) { return p4_len(a, b); }
@@ -243,12 +244,25 @@ struct P4Cfg {
     static constexpr int ST = GP <= 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
     static constexpr int ROWS = HEADS;
-    static constexpr int PITCH = 16 * GP + 16;  // an odd number of 16-byte chunks: 8 rows of an ldmatrix tile in distinct banks
-    static constexpr int VOFF = TK * PITCH, KPOFF = 2 * TK * PITCH, VPOFF = KPOFF + 4 * GP * TK;
-    static constexpr int STAGE = VPOFF + 4 * GP * TK;
+    // rows of K and V: tensor copies swizzle their 16-byte chunks, else an odd number of chunks, so that the 8 rows of an
+    // ldmatrix tile lie in distinct banks
+    static constexpr int PITCH = 16 * GP + (TMA ? 0 : 16);
+    static constexpr int PW = GP <= 4 ? 4 : 8;  // words of a key's parameters: whole 16 bytes
+    static constexpr int VOFF = TK * PITCH, KPOFF = 2 * TK * PITCH, VPOFF = KPOFF + 4 * PW * TK;
+    static constexpr int STAGE = VPOFF + 4 * PW * TK;
     static constexpr int PART = ROWS * (HDP + 2);  // floats of a partial: o, then (ref, l) per row
-    static constexpr int RING = ST * STAGE, SMEM = WARPS * RING;
+    static constexpr int SOFF = ST * STAGE;        // V's steps of the current unit
+    static constexpr int RING = TMA ? (SOFF + 64 * GP + 1023) / 1024 * 1024 : SOFF + 64 * GP;
+    static constexpr int SMEM = WARPS * RING + (TMA ? 1024 : 0);
     static_assert(PART * 4 <= RING, "a partial fits the ring");
+    static_assert(!TMA || GP == 2 || GP == 4, "rows of 32 or 64 bytes");
+    // byte of 16-byte chunk c of row r
+    static __device__ __forceinline__ int at(int r, int c) {
+        return r * PITCH + 16 * (!TMA ? c : GP == 4 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1));
+    }
+};
+struct P4Maps {
+    CUtensorMap k, v;
 };
 // Where the scores (base 2) of unit `t` of row of units `r` of a sequence lie, for the kernel that gathers the weights:
 // [key][ROWS].
@@ -277,39 +291,54 @@ __device__ __forceinline__ void p4_words(const uint32_t* p, uint32_t (&w)[N]) { 
         }
     }
 }
-__device__ __forceinline__ void p4_copy(uint32_t dst, const void* src, int bytes) {
-    if (bytes == 16)
+// Parameters of neighbouring heads may share a sector, which other SMs want too: no hint.
+template <int N>
+__device__ __forceinline__ void p4_copy(uint32_t dst, const void* src) {
+    if (N == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else if (bytes == 8)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 
-template <int GP, int HEADS>
-__global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
-    paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, int param_copy) {
-    using G = P4Cfg<GP, HEADS>;
-    constexpr int TK = G::TK, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PITCH = G::PITCH;
-    extern __shared__ __align__(128) unsigned char p4_sm[];
+template <int GP, int HEADS, bool TMA>
+__global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
+    paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, int param_copy,
+                            const __grid_constant__ P4Maps maps) {
+    using G = P4Cfg<GP, HEADS, TMA>;
+    constexpr int TK = G::TK, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PW = G::PW, LW = PW / 4;
+    extern __shared__ __align__(128) unsigned char p4_raw[];
+    unsigned char* const p4_sm = TMA ? p4_raw + (-smem_u32(p4_raw) & 1023u) : p4_raw;
+    __shared__ __align__(8) uint64_t s_bar[G::WARPS][ST];
     __shared__ PaShared<G> sh;
     const uint64_t policy = policy_evict_first();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int group = a.H / a.KV, hd = a.hd, groups = (hd + 31) >> 5;
+    const int group = a.H / a.KV, hd = a.hd, groups = TMA ? GP : (hd + 31) >> 5;
     griddep_launch();
+    unsigned char* const ring = p4_sm + warp * G::RING;
+    const uint32_t ring_a = smem_u32(ring);
+    if (TMA && lane == 0) {
+        if (warp == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+        }
+        for (int i = 0; i < ST; i++) mbar_init(&s_bar[warp][i], 1);
+        mbar_fence_init();
+    }
+    // parameters behind the head's last group: no copy writes them
+    if (groups < PW)
+        for (int st = 0; st < ST; st++)
+            for (int i = groups; i < PW; i++) {
+                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::KPOFF)[PW * lane + i] = 0u;
+                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::VPOFF)[PW * lane + i] = 0u;
+            }
     const PaRun run = pa_start<G>(a, pl, sh, hd);
     const long long w0 = run.w0, u0 = run.u0;
     const bool joint = run.joint;
-    const int step = run.step, count = run.count;
+    const int step = run.step;
+    int count = run.count;
     PaCursor cur = run.cur;
     long long item0 = run.item0;
-    unsigned char* const ring = p4_sm + warp * G::RING;
-    const uint32_t ring_a = smem_u32(ring);
     if (tid == 0) work.tail[blockIdx.x].ctas = 0;
-    if (groups < GP)  // K's parameters behind the head's last group: no copy writes them
-        for (int st = 0; st < ST; st++)
-            for (int i = groups; i < GP; i++)
-                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::KPOFF)[GP * lane + i] = 0u;
 
     // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
     PaCursor nx = cur;
@@ -324,7 +353,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
             const int pos = nx.t * TK + lane, hn = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
             if (hn != h) {
                 h = hn;
-                hoff = (long long)h * a.kv.p.head_stride;
+                if (!TMA) hoff = (long long)h * a.kv.p.head_stride;
                 hpoff = (long long)h * a.kv.p.phead_stride;
             }
             if (pos < nx.len) {
@@ -339,8 +368,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
     };
     constexpr int LPR = GP <= 2 ? 2 : GP <= 4 ? 4 : 8, RPI = 32 / LPR;  // lanes per row, rows per step
     const int cc = lane & (LPR - 1), cr = lane / LPR;
-    const uint8_t* const kcol = a.kv.p.k + 16 * cc;
-    const uint8_t* const vcol = a.kv.p.v + 16 * cc;
+    // the unit that was looked up last: rows, and by lane j key j's parameters
     auto issue = [&](int st) {
         if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
             p4_flag(a.kv, kPagedErrPage);
@@ -348,27 +376,50 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
         }
         counts = counts << 1 | (ok ? 1u : 0u);
         const uint32_t base = ring_a + st * G::STAGE;
-        const unsigned mask = __ballot_sync(0xffffffffu, ok);
-        long long off = 0;
         if (ok) {
-            off = (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff;
             const long long po = (long long)pg * a.kv.p.ppage_stride + (long long)slot * a.kv.p.ppos_stride + hpoff;
             const uint32_t* const kp = reinterpret_cast<const uint32_t*>(a.kv.p.kp) + po;
             const uint32_t* const vp = reinterpret_cast<const uint32_t*>(a.kv.p.vp) + po;
-            const uint32_t dst = base + G::KPOFF + 4 * GP * lane;
-            for (int i = 0; i < 4 * groups; i += param_copy) {
-                p4_copy(dst + i, reinterpret_cast<const unsigned char*>(kp) + i, param_copy);
-                p4_copy(dst + (G::VPOFF - G::KPOFF) + i, reinterpret_cast<const unsigned char*>(vp) + i, param_copy);
+            const uint32_t dst = base + G::KPOFF + 4 * PW * lane;
+            if (param_copy == 4 * GP && 4 * GP <= 16) {
+                p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst, kp);
+                p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst + (G::VPOFF - G::KPOFF), vp);
+            } else if (GP == 8 && param_copy == 32) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    p4_copy<16>(dst + 4 * i, kp + i);
+                    p4_copy<16>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
+                }
+            } else {
+                for (int i = 0; i < groups; i++) {
+                    p4_copy<4>(dst + 4 * i, kp + i);
+                    p4_copy<4>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
+                }
             }
         }
+        if constexpr (TMA) {
+            uint64_t* bar = &s_bar[warp][st];
+            const bool lead = ok && (lane & (pl.box - 1)) == 0;
+            const unsigned bytes = __popc(__ballot_sync(0xffffffffu, lead)) * pl.box * 32 * GP;
+            if (lane == 0) mbar_expect_tx(bar, bytes);
+            __syncwarp();
+            if (lead) {
+                pa_tensor_copy(base + lane * G::PITCH, &maps.k, h, slot, pg, bar, policy);
+                pa_tensor_copy(base + G::VOFF + lane * G::PITCH, &maps.v, h, slot, pg, bar, policy);
+            }
+        } else {
+            const unsigned mask = __ballot_sync(0xffffffffu, ok);
+            const long long off =
+                ok ? (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff : 0LL;
 #pragma unroll
-        for (int i = 0; i < TK / RPI; i++) {
-            const int row = i * RPI + cr;
-            const long long o = __shfl_sync(0xffffffffu, off, row);
-            if (cc < groups && ((mask >> row) & 1)) {
-                const uint32_t dst = base + row * PITCH + 16 * cc;
-                pa_copy<16>(dst, kcol + o, policy);
-                pa_copy<16>(dst + G::VOFF, vcol + o, policy);
+            for (int i = 0; i < TK / RPI; i++) {
+                const int row = i * RPI + cr;
+                const long long o = __shfl_sync(0xffffffffu, off, row) + 16 * cc;
+                if (cc < groups && ((mask >> row) & 1)) {
+                    const uint32_t dst = base + row * G::PITCH + 16 * cc;
+                    pa_copy<16>(dst, a.kv.p.k + o, policy);
+                    pa_copy<16>(dst + G::VOFF, a.kv.p.v + o, policy);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -376,11 +427,16 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
 
     // lane (g, t): query head g (and g + 8) as B fragments, bytes 4 t .. 4 t + 3 of every 16, its sums over groups as
     // halves; of the results the heads 2 t, 2 t + 1 (and 8 more), for which it keeps the reference, its share of the
-    // sum, the dims 2 g, 2 g + 1 of every 16, and what group g's lowest values add
-    uint32_t qf[GP][E][2], qsum[E][2];
-    float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4], olow[E][2];
+    // sum, the dims 2 g, 2 g + 1 of every 16 in units of 2^(eg - 15 + 24) of their group (the high 16 of a group 16 times
+    // that), and the products with column g (and g + 8) of V's parameters: (step, low) of each group
+    uint32_t qf[GP][E][2], qsum[E][2 * LW];
+    float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4], opar[E][2 * LW];
+    int eg[GP];        // exponent field of V's largest step of each group so far
+    uint32_t ug[GP];   // 2^(15 - eg) and 1 as halves
     bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
+    bool gave_up = false;
     int st = 0;
+    uint32_t phase = 0u;
     const float up = __fmul_rn(a.scale, 1.44269504088896341f);
 
     for (int n = 0; n < count; n++) {
@@ -390,13 +446,18 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
             if (n == 0) {
                 lookup();
 #pragma unroll 1
-                for (int i = 0; i < ST - 1; i++) {
+                for (int i = 0; i < (TMA ? ST : ST - 1); i++) {
                     issue(i);
                     lookup();
                 }
             }
             const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
             const int pos = a.rope.cos_t ? (a.rope_pos ? __ldg(a.rope_pos + cur.b) : cur.len - 1) : 0;
+#pragma unroll
+            for (int i = 0; i < GP; i++) {
+                eg[i] = 0;
+                ug[i] = 0x3C007800u;
+            }
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const int row = qb * ROWS + 8 * e + (HEADS <= 4 ? g & 3 : g);
@@ -416,7 +477,6 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const float inv = q8_inv(amax), sc = __fmul_rn(q8_scale(amax), up);
-                qsum[e][0] = qsum[e][1] = 0u;
 #pragma unroll
                 for (int i = 0; i < 2 * GP; i++) {
                     const uint32_t b = (uint32_t)(q8_round(x[i].x, inv) & 255) | (uint32_t)(q8_round(x[i].y, inv) & 255) << 8 |
@@ -424,15 +484,18 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                     qf[i >> 1][e][i & 1] = b;
                 }
 #pragma unroll
+                for (int i = 0; i < 2 * LW; i++) qsum[e][i] = 0u;
+#pragma unroll
                 for (int i = 0; i < GP; i++) {
                     int sum = __dp4a((int)qf[i][e][1], 0x01010101, __dp4a((int)qf[i][e][0], 0x01010101, 0));
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    // |sum| <= 4064: a multiple of 4 and what is left of it are halves
-                    if (i >> 1 == t) {
-                        const uint32_t hi = __half_as_ushort(__int2half_rn(sum & ~3)), lo = __half_as_ushort(__int2half_rn(sum & 3));
-                        qsum[e][0] |= hi << 16 * (i & 1);
-                        qsum[e][1] |= lo << 16 * (i & 1);
+                    // |sum| <= 4064 as a multiple of 4 beyond it and what that has too much, of the other sign: both are
+                    // halves, and a lowest value that is not finite gives NaN
+                    const int hi = sum >= 0 ? (sum & ~3) + 4 : -((-sum & ~3) + 4);
+                    if ((i & 3) == t) {
+                        qsum[e][i >> 2] = (uint32_t)__half_as_ushort(__int2half_rn(hi)) << 16;
+                        qsum[e][LW + (i >> 2)] = (uint32_t)__half_as_ushort(__int2half_rn(sum - hi)) << 16;
                     }
                 }
 #pragma unroll
@@ -440,82 +503,93 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                     qsl[e][i] = __shfl_sync(0xffffffffu, sc, 4 * (2 * t + i));
                     ref[e][i] = kPaLow;
                     l[e][i] = 0.0f;
-                    olow[e][i] = 0.0f;
                 }
+#pragma unroll
+                for (int i = 0; i < 2 * LW; i++) opar[e][i] = 0.0f;
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d][e][0] = o[d][e][1] = o[d][e][2] = o[d][e][3] = 0.0f;
             }
         }
-        // the next unit's copies go to the stage that the last iteration read
-        __syncwarp();
-        issue(st == 0 ? ST - 1 : st - 1);
-        lookup();
+        if constexpr (!TMA) {
+            // the next unit's copies go to the stage that the last iteration read
+            __syncwarp();
+            issue(st == 0 ? ST - 1 : st - 1);
+            lookup();
+        }
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
         __syncwarp();
+        if constexpr (TMA)
+            if (!pa_wait(&s_bar[warp][st], phase, a.kv.err)) gave_up = true;
         unsigned char* const sb = ring + st * G::STAGE;
         const uint32_t base = ring_a + st * G::STAGE;
+        const unsigned in = __ballot_sync(0xffffffffu, (counts >> (ST - 1)) & 1u);  // keys that count
 
-        // lane j, key j: whether it counts and its parameters are finite; V's steps as halves of 2^(e - 15), e their
-        // largest exponent in the group, and lowest values, both laid out in place by group as the products read them
-        const bool in = (counts >> (ST - 1)) & 1u;
-        bool clean;
-        float bias, fg[GP];
+        // lane j, key j: V's steps in units of their group's largest, laid out by group as the products read them
         {
-            uint32_t kw[GP], vw[GP];
-            p4_words(reinterpret_cast<const uint32_t*>(sb + G::KPOFF) + GP * lane, kw);
-            p4_words(reinterpret_cast<const uint32_t*>(sb + G::VPOFF) + GP * lane, vw);
-            __half2 z = __float2half2_rn(0.0f);
+            uint32_t vw[PW];
+            uint32_t* const vrow = reinterpret_cast<uint32_t*>(sb + G::VPOFF) + PW * lane;
+            if (in != ~0u && !(in >> lane & 1))  // whatever the ring held
 #pragma unroll
-            for (int i = 0; i < GP; i++) {
-                if (!in || i >= groups) vw[i] = 0u;
-                z = __hfma2(p4_h2(kw[i]), __float2half2_rn(0.0f), z);
-                z = __hfma2(p4_h2(vw[i]), __float2half2_rn(0.0f), z);
-            }
-            bias = __low2float(z) + __high2float(z);  // 0 or NaN
-            clean = __all_sync(0xffffffffu, in && bias == 0.0f);
-            if (!in) bias = -INFINITY;
-            __syncwarp();  // all have read their parameters
-            __half* const to = reinterpret_cast<__half*>(sb + G::VPOFF) + 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
+                for (int i = 0; i < PW; i++) vrow[i] = 0u;
+            p4_words(vrow, vw);
+            __half2 top = __hmul2_rn(p4_h2(vw[0]), p4_h2(ug[0]));
 #pragma unroll
-            for (int i = 0; i < GP; i++) {
-                const uint32_t top = min(__reduce_max_sync(0xffffffffu, vw[i] & 0x7fffu) >> 10, 30u);
-                const uint32_t up15 = top == 30u ? 0x0200u : (30u - top) << 10;  // 2^(15 - top)
-                to[32 * i] = __hmul(__ushort_as_half((unsigned short)vw[i]), __ushort_as_half((unsigned short)up15));
-                to[32 * (GP + i)] = __ushort_as_half((unsigned short)(vw[i] >> 16));
-                fg[i] = __uint_as_float((top + 9u + 127u) << 23);  // 2^(top - 15), and 2^24 for V's numbers as subnormal halves
+            for (int i = 1; i < GP; i++) top = __hmax2_nan(top, __hmul2_rn(p4_h2(vw[i]), p4_h2(ug[i])));
+            if (__any_sync(0xffffffffu, !(__low2float(top) < 2.0f))) {  // a larger step than before
+#pragma unroll
+                for (int i = 0; i < GP; i++) {
+                    const int e1 = max(eg[i], (int)min(__reduce_max_sync(0xffffffffu, vw[i] & 0x7fffu) >> 10, 30u));
+                    const float f = __uint_as_float((uint32_t)(127 + eg[i] - e1) << 23);
+                    eg[i] = e1;
+                    ug[i] = 0x3C000000u | (e1 == 30 ? 0x0200u : (uint32_t)(30 - e1) << 10);
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            o[2 * i][e][j] *= f;
+                            o[2 * i + 1][e][j] *= f;
+                        }
+                }
             }
+            __half* const to = reinterpret_cast<__half*>(ring + G::SOFF) + 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
+#pragma unroll
+            for (int i = 0; i < GP; i++) to[32 * i] = __low2half(__hmul2_rn(p4_h2(vw[i]), p4_h2(ug[i])));
         }
         __syncwarp();
 
-        // scores of keys 8 i + g and heads 2 t, + 1, in base 2: the lowest values' share as a product of halves, then the
-        // groups' whole-number dots, which start at the bits of 1.5 * 2^23 (|dot| < 2^16), so an exact subtraction makes
-        // them floats
+        // scores of keys 8 i + g and heads 2 t, + 1, in base 2: the parameters' products with (0, query sum) of each group,
+        // then the groups' whole-number dots, which start at the bits of 1.5 * 2^23 (|dot| < 2^16), so an exact subtraction
+        // makes them floats
         float s[4][E][2];
         {
             const uint32_t* const kp = reinterpret_cast<const uint32_t*>(sb + G::KPOFF);
-            uint32_t low[4];
+            uint32_t par[LW][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint2 w = make_uint2(0u, 0u);
-                if (2 * t < GP) w = *reinterpret_cast<const uint2*>(kp + GP * (8 * i + g) + 2 * t);
-                low[i] = __byte_perm(w.x, w.y, 0x7632);
-            }
+            for (int i = 0; i < LW; i++) pa_ldsm(base + G::KPOFF + 4 * PW * lane + 16 * i, par[i]);
             float acc[2][E][4];
 #pragma unroll
-            for (int m = 0; m < 2; m++) {
-                const uint32_t lf[4] = {low[2 * m], low[2 * m + 1], low[2 * m], low[2 * m + 1]};
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int e = 0; e < E; e++) pa_mma_f16(lf, qsum[e], 0.0f, acc[m][e]);
-            }
+                for (int e = 0; e < E; e++) {
+                    if constexpr (LW == 1) {
+                        const uint32_t pf[4] = {par[0][2 * m], par[0][2 * m + 1], par[0][2 * m], par[0][2 * m + 1]};
+                        pa_mma_f16(pf, qsum[e], 0.0f, acc[m][e]);
+                    } else {
+                        const uint32_t pf[4] = {par[0][2 * m], par[0][2 * m + 1], par[1][2 * m], par[1][2 * m + 1]};
+                        const uint32_t q0[2] = {qsum[e][0], qsum[e][1]}, q1[2] = {qsum[e][2], qsum[e][3]};
+                        pa_mma_f16(pf, q0, 0.0f, acc[m][e]);
+                        pa_mma_f16(pf, q1, acc[m][e]);
+                    }
+                }
 #pragma unroll
             for (int i0 = 0; i0 < GP; i0 += 2) {
                 uint32_t w[4][2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) p4_words(kp + GP * (8 * i + g) + i0, w[i]);
+                for (int i = 0; i < 4; i++) p4_words(kp + PW * (8 * i + g) + i0, w[i]);
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     uint32_t r[4];
-                    pa_ldsm(base + lane * PITCH + 16 * (i0 + k), r);
+                    pa_ldsm(base + G::at(lane, i0 + k), r);
 #pragma unroll
                     for (int m = 0; m < 2; m++) {
                         const uint32_t kf[4] = {r[2 * m] & 0x0F0F0F0Fu, r[2 * m + 1] & 0x0F0F0F0Fu,
@@ -539,15 +613,13 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
 #pragma unroll
                     for (int j = 0; j < 2; j++) s[i][e][j] = __fmul_rn(acc[i >> 1][e][2 * (i & 1) + j], qsl[e][j]);
         }
-        if (!clean) {  // keys that do not count: -inf, whatever the ring held; NaN where a parameter is not finite
+        if (in != ~0u) {  // keys that do not count: -inf, whatever the ring held
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = __shfl_sync(0xffffffffu, bias, 8 * i + g);
+            for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) s[i][e][j] = x == -INFINITY ? -INFINITY : s[i][e][j] + x;
-            }
+                    for (int j = 0; j < 2; j++) s[i][e][j] = in >> (8 * i + g) & 1 ? s[i][e][j] : -INFINITY;
         }
         if (scores.s && (HEADS > 4 || t < 2)) {
             float* const to = scores.s + p4_score_at(scores, pl, cur.b, cur.r, cur.t, ROWS) + 2 * t;
@@ -557,7 +629,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                 for (int e = 0; e < E; e++)
                     *reinterpret_cast<float2*>(to + ROWS * (8 * i + g) + 8 * e) = make_float2(s[i][e][0], s[i][e][1]);
         }
-        float al[E][2];
+        float old[E][2];
         bool same = true;
 #pragma unroll
         for (int e = 0; e < E; e++)
@@ -568,7 +640,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 x = fmaxf(ref[e][j], x - kPaShift);
-                al[e][j] = ex2(ref[e][j] - x);
+                old[e][j] = ref[e][j];
                 same &= ref[e][j] == x;
                 ref[e][j] = x;
             }
@@ -577,12 +649,14 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
             for (int e = 0; e < E; e++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    l[e][j] *= al[e][j];
-                    olow[e][j] *= al[e][j];
+                    const float al = ex2(old[e][j] - ref[e][j]);
+                    l[e][j] *= al;
+#pragma unroll
+                    for (int i = 0; i < LW; i++) opar[e][2 * i + j] *= al;
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
-                        o[d][e][j] *= al[e][j];
-                        o[d][e][2 + j] *= al[e][j];
+                        o[d][e][j] *= al;
+                        o[d][e][2 + j] *= al;
                     }
                 }
         }
@@ -600,29 +674,36 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
                 hi[i][e] = pa_transpose(ph);
                 lo[i][e] = pa_transpose(pa_pack(b0 - hf.x, b1 - hf.y));
             }
-        // the lowest values' share: rows are groups
+        // the parameters' share: rows are their columns
         {
-            uint4 lw = make_uint4(0u, 0u, 0u, 0u);
-            if (g < GP) lw = *reinterpret_cast<const uint4*>(sb + G::VPOFF + 64 * (GP + g) + 16 * t);
+            uint32_t par[LW][4];
+#pragma unroll
+            for (int i = 0; i < LW; i++) pa_ldsm_t(base + G::VPOFF + 4 * PW * lane + 16 * i, par[i]);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 float c[4];
-                const uint32_t a0[4] = {lw.x, 0u, lw.y, 0u}, a1[4] = {lw.z, 0u, lw.w, 0u};
-                if (HEADS <= 4) {
-                    const uint32_t b0[2] = {g < 4 ? hi[0][e] : lo[0][e], g < 4 ? hi[1][e] : lo[1][e]};
-                    const uint32_t b1[2] = {g < 4 ? hi[2][e] : lo[2][e], g < 4 ? hi[3][e] : lo[3][e]};
-                    pa_mma_f16(a0, b0, 0.0f, c);
-                    pa_mma_f16(a1, b1, c);
-                } else {
-                    const uint32_t b0[2] = {hi[0][e], hi[1][e]}, b1[2] = {hi[2][e], hi[3][e]};
-                    const uint32_t b2[2] = {lo[0][e], lo[1][e]}, b3[2] = {lo[2][e], lo[3][e]};
-                    pa_mma_f16(a0, b2, 0.0f, c);
-                    pa_mma_f16(a1, b3, c);
-                    pa_mma_f16(a0, b0, c);
-                    pa_mma_f16(a1, b1, c);
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    const uint32_t pf[4] = {par[0][2 * m], LW > 1 ? par[LW - 1][2 * m] : 0u, par[0][2 * m + 1],
+                                            LW > 1 ? par[LW - 1][2 * m + 1] : 0u};
+                    const uint32_t h0 = hi[2 * m][e], h1 = hi[2 * m + 1][e], l0 = lo[2 * m][e], l1 = lo[2 * m + 1][e];
+                    if (HEADS <= 4) {
+                        const uint32_t b[2] = {g < 4 ? h0 : l0, g < 4 ? h1 : l1};
+                        if (m == 0)
+                            pa_mma_f16(pf, b, 0.0f, c);
+                        else
+                            pa_mma_f16(pf, b, c);
+                    } else {
+                        const uint32_t bl[2] = {l0, l1}, bh[2] = {h0, h1};
+                        if (m == 0)
+                            pa_mma_f16(pf, bl, 0.0f, c);
+                        else
+                            pa_mma_f16(pf, bl, c);
+                        pa_mma_f16(pf, bh, c);
+                    }
                 }
-                olow[e][0] += c[0];
-                olow[e][1] += c[1];
+#pragma unroll
+                for (int i = 0; i < 2 * LW; i++) opar[e][i] += c[i];
             }
         }
         // P.V, a group at a time: V's numbers as subnormal halves (q * 2^-24, the high ones 16 times that), rows g dims 2 g,
@@ -638,8 +719,8 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
 #pragma unroll
         for (int i0 = 0; i0 < GP; i0++) {
             uint32_t r[4];
-            pa_ldsm_t(base + G::VOFF + lane * PITCH + 16 * i0, r);
-            const uint4 sv = *reinterpret_cast<const uint4*>(sb + G::VPOFF + 64 * i0 + 16 * t);
+            pa_ldsm_t(base + G::VOFF + G::at(lane, i0), r);
+            const uint4 sv = *reinterpret_cast<const uint4*>(ring + G::SOFF + 64 * i0 + 16 * t);
             const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
             float c[2][E][4];
 #pragma unroll
@@ -678,38 +759,61 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        o[2 * i0 + k][e][j] = __fmaf_rn(c[k][e][j], k ? fg[i0] * 0.0625f : fg[i0], o[2 * i0 + k][e][j]);
+                    for (int j = 0; j < 4; j++) o[2 * i0 + k][e][j] += c[k][e][j];
         }
-        if (++st == ST) st = 0;
+        if constexpr (TMA) {
+            // the stage is read: the unit ST ahead takes its place
+            if (__any_sync(0xffffffffu, gave_up)) {
+                count = n + 1;  // the run ends here
+                gave_up = true;
+            } else {
+                issue(st);
+                lookup();
+            }
+        }
+        if (++st == ST) {
+            st = 0;
+            phase ^= 1u;
+        }
 
         const bool item_end = cur.t == cur.nt - 1;
         if (n + 1 < count && (joint || !item_end)) {
             cur.t += step;
             continue;
         }
-        // the end of an item or of the run
+        // the end of an item or of the run: a parameter of V that is not finite makes all of its rows NaN
 #pragma unroll
-        for (int e = 0; e < E; e++)
+        for (int e = 0; e < E; e++) {
+            float z[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int d = 0; d < ND; d++)
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+                for (int i = 0; i < LW; i++) z[j] = __fmaf_rn(opar[e][2 * i + j], 0.0f, z[j]);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) z[j] += __shfl_xor_sync(0xffffffffu, z[j], x);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const float f = __uint_as_float((uint32_t)(eg[d >> 1] + 9 + 127 - 4 * (d & 1)) << 23);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float x = __shfl_sync(0xffffffffu, olow[e][j], 4 * (d >> 1) + t);
-                    o[d][e][j] += x;
-                    o[d][e][2 + j] += x;
+                    const float x = __shfl_sync(0xffffffffu, opar[e][2 * (d >> 3) + j], 4 * (2 * (d >> 1 & 3) + 1) + t) + z[j];
+                    o[d][e][j] = __fmaf_rn(o[d][e][j], f, x);
+                    o[d][e][2 + j] = __fmaf_rn(o[d][e][2 + j], f, x);
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
+                l[e][j] += z[j];
+            }
+        }
         if (HEADS <= 4)  // lanes t and t + 2 hold the sums of hi and lo halves of the same heads
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) o[d][0][j] += __shfl_xor_sync(0xffffffffu, o[d][0][j], 2);
-#pragma unroll
-        for (int e = 0; e < E; e++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], x);
         const bool from_start = item0 >= u0;
         if (joint ? run.alone : from_start && item_end) {
             pa_finish<G>(a, pl, work, cur, hd, o, ref, l);
@@ -725,6 +829,14 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS>::WARPS * 32, 1)
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (TMA && gave_up)  // the copies that are still on their way write to this CTA's memory
+        for (int i = 0; i < ST; i++) {
+            pa_wait(&s_bar[warp][st], phase, a.kv.err);
+            if (++st == ST) {
+                st = 0;
+                phase ^= 1u;
+            }
+        }
     pa_end<G>(a, pl, work, sh, run, count, cur, item0, tail, p4_sm, hd, o, ref, l);
 }
 
@@ -761,9 +873,9 @@ __global__ void __launch_bounds__(kP4MassThreads) paged4_mass_kernel(PagedAttn4 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 // The workspace of one call: tails, parts, and where weights are gathered stat and scores.
-template <int GP, int HEADS>
+template <int GP, int HEADS, bool TMA>
 size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* base, PaWork* w, P4Scores* sc) {
-    using G = P4Cfg<GP, HEADS>;
+    using G = P4Cfg<GP, HEADS, TMA>;
     const int qblocks = (H / KV + HEADS - 1) / HEADS;
     const size_t parts = align16(ctas * sizeof(PaTail));
     const size_t stat = align16(parts + (size_t)ctas * G::WARPS * 2 * G::PART * sizeof(float));
@@ -797,10 +909,39 @@ int p4_follow(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t s,
     return JYC_OK;
 }
 
-template <int GP, int HEADS>
+// Map of a cache array as [page][slot][kv head][byte], boxes of `box` slots of one head.
+int p4_map(CUtensorMap* m, uint8_t* base, const PagedAttn4& a, int row, int box) {
+    void* fn = nullptr;
+    if (int e = tensor_map_encoder(&fn)) return e;
+    const jyc_kv_pages_q4& p = a.kv.p;
+    const cuuint64_t dims[4] = {(cuuint64_t)row, (cuuint64_t)a.KV, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
+    // the stride of a dimension of one entry is not used, but has to be one
+    const cuuint64_t strides[3] = {(cuuint64_t)(a.KV > 1 ? p.head_stride : row),
+                                   (cuuint64_t)(p.page_size > 1 ? p.pos_stride : row),
+                                   (cuuint64_t)(p.num_pages > 1 ? p.page_stride : row)};
+    const cuuint32_t boxes[4] = {(cuuint32_t)row, 1, (cuuint32_t)box, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn)(
+        m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return JYC_OK;
+}
+
+// Tensor copies need rows of 32 or 64 bytes, strides below 2^40, and pages that a unit of 32 keys fills or that fill half
+// of one (smaller pages would need a copy each for few rows).
+bool p4_tensor_copies(const PagedAttn4& a) {
+    const jyc_kv_pages_q4& p = a.kv.p;
+    const int groups = (a.hd + 31) / 32;
+    const long long far = std::max(p.page_stride, std::max(p.pos_stride, p.head_stride));
+    const bool nonzero = (p.head_stride > 0 || a.KV == 1) && p.pos_stride > 0 && (p.page_stride > 0 || p.num_pages == 1);
+    return nonzero && far < (1LL << 40) && (groups == 2 || groups == 4) && (p.page_size % 32 == 0 || p.page_size == 16);
+}
+
+template <int GP, int HEADS, bool TMA>
 int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t s) {
-    using G = P4Cfg<GP, HEADS>;
-    if (int e = max_dynamic_smem(reinterpret_cast<const void*>(paged4_attention_kernel<GP, HEADS>), G::SMEM)) return e;
+    using G = P4Cfg<GP, HEADS, TMA>;
+    if (int e = max_dynamic_smem(reinterpret_cast<const void*>(paged4_attention_kernel<GP, HEADS, TMA>), G::SMEM)) return e;
     const int capacity = a.kv.table_stride * a.kv.p.page_size, groups = (a.hd + 31) / 32;
     const long long tiles = ((long long)capacity + G::TK - 1) / G::TK;
     const long long items = (long long)a.kv.num_seqs * pl.units_row;
@@ -808,31 +949,39 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles;
     const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
     pl.tk = G::TK;
+    const jyc_kv_pages_q4& p = a.kv.p;
+    P4Maps maps{};
+    if (TMA) {
+        pl.box = std::min(p.page_size, G::TK);
+        if (int e = p4_map(&maps.k, p.k, a, 16 * GP, pl.box)) return e;
+        if (int e = p4_map(&maps.v, p.v, a, 16 * GP, pl.box)) return e;
+    }
     PaWork w;
     P4Scores sc;
-    p4_work<GP, HEADS>(sms, a.kv.num_seqs, a.H, a.KV, a.kv.p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc);
-    // a key's parameters by the widest copies that all of them allow
-    const jyc_kv_pages_q4& p = a.kv.p;
+    p4_work<GP, HEADS, TMA>(sms, a.kv.num_seqs, a.H, a.KV, p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc);
+    // a key's parameters by one copy where their alignment allows it, else word by word
     const uintptr_t at = (uintptr_t)p.kp | (uintptr_t)p.vp | (uintptr_t)(4 * (p.ppage_stride | p.ppos_stride | p.phead_stride));
-    const int copy = groups % 4 == 0 && at % 16 == 0 ? 16 : groups % 2 == 0 && at % 8 == 0 ? 8 : 4;
-    paged4_attention_kernel<GP, HEADS><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, sc, copy);
+    const int copy = groups == GP && at % (4 * GP) == 0 ? 4 * GP : 4;
+    paged4_attention_kernel<GP, HEADS, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, sc, copy, maps);
     JYC_LAUNCHED();
     if (tiles > 1)  // else an item is one unit: none is split
         if (int e = p4_follow(paged_join_kernel<G>, dim3(ctas), kPaJoinWarps * 32, s, a, pl, w)) return e;
-    if (!sc.s || capacity == 0) return JYC_OK;
+    if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
     const unsigned chunks = (unsigned)std::min({most, (8LL * sms + heads - 1) / heads, 65535LL});
     return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, s, a, pl, w, sc);
 }
 
 // The instantiation of a shape: groups and query heads per unit rounded up.
-#define P4_CASES(F, ...)                                                                     \
-    do {                                                                                     \
-        const int R = H / KV;                                                                \
-        if (hd <= 64) return R <= 4 ? F<2, 4>(__VA_ARGS__) : R <= 8 ? F<2, 8>(__VA_ARGS__) : F<2, 16>(__VA_ARGS__);  \
-        if (hd <= 128) return R <= 4 ? F<4, 4>(__VA_ARGS__) : R <= 8 ? F<4, 8>(__VA_ARGS__) : F<4, 16>(__VA_ARGS__); \
-        if (hd <= 192) return R <= 4 ? F<6, 4>(__VA_ARGS__) : R <= 8 ? F<6, 8>(__VA_ARGS__) : F<6, 16>(__VA_ARGS__); \
-        return R <= 4 ? F<8, 4>(__VA_ARGS__) : R <= 8 ? F<8, 8>(__VA_ARGS__) : F<8, 16>(__VA_ARGS__);                \
+#define P4_HEADS(F, GP, TMA, ...) \
+    return R <= 4 ? F<GP, 4, TMA>(__VA_ARGS__) : R <= 8 ? F<GP, 8, TMA>(__VA_ARGS__) : F<GP, 16, TMA>(__VA_ARGS__)
+#define P4_CASES(F, TMA, ...)                                \
+    do {                                                     \
+        const int R = H / KV;                                \
+        if (hd <= 64) P4_HEADS(F, 2, TMA, __VA_ARGS__);      \
+        if (hd <= 128) P4_HEADS(F, 4, TMA, __VA_ARGS__);     \
+        if (hd <= 192) P4_HEADS(F, 6, false, __VA_ARGS__);   \
+        P4_HEADS(F, 8, false, __VA_ARGS__);                  \
     } while (0)
 
 // ---------------------------------------------------------------------------
@@ -1121,15 +1270,15 @@ int launch_paged4_read(float* K, float* V, int ld, int rows, int KV, int hd, con
     });
 }
 
-template <int GP, int HEADS>
+template <int GP, int HEADS, bool TMA>
 static size_t p4_workspace(int sms, int seqs, int H, int KV, int capacity) {
-    return p4_work<GP, HEADS>(sms, seqs, H, KV, capacity, nullptr, nullptr, nullptr);
+    return p4_work<GP, HEADS, TMA>(sms, seqs, H, KV, capacity, nullptr, nullptr, nullptr);
 }
 
 size_t paged4_attention_workspace(int seqs, int H, int KV, int hd, int capacity) {
     const int sms = sm_count();
     if (sms == 0) return 0;
-    P4_CASES(p4_workspace, sms, seqs, H, KV, capacity);
+    P4_CASES(p4_workspace, false, sms, seqs, H, KV, capacity);  // the same with tensor copies
 }
 
 int launch_paged4_attention(const PagedAttn4& a, void* work, cudaStream_t s) {
@@ -1139,7 +1288,8 @@ int launch_paged4_attention(const PagedAttn4& a, void* work, cudaStream_t s) {
     pl.units_row = KV * pl.qblocks;
     pl.wide_q = aligned16(a.Q, a.ldq);
     pl.wide_rope = pl.wide_q && rope_wide(a.rope);
-    P4_CASES(p4_launch, a, pl, sms, work, s);
+    if (p4_tensor_copies(a)) P4_CASES(p4_launch, true, a, pl, sms, work, s);
+    P4_CASES(p4_launch, false, a, pl, sms, work, s);
 }
 
 int launch_paged4_evict(const PagedEvict4& e, cudaStream_t s) {

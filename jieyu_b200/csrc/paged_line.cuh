@@ -6,6 +6,8 @@
 #include "paged.cuh"
 #include "ptx.cuh"
 
+#include <cuda.h>
+
 namespace jyc {
 
 namespace {  // each file that includes this has its own copies
@@ -149,6 +151,30 @@ __device__ __forceinline__ void pa_next(const typename G::Args& a, const PaPlan&
     c.r = 0;
     c.b++;
     pa_seek<G>(a, pl.tk, c);
+}
+
+// A wait that did not end at once: gives up after 2^31 SM cycles (about a
+// second) and sets the error word; the warp's run then ends with that unit.
+__device__ __noinline__ bool pa_wait_slow(uint64_t* bar, uint32_t parity, int* err) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > (1LL << 31)) {
+            atomicOr(err, kPagedErrWait);
+            return false;
+        }
+    return true;
+}
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, int* err) {
+    return mbar_try_wait(bar, parity) || pa_wait_slow(bar, parity, err);
+}
+// box of a map's tensor [page][slot][kv head][dim] -> shared memory (this CTA's)
+__device__ __forceinline__ void pa_tensor_copy(uint32_t dst, const CUtensorMap* map, int h, int slot, int page,
+                                               uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+        "l"(map), "r"(0), "r"(h), "r"(slot), "r"(page), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
 }
 
 // What the warps of a CTA know of the line.
