@@ -352,7 +352,7 @@ template <int HDP_, int HEADS, bool TMA>
 struct PaCfg {
     using Args = PagedAttn;
     static __device__ __forceinline__ int len(const PagedAttn& a, int b) { return pa_len(a, b); }
-    static constexpr bool STAT = false;
+    static constexpr bool STAT = false, TEAM = false;
     static constexpr int HDP = HDP_;
     static constexpr int TK = HDP <= 128 ? 32 : 16;        // keys of a unit
     // one CTA per SM. Above 64 dims few warps with more units in flight each and room for every accumulator in

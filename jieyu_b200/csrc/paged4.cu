@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <numeric>
 
 namespace jyc {
 
@@ -238,10 +239,19 @@ template <int GP, int HEADS, bool TMA>
 struct P4Cfg {
     using Args = PagedAttn4;
     static __device__ __forceinline__ int len(const PagedAttn4& a, int b) { return p4_len(a, b); }
-    static constexpr bool STAT = true;
-    static constexpr int HDP = 32 * GP, TK = 32;
-    static constexpr int WARPS = GP <= 2 ? 16 : GP <= 4 ? 12 : 8;
-    static constexpr int ST = GP <= 6 ? 3 : 2;
+    static constexpr bool STAT = true, TEAM = true;
+#ifndef P4W
+#define P4W 8
+#define P4ST 2
+#define P4U 2
+#define P4W2 8
+#define P4ST2 3
+#define P4U2 2
+#endif
+    static constexpr int U = GP <= 2 ? P4U2 : GP <= 4 ? P4U : 1;  // keys of a lane
+    static constexpr int HDP = 32 * GP, TK = 32 * U;              // keys of a unit
+    static constexpr int WARPS = GP <= 2 ? P4W2 : GP <= 4 ? P4W : 8;
+    static constexpr int ST = GP <= 2 ? P4ST2 : GP <= 4 ? P4ST : GP <= 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
     static constexpr int ROWS = HEADS;
     // rows of K and V: tensor copies swizzle their 16-byte chunks, else an odd number of chunks, so that the 8 rows of an
@@ -252,7 +262,7 @@ struct P4Cfg {
     static constexpr int STAGE = VPOFF + 4 * PW * TK;
     static constexpr int PART = ROWS * (HDP + 2);  // floats of a partial: o, then (ref, l) per row
     static constexpr int SOFF = ST * STAGE;        // V's steps of the current unit
-    static constexpr int RING = TMA ? (SOFF + 64 * GP + 1023) / 1024 * 1024 : SOFF + 64 * GP;
+    static constexpr int RING = TMA ? (SOFF + 64 * GP * U + 1023) / 1024 * 1024 : SOFF + 64 * GP * U;
     static constexpr int SMEM = WARPS * RING + (TMA ? 1024 : 0);
     static_assert(PART * 4 <= RING, "a partial fits the ring");
     static_assert(!TMA || GP == 2 || GP == 4, "rows of 32 or 64 bytes");
@@ -268,10 +278,10 @@ struct P4Maps {
 // [key][ROWS].
 struct P4Scores {
     float* s;  // nullptr: no weights are gathered
-    long long tiles;
+    long long keys;  // floats of a row of units
 };
-__device__ __forceinline__ size_t p4_score_at(const P4Scores& sc, const PaPlan& pl, int b, int r, int t, int rows) {
-    return ((size_t)((long long)b * pl.units_row + r) * sc.tiles + t) * 32 * rows;
+__device__ __forceinline__ size_t p4_score_at(const P4Scores& sc, const PaPlan& pl, int b, int r, int t, int unit) {
+    return (size_t)((long long)b * pl.units_row * pl.team + r) * sc.keys + (size_t)t * unit;
 }
 __device__ __forceinline__ __half2 p4_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t p4_u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
@@ -305,7 +315,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, int param_copy,
                             const __grid_constant__ P4Maps maps) {
     using G = P4Cfg<GP, HEADS, TMA>;
-    constexpr int TK = G::TK, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PW = G::PW, LW = PW / 4;
+    constexpr int TK = G::TK, U = G::U, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PW = G::PW, LW = PW / 4;
     extern __shared__ __align__(128) unsigned char p4_raw[];
     unsigned char* const p4_sm = TMA ? p4_raw + (-smem_u32(p4_raw) & 1023u) : p4_raw;
     __shared__ __align__(8) uint64_t s_bar[G::WARPS][ST];
@@ -327,10 +337,11 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     // parameters behind the head's last group: no copy writes them
     if (groups < PW)
         for (int st = 0; st < ST; st++)
-            for (int i = groups; i < PW; i++) {
-                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::KPOFF)[PW * lane + i] = 0u;
-                reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::VPOFF)[PW * lane + i] = 0u;
-            }
+            for (int i = groups; i < PW; i++)
+                for (int j = lane; j < TK; j += 32) {
+                    reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::KPOFF)[PW * j + i] = 0u;
+                    reinterpret_cast<uint32_t*>(ring + st * G::STAGE + G::VPOFF)[PW * j + i] = 0u;
+                }
     const PaRun run = pa_start<G>(a, pl, sh, hd);
     const long long w0 = run.w0, u0 = run.u0;
     const bool joint = run.joint;
@@ -340,27 +351,34 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     long long item0 = run.item0;
     if (tid == 0) work.tail[blockIdx.x].ctas = 0;
 
-    // copies: lane j looks up the page of key j of a unit one step before the unit's copies are issued
+    // copies: lane j looks up the pages of keys j and j + 32 of a unit one step before the unit's copies are issued
     PaCursor nx = cur;
     int issued = 0;  // units whose pages are looked up
-    int pg = -1, slot = 0, h = -1;
+    int pg[U], slot[U], h = -1;
     long long hoff = 0, hpoff = 0;  // of kv head h
-    bool ok = false;
-    unsigned counts = 0u;  // whether this lane's key counts, of the unit issued last in bit 0
+    bool ok[U];
+    unsigned counts[U];  // whether this lane's key counts, of the unit issued last in bit 0
+#pragma unroll
+    for (int u = 0; u < U; u++) counts[u] = 0u;
     auto lookup = [&] {
-        ok = false;
+#pragma unroll
+        for (int u = 0; u < U; u++) ok[u] = false;
         if (issued < count) {
-            const int pos = nx.t * TK + lane, hn = pl.qblocks == 1 ? nx.r : nx.r / pl.qblocks;
+            const int r = pa_row<G>(pl, nx), hn = pl.qblocks == 1 ? r : r / pl.qblocks;
             if (hn != h) {
                 h = hn;
                 if (!TMA) hoff = (long long)h * a.kv.p.head_stride;
                 hpoff = (long long)h * a.kv.p.phead_stride;
             }
-            if (pos < nx.len) {
-                const int idx = a.kv.by_page(pos);
-                slot = pos - idx * a.kv.p.page_size;
-                pg = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
-                ok = true;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int pos = nx.t * TK + 32 * u + lane;
+                if (pos < nx.len) {
+                    const int idx = a.kv.by_page(pos);
+                    slot[u] = pos - idx * a.kv.p.page_size;
+                    pg[u] = __ldg(a.kv.table + (size_t)nx.b * a.kv.table_stride + idx);
+                    ok[u] = true;
+                }
             }
             pa_next<G>(a, pl, nx, step);
         }
@@ -368,57 +386,67 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     };
     constexpr int LPR = GP <= 2 ? 2 : GP <= 4 ? 4 : 8, RPI = 32 / LPR;  // lanes per row, rows per step
     const int cc = lane & (LPR - 1), cr = lane / LPR;
-    // the unit that was looked up last: rows, and by lane j key j's parameters
+    // the unit that was looked up last: rows, and by lane j its keys' parameters
     auto issue = [&](int st) {
-        if (ok && (unsigned)pg >= (unsigned)a.kv.p.num_pages) {
-            p4_flag(a.kv, kPagedErrPage);
-            ok = false;
-        }
-        counts = counts << 1 | (ok ? 1u : 0u);
-        const uint32_t base = ring_a + st * G::STAGE;
-        if (ok) {
-            const long long po = (long long)pg * a.kv.p.ppage_stride + (long long)slot * a.kv.p.ppos_stride + hpoff;
-            const uint32_t* const kp = reinterpret_cast<const uint32_t*>(a.kv.p.kp) + po;
-            const uint32_t* const vp = reinterpret_cast<const uint32_t*>(a.kv.p.vp) + po;
-            const uint32_t dst = base + G::KPOFF + 4 * PW * lane;
-            if (param_copy == 4 * GP && 4 * GP <= 16) {
-                p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst, kp);
-                p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst + (G::VPOFF - G::KPOFF), vp);
-            } else if (GP == 8 && param_copy == 32) {
+        unsigned bytes = 0u;
+        uint64_t* const bar = &s_bar[warp][st];
 #pragma unroll
-                for (int i = 0; i < 8; i += 4) {
-                    p4_copy<16>(dst + 4 * i, kp + i);
-                    p4_copy<16>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
-                }
-            } else {
-                for (int i = 0; i < groups; i++) {
-                    p4_copy<4>(dst + 4 * i, kp + i);
-                    p4_copy<4>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
-                }
+        for (int u = 0; u < U; u++) {
+            if (ok[u] && (unsigned)pg[u] >= (unsigned)a.kv.p.num_pages) {
+                p4_flag(a.kv, kPagedErrPage);
+                ok[u] = false;
             }
+            counts[u] = counts[u] << 1 | (ok[u] ? 1u : 0u);
+            if (TMA) bytes += __popc(__ballot_sync(0xffffffffu, ok[u] && (lane & (pl.box - 1)) == 0)) * pl.box * 32 * GP;
         }
-        if constexpr (TMA) {
-            uint64_t* bar = &s_bar[warp][st];
-            const bool lead = ok && (lane & (pl.box - 1)) == 0;
-            const unsigned bytes = __popc(__ballot_sync(0xffffffffu, lead)) * pl.box * 32 * GP;
+        if (TMA) {
             if (lane == 0) mbar_expect_tx(bar, bytes);
             __syncwarp();
-            if (lead) {
-                pa_tensor_copy(base + lane * G::PITCH, &maps.k, h, slot, pg, bar, policy);
-                pa_tensor_copy(base + G::VOFF + lane * G::PITCH, &maps.v, h, slot, pg, bar, policy);
-            }
-        } else {
-            const unsigned mask = __ballot_sync(0xffffffffu, ok);
-            const long long off =
-                ok ? (long long)pg * a.kv.p.page_stride + (long long)slot * a.kv.p.pos_stride + hoff : 0LL;
+        }
 #pragma unroll
-            for (int i = 0; i < TK / RPI; i++) {
-                const int row = i * RPI + cr;
-                const long long o = __shfl_sync(0xffffffffu, off, row) + 16 * cc;
-                if (cc < groups && ((mask >> row) & 1)) {
-                    const uint32_t dst = base + row * G::PITCH + 16 * cc;
-                    pa_copy<16>(dst, a.kv.p.k + o, policy);
-                    pa_copy<16>(dst + G::VOFF, a.kv.p.v + o, policy);
+        for (int u = 0; u < U; u++) {
+            const int key = 32 * u + lane;
+            const uint32_t base = ring_a + st * G::STAGE;
+            if (ok[u]) {
+                const long long po =
+                    (long long)pg[u] * a.kv.p.ppage_stride + (long long)slot[u] * a.kv.p.ppos_stride + hpoff;
+                const uint32_t* const kp = reinterpret_cast<const uint32_t*>(a.kv.p.kp) + po;
+                const uint32_t* const vp = reinterpret_cast<const uint32_t*>(a.kv.p.vp) + po;
+                const uint32_t dst = base + G::KPOFF + 4 * PW * key;
+                if (param_copy == 4 * GP && 4 * GP <= 16) {
+                    p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst, kp);
+                    p4_copy<(4 * GP <= 16 ? 4 * GP : 16)>(dst + (G::VPOFF - G::KPOFF), vp);
+                } else if (GP == 8 && param_copy == 32) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        p4_copy<16>(dst + 4 * i, kp + i);
+                        p4_copy<16>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
+                    }
+                } else {
+                    for (int i = 0; i < groups; i++) {
+                        p4_copy<4>(dst + 4 * i, kp + i);
+                        p4_copy<4>(dst + (G::VPOFF - G::KPOFF) + 4 * i, vp + i);
+                    }
+                }
+            }
+            if constexpr (TMA) {
+                if (ok[u] && (lane & (pl.box - 1)) == 0) {
+                    pa_tensor_copy(base + key * G::PITCH, &maps.k, h, slot[u], pg[u], bar, policy);
+                    pa_tensor_copy(base + G::VOFF + key * G::PITCH, &maps.v, h, slot[u], pg[u], bar, policy);
+                }
+            } else {
+                const unsigned mask = __ballot_sync(0xffffffffu, ok[u]);
+                const long long off =
+                    ok[u] ? (long long)pg[u] * a.kv.p.page_stride + (long long)slot[u] * a.kv.p.pos_stride + hoff : 0LL;
+#pragma unroll
+                for (int i = 0; i < 32 / RPI; i++) {
+                    const int row = i * RPI + cr;
+                    const long long o = __shfl_sync(0xffffffffu, off, row) + 16 * cc;
+                    if (cc < groups && ((mask >> row) & 1)) {
+                        const uint32_t dst = base + (32 * u + row) * G::PITCH + 16 * cc;
+                        pa_copy<16>(dst, a.kv.p.k + o, policy);
+                        pa_copy<16>(dst + G::VOFF, a.kv.p.v + o, policy);
+                    }
                 }
             }
         }
@@ -451,7 +479,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                     lookup();
                 }
             }
-            const int qb = cur.r % pl.qblocks, kvh = cur.r / pl.qblocks;
+            const int r = pa_row<G>(pl, cur), qb = r % pl.qblocks, kvh = r / pl.qblocks;
             const int pos = a.rope.cos_t ? (a.rope_pos ? __ldg(a.rope_pos + cur.b) : cur.len - 1) : 0;
 #pragma unroll
             for (int i = 0; i < GP; i++) {
@@ -522,23 +550,34 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             if (!pa_wait(&s_bar[warp][st], phase, a.kv.err)) gave_up = true;
         unsigned char* const sb = ring + st * G::STAGE;
         const uint32_t base = ring_a + st * G::STAGE;
-        const unsigned in = __ballot_sync(0xffffffffu, (counts >> (ST - 1)) & 1u);  // keys that count
+        unsigned in[U];  // keys that count
+        bool full = true;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            in[u] = __ballot_sync(0xffffffffu, (counts[u] >> (ST - 1)) & 1u);
+            full &= in[u] == ~0u;
+        }
 
-        // lane j, key j: V's steps in units of their group's largest, laid out by group as the products read them
+        // lane j, its keys: V's steps in units of their group's largest, laid out by group as the products read them
         {
-            uint32_t vw[PW];
-            uint32_t* const vrow = reinterpret_cast<uint32_t*>(sb + G::VPOFF) + PW * lane;
-            if (in != ~0u && !(in >> lane & 1))  // whatever the ring held
+            uint32_t vw[U][PW];
+            __half2 top = __float2half2_rn(0.0f);
 #pragma unroll
-                for (int i = 0; i < PW; i++) vrow[i] = 0u;
-            p4_words(vrow, vw);
-            __half2 top = __hmul2_rn(p4_h2(vw[0]), p4_h2(ug[0]));
+            for (int u = 0; u < U; u++) {
+                uint32_t* const vrow = reinterpret_cast<uint32_t*>(sb + G::VPOFF) + PW * (32 * u + lane);
+                if (!full && !(in[u] >> lane & 1))  // whatever the ring held
 #pragma unroll
-            for (int i = 1; i < GP; i++) top = __hmax2_nan(top, __hmul2_rn(p4_h2(vw[i]), p4_h2(ug[i])));
+                    for (int i = 0; i < PW; i++) vrow[i] = 0u;
+                p4_words(vrow, vw[u]);
+#pragma unroll
+                for (int i = 0; i < GP; i++) top = __hmax2_nan(top, __hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i])));
+            }
             if (__any_sync(0xffffffffu, !(__low2float(top) < 2.0f))) {  // a larger step than before
 #pragma unroll
                 for (int i = 0; i < GP; i++) {
-                    const int e1 = max(eg[i], (int)min(__reduce_max_sync(0xffffffffu, vw[i] & 0x7fffu) >> 10, 30u));
+                    uint32_t most = vw[0][i] & 0x7fffu;
+                    if (U > 1) most = max(most, vw[U - 1][i] & 0x7fffu);
+                    const int e1 = max(eg[i], (int)min(__reduce_max_sync(0xffffffffu, most) >> 10, 30u));
                     const float f = __uint_as_float((uint32_t)(127 + eg[i] - e1) << 23);
                     eg[i] = e1;
                     ug[i] = 0x3C000000u | (e1 == 30 ? 0x0200u : (uint32_t)(30 - e1) << 10);
@@ -553,19 +592,23 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             }
             __half* const to = reinterpret_cast<__half*>(ring + G::SOFF) + 8 * ((lane & 7) >> 1) + 2 * (lane >> 3) + (lane & 1);
 #pragma unroll
-            for (int i = 0; i < GP; i++) to[32 * i] = __low2half(__hmul2_rn(p4_h2(vw[i]), p4_h2(ug[i])));
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < GP; i++)
+                    to[32 * (GP * u + i)] = __low2half(__hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i])));
         }
         __syncwarp();
 
         // scores of keys 8 i + g and heads 2 t, + 1, in base 2: the parameters' products with (0, query sum) of each group,
         // then the groups' whole-number dots, which start at the bits of 1.5 * 2^23 (|dot| < 2^16), so an exact subtraction
         // makes them floats
-        float s[4][E][2];
-        {
-            const uint32_t* const kp = reinterpret_cast<const uint32_t*>(sb + G::KPOFF);
+        float s[4 * U][E][2];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t* const kp = reinterpret_cast<const uint32_t*>(sb + G::KPOFF) + 32 * PW * u;
             uint32_t par[LW][4];
 #pragma unroll
-            for (int i = 0; i < LW; i++) pa_ldsm(base + G::KPOFF + 4 * PW * lane + 16 * i, par[i]);
+            for (int i = 0; i < LW; i++) pa_ldsm(base + G::KPOFF + 4 * PW * (32 * u + lane) + 16 * i, par[i]);
             float acc[2][E][4];
 #pragma unroll
             for (int m = 0; m < 2; m++)
@@ -589,7 +632,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     uint32_t r[4];
-                    pa_ldsm(base + G::at(lane, i0 + k), r);
+                    pa_ldsm(base + G::at(32 * u + lane, i0 + k), r);
 #pragma unroll
                     for (int m = 0; m < 2; m++) {
                         const uint32_t kf[4] = {r[2 * m] & 0x0F0F0F0Fu, r[2 * m + 1] & 0x0F0F0F0Fu,
@@ -611,20 +654,20 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) s[i][e][j] = __fmul_rn(acc[i >> 1][e][2 * (i & 1) + j], qsl[e][j]);
+                    for (int j = 0; j < 2; j++) s[4 * u + i][e][j] = __fmul_rn(acc[i >> 1][e][2 * (i & 1) + j], qsl[e][j]);
         }
-        if (in != ~0u) {  // keys that do not count: -inf, whatever the ring held
+        if (!full) {  // keys that do not count: -inf, whatever the ring held
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4 * U; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) s[i][e][j] = in >> (8 * i + g) & 1 ? s[i][e][j] : -INFINITY;
+                    for (int j = 0; j < 2; j++) s[i][e][j] = in[i >> 2] >> (8 * (i & 3) + g) & 1 ? s[i][e][j] : -INFINITY;
         }
         if (scores.s && (HEADS > 4 || t < 2)) {
-            float* const to = scores.s + p4_score_at(scores, pl, cur.b, cur.r, cur.t, ROWS) + 2 * t;
+            float* const to = scores.s + p4_score_at(scores, pl, cur.b, pa_row<G>(pl, cur), cur.t, TK * ROWS) + 2 * t;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4 * U; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
                     *reinterpret_cast<float2*>(to + ROWS * (8 * i + g) + 8 * e) = make_float2(s[i][e][0], s[i][e][1]);
@@ -636,6 +679,10 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 float x = fmaxf(fmaxf(s[0][e][j], s[1][e][j]), fmaxf(s[2][e][j], s[3][e][j]));
+                if (U > 1) {
+                    constexpr int b = 4 * (U - 1);
+                    x = fmaxf(x, fmaxf(fmaxf(s[b][e][j], s[b + 1][e][j]), fmaxf(s[b + 2][e][j], s[b + 3][e][j])));
+                }
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -661,9 +708,9 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                 }
         }
         // weights as halves hi + lo, transposed: column g, keys 8 i + 2 t, + 1
-        uint32_t hi[4][E], lo[4][E];
+        uint32_t hi[4 * U][E], lo[4 * U][E];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4 * U; i++)
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const float b0 = ex2(s[i][e][0] - ref[e][0]), b1 = ex2(s[i][e][1] - ref[e][1]);
@@ -676,81 +723,90 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             }
         // the parameters' share: rows are their columns
         {
-            uint32_t par[LW][4];
+            float c[E][4];
 #pragma unroll
-            for (int i = 0; i < LW; i++) pa_ldsm_t(base + G::VPOFF + 4 * PW * lane + 16 * i, par[i]);
+            for (int u = 0; u < U; u++) {
+                uint32_t par[LW][4];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                float c[4];
+                for (int i = 0; i < LW; i++) pa_ldsm_t(base + G::VPOFF + 4 * PW * (32 * u + lane) + 16 * i, par[i]);
 #pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    const uint32_t pf[4] = {par[0][2 * m], LW > 1 ? par[LW - 1][2 * m] : 0u, par[0][2 * m + 1],
-                                            LW > 1 ? par[LW - 1][2 * m + 1] : 0u};
-                    const uint32_t h0 = hi[2 * m][e], h1 = hi[2 * m + 1][e], l0 = lo[2 * m][e], l1 = lo[2 * m + 1][e];
-                    if (HEADS <= 4) {
-                        const uint32_t b[2] = {g < 4 ? h0 : l0, g < 4 ? h1 : l1};
-                        if (m == 0)
-                            pa_mma_f16(pf, b, 0.0f, c);
-                        else
-                            pa_mma_f16(pf, b, c);
-                    } else {
-                        const uint32_t bl[2] = {l0, l1}, bh[2] = {h0, h1};
-                        if (m == 0)
-                            pa_mma_f16(pf, bl, 0.0f, c);
-                        else
-                            pa_mma_f16(pf, bl, c);
-                        pa_mma_f16(pf, bh, c);
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        const uint32_t pf[4] = {par[0][2 * m], LW > 1 ? par[LW - 1][2 * m] : 0u, par[0][2 * m + 1],
+                                                LW > 1 ? par[LW - 1][2 * m + 1] : 0u};
+                        const int i = 4 * u + 2 * m;
+                        const uint32_t h0 = hi[i][e], h1 = hi[i + 1][e], l0 = lo[i][e], l1 = lo[i + 1][e];
+                        if (HEADS <= 4) {
+                            const uint32_t b[2] = {g < 4 ? h0 : l0, g < 4 ? h1 : l1};
+                            if (i == 0)
+                                pa_mma_f16(pf, b, 0.0f, c[e]);
+                            else
+                                pa_mma_f16(pf, b, c[e]);
+                        } else {
+                            const uint32_t bl[2] = {l0, l1}, bh[2] = {h0, h1};
+                            if (i == 0)
+                                pa_mma_f16(pf, bl, 0.0f, c[e]);
+                            else
+                                pa_mma_f16(pf, bl, c[e]);
+                            pa_mma_f16(pf, bh, c[e]);
+                        }
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < 2 * LW; i++) opar[e][i] += c[i];
             }
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int i = 0; i < 2 * LW; i++) opar[e][i] += c[e][i];
         }
         // P.V, a group at a time: V's numbers as subnormal halves (q * 2^-24, the high ones 16 times that), rows g dims 2 g,
         // rows g + 8 dims 2 g + 1 of 16; a weight times a step as halves: hi rounded, lo what that left and lo's share.
         // 4 heads fill 8 columns with their hi and lo halves
-        uint32_t zl[4];
+        uint32_t zl[4 * U];
         if (HEADS <= 4)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 4 * U; i++) {
                 zl[i] = g < 4 ? 0u : hi[i][0] ^ 0x80008000u;
                 lo[i][0] = g < 4 ? 0u : lo[i][0];
             }
 #pragma unroll
         for (int i0 = 0; i0 < GP; i0++) {
-            uint32_t r[4];
-            pa_ldsm_t(base + G::VOFF + G::at(lane, i0), r);
-            const uint4 sv = *reinterpret_cast<const uint4*>(ring + G::SOFF + 64 * i0 + 16 * t);
-            const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
             float c[2][E][4];
 #pragma unroll
-            for (int m = 0; m < 2; m++) {
-                uint32_t bh[E][2], bl[E][2];
+            for (int u = 0; u < U; u++) {
+                uint32_t r[4];
+                pa_ldsm_t(base + G::VOFF + G::at(32 * u + lane, i0), r);
+                const uint4 sv = *reinterpret_cast<const uint4*>(ring + G::SOFF + 64 * (GP * u + i0) + 16 * t);
+                const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
-                for (int e = 0; e < E; e++)
+                for (int m = 0; m < 2; m++) {
+                    uint32_t bh[E][2], bl[E][2];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const __half2 w = p4_h2(sw[2 * m + i]), ph = p4_h2(hi[2 * m + i][e]), pw = p4_h2(lo[2 * m + i][e]);
-                        if (HEADS <= 4) {
-                            bh[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hmul2_rn(p4_h2(zl[2 * m + i]), w))));
-                        } else {
-                            const __half2 x = __hmul2_rn(ph, w);
-                            bh[e][i] = p4_u(x);
-                            bl[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hneg2(x))));
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const int at = 4 * u + 2 * m + i;
+                            const __half2 w = p4_h2(sw[2 * m + i]), ph = p4_h2(hi[at][e]), pw = p4_h2(lo[at][e]);
+                            if (HEADS <= 4) {
+                                bh[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hmul2_rn(p4_h2(zl[at]), w))));
+                            } else {
+                                const __half2 x = __hmul2_rn(ph, w);
+                                bh[e][i] = p4_u(x);
+                                bl[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hneg2(x))));
+                            }
                         }
-                    }
-                const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+                    const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t mk = k ? 0x00F000F0u : 0x000F000Fu;
-                    const uint32_t vf[4] = {x0 & mk, y0 & mk, x1 & mk, y1 & mk};
+                    for (int k = 0; k < 2; k++) {
+                        const uint32_t mk = k ? 0x00F000F0u : 0x000F000Fu;
+                        const uint32_t vf[4] = {x0 & mk, y0 & mk, x1 & mk, y1 & mk};
 #pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        if (m == 0)
-                            pa_mma_f16(vf, bh[e], 0.0f, c[k][e]);
-                        else
-                            pa_mma_f16(vf, bh[e], c[k][e]);
-                        if (HEADS > 4) pa_mma_f16(vf, bl[e], c[k][e]);
+                        for (int e = 0; e < E; e++) {
+                            if (u == 0 && m == 0)
+                                pa_mma_f16(vf, bh[e], 0.0f, c[k][e]);
+                            else
+                                pa_mma_f16(vf, bh[e], c[k][e]);
+                            if (HEADS > 4) pa_mma_f16(vf, bl[e], c[k][e]);
+                        }
                     }
                 }
             }
@@ -820,7 +876,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
         } else {
             if (joint) break;  // o, ref and l stay in registers
             tail = from_start;
-            pa_store<G>(work.part + ((size_t)(w0 + warp) * 2 + (from_start ? 1 : 0)) * G::PART, true, o, ref, l);
+            pa_store<G>(work.part + ((size_t)(w0 * pl.team + warp) * 2 + (from_start ? 1 : 0)) * G::PART, true, o, ref, l);
         }
         if (n + 1 < count) {
             item0 += cur.nt;
@@ -853,7 +909,7 @@ __global__ void __launch_bounds__(kP4MassThreads) paged4_mass_kernel(PagedAttn4 
         const int page = p4_entry(a.kv, b, (int)j, &slot);
         float sum = 0.0f;
         for (int qb = 0; qb < pl.qblocks; qb++) {
-            const float* s = scores.s + p4_score_at(scores, pl, b, kvh * pl.qblocks + qb, (int)(j >> 5), ROWS) + (j & 31) * ROWS;
+            const float* s = scores.s + p4_score_at(scores, pl, b, kvh * pl.qblocks + qb, (int)j, ROWS);
             float4 x[ROWS / 4];
 #pragma unroll
             for (int i = 0; i < ROWS / 4; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(s) + i);
@@ -885,11 +941,11 @@ size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* b
         return stat;
     }
     const size_t score = align16(stat + (size_t)seqs * H * sizeof(float2));
-    const long long tiles = ((long long)capacity + 31) / 32;
+    const long long keys = ((long long)capacity + G::TK - 1) / G::TK * G::TK * HEADS;
     if (w)
         *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts), reinterpret_cast<float2*>(base + stat)};
-    if (sc) *sc = P4Scores{reinterpret_cast<float*>(base + score), tiles};
-    return score + (size_t)seqs * KV * qblocks * tiles * 32 * HEADS * sizeof(float);
+    if (sc) *sc = P4Scores{reinterpret_cast<float*>(base + score), keys};
+    return score + (size_t)seqs * KV * qblocks * keys * sizeof(float);
 }
 
 // A launch behind the last one, which it waits for by itself.
@@ -944,15 +1000,19 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     if (int e = max_dynamic_smem(reinterpret_cast<const void*>(paged4_attention_kernel<GP, HEADS, TMA>), G::SMEM)) return e;
     const int capacity = a.kv.table_stride * a.kv.p.page_size, groups = (a.hd + 31) / 32;
     const long long tiles = ((long long)capacity + G::TK - 1) / G::TK;
+    // teams of as many neighbouring kv heads as the warps hold evenly: their rows lie side by side where pages hold
+    // positions first
+    pl.team = std::gcd(pl.units_row, (int)G::WARPS);
+    pl.units_row /= pl.team;
     const long long items = (long long)a.kv.num_seqs * pl.units_row;
     // no more CTAs than the longest possible lengths have units for
-    const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles;
-    const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + kPaFewWarps - 1) / kPaFewWarps));
+    const long long units = tiles >= (1LL << 31) / items ? 1LL << 31 : items * tiles, few = std::max(1, kPaFewWarps / pl.team);
+    const int ctas = (int)std::max(1LL, std::min((long long)sms, (units + few - 1) / few));
     pl.tk = G::TK;
     const jyc_kv_pages_q4& p = a.kv.p;
     P4Maps maps{};
     if (TMA) {
-        pl.box = std::min(p.page_size, G::TK);
+        pl.box = std::min(p.page_size, 32);
         if (int e = p4_map(&maps.k, p.k, a, 16 * GP, pl.box)) return e;
         if (int e = p4_map(&maps.v, p.v, a, 16 * GP, pl.box)) return e;
     }
@@ -965,7 +1025,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     paged4_attention_kernel<GP, HEADS, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, sc, copy, maps);
     JYC_LAUNCHED();
     if (tiles > 1)  // else an item is one unit: none is split
-        if (int e = p4_follow(paged_join_kernel<G>, dim3(ctas), kPaJoinWarps * 32, s, a, pl, w)) return e;
+        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, pl.team), kPaWideThreads, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
     const unsigned chunks = (unsigned)std::min({most, (8LL * sms + heads - 1) / heads, 65535LL});
@@ -1276,13 +1336,13 @@ static size_t p4_workspace(int sms, int seqs, int H, int KV, int capacity) {
 }
 
 size_t paged4_attention_workspace(int seqs, int H, int KV, int hd, int capacity) {
-    const int sms = sm_count();
+    const int sms = std::min(sm_count(), kPaMaxCtas);
     if (sms == 0) return 0;
     P4_CASES(p4_workspace, false, sms, seqs, H, KV, capacity);  // the same with tensor copies
 }
 
 int launch_paged4_attention(const PagedAttn4& a, void* work, cudaStream_t s) {
-    const int H = a.H, KV = a.KV, hd = a.hd, sms = sm_count();
+    const int H = a.H, KV = a.KV, hd = a.hd, sms = std::min(sm_count(), kPaMaxCtas);
     PaPlan pl{};
     pl.qblocks = H / KV > 8 ? (H / KV + 15) / 16 : 1;
     pl.units_row = KV * pl.qblocks;

@@ -87,6 +87,7 @@ struct PaPlan {
     bool wide_q;    // 16-byte loads of Q, 8-byte ones of the tables
     int box;        // keys of a tensor copy
     bool wide_rope; // turned4's wide form
+    int team;       // warps that take the same units of neighbouring rows (where G::TEAM; units_row counts teams' rows)
 };
 // The line cut into runs: worker w starts at w * base + min(w, rest).
 struct PaLine {
@@ -115,13 +116,13 @@ struct PaWork {
     float2* stat;      // [sequence][head]: reference and 1 / sum of the weights, or nullptr
 };
 
-// Runs of U units: as many workers as there are warps, or units; a few per CTA
-// at least, whose parts are joined in shared memory.
+// Runs of U units: as many workers (warps, or teams of them) as a CTA has, or
+// units; a few warps per CTA at least, whose parts are joined in shared memory.
 constexpr int kPaFewWarps = 4;
-__device__ __forceinline__ PaLine pa_line(long long U, int ctas, int warps) {
+__device__ __forceinline__ PaLine pa_line(long long U, int ctas, int workers, int few) {
     PaLine l;
-    const long long each = U >> 31 ? warps : ((unsigned)U + ctas - 1) / (unsigned)ctas;
-    l.per_cta = (int)min((long long)warps, max((long long)kPaFewWarps, each));
+    const long long each = U >> 31 ? workers : ((unsigned)U + ctas - 1) / (unsigned)ctas;
+    l.per_cta = (int)min((long long)workers, max((long long)few, each));
     l.workers = min((long long)ctas * l.per_cta, U);
     l.base = l.rest = 0;
     if (U >> 32) {
@@ -137,6 +138,16 @@ __device__ __forceinline__ PaLine pa_line(long long U, int ctas, int warps) {
 struct PaCursor {
     int b, r, t, nt, len;  // sequence, row of units, unit and units in it, length
 };
+// Warps of a team, and a warp's row of units.
+template <class G>
+__device__ __forceinline__ int pa_team(const PaPlan& pl) {
+    return G::TEAM ? pl.team : 1;
+}
+template <class G>
+__device__ __forceinline__ int pa_row(const PaPlan& pl, const PaCursor& c) {
+    const int warp = threadIdx.x >> 5;
+    return G::TEAM ? c.r * pl.team + warp % pl.team : c.r;
+}
 template <class G>
 __device__ __forceinline__ void pa_seek(const typename G::Args& a, int tk, PaCursor& c) {
     c.len = 0;
@@ -196,6 +207,7 @@ template <class G>
 __device__ __forceinline__ PaRun pa_start(const typename G::Args& a, const PaPlan& pl, PaShared<G>& sh, int hd) {
     constexpr int TK = G::TK, WARPS = G::WARPS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.kv.num_seqs;
+    const int team = pa_team<G>(pl), mate = warp / team;  // this warp's team
     PaRun run;
     // where the units of each sequence lie in the line
     const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
@@ -224,14 +236,14 @@ __device__ __forceinline__ PaRun pa_start(const typename G::Args& a, const PaPla
         if (w < warp) ex += sh.scan[w];
         U += sh.scan[w];
     }
-    const PaLine line = run.line = pa_line(U, gridDim.x, WARPS);
+    const PaLine line = run.line = pa_line(U, gridDim.x, WARPS / team, max(1, kPaFewWarps / team));
     const long long w0 = (long long)blockIdx.x * line.per_cta;
     sh.ex[tid] = ex;
     __syncthreads();
     {
-        // warp: where its run starts (the last thread's segment that starts at or before it)
-        const long long u = line.start(w0 + warp);
-        if (warp < line.per_cta && u < U) {
+        // where its run starts (the last thread's segment that starts at or before it)
+        const long long u = line.start(w0 + mate);
+        if (warp == mate * team && mate < line.per_cta && u < U) {
             int lo = 0;
 #pragma unroll
             for (int i = 1 << (31 - __builtin_clz(WARPS * 32)); i > 0; i >>= 1)
@@ -243,8 +255,8 @@ __device__ __forceinline__ PaRun pa_start(const typename G::Args& a, const PaPla
                 if (u < at + n) {
                     const long long k = u - at;
                     const int r = k >> 31 ? (int)(k / nt) : (int)k / nt, t0 = (int)(k - (long long)r * nt);
-                    sh.cur[warp] = PaCursor{b, r, t0, nt, len};
-                    sh.first[warp] = u - t0;  // first unit of the item that the run starts in
+                    sh.cur[mate] = PaCursor{b, r, t0, nt, len};
+                    sh.first[mate] = u - t0;  // first unit of the item that the run starts in
                     break;
                 }
                 at += n;
@@ -253,9 +265,9 @@ __device__ __forceinline__ PaRun pa_start(const typename G::Args& a, const PaPla
     }
     __syncthreads();
 
-    run.worker = warp < line.per_cta;
+    run.worker = mate < line.per_cta;
     run.w0 = w0;
-    run.u0 = line.start(w0 + warp);
+    run.u0 = line.start(w0 + mate);
     run.c0 = line.start(w0);
     run.c1 = line.start(w0 + line.per_cta);
     // joint: every run of the CTA inside one item: its warps take units in turn (neighbours in memory at the same
@@ -266,19 +278,19 @@ __device__ __forceinline__ PaRun pa_start(const typename G::Args& a, const PaPla
         run.joint = run.c1 <= end;
         run.whole = run.c0 == first && run.c1 == end;
     }
-    run.count = run.worker ? (int)(line.start(w0 + warp + 1) - run.u0) : 0;
+    run.count = run.worker ? (int)(line.start(w0 + mate + 1) - run.u0) : 0;
     run.step = run.joint ? line.per_cta : 1;
     run.alone = run.whole && run.c1 - run.c0 == 1;
     run.cur = PaCursor{0, 0, 0, 0, 0};
     run.item0 = 0;
     if (run.joint) {
         run.cur = sh.cur[0];
-        run.cur.t += warp;
+        run.cur.t += mate;
         const int units = (int)(run.c1 - run.c0);
-        run.count = run.worker && warp < units ? (units - warp + run.step - 1) / run.step : 0;
+        run.count = run.worker && mate < units ? (units - mate + run.step - 1) / run.step : 0;
     } else if (run.count > 0) {
-        run.cur = sh.cur[warp];
-        run.item0 = sh.first[warp];
+        run.cur = sh.cur[mate];
+        run.item0 = sh.first[mate];
     }
     return run;
 }
@@ -290,7 +302,7 @@ __device__ __forceinline__ void pa_finish(const typename G::Args& a, const PaPla
                                           const PaCursor& c, int hd, const float (&o)[G::HDP / 16][G::E][4],
                                           const float (&ref)[G::E][2], const float (&l)[G::E][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.H / a.KV;
-    const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
+    const int r = pa_row<G>(pl, c), qb = r % pl.qblocks, kvh = r / pl.qblocks;
 #pragma unroll
     for (int e = 0; e < G::E; e++)
 #pragma unroll
@@ -416,8 +428,11 @@ __device__ __forceinline__ void pa_end(const typename G::Args& a, const PaPlan& 
                                        const float (&l)[G::E][2]) {
     constexpr int HDP = G::HDP, ROWS = G::ROWS, WARPS = G::WARPS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV;
+    const int team = pa_team<G>(pl), mate = warp / team, member = warp - mate * team;
     const PaLine& line = run.line;
     const long long w0 = run.w0, c0 = run.c0, c1 = run.c1;
+    // an item's part of worker w and this member: its later part (0) or its first (1)
+    auto slot_at = [&](long long w, int m, int first) { return (int)(w * team + m) * 2 + first; };
     // CTAs behind this one that hold parts of an item that ends at unit `end`
     auto later = [&](long long end) { return (int)(line.worker(end - 1) / line.per_cta) - (int)blockIdx.x; };
     if (!run.joint) {
@@ -426,20 +441,20 @@ __device__ __forceinline__ void pa_end(const typename G::Args& a, const PaPlan& 
         __syncthreads();
         if (c1 == c0) return;
         const long long first = sh.first[0], end0 = first + sh.cur[0].nt;
-        for (int pass = warp == 0 ? 0 : 1; pass < 2; pass++) {
+        for (int pass = mate == 0 ? 0 : 1; pass < 2; pass++) {
             const bool head = pass == 0;
             if (head ? first >= c0 : !tail) continue;
             const long long end = head ? end0 : item0 + cur.nt;
-            const int own = (int)(w0 + warp) * 2 + (head ? 0 : 1);
+            const int own = slot_at(w0 + mate, member, head ? 0 : 1);
             int np = 1;
-            while (warp + np < line.per_cta && line.start(w0 + warp + np) < end) np++;
+            while (mate + np < line.per_cta && line.start(w0 + mate + np) < end) np++;
             const PaCursor it = head ? sh.cur[0] : cur;
             const bool ends = !head && end <= c1;
-            if (!head && !ends && lane == 0)
+            if (!head && !ends && lane == 0 && member == 0)
                 work.tail[blockIdx.x] = PaTail{later(end), own, it.b, it.r, line.per_cta};
             if (np == 1) continue;
-            const int qb = it.r % pl.qblocks, kvh = it.r / pl.qblocks;
-            auto slot_of = [&](int i) { return i == 0 ? own : (int)(w0 + warp + i) * 2; };
+            const int r = pa_row<G>(pl, it), qb = r % pl.qblocks, kvh = r / pl.qblocks;
+            auto slot_of = [&](int i) { return i == 0 ? own : slot_at(w0 + mate + i, member, 0); };
             for (int r0 = 0; r0 < ROWS && qb * ROWS + r0 < group; r0 += PaSum<G>::RB) {
                 PaSum<G> sum;
                 const int rows = min(PaSum<G>::RB, group - qb * ROWS - r0);
@@ -459,21 +474,21 @@ __device__ __forceinline__ void pa_end(const typename G::Args& a, const PaPlan& 
     if (run.worker) pa_store<G>(reinterpret_cast<float*>(sm + warp * G::RING), count > 0, o, ref, l);
     __syncthreads();
     const PaCursor c = sh.cur[0];
-    const int qb = c.r % pl.qblocks, kvh = c.r / pl.qblocks;
-    const int own = (int)w0 * 2 + (c0 == sh.first[0] ? 1 : 0);
-    float* part = work.part + (size_t)own * G::PART;
-    if (tid == 0 && !run.whole && c0 == sh.first[0])
-        work.tail[blockIdx.x] = PaTail{later(sh.first[0] + c.nt), own, c.b, c.r, line.per_cta};
-    for (int i = tid; i < ROWS * HDP / 4; i += WARPS * 32) {
-        const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
+    const int begins = c0 == sh.first[0] ? 1 : 0;
+    if (tid == 0 && !run.whole && begins)
+        work.tail[blockIdx.x] = PaTail{later(sh.first[0] + c.nt), slot_at(w0, 0, 1), c.b, c.r, line.per_cta};
+    for (int i = tid; i < team * (ROWS * HDP / 4); i += WARPS * 32) {
+        const int m = G::TEAM ? i / (ROWS * HDP / 4) : 0, k = i - m * (ROWS * HDP / 4);
+        const int row = k / (HDP / 4), d = k % (HDP / 4) * 4, r = c.r * team + m, qb = r % pl.qblocks, kvh = r / pl.qblocks;
+        float* part = work.part + (size_t)slot_at(w0, m, begins) * G::PART;
         float M = kPaLow, L = 0.0f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (int w = 0; w < line.per_cta; w++)
-            M = fmaxf(M, reinterpret_cast<const float*>(sm + w * G::RING)[ROWS * HDP + 2 * row]);
+            M = fmaxf(M, reinterpret_cast<const float*>(sm + (w * team + m) * G::RING)[ROWS * HDP + 2 * row]);
 #pragma unroll 1
         for (int w = 0; w < line.per_cta; w++) {
-            const float* wb = reinterpret_cast<const float*>(sm + w * G::RING);
+            const float* wb = reinterpret_cast<const float*>(sm + (w * team + m) * G::RING);
             const float wr = wb[ROWS * HDP + 2 * row], wl = wb[ROWS * HDP + 2 * row + 1];
             if (wl == 0.0f) continue;  // no key (a warp without units left no o)
             const float f = ex2(wr - M);
@@ -511,7 +526,6 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32)
     __shared__ __align__(16) float s_o[kPaJoinWarps][RB][HDP];
     __shared__ float2 s_rl[kPaJoinWarps][RB];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
-    if (G::STAT) griddep_launch();
     griddep_wait();
     const PaTail tail = work.tail[blockIdx.x];
     if (tail.ctas == 0) return;
@@ -539,10 +553,91 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32)
                 L = __fmaf_rn(f, s_rl[w][r].y, L);
                 O = __fmaf_rn(f, s_o[w][r][d], O);
             }
-            const int h = kvh * group + qb * ROWS + r0 + r;
-            if (d < hd) a.out[(size_t)tail.b * a.ldo + (size_t)h * hd + d] = L == 0.0f ? 0.0f : __fdiv_rn(O, L);
-            if (G::STAT && work.stat && d == 0)
-                work.stat[(size_t)tail.b * a.H + h] = make_float2(M, L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L));
+            if (d < hd)
+                a.out[(size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + r0 + r) * hd + d] =
+                    L == 0.0f ? 0.0f : __fdiv_rn(O, L);
+        }
+    }
+}
+
+// The same for teams, whose items go through more CTAs: a CTA of kPaWideThreads threads for each item and row of the
+// team. A warp per query row finds the reference and the parts' factors, then every thread adds four dims of a row over its
+// share of the parts, kPaWideLoads of them in flight, and the shares are added in shared memory (131072 keys of 8 x 128, 148
+// parts: TODO).
+constexpr int kPaWideThreads = 512, kPaWideLoads = 8, kPaMaxCtas = 256;
+template <class G>
+__global__ void __launch_bounds__(kPaWideThreads) paged_join_wide_kernel(typename G::Args a, PaPlan pl, PaWork work) {
+    constexpr int HDP = G::HDP, ROWS = G::ROWS, COLS = ROWS * HDP / 4;
+    constexpr int SIDE = COLS < kPaWideThreads ? kPaWideThreads / COLS : 1, STEP = COLS < kPaWideThreads ? COLS : kPaWideThreads;
+    __shared__ float s_f[ROWS][kPaMaxCtas], s_l[ROWS];
+    __shared__ __align__(16) float4 s_o[kPaWideThreads];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
+    if (G::STAT) griddep_launch();
+    griddep_wait();
+    const PaTail tail = work.tail[blockIdx.x];
+    if (tail.ctas == 0) return;
+    const int team = pa_team<G>(pl), member = blockIdx.y, item = tail.r * team + member;
+    const int np = tail.ctas + 1, qb = item % pl.qblocks, kvh = item / pl.qblocks, rows = min(ROWS, group - qb * ROWS);
+    auto part = [&](int i) {
+        return work.part + (size_t)((i == 0 ? tail.slot : ((int)blockIdx.x + i) * tail.per_cta * team * 2) + member * 2) * G::PART;
+    };
+    for (int row = warp; row < rows; row += kPaWideThreads / 32) {
+        float M = kPaLow, L = 0.0f;
+        float2 rl[kPaMaxCtas / 32];
+#pragma unroll
+        for (int k = 0; k < kPaMaxCtas / 32; k++) {
+            const int i = lane + 32 * k;
+            rl[k] = i < np ? *reinterpret_cast<const float2*>(part(i) + ROWS * HDP + 2 * row) : make_float2(kPaLow, 0.0f);
+            M = fmaxf(M, rl[k].x);
+        }
+        M = warp_max(M);
+#pragma unroll
+        for (int k = 0; k < kPaMaxCtas / 32; k++) {
+            const float f = ex2(rl[k].x - M);
+            if (lane + 32 * k < np) s_f[row][lane + 32 * k] = f;
+            L = __fmaf_rn(rl[k].y, f, L);
+        }
+        L = warp_sum(L);
+        if (lane == 0) {
+            const int h = kvh * group + qb * ROWS + row;
+            s_l[row] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+            if (G::STAT && work.stat) work.stat[(size_t)tail.b * a.H + h] = make_float2(M, s_l[row]);
+        }
+    }
+    __syncthreads();
+    for (int c0 = 0; c0 < COLS; c0 += STEP) {
+        const int col = c0 + tid % STEP, side = tid / STEP, row = col / (HDP / 4), d = col % (HDP / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool live = row < rows && side < SIDE;
+        if (live)
+            for (int i0 = side; i0 < np; i0 += SIDE * kPaWideLoads) {
+                float4 x[kPaWideLoads];
+#pragma unroll
+                for (int k = 0; k < kPaWideLoads; k++)
+                    x[k] = i0 + SIDE * k < np ? *reinterpret_cast<const float4*>(part(i0 + SIDE * k) + row * HDP + d)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < kPaWideLoads; k++) {
+                    const float f = i0 + SIDE * k < np ? s_f[row][i0 + SIDE * k] : 0.0f;
+                    o = make_float4(__fmaf_rn(x[k].x, f, o.x), __fmaf_rn(x[k].y, f, o.y), __fmaf_rn(x[k].z, f, o.z),
+                                    __fmaf_rn(x[k].w, f, o.w));
+                }
+            }
+        if (SIDE > 1) {
+            s_o[tid] = o;
+            __syncthreads();
+            for (int w = 1; side == 0 && w < SIDE; w++) {
+                const float4 x = s_o[w * STEP + tid];
+                o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+            }
+        }
+        if (live && side == 0 && d < hd) {
+            float* to = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd + d;
+            const float inv = s_l[row];
+            to[0] = o.x * inv;
+            to[1] = o.y * inv;
+            to[2] = o.z * inv;
+            to[3] = o.w * inv;
         }
     }
 }
