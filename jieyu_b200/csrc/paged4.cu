@@ -310,9 +310,58 @@ __device__ __forceinline__ void p4_copy(uint32_t dst, const void* src) {
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 
+// Queries as the kernel below reads them, one of these per sequence and head: 32 GP bytes, for every group the word
+// (0, multiple of 4 beyond its sum) and the word (0, what that has too much) as halves, then the scale in base 2.
+// |sum| <= 4064: both are halves, and as they differ in sign a lowest value that is not finite gives NaN.
+__host__ __device__ constexpr int p4_query_bytes(int gp) { return 40 * gp + 16; }
+
+// A warp turns and quantises one query head: lane j holds dims 4 j .. 4 j + 3 of every 128. (In the attention kernel
+// itself this took 7 of the first 10 us of every run, for the instructions of all forms of the rotation; here it runs
+// while that kernel finds its runs and requests its first keys.)
+__global__ void __launch_bounds__(128) paged4_query_kernel(PagedAttn4 a, int gp, bool wide_q, bool wide_rope, unsigned char* out) {
+    griddep_launch();
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, b = (int)(i / a.H), h = (int)(i - (long long)b * a.H);
+    if (b >= a.kv.num_seqs) return;
+    const int len = p4_len(a, b);
+    if (len == 0) return;  // no one reads its queries
+    const float* q = a.Q + (size_t)b * a.ldq + (size_t)h * a.hd;
+    const int pos = a.rope.cos_t ? (a.rope_pos ? __ldg(a.rope_pos + b) : len - 1) : 0;
+    float4 x[2];
+    float amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = 128 * k + 4 * lane;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < a.hd) x[k] = a.rope.cos_t ? turned4(q, d, a.rope, pos, wide_rope) : p4_load4(q + d, wide_q);
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[k].x), fabsf(x[k].y))), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+    }
+    amax = warp_max(amax);
+    const float inv = q8_inv(amax);
+    unsigned char* const to = out + (size_t)i * p4_query_bytes(gp);
+    uint32_t* const sums = reinterpret_cast<uint32_t*>(to + 32 * gp);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t w = (uint32_t)(q8_round(x[k].x, inv) & 255) | (uint32_t)(q8_round(x[k].y, inv) & 255) << 8 |
+                           (uint32_t)(q8_round(x[k].z, inv) & 255) << 16 | (uint32_t)q8_round(x[k].w, inv) << 24;
+        int sum = __dp4a((int)w, 0x01010101, 0);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int group = 4 * k + (lane >> 3);
+        if (group >= gp) continue;
+        reinterpret_cast<uint32_t*>(to)[32 * k + lane] = w;
+        if ((lane & 7) == 0) {
+            const int hi = sum >= 0 ? (sum & ~3) + 4 : -((-sum & ~3) + 4);
+            sums[group] = (uint32_t)__half_as_ushort(__int2half_rn(hi)) << 16;
+            sums[gp + group] = (uint32_t)__half_as_ushort(__int2half_rn(sum - hi)) << 16;
+        }
+    }
+    if (lane == 0) reinterpret_cast<float*>(sums + 2 * gp)[0] = __fmul_rn(q8_scale(amax), __fmul_rn(a.scale, 1.44269504088896341f));
+}
+
 template <int GP, int HEADS, bool TMA>
 __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
-    paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, int param_copy,
+    paged4_attention_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores, const unsigned char* queries, int param_copy,
                             const __grid_constant__ P4Maps maps) {
     using G = P4Cfg<GP, HEADS, TMA>;
     constexpr int TK = G::TK, U = G::U, ST = G::ST, ROWS = G::ROWS, E = G::E, ND = 2 * GP, PW = G::PW, LW = PW / 4;
@@ -465,22 +514,20 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     bool gave_up = false;
     int st = 0;
     uint32_t phase = 0u;
-    const float up = __fmul_rn(a.scale, 1.44269504088896341f);
+    if (count > 0) {
+        lookup();
+#pragma unroll 1
+        for (int i = 0; i < (TMA ? ST : ST - 1); i++) {
+            issue(i);
+            lookup();
+        }
+    }
+    griddep_wait();  // the queries
 
     for (int n = 0; n < count; n++) {
         if (fresh) {
-            // the item's query heads: turned and quantised per head
             fresh = false;
-            if (n == 0) {
-                lookup();
-#pragma unroll 1
-                for (int i = 0; i < (TMA ? ST : ST - 1); i++) {
-                    issue(i);
-                    lookup();
-                }
-            }
             const int r = pa_row<G>(pl, cur), qb = r % pl.qblocks, kvh = r / pl.qblocks;
-            const int pos = a.rope.cos_t ? (a.rope_pos ? __ldg(a.rope_pos + cur.b) : cur.len - 1) : 0;
 #pragma unroll
             for (int i = 0; i < GP; i++) {
                 eg[i] = 0;
@@ -488,47 +535,20 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             }
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const int row = qb * ROWS + 8 * e + (HEADS <= 4 ? g & 3 : g);
-                const bool live = row < group;
-                const float* q = a.Q + (size_t)cur.b * a.ldq + (size_t)(kvh * group + (live ? row : 0)) * hd;
-                float4 x[2 * GP];
-                float amax = 0.0f;
+                const int row = qb * ROWS + 8 * e + (HEADS <= 4 ? g & 3 : g), own = qb * ROWS + 8 * e + 2 * t;
+                const unsigned char* const at = queries + ((size_t)cur.b * a.H + (size_t)kvh * group) * p4_query_bytes(GP);
+                const uint32_t* const q = reinterpret_cast<const uint32_t*>(at + (size_t)row * p4_query_bytes(GP));
 #pragma unroll
-                for (int i = 0; i < 2 * GP; i++) {
-                    const int d = 16 * i + 4 * t;
-                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (live && d < hd) x[i] = a.rope.cos_t ? turned4(q, d, a.rope, pos, pl.wide_rope) : p4_load4(q + d, pl.wide_q);
-                }
+                for (int i = 0; i < 2 * GP; i++) qf[i >> 1][e][i & 1] = row < group ? __ldcg(q + 4 * i + t) : 0u;
 #pragma unroll
-                for (int i = 0; i < 2 * GP; i++)
-                    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const float inv = q8_inv(amax), sc = __fmul_rn(q8_scale(amax), up);
-#pragma unroll
-                for (int i = 0; i < 2 * GP; i++) {
-                    const uint32_t b = (uint32_t)(q8_round(x[i].x, inv) & 255) | (uint32_t)(q8_round(x[i].y, inv) & 255) << 8 |
-                                       (uint32_t)(q8_round(x[i].z, inv) & 255) << 16 | (uint32_t)q8_round(x[i].w, inv) << 24;
-                    qf[i >> 1][e][i & 1] = b;
-                }
-#pragma unroll
-                for (int i = 0; i < 2 * LW; i++) qsum[e][i] = 0u;
-#pragma unroll
-                for (int i = 0; i < GP; i++) {
-                    int sum = __dp4a((int)qf[i][e][1], 0x01010101, __dp4a((int)qf[i][e][0], 0x01010101, 0));
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    // |sum| <= 4064 as a multiple of 4 beyond it and what that has too much, of the other sign: both are
-                    // halves, and a lowest value that is not finite gives NaN
-                    const int hi = sum >= 0 ? (sum & ~3) + 4 : -((-sum & ~3) + 4);
-                    if ((i & 3) == t) {
-                        qsum[e][i >> 2] = (uint32_t)__half_as_ushort(__int2half_rn(hi)) << 16;
-                        qsum[e][LW + (i >> 2)] = (uint32_t)__half_as_ushort(__int2half_rn(sum - hi)) << 16;
-                    }
+                for (int i = 0; i < 2 * LW; i++) {
+                    const int k = 4 * (i % LW) + t;
+                    qsum[e][i] = row < group && k < GP ? __ldcg(q + 8 * GP + (i / LW) * GP + k) : 0u;
                 }
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    qsl[e][i] = __shfl_sync(0xffffffffu, sc, 4 * (2 * t + i));
+                    const int head = HEADS <= 4 ? qb * ROWS + (2 * t + i & 3) : own + i;
+                    qsl[e][i] = head < group ? __ldcg(reinterpret_cast<const float*>(at + (size_t)head * p4_query_bytes(GP) + 40 * GP)) : 0.0f;
                     ref[e][i] = kPaLow;
                     l[e][i] = 0.0f;
                 }
@@ -928,32 +948,33 @@ __global__ void __launch_bounds__(kP4MassThreads) paged4_mass_kernel(PagedAttn4 
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
-// The workspace of one call: tails, parts, and where weights are gathered stat and scores.
+// The workspace of one call: tails, parts, queries, and where weights are gathered stat and scores.
 template <int GP, int HEADS, bool TMA>
-size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* base, PaWork* w, P4Scores* sc) {
+size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* base, PaWork* w, P4Scores* sc,
+               unsigned char** queries) {
     using G = P4Cfg<GP, HEADS, TMA>;
     const int qblocks = (H / KV + HEADS - 1) / HEADS;
     const size_t parts = align16(ctas * sizeof(PaTail));
-    const size_t stat = align16(parts + (size_t)ctas * G::WARPS * 2 * G::PART * sizeof(float));
-    if (capacity == 0) {
-        if (w) *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts), nullptr};
-        if (sc) *sc = P4Scores{nullptr, 0};
-        return stat;
-    }
-    const size_t score = align16(stat + (size_t)seqs * H * sizeof(float2));
+    const size_t query = align16(parts + (size_t)ctas * G::WARPS * 2 * G::PART * sizeof(float));
+    const size_t stat = align16(query + (size_t)seqs * H * p4_query_bytes(GP));
+    const size_t score = align16(stat + (capacity ? (size_t)seqs * H * sizeof(float2) : 0));
     const long long keys = ((long long)capacity + G::TK - 1) / G::TK * G::TK * HEADS;
-    if (w)
-        *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts), reinterpret_cast<float2*>(base + stat)};
-    if (sc) *sc = P4Scores{reinterpret_cast<float*>(base + score), keys};
+    if (base) {
+        *w = PaWork{reinterpret_cast<PaTail*>(base), reinterpret_cast<float*>(base + parts),
+                    capacity ? reinterpret_cast<float2*>(base + stat) : nullptr};
+        *queries = base + query;
+        *sc = P4Scores{capacity ? reinterpret_cast<float*>(base + score) : nullptr, keys};
+    }
     return score + (size_t)seqs * KV * qblocks * keys * sizeof(float);
 }
 
 // A launch behind the last one, which it waits for by itself.
 template <class... Params, class... Args>
-int p4_follow(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t s, Args... args) {
+int p4_follow(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1018,18 +1039,24 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     }
     PaWork w;
     P4Scores sc;
-    p4_work<GP, HEADS, TMA>(sms, a.kv.num_seqs, a.H, a.KV, p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc);
+    unsigned char* queries;
+    p4_work<GP, HEADS, TMA>(sms, a.kv.num_seqs, a.H, a.KV, p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc,
+                            &queries);
+    const long long rows = (long long)a.kv.num_seqs * a.H;
+    paged4_query_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a, GP, pl.wide_q, pl.wide_rope, queries);
+    JYC_LAUNCHED();
     // a key's parameters by one copy where their alignment allows it, else word by word
     const uintptr_t at = (uintptr_t)p.kp | (uintptr_t)p.vp | (uintptr_t)(4 * (p.ppage_stride | p.ppos_stride | p.phead_stride));
     const int copy = groups == GP && at % (4 * GP) == 0 ? 4 * GP : 4;
-    paged4_attention_kernel<GP, HEADS, TMA><<<ctas, G::WARPS * 32, G::SMEM, s>>>(a, pl, w, sc, copy, maps);
-    JYC_LAUNCHED();
+    if (int e = p4_follow(paged4_attention_kernel<GP, HEADS, TMA>, dim3(ctas), G::WARPS * 32, G::SMEM, s, a, pl, w, sc,
+                          (const unsigned char*)queries, copy, maps))
+        return e;
     if (tiles > 1)  // else an item is one unit: none is split
-        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, pl.team), kPaWideThreads, s, a, pl, w)) return e;
+        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, pl.team), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
     const unsigned chunks = (unsigned)std::min({most, (8LL * sms + heads - 1) / heads, 65535LL});
-    return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, s, a, pl, w, sc);
+    return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
 }
 
 // The instantiation of a shape: groups and query heads per unit rounded up.
@@ -1332,7 +1359,7 @@ int launch_paged4_read(float* K, float* V, int ld, int rows, int KV, int hd, con
 
 template <int GP, int HEADS, bool TMA>
 static size_t p4_workspace(int sms, int seqs, int H, int KV, int capacity) {
-    return p4_work<GP, HEADS, TMA>(sms, seqs, H, KV, capacity, nullptr, nullptr, nullptr);
+    return p4_work<GP, HEADS, TMA>(sms, seqs, H, KV, capacity, nullptr, nullptr, nullptr, nullptr);
 }
 
 size_t paged4_attention_workspace(int seqs, int H, int KV, int hd, int capacity) {
@@ -1375,7 +1402,7 @@ int launch_paged4_evict(const PagedEvict4& e, cudaStream_t s) {
     const int groups = (e.hd + 31) / 32, lanes = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
     const long long rows = (long long)items * e.budget, per = (long long)kMvThreads / lanes * kMvRows;
     const auto kernel = lanes == 1 ? paged4_move_kernel<1> : lanes == 2 ? paged4_move_kernel<2> : lanes == 4 ? paged4_move_kernel<4> : paged4_move_kernel<8>;
-    return p4_follow(kernel, dim3((unsigned)((rows + per - 1) / per)), kMvThreads, s, e, fast_div(e.budget), fast_div(e.KV),
+    return p4_follow(kernel, dim3((unsigned)((rows + per - 1) / per)), kMvThreads, 0, s, e, fast_div(e.budget), fast_div(e.KV),
                      e.kv.by_page);
 }
 
