@@ -240,18 +240,12 @@ struct P4Cfg {
     using Args = PagedAttn4;
     static __device__ __forceinline__ int len(const PagedAttn4& a, int b) { return p4_len(a, b); }
     static constexpr bool STAT = true, TEAM = true;
-#ifndef P4W
-#define P4W 8
-#define P4ST 2
-#define P4U 2
-#define P4W2 8
-#define P4ST2 3
-#define P4U2 2
-#endif
-    static constexpr int U = GP <= 2 ? P4U2 : GP <= 4 ? P4U : 1;  // keys of a lane
-    static constexpr int HDP = 32 * GP, TK = 32 * U;              // keys of a unit
-    static constexpr int WARPS = GP <= 2 ? P4W2 : GP <= 4 ? P4W : 8;
-    static constexpr int ST = GP <= 2 ? P4ST2 : GP <= 4 ? P4ST : GP <= 6 ? 3 : 2;
+    static constexpr int U = GP <= 4 ? 2 : 1;         // keys of a lane
+    static constexpr int HDP = 32 * GP, TK = 32 * U;  // keys of a unit
+    // 131072 keys of 8 x 128: 60 us with 8 warps of 2 stages of 64 keys, 62 with 12 of 3 of 32, 71 with 16 of 2; 64 sequences
+    // of 2112 keys of 8 x 64: 49 us with 12 warps, 55 with 8
+    static constexpr int WARPS = GP <= 2 ? 12 : 8;
+    static constexpr int ST = GP == 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
     static constexpr int ROWS = HEADS;
     // rows of K and V: tensor copies swizzle their 16-byte chunks, else an odd number of chunks, so that the 8 rows of an
