@@ -78,6 +78,18 @@ __device__ __forceinline__ void i8_tmem_ld16(uint32_t ta, int* r) {
         : "r"(ta)
         : "memory");
 }
+__device__ __forceinline__ void i8_tmem_ld32(uint32_t ta, int* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(ta)
+        : "memory");
+}
 __device__ __forceinline__ void i8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -85,6 +97,20 @@ __device__ __forceinline__ void i8_cluster_sync() {
 __device__ __forceinline__ float i8_out(int sum, float as, float ws, bool add, float bias) {
     const float v = __fmul_rn(__int2float_rn(sum), __fmul_rn(as, ws));
     return add ? __fadd_rn(v, bias) : v;
+}
+
+// 32 tokens of this lane's channel, all of which exist
+template <bool BIAS>
+__device__ __forceinline__ void i8_store32(const int* v, const float* as, float ws, float bias, float* to, int ldc) {
+#pragma unroll
+    for (int u = 0; u < 32; u += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(as + u);
+        __stcs(to, i8_out(v[u], a.x, ws, BIAS, bias));
+        __stcs(to += ldc, i8_out(v[u + 1], a.y, ws, BIAS, bias));
+        __stcs(to += ldc, i8_out(v[u + 2], a.z, ws, BIAS, bias));
+        __stcs(to += ldc, i8_out(v[u + 3], a.w, ws, BIAS, bias));
+        to += ldc;
+    }
 }
 
 struct I8Maps {
@@ -104,42 +130,76 @@ struct I8Wait {
     }
 };
 
-// Many tiles: one CTA per SM takes every gridDim.x-th tile of 128 channels x BN tokens, tokens first. Two accumulators: a
-// tile's results leave while the next one's products run.
-template <int BN>
-struct I8Big {
-    static constexpr int kStage = kI8Rows * kI8Chunk + BN * kI8Chunk, kStages = 4;
-    static constexpr int kSmem = 1024 + kStages * kStage;
-};
-template <int BN>
-__global__ void __launch_bounds__(kI8Threads, 1) i8_big_kernel(I8Gemm g, const __grid_constant__ I8Maps maps, int* err) {
-    using C = I8Big<BN>;
+// Many tiles: a pair of CTAs (a cluster of 2) takes every pair-count-th tile of 256 channels x 256 tokens, tokens first.
+// Each CTA holds 128 of the channels and copies 128 of the tokens; the pair's products (cta_group::2, issued by the first
+// CTA) read both halves of the tokens, so that a CTA brings 32 KB for what one alone would need 48 KB for. Two
+// accumulators: a tile's results leave while the next one's products run.
+constexpr int kI8PairTokens = 256, kI8PairStages = 6, kI8PairThreads = 320;
+constexpr int kI8PairStage = (kI8Rows + kI8PairTokens / 2) * kI8Chunk, kI8PairSmem = 1024 + kI8PairStages * kI8PairStage;
+
+__device__ __forceinline__ void i8_pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrives on `bar` of both CTAs when every product this thread issued so far has completed
+__device__ __forceinline__ void i8_pair_commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// address of the first CTA's copy of a shared variable
+__device__ __forceinline__ uint32_t i8_lead(const void* p) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(p)));
+    return at;
+}
+// box -> this CTA's shared memory, its bytes counted by the first CTA's barrier
+__device__ __forceinline__ void i8_pair_copy(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+__global__ void __launch_bounds__(kI8PairThreads, 1) i8_pair_kernel(I8Gemm g, const __grid_constant__ I8Maps maps, int* err) {
+    constexpr int BN = kI8PairTokens, ST = kI8PairStages;
+    constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(2 * kI8Rows >> 4) << 24);
     extern __shared__ unsigned char i8_raw[];
-    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], accf[2], acce[2];
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], accf[2], acce[2];  // full and acce: the first CTA's are used
     __shared__ uint32_t s_tmem;
+    __shared__ __align__(16) float s_as[8][BN / 2];
     __shared__ int s_abort;
     unsigned char* const sm = i8_raw + (-smem_u32(i8_raw) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tt = (g.m + BN - 1) / BN, tiles = (g.n + kI8Rows - 1) / kI8Rows * tt, nch = (g.k + kI8Chunk - 1) / kI8Chunk;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1, pairs = gridDim.x >> 1;
+    const int tt = (g.m + BN - 1) / BN, tiles = (g.n + 2 * kI8Rows - 1) / (2 * kI8Rows) * tt;
+    const int nch = (g.k + kI8Chunk - 1) / kI8Chunk;
     const I8Wait wait{err, &s_abort};
     if (tid == 0) {
-        for (int s = 0; s < C::kStages; s++) {
+        for (int s = 0; s < ST; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], 128);
+            mbar_init(&acce[b], 2 * (kI8PairThreads - 64));
         }
         s_abort = 0;
         mbar_fence_init();
     }
     if (warp == 0) {
         __syncwarp();
-        tmem_alloc(&s_tmem, 2 * BN);
+        tmem_alloc_pair(&s_tmem, 2 * BN);
     }
     tc_fence_before();
     __syncthreads();
+    i8_cluster_sync();  // the other CTA's barriers are there
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     griddep_wait();
@@ -148,73 +208,88 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_big_kernel(I8Gemm g, const _
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
+            for (int tile = blockIdx.x >> 1; ok && tile < tiles; tile += pairs)
                 for (int c = 0; c < nch; c++, it++) {
-                    const int s = it % C::kStages;
-                    if (it >= C::kStages && !(ok = wait(&empty[s], ((it / C::kStages) - 1) & 1))) break;
-                    mbar_expect_tx(&full[s], C::kStage);
-                    i8_copy(sm + s * C::kStage, &maps.w, c * kI8Chunk, tile / tt * kI8Rows, &full[s]);
-                    i8_copy(sm + s * C::kStage + kI8Rows * kI8Chunk, &maps.a, c * kI8Chunk, tile % tt * BN, &full[s]);
+                    const int s = it % ST;
+                    if (it >= ST && !(ok = wait(&empty[s], ((it / ST) - 1) & 1))) break;
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * kI8PairStage);
+                    const uint32_t bar = i8_lead(&full[s]);
+                    unsigned char* const st = sm + s * kI8PairStage;
+                    i8_pair_copy(st, &maps.w, c * kI8Chunk, (tile / tt * 2 + rank) * kI8Rows, bar);
+                    i8_pair_copy(st + kI8Rows * kI8Chunk, &maps.a, c * kI8Chunk, tile % tt * BN + rank * (BN / 2), bar);
                 }
-            // no copy may still be landing when the CTA exits (matters only after an error)
-            for (int j = max(0, it - C::kStages); j < it; j++)
-                mbar_wait_err(&full[j % C::kStages], (j / C::kStages) & 1, err, kErrI8);
+            // no copy may still be landing when the CTAs exit (matters only after an error)
+            if (rank == 0)
+                for (int j = max(0, it - ST); j < it; j++) mbar_wait_err(&full[j % ST], (j / ST) & 1, err, kErrI8);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int it = 0, i = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, i++) {
+            for (int tile = blockIdx.x >> 1; ok && tile < tiles; tile += pairs, i++) {
                 const int b = i & 1;
                 if (i >= 2 && !(ok = wait(&acce[b], ((i >> 1) - 1) & 1))) break;
                 tc_fence_after();
                 for (int c = 0; c < nch; c++, it++) {
-                    const int s = it % C::kStages;
-                    if (!(ok = wait(&full[s], (it / C::kStages) & 1))) break;
+                    const int s = it % ST;
+                    if (!(ok = wait(&full[s], (it / ST) & 1))) break;
                     tc_fence_after();
-                    const uint32_t st = smem_u32(sm + s * C::kStage);
+                    const uint32_t st = smem_u32(sm + s * kI8PairStage);
                     const uint64_t w = sw128_desc(st), a = sw128_desc(st + kI8Rows * kI8Chunk);
 #pragma unroll
                     for (int k = 0; k < kI8Chunk / 32; k++)  // 32 bytes of K, in 16-byte units
-                        i8_mma(tmem + (uint32_t)(BN * b), w + 2 * k, a + 2 * k, i8_idesc(BN), c != 0 || k != 0);
-                    tc_commit(&empty[s]);
+                        i8_pair_mma(tmem + (uint32_t)(BN * b), w + 2 * k, a + 2 * k, idesc, c != 0 || k != 0);
+                    i8_pair_commit(&empty[s]);
                 }
-                if (ok) tc_commit(&accf[b]);
+                if (ok) i8_pair_commit(&accf[b]);
             }
         }
     } else {
-        const int q = warp & 3;
+        // eight warps: 32 channels and half of the tokens each
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        float* const as = s_as[warp - 2];
         int i = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, i++) {
-            const int b = i & 1, j = tile / tt * kI8Rows + 32 * q + lane, t0 = tile % tt * BN;
+        for (int tile = blockIdx.x >> 1; tile < tiles; tile += pairs, i++) {
+            const int b = i & 1, j = (tile / tt * 2 + rank) * kI8Rows + 32 * q + lane, t0 = tile % tt * BN + half * (BN / 2);
             const bool col = j < g.n;
             const float ws = col ? __ldg(g.ws + j) : 0.0f, bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < BN / 2; c += 32) as[c + lane] = t0 + c + lane < g.m ? __ldg(g.as + t0 + c + lane) : 0.0f;
+            __syncwarp();
             if (!__all_sync(0xffffffffu, wait(&accf[b], (i >> 1) & 1))) break;
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(BN * b);
+            const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(BN * b + half * (BN / 2));
+            float* to = g.C + (size_t)t0 * g.ldc + j;
+            const int live = min(BN / 2, g.m - t0);
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                int v[16];
-                i8_tmem_ld16(ta + c, v);
-                const int t = t0 + c + (lane & 15);
-                const float as = t < g.m ? __ldg(g.as + t) : 0.0f;
-                float* to = g.C + (size_t)(t0 + c) * g.ldc + j;
-#pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    const float y = i8_out(v[u], __shfl_sync(0xffffffffu, as, u), ws, g.bias != nullptr, bias);
-                    if (col && t0 + c + u < g.m) to[(size_t)u * g.ldc] = y;
+            for (int c = 0; c < live; c += 32) {
+                int v[32];
+                i8_tmem_ld32(ta + c, v);
+                if (c + 32 <= live && __all_sync(0xffffffffu, col)) {
+                    if (g.bias)
+                        i8_store32<true>(v, as + c, ws, bias, to, g.ldc);
+                    else
+                        i8_store32<false>(v, as + c, ws, bias, to, g.ldc);
+                    to += (size_t)32 * g.ldc;
+                    continue;
                 }
+#pragma unroll
+                for (int u = 0; u < 32; u++, to += g.ldc)
+                    if (col && c + u < live) *to = i8_out(v[u], as[c + u], ws, g.bias != nullptr, bias);
             }
             tc_fence_before();
-            mbar_arrive(&acce[b]);
+            const uint32_t bar = i8_lead(&acce[b]);
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
         }
     }
+    __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    i8_cluster_sync();  // neither CTA's memory goes while the other one uses it
     if (warp == 0) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        tmem_dealloc_pair(tmem, 2 * BN);
     }
 }
 
@@ -363,20 +438,20 @@ int i8_map(CUtensorMap* m, const int8_t* base, int rows, int k, int ld, int box)
 }
 
 template <class Kernel>
-int i8_start(Kernel kernel, const I8Gemm& g, const I8Maps& maps, dim3 grid, int cluster, int smem, cudaStream_t s) {
+int i8_start(Kernel kernel, const I8Gemm& g, const I8Maps& maps, dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t s) {
     if (int e = max_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kI8Threads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = 1;
-    at[1].val.clusterDim.y = 1;
-    at[1].val.clusterDim.z = cluster;
+    at[1].val.clusterDim.x = cluster.x;
+    at[1].val.clusterDim.y = cluster.y;
+    at[1].val.clusterDim.z = cluster.z;
     cfg.attrs = at;
     cfg.numAttrs = 2;
     JYC_CUDA(cudaLaunchKernelEx(&cfg, kernel, g, maps, device_error_word()));
@@ -391,8 +466,8 @@ int i8_few(const I8Gemm& g, I8Maps maps, int sms, cudaStream_t s) {
     const int chunks = (g.k + kI8Chunk - 1) / kI8Chunk;
     int parts = 1;
     while (parts < 8 && tiles * parts * 2 <= 2 * sms && chunks >= 4 * parts) parts *= 2;
-    return i8_start(i8_few_kernel<BN>, g, maps, dim3((g.n + kI8Rows - 1) / kI8Rows, (g.m + BN - 1) / BN, parts), parts,
-                    I8Few<BN>::kSmem, s);
+    return i8_start(i8_few_kernel<BN>, g, maps, dim3((g.n + kI8Rows - 1) / kI8Rows, (g.m + BN - 1) / BN, parts),
+                    dim3(1, 1, parts), kI8Threads, I8Few<BN>::kSmem, s);
 }
 
 }  // namespace
@@ -403,21 +478,31 @@ int launch_quantize_rows(const float* x, int ldx, int rows, int k, int8_t* q, in
     return JYC_OK;
 }
 
-int launch_i8_gemm(const I8Gemm& g, cudaStream_t s) {
+int launch_i8_gemm(const I8Gemm& all, cudaStream_t s) {
     const int sms = sm_count();
     if (sms == 0) return cuda_fail(cudaErrorNoDevice, "matmul_i8: device query");
+    I8Gemm g = all;
     I8Maps maps{};
     if (int e = i8_map(&maps.w, g.W, g.n, g.k, g.ldw, kI8Rows)) return e;
-    constexpr int BN = 256;
-    const long long tiles = (long long)((g.n + kI8Rows - 1) / kI8Rows) * ((g.m + BN - 1) / BN);
-    if (g.m > 128 && tiles * 2 > sms) {
-        if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, BN)) return e;
-        return i8_start(i8_big_kernel<BN>, g, maps, dim3((unsigned)std::min<long long>(tiles, sms)), 1, I8Big<BN>::kSmem, s);
+    const long long tiles = (long long)((g.n + 2 * kI8Rows - 1) / (2 * kI8Rows)) * ((g.m + kI8PairTokens - 1) / kI8PairTokens);
+    if (g.m > 128 && g.n > kI8Rows && tiles * 4 > sms) {
+        if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, kI8PairTokens / 2)) return e;
+        return i8_start(i8_pair_kernel, g, maps, dim3(2 * (unsigned)std::min<long long>(tiles, sms / 2)), dim3(2, 1, 1),
+                        kI8PairThreads, kI8PairSmem, s);
     }
     if (g.m <= 16) return i8_few<16>(g, maps, sms, s);
     if (g.m <= 32) return i8_few<32>(g, maps, sms, s);
     if (g.m <= 64) return i8_few<64>(g, maps, sms, s);
-    return i8_few<128>(g, maps, sms, s);
+    const int most = 65535 * 128;  // token tiles of a launch
+    for (int r0 = 0; r0 < all.m; r0 += most) {
+        g.A = all.A + (size_t)r0 * all.lda;
+        g.as = all.as + r0;
+        g.C = all.C + (size_t)r0 * all.ldc;
+        g.m = std::min(most, all.m - r0);
+        if (int e = i8_few<128>(g, maps, sms, s)) return e;
+        if (all.m - r0 <= most) break;
+    }
+    return JYC_OK;
 }
 
 }  // namespace jyc
