@@ -23,22 +23,59 @@ namespace {
 
 constexpr int kQrThreads = 256;
 
-// A CTA quantises one row: its maximum, then its values, read again.
+// A CTA quantises one row: its maximum, then its values. A thread holds up to QUADS quads of the row in registers, all
+// requested at once (QUADS 0: rows that are longer, or do not lie on 16 bytes, are read again, value by value).
+template <int QUADS>
 __global__ void __launch_bounds__(kQrThreads) quantize_rows_kernel(const float* x, int ldx, int k, int8_t* q, int ldq,
                                                                    float* scale) {
     __shared__ float s_max[kQrThreads / 32];
     const int tid = threadIdx.x;
+    griddep_launch();  // a product that follows may prepare itself
     const float* row = x + (size_t)blockIdx.x * ldx;
     int8_t* to = q + (size_t)blockIdx.x * ldq;
     float amax = 0.0f;
-    for (int i = tid; i < k; i += kQrThreads) amax = fmaxf(amax, fabsf(__ldg(row + i)));
+    float4 v[QUADS > 0 ? QUADS : 1];
+    if constexpr (QUADS > 0) {
+#pragma unroll
+        for (int i = 0; i < QUADS; i++) {
+            const int at = 4 * (tid + i * kQrThreads);
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at + 3 < k)
+                v[i] = __ldg(reinterpret_cast<const float4*>(row + at));
+            else if (at < k) {
+                v[i].x = __ldg(row + at);
+                if (at + 1 < k) v[i].y = __ldg(row + at + 1);
+                if (at + 2 < k) v[i].z = __ldg(row + at + 2);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < QUADS; i++)
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+    } else {
+        for (int i = tid; i < k; i += kQrThreads) amax = fmaxf(amax, fabsf(__ldg(row + i)));
+    }
     amax = warp_max(amax);
     if ((tid & 31) == 0) s_max[tid >> 5] = amax;
     __syncthreads();
     for (int w = 0; w < kQrThreads / 32; w++) amax = fmaxf(amax, s_max[w]);
     const float inv = q8_inv(amax);
     if (tid == 0) scale[blockIdx.x] = q8_scale(amax);
-    for (int i = tid; i < k; i += kQrThreads) to[i] = (int8_t)q8_round(__ldg(row + i), inv);
+    if constexpr (QUADS > 0) {
+#pragma unroll
+        for (int i = 0; i < QUADS; i++) {
+            const int at = 4 * (tid + i * kQrThreads);
+            const int b[4] = {q8_round(v[i].x, inv), q8_round(v[i].y, inv), q8_round(v[i].z, inv), q8_round(v[i].w, inv)};
+            if (at + 3 < k)
+                *reinterpret_cast<uint32_t*>(to + at) =
+                    __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            else
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    if (at + e < k) to[at + e] = (int8_t)b[e];
+        }
+    } else {
+        for (int i = tid; i < k; i += kQrThreads) to[i] = (int8_t)q8_round(__ldg(row + i), inv);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -99,11 +136,11 @@ __device__ __forceinline__ float i8_out(int sum, float as, float ws, bool add, f
     return add ? __fadd_rn(v, bias) : v;
 }
 
-// 32 tokens of this lane's channel, all of which exist
-template <bool BIAS>
-__device__ __forceinline__ void i8_store32(const int* v, const float* as, float ws, float bias, float* to, int ldc) {
+// N tokens of this lane's channel, all of which exist
+template <int N, bool BIAS>
+__device__ __forceinline__ void i8_store(const int* v, const float* as, float ws, float bias, float* to, int ldc) {
 #pragma unroll
-    for (int u = 0; u < 32; u += 4) {
+    for (int u = 0; u < N; u += 4) {
         const float4 a = *reinterpret_cast<const float4*>(as + u);
         __stcs(to, i8_out(v[u], a.x, ws, BIAS, bias));
         __stcs(to += ldc, i8_out(v[u + 1], a.y, ws, BIAS, bias));
@@ -112,10 +149,54 @@ __device__ __forceinline__ void i8_store32(const int* v, const float* as, float 
         to += ldc;
     }
 }
+// This warp's 32 channels of `live` tokens from tensor memory at ta, N at a time, to C; as: the tokens' scales in shared
+// memory. (One warp a scheduler at 20 instructions a result was what bounded the large product: 217 us, 177 with eight
+// warps and this form.)
+template <int N>
+__device__ __forceinline__ void i8_results(const I8Gemm& g, uint32_t ta, const float* as, int live, int j, float* to) {
+    const bool col = j < g.n, all = __all_sync(0xffffffffu, col);
+    const float ws = col ? __ldg(g.ws + j) : 0.0f, bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < live; c += N) {
+        int v[N];
+        if constexpr (N == 32)
+            i8_tmem_ld32(ta + c, v);
+        else
+            i8_tmem_ld16(ta + c, v);
+        if (c + N <= live && all) {
+            if (g.bias)
+                i8_store<N, true>(v, as + c, ws, bias, to, g.ldc);
+            else
+                i8_store<N, false>(v, as + c, ws, bias, to, g.ldc);
+            to += (size_t)N * g.ldc;
+            continue;
+        }
+#pragma unroll
+        for (int u = 0; u < N; u++, to += g.ldc)
+            if (col && c + u < live) *to = i8_out(v[u], as[c + u], ws, g.bias != nullptr, bias);
+    }
+}
+
+// four sums of CTA `rank` of the cluster at the address that they have here
+__device__ __forceinline__ int4 i8_far(uint32_t at, int rank) {
+    uint32_t far;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(far)
+                 : "memory");
+    return v;
+}
 
 struct I8Maps {
     CUtensorMap w, a;
 };
+
+__device__ __forceinline__ void i8_prefetch(const I8Maps& maps) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+}
 
 // Bounded waits of one CTA: after any of them gave up, every later one is skipped.
 struct I8Wait {
@@ -182,6 +263,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) i8_pair_kernel(I8Gemm g, co
     const int nch = (g.k + kI8Chunk - 1) / kI8Chunk;
     const I8Wait wait{err, &s_abort};
     if (tid == 0) {
+        i8_prefetch(maps);
         for (int s = 0; s < ST; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -251,33 +333,14 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) i8_pair_kernel(I8Gemm g, co
         int i = 0;
         for (int tile = blockIdx.x >> 1; tile < tiles; tile += pairs, i++) {
             const int b = i & 1, j = (tile / tt * 2 + rank) * kI8Rows + 32 * q + lane, t0 = tile % tt * BN + half * (BN / 2);
-            const bool col = j < g.n;
-            const float ws = col ? __ldg(g.ws + j) : 0.0f, bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < BN / 2; c += 32) as[c + lane] = t0 + c + lane < g.m ? __ldg(g.as + t0 + c + lane) : 0.0f;
             __syncwarp();
             if (!__all_sync(0xffffffffu, wait(&accf[b], (i >> 1) & 1))) break;
             tc_fence_after();
-            const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(BN * b + half * (BN / 2));
-            float* to = g.C + (size_t)t0 * g.ldc + j;
-            const int live = min(BN / 2, g.m - t0);
-#pragma unroll 1
-            for (int c = 0; c < live; c += 32) {
-                int v[32];
-                i8_tmem_ld32(ta + c, v);
-                if (c + 32 <= live && __all_sync(0xffffffffu, col)) {
-                    if (g.bias)
-                        i8_store32<true>(v, as + c, ws, bias, to, g.ldc);
-                    else
-                        i8_store32<false>(v, as + c, ws, bias, to, g.ldc);
-                    to += (size_t)32 * g.ldc;
-                    continue;
-                }
-#pragma unroll
-                for (int u = 0; u < 32; u++, to += g.ldc)
-                    if (col && c + u < live) *to = i8_out(v[u], as[c + u], ws, g.bias != nullptr, bias);
-            }
+            i8_results<32>(g, tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(BN * b + half * (BN / 2)), as,
+                           min(BN / 2, g.m - t0), j, g.C + (size_t)t0 * g.ldc + j);
             tc_fence_before();
             const uint32_t bar = i8_lead(&acce[b]);
             asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -309,6 +372,7 @@ __global__ void __launch_bounds__(kI8Threads) i8_few_kernel(I8Gemm g, const __gr
     extern __shared__ unsigned char i8_raw[];
     __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], accf;
     __shared__ uint32_t s_tmem;
+    __shared__ __align__(16) float s_as[4][BN];
     __shared__ int s_abort;
     unsigned char* const sm = i8_raw + (-smem_u32(i8_raw) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, parts = gridDim.z, z = blockIdx.z;
@@ -316,6 +380,7 @@ __global__ void __launch_bounds__(kI8Threads) i8_few_kernel(I8Gemm g, const __gr
     const int c0 = (int)((long long)chunks * z / parts), nch = (int)((long long)chunks * (z + 1) / parts) - c0;  // > 0
     const I8Wait wait{err, &s_abort};
     if (tid == 0) {
+        i8_prefetch(maps);
         for (int s = 0; s < C::kStages; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -364,51 +429,70 @@ __global__ void __launch_bounds__(kI8Threads) i8_few_kernel(I8Gemm g, const __gr
         }
     }
     int* const sums = reinterpret_cast<int*>(sm);  // [token][channel]; every product that read the stages is done
-    const int q = warp & 3, j = blockIdx.x * kI8Rows + 32 * q + lane, t0 = blockIdx.y * BN;
-    const bool col = j < g.n;
-    float ws = 0.0f, bias = 0.0f;
+    const int q = warp & 3, j0 = blockIdx.x * kI8Rows, t0 = blockIdx.y * BN, live = min(BN, g.m - t0);
     if (warp >= 2) {
-        ws = col ? __ldg(g.ws + j) : 0.0f;
-        bias = col && g.bias ? __ldg(g.bias + j) : 0.0f;
+        constexpr int N = BN < 32 ? 16 : 32;
+        float* const as = s_as[warp - 2];
+        for (int c = lane; c < live; c += 32) as[c] = __ldg(g.as + t0 + c);
+        __syncwarp();
         const bool ok = __all_sync(0xffffffffu, wait(&accf, 0));
         tc_fence_after();
         const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16);
-        if (ok)
+        if (ok && parts == 1) {
+            i8_results<N>(g, ta, as, live, j0 + 32 * q + lane, g.C + (size_t)t0 * g.ldc + j0 + 32 * q + lane);
+        } else if (ok) {
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                if (t0 + c >= g.m) break;
-                int v[16];
-                i8_tmem_ld16(ta + c, v);
-                if (parts > 1) {
+            for (int c = 0; c < live; c += N) {
+                int v[N];
+                if constexpr (N == 32)
+                    i8_tmem_ld32(ta + c, v);
+                else
+                    i8_tmem_ld16(ta + c, v);
 #pragma unroll
-                    for (int u = 0; u < 16; u++) sums[(c + u) * kI8Rows + 32 * q + lane] = v[u];
-                    continue;
-                }
-                const int t = t0 + c + (lane & 15);
-                const float as = t < g.m ? __ldg(g.as + t) : 0.0f;
-#pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    const float y = i8_out(v[u], __shfl_sync(0xffffffffu, as, u), ws, g.bias != nullptr, bias);
-                    if (col && t0 + c + u < g.m) g.C[(size_t)(t0 + c + u) * g.ldc + j] = y;
-                }
+                for (int u = 0; u < N; u++) sums[(c + u) * kI8Rows + 32 * q + lane] = v[u];
             }
+        }
     }
     if (parts > 1) {
         __syncwarp();
         i8_cluster_sync();
         if (warp >= 2) {
-            const int live = min(BN, g.m - t0), first = live * z / parts, last = live * (z + 1) / parts;
-            for (int t = first; t < last; t++) {
-                int sum = 0;
-                uint32_t at = smem_u32(sums + t * kI8Rows + 32 * q + lane);
-                for (int p = 0; p < parts; p++) {
-                    uint32_t far;
-                    int v;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(at), "r"(p));
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(far) : "memory");
-                    sum += v;
+            // a warp takes a token of this CTA's share, a lane four channels, all parts' sums of it in flight
+            const int j = j0 + 4 * lane, last = live * (z + 1) / parts;
+            const bool wide = j + 3 < g.n && (((uintptr_t)g.C | (uintptr_t)(4 * (long long)g.ldc)) & 15) == 0;
+            float ws[4], bias[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                ws[u] = j + u < g.n ? __ldg(g.ws + j + u) : 0.0f;
+                bias[u] = g.bias && j + u < g.n ? __ldg(g.bias + j + u) : 0.0f;
+            }
+            for (int t = live * z / parts + q; t < last; t += 4) {
+                const uint32_t at = smem_u32(sums + t * kI8Rows + 4 * lane);
+                int4 v[8];
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    v[p] = make_int4(0, 0, 0, 0);
+                    if (p < parts) v[p] = i8_far(at, p);
                 }
-                if (col) g.C[(size_t)(t0 + t) * g.ldc + j] = i8_out(sum, __ldg(g.as + t0 + t), ws, g.bias != nullptr, bias);
+                int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    sum[0] += v[p].x;
+                    sum[1] += v[p].y;
+                    sum[2] += v[p].z;
+                    sum[3] += v[p].w;
+                }
+                const float as = __ldg(g.as + t0 + t);
+                float y[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) y[u] = i8_out(sum[u], as, ws[u], g.bias != nullptr, bias[u]);
+                float* to = g.C + (size_t)(t0 + t) * g.ldc + j;
+                if (wide)
+                    *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                else
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        if (j + u < g.n) to[u] = y[u];
             }
         }
         __syncwarp();
@@ -464,8 +548,10 @@ int i8_few(const I8Gemm& g, I8Maps maps, int sms, cudaStream_t s) {
     if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, BN)) return e;
     const long long tiles = (long long)((g.n + kI8Rows - 1) / kI8Rows) * ((g.m + BN - 1) / BN);
     const int chunks = (g.k + kI8Chunk - 1) / kI8Chunk;
+    // parts of K: joining them costs about 3 us, so only where the tiles leave many SMs idle (32 tiles, 128 tokens of 4096 x
+    // 4096: TODO)
     int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 2 * sms && chunks >= 4 * parts) parts *= 2;
+    while (parts < 8 && tiles * 5 < 3 * sms && tiles * parts * 2 <= 2 * sms && chunks >= 4 * parts) parts *= 2;
     return i8_start(i8_few_kernel<BN>, g, maps, dim3((g.n + kI8Rows - 1) / kI8Rows, (g.m + BN - 1) / BN, parts),
                     dim3(1, 1, parts), kI8Threads, I8Few<BN>::kSmem, s);
 }
@@ -473,7 +559,13 @@ int i8_few(const I8Gemm& g, I8Maps maps, int sms, cudaStream_t s) {
 }  // namespace
 
 int launch_quantize_rows(const float* x, int ldx, int rows, int k, int8_t* q, int ldq, float* scale, cudaStream_t s) {
-    quantize_rows_kernel<<<rows, kQrThreads, 0, s>>>(x, ldx, k, q, ldq, scale);
+    const bool wide = aligned16(x, ldx) && ((uintptr_t)q & 3) == 0 && (ldq & 3) == 0;
+    const int quads = (k + 4 * kQrThreads - 1) / (4 * kQrThreads);
+    const auto kernel = !wide || quads > 16 ? quantize_rows_kernel<0>
+                        : quads <= 1        ? quantize_rows_kernel<1>
+                        : quads <= 4        ? quantize_rows_kernel<4>
+                                            : quantize_rows_kernel<16>;
+    kernel<<<rows, kQrThreads, 0, s>>>(x, ldx, k, q, ldq, scale);
     JYC_LAUNCHED();
     return JYC_OK;
 }
