@@ -61,16 +61,10 @@ __device__ __forceinline__ uint32_t p4_params(float lo, float hi) {
 }
 __device__ __forceinline__ float p4_step(uint32_t p) { return __half2float(__ushort_as_half((unsigned short)p)); }
 __device__ __forceinline__ float p4_low(uint32_t p) { return __half2float(__ushort_as_half((unsigned short)(p >> 16))); }
-__device__ __forceinline__ uint32_t p4_q(float x, float low, float inv) {
-    return (uint32_t)min(max(__float2int_rn(__fmul_rn(__fsub_rn(x, low), inv)), 0), 15);
-}
-
 // ---------------------------------------------------------------------------
-// Append and read back: a warp takes kP4Units * (32 / LANES) heads of K or of V
-// of one row. LANES lanes hold a head, QUADS quads of dims each; a group of 32
-// dims is 8 neighbouring lanes, so its range is three exchanges and its 16 bytes
-// four words of the lower four lanes (whose high bits come from the upper four).
-constexpr int kP4Units = 4, kP4Threads = 128;
+// Append and read back: a warp takes UNITS * (32 / LANES) heads of K or of V of one
+// row, the loads of all units in flight. The bookkeeping of a row is shared.
+constexpr int kP4Threads = 128;
 
 struct P4Row {
     int row, head;  // first head of this lane
@@ -78,7 +72,7 @@ struct P4Row {
     int page, slot;  // page: as p4_entry returns it, -1: nothing to do
     int pos;
 };
-template <int LANES>
+template <int LANES, int UNITS>
 __device__ __forceinline__ P4Row p4_row(int rows, int chunks, const FastDiv& by_row, const int* row_seq,
                                         const int* row_pos, const PagedKV4& kv) {
     const int w = blockIdx.x * (kP4Threads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -86,7 +80,7 @@ __device__ __forceinline__ P4Row p4_row(int rows, int chunks, const FastDiv& by_
     x.row = by_row(w);
     const int r = w - x.row * 2 * chunks;
     x.is_k = r < chunks;
-    x.head = (x.is_k ? r : r - chunks) * kP4Units * (32 / LANES) + lane / LANES;
+    x.head = (x.is_k ? r : r - chunks) * UNITS * (32 / LANES) + lane / LANES;
     x.page = -1;
     x.slot = 0;
     x.pos = -1;
@@ -97,18 +91,31 @@ __device__ __forceinline__ P4Row p4_row(int rows, int chunks, const FastDiv& by_
     return x;
 }
 
-template <int LANES, int QUADS>
+// four values as bytes 0 .. 15: held in range (a NaN as 0), then rounded by the sum with 1.5 * 2^23
+__device__ __forceinline__ uint32_t p4_bytes(float4 x, float low, float inv) {
+    auto q = [&](float v) {
+        return __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(v, low), inv), 0.0f), 15.0f), 12582912.0f));
+    };
+    return __byte_perm(__byte_perm(q(x.x), q(x.y), 0x0040), __byte_perm(q(x.z), q(x.w), 0x0040), 0x5410);
+}
+
+// Four lanes hold a group: lane i its dims 4 i .. 4 i + 3 and 16 more, whose numbers are the low and the high bits of its
+// word; the group's range is two exchanges. Pairs that lie on quads turn by table entries that a lane reads once for all
+// of its heads. (A lane with four dims needs three, and the high bits of another lane: 231
+// instructions a head of 128 and warp against 128, and the kernel is bound by them: 16384 rows of 8 x 128 TODO us.)
+enum { P4_PLAIN = 0, P4_PAIRS = 1, P4_HALVES = 2, P4_ODD = 3 };  // how K turns
+template <int LANES, int UNITS, int MODE>
 __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* K, const float* V, int ld, int rows,
                                                                    int KV, int hd, const int* row_seq,
                                                                    const int* row_pos, const int* rope_pos,
                                                                    PagedKV4 kv, RopeView rope, int chunks,
-                                                                   FastDiv by_row, bool vec, bool wide_rope) {
+                                                                   FastDiv by_row, bool vec) {
     constexpr int SIDE = 32 / LANES;
-    const int sub = threadIdx.x & (LANES - 1), nq = hd >> 2, groups = (hd + 31) >> 5;
-    const P4Row x = p4_row<LANES>(rows, chunks, by_row, row_seq, row_pos, kv);
+    const int sub = threadIdx.x & (LANES - 1), group = sub >> 2, d0 = 32 * group + 4 * (sub & 3), groups = (hd + 31) >> 5;
+    const P4Row x = p4_row<LANES, UNITS>(rows, chunks, by_row, row_seq, row_pos, kv);
     if (x.page == -1) return;
     int turn = x.pos;
-    if (rope.cos_t) {
+    if (MODE != P4_PLAIN) {
         // a row that cannot turn is not written: neither its K nor its V
         if (rope_pos) turn = __ldg(rope_pos + x.row);
         if (turn < 0 || turn >= rope.len) {
@@ -116,65 +123,107 @@ __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* 
             return;
         }
     }
-    const bool rot = rope.cos_t && x.is_k;
-    float4 v[kP4Units][QUADS];
+    const bool in0 = d0 < hd, in1 = d0 + 16 < hd;
+    float4 v[UNITS][2];
     const float* src = (x.is_k ? K : V) + (size_t)x.row * ld + (size_t)x.head * hd;
 #pragma unroll
-    for (int i = 0; i < kP4Units; i++)
+    for (int i = 0; i < UNITS; i++)
 #pragma unroll
-        for (int t = 0; t < QUADS; t++) {
-            const int qd = sub + LANES * t;
-            const float* head = src + i * SIDE * hd;
-            if (qd >= nq || x.head + i * SIDE >= KV)
-                v[i][t] = make_float4(0.f, 0.f, 0.f, 0.f);
-            else if (rot)
-                v[i][t] = turned4(head, 4 * qd, rope, turn, wide_rope);
+        for (int t = 0; t < 2; t++) {
+            const bool in = (t ? in1 : in0) && x.head + i * SIDE < KV;
+            const float* at = src + i * SIDE * hd + d0 + 16 * t;
+            v[i][t] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!in) continue;
+            if (MODE == P4_ODD && x.is_k)
+                v[i][t] = turned4(src + i * SIDE * hd, d0 + 16 * t, rope, turn, false);
             else
-                v[i][t] = p4_load4(head + 4 * qd, vec);
+                v[i][t] = p4_load4(at, MODE == P4_PAIRS || MODE == P4_HALVES || vec);
         }
+    if (MODE == P4_PAIRS && x.is_k) {
+        float2 c[2], sn[2];
+        const size_t tab = (size_t)turn * rope.half;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int d = d0 + 16 * t;
+            const bool use = d < 2 * rope.half;
+            c[t] = use ? __ldg(reinterpret_cast<const float2*>(rope.cos_t + tab + d / 2)) : make_float2(1.0f, 1.0f);
+            sn[t] = use ? __ldg(reinterpret_cast<const float2*>(rope.sin_t + tab + d / 2)) : make_float2(0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            if (d0 + 16 * t < 2 * rope.half)
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) {
+                    const float4 a = v[i][t];
+                    turn_pair(a.x, a.y, c[t].x, sn[t].x, v[i][t].x, v[i][t].y);
+                    turn_pair(a.z, a.w, c[t].y, sn[t].y, v[i][t].z, v[i][t].w);
+                }
+    }
+    if (MODE == P4_HALVES && x.is_k) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int d = d0 + 16 * t;
+            if (d >= 2 * rope.half) continue;
+            const bool first = d < rope.half;
+            const int other = first ? rope.half : -rope.half;
+            const size_t tab = (size_t)turn * rope.half + (first ? d : d - rope.half);
+            const float4 c = __ldg(reinterpret_cast<const float4*>(rope.cos_t + tab));
+            const float4 sn = __ldg(reinterpret_cast<const float4*>(rope.sin_t + tab));
+            float4 w[UNITS];
+#pragma unroll
+            for (int i = 0; i < UNITS; i++)
+                w[i] = x.head + i * SIDE < KV ? p4_load4(src + i * SIDE * hd + d + other, true) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const float4 a = first ? v[i][t] : w[i], b = first ? w[i] : v[i][t];
+                float4 r0, r1;
+                turn_pair(a.x, b.x, c.x, sn.x, r0.x, r1.x);
+                turn_pair(a.y, b.y, c.y, sn.y, r0.y, r1.y);
+                turn_pair(a.z, b.z, c.z, sn.z, r0.z, r1.z);
+                turn_pair(a.w, b.w, c.w, sn.w, r0.w, r1.w);
+                v[i][t] = first ? r0 : r1;
+            }
+        }
+    }
     if (!p4_valid(kv, x.page)) return;
-    uint8_t* dst = (x.is_k ? kv.p.k : kv.p.v) + p4_off(kv.p, x.page, x.slot, x.head);
-    uint32_t* par = reinterpret_cast<uint32_t*>(x.is_k ? kv.p.kp : kv.p.vp) + p4_poff(kv.p, x.page, x.slot, x.head);
+    uint8_t* dst = (x.is_k ? kv.p.k : kv.p.v) + p4_off(kv.p, x.page, x.slot, x.head) + 4 * sub;
+    uint32_t* par = reinterpret_cast<uint32_t*>(x.is_k ? kv.p.kp : kv.p.vp) + p4_poff(kv.p, x.page, x.slot, x.head) + group;
 #pragma unroll
-    for (int i = 0; i < kP4Units; i++) {
-        const bool live = x.head + i * SIDE < KV;
-#pragma unroll
-        for (int t = 0; t < QUADS; t++) {
-            const int qd = sub + LANES * t, group = qd >> 3;
-            const float4 a = v[i][t];
-            float lo = INFINITY, hi = -INFINITY;
-            if (qd < nq) {
-                lo = fminf(fminf(fminf(fminf(lo, a.x), a.y), a.z), a.w);
-                hi = fmaxf(fmaxf(fmaxf(fmaxf(hi, a.x), a.y), a.z), a.w);
-            }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            const uint32_t p = p4_params(lo, hi);
-            const float step = p4_step(p), low = p4_low(p), inv = step > 0.0f ? __fdiv_rn(1.0f, step) : 0.0f;
-            uint32_t w = 0u;
-            if (qd < nq)
-                w = p4_q(a.x, low, inv) | p4_q(a.y, low, inv) << 8 | p4_q(a.z, low, inv) << 16 | p4_q(a.w, low, inv) << 24;
-            const uint32_t up = __shfl_xor_sync(0xffffffffu, w, 4);
-            if (!live || group >= groups) continue;
-            if ((sub & 7) < 4)
-                *reinterpret_cast<uint32_t*>(dst + i * SIDE * kv.p.head_stride + 16 * group + 4 * (sub & 3)) = w | up << 4;
-            if ((sub & 7) == 0) par[i * SIDE * kv.p.phead_stride + group] = p;
+    for (int i = 0; i < UNITS; i++) {
+        const float4 a = v[i][0], c = v[i][1];
+        float lo = INFINITY, hi = -INFINITY;
+        if (in0) {
+            lo = fminf(fminf(a.x, a.y), fminf(a.z, a.w));
+            hi = fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w));
         }
-        if (live && x.is_k && sub == 0 && kv.p.mass)
-            kv.p.mass[p4_moff(kv.p, x.page, x.slot, x.head + i * SIDE)] = 0.0f;
+        if (in1) {
+            lo = fminf(lo, fminf(fminf(c.x, c.y), fminf(c.z, c.w)));
+            hi = fmaxf(hi, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const uint32_t p = p4_params(lo, hi);
+        const float step = p4_step(p), low = p4_low(p), inv = step > 0.0f ? __fdiv_rn(1.0f, step) : 0.0f;
+        const uint32_t w = (in0 ? p4_bytes(a, low, inv) : 0u) | (in1 ? p4_bytes(c, low, inv) << 4 : 0u);
+        if (x.head + i * SIDE >= KV || group >= groups) continue;
+        *reinterpret_cast<uint32_t*>(dst + i * SIDE * kv.p.head_stride) = w;
+        if ((sub & 3) == 0) par[i * SIDE * kv.p.phead_stride] = p;
+        if (x.is_k && sub == 0 && kv.p.mass) kv.p.mass[p4_moff(kv.p, x.page, x.slot, x.head + i * SIDE)] = 0.0f;
     }
 }
 
+// Eight neighbouring lanes read a group, two of them each word.
+constexpr int kP4Units = 4;
 template <int LANES, int QUADS>
 __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float* V, int ld, int rows, int KV, int hd,
                                                                  const int* row_seq, const int* row_pos, PagedKV4 kv,
                                                                  int chunks, FastDiv by_row, bool vec) {
     constexpr int SIDE = 32 / LANES;
     const int sub = threadIdx.x & (LANES - 1), nq = hd >> 2;
-    const P4Row x = p4_row<LANES>(rows, chunks, by_row, row_seq, row_pos, kv);
+    const P4Row x = p4_row<LANES, kP4Units>(rows, chunks, by_row, row_seq, row_pos, kv);
     if (x.page == -1 || !p4_valid(kv, x.page)) return;
     const uint8_t* src = (x.is_k ? kv.p.k : kv.p.v) + p4_off(kv.p, x.page, x.slot, x.head);
     const uint32_t* par =
@@ -1305,11 +1354,10 @@ PagedKV4 shifted(PagedKV4 kv, const int* row_seq, int r0) {
     return kv;
 }
 
-// Rows in launches of fewer than 2^30 warps. f(first row, rows, CTAs, warps that share K or V of a row).
+// Rows in launches of fewer than 2^30 warps of `per` heads. f(first row, rows, CTAs, warps that share K or V of a row).
 template <class F>
-int row_launches(int rows, int KV, int hd, F f) {
-    const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : 32, per = kP4Units * (32 / lanes), chunks = (KV + per - 1) / per;
-    const int most = std::max(1, (1 << 30) / (2 * chunks)), warps = kP4Threads / 32;
+int row_launches(int rows, int KV, int per, F f) {
+    const int chunks = (KV + per - 1) / per, most = std::max(1, (1 << 30) / (2 * chunks)), warps = kP4Threads / 32;
     for (int r0 = 0; r0 < rows; r0 += most) {
         const int n = std::min(most, rows - r0);
         f(r0, n, (unsigned)(((long long)n * 2 * chunks + warps - 1) / warps), chunks);
@@ -1319,21 +1367,38 @@ int row_launches(int rows, int KV, int hd, F f) {
     return JYC_OK;
 }
 
+template <int LANES, int UNITS>
+auto append_of(int mode) {
+    return mode == P4_PLAIN    ? paged4_append_kernel<LANES, UNITS, P4_PLAIN>
+           : mode == P4_PAIRS  ? paged4_append_kernel<LANES, UNITS, P4_PAIRS>
+           : mode == P4_HALVES ? paged4_append_kernel<LANES, UNITS, P4_HALVES>
+                               : paged4_append_kernel<LANES, UNITS, P4_ODD>;
+}
+
 }  // namespace
 
 int launch_paged4_append(const float* K, const float* V, int ld, int rows, int KV, int hd, const int* row_seq,
                          const int* row_pos, const int* rope_pos, const PagedKV4& kv, const RopeView& rope,
                          cudaStream_t s) {
     const bool vec = aligned16(K, ld) && aligned16(V, ld), wide = vec && rope_wide(rope);
-    const auto kernel = hd <= 32    ? paged4_append_kernel<8, 1>
-                        : hd <= 64  ? paged4_append_kernel<16, 1>
-                        : hd <= 128 ? paged4_append_kernel<32, 1>
-                                    : paged4_append_kernel<32, 2>;
-    return row_launches(rows, KV, hd, [&](int r0, int n, unsigned grid, int chunks) {
+    const int lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, side = 32 / lanes;
+    // four blocks of heads a warp where the rows have them and fill the SMs so: less bookkeeping a head; one otherwise
+    // (8 rows of 8 x 128: TODO)
+    const bool many = KV > 2 * side && (long long)rows * KV >= 64LL * sm_count();
+    const int mode = !rope.cos_t ? P4_PLAIN : !wide ? P4_ODD : rope.halves ? P4_HALVES : P4_PAIRS;
+    const auto kernel = many ? (lanes == 4    ? append_of<4, 4>(mode)
+                                : lanes == 8  ? append_of<8, 4>(mode)
+                                : lanes == 16 ? append_of<16, 4>(mode)
+                                              : append_of<32, 4>(mode))
+                             : (lanes == 4    ? append_of<4, 1>(mode)
+                                : lanes == 8  ? append_of<8, 1>(mode)
+                                : lanes == 16 ? append_of<16, 1>(mode)
+                                              : append_of<32, 1>(mode));
+    return row_launches(rows, KV, (many ? 4 : 1) * side, [&](int r0, int n, unsigned grid, int chunks) {
         kernel<<<grid, kP4Threads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
                                            row_seq ? row_seq + r0 : nullptr, row_pos + r0,
                                            rope_pos ? rope_pos + r0 : nullptr, shifted(kv, row_seq, r0), rope, chunks,
-                                           fast_div(2 * chunks), vec, wide);
+                                           fast_div(2 * chunks), vec);
     });
 }
 
@@ -1344,7 +1409,7 @@ int launch_paged4_read(float* K, float* V, int ld, int rows, int KV, int hd, con
                         : hd <= 64  ? paged4_read_kernel<16, 1>
                         : hd <= 128 ? paged4_read_kernel<32, 1>
                                     : paged4_read_kernel<32, 2>;
-    return row_launches(rows, KV, hd, [&](int r0, int n, unsigned grid, int chunks) {
+    return row_launches(rows, KV, kP4Units * (32 / (hd <= 32 ? 8 : hd <= 64 ? 16 : 32)), [&](int r0, int n, unsigned grid, int chunks) {
         kernel<<<grid, kP4Threads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
                                            row_seq ? row_seq + r0 : nullptr, row_pos + r0, shifted(kv, row_seq, r0),
                                            chunks, fast_div(2 * chunks), vec);
