@@ -1134,11 +1134,11 @@ __device__ __forceinline__ uint32_t ev_key(float m) { return f32_order_key(m + 0
 __device__ __forceinline__ void ev_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int ev_far(const int* p, int rank) {
+__device__ __forceinline__ int2 ev_far2(const int* p, int rank) {
     uint32_t at;
-    int v;
+    int2 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
     return v;
 }
 
@@ -1147,7 +1147,8 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
     int* const copies = ev_sm;                        // [bin][copy]
     int* const sums = ev_sm + kEvCopies * kEvBins;    // [digit][bin]: this CTA's counts
     uint32_t* const keys = reinterpret_cast<uint32_t*>(ev_sm + (kEvCopies + 3) * kEvBins);
-    __shared__ int s_warp[kEvWarps], s_digit, s_above, s_count[2], s_more[kEvWarps], s_equal[kEvWarps];
+    __shared__ __align__(8) int s_count[2];
+    __shared__ int s_warp[kEvWarps], s_digit, s_above, s_more[kEvWarps], s_equal[kEvWarps];
     griddep_launch();
     const int rank = blockIdx.x % ctas, item = blockIdx.x / ctas, b = item / e.KV, h = item - b * e.KV;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1176,7 +1177,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
         return p4_valid(e.kv, page) ? ev_key(e.kv.p.mass[p4_moff(e.kv.p, page, slot, h)]) : 0u;
     };
     if (cached) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = w0 + lane; i < w1; i += 32) keys[i] = fetch(i);
     }
     auto key = [&](int i) { return cached ? keys[i] : fetch(i); };
@@ -1205,10 +1206,18 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
         if (ctas > 1) {
             __syncwarp();
             ev_cluster_sync();
-            for (int r = 0; r < ctas; r++)
-                if (r != rank)
+            // all CTAs' counts in flight at once (one after another they were 9 of each digit's 13 us)
+            int2 far[kEvMaxCluster];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) mine[k] += ev_far(sums + d * kEvBins + 2 * tid + k, r);
+            for (int r = 0; r < kEvMaxCluster; r++) {
+                far[r] = make_int2(0, 0);
+                if (r < ctas && r != rank) far[r] = ev_far2(sums + d * kEvBins + 2 * tid, r);
+            }
+#pragma unroll
+            for (int r = 0; r < kEvMaxCluster; r++) {
+                mine[0] += far[r].x;
+                mine[1] += far[r].y;
+            }
         }
         // counts of all bins above this thread's: a suffix sum over the CTA
         const int both = mine[0] + mine[1];
@@ -1261,10 +1270,9 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
     if (ctas > 1) {
         __syncwarp();
         ev_cluster_sync();
-        for (int r = 0; r < rank; r++) {
-            out += ev_far(&s_count[0], r);
-            ties += ev_far(&s_count[1], r);
-        }
+        const int2 v = lane < rank ? ev_far2(s_count, lane) : make_int2(0, 0);
+        out += __reduce_add_sync(0xffffffffu, v.x);
+        ties += __reduce_add_sync(0xffffffffu, v.y);
     }
     // of rows at the border the first `left` in order are kept
     out += min(ties, left);
@@ -1285,7 +1293,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
 
 // A row is copied by as many lanes as it has 16-byte chunks (rounded up to a power of two), each with one chunk of K and
 // one of V, the parameters word by word among them; kMvRows rows of a thread in flight.
-constexpr int kMvThreads = 256, kMvRows = 4;
+constexpr int kMvThreads = 256, kMvRows = 2;
 template <int LANES>
 __global__ void __launch_bounds__(kMvThreads) paged4_move_kernel(PagedEvict4 e, FastDiv by_budget, FastDiv by_kv,
                                                                  FastDiv by_new_page) {
