@@ -1119,36 +1119,36 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
 // of lanes copy them.
 //
 // Select: the border among the masses' order keys (the `want`-th largest) digit by
-// digit, 11, 11 and 10 bits: each CTA counts the digits of its slice of the positions in
+// digit, 8 bits each: each CTA counts the digits of its slice of the positions in
 // shared memory, all CTAs of the cluster add up all counts and find the same digit. Then
 // kept positions are counted slice by slice and warp by warp, and written in their order.
 // Keys of slices up to kEvSpan positions stay in shared memory (131072 positions of one
 // sequence: 8 CTAs a head), those of longer ones are read again for each digit. Masses
-// differ little in their first digit, so the counts have kEvCopies copies, a lane's own of 8.
+// differ little in their first digit: each lane has counts of its own. (Digits of 11 bits
+// need one pass less, but 2048 counts to clear, add up and exchange: 9 us a digit against TODO.)
 constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvSpan = 24576;
-constexpr int kEvBins = 2048, kEvCopies = 8, kEvMaxCluster = 8;
-constexpr int kEvSmem = ((kEvCopies + 3) * kEvBins + kEvSpan) * 4;
+constexpr int kEvBins = 256, kEvDigits = 4, kEvMaxCluster = 8;
+constexpr int kEvSmem = ((32 + kEvDigits) * kEvBins + kEvSpan) * 4;
 
 // larger mass -> larger key; NaN below every number, -0 as 0
 __device__ __forceinline__ uint32_t ev_key(float m) { return f32_order_key(m + 0.0f); }
 __device__ __forceinline__ void ev_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int2 ev_far2(const int* p, int rank) {
+__device__ __forceinline__ int ev_far(const int* p, int rank) {
     uint32_t at;
-    int2 v;
+    int v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
 
 __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict4 e, int ctas) {
     extern __shared__ int ev_sm[];
-    int* const copies = ev_sm;                        // [bin][copy]
-    int* const sums = ev_sm + kEvCopies * kEvBins;    // [digit][bin]: this CTA's counts
-    uint32_t* const keys = reinterpret_cast<uint32_t*>(ev_sm + (kEvCopies + 3) * kEvBins);
-    __shared__ __align__(8) int s_count[2];
-    __shared__ int s_warp[kEvWarps], s_digit, s_above, s_more[kEvWarps], s_equal[kEvWarps];
+    int* const counts = ev_sm;                // [bin][lane]
+    int* const sums = ev_sm + 32 * kEvBins;   // [digit][bin]: this CTA's
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(ev_sm + (32 + kEvDigits) * kEvBins);
+    __shared__ int s_warp[kEvWarps], s_digit, s_above, s_count[2], s_more[kEvWarps], s_equal[kEvWarps];
     griddep_launch();
     const int rank = blockIdx.x % ctas, item = blockIdx.x / ctas, b = item / e.KV, h = item - b * e.KV;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1184,60 +1184,53 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
     uint32_t border = 0u;
     int left = want;  // of those that share the border's digits, how many are kept
 #pragma unroll 1
-    for (int d = 0; d < 3; d++) {
-        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d < 2 ? 2048 : 1024;
-        for (int i = tid; i < kEvCopies * kEvBins / 4; i += kEvThreads) reinterpret_cast<int4*>(copies)[i] = make_int4(0, 0, 0, 0);
+    for (int d = 0; d < kEvDigits; d++) {
+        const int shift = 24 - 8 * d;
+        for (int i = tid; i < 32 * kEvBins / 4; i += kEvThreads) reinterpret_cast<int4*>(counts)[i] = make_int4(0, 0, 0, 0);
         __syncthreads();
 #pragma unroll 4
         for (int i = w0 + lane; i < w1; i += 32) {
             const uint32_t k = key(i);
-            if (d == 0 || (k ^ border) >> (d == 1 ? 21 : 10) == 0)
-                atomicAdd(&copies[(k >> shift & (bins - 1)) * kEvCopies + (lane & (kEvCopies - 1))], 1);
+            if (d == 0 || (k ^ border) >> (shift + 8) == 0) atomicAdd(&counts[(k >> shift & (kEvBins - 1)) * 32 + lane], 1);
         }
         __syncthreads();
-        int mine[2];  // counts of bins 2 tid, 2 tid + 1
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int4* c = reinterpret_cast<const int4*>(copies + (2 * tid + k) * kEvCopies);
-            const int4 x = c[0], y = c[1];
-            mine[k] = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
-            sums[d * kEvBins + 2 * tid + k] = mine[k];
+        for (int i = 0; i < kEvBins / kEvWarps; i++) {
+            const int bin = warp * (kEvBins / kEvWarps) + i, n = __reduce_add_sync(0xffffffffu, counts[bin * 32 + lane]);
+            if (lane == 0) sums[d * kEvBins + bin] = n;
         }
-        if (ctas > 1) {
-            __syncwarp();
+        __syncwarp();
+        if (ctas > 1)
             ev_cluster_sync();
-            // all CTAs' counts in flight at once (one after another they were 9 of each digit's 13 us)
-            int2 far[kEvMaxCluster];
+        else
+            __syncthreads();
+        // this thread's bin over all CTAs, all of their counts in flight at once, and a suffix sum over the bins
+        int mine = 0;
+        if (tid < kEvBins) {
+            int far[kEvMaxCluster];
 #pragma unroll
             for (int r = 0; r < kEvMaxCluster; r++) {
-                far[r] = make_int2(0, 0);
-                if (r < ctas && r != rank) far[r] = ev_far2(sums + d * kEvBins + 2 * tid, r);
+                far[r] = 0;
+                if (r < ctas) far[r] = r == rank ? sums[d * kEvBins + tid] : ev_far(sums + d * kEvBins + tid, r);
             }
 #pragma unroll
-            for (int r = 0; r < kEvMaxCluster; r++) {
-                mine[0] += far[r].x;
-                mine[1] += far[r].y;
-            }
+            for (int r = 0; r < kEvMaxCluster; r++) mine += far[r];
         }
-        // counts of all bins above this thread's: a suffix sum over the CTA
-        const int both = mine[0] + mine[1];
-        int incl = both;
+        int above = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_down_sync(0xffffffffu, incl, o);
-            if (lane + o < 32) incl += x;
+            const int x = __shfl_down_sync(0xffffffffu, above, o);
+            if (lane + o < 32) above += x;
         }
-        if (lane == 0) s_warp[warp] = incl;
+        if (lane == 0) s_warp[warp] = above;
         __syncthreads();
-        int above = incl - both;
-        for (int w = warp + 1; w < kEvWarps; w++) above += s_warp[w];
+        above -= mine;
 #pragma unroll
-        for (int k = 1; k >= 0; k--) {
-            if (above < left && above + mine[k] >= left) {  // one thread of the CTA
-                s_digit = 2 * tid + k;
-                s_above = above;
-            }
-            above += mine[k];
+        for (int w = 1; w < kEvBins / 32; w++)
+            if (w > warp) above += s_warp[w];
+        if (tid < kEvBins && above < left && above + mine >= left) {  // one thread of the CTA
+            s_digit = tid;
+            s_above = above;
         }
         __syncthreads();
         border |= (uint32_t)s_digit << shift;
@@ -1270,12 +1263,12 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
     if (ctas > 1) {
         __syncwarp();
         ev_cluster_sync();
-        const int2 v = lane < rank ? ev_far2(s_count, lane) : make_int2(0, 0);
-        out += __reduce_add_sync(0xffffffffu, v.x);
-        ties += __reduce_add_sync(0xffffffffu, v.y);
+        out += __reduce_add_sync(0xffffffffu, lane < rank ? ev_far(&s_count[0], lane) : 0);
+        ties += __reduce_add_sync(0xffffffffu, lane < rank ? ev_far(&s_count[1], lane) : 0);
     }
     // of rows at the border the first `left` in order are kept
     out += min(ties, left);
+#pragma unroll 4
     for (int i0 = w0; i0 < w1; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t k = i < w1 ? key(i) : 0u;
