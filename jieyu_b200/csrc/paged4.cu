@@ -326,6 +326,23 @@ struct P4Scores {
 __device__ __forceinline__ size_t p4_score_at(const P4Scores& sc, const PaPlan& pl, int b, int r, int t, int unit) {
     return (size_t)((long long)b * pl.units_row * pl.team + r) * sc.keys + (size_t)t * unit;
 }
+// two fp32 operations in one instruction
+__device__ __forceinline__ void p4_add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void p4_mul2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void p4_fma2(float& x, float& y, float a, float b, float c, float d) {  // += (a, b) * (c, d)
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+        "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+}
 __device__ __forceinline__ __half2 p4_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t p4_u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 template <int N>
@@ -706,8 +723,11 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                             int c[4];
                             pa_mma_s8(kf, qf[i0 + k][e], 0x4B400000, c);
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                acc[m][e][j] = __fmaf_rn(j < 2 ? s0 : s1, __fsub_rn(__int_as_float(c[j]), 12582912.0f), acc[m][e][j]);
+                            for (int j = 0; j < 4; j += 2) {
+                                float x = __int_as_float(c[j]), y = __int_as_float(c[j + 1]);
+                                p4_add2(x, y, -12582912.0f, -12582912.0f);
+                                p4_fma2(acc[m][e][j], acc[m][e][j + 1], j ? s1 : s0, j ? s1 : s0, x, y);
+                            }
                         }
                     }
                 }
@@ -716,8 +736,11 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) s[4 * u + i][e][j] = __fmul_rn(acc[i >> 1][e][2 * (i & 1) + j], qsl[e][j]);
+                {
+                    s[4 * u + i][e][0] = acc[i >> 1][e][2 * (i & 1)];
+                    s[4 * u + i][e][1] = acc[i >> 1][e][2 * (i & 1) + 1];
+                    p4_mul2(s[4 * u + i][e][0], s[4 * u + i][e][1], qsl[e][0], qsl[e][1]);
+                }
         }
         if (!full) {  // keys that do not count: -inf, whatever the ring held
 #pragma unroll
@@ -776,13 +799,14 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
         for (int i = 0; i < 4 * U; i++)
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const float b0 = ex2(s[i][e][0] - ref[e][0]), b1 = ex2(s[i][e][1] - ref[e][1]);
-                l[e][0] += b0;
-                l[e][1] += b1;
+                p4_add2(s[i][e][0], s[i][e][1], -ref[e][0], -ref[e][1]);
+                float b0 = ex2(s[i][e][0]), b1 = ex2(s[i][e][1]);
+                p4_add2(l[e][0], l[e][1], b0, b1);
                 const uint32_t ph = pa_pack(b0, b1);
-                const float2 hf = __half22float2(p4_h2(ph));
+                const float2 hf = __half22float2(p4_h2(ph ^ 0x80008000u));
+                p4_add2(b0, b1, hf.x, hf.y);
                 hi[i][e] = pa_transpose(ph);
-                lo[i][e] = pa_transpose(pa_pack(b0 - hf.x, b1 - hf.y));
+                lo[i][e] = pa_transpose(pa_pack(b0, b1));
             }
         // the parameters' share: rows are their columns
         {
@@ -878,7 +902,8 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) o[2 * i0 + k][e][j] += c[k][e][j];
+                    for (int j = 0; j < 4; j += 2)
+                        p4_add2(o[2 * i0 + k][e][j], o[2 * i0 + k][e][j + 1], c[k][e][j], c[k][e][j + 1]);
         }
         if constexpr (TMA) {
             // the stage is read: the unit ST ahead takes its place
@@ -1098,7 +1123,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
         if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, pl.team), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
-    const unsigned chunks = (unsigned)std::min({most, (8LL * sms + heads - 1) / heads, 65535LL});
+    const unsigned chunks = (unsigned)std::min({most, (32LL * sms + heads - 1) / heads, 65535LL});
     return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
 }
 
