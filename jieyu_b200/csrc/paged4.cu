@@ -289,11 +289,13 @@ struct P4Cfg {
     using Args = PagedAttn4;
     static __device__ __forceinline__ int len(const PagedAttn4& a, int b) { return p4_len(a, b); }
     static constexpr bool STAT = true, TEAM = true;
-    static constexpr int U = GP <= 4 ? 2 : 1;         // keys of a lane
-    static constexpr int HDP = 32 * GP, TK = 32 * U;  // keys of a unit
-    // 131072 keys of 8 x 128: 60 us with 8 warps of 2 stages of 64 keys, 62 with 12 of 3 of 32, 71 with 16 of 2; 64 sequences
-    // of 2112 keys of 8 x 64: 49 us with 12 warps, 55 with 8
-    static constexpr int WARPS = GP <= 2 ? 12 : 8;
+    static constexpr bool WIDE = GP == 4 && HEADS > 8;
+    static constexpr int U = GP <= 2 || WIDE ? 2 : 1;  // keys of a lane
+    static constexpr int HDP = 32 * GP, TK = 32 * U;   // keys of a unit
+    // few warps of long units against more of short ones: 131072 keys of 8 x 128, 4 heads each, 57 us with 12 warps of 32
+    // keys, 58 with 8 of 64, 70 with 16 of 32; with 16 heads each, 65536 keys, 65 us with 8 of 64, 74 with 12 of 32; 64
+    // sequences of 2112 keys of 8 x 64 50 us with 12 warps of 64, 55 with 8
+    static constexpr int WARPS = GP <= 4 && !WIDE ? 12 : 8;
     static constexpr int ST = GP == 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
     static constexpr int ROWS = HEADS;
@@ -1120,7 +1122,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
                           (const unsigned char*)queries, copy, maps))
         return e;
     if (tiles > 1)  // else an item is one unit: none is split
-        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, pl.team), kPaWideThreads, 0, s, a, pl, w)) return e;
+        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, (G::ROWS * pl.team + pa_wide_rows<G>(pl.team) - 1) / pa_wide_rows<G>(pl.team)), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
     const unsigned chunks = (unsigned)std::min({most, (32LL * sms + heads - 1) / heads, 65535LL});

@@ -470,13 +470,17 @@ __device__ __forceinline__ void pa_end(const typename G::Args& a, const PaPlan& 
     }
     if (run.alone) return;  // written
 
+    const int begins = c0 == sh.first[0] ? 1 : 0;
+    if (tid == 0 && !run.whole && begins)
+        work.tail[blockIdx.x] = PaTail{later(sh.first[0] + sh.cur[0].nt), slot_at(w0, 0, 1), sh.cur[0].b, sh.cur[0].r, line.per_cta};
+    if (G::TEAM && line.per_cta == 1 && !run.whole) {  // one worker: its sums are the CTA's part
+        if (run.worker) pa_store<G>(work.part + (size_t)slot_at(w0, member, begins) * G::PART, true, o, ref, l);
+        return;
+    }
     // join the CTA's workers (their rings are free now)
     if (run.worker) pa_store<G>(reinterpret_cast<float*>(sm + warp * G::RING), count > 0, o, ref, l);
     __syncthreads();
     const PaCursor c = sh.cur[0];
-    const int begins = c0 == sh.first[0] ? 1 : 0;
-    if (tid == 0 && !run.whole && begins)
-        work.tail[blockIdx.x] = PaTail{later(sh.first[0] + c.nt), slot_at(w0, 0, 1), c.b, c.r, line.per_cta};
     for (int i = tid; i < team * (ROWS * HDP / 4); i += WARPS * 32) {
         const int m = G::TEAM ? i / (ROWS * HDP / 4) : 0, k = i - m * (ROWS * HDP / 4);
         const int row = k / (HDP / 4), d = k % (HDP / 4) * 4, r = c.r * team + m, qb = r % pl.qblocks, kvh = r / pl.qblocks;
@@ -560,85 +564,98 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32)
     }
 }
 
-// The same for teams, whose items go through more CTAs: a CTA of kPaWideThreads threads for each item and row of the
-// team. A warp per query row finds the reference and the parts' factors, then every thread adds four dims of a row over its
-// share of the parts, kPaWideLoads of them in flight, and the shares are added in shared memory (131072 keys of 8 x 128, 148
-// parts: TODO).
-constexpr int kPaWideThreads = 512, kPaWideLoads = 8, kPaMaxCtas = 256;
+// The same for teams, whose items go through more CTAs: blockIdx.y takes pa_wide_rows query rows of a team's rows.
+// One row at a time: the threads find the reference and the parts' factors, then each adds four dims over its share of the
+// parts, kPaWideLoads of them in flight, and the shares are added in shared memory. Small CTAs, as most find nothing to
+// join. (148 parts of 8 heads' 4 rows of 128: 10 us with 512 threads for 4 rows, TODO with these.)
+constexpr int kPaWideThreads = 128, kPaWideLoads = 16, kPaMaxCtas = 256;
+template <class G>
+__host__ __device__ constexpr int pa_wide_rows(int team) {
+    return G::ROWS * team > 32 ? (G::ROWS * team + 31) / 32 : 1;
+}
 template <class G>
 __global__ void __launch_bounds__(kPaWideThreads) paged_join_wide_kernel(typename G::Args a, PaPlan pl, PaWork work) {
-    constexpr int HDP = G::HDP, ROWS = G::ROWS, COLS = ROWS * HDP / 4;
-    constexpr int SIDE = COLS < kPaWideThreads ? kPaWideThreads / COLS : 1, STEP = COLS < kPaWideThreads ? COLS : kPaWideThreads;
-    __shared__ float s_f[ROWS][kPaMaxCtas], s_l[ROWS];
+    constexpr int HDP = G::HDP, ROWS = G::ROWS, COLS = HDP / 4, SIDE = kPaWideThreads / COLS, WARPS = kPaWideThreads / 32;
+    constexpr int REFS = kPaMaxCtas / kPaWideThreads;
+    static_assert(COLS <= kPaWideThreads, "a row's columns fit the threads");
+    __shared__ float s_f[kPaMaxCtas], s_m[WARPS], s_l[WARPS];
     __shared__ __align__(16) float4 s_o[kPaWideThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.H / a.KV, hd = a.hd;
     if (G::STAT) griddep_launch();
     griddep_wait();
     const PaTail tail = work.tail[blockIdx.x];
     if (tail.ctas == 0) return;
-    const int team = pa_team<G>(pl), member = blockIdx.y, item = tail.r * team + member;
-    const int np = tail.ctas + 1, qb = item % pl.qblocks, kvh = item / pl.qblocks, rows = min(ROWS, group - qb * ROWS);
-    auto part = [&](int i) {
-        return work.part + (size_t)((i == 0 ? tail.slot : ((int)blockIdx.x + i) * tail.per_cta * team * 2) + member * 2) * G::PART;
-    };
-    for (int row = warp; row < rows; row += kPaWideThreads / 32) {
+    const int team = pa_team<G>(pl), np = tail.ctas + 1, each = pa_wide_rows<G>(team);
+    for (int k = 0; k < each; k++) {
+        const int at = blockIdx.y * each + k, member = at / ROWS, row = at - member * ROWS;
+        const int item = tail.r * team + member, qb = item % pl.qblocks, kvh = item / pl.qblocks;
+        if (member >= team || qb * ROWS + row >= group) continue;  // the whole CTA
+        const int h = kvh * group + qb * ROWS + row;
+        auto part = [&](int i) {
+            return work.part + (size_t)((i == 0 ? tail.slot : ((int)blockIdx.x + i) * tail.per_cta * team * 2) + member * 2) * G::PART;
+        };
+        float2 rl[REFS];
         float M = kPaLow, L = 0.0f;
-        float2 rl[kPaMaxCtas / 32];
 #pragma unroll
-        for (int k = 0; k < kPaMaxCtas / 32; k++) {
-            const int i = lane + 32 * k;
-            rl[k] = i < np ? *reinterpret_cast<const float2*>(part(i) + ROWS * HDP + 2 * row) : make_float2(kPaLow, 0.0f);
-            M = fmaxf(M, rl[k].x);
+        for (int i = 0; i < REFS; i++) {
+            const int n = tid + kPaWideThreads * i;
+            rl[i] = n < np ? *reinterpret_cast<const float2*>(part(n) + ROWS * HDP + 2 * row) : make_float2(kPaLow, 0.0f);
+            M = fmaxf(M, rl[i].x);
         }
-        M = warp_max(M);
+        // the first loads of the rows need no factors
+        const int col = tid % COLS, side = tid / COLS, d = 4 * col;
+        float4 x[kPaWideLoads];
+        auto load = [&](int i0) {
 #pragma unroll
-        for (int k = 0; k < kPaMaxCtas / 32; k++) {
-            const float f = ex2(rl[k].x - M);
-            if (lane + 32 * k < np) s_f[row][lane + 32 * k] = f;
-            L = __fmaf_rn(rl[k].y, f, L);
+            for (int i = 0; i < kPaWideLoads; i++)
+                x[i] = side < SIDE && i0 + SIDE * i < np ? *reinterpret_cast<const float4*>(part(i0 + SIDE * i) + row * HDP + d)
+                                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        load(side);
+        M = warp_max(M);
+        if (lane == 0) s_m[warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) M = fmaxf(M, s_m[w]);
+#pragma unroll
+        for (int i = 0; i < REFS; i++) {
+            const float f = ex2(rl[i].x - M);
+            s_f[tid + kPaWideThreads * i] = f;
+            L = __fmaf_rn(rl[i].y, f, L);
         }
         L = warp_sum(L);
-        if (lane == 0) {
-            const int h = kvh * group + qb * ROWS + row;
-            s_l[row] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-            if (G::STAT && work.stat) work.stat[(size_t)tail.b * a.H + h] = make_float2(M, s_l[row]);
-        }
-    }
-    __syncthreads();
-    for (int c0 = 0; c0 < COLS; c0 += STEP) {
-        const int col = c0 + tid % STEP, side = tid / STEP, row = col / (HDP / 4), d = col % (HDP / 4) * 4;
+        if (lane == 0) s_l[warp] = L;
+        __syncthreads();
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) L += s_l[w];
+        const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+        if (G::STAT && work.stat && tid == 0) work.stat[(size_t)tail.b * a.H + h] = make_float2(M, inv);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool live = row < rows && side < SIDE;
-        if (live)
-            for (int i0 = side; i0 < np; i0 += SIDE * kPaWideLoads) {
-                float4 x[kPaWideLoads];
+        for (int i0 = side; i0 < np; i0 += SIDE * kPaWideLoads) {
+            if (i0 != side) load(i0);
 #pragma unroll
-                for (int k = 0; k < kPaWideLoads; k++)
-                    x[k] = i0 + SIDE * k < np ? *reinterpret_cast<const float4*>(part(i0 + SIDE * k) + row * HDP + d)
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int k = 0; k < kPaWideLoads; k++) {
-                    const float f = i0 + SIDE * k < np ? s_f[row][i0 + SIDE * k] : 0.0f;
-                    o = make_float4(__fmaf_rn(x[k].x, f, o.x), __fmaf_rn(x[k].y, f, o.y), __fmaf_rn(x[k].z, f, o.z),
-                                    __fmaf_rn(x[k].w, f, o.w));
-                }
-            }
-        if (SIDE > 1) {
-            s_o[tid] = o;
-            __syncthreads();
-            for (int w = 1; side == 0 && w < SIDE; w++) {
-                const float4 x = s_o[w * STEP + tid];
-                o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+            for (int i = 0; i < kPaWideLoads; i++) {
+                const float f = i0 + SIDE * i < np ? s_f[i0 + SIDE * i] : 0.0f;
+                o = make_float4(__fmaf_rn(x[i].x, f, o.x), __fmaf_rn(x[i].y, f, o.y), __fmaf_rn(x[i].z, f, o.z),
+                                __fmaf_rn(x[i].w, f, o.w));
             }
         }
-        if (live && side == 0 && d < hd) {
-            float* to = a.out + (size_t)tail.b * a.ldo + (size_t)(kvh * group + qb * ROWS + row) * hd + d;
-            const float inv = s_l[row];
+        s_o[tid] = o;
+        __syncthreads();
+        if (side == 0 && d < hd) {
+#pragma unroll
+            for (int w = 1; w < SIDE; w++) {
+                const float4 y = s_o[w * COLS + tid];
+                o = make_float4(o.x + y.x, o.y + y.y, o.z + y.z, o.w + y.w);
+            }
+            float* to = a.out + (size_t)tail.b * a.ldo + (size_t)h * hd + d;
             to[0] = o.x * inv;
             to[1] = o.y * inv;
             to[2] = o.z * inv;
             to[3] = o.w * inv;
         }
+        __syncthreads();  // the next row takes the shared arrays
     }
 }
 
