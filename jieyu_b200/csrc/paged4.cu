@@ -986,33 +986,57 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     pa_end<G>(a, pl, work, sh, run, count, cur, item0, tail, p4_sm, hd, o, ref, l);
 }
 
-// The weights of the scores that the kernel above left, added to their keys' mass: a thread per key.
-constexpr int kP4MassThreads = 256;
+// The weights of the scores that the kernel above left, added to their keys' mass: kP4MassKeys keys of a thread in flight.
+constexpr int kP4MassThreads = 128, kP4MassKeys = 4;
 template <int ROWS>
 __global__ void __launch_bounds__(kP4MassThreads) paged4_mass_kernel(PagedAttn4 a, PaPlan pl, PaWork work, P4Scores scores) {
     griddep_wait();
     const int b = blockIdx.x / a.KV, kvh = blockIdx.x - b * a.KV, group = a.H / a.KV;
     const int len = p4_len(a, b);
     const float2* const stat = work.stat + (size_t)b * a.H + (size_t)kvh * group;
-    for (long long j = (long long)blockIdx.y * kP4MassThreads + threadIdx.x; j < len; j += (long long)gridDim.y * kP4MassThreads) {
-        int slot;
-        const int page = p4_entry(a.kv, b, (int)j, &slot);
-        float sum = 0.0f;
-        for (int qb = 0; qb < pl.qblocks; qb++) {
-            const float* s = scores.s + p4_score_at(scores, pl, b, kvh * pl.qblocks + qb, (int)j, ROWS);
-            float4 x[ROWS / 4];
+    float2 ri[ROWS];
+    auto stats = [&](int qb) {
 #pragma unroll
-            for (int i = 0; i < ROWS / 4; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(s) + i);
+        for (int i = 0; i < ROWS; i++) ri[i] = qb * ROWS + i < group ? __ldcg(stat + qb * ROWS + i) : make_float2(0.0f, 0.0f);
+    };
+    stats(0);
+    for (long long j0 = (long long)blockIdx.y * kP4MassThreads * kP4MassKeys + threadIdx.x; j0 < len;
+         j0 += (long long)gridDim.y * kP4MassThreads * kP4MassKeys) {
+        int slot[kP4MassKeys], page[kP4MassKeys];
+        float sum[kP4MassKeys];
 #pragma unroll
-            for (int i = 0; i < ROWS; i++) {
-                if (qb * ROWS + i >= group) break;
-                const float2 ri = __ldcg(stat + qb * ROWS + i);
-                const float4 v = x[i >> 2];
-                const float y = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-                sum += ex2(y - ri.x) * ri.y;
-            }
+        for (int k = 0; k < kP4MassKeys; k++) {
+            const long long j = j0 + k * kP4MassThreads;
+            sum[k] = 0.0f;
+            page[k] = j < len ? p4_entry(a.kv, b, (int)j, &slot[k]) : -1;
         }
-        if (p4_valid(a.kv, page)) atomicAdd(a.kv.p.mass + p4_moff(a.kv.p, page, slot, kvh), sum);
+        for (int qb = 0; qb < pl.qblocks; qb++) {
+            const float* s = scores.s + p4_score_at(scores, pl, b, kvh * pl.qblocks + qb, (int)j0, ROWS);
+            float4 x[kP4MassKeys][ROWS / 4];
+#pragma unroll
+            for (int k = 0; k < kP4MassKeys; k++)
+#pragma unroll
+                for (int i = 0; i < ROWS / 4; i++)
+                    x[k][i] = page[k] != -1 ? __ldcg(reinterpret_cast<const float4*>(s + (size_t)k * kP4MassThreads * ROWS) + i)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (pl.qblocks > 1) stats(qb);
+#pragma unroll
+            for (int k = 0; k < kP4MassKeys; k++)
+#pragma unroll
+                for (int i = 0; i < ROWS; i += 4) {
+                    // rows behind the last head have no stat
+                    const float4 v = x[k][i / 4];
+                    const int left = group - qb * ROWS - i;
+                    if (left > 0) sum[k] += ex2(v.x - ri[i].x) * ri[i].y;
+                    if (left > 1) sum[k] += ex2(v.y - ri[i + 1].x) * ri[i + 1].y;
+                    if (left > 2) sum[k] += ex2(v.z - ri[i + 2].x) * ri[i + 2].y;
+                    if (left > 3) sum[k] += ex2(v.w - ri[i + 3].x) * ri[i + 3].y;
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < kP4MassKeys; k++)
+            if (page[k] != -1 && p4_valid(a.kv, page[k]))
+                atomicAdd(a.kv.p.mass + p4_moff(a.kv.p, page[k], slot[k], kvh), sum[k]);
     }
 }
 
@@ -1124,7 +1148,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     if (tiles > 1)  // else an item is one unit: none is split
         if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, (G::ROWS * pl.team + pa_wide_rows<G>(pl.team) - 1) / pa_wide_rows<G>(pl.team)), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
-    const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads - 1) / kP4MassThreads;
+    const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads * kP4MassKeys - 1) / (kP4MassThreads * kP4MassKeys);
     const unsigned chunks = (unsigned)std::min({most, (32LL * sms + heads - 1) / heads, 65535LL});
     return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
 }
