@@ -521,6 +521,12 @@ JYC_API int jyc_sample_batch(const float* logits, int ld, int rows, int vocab_si
 // Rotary rows, 8-bit products and the 4-bit paged cache.
 namespace {
 
+// Whether an array of 4-byte numbers does not lie on 4 bytes.
+template <class... P>
+bool askew(P... p) {
+    return ((0 | ... | (uintptr_t)p) & 3) != 0;
+}
+
 int check_rope_view(const char* what, const jyc_rope* r, int head_dim, RopeView* v) {
     auto bad = [&](const char* msg) { return arg_error(std::string(what) + ": " + msg); };
     *v = RopeView{nullptr, nullptr, 0, 0, false};
@@ -580,6 +586,7 @@ JYC_API int jyc_rope_rows(const float* X, int ldx, float* Y, int ldy, int rows, 
         return arg_error("rope_rows: ldx and ldy must hold num_heads * head_dim");
     if (rows == 0) return JYC_OK;
     if (!X || !Y || !row_pos) return arg_error("rope_rows: null pointer");
+    if (askew(X, Y, row_pos)) return arg_error("rope_rows: misaligned array");
     if (X == Y && ldx != ldy) return arg_error("rope_rows: in place needs ldx == ldy");
     return launch_rope_rows(X, ldx, Y, ldy, rows, num_heads, head_dim, row_pos, r, S(stream));
 }
@@ -591,6 +598,7 @@ JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_
     if (ldx < k || ldq < k) return arg_error("quantize_rows_i8: ldx and ldq must hold k");
     if (rows == 0) return JYC_OK;
     if (!x || !q || !scale) return arg_error("quantize_rows_i8: null pointer");
+    if (askew(x, scale)) return arg_error("quantize_rows_i8: misaligned array");
     return launch_quantize_rows(x, ldx, rows, k, q, ldq, scale, S(stream));
 }
 
@@ -604,6 +612,7 @@ JYC_API int jyc_matmul_i8(const int8_t* A, int lda, const float* a_scale, const 
     if ((lda | ldw) & 15) return arg_error("matmul_i8: lda and ldw must be multiples of 16");
     if (m == 0) return JYC_OK;
     if (!A || !a_scale || !W || !w_scale || !C) return arg_error("matmul_i8: null pointer");
+    if (askew(a_scale, w_scale, bias, C)) return arg_error("matmul_i8: misaligned array");
     if (((uintptr_t)A | (uintptr_t)W) & 15) return arg_error("matmul_i8: A and W must be 16-byte aligned");
     return launch_i8_gemm(I8Gemm{A, lda, a_scale, W, ldw, w_scale, bias, C, ldc, m, n, k}, S(stream));
 }
@@ -621,6 +630,7 @@ JYC_API int jyc_kv_append_paged_q4(const float* K, const float* V, int ld, int r
     if (!row_seq && rows > num_seqs) return arg_error("kv_append_paged_q4: more rows than sequences without row_seq");
     if (rows == 0) return JYC_OK;
     if (!K || !V || !row_pos) return arg_error("kv_append_paged_q4: null pointer");
+    if (askew(K, V, row_seq, row_pos, rope_pos)) return arg_error("kv_append_paged_q4: misaligned array");
     PagedKV4 kv;
     TRY(paged4_view(pages, page_table, table_stride, num_seqs, &kv));
     return launch_paged4_append(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, rope_pos, kv, r, S(stream));
@@ -636,6 +646,7 @@ JYC_API int jyc_kv_read_paged_q4(float* K, float* V, int ld, int rows, int num_k
     if (!row_seq && rows > num_seqs) return arg_error("kv_read_paged_q4: more rows than sequences without row_seq");
     if (rows == 0) return JYC_OK;
     if (!K || !V || !row_pos) return arg_error("kv_read_paged_q4: null pointer");
+    if (askew(K, V, row_seq, row_pos)) return arg_error("kv_read_paged_q4: misaligned array");
     PagedKV4 kv;
     TRY(paged4_view(pages, page_table, table_stride, num_seqs, &kv));
     return launch_paged4_read(K, V, ld, rows, num_kv_heads, head_dim, row_seq, row_pos, kv, S(stream));
@@ -671,6 +682,7 @@ JYC_API int jyc_attention_paged_q4(const float* Q, int ldq, float* out, int ldo,
     if ((long long)num_seqs * num_heads > kMaxItems) return arg_error("attention_paged_q4: num_seqs * num_heads above 2^31 - 1");
     if (num_seqs == 0) return JYC_OK;
     if (!Q || !out || !seq_lens) return arg_error("attention_paged_q4: null pointer");
+    if (askew(Q, out, seq_lens, rope_pos)) return arg_error("attention_paged_q4: misaligned array");
     const int capacity = pages->mass ? table_stride * pages->page_size : 0;
     const size_t need = paged4_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim, capacity);
     if (need == 0) return cuda_fail(cudaErrorNoDevice, "attention_paged_q4: device query");
@@ -702,6 +714,7 @@ JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, i
         return arg_error("kv_evict_paged_q4: num_seqs * num_kv_heads * budget above 2^30");
     if (num_seqs == 0) return JYC_OK;
     if (!seq_lens || !new_table || !new_lens || !kept) return arg_error("kv_evict_paged_q4: null pointer");
+    if (askew(seq_lens, new_table, new_lens, kept)) return arg_error("kv_evict_paged_q4: misaligned array");
     if (seq_lens == new_lens) return arg_error("kv_evict_paged_q4: new_lens must be another array than seq_lens");
     PagedEvict4 e{};
     e.lens = seq_lens; e.budget = budget; e.recent = recent; e.KV = num_kv_heads; e.hd = head_dim;

@@ -548,10 +548,13 @@ int i8_few(const I8Gemm& g, I8Maps maps, int sms, cudaStream_t s) {
     if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, BN)) return e;
     const long long tiles = (long long)((g.n + kI8Rows - 1) / kI8Rows) * ((g.m + BN - 1) / BN);
     const int chunks = (g.k + kI8Chunk - 1) / kI8Chunk;
-    // parts of K: joining them costs about 3 us, so only where the tiles leave many SMs idle (32 tiles, 128 tokens of 4096 x
-    // 4096: TODO)
+    // parts of K where the tiles leave many SMs idle, two CTAs on each at most (behind a flushed L2, the launch among them:
+    // 128 tokens of 4096 x 4096, 32 tiles, 23 us in one part, 17 in four, 19 in eight; 48 tokens of 14336 x 4096, 112 tiles,
+    // 26 us in one or two, 30 in four); more of them for long rows only (one token of 4096 x 14336 23 us in four, 22 in
+    // eight; of 4096 x 4096 13.2 and 13.4)
+    const int most = chunks >= 64 ? 8 : 4;
     int parts = 1;
-    while (parts < 8 && tiles * 5 < 3 * sms && tiles * parts * 2 <= 2 * sms && chunks >= 4 * parts) parts *= 2;
+    while (parts < most && tiles * 5 < 3 * sms && tiles * parts <= sms && chunks >= 4 * parts) parts *= 2;
     return i8_start(i8_few_kernel<BN>, g, maps, dim3((g.n + kI8Rows - 1) / kI8Rows, (g.m + BN - 1) / BN, parts),
                     dim3(1, 1, parts), kI8Threads, I8Few<BN>::kSmem, s);
 }
@@ -577,6 +580,8 @@ int launch_i8_gemm(const I8Gemm& all, cudaStream_t s) {
     I8Maps maps{};
     if (int e = i8_map(&maps.w, g.W, g.n, g.k, g.ldw, kI8Rows)) return e;
     const long long tiles = (long long)((g.n + 2 * kI8Rows - 1) / (2 * kI8Rows)) * ((g.m + kI8PairTokens - 1) / kI8PairTokens);
+    // the pairs' tiles for a quarter of the SMs or more (129 tokens of 14336 x 4096 27 us, 29 in few tiles; 256 of 4096 x
+    // 4096 22 against 18)
     if (g.m > 128 && g.n > kI8Rows && tiles * 4 > sms) {
         if (int e = i8_map(&maps.a, g.A, g.m, g.k, g.lda, kI8PairTokens / 2)) return e;
         return i8_start(i8_pair_kernel, g, maps, dim3(2 * (unsigned)std::min<long long>(tiles, sms / 2)), dim3(2, 1, 1),

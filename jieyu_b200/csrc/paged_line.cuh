@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kPaJoinWarps * 32)
 // The same for teams, whose items go through more CTAs: blockIdx.y takes pa_wide_rows query rows of a team's rows.
 // One row at a time: the threads find the reference and the parts' factors, then each adds four dims over its share of the
 // parts, kPaWideLoads of them in flight, and the shares are added in shared memory. Small CTAs, as most find nothing to
-// join. (148 parts of 8 heads' 4 rows of 128: 10 us with 512 threads for 4 rows, TODO with these.)
+// join. (148 parts of 8 heads' 4 rows of 128: 8 us, about 10 with 512 threads for the 4 rows at once.)
 constexpr int kPaWideThreads = 128, kPaWideLoads = 16, kPaMaxCtas = 256;
 template <class G>
 __host__ __device__ constexpr int pa_wide_rows(int team) {

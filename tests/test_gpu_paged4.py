@@ -251,6 +251,57 @@ def test_attention(cuda, H, kv, hd, page, hf, rot, halves, gap, lens, mass):
         assert np.array_equal(now, before)
 
 
+# tensor copies of every row size and page, with gaps; head counts that teams of warps divide and do not
+COPIES = [  # H, kv, hd, page, heads_first, gap, lens
+    (32, 8, 128, 32, False, 1, [700, 64, 1]), (12, 6, 128, 16, False, 0, [1000, 17, 16]), (5, 5, 128, 64, False, 3, [333]),
+    (64, 16, 128, 64, True, 0, [129, 0, 2000]), (24, 12, 64, 32, False, 2, [95, 4000]), (8, 8, 64, 16, True, 0, [1, 15, 16, 17]),
+    (36, 3, 64, 64, False, 0, [65, 1300]), (72, 4, 128, 128, False, 0, [640, 1]), (30, 10, 256, 16, False, 1, [70, 500]),
+    (9, 9, 160, 8, True, 0, [260]), (14, 7, 100, 64, False, 0, [128, 3000]), (4, 2, 48, 32, False, 0, [33, 77]),
+]
+
+
+@pytest.mark.parametrize("H,kv,hd,page,hf,gap,lens", COPIES)
+def test_attention_by_every_copy(cuda, H, kv, hd, page, hf, gap, lens):
+    torch = cuda
+    rng = np.random.default_rng(H + hd)
+    pages, table = _table(rng, len(lens), max(lens) // page + 1)
+    pool = P4.Pool(torch, pages, page, kv, hd, table, hf, gap, fill=255)
+    pool.kp.fill_(float("nan"))  # rows that no length reaches, and gaps, hold NaN
+    pool.vp.fill_(float("inf"))
+    pool.mass.zero_()
+    filled = P4.Pool(torch, pages, page, kv, hd, table, hf, gap)
+    filled.put_random(rng, lens)
+    for b, n in enumerate(lens):
+        for j in range(n):
+            at = pool.where(b, j)
+            for x, y, w in ((pool.k, filled.k, 16 * pool.G), (pool.v, filled.v, 16 * pool.G), (pool.kp, filled.kp, pool.G),
+                            (pool.vp, filled.vp, pool.G)):
+                x[at][:, :w] = y[at][:, :w]
+    q, out = torch.randn(len(lens), H * hd, device="cuda"), torch.full((len(lens), H * hd), 8.0, device="cuda")
+    work = P4.workspace(torch, len(lens), H, kv, hd, table.shape[1] * page)
+    _capi.check(P4.attend(torch, pool, q, out, H, _ints(torch, lens), work=work))
+    _check(torch, rng, pool, q, out, [np.zeros((n, kv)) for n in lens], H, lens)
+
+
+def test_many_short_sequences(cuda):
+    """More sequences than a CTA has threads, most of them short or empty."""
+    torch = cuda
+    rng = np.random.default_rng(44)
+    kv, hd, H, page, seqs = 2, 64, 4, 16, 900
+    lens = rng.integers(0, 40, seqs)
+    lens[rng.random(seqs) < 0.3] = 0
+    lens[17] = 3000
+    pages, table = 3 * seqs + 188, np.zeros((seqs, 188), np.int64)
+    order = rng.permutation(pages)
+    table[:, :3] = order[: 3 * seqs].reshape(seqs, 3)
+    table[17] = order[3 * seqs:]
+    pool = P4.Pool(torch, pages, page, kv, hd, table)
+    pool.put_random(rng, None)
+    q, out = torch.randn(seqs, H * hd, device="cuda"), torch.full((seqs, H * hd), 8.0, device="cuda")
+    _capi.check(P4.attend(torch, pool, q, out, H, _ints(torch, lens)))
+    _check(torch, rng, pool, q, out, [np.zeros((max(n, 0), kv)) for n in lens], H, lens)
+
+
 def test_attention_without_a_workspace_and_again(cuda):
     """Scratch in stream order; a second call gives the same bits, and the masses twice the weight."""
     torch = cuda

@@ -225,3 +225,21 @@ def test_scaled_tables_refuse(args, scaling):
     buf = np.zeros(8 * 32, np.float32)
     assert _capi.load().jyc_rope_table_scaled(*args, _ref(scaling), buf.ctypes.data, buf.ctypes.data) == _capi.JYC_ERR_ARG
     assert "rope_table_scaled" in _capi.last_error()
+
+
+@pytest.mark.parametrize("call,names", [
+    (_append, ("K", "V", "seq", "pos", "rope_pos")), (lambda **k: _append(read=True, **k), ("K", "V", "seq", "pos")),
+    (_attend, ("Q", "out", "lens", "rope_pos")), (_evict, ("lens", "new", "new_lens", "kept")), (_turn, ("X", "Y", "pos"))])
+def test_misaligned_arrays_are_refused(call, names):
+    for name in names:
+        assert call(**{name: 4 * A + 2}) == _capi.JYC_ERR_ARG
+        assert "misaligned" in _capi.last_error()
+
+
+@pytest.mark.parametrize("name", ["a_scale", "w_scale", "bias", "C"])
+def test_misaligned_scales_are_refused(name):
+    d = dict(A=A, lda=112, a_scale=A, W=A, ldw=112, w_scale=A, bias=None, C=A, ldc=40, m=3, n=40, k=100)
+    d[name] = A + 1
+    assert _capi.load().jyc_matmul_i8(*d.values(), None) == _capi.JYC_ERR_ARG
+    assert "misaligned" in _capi.last_error()
+    assert _capi.load().jyc_quantize_rows_i8(A + 2, 100, 2, 100, A, 100, A, None) == _capi.JYC_ERR_ARG
