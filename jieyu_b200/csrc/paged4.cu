@@ -266,6 +266,30 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 
 // ---------------------------------------------------------------------------
 // Attention of one new token per sequence.
+//
+// Row j of a kv head is low_jg + step_jg q (group g of 32 dims). With the query as whole numbers x and their sums X_g:
+// s_j = qs sum_g (step_jg (x . q)_jg + low_jg X_g) / sqrt(hd), out = sum_j p_j (low_jg + step_jg q) / sum_j p_j.
+// Each product takes the form whose operands are exact on the tensor cores. Scores: keys are the rows, the query heads of a
+// kv head the columns; the dots x . q of a group are one mma.m16n8k32 of bytes (nibbles masked out of the stored words), made
+// floats by an exact subtraction and added with their step; low X is one mma.m16n8k16 of the stored (step, low) halves
+// against (0, X), X as two halves. Values: rows are dims, the stored words turned by ldmatrix.trans, each nibble masked into
+// a half (q - 8, or 16 times that) in two operations; the weight p_j step_jg as halves hi + lo, made from p's
+// halves by three fp16 operations (the product rounded, what that left, the low half's share); p (low + 8 step) is one product of the
+// stored halves. Steps are taken in units of 2^e of their group, e the largest exponent so far, so that a weight times a
+// step stays within fp16; a step 2^14 below another one of its group starts to lose bits, of 2^-25 of the larger one's
+// share at most. Each unit's product starts from zero and is added in fp32 with round to nearest (the tensor cores' own
+// sums may truncate).
+//
+// A step reads sum(len) * KV * 40 G bytes (G groups). The line of units, runs and joins are paged_line.cuh's; teams of
+// warps take the same keys of neighbouring kv heads, whose rows lie side by side in [page][slot][kv head] (262144 keys of 8 x
+// 128, without products: 95 us, 142 with every head at its own keys). Rows of 32 or 64 bytes come by tensor copies, others and
+// all parameters by cp.async. The reference follows the maximum of the scores; the accumulators are rescaled only where it or
+// a group's e moves.
+//
+// Measured: 131072 keys of 8 x 128 57 us (floor 26), 45 sequences of 1 to 8192 keys with their weights 91 us (floor 37), 513
+// keys of 2 x 64 15 us. At 131072 keys the copies alone, without products, take 45 of 54 us behind a flushed L2, about 20 of
+// them before the first and behind the last key (launches, run search, page table, first copies; parts and the second
+// kernel); issue slots are 42 % busy, the warps waiting for one another's results in chains of products and exchanges.
 __device__ __forceinline__ int p4_len(const PagedAttn4& a, int b) {
     int len = a.lens[b];
     if (len <= 0) return 0;
@@ -348,6 +372,14 @@ __device__ __forceinline__ void p4_fma2(float& x, float& y, float a, float b, fl
 }
 __device__ __forceinline__ __half2 p4_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t p4_u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+// the low (HIGH: the next 4) bits of each half as halves q - 8 (16 (q - 8)): 0x6400 | n is 1024 + n. (Left as they are, q 2^-24,
+// they are exact too, but the tensor cores do not shift subnormals up before they align products: 10 of the sums' 24 bits
+// went. Numbers around 0 keep the sums, which may be truncated, small.)
+template <bool HIGH>
+__device__ __forceinline__ uint32_t p4_whole(uint32_t x) {
+    return p4_u(__hsub2(p4_h2((x & (HIGH ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u),
+                        __half2half2(__ushort_as_half(HIGH ? 0x6480 : 0x6408))));
+}
 template <int N>
 __device__ __forceinline__ void p4_words(const uint32_t* p, uint32_t (&w)[N]) {  // N even
     if constexpr (N % 4 == 0) {
@@ -567,7 +599,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 
     // lane (g, t): query head g (and g + 8) as B fragments, bytes 4 t .. 4 t + 3 of every 16, its sums over groups as
     // halves; of the results the heads 2 t, 2 t + 1 (and 8 more), for which it keeps the reference, its share of the
-    // sum, the dims 2 g, 2 g + 1 of every 16 in units of 2^(eg - 15 + 24) of their group (the high 16 of a group 16 times
+    // sum, the dims 2 g, 2 g + 1 of every 16 in units of 2^(eg - 15) of their group (the high 16 of a group 16 times
     // that), and the products with column g (and g + 8) of V's parameters: (step, low) of each group
     uint32_t qf[GP][E][2], qsum[E][2 * LW];
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4], opar[E][2 * LW];
@@ -653,7 +685,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                     for (int i = 0; i < PW; i++) vrow[i] = 0u;
                 p4_words(vrow, vw[u]);
 #pragma unroll
-                for (int i = 0; i < GP; i++) top = __hmax2_nan(top, __hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i])));
+                for (int i = 0; i < GP; i++) top = __hmax2_nan(top, __habs2(__hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i]))));
             }
             if (__any_sync(0xffffffffu, !(__low2float(top) < 2.0f))) {  // a larger step than before
 #pragma unroll
@@ -848,7 +880,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
                 for (int i = 0; i < 2 * LW; i++) opar[e][i] += c[e][i];
         }
-        // P.V, a group at a time: V's numbers as subnormal halves (q * 2^-24, the high ones 16 times that), rows g dims 2 g,
+        // P.V, a group at a time: V's numbers less 8 as halves (the high ones 16 times that), rows g dims 2 g,
         // rows g + 8 dims 2 g + 1 of 16; a weight times a step as halves: hi rounded, lo what that left and lo's share.
         // 4 heads fill 8 columns with their hi and lo halves
         uint32_t zl[4 * U];
@@ -887,8 +919,8 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                     const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        const uint32_t mk = k ? 0x00F000F0u : 0x000F000Fu;
-                        const uint32_t vf[4] = {x0 & mk, y0 & mk, x1 & mk, y1 & mk};
+                        const uint32_t vf[4] = {k ? p4_whole<true>(x0) : p4_whole<false>(x0), k ? p4_whole<true>(y0) : p4_whole<false>(y0),
+                                                k ? p4_whole<true>(x1) : p4_whole<false>(x1), k ? p4_whole<true>(y1) : p4_whole<false>(y1)};
 #pragma unroll
                         for (int e = 0; e < E; e++) {
                             if (u == 0 && m == 0)
@@ -941,10 +973,13 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             }
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                const float f = __uint_as_float((uint32_t)(eg[d >> 1] + 9 + 127 - 4 * (d & 1)) << 23);
+                const float f = __uint_as_float((uint32_t)(eg[d >> 1] - 15 + 127 - 4 * (d & 1)) << 23);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float x = __shfl_sync(0xffffffffu, opar[e][2 * (d >> 3) + j], 4 * (2 * (d >> 1 & 3) + 1) + t) + z[j];
+                    // low + 8 step of the group's numbers
+                    const float par = opar[e][2 * (d >> 3) + j];
+                    const float x = __fmaf_rn(8.0f, __shfl_sync(0xffffffffu, par, 8 * (d >> 1 & 3) + t),
+                                              __shfl_sync(0xffffffffu, par, 8 * (d >> 1 & 3) + 4 + t)) + z[j];
                     o[d][e][j] = __fmaf_rn(o[d][e][j], f, x);
                     o[d][e][2 + j] = __fmaf_rn(o[d][e][2 + j], f, x);
                 }

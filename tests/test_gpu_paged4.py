@@ -341,6 +341,59 @@ def test_steps_of_every_size(cuda, H, kv, hd, page, scale):
     _check(torch, rng, pool, q, out, None, H, lens)
 
 
+@pytest.mark.parametrize("H,kv,hd,page,n", [(32, 8, 128, 64, 5000), (14, 2, 64, 16, 513), (8, 8, 64, 32, 3000),
+                                            (16, 1, 128, 32, 700), (6, 2, 80, 7, 900), (24, 1, 256, 16, 400),
+                                            (5, 5, 192, 64, 2000)])
+def test_attention_is_as_close_as_plain_fp32(cuda, H, kv, hd, page, n):
+    """The tolerance above is for roundings that all fall the same way. In the root mean square the result is no further from
+    the 64-bit one than four times what elementary fp32 operations are, and 2^-21 of its own size (weights as two halves)."""
+    torch = cuda
+    rng = np.random.default_rng(62)
+    pages, table = _table(rng, 1, n // page + 1)
+    pool = P4.Pool(torch, pages, page, kv, hd, table, mass=False)
+    pool.put_random(rng, [n])
+    q, out = 2 * torch.randn(1, H * hd, device="cuda"), torch.zeros(1, H * hd, device="cuda")
+    _capi.check(P4.attend(torch, pool, q, out, H, _ints(torch, [n])))
+    qi, qs = P.quantise(host(q).astype(np.float64).reshape(H, hd))
+    kq, kst, klo, vq, vst, vlo = pool.rows(0, n)
+    k, v = P4.values(kq, kst, klo), P4.values(vq, vst, vlo)
+    want, _ = P4.attention(qi, qs, k, v)
+    t = lambda x: torch.from_numpy(x.astype(np.float32)).cuda()  # noqa: E731
+    group = H // kv
+    s = torch.einsum("hgd,nhd->hgn", t(qi).reshape(kv, group, hd), t(k)) * (t(qs) / hd ** 0.5).reshape(kv, group, 1)
+    p = (s - s.amax(-1, keepdim=True)).exp()
+    plain = host(torch.einsum("hgn,nhd->hgd", p / p.sum(-1, keepdim=True), t(v)).reshape(H, hd)).astype(np.float64)
+    size = lambda x: np.sqrt(np.mean(x ** 2))  # noqa: E731
+    off = size(host(out).reshape(H, hd) - want)
+    assert off <= 4 * size(plain - want) + 2.0 ** -21 * size(want), (off / size(want), size(plain - want) / size(want))
+
+
+def test_parameters_of_either_sign(cuda):
+    """Values are low + step * q whatever the signs: rows that this library did not write."""
+    torch = cuda
+    rng = np.random.default_rng(61)
+    for H, kv, hd, page in ((8, 2, 128, 64), (12, 2, 64, 32), (3, 1, 192, 16)):
+        lens = [300, 65]
+        pages, table = _table(rng, 2, 300 // page + 1)
+        pool = P4.Pool(torch, pages, page, kv, hd, table)
+        pool.put_random(rng, lens)
+        for p in (pool.kp, pool.vp):
+            p.mul_(torch.from_numpy(rng.choice([-1.0, 1.0, 3.0, -0.01], tuple(p.shape))).cuda().half())
+        q, out = torch.randn(2, H * hd, device="cuda"), torch.zeros(2, H * hd, device="cuda")
+        _capi.check(P4.attend(torch, pool, q, out, H, _ints(torch, lens)))
+        _check_signed(torch, pool, q, out, H, lens)
+
+
+def _check_signed(torch, pool, q, out, H, lens):
+    x = host(q).astype(np.float64).reshape(len(lens), H, pool.hd)
+    for b, n in enumerate(lens):
+        qi, qs = P.quantise(x[b])
+        kq, kst, klo, vq, vst, vlo = pool.rows(b, n)
+        want, _ = P4.attention(qi, qs, P4.values(kq, kst, klo), P4.values(vq, vst, vlo))
+        tol = P4.out_tolerance(n, pool.G, P4.magnitudes(qi, qs, np.abs(kst), klo, pool.hd), (np.abs(vlo) + 15 * np.abs(vst)).max())
+        assert np.abs(host(out)[b].reshape(H, pool.hd) - want).max() <= tol
+
+
 def test_equal_and_extreme_scores(cuda):
     """Rows whose keys are all alike (weights 1 / n), and one key that takes all of the weight."""
     torch = cuda
