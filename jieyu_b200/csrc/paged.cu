@@ -50,16 +50,16 @@ int max_dynamic_smem(const void* kernel, int bytes) {
         const void* kernel;
         uint64_t devices;
     };
-    static Entry done[32];
+    static Entry done[96];
     static std::mutex mu;
     int dev = 0;
     JYC_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lk(mu);
     Entry* e = done;
-    while (e < done + 32 && e->kernel && e->kernel != kernel) e++;
-    if (e < done + 32 && e->kernel && dev < 64 && (e->devices >> dev & 1)) return JYC_OK;
+    while (e < done + 96 && e->kernel && e->kernel != kernel) e++;
+    if (e < done + 96 && e->kernel && dev < 64 && (e->devices >> dev & 1)) return JYC_OK;
     JYC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (e < done + 32 && dev < 64) {
+    if (e < done + 96 && dev < 64) {
         e->kernel = kernel;
         e->devices |= 1ull << dev;
     }

@@ -77,9 +77,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const float* X,
 __global__ void __launch_bounds__(kRopeThreads) rope_rows_odd_kernel(const float* X, int ldx, float* Y, int ldy, int H,
                                                                      int hd, const int* row_pos, RopeView r, int items,
                                                                      int chunks, int* err) {
-    const int row = blockIdx.x / chunks, f = (blockIdx.x - row * chunks) * kRopeThreads + threadIdx.x;
-    if (f >= H * items) return;
-    const int head = f / items, i = f - head * items;
+    const int row = blockIdx.x / chunks;
+    const unsigned f = (blockIdx.x - row * chunks) * kRopeThreads + threadIdx.x;  // up to 127 behind H * items < 2^31
+    if (f >= (unsigned)(H * items)) return;
+    const int head = (int)(f / items), i = (int)(f - head * items);
     const int pos = __ldg(row_pos + row);
     if (pos < 0) return;
     if (pos >= r.len) {

@@ -775,3 +775,139 @@ def test_a_serving_loop(cuda):
             pool.table = dev(torch, pool.table_host)
             lens = host(new_lens).astype(np.int64)
     assert evictions == 1 and np.all(lens == budget + steps - 33)
+
+
+def test_a_captured_step_replays_for_new_rows(cuda):
+    """Products, rotation, append, attention and eviction captured as one graph, without a workspace, give on every replay
+    the bits that the calls give."""
+    torch = cuda
+    rng = np.random.default_rng(31)
+    lib = _capi.load()
+    seqs, hidden, H, kv, hd, page, budget, width = 3, 96, 8, 2, 64, 16, 70, 12
+    wide = (H + 2 * kv) * hd
+    wd = dev(torch, rng.integers(-127, 128, (wide, hidden)).astype(np.int8))
+    wsd = dev(torch, rng.uniform(1e-3, 2e-3, wide).astype(np.float32))
+    cos, sin = P.tables(400, hd)
+    c, s = dev(torch, cos), dev(torch, sin)
+    rp = P4.rope(c, s, False)
+    new_width = -(-budget // page)
+    pages, both = _table(rng, seqs, width + new_width)
+    newd = _ints(torch, both[:, width:])
+    x, turn = torch.zeros(seqs, hidden, device="cuda"), _ints(torch, np.zeros(seqs))
+    pos, lens = _ints(torch, np.zeros(seqs)), _ints(torch, np.ones(seqs))
+
+    class Side:
+        def __init__(self):
+            self.pool = P4.Pool(torch, pages, page, kv, hd, both[:, :width])
+            self.xq = torch.zeros(seqs, hidden, dtype=torch.int8, device="cuda")
+            self.xs, self.qkv = torch.zeros(seqs, device="cuda"), torch.zeros(seqs, wide, device="cuda")
+            self.out = torch.zeros(seqs, H * hd, device="cuda")
+            self.nl = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+            self.kept = torch.zeros(seqs, kv, budget, dtype=torch.int32, device="cuda")
+
+        def step(self):
+            st, qkv = P4.stream_of(torch), self.qkv.data_ptr()
+            _capi.check(lib.jyc_quantize_rows_i8(x.data_ptr(), hidden, seqs, hidden, self.xq.data_ptr(), hidden,
+                                                 self.xs.data_ptr(), st))
+            _capi.check(lib.jyc_matmul_i8(self.xq.data_ptr(), hidden, self.xs.data_ptr(), wd.data_ptr(), hidden,
+                                          wsd.data_ptr(), None, qkv, wide, seqs, wide, hidden, st))
+            _capi.check(lib.jyc_rope_rows(qkv, wide, qkv, wide, seqs, H + kv, hd, turn.data_ptr(), P4.ref(rp), st))
+            k = qkv + 4 * H * hd
+            _capi.check(P4.append(torch, self.pool, k, k + 4 * kv * hd, wide, seqs, None, pos))
+            _capi.check(P4.attend(torch, self.pool, self.qkv, self.out, H, lens))
+            _capi.check(P4.evict(torch, self.pool, lens, budget, 8, newd, self.nl, self.kept))
+
+        def state(self):
+            p = self.pool
+            return [host(t).copy() for t in (self.qkv, self.out, self.nl, self.kept, p.k, p.v, p.kp, p.vp, p.mass)]
+
+    once, again = Side(), Side()
+    state = rng.integers(0, 1000)
+    for side in (once, again):
+        side.pool.put_random(np.random.default_rng(state), None)
+        side.pool.mass.copy_(torch.from_numpy(np.random.default_rng(state).random(tuple(side.pool.mass.shape)).astype(np.float32)))
+        side.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again.step()
+    for n in ([192, 1, 70], [5, 71, 150], [100, 100, 100]):
+        x.normal_()
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        pos.copy_(lens - 1)
+        turn.copy_(lens + 200)
+        once.step()
+        graph.replay()
+        for got, want in zip(again.state(), once.state()):
+            assert np.array_equal(got, want)
+        assert list(host(again.nl)) == [min(m, budget) for m in n]
+
+
+def test_appends_and_evictions_on_two_streams(cuda):
+    """Calls on two streams, of other sequences of one cache, give what they give one after another."""
+    torch = cuda
+    rng = np.random.default_rng(32)
+    kv, hd, page, n, budget = 2, 64, 64, 6000, 500
+    width, new_width = -(-n // page), -(-budget // page)
+    pages, both = _table(rng, 2, width + new_width)
+    K, V = (torch.randn(n, kv * hd, device="cuda") for _ in range(2))
+    pos = _ints(torch, np.arange(n))
+    weight = torch.from_numpy(rng.random((pages, page, kv)).astype(np.float32)).cuda()
+    results = []
+    for overlap in (False, True):
+        pools = [P4.Pool(torch, pages, page, kv, hd, both[b: b + 1, :width]) for b in range(2)]
+        shared = pools[0]
+        for name in ("k", "v", "kp", "vp", "mass"):
+            setattr(pools[1], name, getattr(shared, name))
+        pools[1].desc = shared.desc
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        seq, lens = _ints(torch, np.zeros(n)), _ints(torch, [n])
+        nl, kept = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.zeros(2, 1, kv, budget, dtype=torch.int32, device="cuda")
+        news = [_ints(torch, both[b: b + 1, width:]) for b in range(2)]
+        torch.cuda.synchronize()
+        for b, st in enumerate(streams):
+            _capi.check(P4.append(torch, pools[b], K.data_ptr(), V.data_ptr(), kv * hd, n, seq, pos, stream=st.cuda_stream))
+            if not overlap:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        shared.mass.copy_(weight)
+        torch.cuda.synchronize()
+        for b, st in enumerate(streams):
+            _capi.check(P4.evict(torch, pools[b], lens, budget, 20, news[b], nl[b], kept[b], stream=st.cuda_stream))
+            if not overlap:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append([host(t).copy() for t in (shared.k, shared.v, shared.kp, shared.vp, shared.mass, nl, kept)])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
+    w = host(weight)
+    for b in range(2):
+        m = w[both[b, np.arange(n) // page], np.arange(n) % page]
+        for h in range(kv):
+            assert np.array_equal(results[0][-1][b, 0, h], P4.kept_rows(m[:, h], n, budget, 20))
+
+
+def test_tables_without_room(cuda):
+    """table_stride 0: no sequence has a place, empty ones give zeros and keep nothing."""
+    torch = cuda
+    lib = _capi.load()
+    pool = P4.Pool(torch, 1, 16, 2, 64, np.zeros((2, 1)), fill=5)
+    pool.table = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    some = torch.zeros(4, dtype=torch.int32, device="cuda")
+    mass = pool.mass
+    q, out = torch.randn(2, 4 * 64, device="cuda"), torch.full((2, 4 * 64), 3.0, device="cuda")
+    for lens, bits in (([0, 0], 0), ([1, 0], 1)):
+        n = _ints(torch, lens)
+        _capi.check(lib.jyc_attention_paged_q4(q.data_ptr(), 256, out.data_ptr(), 256, 4, 2, 64, n.data_ptr(), some.data_ptr(),
+                                               0, 2, None, None, P4.ref(pool.desc), None, 0, P4.stream_of(torch)))
+        assert not host(out).any() and lib.jyc_paged_error(1) == bits
+        out.fill_(3.0)
+    x = torch.randn(2, 128, device="cuda")
+    _capi.check(lib.jyc_kv_append_paged_q4(x.data_ptr(), x.data_ptr(), 128, 2, 2, 64, None, some.data_ptr(), some.data_ptr(), 0,
+                                           2, None, None, P4.ref(pool.desc), P4.stream_of(torch)))
+    assert lib.jyc_paged_error(1) == 1
+    assert np.all(host(pool.k) == 5) and np.all(host(mass) == 5.0)
+    kept, nl = (torch.full(s, 9, dtype=torch.int32, device="cuda") for s in ((2, 2, 8), (2,)))
+    _capi.check(lib.jyc_kv_evict_paged_q4(_ints(torch, [0, 0]).data_ptr(), 8, 2, 2, 64, some.data_ptr(), 0, 2, some.data_ptr(), 1,
+                                          nl.data_ptr(), kept.data_ptr(), P4.ref(pool.desc), P4.stream_of(torch)))
+    assert np.all(host(kept) == -1) and np.all(host(nl) == 0)
