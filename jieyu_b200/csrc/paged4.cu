@@ -100,10 +100,9 @@ __device__ __forceinline__ uint32_t p4_bytes(float4 x, float low, float inv) {
 }
 
 // Four lanes hold a group: lane i its dims 4 i .. 4 i + 3 and 16 more, whose numbers are the low and the high bits of its
-// word; the group's range is two exchanges. Pairs that lie on quads turn by table entries that a lane reads once for all
-// of its heads. (A lane with four dims needs three, and the high bits of another lane.) 121 instructions a head of 128 and
-// warp, and bound by them: 16384 rows of 8 x 128 44 us (floor 24); 60 us with the rotation's form chosen value by value, 72
-// with four dims a lane, at 231 instructions.
+// word; the group's range is two exchanges. Of four heads in flight each lane makes one's parameters and passes them on. Pairs that lie on
+// quads turn by table entries that a lane reads once for all of its heads. Measured: 16384 rows of 8 x 128 36 us (floor
+// 24), 45 where every lane makes the parameters of all heads, 60 with the rotation's form chosen value by value, 72 with four dims a lane.
 enum { P4_PLAIN = 0, P4_PAIRS = 1, P4_HALVES = 2, P4_ODD = 3 };  // how K turns
 template <int LANES, int UNITS, int MODE>
 __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* K, const float* V, int ld, int rows,
@@ -189,30 +188,62 @@ __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* 
     if (!p4_valid(kv, x.page)) return;
     uint8_t* dst = (x.is_k ? kv.p.k : kv.p.v) + p4_off(kv.p, x.page, x.slot, x.head) + 4 * sub;
     uint32_t* par = reinterpret_cast<uint32_t*>(x.is_k ? kv.p.kp : kv.p.vp) + p4_poff(kv.p, x.page, x.slot, x.head) + group;
+    float lo[UNITS], hi[UNITS], inv[UNITS];
+    uint32_t p[UNITS];
 #pragma unroll
     for (int i = 0; i < UNITS; i++) {
         const float4 a = v[i][0], c = v[i][1];
-        float lo = INFINITY, hi = -INFINITY;
+        lo[i] = INFINITY;
+        hi[i] = -INFINITY;
         if (in0) {
-            lo = fminf(fminf(a.x, a.y), fminf(a.z, a.w));
-            hi = fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w));
+            lo[i] = fminf(fminf(a.x, a.y), fminf(a.z, a.w));
+            hi[i] = fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w));
         }
         if (in1) {
-            lo = fminf(lo, fminf(fminf(c.x, c.y), fminf(c.z, c.w)));
-            hi = fmaxf(hi, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
+            lo[i] = fminf(lo[i], fminf(fminf(c.x, c.y), fminf(c.z, c.w)));
+            hi[i] = fmaxf(hi[i], fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
         }
+    }
+    // the group's range over its four lanes, then its parameters: of four units each lane makes (and stores) one's
+    const int own = UNITS == 4 ? sub & 3 : 0;
+    float low, high;
+    if constexpr (UNITS == 4) {
+        const bool b1 = sub & 2, b0 = sub & 1;
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int i = 0; i < 2; i++) {
+            lo[i] = fminf(b1 ? lo[i + 2] : lo[i], __shfl_xor_sync(0xffffffffu, b1 ? lo[i] : lo[i + 2], 2));
+            hi[i] = fmaxf(b1 ? hi[i + 2] : hi[i], __shfl_xor_sync(0xffffffffu, b1 ? hi[i] : hi[i + 2], 2));
         }
-        const uint32_t p = p4_params(lo, hi);
-        const float step = p4_step(p), low = p4_low(p), inv = step > 0.0f ? __fdiv_rn(1.0f, step) : 0.0f;
-        const uint32_t w = (in0 ? p4_bytes(a, low, inv) : 0u) | (in1 ? p4_bytes(c, low, inv) << 4 : 0u);
-        if (x.head + i * SIDE >= KV || group >= groups) continue;
-        *reinterpret_cast<uint32_t*>(dst + i * SIDE * kv.p.head_stride) = w;
-        if ((sub & 3) == 0) par[i * SIDE * kv.p.phead_stride] = p;
-        if (x.is_k && sub == 0 && kv.p.mass) kv.p.mass[p4_moff(kv.p, x.page, x.slot, x.head + i * SIDE)] = 0.0f;
+        low = fminf(b0 ? lo[1] : lo[0], __shfl_xor_sync(0xffffffffu, b0 ? lo[0] : lo[1], 1));
+        high = fmaxf(b0 ? hi[1] : hi[0], __shfl_xor_sync(0xffffffffu, b0 ? hi[0] : hi[1], 1));
+    } else {
+        static_assert(UNITS == 1 || UNITS == 4, "");
+        low = fminf(lo[0], __shfl_xor_sync(0xffffffffu, lo[0], 1));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 2));
+        high = fmaxf(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], 1));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+    }
+    p[0] = p4_params(low, high);
+    inv[0] = p4_step(p[0]) > 0.0f ? __frcp_rn(p4_step(p[0])) : 0.0f;
+    const int head = x.head + own * SIDE;
+    if (head < KV && group < groups && (UNITS == 4 || (sub & 3) == 0)) {
+        par[own * SIDE * kv.p.phead_stride] = p[0];
+        if (x.is_k && sub < 4 && kv.p.mass) kv.p.mass[p4_moff(kv.p, x.page, x.slot, head)] = 0.0f;
+    }
+    if constexpr (UNITS == 4) {
+        const uint32_t mine = p[0];
+        const float inverse = inv[0];
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            p[i] = __shfl_sync(0xffffffffu, mine, i, 4);
+            inv[i] = __shfl_sync(0xffffffffu, inverse, i, 4);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < UNITS; i++) {
+        const float base = p4_low(p[i]);
+        const uint32_t w = (in0 ? p4_bytes(v[i][0], base, inv[i]) : 0u) | (in1 ? p4_bytes(v[i][1], base, inv[i]) << 4 : 0u);
+        if (x.head + i * SIDE < KV && group < groups) *reinterpret_cast<uint32_t*>(dst + i * SIDE * kv.p.head_stride) = w;
     }
 }
 
@@ -1184,7 +1215,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     if (tiles > 1)  // else an item is one unit: none is split
         if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, (G::ROWS * pl.team + pa_wide_rows<G>(pl.team) - 1) / pa_wide_rows<G>(pl.team)), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
-    const long long heads = (long long)a.kv.num_seqs * a.KV, most = (capacity + kP4MassThreads * kP4MassKeys - 1) / (kP4MassThreads * kP4MassKeys);
+    const long long heads = (long long)a.kv.num_seqs * a.KV, most = ((long long)capacity + kP4MassThreads * kP4MassKeys - 1) / (kP4MassThreads * kP4MassKeys);
     const unsigned chunks = (unsigned)std::min({most, (32LL * sms + heads - 1) / heads, 65535LL});
     return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
 }
@@ -1471,7 +1502,7 @@ int launch_paged4_append(const float* K, const float* V, int ld, int rows, int K
     const bool vec = aligned16(K, ld) && aligned16(V, ld), wide = vec && rope_wide(rope);
     const int lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, side = 32 / lanes;
     // four blocks of heads a warp where the rows have them and fill the SMs so: less bookkeeping a head; one otherwise
-    // (with the read-back: 16384 rows of 8 x 128 75 us, 83 with one; 8 rows 13 us with either)
+    // (with the read-back: 16384 rows of 8 x 128 66 us, 83 with one; 8 rows 13 us with either)
     const bool many = KV > 2 * side && (long long)rows * KV >= 64LL * sm_count();
     const int mode = !rope.cos_t ? P4_PLAIN : !wide ? P4_ODD : rope.halves ? P4_HALVES : P4_PAIRS;
     const auto kernel = many ? (lanes == 4    ? append_of<4, 4>(mode)
