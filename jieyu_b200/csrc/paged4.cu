@@ -445,6 +445,7 @@ __host__ __device__ constexpr int p4_query_bytes(int gp) { return 40 * gp + 16; 
 // itself this took 7 of the first 10 us of every run, for the instructions of all forms of the rotation; here it runs
 // while that kernel finds its runs and requests its first keys.)
 __global__ void __launch_bounds__(128) paged4_query_kernel(PagedAttn4 a, int gp, bool wide_q, bool wide_rope, unsigned char* out) {
+    griddep_wait();  // before the next kernel may start: it reads what stood here before this one
     griddep_launch();
     const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, b = (int)(i / a.H), h = (int)(i - (long long)b * a.H);
@@ -1204,8 +1205,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     p4_work<GP, HEADS, TMA>(sms, a.kv.num_seqs, a.H, a.KV, p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc,
                             &queries);
     const long long rows = (long long)a.kv.num_seqs * a.H;
-    paged4_query_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a, GP, pl.wide_q, pl.wide_rope, queries);
-    JYC_LAUNCHED();
+    if (int e = p4_follow(paged4_query_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, a, GP, pl.wide_q, pl.wide_rope, queries)) return e;
     // a key's parameters by one copy where their alignment allows it, else word by word
     const uintptr_t at = (uintptr_t)p.kp | (uintptr_t)p.vp | (uintptr_t)(4 * (p.ppage_stride | p.ppos_stride | p.phead_stride));
     const int copy = groups == GP && at % (4 * GP) == 0 ? 4 * GP : 4;
