@@ -13,6 +13,7 @@
 // 12.1 would do); 48 tokens of 14336 x 4090 23 us (floor 9.5), one token of 4096 x 4096 12.5 us (floor 2.6): two launches and
 // the first and last steps of a CTA (tensor memory, first copies, results) are half of it.
 #include "i8.cuh"
+#include "follow.cuh"
 #include "kernels.cuh"
 #include "mega.cuh"
 #include "paged.cuh"
@@ -35,6 +36,7 @@ __global__ void __launch_bounds__(kQrThreads) quantize_rows_kernel(const float* 
                                                                    float* scale) {
     __shared__ float s_max[kQrThreads / 32];
     const int tid = threadIdx.x;
+    griddep_wait();
     griddep_launch();  // a product that follows may prepare itself
     const float* row = x + (size_t)blockIdx.x * ldx;
     int8_t* to = q + (size_t)blockIdx.x * ldq;
@@ -573,9 +575,7 @@ int launch_quantize_rows(const float* x, int ldx, int rows, int k, int8_t* q, in
                         : quads <= 1        ? quantize_rows_kernel<1>
                         : quads <= 4        ? quantize_rows_kernel<4>
                                             : quantize_rows_kernel<16>;
-    kernel<<<rows, kQrThreads, 0, s>>>(x, ldx, k, q, ldq, scale);
-    JYC_LAUNCHED();
-    return JYC_OK;
+    return launch_follow(kernel, dim3(rows), kQrThreads, 0, s, x, ldx, k, q, ldq, scale);
 }
 
 int launch_i8_gemm(const I8Gemm& all, cudaStream_t s) {

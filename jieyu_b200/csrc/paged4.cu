@@ -3,6 +3,7 @@
 // (the scores and softmax of attention_q8, libs/model_libs/attention/attention_q8.h:38-184), which leaves
 // each key's weight on it, and the rows of least weight are left behind.
 #include "paged4.cuh"
+#include "follow.cuh"
 #include "paged_line.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* 
                                                                    const int* row_pos, const int* rope_pos,
                                                                    PagedKV4 kv, RopeView rope, int chunks,
                                                                    FastDiv by_row, bool vec) {
+    griddep_wait();
     constexpr int SIDE = 32 / LANES;
     const int sub = threadIdx.x & (LANES - 1), group = sub >> 2, d0 = 32 * group + 4 * (sub & 3), groups = (hd + 31) >> 5;
     const P4Row x = p4_row<LANES, UNITS>(rows, chunks, by_row, row_seq, row_pos, kv);
@@ -253,6 +255,7 @@ template <int LANES, int QUADS>
 __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float* V, int ld, int rows, int KV, int hd,
                                                                  const int* row_seq, const int* row_pos, PagedKV4 kv,
                                                                  int chunks, FastDiv by_row, bool vec) {
+    griddep_wait();
     constexpr int SIDE = 32 / LANES;
     const int sub = threadIdx.x & (LANES - 1), nq = hd >> 2;
     const P4Row x = p4_row<LANES, kP4Units>(rows, chunks, by_row, row_seq, row_pos, kv);
@@ -445,7 +448,7 @@ __host__ __device__ constexpr int p4_query_bytes(int gp) { return 40 * gp + 16; 
 // itself this took 7 of the first 10 us of every run, for the instructions of all forms of the rotation; here it runs
 // while that kernel finds its runs and requests its first keys.)
 __global__ void __launch_bounds__(128) paged4_query_kernel(PagedAttn4 a, int gp, bool wide_q, bool wide_rope, unsigned char* out) {
-    griddep_wait();  // before the next kernel may start: it reads what stood here before this one
+    griddep_wait();  // first: the next kernel reads lengths, tables and pages before it waits for this one
     griddep_launch();
     const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, b = (int)(i / a.H), h = (int)(i - (long long)b * a.H);
@@ -1130,24 +1133,6 @@ size_t p4_work(int ctas, int seqs, int H, int KV, int capacity, unsigned char* b
     return score + (size_t)seqs * KV * qblocks * keys * sizeof(float);
 }
 
-// A launch behind the last one, which it waits for by itself.
-template <class... Params, class... Args>
-int p4_follow(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    JYC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-    JYC_LAUNCHED();
-    return JYC_OK;
-}
-
 // Map of a cache array as [page][slot][kv head][byte], boxes of `box` slots of one head.
 int p4_map(CUtensorMap* m, uint8_t* base, const PagedAttn4& a, int row, int box) {
     void* fn = nullptr;
@@ -1205,19 +1190,19 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     p4_work<GP, HEADS, TMA>(sms, a.kv.num_seqs, a.H, a.KV, p.mass ? capacity : 0, static_cast<unsigned char*>(work), &w, &sc,
                             &queries);
     const long long rows = (long long)a.kv.num_seqs * a.H;
-    if (int e = p4_follow(paged4_query_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, a, GP, pl.wide_q, pl.wide_rope, queries)) return e;
+    if (int e = launch_follow(paged4_query_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, a, GP, pl.wide_q, pl.wide_rope, queries)) return e;
     // a key's parameters by one copy where their alignment allows it, else word by word
     const uintptr_t at = (uintptr_t)p.kp | (uintptr_t)p.vp | (uintptr_t)(4 * (p.ppage_stride | p.ppos_stride | p.phead_stride));
     const int copy = groups == GP && at % (4 * GP) == 0 ? 4 * GP : 4;
-    if (int e = p4_follow(paged4_attention_kernel<GP, HEADS, TMA>, dim3(ctas), G::WARPS * 32, G::SMEM, s, a, pl, w, sc,
+    if (int e = launch_follow(paged4_attention_kernel<GP, HEADS, TMA>, dim3(ctas), G::WARPS * 32, G::SMEM, s, a, pl, w, sc,
                           (const unsigned char*)queries, copy, maps))
         return e;
     if (tiles > 1)  // else an item is one unit: none is split
-        if (int e = p4_follow(paged_join_wide_kernel<G>, dim3(ctas, (G::ROWS * pl.team + pa_wide_rows<G>(pl.team) - 1) / pa_wide_rows<G>(pl.team)), kPaWideThreads, 0, s, a, pl, w)) return e;
+        if (int e = launch_follow(paged_join_wide_kernel<G>, dim3(ctas, (G::ROWS * pl.team + pa_wide_rows<G>(pl.team) - 1) / pa_wide_rows<G>(pl.team)), kPaWideThreads, 0, s, a, pl, w)) return e;
     if (!sc.s) return JYC_OK;
     const long long heads = (long long)a.kv.num_seqs * a.KV, most = ((long long)capacity + kP4MassThreads * kP4MassKeys - 1) / (kP4MassThreads * kP4MassKeys);
     const unsigned chunks = (unsigned)std::min({most, (32LL * sms + heads - 1) / heads, 65535LL});
-    return p4_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
+    return launch_follow(paged4_mass_kernel<G::ROWS>, dim3((unsigned)heads, chunks), kP4MassThreads, 0, s, a, pl, w, sc);
 }
 
 // The instantiation of a shape: groups and query heads per unit rounded up.
@@ -1267,6 +1252,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) paged4_select_kernel(PagedEvict
     int* const sums = ev_sm + 32 * kEvBins;   // [digit][bin]: this CTA's
     uint32_t* const keys = reinterpret_cast<uint32_t*>(ev_sm + (32 + kEvDigits) * kEvBins);
     __shared__ int s_warp[kEvWarps], s_digit, s_above, s_count[2], s_more[kEvWarps], s_equal[kEvWarps];
+    griddep_wait();
     griddep_launch();
     const int rank = blockIdx.x % ctas, item = blockIdx.x / ctas, b = item / e.KV, h = item - b * e.KV;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1479,8 +1465,7 @@ int row_launches(int rows, int KV, int per, F f) {
     const int chunks = (KV + per - 1) / per, most = std::max(1, (1 << 30) / (2 * chunks)), warps = kP4Threads / 32;
     for (int r0 = 0; r0 < rows; r0 += most) {
         const int n = std::min(most, rows - r0);
-        f(r0, n, (unsigned)(((long long)n * 2 * chunks + warps - 1) / warps), chunks);
-        JYC_LAUNCHED();
+        if (int e = f(r0, n, (unsigned)(((long long)n * 2 * chunks + warps - 1) / warps), chunks)) return e;
         if (rows - r0 <= most) break;
     }
     return JYC_OK;
@@ -1514,10 +1499,9 @@ int launch_paged4_append(const float* K, const float* V, int ld, int rows, int K
                                 : lanes == 16 ? append_of<16, 1>(mode)
                                               : append_of<32, 1>(mode));
     return row_launches(rows, KV, (many ? 4 : 1) * side, [&](int r0, int n, unsigned grid, int chunks) {
-        kernel<<<grid, kP4Threads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
-                                           row_seq ? row_seq + r0 : nullptr, row_pos + r0,
-                                           rope_pos ? rope_pos + r0 : nullptr, shifted(kv, row_seq, r0), rope, chunks,
-                                           fast_div(2 * chunks), vec);
+        return launch_follow(kernel, dim3(grid), kP4Threads, 0, s, K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
+                             row_seq ? row_seq + r0 : nullptr, row_pos + r0, rope_pos ? rope_pos + r0 : nullptr,
+                             shifted(kv, row_seq, r0), rope, chunks, fast_div(2 * chunks), vec);
     });
 }
 
@@ -1529,9 +1513,9 @@ int launch_paged4_read(float* K, float* V, int ld, int rows, int KV, int hd, con
                         : hd <= 128 ? paged4_read_kernel<32, 1>
                                     : paged4_read_kernel<32, 2>;
     return row_launches(rows, KV, kP4Units * (32 / (hd <= 32 ? 8 : hd <= 64 ? 16 : 32)), [&](int r0, int n, unsigned grid, int chunks) {
-        kernel<<<grid, kP4Threads, 0, s>>>(K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
-                                           row_seq ? row_seq + r0 : nullptr, row_pos + r0, shifted(kv, row_seq, r0),
-                                           chunks, fast_div(2 * chunks), vec);
+        return launch_follow(kernel, dim3(grid), kP4Threads, 0, s, K + (size_t)r0 * ld, V + (size_t)r0 * ld, ld, n, KV, hd,
+                             row_seq ? row_seq + r0 : nullptr, row_pos + r0, shifted(kv, row_seq, r0), chunks,
+                             fast_div(2 * chunks), vec);
     });
 }
 
@@ -1569,18 +1553,20 @@ int launch_paged4_evict(const PagedEvict4& e, cudaStream_t s) {
     cfg.blockDim = dim3(kEvThreads);
     cfg.dynamicSmemBytes = kEvSmem;
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = ctas;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     JYC_CUDA(cudaLaunchKernelEx(&cfg, paged4_select_kernel, e, ctas));
     JYC_LAUNCHED();
     const int groups = (e.hd + 31) / 32, lanes = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
     const long long rows = (long long)items * e.budget, per = (long long)kMvThreads / lanes * kMvRows;
     const auto kernel = lanes == 1 ? paged4_move_kernel<1> : lanes == 2 ? paged4_move_kernel<2> : lanes == 4 ? paged4_move_kernel<4> : paged4_move_kernel<8>;
-    return p4_follow(kernel, dim3((unsigned)((rows + per - 1) / per)), kMvThreads, 0, s, e, fast_div(e.budget), fast_div(e.KV),
+    return launch_follow(kernel, dim3((unsigned)((rows + per - 1) / per)), kMvThreads, 0, s, e, fast_div(e.budget), fast_div(e.KV),
                      e.kv.by_page);
 }
 

@@ -1,6 +1,8 @@
 // rope.cu — rotary positions of rows (rope_pos's rotation, libs/model_libs/rope/rope.h:108-110, for any row
 // positions, both pair layouts and a part of the head).
 #include "rope.cuh"
+#include "follow.cuh"
+#include "ptx.cuh"
 
 #include <algorithm>
 
@@ -20,6 +22,7 @@ template <bool HALVES>
 __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const float* X, int ldx, float* Y, int ldy, int H,
                                                                  int hd, const int* row_pos, RopeView r, int items,
                                                                  int side, int steps, int chunks, int* err) {
+    griddep_wait();
     const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks, at = threadIdx.x / items;
     if (at >= side) return;
     const int i = threadIdx.x - at * items, rot = 2 * r.half, turning = HALVES ? r.half / 4 : rot / 4;
@@ -77,6 +80,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const float* X,
 __global__ void __launch_bounds__(kRopeThreads) rope_rows_odd_kernel(const float* X, int ldx, float* Y, int ldy, int H,
                                                                      int hd, const int* row_pos, RopeView r, int items,
                                                                      int chunks, int* err) {
+    griddep_wait();
     const int row = blockIdx.x / chunks;
     const unsigned f = (blockIdx.x - row * chunks) * kRopeThreads + threadIdx.x;  // up to 127 behind H * items < 2^31
     if (f >= (unsigned)(H * items)) return;
@@ -118,16 +122,13 @@ int launch_rope_rows(const float* X, int ldx, float* Y, int ldy, int rows, int H
         const int n = std::min(most, rows - r0);
         const float* x = X + (size_t)r0 * ldx;
         float* y = Y + (size_t)r0 * ldy;
-        if (!wide)
-            rope_rows_odd_kernel<<<(unsigned)n * chunks, kRopeThreads, 0, s>>>(x, ldx, y, ldy, H, hd, row_pos + r0, r, items,
-                                                                               chunks, err);
-        else if (r.halves)
-            rope_rows_kernel<true><<<(unsigned)n * chunks, kRopeThreads, 0, s>>>(x, ldx, y, ldy, H, hd, row_pos + r0, r,
-                                                                                 items, side, steps, chunks, err);
-        else
-            rope_rows_kernel<false><<<(unsigned)n * chunks, kRopeThreads, 0, s>>>(x, ldx, y, ldy, H, hd, row_pos + r0, r,
-                                                                                  items, side, steps, chunks, err);
-        JYC_LAUNCHED();
+        const dim3 grid((unsigned)n * chunks);
+        const auto kernel = r.halves ? rope_rows_kernel<true> : rope_rows_kernel<false>;
+        if (int e = wide ? launch_follow(kernel, grid, kRopeThreads, 0, s, x, ldx, y, ldy, H, hd, row_pos + r0, r, items, side,
+                                         steps, chunks, err)
+                         : launch_follow(rope_rows_odd_kernel, grid, kRopeThreads, 0, s, x, ldx, y, ldy, H, hd, row_pos + r0, r,
+                                         items, chunks, err))
+            return e;
         if (rows - r0 <= most) break;
     }
     return JYC_OK;
