@@ -8,9 +8,9 @@
 // (TMA) in the 128-byte swizzle that the products read. Copies fill what lies outside of A, W and k with zeros, so edges
 // need no care but at the stores. Whole-number sums are exact, so K may be split in any way with the same result.
 //
-// Measured, with the rows' quantising: 4096 tokens of 14336 x 4096 220 us, of them 17 quantising (the product alone 177 us
+// Measured, with the rows' quantising: 4096 tokens of 14336 x 4096 219 us, of them 17 quantising (the product alone 177 us
 // back to back, 2.7 P operations a second; 151 without its stores, 140 without copies and stores, 13 rounds of tiles where
-// 12.1 would do); 48 tokens of 14336 x 4090 23 us (floor 9.5), one token of 4096 x 4096 12.5 us (floor 2.6): two launches and
+// 12.1 would do); 48 tokens of 14336 x 4090 22 us (floor 9.5), one token of 4096 x 4096 12 us (floor 2.6): two launches and
 // the first and last steps of a CTA (tensor memory, first copies, results) are half of it.
 #include "i8.cuh"
 #include "follow.cuh"

@@ -101,9 +101,10 @@ __device__ __forceinline__ uint32_t p4_bytes(float4 x, float low, float inv) {
 }
 
 // Four lanes hold a group: lane i its dims 4 i .. 4 i + 3 and 16 more, whose numbers are the low and the high bits of its
-// word; the group's range is two exchanges. Of four heads in flight each lane makes one's parameters and passes them on. Pairs that lie on
-// quads turn by table entries that a lane reads once for all of its heads. Measured: 16384 rows of 8 x 128 36 us (floor
-// 24), 45 where every lane makes the parameters of all heads, 60 with the rotation's form chosen value by value, 72 with four dims a lane.
+// word; the group's range is two exchanges. Of four heads in flight each lane makes one's parameters and passes them on.
+// Pairs that lie on quads turn by table entries that a lane reads once for all of its heads. Bound by its instructions, 84
+// a head of 128 and warp: 16384 rows of 8 x 128 33 us (floor 24), 45 where every lane makes the parameters of all heads, 60 with the rotation's
+// form chosen value by value too, 72 with four dims a lane.
 enum { P4_PLAIN = 0, P4_PAIRS = 1, P4_HALVES = 2, P4_ODD = 3 };  // how K turns
 template <int LANES, int UNITS, int MODE>
 __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* K, const float* V, int ld, int rows,
@@ -320,10 +321,10 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 // all parameters by cp.async. The reference follows the maximum of the scores; the accumulators are rescaled only where it or
 // a group's e moves.
 //
-// Measured: 131072 keys of 8 x 128 57 us (floor 26), 45 sequences of 1 to 8192 keys with their weights 91 us (floor 37), 513
-// keys of 2 x 64 15 us. At 131072 keys the copies alone, without products, take 45 of 54 us behind a flushed L2, about 20 of
-// them before the first and behind the last key (launches, run search, page table, first copies; parts and the second
-// kernel); issue slots are 42 % busy, the warps waiting for one another's results in chains of products and exchanges.
+// Measured: 131072 keys of 8 x 128 60 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-105 us (floor
+// 37), 513 keys of 2 x 64 14 us. At 131072 keys about 20 us pass before the first and behind the last key (launches, run
+// search, page table, first copies; parts and the join); between them issue slots are 54 % busy, the warps waiting for one
+// another's results in chains of products and exchanges (the copies without products take 45 us behind a flushed L2).
 __device__ __forceinline__ int p4_len(const PagedAttn4& a, int b) {
     int len = a.lens[b];
     if (len <= 0) return 0;
@@ -351,9 +352,10 @@ struct P4Cfg {
     static constexpr bool WIDE = GP == 4 && HEADS > 8;
     static constexpr int U = GP <= 2 || WIDE ? 2 : 1;  // keys of a lane
     static constexpr int HDP = 32 * GP, TK = 32 * U;   // keys of a unit
-    // few warps of long units against more of short ones: 131072 keys of 8 x 128, 4 heads each, 57 us with 12 warps of 32
-    // keys, 58 with 8 of 64, 70 with 16 of 32; with 16 heads each, 65536 keys, 65 us with 8 of 64, 74 with 12 of 32; 64
-    // sequences of 2112 keys of 8 x 64 50 us with 12 warps of 64, 55 with 8
+    // few warps of long units against more of short ones: 131072 keys of 8 x 128, 4 heads each, 61.5 us with 12 warps of 32
+    // keys, 62 with 8 of 64 (48 sequences of up to 8192 keys 96-103 and 102-104); with V as subnormal halves, which was 4 us
+    // faster, 57, 58 and 70 with 16 of 32; 16 heads each, 65536 keys, 65 us with 8 of 64, 74 with 12 of 32; 64 sequences of
+    // 2112 keys of 8 x 64 50 us with 12 warps of 64, 55 with 8
     static constexpr int WARPS = GP <= 4 && !WIDE ? 12 : 8;
     static constexpr int ST = GP == 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
@@ -1487,7 +1489,7 @@ int launch_paged4_append(const float* K, const float* V, int ld, int rows, int K
     const bool vec = aligned16(K, ld) && aligned16(V, ld), wide = vec && rope_wide(rope);
     const int lanes = hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, side = 32 / lanes;
     // four blocks of heads a warp where the rows have them and fill the SMs so: less bookkeeping a head; one otherwise
-    // (with the read-back: 16384 rows of 8 x 128 66 us, 83 with one; 8 rows 13 us with either)
+    // (with the read-back, as then measured: 16384 rows of 8 x 128 75 us, 83 with one; 8 rows 13 us with either)
     const bool many = KV > 2 * side && (long long)rows * KV >= 64LL * sm_count();
     const int mode = !rope.cos_t ? P4_PLAIN : !wide ? P4_ODD : rope.halves ? P4_HALVES : P4_PAIRS;
     const auto kernel = many ? (lanes == 4    ? append_of<4, 4>(mode)

@@ -17,7 +17,7 @@ constexpr int kRopeHeads = 4;  // heads of a thread
 // pairs of neighbours, or four dims that stay) in up to kRopeHeads heads of a row, all of whose loads are in flight
 // at once; its table entries are read once for all of them. Neighbouring threads hold neighbouring items, then
 // heads. It reads all that it turns before it writes, so Y may be X. Measured: 16384 rows of 40 x 128, half of each head
-// turned, 101 us, 6.6 TB/s (293 us with a pair or a dim a thread); 64 rows 4 us, most of the call's 8 its launch.
+// turned, 99 us, 6.8 TB/s (293 us with a pair or a dim a thread); 64 rows 4 us, most of the call's 8 its launch.
 template <bool HALVES>
 __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const float* X, int ldx, float* Y, int ldy, int H,
                                                                  int hd, const int* row_pos, RopeView r, int items,
