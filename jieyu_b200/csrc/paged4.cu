@@ -310,18 +310,26 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 // against (0, X), X as two halves. Values: rows are dims, the stored words turned by ldmatrix.trans, each nibble masked into
 // a half (q - 8, or 16 times that) in two operations; the weight p_j step_jg as halves hi + lo, made from p's
 // halves by three fp16 operations (the product rounded, what that left, the low half's share); p (low + 8 step) is one product of the
-// stored halves. Steps are taken in units of 2^e of their group, e the largest exponent so far, so that a weight times a
-// step stays within fp16; a step 2^14 below another one of its group starts to lose bits, of 2^-25 of the larger one's
-// share at most. Each unit's product starts from zero and is added in fp32 with round to nearest (the tensor cores' own
+// stored halves. Each unit's product starts from zero and is added in fp32 with round to nearest (the tensor cores' own
 // sums may truncate).
+//
+// A key counts by its weight, so that one that is large and hardly seen must not cost the others their bits. Steps are
+// taken in units of 2^e of their group, which follow the units of keys up and down, so that a weight times a step stays
+// within fp16; the weights of a unit whose keys all score low are taken 2^d up and its sums 2^d down again, so that its
+// largest weight is 2^9 at least. Where the values of each group lie within 2^8 of one another (p4_fits) their steps are
+// exact (or next to far larger lows), and fp16's roundings, 2^-19.7 a key at most, are small against sum p (|low| + 15 step),
+// which is 2^4.9 at least (64 that all fall the same way: 2^-18). A unit whose keys lie further apart is added key by key in
+// fp32. 131072 keys of 8 x 128: 62 us (60 with one e for all keys so far, where one step of 8736 made steps of 1e-4 zeros
+// whatever its weight); behind a flushed L2 69, 85 with one key in 1000 far above the others, 218 with steps of 1e-4 to 0.1
+// in every unit.
 //
 // A step reads sum(len) * KV * 40 G bytes (G groups). The line of units, runs and joins are paged_line.cuh's; teams of
 // warps take the same keys of neighbouring kv heads, whose rows lie side by side in [page][slot][kv head] (262144 keys of 8 x
 // 128, without products: 95 us, 142 with every head at its own keys). Rows of 32 or 64 bytes come by tensor copies, others and
-// all parameters by cp.async. The reference follows the maximum of the scores; the accumulators are rescaled only where it or
-// a group's e moves.
+// all parameters by cp.async. The reference follows the maximum of the scores; the accumulators are rescaled only where it
+// or a group's e moves.
 //
-// Measured: 131072 keys of 8 x 128 60 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-105 us (floor
+// Measured: 131072 keys of 8 x 128 62 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-105 us (floor
 // 37), 513 keys of 2 x 64 14 us. At 131072 keys about 20 us pass before the first and behind the last key (launches, run
 // search, page table, first copies; parts and the join); between them issue slots are 54 % busy, the warps waiting for one
 // another's results in chains of products and exchanges (the copies without products take 45 us behind a flushed L2).
@@ -408,6 +416,17 @@ __device__ __forceinline__ void p4_fma2(float& x, float& y, float a, float b, fl
 }
 __device__ __forceinline__ __half2 p4_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t p4_u(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+// 2^k as a half (-24 <= k <= 15) and as a float
+__device__ __forceinline__ uint32_t p4_half_pow2(int k) { return k >= -14 ? (uint32_t)(k + 15) << 10 : 1u << (k + 24); }
+__device__ __forceinline__ float p4_pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+// What takes V's (step, low) of a group to units of 2^(e - 15), lows by eighths: both below 2 where they fit.
+__device__ __forceinline__ uint32_t p4_units(int e) { return p4_half_pow2(15 - e) | p4_half_pow2(12 - e) << 16; }
+// Whether a key's step and low keep all of their bits in units of 2^(e - 15): the step below 2 of them, low below 16, and
+// the step at 2^-8 at least or low at 1.
+__device__ __forceinline__ bool p4_fits(uint32_t par, int e) {
+    const float step = fabsf(p4_step(par)), low = fabsf(p4_low(par));
+    return step < p4_pow2(e - 14) && low < p4_pow2(e - 11) && (step >= p4_pow2(e - 23) || low >= p4_pow2(e - 15));
+}
 // the low (HIGH: the next 4) bits of each half as halves q - 8 (16 (q - 8)): 0x6400 | n is 1024 + n. (Left as they are, q 2^-24,
 // they are exact too, but the tensor cores do not shift subnormals up before they align products: 10 of the sums' 24 bits
 // went. Numbers around 0 keep the sums, which may be truncated, small.)
@@ -640,8 +659,8 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
     // that), and the products with column g (and g + 8) of V's parameters: (step, low) of each group
     uint32_t qf[GP][E][2], qsum[E][2 * LW];
     float qsl[E][2], ref[E][2], l[E][2], o[ND][E][4], opar[E][2 * LW];
-    int eg[GP];        // exponent field of V's largest step of each group so far
-    uint32_t ug[GP];   // 2^(15 - eg) and 1 as halves
+    int eg[GP];        // exponent field of V's units of each group
+    uint32_t ug[GP];   // p4_units of it
     bool fresh = true, tail = false;  // tail: the run ends inside an item that it starts
     bool gave_up = false;
     int st = 0;
@@ -663,7 +682,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
             for (int i = 0; i < GP; i++) {
                 eg[i] = 0;
-                ug[i] = 0x3C007800u;
+                ug[i] = p4_units(0);
             }
 #pragma unroll
             for (int e = 0; e < E; e++) {
@@ -710,29 +729,50 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             full &= in[u] == ~0u;
         }
 
-        // lane j, its keys: V's steps in units of their group's largest, laid out by group as the products read them
+        // lane j, its keys: V's steps in units of their group, laid out by group as the products read them
+        bool apart = false;  // the unit's values do not fit units of any size
         {
             uint32_t vw[U][PW];
-            __half2 top = __float2half2_rn(0.0f);
+            __half2 top = __float2half2_rn(0.0f), bottom = __float2half2_rn(2.0f);
 #pragma unroll
             for (int u = 0; u < U; u++) {
+                const bool live = full || (in[u] >> lane & 1);
                 uint32_t* const vrow = reinterpret_cast<uint32_t*>(sb + G::VPOFF) + PW * (32 * u + lane);
-                if (!full && !(in[u] >> lane & 1))  // whatever the ring held
+                if (!live)  // whatever the ring held
 #pragma unroll
                     for (int i = 0; i < PW; i++) vrow[i] = 0u;
                 p4_words(vrow, vw[u]);
 #pragma unroll
-                for (int i = 0; i < GP; i++) top = __hmax2_nan(top, __habs2(__hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i]))));
+                for (int i = 0; i < GP; i++) {
+                    const __half2 x = __habs2(__hmul2_rn(p4_h2(vw[u][i]), p4_h2(ug[i])));
+                    top = __hmax2_nan(top, x);
+                    if (i < groups && live) bottom = __hmin2(bottom, x);
+                }
             }
-            if (__any_sync(0xffffffffu, !(__low2float(top) < 2.0f))) {  // a larger step than before
+            const bool fits = __hblt2(top, __float2half2_rn(2.0f)) && __low2float(bottom) >= 0x1p-8f;
+            if (!__all_sync(0xffffffffu, fits)) {  // other units for the groups that do not fit theirs
 #pragma unroll
                 for (int i = 0; i < GP; i++) {
-                    uint32_t most = vw[0][i] & 0x7fffu;
-                    if (U > 1) most = max(most, vw[U - 1][i] & 0x7fffu);
-                    const int e1 = max(eg[i], (int)min(__reduce_max_sync(0xffffffffu, most) >> 10, 30u));
-                    const float f = __uint_as_float((uint32_t)(127 + eg[i] - e1) << 23);
+                    auto all_fit = [&](int e1) {
+                        bool y = true;
+#pragma unroll
+                        for (int u = 0; u < U; u++) y &= p4_fits(vw[u][i], e1) || !(in[u] >> lane & 1);
+                        return __all_sync(0xffffffffu, y) != 0;
+                    };
+                    if (all_fit(eg[i])) continue;
+                    uint32_t most = 0u;  // bits of the largest step, or of an eighth of the largest low
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t step = vw[u][i] & 0x7fffu, low = vw[u][i] >> 16 & 0x7fffu;
+                        most = max(most, max(step, low > 0x0c00u ? low - 0x0c00u : low ? 1u : 0u));
+                    }
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    if (most == 0u) continue;  // zeros
+                    const int e1 = min((int)(most >> 10), 30);
+                    apart |= !all_fit(e1);
+                    const float f = p4_pow2(eg[i] - e1);
                     eg[i] = e1;
-                    ug[i] = 0x3C000000u | (e1 == 30 ? 0x0200u : (uint32_t)(30 - e1) << 10);
+                    ug[i] = p4_units(e1);
 #pragma unroll
                     for (int e = 0; e < E; e++)
 #pragma unroll
@@ -830,8 +870,9 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                 for (int e = 0; e < E; e++)
                     *reinterpret_cast<float2*>(to + ROWS * (8 * i + g) + 8 * e) = make_float2(s[i][e][0], s[i][e][1]);
         }
-        float old[E][2];
-        bool same = true;
+        // the reference follows the maximum; a unit that scores 2^4 and more below it takes its weights 2^d up
+        float top[E][2], down[E][2];  // down: 2^-d
+        bool near = true;
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
@@ -844,17 +885,22 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                x = fmaxf(ref[e][j], x - kPaShift);
-                old[e][j] = ref[e][j];
-                same &= ref[e][j] == x;
-                ref[e][j] = x;
+                top[e][j] = x - kPaShift;
+                down[e][j] = 1.0f;
+                near &= top[e][j] <= ref[e][j] && top[e][j] > ref[e][j] - 4.0f;
             }
-        if (!__all_sync(0xffffffffu, same)) {
+        if (__all_sync(0xffffffffu, near)) {
+#pragma unroll
+            for (int i = 0; i < 4 * U; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++) p4_add2(s[i][e][0], s[i][e][1], -ref[e][0], -ref[e][1]);
+        } else {
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float al = ex2(old[e][j] - ref[e][j]);
+                    const float to = fmaxf(ref[e][j], top[e][j]), al = ex2(ref[e][j] - to);
+                    ref[e][j] = to;
                     l[e][j] *= al;
 #pragma unroll
                     for (int i = 0; i < LW; i++) opar[e][2 * i + j] *= al;
@@ -863,119 +909,186 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                         o[d][e][j] *= al;
                         o[d][e][2 + j] *= al;
                     }
+                    // (with no key, or behind all that fp32 holds, the weights stay as they are)
+                    const float d = floorf(to - top[e][j]);
+                    const bool up = d >= 4.0f && d <= 126.0f;
+                    if (up) down[e][j] = p4_pow2(-(int)d);
+#pragma unroll
+                    for (int i = 0; i < 4 * U; i++) s[i][e][j] = s[i][e][j] - to + (up ? d : 0.0f);
                 }
         }
-        // weights as halves hi + lo, transposed: column g, keys 8 i + 2 t, + 1
-        uint32_t hi[4 * U][E], lo[4 * U][E];
 #pragma unroll
         for (int i = 0; i < 4 * U; i++)
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                p4_add2(s[i][e][0], s[i][e][1], -ref[e][0], -ref[e][1]);
-                float b0 = ex2(s[i][e][0]), b1 = ex2(s[i][e][1]);
-                p4_add2(l[e][0], l[e][1], b0, b1);
-                const uint32_t ph = pa_pack(b0, b1);
-                const float2 hf = __half22float2(p4_h2(ph ^ 0x80008000u));
-                p4_add2(b0, b1, hf.x, hf.y);
-                hi[i][e] = pa_transpose(ph);
-                lo[i][e] = pa_transpose(pa_pack(b0, b1));
+                s[i][e][0] = ex2(s[i][e][0]);
+                s[i][e][1] = ex2(s[i][e][1]);
+                p4_fma2(l[e][0], l[e][1], s[i][e][0], s[i][e][1], down[e][0], down[e][1]);
             }
-        // the parameters' share: rows are their columns
-        {
-            float c[E][4];
+        if (!apart) {
+            // weights as halves hi + lo, transposed: column g, keys 8 i + 2 t, + 1
+            uint32_t hi[4 * U][E], lo[4 * U][E];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                uint32_t par[LW][4];
+            for (int i = 0; i < 4 * U; i++)
 #pragma unroll
-                for (int i = 0; i < LW; i++) pa_ldsm_t(base + G::VPOFF + 4 * PW * (32 * u + lane) + 16 * i, par[i]);
+                for (int e = 0; e < E; e++) {
+                    float b0 = s[i][e][0], b1 = s[i][e][1];
+                    const uint32_t ph = pa_pack(b0, b1);
+                    const float2 hf = __half22float2(p4_h2(ph ^ 0x80008000u));
+                    p4_add2(b0, b1, hf.x, hf.y);
+                    hi[i][e] = pa_transpose(ph);
+                    lo[i][e] = pa_transpose(pa_pack(b0, b1));
+                }
+            // the parameters' share: rows are their columns
+            {
+                float c[E][4];
 #pragma unroll
-                for (int e = 0; e < E; e++)
+                for (int u = 0; u < U; u++) {
+                    uint32_t par[LW][4];
 #pragma unroll
-                    for (int m = 0; m < 2; m++) {
-                        const uint32_t pf[4] = {par[0][2 * m], LW > 1 ? par[LW - 1][2 * m] : 0u, par[0][2 * m + 1],
-                                                LW > 1 ? par[LW - 1][2 * m + 1] : 0u};
-                        const int i = 4 * u + 2 * m;
-                        const uint32_t h0 = hi[i][e], h1 = hi[i + 1][e], l0 = lo[i][e], l1 = lo[i + 1][e];
-                        if (HEADS <= 4) {
-                            const uint32_t b[2] = {g < 4 ? h0 : l0, g < 4 ? h1 : l1};
-                            if (i == 0)
-                                pa_mma_f16(pf, b, 0.0f, c[e]);
-                            else
-                                pa_mma_f16(pf, b, c[e]);
-                        } else {
-                            const uint32_t bl[2] = {l0, l1}, bh[2] = {h0, h1};
-                            if (i == 0)
-                                pa_mma_f16(pf, bl, 0.0f, c[e]);
-                            else
-                                pa_mma_f16(pf, bl, c[e]);
-                            pa_mma_f16(pf, bh, c[e]);
-                        }
-                    }
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++)
-#pragma unroll
-                for (int i = 0; i < 2 * LW; i++) opar[e][i] += c[e][i];
-        }
-        // P.V, a group at a time: V's numbers less 8 as halves (the high ones 16 times that), rows g dims 2 g,
-        // rows g + 8 dims 2 g + 1 of 16; a weight times a step as halves: hi rounded, lo what that left and lo's share.
-        // 4 heads fill 8 columns with their hi and lo halves
-        uint32_t zl[4 * U];
-        if (HEADS <= 4)
-#pragma unroll
-            for (int i = 0; i < 4 * U; i++) {
-                zl[i] = g < 4 ? 0u : hi[i][0] ^ 0x80008000u;
-                lo[i][0] = g < 4 ? 0u : lo[i][0];
-            }
-#pragma unroll
-        for (int i0 = 0; i0 < GP; i0++) {
-            float c[2][E][4];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                uint32_t r[4];
-                pa_ldsm_t(base + G::VOFF + G::at(32 * u + lane, i0), r);
-                const uint4 sv = *reinterpret_cast<const uint4*>(ring + G::SOFF + 64 * (GP * u + i0) + 16 * t);
-                const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    uint32_t bh[E][2], bl[E][2];
+                    for (int i = 0; i < LW; i++) pa_ldsm_t(base + G::VPOFF + 4 * PW * (32 * u + lane) + 16 * i, par[i]);
 #pragma unroll
                     for (int e = 0; e < E; e++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int at = 4 * u + 2 * m + i;
-                            const __half2 w = p4_h2(sw[2 * m + i]), ph = p4_h2(hi[at][e]), pw = p4_h2(lo[at][e]);
+                        for (int m = 0; m < 2; m++) {
+                            const uint32_t pf[4] = {par[0][2 * m], LW > 1 ? par[LW - 1][2 * m] : 0u, par[0][2 * m + 1],
+                                                    LW > 1 ? par[LW - 1][2 * m + 1] : 0u};
+                            const int i = 4 * u + 2 * m;
+                            const uint32_t h0 = hi[i][e], h1 = hi[i + 1][e], l0 = lo[i][e], l1 = lo[i + 1][e];
                             if (HEADS <= 4) {
-                                bh[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hmul2_rn(p4_h2(zl[at]), w))));
+                                const uint32_t b[2] = {g < 4 ? h0 : l0, g < 4 ? h1 : l1};
+                                if (i == 0)
+                                    pa_mma_f16(pf, b, 0.0f, c[e]);
+                                else
+                                    pa_mma_f16(pf, b, c[e]);
                             } else {
-                                const __half2 x = __hmul2_rn(ph, w);
-                                bh[e][i] = p4_u(x);
-                                bl[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hneg2(x))));
+                                const uint32_t bl[2] = {l0, l1}, bh[2] = {h0, h1};
+                                if (i == 0)
+                                    pa_mma_f16(pf, bl, 0.0f, c[e]);
+                                else
+                                    pa_mma_f16(pf, bl, c[e]);
+                                pa_mma_f16(pf, bh, c[e]);
                             }
                         }
-                    const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+                }
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint32_t vf[4] = {k ? p4_whole<true>(x0) : p4_whole<false>(x0), k ? p4_whole<true>(y0) : p4_whole<false>(y0),
-                                                k ? p4_whole<true>(x1) : p4_whole<false>(x1), k ? p4_whole<true>(y1) : p4_whole<false>(y1)};
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int i = 0; i < 2 * LW; i++) opar[e][i] = __fmaf_rn(c[e][i], down[e][i & 1], opar[e][i]);
+            }
+            // P.V, a group at a time: V's numbers less 8 as halves (the high ones 16 times that), rows g dims 2 g,
+            // rows g + 8 dims 2 g + 1 of 16; a weight times a step as halves: hi rounded, lo what that left and lo's share.
+            // 4 heads fill 8 columns with their hi and lo halves
+            uint32_t zl[4 * U];
+            if (HEADS <= 4)
+#pragma unroll
+                for (int i = 0; i < 4 * U; i++) {
+                    zl[i] = g < 4 ? 0u : hi[i][0] ^ 0x80008000u;
+                    lo[i][0] = g < 4 ? 0u : lo[i][0];
+                }
+#pragma unroll
+            for (int i0 = 0; i0 < GP; i0++) {
+                float c[2][E][4];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    uint32_t r[4];
+                    pa_ldsm_t(base + G::VOFF + G::at(32 * u + lane, i0), r);
+                    const uint4 sv = *reinterpret_cast<const uint4*>(ring + G::SOFF + 64 * (GP * u + i0) + 16 * t);
+                    const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        uint32_t bh[E][2], bl[E][2];
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const int at = 4 * u + 2 * m + i;
+                                const __half2 w = p4_h2(sw[2 * m + i]), ph = p4_h2(hi[at][e]), pw = p4_h2(lo[at][e]);
+                                if (HEADS <= 4) {
+                                    bh[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hmul2_rn(p4_h2(zl[at]), w))));
+                                } else {
+                                    const __half2 x = __hmul2_rn(ph, w);
+                                    bh[e][i] = p4_u(x);
+                                    bl[e][i] = p4_u(__hfma2(pw, w, __hfma2(ph, w, __hneg2(x))));
+                                }
+                            }
+                        const uint32_t x0 = r[2 * m], x1 = r[2 * m + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t vf[4] = {k ? p4_whole<true>(x0) : p4_whole<false>(x0), k ? p4_whole<true>(y0) : p4_whole<false>(y0),
+                                                    k ? p4_whole<true>(x1) : p4_whole<false>(x1), k ? p4_whole<true>(y1) : p4_whole<false>(y1)};
+#pragma unroll
+                            for (int e = 0; e < E; e++) {
+                                if (u == 0 && m == 0)
+                                    pa_mma_f16(vf, bh[e], 0.0f, c[k][e]);
+                                else
+                                    pa_mma_f16(vf, bh[e], c[k][e]);
+                                if (HEADS > 4) pa_mma_f16(vf, bl[e], c[k][e]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2)
+                            p4_fma2(o[2 * i0 + k][e][j], o[2 * i0 + k][e][j + 1], c[k][e][j], c[k][e][j + 1], down[e][0], down[e][1]);
+            }
+        } else {
+            // key by key in fp32: the weights lie over K's rows, from where every lane takes those of its heads
+            float* const pw = reinterpret_cast<float*>(sb);  // [key][ROWS]
+            static_assert(4 * 32 * ROWS <= TK * G::PITCH, "32 keys' weights fit K's rows");
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                __syncwarp();  // K's rows are read, and the last keys' weights
+                if (HEADS > 4 || t < 2)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            *reinterpret_cast<float2*>(pw + ROWS * (8 * i + g) + 8 * e + 2 * t) =
+                                make_float2(s[4 * u + i][e][0] * down[e][0], s[4 * u + i][e][1] * down[e][1]);
+                __syncwarp();
+#pragma unroll 1
+                for (int k = 0; k < 32; k++) {
+                    const unsigned char* const par = sb + G::VPOFF + 4 * PW * (32 * u + k);
+                    float2 p[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        p[e] = HEADS > 4 || t < 2 ? *reinterpret_cast<const float2*>(pw + ROWS * k + 8 * e + 2 * t)
+                                                  : make_float2(0.0f, 0.0f);  // their heads are counted at t - 2
+#pragma unroll
+                    for (int i = 0; i < LW; i++) {
+                        const float x = __half2float(reinterpret_cast<const __half*>(par)[8 * i + g]);
 #pragma unroll
                         for (int e = 0; e < E; e++) {
-                            if (u == 0 && m == 0)
-                                pa_mma_f16(vf, bh[e], 0.0f, c[k][e]);
-                            else
-                                pa_mma_f16(vf, bh[e], c[k][e]);
-                            if (HEADS > 4) pa_mma_f16(vf, bl[e], c[k][e]);
+                            opar[e][2 * i] = __fmaf_rn(p[e].x, x, opar[e][2 * i]);
+                            opar[e][2 * i + 1] = __fmaf_rn(p[e].y, x, opar[e][2 * i + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < GP; i++) {
+                        const float step = p4_step(reinterpret_cast<const uint32_t*>(par)[i]) * p4_pow2(15 - eg[i]);
+                        const int n2 = *reinterpret_cast<const unsigned short*>(sb + G::VOFF + G::at(32 * u + k, i) + 2 * g);
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {  // the low and the high bits: 16 times their numbers
+                            const float x = (float)(c ? (n2 & 0xF0) - 128 : (n2 & 15) - 8) * step;
+                            const float y = (float)(c ? (n2 >> 8 & 0xF0) - 128 : (n2 >> 8 & 15) - 8) * step;
+#pragma unroll
+                            for (int e = 0; e < E; e++) {
+                                o[2 * i + c][e][0] = __fmaf_rn(p[e].x, x, o[2 * i + c][e][0]);
+                                o[2 * i + c][e][1] = __fmaf_rn(p[e].y, x, o[2 * i + c][e][1]);
+                                o[2 * i + c][e][2] = __fmaf_rn(p[e].x, y, o[2 * i + c][e][2]);
+                                o[2 * i + c][e][3] = __fmaf_rn(p[e].y, y, o[2 * i + c][e][3]);
+                            }
                         }
                     }
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int e = 0; e < E; e++)
-#pragma unroll
-                    for (int j = 0; j < 4; j += 2)
-                        p4_add2(o[2 * i0 + k][e][j], o[2 * i0 + k][e][j + 1], c[k][e][j], c[k][e][j + 1]);
+            if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // tensor copies write there next
+            __syncwarp();
         }
         if constexpr (TMA) {
             // the stage is read: the unit ST ahead takes its place
