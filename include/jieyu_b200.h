@@ -420,7 +420,7 @@ JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_
  * and theirs, C rows of stride ldc floats; bias may be NULL. A and W are
  * 16-byte aligned, lda and ldw multiples of 16; what lies between k and a
  * row's stride does not count. k <= 131071 (127^2 k, and 128^2 k, stay below
- * 2^31). Nothing is allocated. */
+ * 2^31), m and n <= 2^31 - 256. Nothing is allocated. */
 JYC_API int jyc_matmul_i8(const int8_t* A, int lda, const float* a_scale, const int8_t* W, int ldw,
                           const float* w_scale, const float* bias, float* C, int ldc, int m, int n, int k,
                           void* stream);

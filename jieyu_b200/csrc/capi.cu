@@ -608,6 +608,7 @@ JYC_API int jyc_matmul_i8(const int8_t* A, int lda, const float* a_scale, const 
     clear_error();
     if (m < 0 || n <= 0 || k <= 0) return arg_error("matmul_i8: need m >= 0 and n, k > 0");
     if (k > 131071) return arg_error("matmul_i8: k above 131071 can pass 32-bit sums");
+    if (m > 0x7fffff00 || n > 0x7fffff00) return arg_error("matmul_i8: m and n must be at most 2^31 - 256");
     if (lda < k || ldw < k || ldc < n) return arg_error("matmul_i8: lda and ldw must hold k, ldc must hold n");
     if ((lda | ldw) & 15) return arg_error("matmul_i8: lda and ldw must be multiples of 16");
     if (m == 0) return JYC_OK;

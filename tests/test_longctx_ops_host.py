@@ -151,6 +151,16 @@ def test_matmul_i8_refuses(kw):
     assert "matmul_i8" in _capi.last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(m=2**31 - 255), dict(m=2**31 - 1), dict(n=2**31 - 255, ldc=2**31 - 1),
+                                dict(n=2**31 - 1, ldc=2**31 - 1)])
+def test_matmul_i8_refuses_more_tiles_than_an_int_counts(kw):
+    """A tile of 256 channels or tokens that starts below 2^31 must also end there: places are counted in ints."""
+    d = dict(A=A, lda=16, a_scale=A, W=A, ldw=16, w_scale=A, bias=None, C=A, ldc=40, m=3, n=40, k=16)
+    d.update(kw)
+    assert _capi.load().jyc_matmul_i8(*d.values(), None) == _capi.JYC_ERR_ARG
+    assert "matmul_i8" in _capi.last_error()
+
+
 def test_empty_calls_do_nothing():
     lib = _capi.load()
     assert _append(rows=0, K=None, V=None, pos=None) == _capi.JYC_OK
