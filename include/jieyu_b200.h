@@ -409,7 +409,8 @@ JYC_API int jyc_rope_rows(const float* X, int ldx, float* Y, int ldy, int rows, 
 
 /* Rows of x [rows][k] (row stride ldx floats) in 8 bits with one scale each:
  * kv_pack_q8's rule over a whole row (jyc_kv_pack_q8), q at row stride ldq bytes. A NaN
- * counts as 0; a row with an infinity gets an infinite scale and zeros. k > 0. */
+ * counts as 0; a row with an infinity gets an infinite scale and zeros.
+ * 0 < k <= 2^31 - 1024. */
 JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_t* q, int ldq, float* scale,
                                  void* stream);
 

@@ -595,6 +595,7 @@ JYC_API int jyc_quantize_rows_i8(const float* x, int ldx, int rows, int k, int8_
                                  void* stream) {
     clear_error();
     if (rows < 0 || k <= 0) return arg_error("quantize_rows_i8: need rows >= 0 and k > 0");
+    if (k > 0x7ffffc00) return arg_error("quantize_rows_i8: k must be at most 2^31 - 1024");
     if (ldx < k || ldq < k) return arg_error("quantize_rows_i8: ldx and ldq must hold k");
     if (rows == 0) return JYC_OK;
     if (!x || !q || !scale) return arg_error("quantize_rows_i8: null pointer");

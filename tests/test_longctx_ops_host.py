@@ -161,6 +161,13 @@ def test_matmul_i8_refuses_more_tiles_than_an_int_counts(kw):
     assert "matmul_i8" in _capi.last_error()
 
 
+@pytest.mark.parametrize("k", [2**31 - 1023, 2**31 - 1])
+def test_quantize_rows_refuses_rows_that_an_int_steps_over(k):
+    """256 threads take quads of a row in turn: the step behind the last one must stay below 2^31."""
+    assert _capi.load().jyc_quantize_rows_i8(A, 2**31 - 1, 2, k, A, 2**31 - 1, A, None) == _capi.JYC_ERR_ARG
+    assert "quantize_rows_i8" in _capi.last_error()
+
+
 def test_empty_calls_do_nothing():
     lib = _capi.load()
     assert _append(rows=0, K=None, V=None, pos=None) == _capi.JYC_OK
