@@ -564,6 +564,12 @@ int check_paged4(const char* what, int num_kv_heads, int head_dim, const int* pa
 // Of one launch's grid: heads of sequences.
 constexpr long long kMaxItems = 0x7fffffffLL;
 
+// Whether a size_t counts the scores that attention leaves for its weights: a float per place of a sequence and query
+// head, of which a kv head's are rounded up to 16 at most.
+bool scores_countable(int num_seqs, int num_heads, int capacity) {
+    return (double)num_seqs * num_heads * (capacity + 64.0) * (16 * sizeof(float)) < 9e18;
+}
+
 int paged4_view(const jyc_kv_pages_q4* pages, const int* page_table, int table_stride, int num_seqs, PagedKV4* kv) {
     int* err = paged_error_word();
     if (!err) return cuda_fail(cudaErrorNoDevice, "paged error word");
@@ -659,7 +665,7 @@ JYC_API size_t jyc_attention_paged_q4_workspace(int num_seqs, int num_heads, int
     clear_error();
     if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
         head_dim % 4 || head_dim > 256 || capacity < 0 || capacity > 0x7fffff00 ||
-        (long long)num_seqs * num_heads > kMaxItems) {
+        (long long)num_seqs * num_heads > kMaxItems || !scores_countable(num_seqs, num_heads, capacity)) {
         arg_error("attention_paged_q4_workspace: bad shape");
         return 0;
     }
@@ -686,6 +692,7 @@ JYC_API int jyc_attention_paged_q4(const float* Q, int ldq, float* out, int ldo,
     if (!Q || !out || !seq_lens) return arg_error("attention_paged_q4: null pointer");
     if (askew(Q, out, seq_lens, rope_pos)) return arg_error("attention_paged_q4: misaligned array");
     const int capacity = pages->mass ? table_stride * pages->page_size : 0;
+    if (!scores_countable(num_seqs, num_heads, capacity)) return arg_error("attention_paged_q4: too many places for a workspace");
     const size_t need = paged4_attention_workspace(num_seqs, num_heads, num_kv_heads, head_dim, capacity);
     if (need == 0) return cuda_fail(cudaErrorNoDevice, "attention_paged_q4: device query");
     if (workspace && workspace_bytes < need) return arg_error("attention_paged_q4: workspace too small");

@@ -117,6 +117,18 @@ def test_workspace_query_refuses_bad_shapes():
         assert "workspace" in _capi.last_error()
 
 
+def test_more_scores_than_bytes_count_are_refused():
+    """A workspace of 2^64 bytes and more: its size would come out small, and the scores would lie behind it."""
+    f = _capi.load().jyc_attention_paged_q4_workspace
+    for H, kv in ((16, 16), (16, 1), (15, 3)):
+        assert f(1 << 27, H, kv, 4, 0x7fffff00) == 0
+        assert "bad shape" in _capi.last_error()
+        assert _attend(seqs=1 << 27, H=H, kv=kv, hd=4, width=1, pages=_pages(page_size=0x7fffff00)) == _capi.JYC_ERR_ARG
+        assert "attention_paged_q4" in _capi.last_error()
+    assert _attend(seqs=1 << 26, H=16, kv=16, hd=4, width=1, work=A, bytes=1 << 62,
+                   pages=_pages(page_size=0x7fffff00)) == _capi.JYC_ERR_ARG
+
+
 def _turn(**kw):
     d = dict(X=A, ldx=128, Y=2 * A, ldy=128, rows=3, heads=2, hd=64, pos=A, rope=_rope())
     d.update(kw)
