@@ -190,3 +190,40 @@ def test_two_streams(cuda):
                                               c.data_ptr(), n, m, n, k, st.cuda_stream))
         for a, sa, w, sw, _, c, _ in sets:
             assert np.array_equal(host(c), _expected(a, sa, w, sw, None))
+
+
+@pytest.mark.parametrize("va,vw", [(-128, -128), (127, -128), (None, None)])
+def test_largest_sums_of_pairs_of_ctas(cuda, va, vw):
+    """k = 131071 where there are tiles of 256 x 256 for a quarter of the SMs: the form whose CTAs work in pairs."""
+    torch = cuda
+    m, n, k, ld = 300, 4865, 131071, 131072
+    if va is None:
+        a, w = (torch.randint(-128, 128, (r, ld), dtype=torch.int8, device="cuda") for r in (m, n))
+    else:
+        a = torch.full((m, ld), va, dtype=torch.int8, device="cuda")
+        w = torch.full((n, ld), vw, dtype=torch.int8, device="cuda")
+    sa, sw = np.linspace(0.5, 2, m).astype(np.float32), np.linspace(1e-3, 1, n).astype(np.float32)
+    bias = np.random.default_rng(3).normal(size=n).astype(np.float32)
+    sad, swd, bd = dev(torch, sa), dev(torch, sw), dev(torch, bias)
+    c = torch.full((m, n + 3), 7.0, device="cuda")
+    _capi.check(_capi.load().jyc_matmul_i8(a.data_ptr(), ld, sad.data_ptr(), w.data_ptr(), ld, swd.data_ptr(), bd.data_ptr(),
+                                           c.data_ptr(), n + 3, m, n, k, _stream(torch)))
+    if va is None:
+        whole = torch.cat([a[:, :k].double() @ w[j: j + 500, :k].double().T for j in range(0, n, 500)], 1).cpu().numpy()
+    else:
+        whole = np.full((m, n), float(va) * vw * k)
+    y = P.r32(P.r32(whole) * P.r32(sa.astype(np.float64)[:, None] * sw.astype(np.float64)))
+    got = host(c)
+    assert np.array_equal(got[:, :n], P.r32(y + bias.astype(np.float64)).astype(np.float32)) and np.all(got[:, n:] == 7.0)
+
+
+def test_scales_that_are_not_numbers_of_pairs_of_ctas(cuda):
+    rng = np.random.default_rng(5)
+    m, n, k = 300, 4900, 100
+    a, sa, w, sw = _inputs(rng, m, n, k)
+    sa[[1, 200, 299]], sw[[5, 4899]], sw[6] = (np.inf, np.nan, -np.inf), np.nan, 0.0
+    a[1] = 0
+    with np.errstate(invalid="ignore"):
+        want = _expected(a, sa, w, sw, None)
+    got = _run(cuda, a, sa, w, sw, None, m, n, k)
+    assert np.array_equal(got, want, equal_nan=True) and np.isfinite(np.delete(got, (1, 200, 299), 0)[:, 7:4899]).all()
