@@ -316,12 +316,12 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 // A key counts by its weight, so that one that is large and hardly seen must not cost the others their bits. Steps are
 // taken in units of 2^e of their group, which follow the units of keys up and down, so that a weight times a step stays
 // within fp16; the weights of a unit whose keys all score low are taken 2^d up and its sums 2^d down again, so that its
-// largest weight is 2^9 at least. Where the values of each group lie within 2^8 of one another (p4_fits) their steps are
-// exact (or next to far larger lows), and fp16's roundings, 2^-19.7 a key at most, are small against sum p (|low| + 15 step),
-// which is 2^4.9 at least (64 that all fall the same way: 2^-18). A unit whose keys lie further apart is added key by key in
-// fp32. 131072 keys of 8 x 128: 62 us (60 with one e for all keys so far, where one step of 8736 made steps of 1e-4 zeros
-// whatever its weight); behind a flushed L2 69, 85 with one key in 1000 far above the others, 218 with steps of 1e-4 to 0.1
-// in every unit.
+// largest weight is 2^9 at least (2^5 of values within 2^4 of one another). Where the values of each group lie within 2^8 of
+// one another (p4_fits) their steps are exact (or next to far larger lows), and fp16's roundings, 2^-19.7 a key at most, are
+// small against sum p (|low| + 15 step), which is 2^4.9 at least (64 that all fall the same way: 2^-18). A unit whose keys
+// lie further apart is added key by key in fp32. 131072 keys of 8 x 128: 60.4 us (59.0 with one e for all keys so far, where
+// one step of 8736 made steps of 1e-4 zeros whatever its weight); behind a flushed L2 67, 81 with one key in 1000 far above
+// the others, 210 with steps of 1e-4 to 0.1 in every unit.
 //
 // A step reads sum(len) * KV * 40 G bytes (G groups). The line of units, runs and joins are paged_line.cuh's; teams of
 // warps take the same keys of neighbouring kv heads, whose rows lie side by side in [page][slot][kv head] (262144 keys of 8 x
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 // all parameters by cp.async. The reference follows the maximum of the scores; the accumulators are rescaled only where it
 // or a group's e moves.
 //
-// Measured: 131072 keys of 8 x 128 62 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-105 us (floor
+// Measured: 131072 keys of 8 x 128 60 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-111 us (floor
 // 37), 513 keys of 2 x 64 14 us. At 131072 keys about 20 us pass before the first and behind the last key (launches, run
 // search, page table, first copies; parts and the join); between them issue slots are 54 % busy, the warps waiting for one
 // another's results in chains of products and exchanges (the copies without products take 45 us behind a flushed L2).
@@ -732,6 +732,7 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 
         // lane j, its keys: V's steps in units of their group, laid out by group as the products read them
         bool apart = false;  // the unit's values do not fit units of any size
+        float room;          // how far below the reference its keys may score: 2^4, or 2^8 of values within 2^4
         {
             uint32_t vw[U][PW];
             __half2 top = __float2half2_rn(0.0f), bottom = __float2half2_rn(2.0f);
@@ -750,8 +751,9 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                     if (i < groups && live) bottom = __hmin2(bottom, x);
                 }
             }
-            const bool fits = __hblt2(top, __float2half2_rn(2.0f)) && __low2float(bottom) >= 0x1p-8f;
-            if (!__all_sync(0xffffffffu, fits)) {  // other units for the groups that do not fit theirs
+            const bool small = __hblt2(top, __float2half2_rn(2.0f));
+            room = __all_sync(0xffffffffu, small && __low2float(bottom) >= 0x1p-4f) ? 8.0f : 4.0f;
+            if (!__all_sync(0xffffffffu, small && __low2float(bottom) >= 0x1p-8f)) {  // other units for the groups that do not fit theirs
 #pragma unroll
                 for (int i = 0; i < GP; i++) {
                     auto all_fit = [&](int e1) {
@@ -871,9 +873,9 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                 for (int e = 0; e < E; e++)
                     *reinterpret_cast<float2*>(to + ROWS * (8 * i + g) + 8 * e) = make_float2(s[i][e][0], s[i][e][1]);
         }
-        // the reference follows the maximum; a unit that scores 2^4 and more below it takes its weights 2^d up
+        // the reference follows the maximum; a unit that scores far below it takes its weights 2^d up
         float top[E][2], down[E][2];  // down: 2^-d
-        bool near = true;
+        bool raise = false, near = true;
 #pragma unroll
         for (int e = 0; e < E; e++)
 #pragma unroll
@@ -888,14 +890,10 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 top[e][j] = x - kPaShift;
                 down[e][j] = 1.0f;
-                near &= top[e][j] <= ref[e][j] && top[e][j] > ref[e][j] - 4.0f;
+                raise |= top[e][j] > ref[e][j];
+                near &= top[e][j] > ref[e][j] - room;
             }
-        if (__all_sync(0xffffffffu, near)) {
-#pragma unroll
-            for (int i = 0; i < 4 * U; i++)
-#pragma unroll
-                for (int e = 0; e < E; e++) p4_add2(s[i][e][0], s[i][e][1], -ref[e][0], -ref[e][1]);
-        } else {
+        if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
@@ -910,22 +908,24 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
                         o[d][e][j] *= al;
                         o[d][e][2 + j] *= al;
                     }
-                    // (with no key, or behind all that fp32 holds, the weights stay as they are)
-                    const float d = floorf(to - top[e][j]);
-                    const bool up = d >= 4.0f && d <= 126.0f;
-                    if (up) down[e][j] = p4_pow2(-(int)d);
-#pragma unroll
-                    for (int i = 0; i < 4 * U; i++) s[i][e][j] = s[i][e][j] - to + (up ? d : 0.0f);
                 }
         }
 #pragma unroll
         for (int i = 0; i < 4 * U; i++)
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                s[i][e][0] = ex2(s[i][e][0]);
-                s[i][e][1] = ex2(s[i][e][1]);
-                p4_fma2(l[e][0], l[e][1], s[i][e][0], s[i][e][1], down[e][0], down[e][1]);
-            }
+            for (int e = 0; e < E; e++) p4_add2(s[i][e][0], s[i][e][1], -ref[e][0], -ref[e][1]);
+        if (!__all_sync(0xffffffffu, near))
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    // (with no key, or behind all that fp32 holds, the weights stay as they are)
+                    const float d = floorf(ref[e][j] - top[e][j]);
+                    const bool up = d >= 4.0f && d <= 126.0f;
+                    if (up) down[e][j] = p4_pow2(-(int)d);
+#pragma unroll
+                    for (int i = 0; i < 4 * U; i++) s[i][e][j] += up ? d : 0.0f;
+                }
         if (!apart) {
             // weights as halves hi + lo, transposed: column g, keys 8 i + 2 t, + 1
             uint32_t hi[4 * U][E], lo[4 * U][E];
@@ -933,7 +933,8 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
             for (int i = 0; i < 4 * U; i++)
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    float b0 = s[i][e][0], b1 = s[i][e][1];
+                    float b0 = ex2(s[i][e][0]), b1 = ex2(s[i][e][1]);
+                    p4_fma2(l[e][0], l[e][1], b0, b1, down[e][0], down[e][1]);
                     const uint32_t ph = pa_pack(b0, b1);
                     const float2 hf = __half22float2(p4_h2(ph ^ 0x80008000u));
                     p4_add2(b0, b1, hf.x, hf.y);
@@ -1044,13 +1045,15 @@ __global__ void __launch_bounds__(P4Cfg<GP, HEADS, TMA>::WARPS * 32, 1)
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 __syncwarp();  // K's rows are read, and the last keys' weights
-                if (HEADS > 4 || t < 2)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int e = 0; e < E; e++)
-                            *reinterpret_cast<float2*>(pw + ROWS * (8 * i + g) + 8 * e + 2 * t) =
-                                make_float2(s[4 * u + i][e][0] * down[e][0], s[4 * u + i][e][1] * down[e][1]);
+                    for (int e = 0; e < E; e++) {
+                        const float p0 = ex2(s[4 * u + i][e][0]) * down[e][0], p1 = ex2(s[4 * u + i][e][1]) * down[e][1];
+                        p4_add2(l[e][0], l[e][1], p0, p1);
+                        if (HEADS > 4 || t < 2)
+                            *reinterpret_cast<float2*>(pw + ROWS * (8 * i + g) + 8 * e + 2 * t) = make_float2(p0, p1);
+                    }
                 __syncwarp();
 #pragma unroll 1
                 for (int k = 0; k < 32; k++) {

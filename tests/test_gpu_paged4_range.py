@@ -33,7 +33,7 @@ def _check(torch, pool, q, out, H, lens):
     """The bound of _paged4.out_tolerance with each head's and group's own weighted sum in the place of the largest value.
     A unit of up to 64 keys goes into the tensor cores only where its largest weight is 2^9 at least and a group's steps and
     lows fit units in which steps are below 2 and lows below 16, steps at 2^-8 at least or lows at 1: the sum is 2^9 * 15 *
-    2^-8 > 2^4.9 at least, and of a key the product of weight and step is off by half of 2^-24 before it is multiplied by up
+    2^-8 > 2^4.9 at least (as 2^5 * 15 * 2^-4 is, the other form: weights from 2^5, steps from 2^-4), and of a key the product of weight and step is off by half of 2^-24 before it is multiplied by up
     to 8, and its weight by as much before it is multiplied by low + 8 step, up to 32: 2^-22 + 2^-20 together, 64 times at
     most 2^-13.6, 2^-18 (64 half steps) of the sum. Steps below 2^-14, next to lows of 1 at least, are off by 2^-25 before
     they are multiplied by up to 8: 4 half steps."""
