@@ -122,7 +122,8 @@ JYC_API int jyc_rope_table(int max_seq, int head_dim, float theta,
  *                    `low`, rounded up, both within 0 .. rot_dim - 1,
  *                    t = 1 - (j - j_low) / (j_high - j_low) held within 0 .. 1;
  *                    cos and sin are multiplied by attention (0: 0.1 ln(factor) + 1).
- * factor >= 1; low < high and original_len > 0 where they are used. */
+ * factor >= 1; 0 < low < high and original_len > 0 where they are used; NTK
+ * needs rot_dim > 2, RAMP theta > 1. */
 enum { JYC_ROPE_NONE = 0, JYC_ROPE_LINEAR = 1, JYC_ROPE_NTK = 2, JYC_ROPE_BANDS = 3, JYC_ROPE_RAMP = 4 };
 typedef struct jyc_rope_scaling {
     int kind;
@@ -458,7 +459,8 @@ typedef struct jyc_kv_pages_q4 {
 /* jyc_kv_append_paged_q8 for these pages. rope NULL: K arrives turned; else
  * row i turns by rope_pos[i] (rope_pos NULL: row_pos[i]; they differ once rows
  * were evicted; a negative one, like one behind the tables, skips the row and
- * sets bit 4). The rows' mass, where there is one, starts at 0. */
+ * sets bit 4). The rows' mass, where there is one, starts at 0, and grows by
+ * the calls of jyc_attention_paged_q4 alone. */
 JYC_API int jyc_kv_append_paged_q4(const float* K, const float* V, int ld, int rows, int num_kv_heads, int head_dim,
                                    const int* row_seq, const int* row_pos, const int* page_table, int table_stride,
                                    int num_seqs, const jyc_rope* rope, const int* rope_pos,
@@ -498,11 +500,12 @@ JYC_API size_t jyc_attention_paged_q4_workspace(int num_seqs, int num_heads, int
  * the pages of new_table [num_seqs][new_stride] (new_stride * page_size >=
  * budget); new_lens[s] = min(seq_lens[s], budget) (not below 0). kept
  * [num_seqs][num_kv_heads][budget] gets their old positions, -1 behind the
- * last. The pages of new_table are other ones than those of page_table (a
- * sequence that keeps all of its rows may name its old pages, which then stay
- * as they are); afterwards the old pages are free. new_lens is another array
- * than seq_lens. pages->mass must be there. 0 <= recent <= budget, budget > 0,
- * num_seqs * num_kv_heads * budget <= 2^30.
+ * last. Rows that no query has attended to since they were appended tie at 0.
+ * The pages of new_table are other ones than those of page_table (a sequence
+ * that keeps all of its rows may name its old pages at their old places, which
+ * then stay as they are); afterwards the old pages are free. new_lens is another
+ * array than seq_lens. pages->mass must be there. 0 <= recent <= budget,
+ * budget > 0, num_seqs * num_kv_heads * budget <= 2^30.
  * A row whose old or new page is out of range is not copied (error word). */
 JYC_API int jyc_kv_evict_paged_q4(const int* seq_lens, int budget, int recent, int num_kv_heads, int head_dim,
                                   const int* page_table, int table_stride, int num_seqs, const int* new_table,

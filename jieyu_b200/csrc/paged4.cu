@@ -102,9 +102,10 @@ __device__ __forceinline__ uint32_t p4_bytes(float4 x, float low, float inv) {
 
 // Four lanes hold a group: lane i its dims 4 i .. 4 i + 3 and 16 more, whose numbers are the low and the high bits of its
 // word; the group's range is two exchanges. Of four heads in flight each lane makes one's parameters and passes them on.
-// Pairs that lie on quads turn by table entries that a lane reads once for all of its heads. Bound by its instructions, 84
-// a head of 128 and warp: 16384 rows of 8 x 128 33 us (floor 24), 45 where every lane makes the parameters of all heads, 60 with the rotation's
-// form chosen value by value too, 72 with four dims a lane.
+// Pairs that lie on quads turn by table entries that a lane reads once for all of its heads; others, which are rare, value
+// by value (P4_ODD: 78 us behind a flushed L2 where quads take 40 to 48). Bound by its instructions, 84 a head of 128 and
+// warp: 16384 rows of 8 x 128 33 us (floor 24), 45 where every lane makes the parameters of all heads, 60 with the
+// rotation's form chosen value by value too, 72 with four dims a lane.
 enum { P4_PLAIN = 0, P4_PAIRS = 1, P4_HALVES = 2, P4_ODD = 3 };  // how K turns
 template <int LANES, int UNITS, int MODE>
 __global__ void __launch_bounds__(kP4Threads) paged4_append_kernel(const float* K, const float* V, int ld, int rows,
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kP4Threads) paged4_read_kernel(float* K, float
 //
 // Measured: 131072 keys of 8 x 128 60 us (floor 26), 48 sequences of up to 8192 keys with their weights 98-111 us (floor
 // 37), 513 keys of 2 x 64 14 us. At 131072 keys about 20 us pass before the first and behind the last key (launches, run
-// search, page table, first copies; parts and the join); between them issue slots are 54 % busy, the warps waiting for one
+// search, page table, first copies; parts and the join); between them issue slots are 55 % busy, the warps waiting for one
 // another's results in chains of products and exchanges (the copies without products take 45 us behind a flushed L2).
 __device__ __forceinline__ int p4_len(const PagedAttn4& a, int b) {
     int len = a.lens[b];
@@ -1288,7 +1289,7 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
     const int capacity = a.kv.table_stride * a.kv.p.page_size, groups = (a.hd + 31) / 32;
     const long long tiles = ((long long)capacity + G::TK - 1) / G::TK;
     // teams of as many neighbouring kv heads as the warps hold evenly: their rows lie side by side where pages hold
-    // positions first
+    // positions first (5 and 7 heads share no divisor with the warps: 78 and 81 us, 68 with 6 or 8 of as many keys in all)
     pl.team = std::gcd(pl.units_row, (int)G::WARPS);
     pl.units_row /= pl.team;
     const long long items = (long long)a.kv.num_seqs * pl.units_row;
@@ -1345,7 +1346,8 @@ int p4_launch(const PagedAttn4& a, PaPlan pl, int sms, void* work, cudaStream_t 
 // shared memory, all CTAs of the cluster add up all counts and find the same digit. Then
 // kept positions are counted slice by slice and warp by warp, and written in their order.
 // Keys of slices up to kEvSpan positions stay in shared memory (131072 positions of one
-// sequence: 8 CTAs a head), those of longer ones are read again for each digit. Masses
+// sequence: 8 CTAs a head), those of longer ones are read again for each digit (10
+// sequences of 8 heads: 44 us at 24000 positions, 89 at 25500). Masses
 // differ little in their first digit: each lane has counts of its own. (Digits of 11 bits
 // need one pass less, but 2048 counts to clear, add up and exchange: for 131072 positions 40 us against 33.)
 constexpr int kEvThreads = 1024, kEvWarps = kEvThreads / 32, kEvSpan = 24576;
