@@ -365,7 +365,8 @@ struct P4Cfg {
     // keys, 62 with 8 of 64 (48 sequences of up to 8192 keys 96-103 and 102-104); with V as subnormal halves, which was 4 us
     // faster, 57, 58 and 70 with 16 of 32; 16 heads each, 65536 keys, 65 us with 8 of 64, 74 with 12 of 32; 64 sequences of
     // 2112 keys of 8 x 64, 4 heads each, 50 us with 12 warps of 64, 55 with 8. With 16 heads each the 168 registers of 12
-    // warps do not hold a unit: behind a flushed L2 108 us, 98 with 8; 4 kv heads in pages of 5 80 and 63
+    // warps do not hold a unit: behind a flushed L2 108 us, 98 with 8; 4 kv heads in pages of 5 80 and 63. (Heads above
+    // 128 with 16 heads each spill 260 to 500 bytes a thread at 255 registers: 30000 keys of 4 x 256 take 76 us.)
     static constexpr int WARPS = GP <= 4 && HEADS <= 8 ? 12 : 8;
     static constexpr int ST = GP == 6 ? 3 : 2;
     static constexpr int E = HEADS <= 8 ? 1 : 2;  // n8 tiles of heads
