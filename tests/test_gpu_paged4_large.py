@@ -156,3 +156,82 @@ def test_evictions_of_long_slices(cuda, kv, page, lens, budget, recent, kind):
             sp, ss = page_of[rows[ok]], rows[ok] % page
             assert np.array_equal(k1[dp, ds, h], k0[sp, ss, h])
             assert np.array_equal(m1[dp, ds, h], m0[sp, ss, h], equal_nan=True)
+
+
+def test_a_captured_fork_and_join_replays(cuda):
+    """One graph whose calls run on two streams that part and meet, behind copies and clears: each call's first kernel may
+    start while the last one of its stream ends, and waits for all that it follows."""
+    torch = cuda
+    lib = _capi.load()
+    rng = np.random.default_rng(51)
+    seqs, hidden, H, kv, hd, page, width, budget = 3, 640, 8, 2, 64, 16, 40, 100
+    wide = (H + 2 * kv) * hd
+    pages = seqs * (width + 7)
+    both = rng.permutation(pages).reshape(seqs, width + 7)
+    w = dev(torch, rng.integers(-127, 128, (wide, hidden)).astype(np.int8))
+    ws = dev(torch, rng.uniform(1e-3, 2e-3, wide).astype(np.float32))
+    cos, sin = P.tables(1000, hd)
+    c, s = dev(torch, cos), dev(torch, sin)
+    rp = P4.rope(c, s, True)
+    newd = _ints(torch, both[:, width:])
+    x, lens, turn = torch.zeros(seqs, hidden, device="cuda"), _ints(torch, [1] * seqs), _ints(torch, [0] * seqs)
+
+    class Side:
+        def __init__(self):
+            self.pool = P4.Pool(torch, pages, page, kv, hd, both[:, :width])
+            self.pool.put_random(np.random.default_rng(1), None)
+            self.other = P4.Pool(torch, pages, page, kv, hd, both[:, :width])
+            self.other.put_random(np.random.default_rng(2), None)
+            self.mass = torch.rand(tuple(self.pool.mass.shape), generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+            self.xq, self.xs = torch.zeros(seqs, hidden, dtype=torch.int8, device="cuda"), torch.zeros(seqs, device="cuda")
+            self.x, self.qkv = torch.zeros(seqs, hidden, device="cuda"), torch.zeros(seqs, wide, device="cuda")
+            self.out, self.far = (torch.zeros(seqs, H * hd, device="cuda") for _ in range(2))
+            self.nl, self.pos = (torch.zeros(seqs, dtype=torch.int32, device="cuda") for _ in range(2))
+            self.kept = torch.zeros(seqs, kv, budget, dtype=torch.int32, device="cuda")
+            self.work = P4.workspace(torch, seqs, H, kv, hd, width * page)
+            self.aside = torch.cuda.Stream()
+
+        def step(self):
+            main, aside = torch.cuda.current_stream(), self.aside
+            self.x.copy_(x)  # a copy, then a call
+            _capi.check(lib.jyc_quantize_rows_i8(self.x.data_ptr(), hidden, seqs, hidden, self.xq.data_ptr(), hidden,
+                                                 self.xs.data_ptr(), main.cuda_stream))
+            _capi.check(lib.jyc_matmul_i8(self.xq.data_ptr(), hidden, self.xs.data_ptr(), w.data_ptr(), hidden, ws.data_ptr(), None,
+                                          self.qkv.data_ptr(), wide, seqs, wide, hidden, main.cuda_stream))
+            aside.wait_stream(main)  # both streams read the products from here on
+            with torch.cuda.stream(aside):
+                self.other.mass.copy_(self.mass)
+                _capi.check(P4.attend(torch, self.other, self.qkv, self.far, H, lens, rp, turn))
+                _capi.check(P4.evict(torch, self.other, lens, budget, 8, newd, self.nl, self.kept))
+            self.pos.copy_(lens)
+            self.pos.sub_(1)
+            k = self.qkv.data_ptr() + 4 * H * hd
+            _capi.check(P4.append(torch, self.pool, k, k + 4 * kv * hd, wide, seqs, None, self.pos, rp, turn))
+            self.pool.mass.zero_()
+            _capi.check(P4.attend(torch, self.pool, self.qkv, self.out, H, lens, rp, turn, self.work))
+            main.wait_stream(aside)
+            # both sides' results are read and written again: the first kernel follows two streams
+            _capi.check(lib.jyc_rope_rows(self.far.data_ptr(), H * hd, self.out.data_ptr(), H * hd, 1, H, hd, turn.data_ptr(),
+                                          P4.ref(rp), main.cuda_stream))
+
+        def state(self):
+            return [host(t).copy() for t in (self.qkv, self.out, self.far, self.nl, self.kept, self.pool.k, self.pool.vp,
+                                             self.pool.mass, self.other.k, self.other.kp, self.other.mass)]
+
+    once, again = Side(), Side()
+    for side in (once, again):
+        side.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again.step()
+    for n in ([600, 1, 99], [100, 101, 640], [333, 640, 7]):
+        x.normal_()
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        turn.copy_(lens + 300)
+        torch.cuda.synchronize()
+        once.step()
+        torch.cuda.synchronize()
+        graph.replay()
+        for got, want in zip(again.state(), once.state()):
+            assert np.array_equal(got, want, equal_nan=got.dtype.kind == "f")
